@@ -1,8 +1,8 @@
-"""Build ``libpiper_merge.so`` in-tree with nvcc for sm_100a.
+"""Build ``libpiper_merge.so`` and ``libpiper_fp4.so`` in-tree with nvcc for sm_100a.
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
-``__graft_entry__.build()``). The build is skipped when the library is newer
-than every source file.
+``__graft_entry__.build()``). A library newer than every source file of its
+own is left as it is.
 """
 
 from __future__ import annotations
@@ -17,6 +17,12 @@ ROOT = PKG.parent
 SOURCES = [PKG / "csrc" / "merge.cu"]
 DEPS = SOURCES + [PKG / "csrc" / "ptx.cuh", PKG / "csrc" / "numerics.cuh", ROOT / "include" / "piper_merge.h"]
 OUT = PKG / "libpiper_merge.so"
+FP4_SOURCES = [PKG / "csrc" / "fp4.cu"]
+FP4_DEPS = FP4_SOURCES + [
+    *(PKG / "csrc" / n for n in ("fp4_quant.cuh", "fp4_linear.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
+    ROOT / "include" / "piper_fp4.h",
+]
+FP4_OUT = PKG / "libpiper_fp4.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,26 +43,38 @@ def nvcc() -> str:
     return cand if Path(cand).exists() else "nvcc"
 
 
-def up_to_date() -> bool:
-    if not OUT.exists():
+def up_to_date(out: Path = OUT, deps: list[Path] = DEPS) -> bool:
+    if not out.exists():
         return False
-    t = OUT.stat().st_mtime
-    return all(p.stat().st_mtime <= t for p in DEPS)
+    t = out.stat().st_mtime
+    return all(p.stat().st_mtime <= t for p in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and up_to_date():
-        return OUT
-    tmp = OUT.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", str(tmp), *map(str, SOURCES)]
+def _compile(out: Path, sources: list[Path], verbose: bool) -> None:
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [nvcc(), *NVCC_FLAGS, "-o", str(tmp), *map(str, sources)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True, cwd=str(ROOT))
-    os.replace(tmp, OUT)
+    os.replace(tmp, out)
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """The merges' library; the FP4 operators' is built beside it."""
+    build_fp4(force, verbose)
+    if force or not up_to_date():
+        _compile(OUT, SOURCES, verbose)
     return OUT
+
+
+def build_fp4(force: bool = False, verbose: bool = False) -> Path:
+    if force or not up_to_date(FP4_OUT, FP4_DEPS):
+        _compile(FP4_OUT, FP4_SOURCES, verbose)
+    return FP4_OUT
 
 
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(OUT)
+    print(FP4_OUT)

@@ -1,0 +1,370 @@
+// fp4.cu - host side and C ABI (include/piper_fp4.h) of the FP4 operators.
+#include "../../include/piper_fp4.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <string>
+
+#include "fp4_linear.cuh"
+#include "fp4_quant.cuh"
+
+namespace {
+
+thread_local std::string g_error;
+std::atomic<uint64_t> g_launches{0};
+
+int fail(int code, const char* message) {
+  g_error = message;
+  return code;
+}
+
+int cuda_fail(const char* what, cudaError_t e) {
+  g_error = std::string(what) + ": " + cudaGetErrorString(e);
+  return PIPER_FP4_ECUDA;
+}
+
+#define FP4_REQUIRE(condition, message) \
+  if (!(condition)) return fail(PIPER_FP4_EINVAL, message)
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    cudaGetLastError();
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr) : nullptr;
+  }();
+  return fn;
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+int64_t align256(int64_t a) { return up(a, 256); }
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int block_of(const piper_fp4_matrix& m) { return m.format == PIPER_FP4_MX ? 32 : 16; }
+size_t width(int dtype) { return dtype == PIPER_FP4_BF16 ? 2 : 4; }
+
+int check_matrix(const piper_fp4_matrix* m) {
+  FP4_REQUIRE(m != nullptr, "FP4: null matrix.");
+  FP4_REQUIRE(m->format == PIPER_FP4_MX || m->format == PIPER_FP4_NV, "FP4: unknown format.");
+  FP4_REQUIRE(m->batch > 0 && m->rows > 0 && m->cols > 0, "FP4 requires a non-empty matrix.");
+  FP4_REQUIRE(m->cols % block_of(*m) == 0,
+              m->format == PIPER_FP4_MX ? "MXFP4 requires columns divisible by 32." : "NVFP4 requires columns divisible by 16.");
+  FP4_REQUIRE(m->batch <= (int64_t{1} << 20) && m->rows < (int64_t{1} << 31) - 256 && m->cols < (int64_t{1} << 31) - 256 &&
+                  m->batch * up(m->rows, 128) < (int64_t{1} << 31),
+              "FP4: a matrix has at most 2^31 rows over its batch and 2^31 columns.");
+  FP4_REQUIRE(m->format == PIPER_FP4_NV || m->second == nullptr, "MXFP4 has no second-level scale.");
+  return PIPER_FP4_OK;
+}
+
+int check_buffers(const piper_fp4_matrix* m) {
+  FP4_REQUIRE(m->codes != nullptr && m->scale != nullptr, "FP4: null codes or scales.");
+  return PIPER_FP4_OK;
+}
+
+int check_dtype(int dtype) {
+  FP4_REQUIRE(dtype == PIPER_FP4_BF16 || dtype == PIPER_FP4_F32, "FP4 supports bfloat16 and float32 values.");
+  return PIPER_FP4_OK;
+}
+
+cudaError_t launched() {
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return cudaGetLastError();
+}
+
+// Scales per row (row-major) or scale tiles per row (swizzled).
+int scale_cols(const piper_fp4_matrix& m) {
+  const int64_t blocks = m.cols / block_of(m);
+  return static_cast<int>(m.swizzled ? (blocks + 3) / 4 : blocks);
+}
+
+#define FP4_DISPATCH(dtype, format, CALL)                          \
+  do {                                                             \
+    if ((dtype) == PIPER_FP4_BF16) {                               \
+      if ((format) == PIPER_FP4_MX) { CALL(fp4::kBF16, fp4::kMX); } \
+      else { CALL(fp4::kBF16, fp4::kNV); }                         \
+    } else {                                                       \
+      if ((format) == PIPER_FP4_MX) { CALL(fp4::kF32, fp4::kMX); } \
+      else { CALL(fp4::kF32, fp4::kNV); }                          \
+    }                                                              \
+  } while (0)
+
+// ---------------------------------------------------------------- the product
+// Scratch of a product: quantized tokens, and the weight's parts that are not
+// stored as the product reads them.
+struct LinearPlan {
+  bool move_codes, move_scale;
+  int64_t k_padded;                    // columns up to a whole scale tile
+  int64_t x_codes, x_scale, w_codes, w_scale, total;  // byte offsets
+  int64_t w_code_pitch, scale_tiles, scale_rows;
+};
+
+LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
+  LinearPlan p{};
+  const int tile = block_of(w) * 4;
+  p.scale_tiles = (w.cols + tile - 1) / tile;
+  p.k_padded = p.scale_tiles * tile;
+  p.move_codes = w.cols % 32 != 0 || !aligned(w.codes, 16);
+  p.move_scale = !w.swizzled || w.cols % 64 != 0 || !aligned(w.scale, 16);
+  p.w_code_pitch = up(w.cols / 2, 16);
+  // every expert starts on a tile of 128 token rows; one more for a second tile that is read and not used
+  p.scale_rows = (tokens / 128 + w.batch + 2) * 128;
+  int64_t at = 0;
+  p.x_codes = at;
+  at += align256(tokens * (p.k_padded / 2));
+  p.x_scale = at;
+  at += align256(p.scale_rows * p.scale_tiles * 4);
+  p.w_codes = at;
+  if (p.move_codes) at += align256(w.batch * w.rows * p.w_code_pitch);
+  p.w_scale = at;
+  if (p.move_scale) at += align256(w.batch * up(w.rows, 128) * p.scale_tiles * 4);
+  p.total = at;
+  return p;
+}
+
+// Map of rows of packed codes, in boxes of 256 values x `box_rows` rows with the 128-byte swizzle.
+bool code_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t pitch, int64_t rows, int box_rows) {
+  const auto enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  const cuuint32_t box[2] = {fp4::kStageBytes, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t one[2] = {1u, 1u};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, int FMT, int BN>
+cudaError_t launch_linear(const fp4::LinearArgs& args, int64_t items, cudaStream_t stream) {
+  using S = fp4::LinearShape<FMT, BN>;
+  auto kernel = fp4::linear_kernel<DT, FMT, BN>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  kernel<<<static_cast<unsigned>(items), fp4::kLinearThreads, S::kSmem, stream>>>(args);
+  return launched();
+}
+
+}  // namespace
+
+extern "C" {
+
+int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_stride, int32_t dtype, int32_t scale_mode,
+                       int32_t second_mode, uint32_t* maxima, void* stream) {
+  if (int rc = check_matrix(m)) return rc;
+  if (int rc = check_buffers(m)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(x != nullptr, "FP4 quantisation: null input.");
+  FP4_REQUIRE(x_stride >= m->cols, "FP4 quantisation: rows of the input overlap.");
+  FP4_REQUIRE(scale_mode >= 0 && scale_mode <= 3, "Unsupported MX scaling mode id.");
+  FP4_REQUIRE(second_mode >= 0 && second_mode <= 2, "FP4 quantisation: unknown second-level mode.");
+  FP4_REQUIRE((second_mode == PIPER_FP4_SECOND_NONE) == (m->second == nullptr),
+              "FP4 quantisation: the second-level scale does not match its mode.");
+  FP4_REQUIRE(aligned(m->codes, 4) && (!m->swizzled || aligned(m->scale, 4)),
+              "FP4 quantisation: codes and swizzled scales start on 4-byte boundaries.");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int tile = block_of(*m) * 4;
+  fp4::QuantArgs q{};
+  q.x = x;
+  q.x_stride = x_stride;
+  q.rows = m->rows;
+  q.rows_padded = m->swizzled ? up(m->rows, 128) : m->rows;
+  q.batch = m->batch;
+  q.cols = static_cast<int32_t>(m->cols);
+  q.octets = static_cast<int32_t>((m->swizzled ? up(m->cols, tile) : m->cols) / 8);
+  q.vec = aligned(x, 16) && (x_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  q.codes = static_cast<uint8_t*>(m->codes);
+  q.code_pitch = m->cols / 2;
+  q.scale = static_cast<uint8_t*>(m->scale);
+  q.scale_cols = scale_cols(*m);
+  q.swizzled = m->swizzled != 0;
+  q.words = m->cols % tile == 0 || m->swizzled ? aligned(m->scale, 4) : 0;
+  q.scale_mode = scale_mode;
+  q.second_mode = second_mode;
+  q.second = m->second;
+  if (second_mode == PIPER_FP4_SECOND_COMPUTE) {
+    FP4_REQUIRE(maxima != nullptr, "FP4 quantisation: computing second-level scales needs room for the maxima.");
+    FP4_REQUIRE(m->batch <= 65535, "FP4 quantisation: at most 65535 matrices with second-level scales.");
+    q.amax = maxima;
+    q.reverse = 1;
+    cudaError_t e = cudaMemsetAsync(maxima, 0, sizeof(uint32_t) * m->batch, s);
+    if (e != cudaSuccess) return cuda_fail("cudaMemsetAsync", e);
+    const int64_t blocks = (m->rows * (m->cols / 8) + fp4::kOctetsPerBlock - 1) / fp4::kOctetsPerBlock;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 8)), static_cast<unsigned>(m->batch));
+    if (dtype == PIPER_FP4_BF16) fp4::amax_kernel<fp4::kBF16><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
+    else fp4::amax_kernel<fp4::kF32><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
+    if ((e = launched()) != cudaSuccess) return cuda_fail("amax kernel", e);
+  }
+  const int64_t blocks = (q.batch * q.rows_padded * q.octets + fp4::kOctetsPerBlock - 1) / fp4::kOctetsPerBlock;
+  FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 quantisation: too many values for one call.");
+#define CALL(D, F) fp4::quantize_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q)
+  FP4_DISPATCH(dtype, m->format, CALL);
+#undef CALL
+  const cudaError_t e = launched();
+  return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("quantize kernel", e);
+}
+
+int piper_fp4_dequantize(const piper_fp4_matrix* m, void* y, int32_t dtype, void* stream) {
+  if (int rc = check_matrix(m)) return rc;
+  if (int rc = check_buffers(m)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(y != nullptr, "FP4 dequantisation: null output.");
+  fp4::DequantArgs d{};
+  d.codes = static_cast<const uint8_t*>(m->codes);
+  d.scale = static_cast<const uint8_t*>(m->scale);
+  d.second = m->second;
+  d.y = y;
+  d.rows = m->rows;
+  d.batch = m->batch;
+  d.cols = static_cast<int32_t>(m->cols);
+  d.swizzled = m->swizzled != 0;
+  d.scale_cols = scale_cols(*m);
+  d.vec = aligned(m->codes, 4) && aligned(y, 16);
+  const int64_t blocks = (m->batch * m->rows * (m->cols / 8) + fp4::kOctetsPerBlock - 1) / fp4::kOctetsPerBlock;
+  FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 dequantisation: too many values for one call.");
+#define CALL(D, F) \
+  fp4::dequantize_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, static_cast<cudaStream_t>(stream)>>>(d)
+  FP4_DISPATCH(dtype, m->format, CALL);
+#undef CALL
+  const cudaError_t e = launched();
+  return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("dequantize kernel", e);
+}
+
+int piper_fp4_linear_workspace(const piper_fp4_matrix* w, int64_t tokens, size_t* bytes) {
+  if (int rc = check_matrix(w)) return rc;
+  FP4_REQUIRE(bytes != nullptr && tokens >= 0, "FP4 product: bad workspace query.");
+  *bytes = static_cast<size_t>(plan_linear(*w, tokens).total);
+  return PIPER_FP4_OK;
+}
+
+int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride, int64_t tokens, const int32_t* ends,
+                     const float* act_second, int32_t scale_mode, void* y, int32_t dtype, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_buffers(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31) - w->batch * 128 - 1024, "FP4 product: too many tokens for one call.");
+  if (tokens == 0) return PIPER_FP4_OK;
+  FP4_REQUIRE(x != nullptr && y != nullptr, "FP4 product: null input or output.");
+  FP4_REQUIRE(x_stride >= w->cols || tokens == 1, "FP4 product: rows of the input overlap.");
+  FP4_REQUIRE(ends != nullptr || w->batch == 1, "FP4 product: several matrices need the ends of their rows.");
+  FP4_REQUIRE(scale_mode >= 0 && scale_mode <= 3, "Unsupported MX scaling mode id.");
+  FP4_REQUIRE(act_second == nullptr || w->format == PIPER_FP4_NV, "MXFP4 activations have no second-level scale.");
+  const LinearPlan p = plan_linear(*w, tokens);
+  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256))
+    return fail(PIPER_FP4_EWORKSPACE, "FP4 product: workspace missing, too small or not 256-byte aligned.");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+
+  fp4::QuantArgs q{};
+  q.x = x;
+  q.x_stride = x_stride;
+  q.rows = q.rows_padded = tokens;
+  q.batch = 1;
+  q.cols = static_cast<int32_t>(w->cols);
+  q.octets = static_cast<int32_t>(p.k_padded / 8);
+  q.vec = aligned(x, 16) && (x_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  q.codes = ws + p.x_codes;
+  q.code_pitch = p.k_padded / 2;
+  q.scale = ws + p.x_scale;
+  q.scale_cols = static_cast<int32_t>(p.scale_tiles);
+  q.swizzled = q.words = q.pad_codes = 1;
+  q.scale_mode = scale_mode;
+  q.second_mode = act_second != nullptr ? PIPER_FP4_SECOND_GIVEN : PIPER_FP4_SECOND_NONE;
+  q.second = const_cast<float*>(act_second);
+  q.ends = ends;
+  q.experts = static_cast<int32_t>(w->batch);
+  q.y = y;
+  q.y_cols = w->rows;
+  fp4::RepackArgs r{};
+  r.codes = static_cast<const uint8_t*>(w->codes);
+  r.code_row = w->cols / 2;
+  r.code_pitch = p.w_code_pitch;
+  r.scale = static_cast<const uint8_t*>(w->scale);
+  r.rows = w->rows;
+  r.batch = w->batch;
+  r.scale_cols = static_cast<int32_t>(w->cols / block_of(*w));
+  r.swizzled = w->swizzled != 0;
+  if (p.move_scale) {
+    r.scale_out = ws + p.w_scale;
+    r.words = w->batch * up(w->rows, 128) * p.scale_tiles;
+  }
+  if (p.move_codes) {
+    r.codes_out = ws + p.w_codes;
+    r.pieces = w->batch * w->rows * (p.w_code_pitch / 16);
+  }
+  const int64_t quant_blocks = (tokens * q.octets + fp4::kOctetsPerBlock - 1) / fp4::kOctetsPerBlock;
+  const int64_t blocks = quant_blocks + (r.words + r.pieces + fp4::kQuantThreads - 1) / fp4::kQuantThreads;
+  FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 product: too many values for one call.");
+
+  fp4::LinearArgs a{};
+  const int64_t per_expert = tokens / w->batch;
+  const int bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 256;
+  const void* codes = p.move_codes ? ws + p.w_codes : w->codes;
+  if (!code_map(&a.w_map, codes, p.w_code_pitch, p.w_code_pitch, w->batch * w->rows, fp4::kTileRows) ||
+      !code_map(&a.x_map, q.codes, q.code_pitch, q.code_pitch, tokens, bn))
+    return fail(PIPER_FP4_ECUDA, "FP4 product: cuTensorMapEncodeTiled failed.");
+  a.w_scale = p.move_scale ? ws + p.w_scale : static_cast<const uint8_t*>(w->scale);
+  a.x_scale = q.scale;
+  a.w_second = w->second;
+  a.x_second = act_second;
+  a.ends = ends;
+  a.y = y;
+  a.tokens = tokens;
+  a.rows = static_cast<int32_t>(w->rows);
+  a.row_tiles = static_cast<int32_t>((w->rows + 127) / 128);
+  a.k_steps = static_cast<int32_t>((w->cols + 63) / 64);
+  a.scale_tiles = static_cast<int32_t>(p.scale_tiles);
+  a.experts = static_cast<int32_t>(w->batch);
+  // with experts: an upper bound on the token tiles, as the ends are on the device
+  const int64_t token_tiles = ends == nullptr ? (tokens + bn - 1) / bn : tokens / bn + std::min(w->batch, tokens);
+  const int64_t items = token_tiles * a.row_tiles;
+  FP4_REQUIRE(items < (int64_t{1} << 31), "FP4 product: too many tiles for one call.");
+
+#define CALL(D, F) \
+  fp4::prepare_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q, r, static_cast<uint32_t>(quant_blocks))
+  FP4_DISPATCH(dtype, w->format, CALL);
+#undef CALL
+  cudaError_t e = launched();
+  if (e != cudaSuccess) return cuda_fail("prepare kernel", e);
+#define CALL(D, F)                                            \
+  e = bn == 32 ? launch_linear<D, F, 32>(a, items, s)         \
+               : bn == 128 ? launch_linear<D, F, 128>(a, items, s) : launch_linear<D, F, 256>(a, items, s)
+  FP4_DISPATCH(dtype, w->format, CALL);
+#undef CALL
+  return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("linear kernel", e);
+}
+
+int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, int64_t tokens, int32_t dtype, size_t* bytes) {
+  return fail(PIPER_FP4_EINVAL, "FP4 gradient: not built.");
+}
+int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_stride, int64_t tokens,
+                         const int32_t* ends, void* dx, int32_t dtype, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  return fail(PIPER_FP4_EINVAL, "FP4 gradient: not built.");
+}
+
+const char* piper_fp4_last_error(void) { return g_error.c_str(); }
+
+int piper_fp4_device_status(void* stream, uint32_t* status) {
+  cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("cudaStreamSynchronize", e);
+  unsigned int v = 0, zero = 0;
+  e = cudaMemcpyFromSymbol(&v, pm::g_status, sizeof(v));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(pm::g_status, &zero, sizeof(zero));
+  if (e != cudaSuccess) return cuda_fail("status word", e);
+  if (status) *status = v;
+  return v == 0 ? PIPER_FP4_OK : fail(PIPER_FP4_ETIMEOUT, "a bounded device-side wait timed out.");
+}
+
+const char* piper_fp4_version(void) { return "piper-fp4 0.1 sm_100a"; }
+
+uint64_t piper_fp4_launches(void) { return g_launches.load(std::memory_order_relaxed); }
+
+}  // extern "C"

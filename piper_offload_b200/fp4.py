@@ -1,0 +1,336 @@
+"""4-bit floating-point operators around the merge: make FP4 weights, use them, differentiate through them.
+
+The merges change packed weights in place; these functions make such weights
+from dense ones and multiply with them, in the layouts the merges read and
+write (:class:`~.weights.MXWeight` with e2m1 elements, :class:`~.weights.NVFP4Weight`,
+and their stacks of experts), on sm_100a kernels of ``libpiper_fp4.so``:
+
+* :func:`quantize_mxfp4`, :func:`quantize_nvfp4`, :func:`dequantize_fp4`;
+* :func:`linear_fp4`: tokens times a weight, the tokens quantised on the way;
+* :func:`grouped_linear_fp4`: the same with one weight per expert, the tokens
+  sorted by expert and the ends of their groups on the device;
+* :func:`linear_fp4_grad_input`, :func:`grouped_linear_fp4_grad_input`: the
+  gradients with respect to the tokens. The two products are differentiable:
+  they use these when their input requires a gradient.
+
+Definitions. A block of a row (32 values in MXFP4, 16 in NVFP4) with the
+largest magnitude ``a`` is stored as ``e2m1(clamp(x / s, -6, 6)) * s``, nearest
+with ties to even. MXFP4: ``s`` is a power of two that ``scaling_mode`` derives
+from ``a``. NVFP4: ``s = e4m3(clamp(a / 6 / g, 2**-6, 448)) * g``, where the
+second-level scale ``g`` is 1, given, or ``max(max|x| / 2688, 2**-23)`` over
+the matrix. A block that holds a NaN reads back as NaN; infinities saturate.
+Products are over these values, summed in fp32 and rounded once to the type
+of the tokens.
+
+All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
+take workspaces from PyTorch's caching allocator on it, do not synchronise,
+and raise ``ValueError`` for arguments that they do not take.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any
+
+import torch
+
+from . import _native_fp4 as nat
+from . import kernels as K
+from .adapters import mx_scaling_mode_id
+from .weights import MXActQuantKwargs, MXExperts, MXScalingMode, MXWeight, NVFP4Experts, NVFP4Weight
+
+_DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float32: nat.DT_F32}
+_FP4 = K._FP4_DTYPE
+_E8M0 = K._E8M0_DTYPE
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"FP4 {what} supports bfloat16 and float32 values, got {t.dtype}.")
+    return dt
+
+
+def _matrix(w: Any) -> tuple[nat.Matrix, int, torch.Tensor]:
+    """(descriptor, MX scaling mode of activations, codes) of a packed weight or stack, checked."""
+    q, s = w.qdata, w.scale
+    if q.device.type != "cuda":
+        raise ValueError("FP4 operators require CUDA tensors.")
+    if q.dtype is not torch.uint8:
+        raise ValueError(f"FP4 operators expect packed uint8 codes, got {q.dtype}.")
+    if q.ndim not in (2, 3) or s.ndim != q.ndim:
+        raise ValueError("FP4 operators expect rank-two weights, or rank-three stacks of experts.")
+    if not q.is_contiguous() or not s.is_contiguous():
+        raise ValueError("FP4 operators require contiguous codes and scales.")
+    if s.device != q.device:
+        raise ValueError("FP4 operators require all tensors on one CUDA device.")
+    batch = q.shape[0] if q.ndim == 3 else 1
+    rows, cols = q.shape[-2], q.shape[-1] * 2
+    if batch == 0 or rows == 0 or cols == 0:
+        raise ValueError("FP4 operators require non-empty weights.")
+    swizzled = bool(w.is_swizzled_scales)
+    second = None
+    elem = getattr(w, "elem_dtype", None)
+    mode: int | None = 0
+    if elem is not None:
+        if elem is not _FP4 or _FP4 is None:
+            raise ValueError(f"FP4 operators support MX weights with e2m1 elements, got {elem}.")
+        if w.block_size != 32 or cols % 32:
+            raise ValueError("MXFP4 weights have blocks of 32 and columns divisible by 32.")
+        if s.dtype is not torch.uint8 and s.dtype is not _E8M0:
+            raise ValueError(f"MXFP4 weights have E8M0 scales, got {s.dtype}.")
+        expected = K.mx_expected_scale_shape(rows, cols, swizzled=swizzled)
+        mode = mx_scaling_mode_id(w)
+        if mode is None:
+            raise ValueError("MXFP4 activations support FLOOR, RCEIL, CEIL and EVEN scale rounding.")
+        fmt = nat.FMT_MX
+    else:
+        if w.block_size != 16 or cols % 16:
+            raise ValueError("NVFP4 weights have blocks of 16 and columns divisible by 16.")
+        if s.dtype is not torch.float8_e4m3fn:
+            raise ValueError(f"NVFP4 weights have E4M3FN scales, got {s.dtype}.")
+        expected = K.nvfp4_expected_scale_shape(rows, cols, swizzled=swizzled)
+        second = w.per_tensor_scale
+        if second is not None and (second.dtype is not torch.float32 or second.numel() != batch
+                                   or second.device != q.device or not second.is_contiguous()):
+            raise ValueError("NVFP4 second-level scales are one contiguous float32 value per matrix on its device.")
+        fmt = nat.FMT_NV
+    if s.shape[-2:] != expected or (q.ndim == 3 and s.shape[0] != batch):
+        raise ValueError(f"FP4 scale shape {tuple(s.shape)} does not match its layout.")
+    m = nat.Matrix(q.data_ptr(), s.data_ptr(), None if second is None else second.data_ptr(), batch, rows, cols, fmt,
+                   swizzled)
+    return m, mode, q
+
+
+class _on:
+    """The device of a call, entered only where it is not the current one."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device) -> None:
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self) -> None:
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc: Any) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor:
+    need = ctypes.c_size_t(0)
+    nat.check(query(*args, ctypes.byref(need)))
+    return torch.empty(need.value, dtype=torch.uint8, device=device)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as a matrix whose rows are contiguous and do not overlap (a view where it is one)."""
+    if x.ndim != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if x.stride(1) != 1 or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
+        x = x.contiguous()
+    return x
+
+
+# ------------------------------------------------------------------ quantisation
+def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torch.Tensor | None,
+              second_mode: int) -> tuple[torch.Tensor, torch.Tensor]:
+    block = 32 if fmt == nat.FMT_MX else 16
+    if x.device.type != "cuda":
+        raise ValueError("FP4 quantisation requires CUDA tensors.")
+    dt = _dtype(x, "quantisation")
+    if x.ndim not in (2, 3):
+        raise ValueError("FP4 quantisation expects a matrix, or a stack of them.")
+    rows, cols = x.shape[-2:]
+    if x.numel() == 0:
+        raise ValueError("FP4 quantisation requires non-empty tensors.")
+    if cols % block:
+        raise ValueError(f"{'MXFP4' if fmt == nat.FMT_MX else 'NVFP4'} quantisation requires columns divisible by {block}.")
+    x2 = _rows(x.detach())
+    lead = x.shape[:-2]
+    shape = (K.mx_expected_scale_shape if fmt == nat.FMT_MX else K.nvfp4_expected_scale_shape)(rows, cols, swizzled=swizzled)
+    codes = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((*lead, *shape), dtype=torch.uint8, device=x.device)
+    m = nat.Matrix(codes.data_ptr(), scale.data_ptr(), None if second is None else second.data_ptr(),
+                   lead[0] if lead else 1, rows, cols, fmt, swizzled)
+    maxima = torch.empty(m.batch, dtype=torch.int32, device=x.device) if second_mode == nat.SECOND_COMPUTE else None
+    with _on(x.device):
+        nat.check(nat.load().piper_fp4_quantize(
+            ctypes.byref(m), x2.data_ptr(), x2.stride(0), dt, mode, second_mode,
+            None if maxima is None else maxima.data_ptr(), nat.current_stream_handle(x.device)))
+    return codes, scale
+
+
+def quantize_mxfp4(x: torch.Tensor, *, scaling_mode: str | int = "floor", swizzled: bool = False) -> MXWeight | MXExperts:
+    """``x`` (rows, cols), or a stack (experts, rows, cols), as MXFP4.
+
+    ``scaling_mode`` is kept with the result: its tokens are quantised the same way.
+    """
+    name = {v: k for k, v in K._MX_SCALING_MODES.items()}.get(scaling_mode, scaling_mode)
+    if name not in K._MX_SCALING_MODES:
+        raise ValueError(f"Unsupported MX scaling mode {scaling_mode!r}.")
+    if _FP4 is None:
+        raise ValueError("MXFP4 weights need torch.float4_e2m1fn_x2.")
+    codes, scale = _quantize(x, nat.FMT_MX, K._MX_SCALING_MODES[name], swizzled, None, nat.SECOND_NONE)
+    kind = MXExperts if x.ndim == 3 else MXWeight
+    return kind(codes, scale, _FP4, orig_dtype=x.dtype, is_swizzled_scales=swizzled,
+                act_quant_kwargs=MXActQuantKwargs(MXScalingMode(name)))
+
+
+def quantize_nvfp4(x: torch.Tensor, *, two_level: bool = True, per_tensor_scale: torch.Tensor | None = None,
+                   swizzled: bool = False) -> NVFP4Weight | NVFP4Experts:
+    """``x`` (rows, cols), or a stack (experts, rows, cols), as NVFP4.
+
+    With ``two_level`` each matrix gets a second-level scale: ``per_tensor_scale``
+    (fp32, one per matrix) where given, else one computed from its largest value.
+    """
+    batch = x.shape[0] if x.ndim == 3 else 1
+    second, second_mode = None, nat.SECOND_NONE
+    if per_tensor_scale is not None:
+        if not two_level:
+            raise ValueError("NVFP4 quantisation without a second level takes no per_tensor_scale.")
+        if (per_tensor_scale.dtype is not torch.float32 or per_tensor_scale.numel() != batch
+                or per_tensor_scale.device != x.device):
+            raise ValueError("NVFP4 second-level scales are one float32 value per matrix on its device.")
+        second, second_mode = per_tensor_scale.detach().reshape(batch).contiguous(), nat.SECOND_GIVEN
+    elif two_level and x.device.type == "cuda":
+        second, second_mode = torch.empty(batch, dtype=torch.float32, device=x.device), nat.SECOND_COMPUTE
+    codes, scale = _quantize(x, nat.FMT_NV, 0, swizzled, second, second_mode)
+    kind = NVFP4Experts if x.ndim == 3 else NVFP4Weight
+    return kind(codes, scale.view(torch.float8_e4m3fn), second, orig_dtype=x.dtype, is_swizzled_scales=swizzled)
+
+
+def dequantize_fp4(weight: Any, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The values of a packed weight or stack, rounded once to ``dtype`` (default: the weight's original type)."""
+    m, _, q = _matrix(weight)
+    y = torch.empty((*q.shape[:-1], m.cols), dtype=dtype or weight.orig_dtype, device=q.device)
+    dt = _dtype(y, "dequantisation")
+    with _on(q.device):
+        nat.check(nat.load().piper_fp4_dequantize(ctypes.byref(m), y.data_ptr(), dt, nat.current_stream_handle(q.device)))
+    return y
+
+
+# ---------------------------------------------------------------------- products
+def _check_ends(ends: torch.Tensor, batch: int, device: torch.device) -> None:
+    if ends.dtype is not torch.int32 or ends.ndim != 1 or ends.shape[0] != batch or not ends.is_contiguous():
+        raise ValueError("Group ends are one contiguous int32 vector with an entry per expert.")
+    if ends.device != device:
+        raise ValueError("FP4 operators require all tensors on one CUDA device.")
+
+
+def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: torch.Tensor | None) -> torch.Tensor:
+    m, mode, q = _matrix(weight)
+    device = q.device
+    if x.device != device:
+        raise ValueError("FP4 operators require all tensors on one CUDA device.")
+    dt = _dtype(x, "product")
+    if x.ndim < 1 or x.shape[-1] != m.cols:
+        raise ValueError(f"FP4 product: the input has {tuple(x.shape)}, the weight {m.cols} columns.")
+    if act_scale is not None:
+        if m.format != nat.FMT_NV:
+            raise ValueError("MXFP4 activations have no second-level scale.")
+        if act_scale.dtype is not torch.float32 or act_scale.numel() != 1 or act_scale.device != device:
+            raise ValueError("The activations' second-level scale is one float32 value on their device.")
+    x2 = _rows(x)
+    tokens = x2.shape[0]
+    y = torch.empty((*x.shape[:-1], m.rows), dtype=x.dtype, device=device)
+    if tokens == 0:
+        return y
+    lib = nat.load()
+    ref = ctypes.byref(m)
+    ws = _workspace(lib.piper_fp4_linear_workspace, device, ref, tokens)
+    with _on(device):
+        nat.check(lib.piper_fp4_linear(
+            ref, x2.data_ptr(), x2.stride(0), tokens, None if ends is None else ends.data_ptr(),
+            None if act_scale is None else act_scale.data_ptr(), mode, y.data_ptr(), dt, ws.data_ptr(), ws.numel(),
+            nat.current_stream_handle(device)))
+    return y
+
+
+def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> torch.Tensor:
+    m, _, q = _matrix(weight)
+    device = q.device
+    if grad.device != device:
+        raise ValueError("FP4 operators require all tensors on one CUDA device.")
+    dt = _dtype(grad, "gradient")
+    if grad.ndim < 1 or grad.shape[-1] != m.rows:
+        raise ValueError(f"FP4 gradient: the output's gradient has {tuple(grad.shape)}, the weight {m.rows} rows.")
+    g2 = _rows(grad)
+    tokens = g2.shape[0]
+    dx = torch.empty((*grad.shape[:-1], m.cols), dtype=grad.dtype, device=device)
+    if tokens == 0:
+        return dx
+    lib = nat.load()
+    ref = ctypes.byref(m)
+    ws = _workspace(lib.piper_fp4_grad_input_workspace, device, ref, tokens, dt)
+    with _on(device):
+        nat.check(lib.piper_fp4_grad_input(
+            ref, g2.data_ptr(), g2.stride(0), tokens, None if ends is None else ends.data_ptr(), dx.data_ptr(), dt,
+            ws.data_ptr(), ws.numel(), nat.current_stream_handle(device)))
+    return dx
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, ends, act_scale):
+        # saved so that a buffer changed by torch before the backward pass raises instead of giving another's gradient
+        ctx.save_for_backward(weight.qdata, weight.scale, getattr(weight, "per_tensor_scale", None), ends)
+        ctx.weight = weight
+        return _linear(x, weight, ends, act_scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _grad_input(grad, ctx.weight, ctx.saved_tensors[3]), None, None, None
+
+
+def _product(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: torch.Tensor | None) -> torch.Tensor:
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Product.apply(x, weight, ends, act_scale)
+    return _linear(x, weight, ends, act_scale)
+
+
+def linear_fp4(x: torch.Tensor, weight: MXWeight | NVFP4Weight, *,
+               act_per_tensor_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """``quantised(x) @ weight.T`` for ``x`` (..., cols); the result is (..., rows) in the type of ``x``.
+
+    ``x`` is quantised in the weight's format: MXFP4 with the weight's
+    ``act_quant_kwargs.scaling_mode``, NVFP4 with the second-level scale
+    ``act_per_tensor_scale`` where one is given. Differentiable with respect to
+    ``x`` (straight through its quantisation); the weight is constant.
+    """
+    if weight.qdata.ndim != 2:
+        raise ValueError("linear_fp4 takes one weight; grouped_linear_fp4 takes a stack of experts.")
+    return _product(x, weight, None, act_per_tensor_scale)
+
+
+def grouped_linear_fp4(x: torch.Tensor, experts: MXExperts | NVFP4Experts, group_ends: torch.Tensor, *,
+                       act_per_tensor_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`linear_fp4` with a weight per expert over rows sorted by expert.
+
+    ``x`` is (tokens, cols); expert ``e`` has the rows ``group_ends[e - 1]`` to
+    ``group_ends[e]`` (int32 on the device, non-decreasing, not read by the
+    host). Experts may have no rows; rows past the last end come out as zeros.
+    """
+    if experts.qdata.ndim != 3 or x.ndim != 2:
+        raise ValueError("grouped_linear_fp4 takes a stack of experts and rank-two tokens.")
+    _check_ends(group_ends, experts.qdata.shape[0], experts.qdata.device)
+    return _product(x, experts, group_ends, act_per_tensor_scale)
+
+
+def linear_fp4_grad_input(grad: torch.Tensor, weight: MXWeight | NVFP4Weight) -> torch.Tensor:
+    """``grad @ dequantised(weight)`` for ``grad`` (..., rows): :func:`linear_fp4`'s gradient, in the type of ``grad``."""
+    if weight.qdata.ndim != 2:
+        raise ValueError("linear_fp4_grad_input takes one weight; grouped_linear_fp4_grad_input takes a stack of experts.")
+    return _grad_input(grad, weight, None)
+
+
+def grouped_linear_fp4_grad_input(grad: torch.Tensor, experts: MXExperts | NVFP4Experts,
+                                  group_ends: torch.Tensor) -> torch.Tensor:
+    """:func:`grouped_linear_fp4`'s gradient with respect to its tokens; rows past the last end get zeros."""
+    if experts.qdata.ndim != 3 or grad.ndim != 2:
+        raise ValueError("grouped_linear_fp4_grad_input takes a stack of experts and a rank-two gradient.")
+    _check_ends(group_ends, experts.qdata.shape[0], experts.qdata.device)
+    return _grad_input(grad, experts, group_ends)

@@ -189,6 +189,51 @@ class MXWeight:
 
 
 @dataclass
+class NVFP4Experts:
+    """A layer's experts in NVFP4, stacked: ``qdata`` (experts, rows, cols / 2),
+    ``scale`` with one leading axis more than :class:`NVFP4Weight`'s, and one
+    second-level scale per expert. :meth:`expert` gives one of them as a weight
+    over the same storage, so that a merge into it changes the stack."""
+
+    qdata: torch.Tensor
+    scale: torch.Tensor
+    per_tensor_scale: torch.Tensor | None = None
+    block_size: int = 16
+    orig_dtype: torch.dtype = torch.bfloat16
+    is_swizzled_scales: bool = False
+
+    @property
+    def shape(self) -> tuple[int, int, int]:
+        return self.qdata.shape[0], self.qdata.shape[1], self.qdata.shape[2] * 2
+
+    def expert(self, index: int) -> NVFP4Weight:
+        second = None if self.per_tensor_scale is None else self.per_tensor_scale[index:index + 1]
+        return NVFP4Weight(self.qdata[index], self.scale[index], second, self.block_size, self.orig_dtype,
+                           self.is_swizzled_scales)
+
+
+@dataclass
+class MXExperts:
+    """A layer's experts in MXFP4, stacked as :class:`NVFP4Experts` are."""
+
+    qdata: torch.Tensor
+    scale: torch.Tensor
+    elem_dtype: Any
+    block_size: int = 32
+    orig_dtype: torch.dtype = torch.bfloat16
+    is_swizzled_scales: bool = False
+    act_quant_kwargs: Any = field(default_factory=MXActQuantKwargs)
+
+    @property
+    def shape(self) -> tuple[int, int, int]:
+        return self.qdata.shape[0], self.qdata.shape[1], self.qdata.shape[2] * 2
+
+    def expert(self, index: int) -> MXWeight:
+        return MXWeight(self.qdata[index], self.scale[index], self.elem_dtype, self.block_size, self.orig_dtype,
+                        self.is_swizzled_scales, self.act_quant_kwargs)
+
+
+@dataclass
 class GGUFWeight:
     raw: torch.Tensor
     quant_type: int
