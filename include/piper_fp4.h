@@ -63,9 +63,10 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
  * formed in fp32 and rounded once. */
 int piper_fp4_dequantize(const piper_fp4_matrix* m, void* y, int32_t dtype, void* stream);
 
-/* Scratch bytes that piper_fp4_linear / piper_fp4_grad_input need. */
+/* Scratch bytes that piper_fp4_linear / piper_fp4_grad_input need (0: none). */
 int piper_fp4_linear_workspace(const piper_fp4_matrix* w, int64_t tokens, size_t* bytes);
-int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, int64_t tokens, int32_t dtype, size_t* bytes);
+int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, const void* dy, int64_t dy_stride, int64_t tokens,
+                                   int32_t dtype, size_t* bytes);
 
 /* y[t] = w . quantised(x[t]): y is (tokens, rows), x is (tokens, cols) with
  * rows `x_stride` values apart. x is quantised in w's format, with

@@ -82,7 +82,7 @@ def load() -> ctypes.CDLL:
         lib.piper_fp4_quantize.argtypes = [mat, vp, i64, i32, i32, i32, vp, vp]
         lib.piper_fp4_dequantize.argtypes = [mat, vp, i32, vp]
         lib.piper_fp4_linear_workspace.argtypes = [mat, i64, ctypes.POINTER(sz)]
-        lib.piper_fp4_grad_input_workspace.argtypes = [mat, i64, i32, ctypes.POINTER(sz)]
+        lib.piper_fp4_grad_input_workspace.argtypes = [mat, vp, i64, i64, i32, ctypes.POINTER(sz)]
         lib.piper_fp4_linear.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, i32, vp, sz, vp]
         lib.piper_fp4_grad_input.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, sz, vp]
         lib.piper_fp4_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint32)]

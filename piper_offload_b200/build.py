@@ -19,7 +19,7 @@ DEPS = SOURCES + [PKG / "csrc" / "ptx.cuh", PKG / "csrc" / "numerics.cuh", ROOT 
 OUT = PKG / "libpiper_merge.so"
 FP4_SOURCES = [PKG / "csrc" / "fp4.cu"]
 FP4_DEPS = FP4_SOURCES + [
-    *(PKG / "csrc" / n for n in ("fp4_quant.cuh", "fp4_linear.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
+    *(PKG / "csrc" / n for n in ("fp4_quant.cuh", "fp4_tiles.cuh", "fp4_linear.cuh", "fp4_grad.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
     ROOT / "include" / "piper_fp4.h",
 ]
 FP4_OUT = PKG / "libpiper_fp4.so"

@@ -10,6 +10,7 @@
 #include <cstring>
 #include <string>
 
+#include "fp4_grad.cuh"
 #include "fp4_linear.cuh"
 #include "fp4_quant.cuh"
 
@@ -141,6 +142,11 @@ bool code_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t pit
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Token tiles of all experts and of the rows after them: an upper bound where the ends are on the device.
+int64_t token_tiles(const fp4::Groups& g, int bn) {
+  return g.ends == nullptr ? (g.tokens + bn - 1) / bn : g.tokens / bn + std::min<int64_t>(g.experts + 1, g.tokens);
+}
+
 template <int DT, int FMT, int BN>
 cudaError_t launch_linear(const fp4::LinearArgs& args, int64_t items, cudaStream_t stream) {
   using S = fp4::LinearShape<FMT, BN>;
@@ -148,6 +154,33 @@ cudaError_t launch_linear(const fp4::LinearArgs& args, int64_t items, cudaStream
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   kernel<<<static_cast<unsigned>(items), fp4::kLinearThreads, S::kSmem, stream>>>(args);
+  return launched();
+}
+
+// --------------------------------------------------------------- the gradient
+struct GradPlan {
+  bool move;      // dy goes through the workspace
+  int terms;      // bf16 terms per value
+  int64_t pitch;  // values between its rows there
+  int64_t total;  // bytes
+};
+
+GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, int64_t tokens, int dtype) {
+  GradPlan p{};
+  p.terms = dtype == PIPER_FP4_F32 ? 3 : 1;
+  p.move = p.terms > 1 || !aligned(dy, 16) || (stride % 8 != 0 && tokens > 1);
+  p.pitch = up(w.rows, 8);
+  p.total = p.move ? align256(p.terms * tokens * p.pitch * 2) : 0;
+  return p;
+}
+
+template <int DT, int FMT, int BN>
+cudaError_t launch_grad(const fp4::GradArgs& args, int64_t items, cudaStream_t stream) {
+  using S = fp4::GradShape<BN>;
+  auto kernel = fp4::grad_kernel<DT, FMT, BN>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  kernel<<<static_cast<unsigned>(items), fp4::kGradThreads, S::kSmem, stream>>>(args);
   return launched();
 }
 
@@ -280,8 +313,6 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   q.second = const_cast<float*>(act_second);
   q.ends = ends;
   q.experts = static_cast<int32_t>(w->batch);
-  q.y = y;
-  q.y_cols = w->rows;
   fp4::RepackArgs r{};
   r.codes = static_cast<const uint8_t*>(w->codes);
   r.code_row = w->cols / 2;
@@ -314,17 +345,12 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   a.x_scale = q.scale;
   a.w_second = w->second;
   a.x_second = act_second;
-  a.ends = ends;
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->rows + 127) / 128)};
   a.y = y;
-  a.tokens = tokens;
   a.rows = static_cast<int32_t>(w->rows);
-  a.row_tiles = static_cast<int32_t>((w->rows + 127) / 128);
   a.k_steps = static_cast<int32_t>((w->cols + 63) / 64);
   a.scale_tiles = static_cast<int32_t>(p.scale_tiles);
-  a.experts = static_cast<int32_t>(w->batch);
-  // with experts: an upper bound on the token tiles, as the ends are on the device
-  const int64_t token_tiles = ends == nullptr ? (tokens + bn - 1) / bn : tokens / bn + std::min(w->batch, tokens);
-  const int64_t items = token_tiles * a.row_tiles;
+  const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
   FP4_REQUIRE(items < (int64_t{1} << 31), "FP4 product: too many tiles for one call.");
 
 #define CALL(D, F) \
@@ -341,13 +367,74 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("linear kernel", e);
 }
 
-int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, int64_t tokens, int32_t dtype, size_t* bytes) {
-  return fail(PIPER_FP4_EINVAL, "FP4 gradient: not built.");
+int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, const void* dy, int64_t dy_stride, int64_t tokens,
+                                   int32_t dtype, size_t* bytes) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(bytes != nullptr && tokens >= 0, "FP4 gradient: bad workspace query.");
+  *bytes = static_cast<size_t>(plan_grad(*w, dy, dy_stride, tokens, dtype).total);
+  return PIPER_FP4_OK;
 }
+
 int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_stride, int64_t tokens,
                          const int32_t* ends, void* dx, int32_t dtype, void* workspace, size_t workspace_bytes,
                          void* stream) {
-  return fail(PIPER_FP4_EINVAL, "FP4 gradient: not built.");
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_buffers(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 29), "FP4 gradient: too many tokens for one call.");
+  if (tokens == 0) return PIPER_FP4_OK;
+  FP4_REQUIRE(dy != nullptr && dx != nullptr, "FP4 gradient: null gradient or output.");
+  FP4_REQUIRE(dy_stride >= w->rows || tokens == 1, "FP4 gradient: rows of the gradient overlap.");
+  FP4_REQUIRE(ends != nullptr || w->batch == 1, "FP4 gradient: several matrices need the ends of their rows.");
+  const GradPlan p = plan_grad(*w, dy, dy_stride, tokens, dtype);
+  if (p.total > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256)))
+    return fail(PIPER_FP4_EWORKSPACE, "FP4 gradient: workspace missing, too small or not 256-byte aligned.");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  fp4::GradArgs a{};
+  a.codes = static_cast<const uint8_t*>(w->codes);
+  a.scale = static_cast<const uint8_t*>(w->scale);
+  a.second = w->second;
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 127) / 128)};
+  a.dx = dx;
+  a.code_pitch = w->cols / 2;
+  a.rows = static_cast<int32_t>(w->rows);
+  a.cols = static_cast<int32_t>(w->cols);
+  a.swizzled = w->swizzled != 0;
+  a.scale_cols = scale_cols(*w);
+  a.terms = p.terms;
+  a.piece = aligned(w->codes, 16) && a.code_pitch % 16 == 0 ? 16 : aligned(w->codes, 8) ? 8 : 1;
+
+  const int64_t per_expert = tokens / w->batch;
+  const int bn = per_expert <= 32 ? 32 : per_expert <= 128 ? 128 : 256;
+  const void* src = p.move ? workspace : dy;
+  const int64_t pitch = p.move ? p.pitch : tokens > 1 ? dy_stride : up(w->rows, 8);
+  const auto enc = tensor_map_encoder();
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(w->rows), static_cast<cuuint64_t>(p.terms * tokens)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch * 2)};
+  const cuuint32_t box[2] = {fp4::kGradStageRows, static_cast<cuuint32_t>(bn)};
+  const cuuint32_t one[2] = {1u, 1u};
+  if (enc == nullptr || enc(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(src), dims, strides, box, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(PIPER_FP4_ECUDA, "FP4 gradient: cuTensorMapEncodeTiled failed.");
+  const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
+  const int64_t split_blocks = tokens * ((w->rows + 255) / 256);
+  FP4_REQUIRE(items < (int64_t{1} << 31) && split_blocks < (int64_t{1} << 31), "FP4 gradient: too many tiles for one call.");
+  cudaError_t e = cudaSuccess;
+  if (p.move) {
+    auto kernel = dtype == PIPER_FP4_BF16 ? fp4::split_kernel<fp4::kBF16> : fp4::split_kernel<fp4::kF32>;
+    kernel<<<static_cast<unsigned>(split_blocks), 256, 0, s>>>(dy, dy_stride, tokens, a.rows, p.pitch,
+                                                               static_cast<__nv_bfloat16*>(workspace));
+    if ((e = launched()) != cudaSuccess) return cuda_fail("split kernel", e);
+  }
+#define CALL(D, F)                                    \
+  e = bn == 32 ? launch_grad<D, F, 32>(a, items, s)   \
+               : bn == 128 ? launch_grad<D, F, 128>(a, items, s) : launch_grad<D, F, 256>(a, items, s)
+  FP4_DISPATCH(dtype, w->format, CALL);
+#undef CALL
+  return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("gradient kernel", e);
 }
 
 const char* piper_fp4_last_error(void) { return g_error.c_str(); }

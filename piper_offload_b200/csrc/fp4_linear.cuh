@@ -14,14 +14,13 @@
 
 #include "fp4_ptx.cuh"
 #include "fp4_quant.cuh"
+#include "fp4_tiles.cuh"
 
 namespace fp4 {
 
-constexpr int kTileRows = 128;       // weight rows per tile
 constexpr int kStageCols = 256;      // K values per stage
 constexpr int kStageBytes = kStageCols / 2;
 constexpr int kLinearThreads = 192;  // producer warp, tensor-core warp, four epilogue warps
-constexpr int kSmemMax = 232448;
 
 struct LinearArgs {
   CUtensorMap w_map, x_map;
@@ -29,15 +28,11 @@ struct LinearArgs {
   const uint8_t* x_scale;  // swizzled tiles, experts on 128-row tiles
   const float* w_second;   // (experts) or NULL
   const float* x_second;   // one or NULL
-  const int32_t* ends;     // (experts) or NULL
+  Groups groups;           // row tiles: of 128 outputs
   void* y;
-  int64_t tokens;
   int32_t rows;            // outputs per expert
-  int32_t row_tiles;
   int32_t k_steps;         // of 64 values
   int32_t scale_tiles;     // tiles of 4 scales per row (weight and tokens alike)
-  int32_t experts;
-  int32_t early;           // the weight's buffers are the caller's own, written before this pair of launches
 };
 
 template <int FMT, int BN>
@@ -58,71 +53,6 @@ struct LinearShape {
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
-struct TileAt {
-  int32_t expert, row_tile;
-  int32_t first, count;  // token rows of the tile
-  int32_t scale_row;     // row of the tile's first token in the padded scale buffer
-};
-
-// The tile of work item `id`: token tiles are the inner index, so that the
-// tiles of one weight strip run together and its bytes are read from HBM once.
-// One warp calls; false past the last item.
-__device__ __forceinline__ bool find_tile(const LinearArgs& p, int id, int bn, TileAt& t) {
-  if (p.ends == nullptr) {
-    const int per = static_cast<int>((p.tokens + bn - 1) / bn);
-    t.expert = 0;
-    t.row_tile = id / per;
-    const int nt = id - t.row_tile * per;
-    t.first = nt * bn;
-    t.count = min(static_cast<int64_t>(bn), p.tokens - t.first);
-    t.scale_row = t.first;
-    return t.row_tile < p.row_tiles;
-  }
-  const int lane = threadIdx.x & 31;
-  int64_t before = 0;
-  for (int e0 = 0; e0 < p.experts; e0 += 32) {
-    const int e = e0 + lane;
-    int start = 0, n = 0;
-    if (e < p.experts) {
-      const int tk = static_cast<int>(p.tokens);
-      start = e > 0 ? min(max(p.ends[e - 1], 0), tk) : 0;
-      n = max(min(max(p.ends[e], 0), tk) - start, 0);
-    }
-    const int per = (n + bn - 1) / bn;
-    int64_t sum = static_cast<int64_t>(per) * p.row_tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + sum > id);
-    if (hit != 0u) {
-      const int l = __ffs(hit) - 1;
-      const int64_t base = before + __shfl_sync(0xFFFFFFFFu, sum, l) -
-                           static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, per, l)) * p.row_tiles;
-      const int per_l = __shfl_sync(0xFFFFFFFFu, per, l);
-      const int start_l = __shfl_sync(0xFFFFFFFFu, start, l);
-      const int n_l = __shfl_sync(0xFFFFFFFFu, n, l);
-      const int in = static_cast<int>(id - base);
-      t.expert = e0 + l;
-      t.row_tile = in / per_l;
-      const int nt = in - t.row_tile * per_l;
-      t.first = start_l + nt * bn;
-      t.count = min(bn, n_l - nt * bn);
-      t.scale_row = static_cast<int>(padded_start(start_l, t.expert)) + nt * bn;
-      return true;
-    }
-    before += __shfl_sync(0xFFFFFFFFu, sum, 31);
-  }
-  return false;
-}
-
-template <int DT>
-__device__ __forceinline__ void store_value(void* y, int64_t at, float v) {
-  if constexpr (DT == kBF16) static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
-  else static_cast<float*>(y)[at] = v;
-}
-
 template <int DT, int FMT, int BN>
 __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
     linear_kernel(const __grid_constant__ LinearArgs p) {
@@ -139,7 +69,7 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     TileAt t;
-    const bool ok = find_tile(p, blockIdx.x, BN, t);
+    const bool ok = find_tile(p.groups, blockIdx.x, BN, t);
     if (lane == 0) {
       *have = ok;
       if (ok) *shared_tile = t;
@@ -165,12 +95,14 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
   // token columns that the tensor core computes
   const uint32_t n_mma = static_cast<uint32_t>((t.count + 15) & ~15);
 
-  if (*have) {
+  if (*have && t.expert == p.groups.experts) {
+    store_zeros<DT>(p.y, t, p.rows);
+  } else if (*have) {
     if (warp == 0) {
       if (lane == 0) {
         const int64_t w_row = static_cast<int64_t>(t.expert) * p.rows + t.row_tile * kTileRows;
         const uint8_t* w_scale =
-            p.w_scale + (static_cast<int64_t>(t.expert) * p.row_tiles + t.row_tile) * p.scale_tiles * 512;
+            p.w_scale + (static_cast<int64_t>(t.expert) * p.groups.row_tiles + t.row_tile) * p.scale_tiles * 512;
         const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(t.scale_row >> 7) * p.scale_tiles * 512;
         grid_wait();
         int issued = 0;
@@ -229,22 +161,9 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
       float alpha = 1.0f;
       if (p.w_second != nullptr) alpha = p.w_second[t.expert];
       if (p.x_second != nullptr) alpha *= *p.x_second;
-      const int n = t.row_tile * kTileRows + (warp & 3) * 32 + lane;
       const bool ok = pm::mbar_wait(done, 0, pm::kStatusTimeoutMma);
       pm::tc_fence_after();
-      if (__all_sync(0xFFFFFFFFu, ok)) {
-        const uint32_t from = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        for (int c = 0; c < t.count; c += 32) {
-          float v[32];
-          pm::tmem_ld32(from + c, v);
-          if (n < p.rows) {
-            const int64_t at = static_cast<int64_t>(t.first + c) * p.rows + n;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < t.count) store_value<DT>(p.y, at + static_cast<int64_t>(j) * p.rows, v[j] * alpha);
-          }
-        }
-      }
+      if (__all_sync(0xFFFFFFFFu, ok)) store_tile<DT>(tmem, p.y, t, p.rows, alpha, 0, BN);
       pm::tc_fence_before();
     }
   }

@@ -79,8 +79,6 @@ struct QuantArgs {
   // tokens of experts
   const int32_t* ends;   // NULL: rows as they are
   int32_t experts;
-  void* y;               // rows past the last expert become zero
-  int64_t y_cols;
 };
 
 template <int DT>
@@ -249,18 +247,11 @@ __device__ void quantize_octets(const QuantArgs& q, int64_t first) {
     if (!inside[u]) continue;
 
     int64_t srow = rin;
-    bool live = rin < q.rows;
+    const bool live = rin < q.rows;
     if (q.ends != nullptr) {
       const int x = expert_of_row(q.ends, q.experts, rin);
       const int64_t start = x > 0 ? q.ends[x - 1] : 0;
-      if (x >= q.experts || start < 0 || start > rin) {  // no expert: its output row is zero
-        const int64_t at = rin * q.y_cols;
-        for (int64_t n = oct[u]; n < q.y_cols; n += q.octets) {
-          if constexpr (DT == kBF16) static_cast<uint16_t*>(q.y)[at + n] = 0;
-          else static_cast<float*>(q.y)[at + n] = 0.0f;
-        }
-        continue;
-      }
+      if (x >= q.experts || start < 0 || start > rin) continue;  // a row of no expert
       srow = padded_start(start, x) + (rin - start);
     }
     const int c = static_cast<int>(oct[u]) / kLanes;

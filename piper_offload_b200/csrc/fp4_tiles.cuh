@@ -1,0 +1,114 @@
+// fp4_tiles.cuh - which tile a block works on, shared by the FP4 products and gradients.
+#pragma once
+#include "fp4_quant.cuh"
+
+namespace fp4 {
+
+constexpr int kTileRows = 128;  // weight rows (or columns, for a gradient) per tile
+constexpr int kSmemMax = 232448;
+
+// Tokens split among experts, and how many row tiles each expert's weight has.
+struct Groups {
+  const int32_t* ends;  // (experts) or NULL: one weight for all tokens
+  int64_t tokens;
+  int32_t experts;
+  int32_t row_tiles;
+};
+
+struct TileAt {
+  int32_t expert;        // == experts: rows of no expert, whose results are zero
+  int32_t row_tile;
+  int32_t first, count;  // token rows of the tile
+  int32_t scale_row;     // row of the tile's first token in a scale buffer whose experts start on 128-row tiles
+};
+
+// The tile of work item `id`: token tiles are the inner index, so that the
+// tiles of one weight strip run together and its bytes are read from HBM once.
+// One warp calls; false past the last item. The ends are used as they are
+// found: values out of order give other rows' results, never an address
+// outside the buffers.
+__device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileAt& t) {
+  const int tokens = static_cast<int>(p.tokens);
+  if (p.ends == nullptr) {
+    const int per = (tokens + bn - 1) / bn;
+    t.expert = 0;
+    t.row_tile = id / per;
+    const int nt = id - t.row_tile * per;
+    t.first = t.scale_row = nt * bn;
+    t.count = min(bn, tokens - t.first);
+    return t.row_tile < p.row_tiles;
+  }
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+    const int e = e0 + lane;
+    int start = 0, n = 0;
+    if (e <= p.experts) {
+      start = e > 0 ? min(max(p.ends[e - 1], 0), tokens) : 0;
+      n = max((e < p.experts ? min(max(p.ends[e], 0), tokens) : tokens) - start, 0);
+    }
+    const int per = (n + bn - 1) / bn;
+    int64_t sum = static_cast<int64_t>(per) * p.row_tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + sum > id);
+    if (hit != 0u) {
+      const int l = __ffs(hit) - 1;
+      const int per_l = __shfl_sync(0xFFFFFFFFu, per, l);
+      const int start_l = __shfl_sync(0xFFFFFFFFu, start, l);
+      const int n_l = __shfl_sync(0xFFFFFFFFu, n, l);
+      const int64_t base = before + __shfl_sync(0xFFFFFFFFu, sum, l) - static_cast<int64_t>(per_l) * p.row_tiles;
+      const int in = static_cast<int>(id - base);
+      t.expert = e0 + l;
+      t.row_tile = in / per_l;
+      const int nt = in - t.row_tile * per_l;
+      t.first = start_l + nt * bn;
+      t.count = min(bn, n_l - nt * bn);
+      t.scale_row = static_cast<int>(padded_start(start_l, t.expert)) + nt * bn;
+      return true;
+    }
+    before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  return false;
+}
+
+template <int DT>
+__device__ __forceinline__ void store_value(void* y, int64_t at, float v) {
+  if constexpr (DT == kBF16) static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+  else static_cast<float*>(y)[at] = v;
+}
+
+// A whole block zeroes its tile of y (tokens x cols).
+template <int DT>
+__device__ __forceinline__ void store_zeros(void* y, const TileAt& t, int cols) {
+  const int c0 = t.row_tile * kTileRows, n = min(kTileRows, cols - c0);
+  for (int i = threadIdx.x; i < t.count * kTileRows; i += blockDim.x)
+    if ((i & (kTileRows - 1)) < n)
+      store_value<DT>(y, static_cast<int64_t>(t.first + i / kTileRows) * cols + c0 + (i & (kTileRows - 1)), 0.0f);
+}
+
+// Four epilogue warps' share of a finished tile: tensor-memory lane = column of
+// y, tensor-memory column = token. A warp stores 32 neighbouring outputs of
+// one token at a time: whole 64-byte (bf16) or 128-byte runs.
+template <int DT>
+__device__ __forceinline__ void store_tile(uint32_t tmem, void* y, const TileAt& t, int cols, float alpha, int from_col,
+                                           int to_col) {
+  const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int n = t.row_tile * kTileRows + quarter * 32 + lane;
+  const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  for (int c = from_col; c < min(to_col, t.count); c += 32) {
+    float v[32];
+    pm::tmem_ld32(at + c, v);
+    if (n < cols) {
+      const int64_t base = static_cast<int64_t>(t.first + c) * cols + n;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c + j < t.count) store_value<DT>(y, base + static_cast<int64_t>(j) * cols, v[j] * alpha);
+    }
+  }
+}
+
+}  // namespace fp4

@@ -264,7 +264,7 @@ def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> t
         return dx
     lib = nat.load()
     ref = ctypes.byref(m)
-    ws = _workspace(lib.piper_fp4_grad_input_workspace, device, ref, tokens, dt)
+    ws = _workspace(lib.piper_fp4_grad_input_workspace, device, ref, g2.data_ptr(), g2.stride(0), tokens, dt)
     with _on(device):
         nat.check(lib.piper_fp4_grad_input(
             ref, g2.data_ptr(), g2.stride(0), tokens, None if ends is None else ends.data_ptr(), dx.data_ptr(), dt,
