@@ -44,6 +44,26 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
+// Encodes a 2-D map of 128-byte wide, 128-byte swizzled boxes. The encoder wants
+// a current context, which a thread that has made no runtime call yet (autograd's
+// own, for one) lacks: then the runtime makes its device's current first.
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t pitch_bytes,
+                int box_cols, int box_rows) {
+  const auto enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t one[2] = {1u, 1u};
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    if (enc(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+      return true;
+    if (cudaFree(nullptr) != cudaSuccess) return false;
+  }
+  return false;
+}
+
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 int64_t align256(int64_t a) { return up(a, 256); }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -100,6 +120,7 @@ int scale_cols(const piper_fp4_matrix& m) {
 // Scratch of a product: quantized tokens, and the weight's parts that are not
 // stored as the product reads them.
 struct LinearPlan {
+  int bn, token_tile;                  // tokens per tile; per 128-row tile of scales
   bool move_codes, move_scale;
   int64_t k_padded;                    // columns up to a whole scale tile
   int64_t x_codes, x_scale, w_codes, w_scale, total;  // byte offsets
@@ -108,14 +129,17 @@ struct LinearPlan {
 
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
+  const int64_t per_expert = tokens / w.batch;
+  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 256;
+  p.token_tile = std::min(p.bn, 128);
   const int tile = block_of(w) * 4;
   p.scale_tiles = (w.cols + tile - 1) / tile;
   p.k_padded = p.scale_tiles * tile;
   p.move_codes = w.cols % 32 != 0 || !aligned(w.codes, 16);
   p.move_scale = !w.swizzled || w.cols % 64 != 0 || !aligned(w.scale, 16);
   p.w_code_pitch = up(w.cols / 2, 16);
-  // every expert starts on a tile of 128 token rows; one more for a second tile that is read and not used
-  p.scale_rows = (tokens / 128 + w.batch + 2) * 128;
+  // first_scale_row's numbers end below this; one more for a second tile that is read and not used
+  p.scale_rows = (tokens / p.token_tile + w.batch + 2) * 128;
   int64_t at = 0;
   p.x_codes = at;
   at += align256(tokens * (p.k_padded / 2));
@@ -131,15 +155,7 @@ LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
 
 // Map of rows of packed codes, in boxes of 256 values x `box_rows` rows with the 128-byte swizzle.
 bool code_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t pitch, int64_t rows, int box_rows) {
-  const auto enc = tensor_map_encoder();
-  if (enc == nullptr) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-  const cuuint32_t box[2] = {fp4::kStageBytes, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t one[2] = {1u, 1u};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, row_bytes, rows, pitch, fp4::kStageBytes, box_rows);
 }
 
 // Token tiles of all experts and of the rows after them: an upper bound where the ends are on the device.
@@ -282,7 +298,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   if (int rc = check_matrix(w)) return rc;
   if (int rc = check_buffers(w)) return rc;
   if (int rc = check_dtype(dtype)) return rc;
-  FP4_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 31) - w->batch * 128 - 1024, "FP4 product: too many tokens for one call.");
+  FP4_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 28) && w->batch <= (int64_t{1} << 20), "FP4 product: too many tokens for one call.");
   if (tokens == 0) return PIPER_FP4_OK;
   FP4_REQUIRE(x != nullptr && y != nullptr, "FP4 product: null input or output.");
   FP4_REQUIRE(x_stride >= w->cols || tokens == 1, "FP4 product: rows of the input overlap.");
@@ -311,6 +327,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   q.scale_mode = scale_mode;
   q.second_mode = act_second != nullptr ? PIPER_FP4_SECOND_GIVEN : PIPER_FP4_SECOND_NONE;
   q.second = const_cast<float*>(act_second);
+  q.token_tile = p.token_tile;
   q.ends = ends;
   q.experts = static_cast<int32_t>(w->batch);
   fp4::RepackArgs r{};
@@ -335,8 +352,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 product: too many values for one call.");
 
   fp4::LinearArgs a{};
-  const int64_t per_expert = tokens / w->batch;
-  const int bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 256;
+  const int bn = p.bn;
   const void* codes = p.move_codes ? ws + p.w_codes : w->codes;
   if (!code_map(&a.w_map, codes, p.w_code_pitch, p.w_code_pitch, w->batch * w->rows, fp4::kTileRows) ||
       !code_map(&a.x_map, q.codes, q.code_pitch, q.code_pitch, tokens, bn))
@@ -410,14 +426,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   const int bn = per_expert <= 32 ? 32 : per_expert <= 128 ? 128 : 256;
   const void* src = p.move ? workspace : dy;
   const int64_t pitch = p.move ? p.pitch : tokens > 1 ? dy_stride : up(w->rows, 8);
-  const auto enc = tensor_map_encoder();
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(w->rows), static_cast<cuuint64_t>(p.terms * tokens)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch * 2)};
-  const cuuint32_t box[2] = {fp4::kGradStageRows, static_cast<cuuint32_t>(bn)};
-  const cuuint32_t one[2] = {1u, 1u};
-  if (enc == nullptr || enc(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(src), dims, strides, box, one,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+  if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, src, w->rows, p.terms * tokens, pitch * 2, fp4::kGradStageRows, bn))
     return fail(PIPER_FP4_ECUDA, "FP4 gradient: cuTensorMapEncodeTiled failed.");
   const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
   const int64_t split_blocks = tokens * ((w->rows + 255) / 256);

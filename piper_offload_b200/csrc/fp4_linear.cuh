@@ -25,7 +25,7 @@ constexpr int kLinearThreads = 192;  // producer warp, tensor-core warp, four ep
 struct LinearArgs {
   CUtensorMap w_map, x_map;
   const uint8_t* w_scale;  // swizzled tiles, experts on 128-row tiles
-  const uint8_t* x_scale;  // swizzled tiles, experts on 128-row tiles
+  const uint8_t* x_scale;  // swizzled tiles, rows as first_scale_row places them
   const float* w_second;   // (experts) or NULL
   const float* x_second;   // one or NULL
   Groups groups;           // row tiles: of 128 outputs
@@ -128,7 +128,6 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
       __syncwarp();
     } else if (warp == 1) {
       if (lane == 0) {
-        const uint32_t x_col = static_cast<uint32_t>(t.scale_row & 127) >> 5;  // where the tokens begin in their tile
         for (int i = 0; i < stages; ++i) {
           const int s = i % S::kStages;
           // the scale buffer's last readers, two stages ago, have finished
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
           for (int j = 0; j < steps; ++j) {
             const uint32_t tile = FMT == kNV ? j : j >> 1, id = FMT == kNV ? 0u : (j & 1) * 2u;
             umma_fp4<FMT>(tmem, a + j * 2, b + j * 2, idesc_fp4(kTileRows, n_mma, FMT == kMX, id), sw + tile * 4,
-                          sx + tile * 4 * S::kXBlocks + x_col, (i | j) != 0);
+                          sx + tile * 4 * S::kXBlocks, (i | j) != 0);
           }
           pm::umma_commit(&empty[s]);
         }

@@ -15,7 +15,8 @@ __device__ __forceinline__ constexpr uint32_t idesc_fp4(uint32_t m, uint32_t n, 
 }
 
 // D += A * B over K = 64 with one scale per 16 (NVFP4, four scale bytes of a
-// column) or per 32 values (MXFP4, two bytes).
+// column) or per 32 values (MXFP4, two bytes). The scales' tensor-memory
+// addresses are multiples of four columns.
 template <int FMT>
 __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                          uint32_t accumulate) {

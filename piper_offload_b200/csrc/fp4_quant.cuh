@@ -4,7 +4,8 @@
 // times one scale. With a = max|x| over the block:
 //   MXFP4  scale 2^(e - 127), e from the exponent of a (scale_mode);
 //   NVFP4  scale u = e4m3(clamp(a / 6 [/ g], 2^-6, 448)), g the second level;
-//   code = e2m1(x / scale), nearest, ties to even, saturating at 6.
+//   code = e2m1(x / scale), nearest, ties to even, saturating at 6; with a
+//   second level x * ((1 / g) / u), each step rounded to fp32.
 // These are the merges' formulas (numerics.cuh), with IEEE quotients, and one
 // rule of its own: a NaN in a block makes its scale NaN (e8m0 255, e4m3 127),
 // so the whole block and what is computed from it read as NaN.
@@ -39,10 +40,12 @@ __host__ __device__ __forceinline__ int64_t swizzled_byte(int64_t r, int64_t c, 
   return ((r >> 7) * ct + (c >> 2)) * 512 + (rin & 31) * 16 + (rin >> 5) * 4 + static_cast<int>(c & 3);
 }
 
-// First row of expert e's rows in a buffer of scales whose experts start on
-// 128-row tiles. With ceil(n / 128) tiles of n rows, floor(start / 128) + e
-// tiles always lie before expert e, so no scan over the experts is needed.
-__host__ __device__ __forceinline__ int64_t padded_start(int64_t start, int64_t e) { return ((start >> 7) + e) << 7; }
+// Scale rows of tokens. Every run of `tile` (at most 128) tokens of an expert
+// starts on a 128-row tile of scales, because the tensor core reads them from
+// its tile's first column. Expert e's first run is number start / tile + e:
+// with ceil(n / tile) runs of n rows, at least that many numbers lie before
+// it, so no scan over the experts is needed.
+__host__ __device__ __forceinline__ int64_t first_scale_row(int64_t start, int64_t e, int tile) { return (start / tile + e) * 128; }
 
 // Expert whose rows hold row t (the first with ends[e] > t, or `experts`).
 __device__ __forceinline__ int expert_of_row(const int32_t* ends, int experts, int64_t t) {
@@ -77,8 +80,9 @@ struct QuantArgs {
   float* second;         // (batch): read (given) or written (compute)
   const uint32_t* amax;  // (batch) bits of max|x| (compute)
   // tokens of experts
-  const int32_t* ends;   // NULL: rows as they are
+  const int32_t* ends;   // NULL: one weight for all
   int32_t experts;
+  int32_t token_tile;    // 0: rows are a weight's; else tokens in runs of so many (first_scale_row)
 };
 
 template <int DT>
@@ -124,7 +128,8 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax, int mode) {
   if (mode == kRceil) bits = __float_as_uint(__fdiv_rn(__uint_as_float(amax), 6.0f));
   else if (mode == kEven) bits += 1u << 21;
   int e = static_cast<int>(bits >> 23);
-  if ((mode == kRceil || mode == kCeil) && (bits & 0x7FFFFFu) != 0u) ++e;
+  // above a power of two; 2^-127, the least scale, is half the least normal number
+  if ((mode == kRceil || mode == kCeil) && (bits & 0x7FFFFFu) > (e == 0 ? 1u << 22 : 0u)) ++e;
   if (mode != kRceil) e -= 2;
   return static_cast<uint32_t>(min(max(e, 0), 254));
 }
@@ -240,19 +245,26 @@ __device__ void quantize_octets(const QuantArgs& q, int64_t first) {
       inv_g = __fdiv_rn(1.0f, g);
     }
     const Scaled<FMT> s = quantize8<FMT>(v[u], q.scale_mode, two, g, inv_g);
+    const bool live = rin < q.rows;
+    const bool padding = !live || static_cast<int>(oct[u]) * 8 >= q.cols;
+    const uint32_t byte = padding ? 0u : s.byte;
     // gather the scales of this lane and the next three blocks
-    uint32_t word = s.byte;
+    uint32_t word = byte;
     word |= __shfl_down_sync(0xFFFFFFFFu, word, kLanes) << 8;
     word |= __shfl_down_sync(0xFFFFFFFFu, word, 2 * kLanes) << 16;
     if (!inside[u]) continue;
 
     int64_t srow = rin;
-    const bool live = rin < q.rows;
-    if (q.ends != nullptr) {
-      const int x = expert_of_row(q.ends, q.experts, rin);
-      const int64_t start = x > 0 ? q.ends[x - 1] : 0;
-      if (x >= q.experts || start < 0 || start > rin) continue;  // a row of no expert
-      srow = padded_start(start, x) + (rin - start);
+    if (q.token_tile != 0) {
+      int x = 0;
+      int64_t start = 0;
+      if (q.ends != nullptr) {
+        x = expert_of_row(q.ends, q.experts, rin);
+        start = x > 0 ? q.ends[x - 1] : 0;
+        if (x >= q.experts || start < 0 || start > rin) continue;  // a row of no expert
+      }
+      const int o = static_cast<int>(rin - start);
+      srow = first_scale_row(start, x, q.token_tile) + static_cast<int64_t>(o / q.token_tile) * 128 + o % q.token_tile;
     }
     const int c = static_cast<int>(oct[u]) / kLanes;
     const int lanes = static_cast<int>(oct[u]) % kLanes;
@@ -262,17 +274,17 @@ __device__ void quantize_octets(const QuantArgs& q, int64_t first) {
       if (words) {
         if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
       } else if (lanes == 0) {
-        *at = static_cast<uint8_t>(s.byte);
+        *at = static_cast<uint8_t>(byte);
       }
     } else {
       uint8_t* at = q.scale + (e * q.rows + rin) * q.scale_cols + c;
       if (words) {
         if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
       } else if (lanes == 0) {
-        *at = static_cast<uint8_t>(s.byte);
+        *at = static_cast<uint8_t>(byte);
       }
     }
-    if (live && (q.pad_codes || static_cast<int>(oct[u]) * 8 < q.cols))
+    if (live && (q.pad_codes || !padding))
       *reinterpret_cast<uint32_t*>(q.codes + (e * q.rows + rin) * q.code_pitch + oct[u] * 4) = s.codes;
   }
 }

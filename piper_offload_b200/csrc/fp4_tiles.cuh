@@ -19,7 +19,7 @@ struct TileAt {
   int32_t expert;        // == experts: rows of no expert, whose results are zero
   int32_t row_tile;
   int32_t first, count;  // token rows of the tile
-  int32_t scale_row;     // row of the tile's first token in a scale buffer whose experts start on 128-row tiles
+  int32_t scale_row;     // scale row of the tile's first token (first_scale_row), a multiple of 128
 };
 
 // The tile of work item `id`: token tiles are the inner index, so that the
@@ -34,7 +34,8 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
     t.expert = 0;
     t.row_tile = id / per;
     const int nt = id - t.row_tile * per;
-    t.first = t.scale_row = nt * bn;
+    t.first = nt * bn;
+    t.scale_row = nt * max(bn, 128);
     t.count = min(bn, tokens - t.first);
     return t.row_tile < p.row_tiles;
   }
@@ -67,7 +68,7 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
       const int nt = in - t.row_tile * per_l;
       t.first = start_l + nt * bn;
       t.count = min(bn, n_l - nt * bn);
-      t.scale_row = static_cast<int>(padded_start(start_l, t.expert)) + nt * bn;
+      t.scale_row = static_cast<int>(first_scale_row(start_l, t.expert, min(bn, 128))) + nt * max(bn, 128);
       return true;
     }
     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
