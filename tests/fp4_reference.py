@@ -58,7 +58,7 @@ def mx_scale(top: np.ndarray, mode: str) -> np.ndarray:
 def quantize(x: np.ndarray, fmt: str, *, mode: str = "floor", second: float | None = None):
     """(codes (rows, cols), scale bytes (rows, blocks)) of a float64 matrix holding the input's exact values."""
     rows, cols = x.shape
-    b = x.reshape(rows, -1, BLOCK[fmt])
+    b = x.reshape(rows, cols // BLOCK[fmt], BLOCK[fmt])
     top = np.where(np.isnan(b).any(-1), np.nan, np.abs(np.where(np.isnan(b), 0, b)).max(-1))
     with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
         if fmt == "mxfp4":
