@@ -94,6 +94,18 @@ int check_dtype(int dtype) {
   return PIPER_FP4_OK;
 }
 
+int sm_count() {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> cached[kMaxDevices] = {};
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < kMaxDevices && (n = cached[dev].load(std::memory_order_relaxed)) > 0) return n;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  n = n > 0 ? n : 148;
+  if (dev >= 0 && dev < kMaxDevices) cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 cudaError_t launched() {
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return cudaGetLastError();
@@ -120,7 +132,7 @@ int scale_cols(const piper_fp4_matrix& m) {
 // Scratch of a product: quantized tokens, and the weight's parts that are not
 // stored as the product reads them.
 struct LinearPlan {
-  int bn, token_tile;                  // tokens per tile; per 128-row tile of scales
+  int bn;                              // tokens per tile
   bool move_codes, move_scale;
   int64_t k_padded;                    // columns up to a whole scale tile
   int64_t x_codes, x_scale, w_codes, w_scale, total;  // byte offsets
@@ -130,16 +142,15 @@ struct LinearPlan {
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = tokens / w.batch;
-  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 256;
-  p.token_tile = std::min(p.bn, 128);
+  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 192;
   const int tile = block_of(w) * 4;
   p.scale_tiles = (w.cols + tile - 1) / tile;
   p.k_padded = p.scale_tiles * tile;
   p.move_codes = w.cols % 32 != 0 || !aligned(w.codes, 16);
   p.move_scale = !w.swizzled || w.cols % 64 != 0 || !aligned(w.scale, 16);
   p.w_code_pitch = up(w.cols / 2, 16);
-  // first_scale_row's numbers end below this; one more for a second tile that is read and not used
-  p.scale_rows = (tokens / p.token_tile + w.batch + 2) * 128;
+  // one more than first_scale_row's numbers can reach
+  p.scale_rows = (tokens / p.bn + w.batch + 1) * fp4::scale_rows_per_tile(p.bn);
   int64_t at = 0;
   p.x_codes = at;
   at += align256(tokens * (p.k_padded / 2));
@@ -169,8 +180,19 @@ cudaError_t launch_linear(const fp4::LinearArgs& args, int64_t items, cudaStream
   auto kernel = fp4::linear_kernel<DT, FMT, BN>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  kernel<<<static_cast<unsigned>(items), fp4::kLinearThreads, S::kSmem, stream>>>(args);
-  return launched();
+  // may start while the launch before it still quantizes; the kernel waits where it needs that
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count())));
+  config.blockDim = dim3(fp4::kLinearThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  e = cudaLaunchKernelEx(&config, kernel, args);
+  return e == cudaSuccess ? launched() : e;
 }
 
 // --------------------------------------------------------------- the gradient
@@ -327,7 +349,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   q.scale_mode = scale_mode;
   q.second_mode = act_second != nullptr ? PIPER_FP4_SECOND_GIVEN : PIPER_FP4_SECOND_NONE;
   q.second = const_cast<float*>(act_second);
-  q.token_tile = p.token_tile;
+  q.token_tile = p.bn;
   q.ends = ends;
   q.experts = static_cast<int32_t>(w->batch);
   fp4::RepackArgs r{};
@@ -366,7 +388,10 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   a.rows = static_cast<int32_t>(w->rows);
   a.k_steps = static_cast<int32_t>((w->cols + 63) / 64);
   a.scale_tiles = static_cast<int32_t>(p.scale_tiles);
+  a.early = !p.move_codes && !p.move_scale;
+  a.vec = aligned(y, 16) && w->rows % 8 == 0;
   const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
+  a.items = static_cast<int32_t>(items);
   FP4_REQUIRE(items < (int64_t{1} << 31), "FP4 product: too many tiles for one call.");
 
 #define CALL(D, F) \
@@ -377,7 +402,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   if (e != cudaSuccess) return cuda_fail("prepare kernel", e);
 #define CALL(D, F)                                            \
   e = bn == 32 ? launch_linear<D, F, 32>(a, items, s)         \
-               : bn == 128 ? launch_linear<D, F, 128>(a, items, s) : launch_linear<D, F, 256>(a, items, s)
+               : bn == 128 ? launch_linear<D, F, 128>(a, items, s) : launch_linear<D, F, 192>(a, items, s)
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("linear kernel", e);
@@ -420,6 +445,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   a.swizzled = w->swizzled != 0;
   a.scale_cols = scale_cols(*w);
   a.terms = p.terms;
+  a.vec = aligned(dx, 16) && w->cols % 8 == 0;
   a.piece = aligned(w->codes, 16) && a.code_pitch % 16 == 0 ? 16 : aligned(w->codes, 8) ? 8 : 1;
 
   const int64_t per_expert = tokens / w->batch;

@@ -36,6 +36,7 @@ struct GradArgs {
   int32_t swizzled;
   int32_t scale_cols;   // scales, or tiles of them, per row
   int32_t terms;
+  int32_t vec;          // rows of dx start on 16-byte boundaries
   int32_t piece;        // bytes that aligned loads of codes may take: 16, 8 or 1
 };
 
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
   const uint32_t n_mma = static_cast<uint32_t>((t.count + 15) & ~15);
 
   if (*have && t.expert == p.groups.experts) {
-    store_zeros<DT>(p.dx, t, p.cols);
+    store_zeros<DT>(p.dx, t, p.cols, threadIdx.x, kGradThreads);
   } else if (*have) {
     if (warp == 0) {
       if (lane == 0) {
@@ -246,11 +247,13 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
       ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(done, 0, pm::kStatusTimeoutMma));
       pm::tc_fence_after();
       if (ok) {
+        // the sums are complete, so the stages are free: each warp takes 2 KB of them
+        uint8_t* mine = smem + (warp - 2) * 2048;
         if constexpr (BN >= 64) {  // two warps share each quarter of the lanes: halves of the tokens
           const int half = warp >= 6;
-          store_tile<DT>(tmem, p.dx, t, p.cols, alpha, half * (BN / 2), (half + 1) * (BN / 2));
+          store_tile<DT>(tmem, p.dx, t, p.cols, alpha, half * (BN / 2), (half + 1) * (BN / 2), mine, p.vec != 0);
         } else if (warp < 6) {
-          store_tile<DT>(tmem, p.dx, t, p.cols, alpha, 0, BN);
+          store_tile<DT>(tmem, p.dx, t, p.cols, alpha, 0, BN, mine, p.vec != 0);
         }
       }
       pm::tc_fence_before();

@@ -33,55 +33,58 @@ struct LinearArgs {
   int32_t rows;            // outputs per expert
   int32_t k_steps;         // of 64 values
   int32_t scale_tiles;     // tiles of 4 scales per row (weight and tokens alike)
+  int32_t items;           // bound on the tiles
+  int32_t early;           // the weight is used where it is: loads of it need not wait for the launch before
+  int32_t vec;             // rows of y start on 16-byte boundaries
 };
 
 template <int FMT, int BN>
 struct LinearShape {
   static constexpr int kTiles = FMT == kNV ? 4 : 2;                 // scale tiles per stage and 128 rows
-  static constexpr int kXBlocks = BN > 128 ? BN / 128 : 1;          // 128-token scale blocks per tile
+  static constexpr int kXBlocks = (BN + 127) / 128;                 // 128-token scale blocks per tile
   static constexpr int kW = kTileRows * kStageBytes;
   static constexpr int kX = BN * kStageBytes;
   static constexpr int kSW = kTiles * 512;
   static constexpr int kSX = kXBlocks * kTiles * 512;
   static constexpr int kStage = kW + kX + kSW + kSX;
-  static constexpr int kCtas = BN <= 128 ? 2 : 1;                   // resident per SM
-  static constexpr int kStages = (kSmemMax / kCtas - 3072) / kStage < 8 ? (kSmemMax / kCtas - 3072) / kStage : 8;
-  static constexpr int kSmem = kStages * kStage + 1024 + 256;
-  // tensor memory: accumulator, then two buffers of scales
+  static constexpr int kOut = 4 * 2048;                             // 32 tokens x 32 outputs of each epilogue warp
+  static constexpr int kStages = (kSmemMax - 2048 - kOut) / kStage < 9 ? (kSmemMax - 2048 - kOut) / kStage : 9;
+  static constexpr int kSmem = kStages * kStage + kOut + 1024 + 512;
+  // tensor memory: two accumulators, then two buffers of scales
   static constexpr int kScaleCols = kTiles * 4 * (1 + kXBlocks);
-  static constexpr int kCols = BN + 2 * kScaleCols;
+  static constexpr int kCols = 2 * BN + 2 * kScaleCols;
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kCols <= 512 && kStages >= 4, "the tile does not fit");
 };
 
+// One persistent block per SM. Roles run through the same tiles on their own:
+// the producer and the tensor-core warp are up to two accumulators ahead of
+// the epilogue.
 template <int DT, int FMT, int BN>
-__global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
-    linear_kernel(const __grid_constant__ LinearArgs p) {
+__global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_constant__ LinearArgs p) {
   using S = LinearShape<FMT, BN>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStage);
+  uint8_t* out = smem + S::kStages * S::kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out + S::kOut);
   uint64_t* empty = full + S::kStages;
-  uint64_t* done = empty + S::kStages;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
-  TileAt* shared_tile = reinterpret_cast<TileAt*>(tmem_at + 2);
-  int32_t* have = reinterpret_cast<int32_t*>(shared_tile + 1);
+  uint64_t* acc_full = empty + S::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    TileAt t;
-    const bool ok = find_tile(p.groups, blockIdx.x, BN, t);
-    if (lane == 0) {
-      *have = ok;
-      if (ok) *shared_tile = t;
-      pm::prefetch_tmap(&p.w_map);
-      pm::prefetch_tmap(&p.x_map);
-      for (int s = 0; s < S::kStages; ++s) {
-        pm::mbar_init(&full[s], 1);
-        pm::mbar_init(&empty[s], 1);
-      }
-      pm::mbar_init(done, 1);
-      pm::fence_mbar_init();
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    pm::prefetch_tmap(&p.w_map);
+    pm::prefetch_tmap(&p.x_map);
+    for (int s = 0; s < S::kStages; ++s) {
+      pm::mbar_init(&full[s], 1);
+      pm::mbar_init(&empty[s], 1);
     }
+    for (int b = 0; b < 2; ++b) {
+      pm::mbar_init(&acc_full[b], 1);
+      pm::mbar_init(&acc_empty[b], 4);
+    }
+    pm::fence_mbar_init();
   } else if (warp == 1) {
     pm::tmem_alloc(tmem_at, S::kAlloc);
     pm::tmem_relinquish();
@@ -89,81 +92,137 @@ __global__ void __launch_bounds__(kLinearThreads, LinearShape<FMT, BN>::kCtas)
   pm::tc_fence_before();
   __syncthreads();
   pm::tc_fence_after();
-  const uint32_t tmem = *tmem_at;
-  const TileAt t = *shared_tile;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
   const int stages = (p.k_steps + 3) / 4;
-  // token columns that the tensor core computes
-  const uint32_t n_mma = static_cast<uint32_t>((t.count + 15) & ~15);
 
-  if (*have && t.expert == p.groups.experts) {
-    store_zeros<DT>(p.y, t, p.rows);
-  } else if (*have) {
-    if (warp == 0) {
+  if (warp == 0) {
+    int it = 0;       // stages issued
+    bool ok = true, waited = false;
+    TileAt t;
+    for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+      if (t.expert == p.groups.experts) continue;
       if (lane == 0) {
-        const int64_t w_row = static_cast<int64_t>(t.expert) * p.rows + t.row_tile * kTileRows;
+        const int w_row = t.expert * p.rows + t.row_tile * kTileRows;
         const uint8_t* w_scale =
             p.w_scale + (static_cast<int64_t>(t.expert) * p.groups.row_tiles + t.row_tile) * p.scale_tiles * 512;
         const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(t.scale_row >> 7) * p.scale_tiles * 512;
-        grid_wait();
-        int issued = 0;
-        for (int i = 0; i < stages; ++i) {
-          const int s = i % S::kStages;
-          if (i >= S::kStages && !pm::mbar_wait(&empty[s], ((i / S::kStages) - 1) & 1, pm::kStatusTimeoutLoad)) break;
+        const auto load_w = [&](int i, int s) {
           uint8_t* at = smem + s * S::kStage;
           const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
           pm::mbar_arrive_expect_tx(&full[s], S::kW + S::kX + tiles * 512 * (1 + S::kXBlocks));
-          pm::tma_load_2d(at, &p.w_map, i * kStageBytes, static_cast<int>(w_row), &full[s]);
-          pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, t.first, &full[s]);
+          pm::tma_load_2d(at, &p.w_map, i * kStageBytes, w_row, &full[s]);
           pm::bulk_g2s(at + S::kW + S::kX, w_scale + static_cast<int64_t>(i) * S::kTiles * 512, tiles * 512, &full[s]);
+        };
+        const auto load_x = [&](int i, int s) {
+          uint8_t* at = smem + s * S::kStage;
+          const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
+          pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, t.first, &full[s]);
 #pragma unroll
           for (int b = 0; b < S::kXBlocks; ++b)
             pm::bulk_g2s(at + S::kW + S::kX + S::kSW + b * S::kTiles * 512,
                          x_scale + (static_cast<int64_t>(b) * p.scale_tiles + i * S::kTiles) * 512, tiles * 512, &full[s]);
-          issued = i + 1;
+        };
+        int i = 0;
+        if (!waited) {
+          // the first tile: the weight's part of every stage goes out before the tokens are quantized
+          const int ahead = p.early ? min(stages, S::kStages) : 0;
+          for (int j = 0; j < ahead; ++j) load_w(j, j);
+          grid_wait();
+          waited = true;
+          for (; i < ahead; ++i) load_x(i, i);
+          it = ahead;
         }
-        // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
-        for (int i = max(0, issued - S::kStages); i < issued; ++i)
-          pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
-      }
-      __syncwarp();
-    } else if (warp == 1) {
-      if (lane == 0) {
-        for (int i = 0; i < stages; ++i) {
-          const int s = i % S::kStages;
-          // the scale buffer's last readers, two stages ago, have finished
-          if (i >= 2 && !pm::mbar_wait(&empty[(i - 2) % S::kStages], ((i - 2) / S::kStages) & 1, pm::kStatusTimeoutMma)) break;
-          if (!pm::mbar_wait(&full[s], (i / S::kStages) & 1, pm::kStatusTimeoutMma)) break;
-          pm::tc_fence_after();
-          const uint32_t at = pm::smem_u32(smem + s * S::kStage);
-          const uint32_t sw = tmem + BN + (i & 1) * S::kScaleCols, sx = sw + S::kTiles * 4;
-          const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
-          for (int j = 0; j < tiles; ++j) {
-            tmem_cp_scales(sw + j * 4, pm::smem_desc(at + S::kW + S::kX + j * 512, 0, 128));
-#pragma unroll
-            for (int b = 0; b < S::kXBlocks; ++b)
-              tmem_cp_scales(sx + (j * S::kXBlocks + b) * 4,
-                             pm::smem_desc(at + S::kW + S::kX + S::kSW + (b * S::kTiles + j) * 512, 0, 128));
+        for (; i < stages; ++i, ++it) {
+          const int s = it % S::kStages;
+          if (it >= S::kStages && !pm::mbar_wait(&empty[s], ((it / S::kStages) - 1) & 1, pm::kStatusTimeoutLoad)) {
+            ok = false;
+            break;
           }
-          const uint64_t a = pm::smem_desc_sw(at, 16, 1024, 2), b = pm::smem_desc_sw(at + S::kW, 16, 1024, 2);
-          const int steps = min(4, p.k_steps - i * 4);
-          for (int j = 0; j < steps; ++j) {
-            const uint32_t tile = FMT == kNV ? j : j >> 1, id = FMT == kNV ? 0u : (j & 1) * 2u;
-            umma_fp4<FMT>(tmem, a + j * 2, b + j * 2, idesc_fp4(kTileRows, n_mma, FMT == kMX, id), sw + tile * 4,
-                          sx + tile * 4 * S::kXBlocks, (i | j) != 0);
+          load_w(i, s);
+          load_x(i, s);
+        }
+      }
+      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+    }
+    if (lane == 0) {
+      if (!waited) grid_wait();  // no block ends before the launch it depends on
+      // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
+      for (int i = max(0, it - S::kStages); i < it; ++i)
+        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    int it = 0, n = 0;  // stages used, tiles begun
+    bool ok = true;
+    TileAt t;
+    for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+      if (t.expert == p.groups.experts) continue;
+      const int b = n & 1;
+      const uint32_t d = tmem + b * BN;
+      const uint32_t n_mma = (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t.count, 0)) + 15u) & ~15u;  // computed token columns
+      const uint32_t idesc = idesc_fp4(kTileRows, n_mma, FMT == kMX, 0);
+      ok = n < 2 || __all_sync(0xFFFFFFFFu, pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma));
+      pm::tc_fence_after();
+      for (int i = 0; ok && i < stages; ++i, ++it) {
+        const int s = it % S::kStages;
+        // the scale buffer's last readers, two stages ago, have finished
+        ok = it < 2 || pm::mbar_wait(&empty[(it - 2) % S::kStages], ((it - 2) / S::kStages) & 1, pm::kStatusTimeoutMma);
+        ok = ok && pm::mbar_wait(&full[s], (it / S::kStages) & 1, pm::kStatusTimeoutMma);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        pm::tc_fence_after();
+        const uint32_t at = pm::smem_u32(smem) + s * S::kStage;
+        const uint32_t sw = tmem + 2 * BN + (it & 1) * S::kScaleCols, sx = sw + S::kTiles * 4;
+        const int tiles = p.scale_tiles - i * S::kTiles, steps = p.k_steps - i * 4;
+        if (elect_one()) {
+          const uint64_t ws = pm::smem_desc(at + S::kW + S::kX, 0, 128);
+          const uint64_t xs = pm::smem_desc(at + S::kW + S::kX + S::kSW, 0, 128);
+#pragma unroll
+          for (int j = 0; j < S::kTiles; ++j) {
+            if (j < tiles) {
+              tmem_cp_scales(sw + j * 4, ws + j * (512 >> 4));
+#pragma unroll
+              for (int k = 0; k < S::kXBlocks; ++k)
+                tmem_cp_scales(sx + (j * S::kXBlocks + k) * 4, xs + (k * S::kTiles + j) * (512 >> 4));
+            }
+          }
+          const uint64_t a = pm::smem_desc_sw(at, 16, 1024, 2), x = pm::smem_desc_sw(at + S::kW, 16, 1024, 2);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            constexpr uint32_t kSecondHalf = (2u << 4) | (2u << 29);  // scale bytes 2 and 3 of a column
+            const uint32_t tile = FMT == kNV ? j : j >> 1;
+            if (j < steps)
+              umma_fp4<FMT>(d, a + j * 2, x + j * 2, FMT == kMX && (j & 1) ? idesc | kSecondHalf : idesc, sw + tile * 4,
+                            sx + tile * 4 * S::kXBlocks, (i | j) != 0);
           }
           pm::umma_commit(&empty[s]);
+          if (i + 1 == stages) pm::umma_commit(&acc_full[b]);
         }
-        pm::umma_commit(done);
+        __syncwarp();
       }
-      __syncwarp();
-    } else {
-      float alpha = 1.0f;
-      if (p.w_second != nullptr) alpha = p.w_second[t.expert];
-      if (p.x_second != nullptr) alpha *= *p.x_second;
-      const bool ok = pm::mbar_wait(done, 0, pm::kStatusTimeoutMma);
+      ++n;
+    }
+    __syncwarp();
+  } else {
+    const float x_second = p.x_second != nullptr ? *p.x_second : 1.0f;
+    uint8_t* mine = out + (warp & 3) * 2048;
+    int n = 0;
+    TileAt t;
+    for (int id = blockIdx.x; id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+      if (t.expert == p.groups.experts) {
+        store_zeros<DT>(p.y, t, p.rows, threadIdx.x - 64, 128);
+        continue;
+      }
+      const int b = n & 1;
+      const float alpha = (p.w_second != nullptr ? p.w_second[t.expert] : 1.0f) * x_second;
+      const bool ok = pm::mbar_wait(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
       pm::tc_fence_after();
-      if (__all_sync(0xFFFFFFFFu, ok)) store_tile<DT>(tmem, p.y, t, p.rows, alpha, 0, BN);
+      store_tile<DT>(tmem + b * BN, p.y, t, p.rows, alpha, 0, BN, mine, p.vec != 0);
       pm::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) pm::mbar_arrive(&acc_empty[b]);
+      ++n;
     }
   }
   __syncthreads();

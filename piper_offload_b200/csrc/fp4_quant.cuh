@@ -14,8 +14,8 @@
 // 512-byte (bf16) runs and its code stores 128-byte ones; a block's maximum
 // takes one or two shuffles; four scales leave as one word.
 #pragma once
+#include "fp4_ptx.cuh"
 #include "numerics.cuh"
-#include "ptx.cuh"
 
 namespace fp4 {
 
@@ -40,12 +40,15 @@ __host__ __device__ __forceinline__ int64_t swizzled_byte(int64_t r, int64_t c, 
   return ((r >> 7) * ct + (c >> 2)) * 512 + (rin & 31) * 16 + (rin >> 5) * 4 + static_cast<int>(c & 3);
 }
 
-// Scale rows of tokens. Every run of `tile` (at most 128) tokens of an expert
-// starts on a 128-row tile of scales, because the tensor core reads them from
-// its tile's first column. Expert e's first run is number start / tile + e:
-// with ceil(n / tile) runs of n rows, at least that many numbers lie before
-// it, so no scan over the experts is needed.
-__host__ __device__ __forceinline__ int64_t first_scale_row(int64_t start, int64_t e, int tile) { return (start / tile + e) * 128; }
+// Scale rows of tokens. Every tile of `tile` tokens of an expert starts on a
+// 128-row tile of scales, because the tensor core reads them from its first
+// column. Expert e's first tile is number start / tile + e: with ceil(n / tile)
+// tiles of n rows, at least that many numbers lie before it, so no scan over
+// the experts is needed.
+__host__ __device__ __forceinline__ int scale_rows_per_tile(int tile) { return (tile + 127) & ~127; }
+__host__ __device__ __forceinline__ int64_t first_scale_row(int64_t start, int64_t e, int tile) {
+  return (start / tile + e) * scale_rows_per_tile(tile);
+}
 
 // Expert whose rows hold row t (the first with ends[e] > t, or `experts`).
 __device__ __forceinline__ int expert_of_row(const int32_t* ends, int experts, int64_t t) {
@@ -82,7 +85,7 @@ struct QuantArgs {
   // tokens of experts
   const int32_t* ends;   // NULL: one weight for all
   int32_t experts;
-  int32_t token_tile;    // 0: rows are a weight's; else tokens in runs of so many (first_scale_row)
+  int32_t token_tile;    // 0: rows are a weight's; else tokens in tiles of so many (first_scale_row)
 };
 
 template <int DT>
@@ -264,7 +267,8 @@ __device__ void quantize_octets(const QuantArgs& q, int64_t first) {
         if (x >= q.experts || start < 0 || start > rin) continue;  // a row of no expert
       }
       const int o = static_cast<int>(rin - start);
-      srow = first_scale_row(start, x, q.token_tile) + static_cast<int64_t>(o / q.token_tile) * 128 + o % q.token_tile;
+      srow = first_scale_row(start, x, q.token_tile) +
+             static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
     }
     const int c = static_cast<int>(oct[u]) / kLanes;
     const int lanes = static_cast<int>(oct[u]) % kLanes;
@@ -471,6 +475,7 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
 template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads)
     prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t quant_blocks) {
+  grid_launch_dependents();
   if (blockIdx.x < quant_blocks) quantize_octets<DT, FMT>(q, static_cast<int64_t>(blockIdx.x) * kOctetsPerBlock);
   else repack(p, static_cast<int64_t>(blockIdx.x - quant_blocks) * kQuantThreads + threadIdx.x);
 }

@@ -1,5 +1,6 @@
 // fp4_tiles.cuh - which tile a block works on, shared by the FP4 products and gradients.
 #pragma once
+#include "fp4_ptx.cuh"
 #include "fp4_quant.cuh"
 
 namespace fp4 {
@@ -35,7 +36,7 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
     t.row_tile = id / per;
     const int nt = id - t.row_tile * per;
     t.first = nt * bn;
-    t.scale_row = nt * max(bn, 128);
+    t.scale_row = nt * scale_rows_per_tile(bn);
     t.count = min(bn, tokens - t.first);
     return t.row_tile < p.row_tiles;
   }
@@ -68,7 +69,7 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
       const int nt = in - t.row_tile * per_l;
       t.first = start_l + nt * bn;
       t.count = min(bn, n_l - nt * bn);
-      t.scale_row = static_cast<int>(first_scale_row(start_l, t.expert, min(bn, 128))) + nt * max(bn, 128);
+      t.scale_row = static_cast<int>(first_scale_row(start_l, t.expert, bn)) + nt * scale_rows_per_tile(bn);
       return true;
     }
     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -82,32 +83,74 @@ __device__ __forceinline__ void store_value(void* y, int64_t at, float v) {
   else static_cast<float*>(y)[at] = v;
 }
 
-// A whole block zeroes its tile of y (tokens x cols).
+// `threads` threads zero a tile of y (tokens x cols).
 template <int DT>
-__device__ __forceinline__ void store_zeros(void* y, const TileAt& t, int cols) {
+__device__ __forceinline__ void store_zeros(void* y, const TileAt& t, int cols, int thread, int threads) {
   const int c0 = t.row_tile * kTileRows, n = min(kTileRows, cols - c0);
-  for (int i = threadIdx.x; i < t.count * kTileRows; i += blockDim.x)
+  for (int i = thread; i < t.count * kTileRows; i += threads)
     if ((i & (kTileRows - 1)) < n)
       store_value<DT>(y, static_cast<int64_t>(t.first + i / kTileRows) * cols + c0 + (i & (kTileRows - 1)), 0.0f);
 }
 
 // Four epilogue warps' share of a finished tile: tensor-memory lane = column of
-// y, tensor-memory column = token. A warp stores 32 neighbouring outputs of
-// one token at a time: whole 64-byte (bf16) or 128-byte runs.
+// y, tensor-memory column = token, so that a warp's 32 lanes are neighbours in
+// y's rows. bf16: 32 tokens at a time are read as the fragments of 8x8
+// matrices, rounded, transposed by stmatrix into the warp's own 2 KB of shared
+// memory (`stage`; 64-byte rows, 16-byte pieces XORed with the row against
+// bank conflicts) and leave as 16-byte pieces of y's rows: 4 stores per 32 x 32
+// outputs instead of 32. fp32: a token's 32 outputs are one 128-byte run.
 template <int DT>
 __device__ __forceinline__ void store_tile(uint32_t tmem, void* y, const TileAt& t, int cols, float alpha, int from_col,
-                                           int to_col) {
+                                           int to_col, uint8_t* stage, bool vec) {
   const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const int n = t.row_tile * kTileRows + quarter * 32 + lane;
+  const int n0 = t.row_tile * kTileRows + quarter * 32;
   const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  for (int c = from_col; c < min(to_col, t.count); c += 32) {
-    float v[32];
-    pm::tmem_ld32(at + c, v);
-    if (n < cols) {
-      const int64_t base = static_cast<int64_t>(t.first + c) * cols + n;
+  const int end = min(to_col, t.count);
+  if constexpr (DT == kBF16) {
+    const uint32_t base = pm::smem_u32(stage);
+    const int piece = lane & 3;
+    const int left = cols - n0 - piece * 8;  // outputs of this lane's piece that exist
+    for (int c = from_col; c < end; c += 32) {
+      uint32_t lo[16], hi[16];
+      tmem_ld_fragments(at + c, lo);
+      tmem_ld_fragments(at + (16u << 16) + c, hi);
+      tmem_ld_fragments_wait(lo, hi);
+      __syncwarp();  // the warp has read the last 32 tokens out of its stage
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (c + j < t.count) store_value<DT>(y, base + static_cast<int64_t>(j) * cols, v[j] * alpha);
+      for (int j = 0; j < 4; ++j) {
+        const int token = j * 8 + (lane & 7);
+        const uint32_t to = base + token * 64 + (((lane >> 3) ^ ((token >> 1) & 3)) << 4);
+        stmatrix_trans(to, bf16_pair(lo[4 * j], lo[4 * j + 1], alpha), bf16_pair(lo[4 * j + 2], lo[4 * j + 3], alpha),
+                       bf16_pair(hi[4 * j], hi[4 * j + 1], alpha), bf16_pair(hi[4 * j + 2], hi[4 * j + 3], alpha));
+      }
+      __syncwarp();
+      uint16_t* row = static_cast<uint16_t*>(y) + (static_cast<int64_t>(t.first + c + (lane >> 2)) * cols + n0 + piece * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j, row += static_cast<int64_t>(8) * cols) {
+        const int token = j * 8 + (lane >> 2);
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + token * 64 + ((piece ^ ((token >> 1) & 3)) << 4));
+        if (c + token >= end) break;
+        if (vec && left >= 8) {
+          *reinterpret_cast<uint4*>(row) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < left) row[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+        }
+      }
+    }
+  } else {
+    const int n = n0 + lane;
+    for (int c = from_col; c < end; c += 32) {
+      float v[32];
+      pm::tmem_ld32(at + c, v);
+      if (n < cols) {
+        float* to = static_cast<float*>(y) + (static_cast<int64_t>(t.first + c) * cols + n);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (c + j < end) to[static_cast<int64_t>(j) * cols] = v[j] * alpha;
+      }
     }
   }
 }
