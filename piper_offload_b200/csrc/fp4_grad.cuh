@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
   int32_t* have = reinterpret_cast<int32_t*>(tmem_at + 1);
   TileAt* shared_tile = reinterpret_cast<TileAt*>(have + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (warp == 0) {
     TileAt t;
     const bool ok = find_tile(p.groups, blockIdx.x, BN, t);
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
   pm::tc_fence_before();
   __syncthreads();
   pm::tc_fence_after();
-  const uint32_t tmem = *tmem_at;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
   const TileAt t = *shared_tile;
   const int blocks = (p.rows + kGradStageRows - 1) / kGradStageRows;  // of 64 rows of w
   const int stages = blocks * p.terms;
@@ -162,36 +162,38 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
     store_zeros<DT>(p.dx, t, p.cols, threadIdx.x, kGradThreads);
   } else if (*have) {
     if (warp == 0) {
-      if (lane == 0) {
-        grid_wait();
-        int issued = 0;
-        int block = 0, term = 0;
-        for (int i = 0; i < stages; ++i) {
-          const int s = i % S::kStages;
-          if (i >= S::kStages && !pm::mbar_wait(&empty[s], ((i / S::kStages) - 1) & 1, pm::kStatusTimeoutLoad)) break;
+      grid_wait();
+      const int first = __shfl_sync(0xFFFFFFFFu, t.first, 0);
+      int issued = 0, block = 0, row = first;
+      for (int i = 0; i < stages; ++i) {
+        const int s = i % S::kStages;
+        const bool ok = i < S::kStages || pm::mbar_wait(&empty[s], ((i / S::kStages) - 1) & 1, pm::kStatusTimeoutLoad);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        if (elect_one()) {
           pm::mbar_arrive_expect_tx(&full[s], S::kB);
-          pm::tma_load_2d(smem + s * S::kStage + S::kA, &p.dy_map, block * kGradStageRows,
-                          static_cast<int>(term * p.groups.tokens) + t.first, &full[s]);
-          issued = i + 1;
-          if (++block == blocks) {
-            block = 0;
-            ++term;
-          }
+          pm::tma_load_2d(smem + s * S::kStage + S::kA, &p.dy_map, block * kGradStageRows, row, &full[s]);
         }
-        // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
-        for (int i = max(0, issued - S::kStages); i < issued; ++i)
-          pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+        __syncwarp();
+        issued = i + 1;
+        if (++block == blocks) {  // the next term
+          block = 0;
+          row += static_cast<int>(p.groups.tokens);
+        }
       }
+      // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
+      for (int i = max(0, issued - S::kStages); i < issued; ++i)
+        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
       __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0) {
-        const uint32_t idesc = idesc_grad(n_mma);
-        for (int i = 0; i < stages; ++i) {
-          const int s = i % S::kStages;
-          if (!pm::mbar_wait(&full[s], (i / S::kStages) & 1, pm::kStatusTimeoutMma)) break;
-          if (!pm::mbar_wait(&ready[s], (i / S::kStages) & 1, pm::kStatusTimeoutMma)) break;
-          pm::tc_fence_after();
-          const uint32_t at = pm::smem_u32(smem + s * S::kStage);
+      const uint32_t idesc = idesc_grad(__shfl_sync(0xFFFFFFFFu, n_mma, 0));
+      for (int i = 0; i < stages; ++i) {
+        const int s = i % S::kStages;
+        const bool ok = pm::mbar_wait(&full[s], (i / S::kStages) & 1, pm::kStatusTimeoutMma) &&
+                        pm::mbar_wait(&ready[s], (i / S::kStages) & 1, pm::kStatusTimeoutMma);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        pm::tc_fence_after();
+        const uint32_t at = pm::smem_u32(smem) + s * S::kStage;
+        if (elect_one()) {
           // w: 64-column blocks 8 KB apart, groups of 8 rows 1 KB apart; dy: 128-byte rows of 64 values
           const uint64_t a = pm::smem_desc_sw(at, kGradStageRows * 128, 1024, 2);
           const uint64_t b = pm::smem_desc_sw(at + S::kA, 16, 1024, 2);
@@ -199,8 +201,9 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kerne
           for (int j = 0; j < kGradStageRows / 16; ++j)
             pm::umma_f16(tmem, a + j * (2048 >> 4), b + j * (32 >> 4), idesc, (i | j) != 0);
           pm::umma_commit(&empty[s]);
+          if (i + 1 == stages) pm::umma_commit(done);
         }
-        pm::umma_commit(done);
+        __syncwarp();
       }
       __syncwarp();
     } else {

@@ -96,63 +96,65 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
   const int stages = (p.k_steps + 3) / 4;
 
   if (warp == 0) {
-    int it = 0;       // stages issued
+    Ring<S::kStages> ring;
+    int it = 0;  // stages issued
     bool ok = true, waited = false;
     TileAt t;
     for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
       if (t.expert == p.groups.experts) continue;
-      if (lane == 0) {
-        const int w_row = t.expert * p.rows + t.row_tile * kTileRows;
-        const uint8_t* w_scale =
-            p.w_scale + (static_cast<int64_t>(t.expert) * p.groups.row_tiles + t.row_tile) * p.scale_tiles * 512;
-        const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(t.scale_row >> 7) * p.scale_tiles * 512;
-        const auto load_w = [&](int i, int s) {
-          uint8_t* at = smem + s * S::kStage;
-          const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
-          pm::mbar_arrive_expect_tx(&full[s], S::kW + S::kX + tiles * 512 * (1 + S::kXBlocks));
-          pm::tma_load_2d(at, &p.w_map, i * kStageBytes, w_row, &full[s]);
-          pm::bulk_g2s(at + S::kW + S::kX, w_scale + static_cast<int64_t>(i) * S::kTiles * 512, tiles * 512, &full[s]);
-        };
-        const auto load_x = [&](int i, int s) {
-          uint8_t* at = smem + s * S::kStage;
-          const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
-          pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, t.first, &full[s]);
+      const int w_row = __shfl_sync(0xFFFFFFFFu, t.expert * p.rows + t.row_tile * kTileRows, 0);
+      const int x_row = __shfl_sync(0xFFFFFFFFu, t.first, 0);
+      const uint8_t* w_scale =
+          p.w_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.expert * p.groups.row_tiles + t.row_tile, 0)) * p.scale_tiles * 512;
+      const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.scale_row >> 7, 0)) * p.scale_tiles * 512;
+      const auto load_w = [&](int i, int s) {
+        uint8_t* at = smem + s * S::kStage;
+        const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
+        pm::mbar_arrive_expect_tx(&full[s], S::kW + S::kX + tiles * 512 * (1 + S::kXBlocks));
+        pm::tma_load_2d(at, &p.w_map, i * kStageBytes, w_row, &full[s]);
+        pm::bulk_g2s(at + S::kW + S::kX, w_scale + static_cast<int64_t>(i) * S::kTiles * 512, tiles * 512, &full[s]);
+      };
+      const auto load_x = [&](int i, int s) {
+        uint8_t* at = smem + s * S::kStage;
+        const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
+        pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, x_row, &full[s]);
 #pragma unroll
-          for (int b = 0; b < S::kXBlocks; ++b)
-            pm::bulk_g2s(at + S::kW + S::kX + S::kSW + b * S::kTiles * 512,
-                         x_scale + (static_cast<int64_t>(b) * p.scale_tiles + i * S::kTiles) * 512, tiles * 512, &full[s]);
-        };
+        for (int b = 0; b < S::kXBlocks; ++b)
+          pm::bulk_g2s(at + S::kW + S::kX + S::kSW + b * S::kTiles * 512,
+                       x_scale + (static_cast<int64_t>(b) * p.scale_tiles + i * S::kTiles) * 512, tiles * 512, &full[s]);
+      };
+      if (elect_one()) {
         int i = 0;
         if (!waited) {
           // the first tile: the weight's part of every stage goes out before the tokens are quantized
           const int ahead = p.early ? min(stages, S::kStages) : 0;
           for (int j = 0; j < ahead; ++j) load_w(j, j);
           grid_wait();
-          waited = true;
-          for (; i < ahead; ++i) load_x(i, i);
-          it = ahead;
+          for (; i < ahead; ++i, ++it, ring.next()) load_x(i, i);
         }
-        for (; i < stages; ++i, ++it) {
-          const int s = it % S::kStages;
-          if (it >= S::kStages && !pm::mbar_wait(&empty[s], ((it / S::kStages) - 1) & 1, pm::kStatusTimeoutLoad)) {
-            ok = false;
-            break;
-          }
-          load_w(i, s);
-          load_x(i, s);
+        for (; i < stages; ++i, ++it, ring.next()) {
+          ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+          if (!ok) break;
+          load_w(i, ring.slot);
+          load_x(i, ring.slot);
         }
       }
-      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+      __syncwarp();
+      waited = true;
+      // the elected lane may be another one next time
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      it = __reduce_max_sync(0xFFFFFFFFu, it);
+      ring.slot = it % S::kStages;
+      ring.round = (it / S::kStages) & 1;
     }
-    if (lane == 0) {
-      if (!waited) grid_wait();  // no block ends before the launch it depends on
-      // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
-      for (int i = max(0, it - S::kStages); i < it; ++i)
-        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
-    }
+    if (!waited) grid_wait();  // no block ends before the launch it depends on
+    // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
+    for (int i = max(0, it - S::kStages); i < it; ++i)
+      pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
     __syncwarp();
   } else if (warp == 1) {
-    int it = 0, n = 0;  // stages used, tiles begun
+    Ring<S::kStages> ring, old;  // this stage; the one two stages ago
+    int it = 0, n = 0;           // stages used, tiles begun
     bool ok = true;
     TileAt t;
     for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
@@ -161,20 +163,21 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
       const uint32_t d = tmem + b * BN;
       const uint32_t n_mma = (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t.count, 0)) + 15u) & ~15u;  // computed token columns
       const uint32_t idesc = idesc_fp4(kTileRows, n_mma, FMT == kMX, 0);
-      ok = n < 2 || __all_sync(0xFFFFFFFFu, pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma));
-      pm::tc_fence_after();
-      for (int i = 0; ok && i < stages; ++i, ++it) {
-        const int s = it % S::kStages;
-        // the scale buffer's last readers, two stages ago, have finished
-        ok = it < 2 || pm::mbar_wait(&empty[(it - 2) % S::kStages], ((it - 2) / S::kStages) & 1, pm::kStatusTimeoutMma);
-        ok = ok && pm::mbar_wait(&full[s], (it / S::kStages) & 1, pm::kStatusTimeoutMma);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
+      if (elect_one()) {
+        ok = n < 2 || pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
         pm::tc_fence_after();
-        const uint32_t at = pm::smem_u32(smem) + s * S::kStage;
-        const uint32_t sw = tmem + 2 * BN + (it & 1) * S::kScaleCols, sx = sw + S::kTiles * 4;
-        const int tiles = p.scale_tiles - i * S::kTiles, steps = p.k_steps - i * 4;
-        if (elect_one()) {
+        for (int i = 0; ok && i < stages; ++i, ++it, ring.next()) {
+          // the scale buffer's last readers, two stages ago, have finished
+          if (it >= 2) {
+            ok = pm::mbar_wait(&empty[old.slot], old.round, pm::kStatusTimeoutMma);
+            old.next();
+          }
+          ok = ok && pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+          if (!ok) break;
+          pm::tc_fence_after();
+          const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
+          const uint32_t sw = tmem + 2 * BN + (it & 1) * S::kScaleCols, sx = sw + S::kTiles * 4;
+          const int tiles = p.scale_tiles - i * S::kTiles, steps = p.k_steps - i * 4;
           const uint64_t ws = pm::smem_desc(at + S::kW + S::kX, 0, 128);
           const uint64_t xs = pm::smem_desc(at + S::kW + S::kX + S::kSW, 0, 128);
 #pragma unroll
@@ -195,12 +198,20 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
               umma_fp4<FMT>(d, a + j * 2, x + j * 2, FMT == kMX && (j & 1) ? idesc | kSecondHalf : idesc, sw + tile * 4,
                             sx + tile * 4 * S::kXBlocks, (i | j) != 0);
           }
-          pm::umma_commit(&empty[s]);
-          if (i + 1 == stages) pm::umma_commit(&acc_full[b]);
+          pm::umma_commit(&empty[ring.slot]);
         }
-        __syncwarp();
+        pm::umma_commit(&acc_full[b]);
       }
+      __syncwarp();
       ++n;
+      // the elected lane may be another one next time
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      it = __reduce_max_sync(0xFFFFFFFFu, it);
+      ring.slot = it % S::kStages;
+      ring.round = (it / S::kStages) & 1;
+      const int before = max(it - 2, 0);
+      old.slot = before % S::kStages;
+      old.round = (before / S::kStages) & 1;
     }
     __syncwarp();
   } else {

@@ -91,6 +91,21 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0u;
 }
 
+// A place in a ring of N barriers and the parity of its current round, kept by
+// addition: the remainder and quotient of a running count cost more than the
+// wait they are for.
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t round = 0;  // parity
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      round ^= 1u;
+    }
+  }
+};
+
 // Programmatic launches: let the next kernel start its own set-up / wait for
 // everything the previous one wrote.
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
