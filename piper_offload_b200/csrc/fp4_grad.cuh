@@ -98,24 +98,6 @@ __device__ __forceinline__ Piece load_piece(const GradArgs& p, int64_t expert, i
   return out;
 }
 
-// Four codes of `nibbles` (low 16 bits) times a bf16 pair, as two bf16 pairs.
-// The magnitudes' bf16 bytes come from two 8-entry tables; a selector with bit
-// 3 set would replicate the byte's sign, which gives the sign bits.
-__device__ __forceinline__ void decode4(uint32_t nibbles, __nv_bfloat162 scale, uint32_t& lo, uint32_t& hi) {
-  const uint32_t sel = nibbles & 0x7777u;
-  const uint32_t top = __byte_perm(0x3F3F3F00u, 0x40404040u, sel);
-  const uint32_t low = __byte_perm(0xC0800000u, 0xC0804000u, sel);
-  // 0x80 for a positive code, 0xFF for a negative one
-  uint32_t sign;
-  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(sign) : "r"(0x80808080u), "r"(nibbles));
-  const uint32_t high = top | ((sign << 7) & 0x80808080u);
-  uint32_t a = __byte_perm(low, high, 0x5140), b = __byte_perm(low, high, 0x7362);
-  __nv_bfloat162 x = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), scale);
-  __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&b), scale);
-  lo = *reinterpret_cast<uint32_t*>(&x);
-  hi = *reinterpret_cast<uint32_t*>(&y);
-}
-
 template <int DT, int FMT, int BN>
 __global__ void __launch_bounds__(kGradThreads, GradShape<BN>::kCtas) grad_kernel(const __grid_constant__ GradArgs p) {
   using S = GradShape<BN>;

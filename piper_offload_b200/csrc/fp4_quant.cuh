@@ -10,9 +10,12 @@
 // rule of its own: a NaN in a block makes its scale NaN (e8m0 255, e4m3 127),
 // so the whole block and what is computed from it read as NaN.
 //
-// Bound: HBM. One pass, 8 values a lane, so that a warp's loads are whole
-// 512-byte (bf16) runs and its code stores 128-byte ones; a block's maximum
-// takes one or two shuffles; four scales leave as one word.
+// Bound: HBM, with instructions close behind (a first version with 8 values a
+// lane and a division per lane for its place took 45 instructions a value and
+// 4.7x the time). A lane holds 16 neighbouring values: one 32-byte load
+// (bf16), one 8-byte store, no shuffle for an NVFP4 block and one for an
+// MXFP4 block; four rows are in flight per lane, and only a block of threads
+// divides to find its place.
 #pragma once
 #include "fp4_ptx.cuh"
 #include "numerics.cuh"
@@ -25,8 +28,9 @@ enum : int { kFloor = 0, kRceil = 1, kCeil = 2, kEven = 3 };
 enum : int { kSecondNone = 0, kSecondGiven = 1, kSecondCompute = 2 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;  // octets of 8 values per thread
-constexpr int kOctetsPerBlock = kQuantThreads * kQuantUnroll;
+constexpr int kQuantRows = 4;   // rows in flight per lane
+constexpr int kUnit = 16;       // values per lane and row
+constexpr int kSmallThreads = 512;
 
 template <int FMT>
 __host__ __device__ constexpr int block_values() { return FMT == kMX ? 32 : 16; }
@@ -35,9 +39,9 @@ template <int FMT>
 __host__ __device__ constexpr int tile_cols() { return 4 * block_values<FMT>(); }
 
 // Byte of scale (r, c) in the swizzled layout with `ct` tiles per row of tiles.
-__host__ __device__ __forceinline__ int64_t swizzled_byte(int64_t r, int64_t c, int64_t ct) {
+__host__ __device__ __forceinline__ int64_t swizzled_byte(int64_t r, int c, int ct) {
   const int rin = static_cast<int>(r & 127);
-  return ((r >> 7) * ct + (c >> 2)) * 512 + (rin & 31) * 16 + (rin >> 5) * 4 + static_cast<int>(c & 3);
+  return ((r >> 7) * ct + (c >> 2)) * 512 + (rin & 31) * 16 + (rin >> 5) * 4 + (c & 3);
 }
 
 // Scale rows of tokens. Every tile of `tile` tokens of an expert starts on a
@@ -65,17 +69,18 @@ struct QuantArgs {
   const void* x;
   int64_t x_stride;      // values between rows
   int64_t rows;          // rows per matrix
-  int64_t rows_padded;   // rows that get scales (a multiple of 128 when swizzled, without `ends`)
+  int64_t rows_padded;   // rows that get scales (a multiple of 128 for swizzled weights)
   int64_t batch;
   int32_t cols;
-  int32_t octets;        // octets per row that are walked (padding included)
-  int32_t vec;           // rows of x start on 16-byte boundaries
+  int32_t units;         // units of 16 columns per row that are walked (padding included)
+  int32_t vec;           // rows of x start on 32-byte boundaries
   uint8_t* codes;
   int64_t code_pitch;    // bytes between rows
   uint8_t* scale;
   int32_t scale_cols;    // scales per row (row-major) or tiles per row (swizzled)
   int32_t swizzled;
-  int32_t words;         // four scales leave as one word: lanes and words stay aligned across rows
+  int32_t words;         // four scales leave as one aligned word
+  int32_t pairs;         // 8-byte stores of codes are aligned
   int32_t pad_codes;     // also write the codes of padding columns (as zeros)
   int32_t scale_mode;
   int32_t second_mode;
@@ -88,41 +93,81 @@ struct QuantArgs {
   int32_t token_tile;    // 0: rows are a weight's; else tokens in tiles of so many (first_scale_row)
 };
 
+// Lanes that share a row: 32, or fewer (at least a tile of scales) for short rows.
+__host__ __device__ __forceinline__ int lanes_per_row(int units) { return units > 16 ? 32 : units > 8 ? 16 : 8; }
+// Blocks of kQuantThreads threads that a walk takes.
+__host__ __device__ __forceinline__ int64_t quant_row_blocks(const QuantArgs& q) {
+  const int rows = kQuantThreads / lanes_per_row(q.units) * kQuantRows;
+  return (q.rows_padded + rows - 1) / rows;
+}
+__host__ __device__ __forceinline__ int64_t quant_blocks(const QuantArgs& q) {
+  return q.batch * quant_row_blocks(q) * ((q.units + 31) / 32);
+}
+
+// 16 neighbouring values as they are stored.
 template <int DT>
-__device__ __forceinline__ void load8(const void* base, int64_t at, bool vec, float (&v)[8]) {
+struct Raw {
+  uint32_t w[DT == kBF16 ? 8 : 16];
+};
+
+__device__ __forceinline__ void load32(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_unit(const void* x, int64_t at, bool vec) {
+  Raw<DT> r;
   if constexpr (DT == kBF16) {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    const uint16_t* p = static_cast<const uint16_t*>(x) + at;
     if (vec) {
-      const uint4 q = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      }
+      load32(p, r.w);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
+      for (int i = 0; i < 8; ++i) r.w[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
     }
   } else {
-    const float* p = static_cast<const float*>(base) + at;
+    const uint32_t* p = static_cast<const uint32_t*>(x) + at;
     if (vec) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      load32(p, r.w);
+      load32(p + 8, r.w + 8);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[i];
+      for (int i = 0; i < 16; ++i) r.w[i] = p[i];
     }
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void to_floats(const Raw<DT>& r, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (DT == kBF16) v[i] = __uint_as_float(i & 1 ? r.w[i >> 1] & 0xFFFF0000u : r.w[i >> 1] << 16);
+    else v[i] = __uint_as_float(r.w[i]);
   }
 }
 
-// Bits of max|v|: as integers a NaN is above infinity, so it is never lost.
-__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
-  uint32_t m = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return m;
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Bits of max|v|. A NaN stays one, and as an integer it is above infinity.
+__device__ __forceinline__ uint32_t amax16(const float (&v)[16]) {
+  float m = max3_abs_nan(v[0], v[1], v[2]), n = max3_abs_nan(v[3], v[4], v[5]);
+  m = max3_abs_nan(m, v[6], v[7]);
+  n = max3_abs_nan(n, v[8], v[9]);
+  m = max3_abs_nan(m, v[10], v[11]);
+  n = max3_abs_nan(n, v[12], v[13]);
+  return __float_as_uint(max3_abs_nan(max3_abs_nan(m, v[14], v[15]), n, n)) & 0x7FFFFFFFu;
 }
 
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax, int mode) {
@@ -149,270 +194,343 @@ __device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax, bool two, float
   return pm::enc_e4m3(fminf(fmaxf(s, 0.015625f), 448.0f));
 }
 
-// Codes of 8 values (the first in the lowest nibble). `mul` multiplies; where
-// `unit` is nonzero the quotient v / unit is wanted instead and mul = 1 / unit:
-// one residual step makes v * mul the correctly rounded quotient's side of
-// every rounding boundary (boundaries times a 4-bit unit are exact in fp32, so
-// a quotient that is not on a boundary is over half an ulp away from it, and
-// one that is comes out exactly).
-__device__ __forceinline__ uint32_t encode8(const float (&v)[8], float mul, float unit) {
-  float q[8];
+// Codes of 16 values (the first in the lowest nibble). kQuotient: v / unit is
+// wanted, mul = 1 / unit, and one residual step makes v * mul fall on the
+// quotient's side of every rounding boundary: boundaries times a 4-bit unit
+// are exact in fp32, so a quotient that is not on a boundary is over half an
+// ulp away from it, and one that is comes out exactly.
+template <bool kQuotient>
+__device__ __forceinline__ uint2 encode16(const float (&v)[16], float mul, float unit) {
+  uint32_t w[2] = {0u, 0u};
+  const float2 m2 = make_float2(mul, mul), u2 = make_float2(-unit, -unit);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    q[i] = __fmul_rn(v[i], mul);
-    if (unit != 0.0f) q[i] = __fmaf_rn(__fmaf_rn(-q[i], unit, v[i]), mul, q[i]);
+    const float2 x = make_float2(v[2 * i], v[2 * i + 1]);
+    float2 q = __fmul2_rn(x, m2);
+    if constexpr (kQuotient) q = __ffma2_rn(__ffma2_rn(q, u2, x), m2, q);
+    w[i >> 2] |= pm::enc_e2m1x2(q.x, q.y) << (8 * (i & 3));
   }
-  uint32_t w = 0u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= pm::enc_e2m1x2(q[2 * i], q[2 * i + 1]) << (8 * i);
-  return w;
+  return make_uint2(w[0], w[1]);
 }
 
-template <int FMT>
-struct Scaled {
-  uint32_t byte, codes;
+struct Coded {
+  uint2 codes;
+  uint32_t byte;  // the block's scale
 };
 
-// One lane's 8 values of a block that spans neighbouring lanes (all of which call).
+// One lane's 16 values; an MXFP4 block is two neighbouring lanes (the whole warp calls).
 template <int FMT>
-__device__ __forceinline__ Scaled<FMT> quantize8(float (&v)[8], int mode, bool two, float g, float inv_g) {
-  uint32_t m = amax8(v);
-  m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  if constexpr (FMT == kMX) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  Scaled<FMT> out;
+__device__ __forceinline__ Coded quantize16(float (&v)[16], int mode, bool two, float g, float inv_g) {
+  uint32_t m = amax16(v);
+  Coded out;
   if constexpr (FMT == kMX) {
+    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
     out.byte = mx_scale_byte(m, mode);
-    out.codes = encode8(v, mx_inverse(out.byte), 0.0f);
+    out.codes = encode16<false>(v, mx_inverse(out.byte), 0.0f);
   } else {
     out.byte = nv_scale_byte(m, two, g);
     const float unit = pm::dec_e4m3(out.byte);
     if (two) {
-      out.codes = encode8(v, __fdiv_rn(inv_g, unit), 0.0f);
+      out.codes = encode16<false>(v, __fdiv_rn(inv_g, unit), 0.0f);
     } else {
       if (m >= 0x7F800000u) {  // keep infinities out of the residual: 2^20 saturates as they do
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -1048576.0f), 1048576.0f);
+        for (int i = 0; i < 16; ++i) v[i] = fminf(fmaxf(v[i], -1048576.0f), 1048576.0f);
       }
-      out.codes = encode8(v, __fdiv_rn(1.0f, unit), unit);
+      out.codes = encode16<true>(v, __fdiv_rn(1.0f, unit), unit);
     }
   }
   return out;
 }
 
-// A whole block of threads quantizes the octets [first, first + kOctetsPerBlock)
-// of a walk over batch x rows_padded x octets.
-template <int DT, int FMT>
-__device__ void quantize_octets(const QuantArgs& q, int64_t first) {
-  constexpr int kLanes = FMT == kMX ? 4 : 2;  // lanes per block
-  const int64_t total = q.batch * q.rows_padded * q.octets;
-  const int64_t row0 = first / q.octets;
-  const uint32_t col0 = static_cast<uint32_t>(first - row0 * q.octets);
-  const bool words = q.words != 0;
-  const uint32_t lane = threadIdx.x & 31u;
+// The scales of four neighbouring blocks as a word, in the first one's lane.
+template <int FMT>
+__device__ __forceinline__ uint32_t gather_scales(uint32_t byte) {
+  constexpr int kLanes = FMT == kMX ? 2 : 1;
+  uint32_t word = byte | (__shfl_down_sync(0xFFFFFFFFu, byte, kLanes) << 8);
+  return word | (__shfl_down_sync(0xFFFFFFFFu, word, 2 * kLanes) << 16);
+}
 
-  float v[kQuantUnroll][8];
-  int64_t row[kQuantUnroll];
-  uint32_t oct[kQuantUnroll];
-  bool inside[kQuantUnroll];
+// The second-level scale that a maximum gives; not fmaxf: a NaN stays one.
+__device__ __forceinline__ float second_of_amax(uint32_t amax) {
+  const float g = __fdiv_rn(__uint_as_float(amax), 2688.0f);
+  return g < 1.1920928955078125e-07f ? 1.1920928955078125e-07f : g;
+}
+
+// A warp quantizes kQuantRows rows (more where a row is short) x 512 columns of matrix e.
+template <int DT, int FMT>
+__device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk, float g, float inv_g) {
+  constexpr int kLanes = FMT == kMX ? 2 : 1;  // lanes per block
+  const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
+  const int unit = chunk * 32 + (lane & (per - 1));
+  const int step = 32 / per;  // rows side by side in the warp
+  const int64_t first = row0 + lane / per;
+  const bool in_row = unit < q.units, in_cols = unit * kUnit < q.cols;
+
+  Raw<DT> raw[kQuantRows];
 #pragma unroll
-  for (int u = 0; u < kQuantUnroll; ++u) {
-    const uint32_t k = col0 + u * kQuantThreads + threadIdx.x;
-    const uint32_t r = k / static_cast<uint32_t>(q.octets);
-    row[u] = row0 + r;
-    oct[u] = k - r * q.octets;
-    inside[u] = first + u * kQuantThreads + threadIdx.x < total;
-    const int64_t e = q.batch == 1 ? 0 : row[u] / q.rows_padded;
-    const int64_t rin = row[u] - e * q.rows_padded;
-    if (inside[u] && rin < q.rows && static_cast<int>(oct[u]) * 8 < q.cols) {
-      load8<DT>(q.x, (e * q.rows + rin) * q.x_stride + oct[u] * 8, q.vec != 0, v[u]);
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = first + u * step;
+    if (in_cols && r < q.rows) {
+      raw[u] = load_unit<DT>(q.x, (e * q.rows + r) * q.x_stride + unit * kUnit, q.vec != 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+      for (auto& w : raw[u].w) w = 0u;
     }
   }
+  const bool two = FMT == kNV && q.second_mode != kSecondNone;
+  const int c = unit / kLanes;
 #pragma unroll
-  for (int u = 0; u < kQuantUnroll; ++u) {
-    const int64_t e = q.batch == 1 ? 0 : row[u] / q.rows_padded;
-    const int64_t rin = row[u] - e * q.rows_padded;
-    float g = 1.0f, inv_g = 1.0f;
-    const bool two = FMT == kNV && q.second_mode != kSecondNone;
-    if (two && inside[u]) {
-      if (q.second_mode == kSecondGiven) {
-        g = q.second[e];
-      } else {
-        // not fmaxf: a NaN maximum stays one
-        g = __fdiv_rn(__uint_as_float(q.amax[e]), 2688.0f);
-        if (g < 1.1920928955078125e-07f) g = 1.1920928955078125e-07f;
-        if (rin == 0 && oct[u] == 0) q.second[e] = g;
-      }
-      inv_g = __fdiv_rn(1.0f, g);
-    }
-    const Scaled<FMT> s = quantize8<FMT>(v[u], q.scale_mode, two, g, inv_g);
-    const bool live = rin < q.rows;
-    const bool padding = !live || static_cast<int>(oct[u]) * 8 >= q.cols;
-    const uint32_t byte = padding ? 0u : s.byte;
-    // gather the scales of this lane and the next three blocks
-    uint32_t word = byte;
-    word |= __shfl_down_sync(0xFFFFFFFFu, word, kLanes) << 8;
-    word |= __shfl_down_sync(0xFFFFFFFFu, word, 2 * kLanes) << 16;
-    if (!inside[u]) continue;
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = first + u * step;
+    float v[16];
+    to_floats(raw[u], v);
+    const Coded s = quantize16<FMT>(v, q.scale_mode, two, g, inv_g);
+    const bool live = r < q.rows;
+    const uint32_t byte = live && in_cols ? s.byte : 0u;
+    const uint32_t word = gather_scales<FMT>(byte);
+    if (!in_row || r >= q.rows_padded) continue;
 
-    int64_t srow = rin;
+    int64_t srow = r;
     if (q.token_tile != 0) {
       int x = 0;
       int64_t start = 0;
       if (q.ends != nullptr) {
-        x = expert_of_row(q.ends, q.experts, rin);
+        x = expert_of_row(q.ends, q.experts, r);
         start = x > 0 ? q.ends[x - 1] : 0;
-        if (x >= q.experts || start < 0 || start > rin) continue;  // a row of no expert
+        if (x >= q.experts || start < 0 || start > r) continue;  // a row of no expert
       }
-      const int o = static_cast<int>(rin - start);
+      const int o = static_cast<int>(r - start);
       srow = first_scale_row(start, x, q.token_tile) +
              static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
     }
-    const int c = static_cast<int>(oct[u]) / kLanes;
-    const int lanes = static_cast<int>(oct[u]) % kLanes;
-    if (q.swizzled) {
-      uint8_t* base = q.scale + (e * (q.rows_padded >> 7)) * static_cast<int64_t>(q.scale_cols) * 512;
-      uint8_t* at = base + swizzled_byte(srow, c, q.scale_cols);
-      if (words) {
-        if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
-      } else if (lanes == 0) {
-        *at = static_cast<uint8_t>(byte);
-      }
-    } else {
-      uint8_t* at = q.scale + (e * q.rows + rin) * q.scale_cols + c;
-      if (words) {
-        if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
-      } else if (lanes == 0) {
-        *at = static_cast<uint8_t>(byte);
+    uint8_t* at = q.swizzled ? q.scale + e * (q.rows_padded >> 7) * q.scale_cols * 512 + swizzled_byte(srow, c, q.scale_cols)
+                             : q.scale + (e * q.rows + r) * q.scale_cols + c;
+    if (q.words) {
+      if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
+    } else if (lane % kLanes == 0) {
+      *at = static_cast<uint8_t>(byte);
+    }
+    if (live && (q.pad_codes || in_cols)) {
+      uint8_t* to = q.codes + (e * q.rows + r) * q.code_pitch + unit * 8;
+      if (q.pairs) {
+        *reinterpret_cast<uint2*>(to) = s.codes;
+      } else {
+        reinterpret_cast<uint32_t*>(to)[0] = s.codes.x;
+        reinterpret_cast<uint32_t*>(to)[1] = s.codes.y;
       }
     }
-    if (live && (q.pad_codes || !padding))
-      *reinterpret_cast<uint32_t*>(q.codes + (e * q.rows + rin) * q.code_pitch + oct[u] * 4) = s.codes;
   }
+}
+
+// Block `b` of quant_blocks(q).
+template <int DT, int FMT>
+__device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
+  const int chunks = (q.units + 31) / 32;
+  const int64_t per = quant_row_blocks(q);
+  const int64_t rb = b / chunks, e = q.batch == 1 ? 0 : rb / per;
+  const int chunk = static_cast<int>(b - rb * chunks);
+  const int rows = 32 / lanes_per_row(q.units) * kQuantRows;  // per warp
+  const int64_t row0 = (rb - e * per) * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows;
+  float g = 1.0f, inv_g = 1.0f;
+  if (FMT == kNV && q.second_mode != kSecondNone) {
+    g = q.second_mode == kSecondGiven ? q.second[e] : second_of_amax(q.amax[e]);
+    inv_g = __fdiv_rn(1.0f, g);
+    if (q.second_mode == kSecondCompute && rb == e * per && chunk == 0 && threadIdx.x == 0) q.second[e] = g;
+  }
+  quantize_rows<DT, FMT>(q, e, row0, chunk, g, inv_g);
 }
 
 template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantArgs q) {
-  const int64_t b = q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x;
-  quantize_octets<DT, FMT>(q, b * kOctetsPerBlock);
+  quantize_block<DT, FMT>(q, q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x);
+}
+
+// Bits of the largest magnitude of a warp's rows x 512 columns, in every lane.
+template <int DT>
+__device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk) {
+  const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
+  const int unit = chunk * 32 + (lane & (per - 1));
+  const int step = 32 / per;
+  const int64_t first = row0 + lane / per;
+  Raw<DT> raw[kQuantRows];
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = first + u * step;
+    if (unit * kUnit < q.cols && r < q.rows) {
+      raw[u] = load_unit<DT>(q.x, (e * q.rows + r) * q.x_stride + unit * kUnit, q.vec != 0);
+    } else {
+#pragma unroll
+      for (auto& w : raw[u].w) w = 0u;
+    }
+  }
+  uint32_t m = 0u;
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    float v[16];
+    to_floats(raw[u], v);
+    m = max(m, amax16(v));
+  }
+  return __reduce_max_sync(0xFFFFFFFFu, m);
 }
 
 // max|x| of each matrix as integer bits (order does not matter to a maximum).
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) amax_kernel(const __grid_constant__ QuantArgs q, uint32_t* amax) {
-  const int64_t octets = q.cols / 8;
-  const int64_t total = q.rows * octets;
-  const int64_t e = blockIdx.y;
+  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * kQuantRows;
+  const int64_t blocks = quant_row_blocks(q) * chunks;
   uint32_t m = 0u;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kOctetsPerBlock;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kOctetsPerBlock; first < total; first += step) {
-    const int64_t row0 = first / octets;
-    const uint32_t col0 = static_cast<uint32_t>(first - row0 * octets);
-    float v[kQuantUnroll][8];
-#pragma unroll
-    for (int u = 0; u < kQuantUnroll; ++u) {
-      const uint32_t k = col0 + u * kQuantThreads + threadIdx.x;
-      const uint32_t r = k / static_cast<uint32_t>(octets);
-      if (first + u * kQuantThreads + threadIdx.x < total) {
-        load8<DT>(q.x, (e * q.rows + row0 + r) * q.x_stride + (k - r * octets) * 8, q.vec != 0, v[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kQuantUnroll; ++u) m = max(m, amax8(v[u]));
+  for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const int64_t rb = b / chunks;
+    m = max(m, amax_rows<DT>(q, blockIdx.y, rb * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows,
+                             static_cast<int>(b - rb * chunks)));
   }
-  m = __reduce_max_sync(0xFFFFFFFFu, m);
   __shared__ uint32_t part[kQuantThreads / 32];
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < kQuantThreads / 32; ++i) m = max(m, part[i]);
-    atomicMax(amax + e, m);
+    atomicMax(amax + blockIdx.y, m);
   }
 }
 
+// Both passes over a small matrix in one block, the second from L1: one
+// launch instead of a clear, a maximum and a quantisation.
+template <int DT, int FMT>
+__global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __grid_constant__ QuantArgs q) {
+  __shared__ uint32_t part[kSmallThreads / 32];
+  const int64_t e = blockIdx.x;
+  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * kQuantRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pieces = static_cast<int>((q.rows_padded + rows - 1) / rows) * chunks;
+  uint32_t m = 0u;
+  for (int i = warp; i < pieces; i += kSmallThreads / 32)
+    m = max(m, amax_rows<DT>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks));
+  if (lane == 0) part[warp] = m;
+  __syncthreads();
+  const float g = second_of_amax(__reduce_max_sync(0xFFFFFFFFu, part[lane % (kSmallThreads / 32)]));
+  if (threadIdx.x == 0) q.second[e] = g;
+  const float inv_g = __fdiv_rn(1.0f, g);
+  for (int i = warp; i < pieces; i += kSmallThreads / 32)
+    quantize_rows<DT, FMT>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, g, inv_g);
+}
+
 // ------------------------------------------------------------ back to values
+template <int FMT>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return FMT == kMX ? pm::dec_e8m0(byte) : pm::dec_e4m3(byte);
+}
+
+// Four codes of `nibbles` (low 16 bits) times a scale, as two bf16 pairs: a
+// code times a block scale has at most 6 significant bits, so this is exact.
+// The magnitudes' bf16 bytes come from two 8-entry tables; a selector with bit
+// 3 set would replicate the byte's sign, which gives the sign bits.
+__device__ __forceinline__ void decode4(uint32_t nibbles, __nv_bfloat162 scale, uint32_t& lo, uint32_t& hi) {
+  const uint32_t sel = nibbles & 0x7777u;
+  const uint32_t top = __byte_perm(0x3F3F3F00u, 0x40404040u, sel);
+  const uint32_t low = __byte_perm(0xC0800000u, 0xC0804000u, sel);
+  // 0x80 for a positive code, 0xFF for a negative one
+  uint32_t sign;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(sign) : "r"(0x80808080u), "r"(nibbles));
+  const uint32_t high = top | ((sign << 7) & 0x80808080u);
+  uint32_t a = __byte_perm(low, high, 0x5140), b = __byte_perm(low, high, 0x7362);
+  __nv_bfloat162 x = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), scale);
+  __nv_bfloat162 y = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&b), scale);
+  lo = *reinterpret_cast<uint32_t*>(&x);
+  hi = *reinterpret_cast<uint32_t*>(&y);
+}
+
 struct DequantArgs {
   const uint8_t* codes;
   const uint8_t* scale;
   const float* second;  // (batch) or NULL
   void* y;
   int64_t rows, batch;
-  int32_t cols, swizzled, scale_cols, vec;  // vec: codes and y allow whole-octet accesses
+  int32_t cols, swizzled, scale_cols;
+  int32_t vec;          // units of codes and of y are aligned
 };
 
-template <int FMT>
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-  return FMT == kMX ? pm::dec_e8m0(byte) : pm::dec_e4m3(byte);
-}
-
+// Blocks of threads as in a quantisation without padding.
 template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_constant__ DequantArgs d) {
-  constexpr int kLanes = FMT == kMX ? 4 : 2;
-  const int64_t octets = d.cols / 8;
-  const int64_t total = d.batch * d.rows * octets;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kOctetsPerBlock;
-  const int64_t row0 = first / octets;
-  const uint32_t col0 = static_cast<uint32_t>(first - row0 * octets);
-  const int64_t rt = (d.rows + 127) >> 7;
+  constexpr int kLanes = FMT == kMX ? 2 : 1;
+  const int units = d.cols / kUnit, per = lanes_per_row(units), chunks = (units + 31) / 32, step = 32 / per;
+  const int block_rows = kQuantThreads / per * kQuantRows;
+  const int64_t row_blocks = (d.rows + block_rows - 1) / block_rows;
+  const int64_t rb = blockIdx.x / chunks, e = d.batch == 1 ? 0 : rb / row_blocks;
+  const int lane = threadIdx.x & 31;
+  const int unit = static_cast<int>(blockIdx.x - rb * chunks) * 32 + (lane & (per - 1));
+  const int64_t first = (rb - e * row_blocks) * block_rows + (threadIdx.x >> 5) * (step * kQuantRows) + lane / per;
+  const uint8_t* scales = d.swizzled ? d.scale + e * ((d.rows + 127) >> 7) * d.scale_cols * 512 : d.scale + e * d.rows * d.scale_cols;
+  const float g = d.second != nullptr ? d.second[e] : 1.0f;
+  if (unit >= units) return;
+  const int c = unit / kLanes;
+  uint2 codes[kQuantRows];
+  uint32_t byte[kQuantRows];
 #pragma unroll
-  for (int u = 0; u < kQuantUnroll; ++u) {
-    const uint32_t k = col0 + u * kQuantThreads + threadIdx.x;
-    const uint32_t r = k / static_cast<uint32_t>(octets);
-    const int64_t row = row0 + r;
-    const uint32_t oct = k - r * static_cast<uint32_t>(octets);
-    if (first + u * kQuantThreads + threadIdx.x >= total) break;
-    const int64_t e = d.batch == 1 ? 0 : row / d.rows;
-    const int c = static_cast<int>(oct) / kLanes;
-    const uint8_t* sp = d.swizzled ? d.scale + e * rt * d.scale_cols * 512 + swizzled_byte(row - e * d.rows, c, d.scale_cols)
-                                   : d.scale + row * d.scale_cols + c;
-    const float s = scale_value<FMT>(*sp);
-    const float g = d.second != nullptr ? d.second[e] : 1.0f;
-    const uint8_t* cp = d.codes + (row * octets + oct) * 4;
-    uint32_t w;
-    if (d.vec) {
-      w = *reinterpret_cast<const uint32_t*>(cp);
-    } else {
-      w = cp[0] | (cp[1] << 8) | (cp[2] << 16) | (static_cast<uint32_t>(cp[3]) << 24);
-    }
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pm::dec_e2m1x2((w >> (8 * i)) & 0xFFu, v[2 * i], v[2 * i + 1]);
-      v[2 * i] = __fmul_rn(__fmul_rn(v[2 * i], s), g);
-      v[2 * i + 1] = __fmul_rn(__fmul_rn(v[2 * i + 1], s), g);
-    }
-    const int64_t at = (row * octets + oct) * 8;
-    if constexpr (DT == kBF16) {
-      uint16_t* p = static_cast<uint16_t*>(d.y) + at;
-      uint32_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        o[i] = *reinterpret_cast<const uint32_t*>(&b);
-      }
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = first + u * step;
+    codes[u] = make_uint2(0u, 0u);
+    byte[u] = 0u;
+    if (r < d.rows) {
+      byte[u] = d.swizzled ? scales[swizzled_byte(r, c, d.scale_cols)] : scales[r * d.scale_cols + c];
+      const uint8_t* from = d.codes + ((e * d.rows + r) * units + unit) * 8;
       if (d.vec) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+        codes[u] = *reinterpret_cast<const uint2*>(from);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[2 * i] = static_cast<uint16_t>(o[i]);
-          p[2 * i + 1] = static_cast<uint16_t>(o[i] >> 16);
+          codes[u].x |= static_cast<uint32_t>(from[i]) << (8 * i);
+          codes[u].y |= static_cast<uint32_t>(from[4 + i]) << (8 * i);
         }
       }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kQuantRows; ++u) {
+    const int64_t r = first + u * step;
+    if (r >= d.rows) break;
+    const __nv_bfloat162 s = __float2bfloat162_rn(scale_value<FMT>(byte[u]));
+    uint32_t w[8];
+    decode4(codes[u].x, s, w[0], w[1]);
+    decode4(codes[u].x >> 16, s, w[2], w[3]);
+    decode4(codes[u].y, s, w[4], w[5]);
+    decode4(codes[u].y >> 16, s, w[6], w[7]);
+    const int64_t at = ((e * d.rows + r) * units + unit) * kUnit;
+    if (DT == kBF16 && d.second == nullptr) {
+      // exact as they are
     } else {
-      float* p = static_cast<float*>(d.y) + at;
+      uint32_t f[16];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[2 * i] = __float_as_uint(__fmul_rn(__uint_as_float(w[i] << 16), g));
+        f[2 * i + 1] = __float_as_uint(__fmul_rn(__uint_as_float(w[i] & 0xFFFF0000u), g));
+      }
+      if constexpr (DT == kBF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(f[2 * i]), __uint_as_float(f[2 * i + 1]));
+          w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      } else {
+        uint32_t* p = static_cast<uint32_t*>(d.y) + at;
+        if (d.vec) {
+          store32(p, f);
+          store32(p + 8, f + 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = f[i];
+        }
+      }
+    }
+    if constexpr (DT == kBF16) {
+      uint16_t* p = static_cast<uint16_t*>(d.y) + at;
       if (d.vec) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        store32(p, w);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = v[i];
+        for (int i = 0; i < 16; ++i) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
       }
     }
   }
@@ -448,9 +566,9 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
     if (row < p.rows) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t c = tc * 4 + j;
+        const int c = static_cast<int>(tc) * 4 + j;
         if (c < p.scale_cols) {
-          const uint8_t* s = p.swizzled ? p.scale + e * rt * ct * 512 + swizzled_byte(row, c, ct)
+          const uint8_t* s = p.swizzled ? p.scale + e * rt * ct * 512 + swizzled_byte(row, c, static_cast<int>(ct))
                                         : p.scale + (e * p.rows + row) * p.scale_cols + c;
           w |= static_cast<uint32_t>(*s) << (8 * j);
         }
@@ -471,13 +589,13 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
 }
 
 // What a product needs ahead of it, in one launch: blocks below
-// `quant_blocks` quantize tokens, the others lay weights out.
+// `token_blocks` quantize tokens, the others lay weights out.
 template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads)
-    prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t quant_blocks) {
+    prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t token_blocks) {
   grid_launch_dependents();
-  if (blockIdx.x < quant_blocks) quantize_octets<DT, FMT>(q, static_cast<int64_t>(blockIdx.x) * kOctetsPerBlock);
-  else repack(p, static_cast<int64_t>(blockIdx.x - quant_blocks) * kQuantThreads + threadIdx.x);
+  if (blockIdx.x < token_blocks) quantize_block<DT, FMT>(q, blockIdx.x);
+  else repack(p, static_cast<int64_t>(blockIdx.x - token_blocks) * kQuantThreads + threadIdx.x);
 }
 
 }  // namespace fp4
