@@ -133,37 +133,38 @@ constexpr int64_t kSmallMatrix = 65536;
   } while (0)
 
 // ---------------------------------------------------------------- the product
-// Scratch of a product: quantized tokens, and the weight's parts that are not
-// stored as the product reads them.
+// How a product runs, and its scratch: quantized tokens, and codes that are
+// not stored as the product reads them.
 struct LinearPlan {
-  int bn;                              // tokens per tile
-  bool move_codes, move_scale;
-  int64_t k_padded;                    // columns up to a whole scale tile
-  int64_t x_codes, x_scale, w_codes, w_scale, total;  // byte offsets
+  bool fused;       // tokens are quantized by the product itself
+  bool move_codes;
+  int bn;           // tokens per tile
+  int64_t k_padded; // columns up to a whole scale tile
+  int64_t x_codes, x_scale, w_codes, total;  // byte offsets
   int64_t w_code_pitch, scale_tiles, scale_rows;
 };
 
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = tokens / w.batch;
-  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 192;
+  p.fused = per_expert <= 32;
+  p.bn = p.fused ? 32 : per_expert <= 512 ? 128 : 192;
   const int tile = block_of(w) * 4;
   p.scale_tiles = (w.cols + tile - 1) / tile;
   p.k_padded = p.scale_tiles * tile;
   p.move_codes = w.cols % 32 != 0 || !aligned(w.codes, 16);
-  p.move_scale = !w.swizzled || w.cols % 64 != 0 || !aligned(w.scale, 16);
   p.w_code_pitch = up(w.cols / 2, 16);
-  // one more than first_scale_row's numbers can reach
-  p.scale_rows = (tokens / p.bn + w.batch + 1) * fp4::scale_rows_per_tile(p.bn);
   int64_t at = 0;
-  p.x_codes = at;
-  at += align256(tokens * (p.k_padded / 2));
-  p.x_scale = at;
-  at += align256(p.scale_rows * p.scale_tiles * 4);
+  if (!p.fused) {
+    // one more than first_scale_row's numbers can reach
+    p.scale_rows = (tokens / p.bn + w.batch + 1) * fp4::scale_rows_per_tile(p.bn);
+    p.x_codes = at;
+    at += align256(tokens * (p.k_padded / 2));
+    p.x_scale = at;
+    at += align256(p.scale_rows * p.scale_tiles * 4);
+  }
   p.w_codes = at;
   if (p.move_codes) at += align256(w.batch * w.rows * p.w_code_pitch);
-  p.w_scale = at;
-  if (p.move_scale) at += align256(w.batch * up(w.rows, 128) * p.scale_tiles * 4);
   p.total = at;
   return p;
 }
@@ -178,23 +179,40 @@ int64_t token_tiles(const fp4::Groups& g, int bn) {
   return g.ends == nullptr ? (g.tokens + bn - 1) / bn : g.tokens / bn + std::min<int64_t>(g.experts + 1, g.tokens);
 }
 
-template <int DT, int FMT, int BN>
-cudaError_t launch_linear(const fp4::LinearArgs& args, int64_t items, cudaStream_t stream) {
-  using S = fp4::LinearShape<FMT, BN>;
-  auto kernel = fp4::linear_kernel<DT, FMT, BN>;
+// Blocks of a cluster that share a tile's K: as many as keep the SMs busy in
+// one wave, at least two stages for each. 4096 x 14336, one token (32 tiles):
+// TODO us with 8, TODO with 1.
+template <class S>
+int split_of(int64_t items, int stages) {
+  int split = 1;
+  while (S::kCanSplit && split < fp4::kMaxSplit && items * split * 2 <= static_cast<int64_t>(sm_count()) * S::kCtas &&
+         stages >= split * 4)
+    split *= 2;
+  return split;
+}
+
+template <int DT, int FMT, int BN, bool kFused>
+cudaError_t launch_linear(fp4::LinearArgs& args, int64_t items, cudaStream_t stream) {
+  using S = fp4::LinearShape<FMT, BN, kFused>;
+  auto kernel = fp4::linear_kernel<DT, FMT, BN, kFused>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
+  args.split = split_of<S>(items, (args.k_steps + 3) / 4);
+  cudaLaunchAttribute attributes[2] = {};
   // may start while the launch before it still quantizes; the kernel waits where it needs that
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = kFused ? 0 : 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = static_cast<unsigned>(args.split);
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, sm_count())));
-  config.blockDim = dim3(fp4::kLinearThreads);
+  config.gridDim = dim3(static_cast<unsigned>(
+      args.split > 1 ? items * args.split : std::min<int64_t>(items, static_cast<int64_t>(sm_count()) * S::kCtas)));
+  config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.attrs = attributes;
+  config.numAttrs = args.split > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&config, kernel, args);
   return e == cudaSuccess ? launched() : e;
 }
@@ -342,81 +360,94 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   FP4_REQUIRE(scale_mode >= 0 && scale_mode <= 3, "Unsupported MX scaling mode id.");
   FP4_REQUIRE(act_second == nullptr || w->format == PIPER_FP4_NV, "MXFP4 activations have no second-level scale.");
   const LinearPlan p = plan_linear(*w, tokens);
-  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256))
+  if (p.total > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256)))
     return fail(PIPER_FP4_EWORKSPACE, "FP4 product: workspace missing, too small or not 256-byte aligned.");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-
-  fp4::QuantArgs q{};
-  q.x = x;
-  q.x_stride = x_stride;
-  q.rows = q.rows_padded = tokens;
-  q.batch = 1;
-  q.cols = static_cast<int32_t>(w->cols);
-  q.units = static_cast<int32_t>(p.k_padded / fp4::kUnit);
-  q.vec = aligned(x, 32) && (x_stride * static_cast<int64_t>(width(dtype))) % 32 == 0;
-  q.codes = ws + p.x_codes;
-  q.code_pitch = p.k_padded / 2;
-  q.scale = ws + p.x_scale;
-  q.scale_cols = static_cast<int32_t>(p.scale_tiles);
-  q.swizzled = q.words = q.pairs = q.pad_codes = 1;
-  q.scale_mode = scale_mode;
-  q.second_mode = act_second != nullptr ? PIPER_FP4_SECOND_GIVEN : PIPER_FP4_SECOND_NONE;
-  q.second = const_cast<float*>(act_second);
-  q.token_tile = p.bn;
-  q.ends = ends;
-  q.experts = static_cast<int32_t>(w->batch);
-  fp4::RepackArgs r{};
-  r.codes = static_cast<const uint8_t*>(w->codes);
-  r.code_row = w->cols / 2;
-  r.code_pitch = p.w_code_pitch;
-  r.scale = static_cast<const uint8_t*>(w->scale);
-  r.rows = w->rows;
-  r.batch = w->batch;
-  r.scale_cols = static_cast<int32_t>(w->cols / block_of(*w));
-  r.swizzled = w->swizzled != 0;
-  if (p.move_scale) {
-    r.scale_out = ws + p.w_scale;
-    r.words = w->batch * up(w->rows, 128) * p.scale_tiles;
-  }
-  if (p.move_codes) {
-    r.codes_out = ws + p.w_codes;
-    r.pieces = w->batch * w->rows * (p.w_code_pitch / 16);
-  }
-  const int64_t token_blocks = fp4::quant_blocks(q);
-  const int64_t blocks = token_blocks + (r.words + r.pieces + fp4::kQuantThreads - 1) / fp4::kQuantThreads;
-  FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 product: too many values for one call.");
+  const bool x_vec = aligned(x, 32) && (x_stride * static_cast<int64_t>(width(dtype))) % 32 == 0;
 
   fp4::LinearArgs a{};
-  const int bn = p.bn;
-  const void* codes = p.move_codes ? ws + p.w_codes : w->codes;
-  if (!code_map(&a.w_map, codes, p.w_code_pitch, p.w_code_pitch, w->batch * w->rows, fp4::kTileRows) ||
-      !code_map(&a.x_map, q.codes, q.code_pitch, q.code_pitch, tokens, bn))
-    return fail(PIPER_FP4_ECUDA, "FP4 product: cuTensorMapEncodeTiled failed.");
-  a.w_scale = p.move_scale ? ws + p.w_scale : static_cast<const uint8_t*>(w->scale);
-  a.x_scale = q.scale;
+  a.w_scale = static_cast<const uint8_t*>(w->scale);
   a.w_second = w->second;
   a.x_second = act_second;
+  a.x = x;
+  a.x_stride = x_stride;
   a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->rows + 127) / 128)};
   a.y = y;
   a.rows = static_cast<int32_t>(w->rows);
+  a.cols = static_cast<int32_t>(w->cols);
   a.k_steps = static_cast<int32_t>((w->cols + 63) / 64);
   a.scale_tiles = static_cast<int32_t>(p.scale_tiles);
-  a.early = !p.move_codes && !p.move_scale;
+  a.early = !p.move_codes;
   a.vec = aligned(y, 16) && w->rows % 8 == 0;
-  const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
+  a.x_vec = x_vec;
+  a.scale_mode = scale_mode;
+  a.scale_cols = static_cast<int32_t>(w->cols / block_of(*w));
+  if (w->swizzled) {
+    // a K step reads two or four scales of a tile: with whole steps no padding is read
+    const bool bulk = w->cols % 64 == 0 && aligned(w->scale, 16);
+    a.scale_source = bulk ? fp4::kScalesBulk : fp4::kScalesTiles;
+    a.scale_piece = aligned(w->scale, 16) ? 16 : 1;
+  } else {
+    a.scale_source = fp4::kScalesRows;
+    for (a.scale_piece = 16; a.scale_piece > 1 && (a.scale_cols % a.scale_piece != 0 || !aligned(w->scale, a.scale_piece));)
+      a.scale_piece /= 2;
+  }
+  const int64_t items = token_tiles(a.groups, p.bn) * a.groups.row_tiles;
   a.items = static_cast<int32_t>(items);
-  FP4_REQUIRE(items < (int64_t{1} << 31), "FP4 product: too many tiles for one call.");
+  FP4_REQUIRE(items < (int64_t{1} << 31) / fp4::kMaxSplit, "FP4 product: too many tiles for one call.");
 
+  fp4::QuantArgs q{};
+  int64_t token_blocks = 0;
+  if (!p.fused) {
+    q.x = x;
+    q.x_stride = x_stride;
+    q.rows = q.rows_padded = tokens;
+    q.batch = 1;
+    q.cols = static_cast<int32_t>(w->cols);
+    q.units = static_cast<int32_t>(p.k_padded / fp4::kUnit);
+    q.vec = x_vec;
+    q.codes = ws + p.x_codes;
+    q.code_pitch = p.k_padded / 2;
+    q.scale = ws + p.x_scale;
+    q.scale_cols = static_cast<int32_t>(p.scale_tiles);
+    q.swizzled = q.words = q.pairs = q.pad_codes = 1;
+    q.scale_mode = scale_mode;
+    q.second_mode = act_second != nullptr ? PIPER_FP4_SECOND_GIVEN : PIPER_FP4_SECOND_NONE;
+    q.second = const_cast<float*>(act_second);
+    q.token_tile = p.bn;
+    q.ends = ends;
+    q.experts = static_cast<int32_t>(w->batch);
+    token_blocks = fp4::quant_blocks(q);
+  }
+  a.x_scale = q.scale;
+  fp4::RepackArgs r{};
+  if (p.move_codes) {
+    r.codes = static_cast<const uint8_t*>(w->codes);
+    r.codes_out = ws + p.w_codes;
+    r.row_bytes = w->cols / 2;
+    r.pitch = p.w_code_pitch;
+    r.pieces = w->batch * w->rows * (p.w_code_pitch / 16);
+  }
+  const int64_t blocks = token_blocks + (r.pieces + fp4::kQuantThreads - 1) / fp4::kQuantThreads;
+  FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 product: too many values for one call.");
+  const void* codes = p.move_codes ? ws + p.w_codes : w->codes;
+  if (!code_map(&a.w_map, codes, p.w_code_pitch, p.w_code_pitch, w->batch * w->rows, fp4::kTileRows) ||
+      (!p.fused && !code_map(&a.x_map, q.codes, q.code_pitch, q.code_pitch, tokens, p.bn)))
+    return fail(PIPER_FP4_ECUDA, "FP4 product: cuTensorMapEncodeTiled failed.");
+
+  cudaError_t e = cudaSuccess;
+  if (blocks > 0) {
 #define CALL(D, F) \
   fp4::prepare_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q, r, static_cast<uint32_t>(token_blocks))
-  FP4_DISPATCH(dtype, w->format, CALL);
+    FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
-  cudaError_t e = launched();
-  if (e != cudaSuccess) return cuda_fail("prepare kernel", e);
-#define CALL(D, F)                                            \
-  e = bn == 32 ? launch_linear<D, F, 32>(a, items, s)         \
-               : bn == 128 ? launch_linear<D, F, 128>(a, items, s) : launch_linear<D, F, 192>(a, items, s)
+    e = launched();
+    if (e != cudaSuccess) return cuda_fail("prepare kernel", e);
+  }
+#define CALL(D, F)                                                    \
+  e = p.fused ? launch_linear<D, F, 32, true>(a, items, s)            \
+              : p.bn == 128 ? launch_linear<D, F, 128, false>(a, items, s) : launch_linear<D, F, 192, false>(a, items, s)
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("linear kernel", e);

@@ -3,12 +3,20 @@
 // The weight's rows are the tensor core's 128-row operand and the tokens its
 // N side, so a tile is 128 outputs x up to BN tokens and the instruction's N
 // follows the tokens that are there: experts with few rows waste little.
-// A K step is 64 values (32 bytes a row). Operand tiles come by bulk tensor
-// copies in the 128-byte swizzle (256 values a row and stage), block scales as
-// whole 512-byte tiles of the swizzled layout, from shared memory to tensor
-// memory by tcgen05.cp ahead of the products that use them. The scales are
-// applied inside the tensor core; sums are fp32 in tensor memory, and the one
-// rounding is that of the output.
+// A K step is 64 values (32 bytes a row). Codes come by bulk tensor copies in
+// the 128-byte swizzle (256 values a row and stage); block scales reach shared
+// memory as 512-byte tiles of the swizzled layout and go on to tensor memory
+// by tcgen05.cp ahead of the products that use them. The scales are applied
+// inside the tensor core; sums are fp32 in tensor memory, and the one rounding
+// is that of the output.
+//
+// Many tokens: their codes and scales are made by a launch before (prepare_kernel),
+// tiles are 128 or 192 tokens wide. Few tokens (kFused, tiles of 32): the kernel
+// is a stream of weight bytes, so four warps quantize each stage's tokens on
+// the way and there is no launch before. Where there are too few tiles for the
+// SMs, a cluster of blocks splits K; each leaves its sums in its own shared
+// memory and every block adds up its share of the tokens over the cluster, in
+// rank order, so that results do not depend on timing.
 #pragma once
 #include <cuda.h>
 
@@ -20,25 +28,39 @@ namespace fp4 {
 
 constexpr int kStageCols = 256;      // K values per stage
 constexpr int kStageBytes = kStageCols / 2;
-constexpr int kLinearThreads = 192;  // producer warp, tensor-core warp, four epilogue warps
+constexpr int kQuantWarps = 4;       // kFused
+constexpr int kMaxSplit = 8;
+
+// Where the weight's scales come from: whole swizzled tiles by bulk copies, or
+// by a warp that reads them (swizzled tiles with columns that do not exist, or
+// rows) in pieces of 16 / 8 / 4 / 1 bytes.
+enum : int { kScalesBulk = 0, kScalesTiles = 1, kScalesRows = 2 };
 
 struct LinearArgs {
   CUtensorMap w_map, x_map;
-  const uint8_t* w_scale;  // swizzled tiles, experts on 128-row tiles
-  const uint8_t* x_scale;  // swizzled tiles, rows as first_scale_row places them
+  const uint8_t* w_scale;
+  const uint8_t* x_scale;  // swizzled tiles, rows as first_scale_row places them (not kFused)
   const float* w_second;   // (experts) or NULL
   const float* x_second;   // one or NULL
+  const void* x;           // the tokens themselves (kFused)
+  int64_t x_stride;
   Groups groups;           // row tiles: of 128 outputs
   void* y;
-  int32_t rows;            // outputs per expert
+  int32_t rows, cols;      // of one expert's weight
   int32_t k_steps;         // of 64 values
   int32_t scale_tiles;     // tiles of 4 scales per row (weight and tokens alike)
   int32_t items;           // bound on the tiles
-  int32_t early;           // the weight is used where it is: loads of it need not wait for the launch before
+  int32_t split;           // blocks of a cluster that share a tile's K
+  int32_t early;           // the codes are used where they are: loads of them need not wait for the launch before
   int32_t vec;             // rows of y start on 16-byte boundaries
+  int32_t x_vec;           // rows of x start on 32-byte boundaries
+  int32_t scale_mode;      // of the tokens
+  int32_t scale_source;    // kScales...
+  int32_t scale_cols;      // scales per row (kScalesRows)
+  int32_t scale_piece;     // bytes of an aligned load of the weight's scales
 };
 
-template <int FMT, int BN>
+template <int FMT, int BN, bool kFused>
 struct LinearShape {
   static constexpr int kTiles = FMT == kNV ? 4 : 2;                 // scale tiles per stage and 128 rows
   static constexpr int kXBlocks = (BN + 127) / 128;                 // 128-token scale blocks per tile
@@ -48,21 +70,128 @@ struct LinearShape {
   static constexpr int kSX = kXBlocks * kTiles * 512;
   static constexpr int kStage = kW + kX + kSW + kSX;
   static constexpr int kOut = 4 * 2048;                             // 32 tokens x 32 outputs of each epilogue warp
-  static constexpr int kStages = (kSmemMax - 2048 - kOut) / kStage < 9 ? (kSmemMax - 2048 - kOut) / kStage : 9;
+  static constexpr int kCtas = kFused ? 2 : 1;                      // resident per SM
+  static constexpr int kRoom = kSmemMax / kCtas - 2048 - kOut;
+  static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + 1024 + 512;
-  // tensor memory: two accumulators, then two buffers of scales
+  static constexpr int kThreads = 224 + (kFused ? 32 * kQuantWarps : 0);
+  static constexpr bool kCanSplit = BN * kTileRows * 4 <= kStages * kStage;
+  // tensor memory: two accumulators, then buffers of scales, one per stage if they fit
   static constexpr int kScaleCols = kTiles * 4 * (1 + kXBlocks);
-  static constexpr int kCols = 2 * BN + 2 * kScaleCols;
+  static constexpr int kBufs = (512 / kCtas - 2 * BN) / kScaleCols < kStages ? (512 / kCtas - 2 * BN) / kScaleCols : kStages;
+  static constexpr int kCols = 2 * BN + kBufs * kScaleCols;
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-  static_assert(kCols <= 512 && kStages >= 4, "the tile does not fit");
+  static_assert(kCols <= 512 && kAlloc * kCtas <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
 };
 
-// One persistent block per SM. Roles run through the same tiles on their own:
-// the producer and the tensor-core warp are up to two accumulators ahead of
-// the epilogue.
-template <int DT, int FMT, int BN>
-__global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_constant__ LinearArgs p) {
-  using S = LinearShape<FMT, BN>;
+// The scales that one stage needs of the weight: 128 rows x kTiles words, four rows a lane.
+template <int FMT>
+struct ScaleWords {
+  static constexpr int kTiles = FMT == kNV ? 4 : 2;
+  uint32_t w[4][kTiles];
+};
+
+template <int FMT>
+__device__ __forceinline__ ScaleWords<FMT> load_scale_words(const LinearArgs& p, const TileAt& t, int stage, int lane) {
+  constexpr int kTiles = ScaleWords<FMT>::kTiles;
+  constexpr int kBytes = 4 * kTiles;
+  ScaleWords<FMT> s;
+  const int tile0 = stage * kTiles;
+  if (p.scale_source == kScalesTiles) {
+    // a lane's 16 bytes of a tile are its four rows' words
+    const uint8_t* from = p.w_scale + ((static_cast<int64_t>(t.expert) * p.groups.row_tiles + t.row_tile) * p.scale_tiles + tile0) * 512 + lane * 16;
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) {
+      uint32_t v[4] = {0u, 0u, 0u, 0u};
+      const int left = p.scale_cols - (tile0 + k) * 4;  // scales of this tile that exist
+      if (left > 0) {
+        if (p.scale_piece >= 16) {
+          const uint4 q = *reinterpret_cast<const uint4*>(from + k * 512);
+          v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+#pragma unroll
+          for (int b = 0; b < 16; ++b) v[b >> 2] |= static_cast<uint32_t>(from[k * 512 + b]) << (8 * (b & 3));
+        }
+      }
+      const uint32_t mask = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s.w[j][k] = v[j] & mask;
+    }
+    return s;
+  }
+  const int c0 = tile0 * 4, bytes = min(kBytes, p.scale_cols - c0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) s.w[j][k] = 0u;
+    const int row = t.row_tile * kTileRows + j * 32 + lane;
+    if (row >= p.rows) continue;
+    const uint8_t* from = p.w_scale + (static_cast<int64_t>(t.expert) * p.rows + row) * p.scale_cols + c0;
+    if (bytes == kBytes && p.scale_piece >= kBytes) {
+      if constexpr (kBytes == 16) {
+        const uint4 q = *reinterpret_cast<const uint4*>(from);
+        s.w[j][0] = q.x; s.w[j][1] = q.y; s.w[j][2] = q.z; s.w[j][3] = q.w;
+      } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(from);
+        s.w[j][0] = q.x; s.w[j][1] = q.y;
+      }
+    } else if (p.scale_piece >= 4 && bytes % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k)
+        if (k * 4 < bytes) s.w[j][k] = *reinterpret_cast<const uint32_t*>(from + k * 4);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBytes; ++b)
+        if (b < bytes) s.w[j][b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
+    }
+  }
+  return s;
+}
+
+// A warp quantizes a stage's tokens into the operand's swizzled rows and its
+// scale tiles: half a warp a row, eight (fp32: four) rows in flight.
+template <int DT, int FMT>
+__device__ __forceinline__ void quantize_stage(const LinearArgs& p, const TileAt& t, int stage, uint8_t* codes, uint8_t* scales,
+                                               bool two, float g, float inv_g) {
+  constexpr int kDeep = DT == kBF16 ? 4 : 2;
+  const int lane = threadIdx.x & 31, unit = lane & 15;
+  const int col = stage * kStageCols + unit * kUnit;
+  for (int r0 = 0; r0 < t.count; r0 += 2 * kDeep) {
+    Raw<DT> raw[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int r = r0 + 2 * u + (lane >> 4);
+      if (r < t.count && col < p.cols) {
+        raw[u] = load_unit<DT>(p.x, (t.first + r) * p.x_stride + col, p.x_vec != 0);
+      } else {
+#pragma unroll
+        for (auto& w : raw[u].w) w = 0u;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      if (r0 + 2 * u >= t.count) break;  // the same in all lanes
+      const int r = r0 + 2 * u + (lane >> 4);
+      float v[16];
+      to_floats(raw[u], v);
+      const Coded c = quantize16<FMT>(v, p.scale_mode, two, g, inv_g);
+      const uint32_t word = gather_scales<FMT>(col < p.cols ? c.byte : 0u);
+      if (r < t.count) {
+        *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
+        constexpr int kLanes = FMT == kNV ? 4 : 8;  // units per scale tile
+        if (unit % kLanes == 0) *reinterpret_cast<uint32_t*>(scales + (unit / kLanes) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
+      }
+    }
+  }
+}
+
+// Persistent blocks. Roles run through the same tiles on their own: the
+// producers and the tensor-core warp are up to two accumulators ahead of the
+// epilogue.
+template <int DT, int FMT, int BN, bool kFused>
+__global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, LinearShape<FMT, BN, kFused>::kCtas)
+    linear_kernel(const __grid_constant__ LinearArgs p) {
+  using S = LinearShape<FMT, BN, kFused>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
   uint8_t* out = smem + S::kStages * S::kStage;
@@ -75,9 +204,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (warp == 0 && lane == 0) {
     pm::prefetch_tmap(&p.w_map);
-    pm::prefetch_tmap(&p.x_map);
+    if (!kFused) pm::prefetch_tmap(&p.x_map);
     for (int s = 0; s < S::kStages; ++s) {
-      pm::mbar_init(&full[s], 1);
+      pm::mbar_init(&full[s], 1 + (p.scale_source != kScalesBulk) + kFused);
       pm::mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -93,46 +222,53 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
   __syncthreads();
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
-  const int stages = (p.k_steps + 3) / 4;
+  // this block's part of every tile's stages
+  const int all = (p.k_steps + 3) / 4;
+  const int rank = p.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int from = all * rank / p.split, to = all * (rank + 1) / p.split, stages = to - from;
+  const int first_item = blockIdx.x / p.split, item_step = gridDim.x / p.split;
+  TileAt t;
 
   if (warp == 0) {
     Ring<S::kStages> ring;
     int it = 0;  // stages issued
     bool ok = true, waited = false;
-    TileAt t;
-    for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
       if (t.expert == p.groups.experts) continue;
       const int w_row = __shfl_sync(0xFFFFFFFFu, t.expert * p.rows + t.row_tile * kTileRows, 0);
       const int x_row = __shfl_sync(0xFFFFFFFFu, t.first, 0);
+      const bool bulk = p.scale_source == kScalesBulk;
       const uint8_t* w_scale =
           p.w_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.expert * p.groups.row_tiles + t.row_tile, 0)) * p.scale_tiles * 512;
       const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.scale_row >> 7, 0)) * p.scale_tiles * 512;
       const auto load_w = [&](int i, int s) {
         uint8_t* at = smem + s * S::kStage;
         const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
-        pm::mbar_arrive_expect_tx(&full[s], S::kW + S::kX + tiles * 512 * (1 + S::kXBlocks));
+        pm::mbar_arrive_expect_tx(&full[s], S::kW + (kFused ? 0 : S::kX) + tiles * 512 * ((bulk ? 1 : 0) + (kFused ? 0 : S::kXBlocks)));
         pm::tma_load_2d(at, &p.w_map, i * kStageBytes, w_row, &full[s]);
-        pm::bulk_g2s(at + S::kW + S::kX, w_scale + static_cast<int64_t>(i) * S::kTiles * 512, tiles * 512, &full[s]);
+        if (bulk) pm::bulk_g2s(at + S::kW + S::kX, w_scale + static_cast<int64_t>(i) * S::kTiles * 512, tiles * 512, &full[s]);
       };
       const auto load_x = [&](int i, int s) {
-        uint8_t* at = smem + s * S::kStage;
-        const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
-        pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, x_row, &full[s]);
+        if constexpr (!kFused) {
+          uint8_t* at = smem + s * S::kStage;
+          const int tiles = min(S::kTiles, p.scale_tiles - i * S::kTiles);
+          pm::tma_load_2d(at + S::kW, &p.x_map, i * kStageBytes, x_row, &full[s]);
 #pragma unroll
-        for (int b = 0; b < S::kXBlocks; ++b)
-          pm::bulk_g2s(at + S::kW + S::kX + S::kSW + b * S::kTiles * 512,
-                       x_scale + (static_cast<int64_t>(b) * p.scale_tiles + i * S::kTiles) * 512, tiles * 512, &full[s]);
+          for (int b = 0; b < S::kXBlocks; ++b)
+            pm::bulk_g2s(at + S::kW + S::kX + S::kSW + b * S::kTiles * 512,
+                         x_scale + (static_cast<int64_t>(b) * p.scale_tiles + i * S::kTiles) * 512, tiles * 512, &full[s]);
+        }
       };
       if (elect_one()) {
-        int i = 0;
+        int i = from;
         if (!waited) {
           // the first tile: the weight's part of every stage goes out before the tokens are quantized
           const int ahead = p.early ? min(stages, S::kStages) : 0;
-          for (int j = 0; j < ahead; ++j) load_w(j, j);
+          for (int j = 0; j < ahead; ++j) load_w(from + j, j);
           grid_wait();
-          for (; i < ahead; ++i, ++it, ring.next()) load_x(i, i);
+          for (int j = 0; j < ahead; ++j, ++i, ++it, ring.next()) load_x(i, j);
         }
-        for (; i < stages; ++i, ++it, ring.next()) {
+        for (; i < to; ++i, ++it, ring.next()) {
           ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
           if (!ok) break;
           load_w(i, ring.slot);
@@ -144,8 +280,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
       // the elected lane may be another one next time
       ok = __all_sync(0xFFFFFFFFu, ok);
       it = __reduce_max_sync(0xFFFFFFFFu, it);
-      ring.slot = it % S::kStages;
-      ring.round = (it / S::kStages) & 1;
+      ring.at(it);
     }
     if (!waited) grid_wait();  // no block ends before the launch it depends on
     // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
@@ -153,11 +288,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
       pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
     __syncwarp();
   } else if (warp == 1) {
-    Ring<S::kStages> ring, old;  // this stage; the one two stages ago
+    Ring<S::kStages> ring, old;  // this stage; the one kBufs stages ago
     int it = 0, n = 0;           // stages used, tiles begun
     bool ok = true;
-    TileAt t;
-    for (int id = blockIdx.x; ok && id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
       if (t.expert == p.groups.experts) continue;
       const int b = n & 1;
       const uint32_t d = tmem + b * BN;
@@ -166,9 +300,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
       if (elect_one()) {
         ok = n < 2 || pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
         pm::tc_fence_after();
-        for (int i = 0; ok && i < stages; ++i, ++it, ring.next()) {
-          // the scale buffer's last readers, two stages ago, have finished
-          if (it >= 2) {
+        int buf = it % S::kBufs;
+        for (int i = from; ok && i < to; ++i, ++it, ring.next()) {
+          if (S::kBufs < S::kStages && it >= S::kBufs) {
+            // the scale buffer's last readers have finished
             ok = pm::mbar_wait(&empty[old.slot], old.round, pm::kStatusTimeoutMma);
             old.next();
           }
@@ -176,7 +311,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
           if (!ok) break;
           pm::tc_fence_after();
           const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
-          const uint32_t sw = tmem + 2 * BN + (it & 1) * S::kScaleCols, sx = sw + S::kTiles * 4;
+          const uint32_t sw = tmem + 2 * BN + buf * S::kScaleCols, sx = sw + S::kTiles * 4;
+          if (++buf == S::kBufs) buf = 0;
           const int tiles = p.scale_tiles - i * S::kTiles, steps = p.k_steps - i * 4;
           const uint64_t ws = pm::smem_desc(at + S::kW + S::kX, 0, 128);
           const uint64_t xs = pm::smem_desc(at + S::kW + S::kX + S::kSW, 0, 128);
@@ -196,7 +332,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
             const uint32_t tile = FMT == kNV ? j : j >> 1;
             if (j < steps)
               umma_fp4<FMT>(d, a + j * 2, x + j * 2, FMT == kMX && (j & 1) ? idesc | kSecondHalf : idesc, sw + tile * 4,
-                            sx + tile * 4 * S::kXBlocks, (i | j) != 0);
+                            sx + tile * 4 * S::kXBlocks, i != from || j != 0);
           }
           pm::umma_commit(&empty[ring.slot]);
         }
@@ -207,34 +343,94 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_kernel(const __grid_
       // the elected lane may be another one next time
       ok = __all_sync(0xFFFFFFFFu, ok);
       it = __reduce_max_sync(0xFFFFFFFFu, it);
-      ring.slot = it % S::kStages;
-      ring.round = (it / S::kStages) & 1;
-      const int before = max(it - 2, 0);
-      old.slot = before % S::kStages;
-      old.round = (before / S::kStages) & 1;
+      ring.at(it);
+      old.at(max(it - S::kBufs, 0));
     }
     __syncwarp();
-  } else {
+  } else if (warp < 6) {
     const float x_second = p.x_second != nullptr ? *p.x_second : 1.0f;
     uint8_t* mine = out + (warp & 3) * 2048;
     int n = 0;
-    TileAt t;
-    for (int id = blockIdx.x; id < p.items && find_tile(p.groups, id, BN, t); id += gridDim.x) {
+    for (int id = first_item; id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
       if (t.expert == p.groups.experts) {
-        store_zeros<DT>(p.y, t, p.rows, threadIdx.x - 64, 128);
+        if (rank == 0) store_zeros<DT>(p.y, t, p.rows, threadIdx.x - 64, 128);
         continue;
       }
       const int b = n & 1;
-      const float alpha = (p.w_second != nullptr ? p.w_second[t.expert] : 1.0f) * x_second;
       const bool ok = pm::mbar_wait(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       pm::tc_fence_after();
+      if (S::kCanSplit && p.split > 1) {
+        // one tile per cluster; its products are done, so the stages are free
+        store_sums(tmem + b * BN, t, reinterpret_cast<float*>(smem));
+        break;
+      }
+      const float alpha = (p.w_second != nullptr ? p.w_second[t.expert] : 1.0f) * x_second;
       store_tile<DT>(tmem + b * BN, p.y, t, p.rows, alpha, 0, BN, mine, p.vec != 0);
       pm::tc_fence_before();
       __syncwarp();
       if (lane == 0) pm::mbar_arrive(&acc_empty[b]);
       ++n;
     }
+  } else if (warp == 6) {
+    if (p.scale_source != kScalesBulk) {
+      Ring<S::kStages> ring;
+      int it = 0;
+      bool ok = true;
+      for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+        if (t.expert == p.groups.experts) continue;
+        ScaleWords<FMT> ahead[2];  // loads in flight
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ahead[j] = load_scale_words<FMT>(p, t, min(from + j, to - 1), lane);
+        for (int i = from; i < to; ++i, ++it, ring.next()) {
+          const ScaleWords<FMT> now = ahead[0];
+          ahead[0] = ahead[1];
+          if (i + 2 < to) ahead[1] = load_scale_words<FMT>(p, t, i + 2, lane);
+          ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          uint8_t* at = smem + ring.slot * S::kStage + S::kW + S::kX + lane * 16;
+#pragma unroll
+          for (int k = 0; k < S::kTiles; ++k)
+            *reinterpret_cast<uint4*>(at + k * 512) = make_uint4(now.w[0][k], now.w[1][k], now.w[2][k], now.w[3][k]);
+          pm::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) pm::mbar_arrive(&full[ring.slot]);
+        }
+      }
+    }
+  } else if constexpr (kFused) {
+    const bool two = FMT == kNV && p.x_second != nullptr;
+    const float g = two ? *p.x_second : 1.0f, inv_g = __fdiv_rn(1.0f, g);
+    Ring<S::kStages> ring;
+    int it = 0;
+    bool ok = true;
+    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+      if (t.expert == p.groups.experts) continue;
+      for (int i = from; i < to; ++i, ++it, ring.next()) {
+        if (it % kQuantWarps != warp - 7) continue;  // every warp takes its share of the stages
+        ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        uint8_t* at = smem + ring.slot * S::kStage;
+        quantize_stage<DT, FMT>(p, t, i, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
+        pm::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) pm::mbar_arrive(&full[ring.slot]);
+      }
+    }
+  }
+
+  if (S::kCanSplit && p.split > 1) {
+    __syncwarp();
+    cluster_sync();  // every block's sums are written
+    if (find_tile(p.groups, first_item, BN, t) && t.expert != p.groups.experts) {
+      float alpha = p.w_second != nullptr ? p.w_second[t.expert] : 1.0f;
+      if (p.x_second != nullptr) alpha *= *p.x_second;
+      add_cluster_sums<DT>(reinterpret_cast<const float*>(smem), p.y, t, p.rows, alpha, rank, p.split, S::kThreads, p.vec != 0);
+    }
+    __syncwarp();
+    cluster_sync();  // nobody's shared memory goes while others read it
   }
   __syncthreads();
   if (warp == 1) {

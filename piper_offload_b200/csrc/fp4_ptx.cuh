@@ -104,7 +104,36 @@ struct Ring {
       round ^= 1u;
     }
   }
+  // The place of running count `it`.
+  __device__ __forceinline__ void at(int it) {
+    slot = it % N;
+    round = (it / N) & 1;
+  }
 };
+
+// ---------------------------------------------------------------- clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Every thread of every block of the cluster; what was written before is seen after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The four fp32 values at this block's shared-memory address `saddr` in block `rank`.
+__device__ __forceinline__ float4 load_cluster(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
+}
 
 // Programmatic launches: let the next kernel start its own set-up / wait for
 // everything the previous one wrote.

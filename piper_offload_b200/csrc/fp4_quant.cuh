@@ -536,60 +536,30 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
   }
 }
 
-// ------------------------------------------- weights in the product's layout
-// The product reads codes in rows of whole 16-byte pieces and scales in the
-// swizzled layout with zeroed padding. Weights stored otherwise are laid out
-// by this kernel first: row-major scales, columns that are no multiple of 64
-// (padding inside a tile that is used), or unaligned buffers.
+// The product's copies read codes in rows of whole 16-byte pieces. A weight
+// with columns that are no multiple of 32, or that starts elsewhere, is laid
+// out so first.
 struct RepackArgs {
   const uint8_t* codes;
-  uint8_t* codes_out;   // NULL: the codes are used where they are
-  int64_t code_row;     // bytes of a row
-  int64_t code_pitch;   // bytes between rows of codes_out (a multiple of 16)
-  const uint8_t* scale;
-  uint8_t* scale_out;   // NULL: the scales are used where they are
-  int64_t rows, batch;
-  int32_t scale_cols;   // scales per row
-  int32_t swizzled;     // layout of `scale`
-  int64_t words;        // 4-byte words of scale_out
-  int64_t pieces;       // 16-byte pieces of codes_out
+  uint8_t* codes_out;  // NULL: the codes are used where they are
+  int64_t row_bytes;
+  int64_t pitch;       // bytes between rows of codes_out (a multiple of 16)
+  int64_t pieces;      // 16-byte pieces of codes_out
 };
 
 __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
-  const int64_t ct = (p.scale_cols + 3) >> 2, rt = (p.rows + 127) >> 7;
-  if (i < p.words) {
-    const int grp = static_cast<int>(i & 3), lane = static_cast<int>((i >> 2) & 31);
-    const int64_t tile = i >> 7;
-    const int64_t tc = tile % ct, tr = (tile / ct) % rt, e = tile / (ct * rt);
-    const int64_t row = tr * 128 + grp * 32 + lane;
-    uint32_t w = 0u;
-    if (row < p.rows) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = static_cast<int>(tc) * 4 + j;
-        if (c < p.scale_cols) {
-          const uint8_t* s = p.swizzled ? p.scale + e * rt * ct * 512 + swizzled_byte(row, c, static_cast<int>(ct))
-                                        : p.scale + (e * p.rows + row) * p.scale_cols + c;
-          w |= static_cast<uint32_t>(*s) << (8 * j);
-        }
-      }
-    }
-    reinterpret_cast<uint32_t*>(p.scale_out)[i] = w;
-    return;
-  }
-  i -= p.words;
   if (i >= p.pieces) return;
-  const int64_t per = p.code_pitch >> 4;
+  const int64_t per = p.pitch >> 4;
   const int64_t row = i / per, at = (i - row * per) * 16;
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    if (at + j < p.code_row) w[j >> 2] |= static_cast<uint32_t>(p.codes[row * p.code_row + at + j]) << (8 * (j & 3));
-  *reinterpret_cast<uint4*>(p.codes_out + row * p.code_pitch + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (at + j < p.row_bytes) w[j >> 2] |= static_cast<uint32_t>(p.codes[row * p.row_bytes + at + j]) << (8 * (j & 3));
+  *reinterpret_cast<uint4*>(p.codes_out + row * p.pitch + at) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // What a product needs ahead of it, in one launch: blocks below
-// `token_blocks` quantize tokens, the others lay weights out.
+// `token_blocks` quantize tokens, the others lay codes out.
 template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads)
     prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t token_blocks) {

@@ -92,6 +92,64 @@ __device__ __forceinline__ void store_zeros(void* y, const TileAt& t, int cols, 
       store_value<DT>(y, static_cast<int64_t>(t.first + i / kTileRows) * cols + c0 + (i & (kTileRows - 1)), 0.0f);
 }
 
+// Four warps leave a tile's sums in shared memory as (token, 128 outputs).
+__device__ __forceinline__ void store_sums(uint32_t tmem, const TileAt& t, float* sums) {
+  const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  for (int c = 0; c < t.count; c += 32) {
+    float v[32];
+    pm::tmem_ld32(at + c, v);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c + j < t.count) sums[(c + j) * kTileRows + quarter * 32 + lane] = v[j];
+  }
+}
+
+// A block adds up its share of a tile over the cluster, in rank order: four
+// outputs of a token a thread, the ranks' values all in flight at once.
+template <int DT>
+__device__ __forceinline__ void add_cluster_sums(const float* sums, void* y, const TileAt& t, int cols, float alpha, int rank,
+                                                 int split, int threads, bool vec) {
+  const uint32_t base = pm::smem_u32(sums);
+  const int n0 = t.row_tile * kTileRows;
+  for (int i = rank * threads + threadIdx.x; i < t.count * (kTileRows / 4); i += split * threads) {
+    const int n = n0 + (i % (kTileRows / 4)) * 4;
+    if (n >= cols) continue;
+    float4 v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < split) v[r] = load_cluster(base + i * 16, r);
+    float4 sum = v[0];
+#pragma unroll
+    for (int r = 1; r < 8; ++r)
+      if (r < split) {
+        sum.x += v[r].x;
+        sum.y += v[r].y;
+        sum.z += v[r].z;
+        sum.w += v[r].w;
+      }
+    sum.x *= alpha;
+    sum.y *= alpha;
+    sum.z *= alpha;
+    sum.w *= alpha;
+    const int64_t at = static_cast<int64_t>(t.first + i / (kTileRows / 4)) * cols + n;
+    if (vec) {  // rows are 16-byte aligned, so the four outputs exist and lie together
+      if constexpr (DT == kBF16) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(y) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else {
+        *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = sum;
+      }
+    } else {
+      const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < cols) store_value<DT>(y, at + k, f[k]);
+    }
+  }
+}
+
 // Four epilogue warps' share of a finished tile: tensor-memory lane = column of
 // y, tensor-memory column = token, so that a warp's 32 lanes are neighbours in
 // y's rows. bf16: 32 tokens at a time are read as the fragments of 8x8

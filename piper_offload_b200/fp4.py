@@ -119,10 +119,14 @@ class _on:
             self.guard.__exit__(*exc)
 
 
-def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor:
+def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor | None:
     need = ctypes.c_size_t(0)
     nat.check(query(*args, ctypes.byref(need)))
-    return torch.empty(need.value, dtype=torch.uint8, device=device)
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def _span(workspace: torch.Tensor | None) -> tuple[int | None, int]:
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -244,7 +248,7 @@ def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: 
     with _on(device):
         nat.check(lib.piper_fp4_linear(
             ref, x2.data_ptr(), x2.stride(0), tokens, None if ends is None else ends.data_ptr(),
-            None if act_scale is None else act_scale.data_ptr(), mode, y.data_ptr(), dt, ws.data_ptr(), ws.numel(),
+            None if act_scale is None else act_scale.data_ptr(), mode, y.data_ptr(), dt, *_span(ws),
             nat.current_stream_handle(device)))
     return y
 
@@ -268,7 +272,7 @@ def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> t
     with _on(device):
         nat.check(lib.piper_fp4_grad_input(
             ref, g2.data_ptr(), g2.stride(0), tokens, None if ends is None else ends.data_ptr(), dx.data_ptr(), dt,
-            ws.data_ptr(), ws.numel(), nat.current_stream_handle(device)))
+            *_span(ws), nat.current_stream_handle(device)))
     return dx
 
 

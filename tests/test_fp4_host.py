@@ -80,9 +80,9 @@ def test_bad_arguments_are_refused():
                       ({"tokens": 1 << 40}, "tokens"), ({"mode": 4}, "scaling mode"), ({"dtype": 1}, "bfloat16 and float32")):
         with pytest.raises(ValueError, match=match):
             nat.check(linear(**kw))
-    for kw in ({"ws": None}, {"ws": 0x100010}, {"bytes": 64}):
+    for kw in ({"ws": None}, {"ws": 0x100010}, {"bytes": 64}):  # many tokens are quantized into it
         with pytest.raises(RuntimeError, match="workspace"):
-            nat.check(linear(**kw))
+            nat.check(linear(tokens=800, **kw))
     assert linear(tokens=0, x=None, y=None) == nat.OK
 
     several = matrix(batch=3)
