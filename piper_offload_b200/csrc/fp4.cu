@@ -147,8 +147,8 @@ struct LinearPlan {
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = tokens / w.batch;
-  p.fused = per_expert <= 32;
-  p.bn = p.fused ? 32 : per_expert <= 512 ? 128 : 192;
+  p.fused = per_expert <= 8;
+  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 192;
   const int tile = block_of(w) * 4;
   p.scale_tiles = (w.cols + tile - 1) / tile;
   p.k_padded = p.scale_tiles * tile;
@@ -179,16 +179,21 @@ int64_t token_tiles(const fp4::Groups& g, int bn) {
   return g.ends == nullptr ? (g.tokens + bn - 1) / bn : g.tokens / bn + std::min<int64_t>(g.experts + 1, g.tokens);
 }
 
-// Blocks of a cluster that share a tile's K: as many as keep the SMs busy in
-// one wave, at least two stages for each. 4096 x 14336, one token (32 tiles):
-// TODO us with 8, TODO with 1.
+// Blocks of a cluster that share a tile's K: where the tiles leave SMs idle, as
+// many as shorten the run by a rough account in cycles (a stage takes about
+// 450; leaving and adding up sums 2500 and 30 for each token of the tile).
 template <class S>
-int split_of(int64_t items, int stages) {
-  int split = 1;
-  while (S::kCanSplit && split < fp4::kMaxSplit && items * split * 2 <= static_cast<int64_t>(sm_count()) * S::kCtas &&
-         stages >= split * 4)
-    split *= 2;
-  return split;
+int split_of(int64_t items, int stages, int tokens) {
+  int best = 1;
+  double least = 450.0 * stages;
+  for (int split = 2; S::kCanSplit && split <= fp4::kMaxSplit && items * split <= sm_count() && stages >= 2 * split; split *= 2) {
+    const double cycles = 450.0 * ((stages + split - 1) / split) + 2500.0 + 30.0 * tokens;
+    if (cycles < least) {
+      least = cycles;
+      best = split;
+    }
+  }
+  return best;
 }
 
 template <int DT, int FMT, int BN, bool kFused>
@@ -197,7 +202,7 @@ cudaError_t launch_linear(fp4::LinearArgs& args, int64_t items, cudaStream_t str
   auto kernel = fp4::linear_kernel<DT, FMT, BN, kFused>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  args.split = split_of<S>(items, (args.k_steps + 3) / 4);
+  args.split = split_of<S>(items, (args.k_steps + 3) / 4, static_cast<int>(std::min<int64_t>(args.groups.tokens, BN)));
   cudaLaunchAttribute attributes[2] = {};
   // may start while the launch before it still quantizes; the kernel waits where it needs that
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -207,7 +212,7 @@ cudaError_t launch_linear(fp4::LinearArgs& args, int64_t items, cudaStream_t str
   attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(
-      args.split > 1 ? items * args.split : std::min<int64_t>(items, static_cast<int64_t>(sm_count()) * S::kCtas)));
+      args.split > 1 ? items * args.split : std::min<int64_t>(items, sm_count())));
   config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
@@ -447,6 +452,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   }
 #define CALL(D, F)                                                    \
   e = p.fused ? launch_linear<D, F, 32, true>(a, items, s)            \
+      : p.bn == 32 ? launch_linear<D, F, 32, false>(a, items, s)      \
               : p.bn == 128 ? launch_linear<D, F, 128, false>(a, items, s) : launch_linear<D, F, 192, false>(a, items, s)
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL

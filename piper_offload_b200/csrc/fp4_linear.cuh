@@ -11,9 +11,9 @@
 // is that of the output.
 //
 // Many tokens: their codes and scales are made by a launch before (prepare_kernel),
-// tiles are 128 or 192 tokens wide. Few tokens (kFused, tiles of 32): the kernel
-// is a stream of weight bytes, so four warps quantize each stage's tokens on
-// the way and there is no launch before. Where there are too few tiles for the
+// tiles are 32, 128 or 192 tokens wide. A handful (kFused): the kernel is a
+// stream of weight bytes, so eight warps quantize the tokens on the way, each
+// every eighth stage, and there is no launch before. Where there are too few tiles for the
 // SMs, a cluster of blocks splits K; each leaves its sums in its own shared
 // memory and every block adds up its share of the tokens over the cluster, in
 // rank order, so that results do not depend on timing.
@@ -28,7 +28,7 @@ namespace fp4 {
 
 constexpr int kStageCols = 256;      // K values per stage
 constexpr int kStageBytes = kStageCols / 2;
-constexpr int kQuantWarps = 4;       // kFused
+constexpr int kQuantWarps = 8;       // kFused
 constexpr int kMaxSplit = 8;
 
 // Where the weight's scales come from: whole swizzled tiles by bulk copies, or
@@ -70,18 +70,17 @@ struct LinearShape {
   static constexpr int kSX = kXBlocks * kTiles * 512;
   static constexpr int kStage = kW + kX + kSW + kSX;
   static constexpr int kOut = 4 * 2048;                             // 32 tokens x 32 outputs of each epilogue warp
-  static constexpr int kCtas = kFused ? 2 : 1;                      // resident per SM
-  static constexpr int kRoom = kSmemMax / kCtas - 2048 - kOut;
+  static constexpr int kRoom = kSmemMax - 2048 - kOut;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + 1024 + 512;
   static constexpr int kThreads = 224 + (kFused ? 32 * kQuantWarps : 0);
   static constexpr bool kCanSplit = BN * kTileRows * 4 <= kStages * kStage;
   // tensor memory: two accumulators, then buffers of scales, one per stage if they fit
   static constexpr int kScaleCols = kTiles * 4 * (1 + kXBlocks);
-  static constexpr int kBufs = (512 / kCtas - 2 * BN) / kScaleCols < kStages ? (512 / kCtas - 2 * BN) / kScaleCols : kStages;
+  static constexpr int kBufs = (512 - 2 * BN) / kScaleCols < kStages ? (512 - 2 * BN) / kScaleCols : kStages;
   static constexpr int kCols = 2 * BN + kBufs * kScaleCols;
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-  static_assert(kCols <= 512 && kAlloc * kCtas <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
+  static_assert(kCols <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
 };
 
 // The scales that one stage needs of the weight: 128 rows x kTiles words, four rows a lane.
@@ -148,39 +147,48 @@ __device__ __forceinline__ ScaleWords<FMT> load_scale_words(const LinearArgs& p,
   return s;
 }
 
-// A warp quantizes a stage's tokens into the operand's swizzled rows and its
-// scale tiles: half a warp a row, eight (fp32: four) rows in flight.
-template <int DT, int FMT>
-__device__ __forceinline__ void quantize_stage(const LinearArgs& p, const TileAt& t, int stage, uint8_t* codes, uint8_t* scales,
-                                               bool two, float g, float inv_g) {
-  constexpr int kDeep = DT == kBF16 ? 4 : 2;
-  const int lane = threadIdx.x & 31, unit = lane & 15;
-  const int col = stage * kStageCols + unit * kUnit;
-  for (int r0 = 0; r0 < t.count; r0 += 2 * kDeep) {
-    Raw<DT> raw[kDeep];
+// Eight tokens of a stage, as a warp holds them: half a warp a row.
+template <int DT>
+struct TokenBlock {
+  Raw<DT> raw[4];
+};
+
+template <int DT>
+__device__ __forceinline__ TokenBlock<DT> load_tokens(const LinearArgs& p, const TileAt& t, int stage, int row0) {
+  const int lane = threadIdx.x & 31;
+  const int col = stage * kStageCols + (lane & 15) * kUnit;
+  TokenBlock<DT> b;
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      const int r = r0 + 2 * u + (lane >> 4);
-      if (r < t.count && col < p.cols) {
-        raw[u] = load_unit<DT>(p.x, (t.first + r) * p.x_stride + col, p.x_vec != 0);
-      } else {
+  for (int u = 0; u < 4; ++u) {
+    const int r = row0 + 2 * u + (lane >> 4);
+    if (r < t.count && col < p.cols) {
+      b.raw[u] = load_unit<DT>(p.x, (t.first + r) * p.x_stride + col, p.x_vec != 0);
+    } else {
 #pragma unroll
-        for (auto& w : raw[u].w) w = 0u;
-      }
+      for (auto& w : b.raw[u].w) w = 0u;
     }
+  }
+  return b;
+}
+
+// A warp quantizes them into the operand's swizzled rows and its scale tiles.
+template <int DT, int FMT>
+__device__ __forceinline__ void quantize_tokens(const LinearArgs& p, const TileAt& t, const TokenBlock<DT>& b, int stage, int row0,
+                                                uint8_t* codes, uint8_t* scales, bool two, float g, float inv_g) {
+  const int lane = threadIdx.x & 31, unit = lane & 15;
+  const bool in_cols = stage * kStageCols + unit * kUnit < p.cols;
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u) {
-      if (r0 + 2 * u >= t.count) break;  // the same in all lanes
-      const int r = r0 + 2 * u + (lane >> 4);
-      float v[16];
-      to_floats(raw[u], v);
-      const Coded c = quantize16<FMT>(v, p.scale_mode, two, g, inv_g);
-      const uint32_t word = gather_scales<FMT>(col < p.cols ? c.byte : 0u);
-      if (r < t.count) {
-        *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
-        constexpr int kLanes = FMT == kNV ? 4 : 8;  // units per scale tile
-        if (unit % kLanes == 0) *reinterpret_cast<uint32_t*>(scales + (unit / kLanes) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
-      }
+  for (int u = 0; u < 4; ++u) {
+    if (row0 + 2 * u >= t.count) break;  // the same in all lanes
+    const int r = row0 + 2 * u + (lane >> 4);
+    float v[16];
+    to_floats(b.raw[u], v);
+    const Coded c = quantize16<FMT>(v, p.scale_mode, two, g, inv_g);
+    const uint32_t word = gather_scales<FMT>(in_cols ? c.byte : 0u);
+    if (r < t.count) {
+      *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
+      constexpr int kLanes = FMT == kNV ? 4 : 8;  // units per scale tile
+      if (unit % kLanes == 0) *reinterpret_cast<uint32_t*>(scales + (unit / kLanes) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
     }
   }
 }
@@ -189,7 +197,7 @@ __device__ __forceinline__ void quantize_stage(const LinearArgs& p, const TileAt
 // producers and the tensor-core warp are up to two accumulators ahead of the
 // epilogue.
 template <int DT, int FMT, int BN, bool kFused>
-__global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, LinearShape<FMT, BN, kFused>::kCtas)
+__global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
     linear_kernel(const __grid_constant__ LinearArgs p) {
   using S = LinearShape<FMT, BN, kFused>;
   extern __shared__ uint8_t raw[];
@@ -407,17 +415,26 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, Linear
     bool ok = true;
     for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
       if (t.expert == p.groups.experts) continue;
-      for (int i = from; i < to; ++i, ++it, ring.next()) {
-        if (it % kQuantWarps != warp - 7) continue;  // every warp takes its share of the stages
-        ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+      const int mine = warp - 7;
+      int i = from + ((mine - it) & (kQuantWarps - 1));  // every eighth stage is this warp's
+      TokenBlock<DT> next;
+      if (i < to) next = load_tokens<DT>(p, t, i, 0);
+      for (; i < to; i += kQuantWarps) {
+        const TokenBlock<DT> now = next;
+        if (i + kQuantWarps < to) next = load_tokens<DT>(p, t, i + kQuantWarps, 0);
+        ring.at(it + (i - from));
+        ok = it + (i - from) < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         uint8_t* at = smem + ring.slot * S::kStage;
-        quantize_stage<DT, FMT>(p, t, i, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
+        quantize_tokens<DT, FMT>(p, t, now, i, 0, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
+        for (int r0 = 8; r0 < t.count; r0 += 8)
+          quantize_tokens<DT, FMT>(p, t, load_tokens<DT>(p, t, i, r0), i, r0, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
         pm::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) pm::mbar_arrive(&full[ring.slot]);
       }
+      it += stages;
     }
   }
 

@@ -278,6 +278,24 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
       for (auto& w : raw[u].w) w = 0u;
     }
   }
+  // the warp's rows' experts, one row a lane, while the values are on their way
+  int64_t place = 0;
+  if (q.token_tile != 0) {
+    const int64_t r = row0 + lane;
+    int x = 0;
+    int64_t start = 0;
+    if (q.ends != nullptr && lane < kQuantRows * step && r < q.rows) {
+      x = expert_of_row(q.ends, q.experts, r);
+      start = x > 0 ? q.ends[x - 1] : 0;
+    }
+    if (q.ends != nullptr && (x >= q.experts || start < 0 || start > r)) {
+      place = -1;  // a row of no expert
+    } else {
+      const int o = static_cast<int>(r - start);
+      place = first_scale_row(start, x, q.token_tile) +
+              static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
+    }
+  }
   const bool two = FMT == kNV && q.second_mode != kSecondNone;
   const int c = unit / kLanes;
 #pragma unroll
@@ -289,21 +307,8 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
     const bool live = r < q.rows;
     const uint32_t byte = live && in_cols ? s.byte : 0u;
     const uint32_t word = gather_scales<FMT>(byte);
-    if (!in_row || r >= q.rows_padded) continue;
-
-    int64_t srow = r;
-    if (q.token_tile != 0) {
-      int x = 0;
-      int64_t start = 0;
-      if (q.ends != nullptr) {
-        x = expert_of_row(q.ends, q.experts, r);
-        start = x > 0 ? q.ends[x - 1] : 0;
-        if (x >= q.experts || start < 0 || start > r) continue;  // a row of no expert
-      }
-      const int o = static_cast<int>(r - start);
-      srow = first_scale_row(start, x, q.token_tile) +
-             static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
-    }
+    const int64_t srow = q.token_tile != 0 ? __shfl_sync(0xFFFFFFFFu, place, u * step + lane / per) : r;
+    if (!in_row || r >= q.rows_padded || srow < 0) continue;
     uint8_t* at = q.swizzled ? q.scale + e * (q.rows_padded >> 7) * q.scale_cols * 512 + swizzled_byte(srow, c, q.scale_cols)
                              : q.scale + (e * q.rows + r) * q.scale_cols + c;
     if (q.words) {
