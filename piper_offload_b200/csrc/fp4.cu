@@ -117,6 +117,12 @@ int scale_cols(const piper_fp4_matrix& m) {
   return static_cast<int>(m.swizzled ? (blocks + 3) / 4 : blocks);
 }
 
+// Rows that a lane quantizes: several, whose loads are in flight together, once there are blocks for every SM;
+// before that one, as a lane's rows come one after another (777 x 1072: TODO us with 1, TODO with 4).
+int rows_per_lane(const fp4::QuantArgs& q) {
+  return fp4::quant_blocks(q, fp4::kQuantRows) < 2 * sm_count() ? 1 : fp4::kQuantRows;
+}
+
 // Matrices of at most so many values get their second-level scale and their codes in one launch of one block
 // each: 70 x 208 in 5 us instead of 10 in three launches, 256 x 256 in 10 instead of 10.
 constexpr int64_t kSmallMatrix = 65536;
@@ -301,15 +307,18 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
     }
     cudaError_t e = cudaMemsetAsync(maxima, 0, sizeof(uint32_t) * m->batch, s);
     if (e != cudaSuccess) return cuda_fail("cudaMemsetAsync", e);
-    const int64_t blocks = fp4::quant_row_blocks(q) * ((q.units + 31) / 32);
+    const int64_t blocks = fp4::quant_row_blocks(q, fp4::kQuantRows) * ((q.units + 31) / 32);
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 8)), static_cast<unsigned>(m->batch));
     if (dtype == PIPER_FP4_BF16) fp4::amax_kernel<fp4::kBF16><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     else fp4::amax_kernel<fp4::kF32><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     if ((e = launched()) != cudaSuccess) return cuda_fail("amax kernel", e);
   }
-  const int64_t blocks = fp4::quant_blocks(q);
+  const int lane_rows = rows_per_lane(q);
+  const int64_t blocks = fp4::quant_blocks(q, lane_rows);
   FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 quantisation: too many values for one call.");
-#define CALL(D, F) fp4::quantize_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q)
+#define CALL(D, F)                                                                                                \
+  if (lane_rows == 1) fp4::quantize_kernel<D, F, 1><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q); \
+  else fp4::quantize_kernel<D, F, fp4::kQuantRows><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q)
   FP4_DISPATCH(dtype, m->format, CALL);
 #undef CALL
   const cudaError_t e = launched();
@@ -404,6 +413,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
 
   fp4::QuantArgs q{};
   int64_t token_blocks = 0;
+  int lane_rows = 1;
   if (!p.fused) {
     q.x = x;
     q.x_stride = x_stride;
@@ -423,7 +433,8 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     q.token_tile = p.bn;
     q.ends = ends;
     q.experts = static_cast<int32_t>(w->batch);
-    token_blocks = fp4::quant_blocks(q);
+    lane_rows = rows_per_lane(q);
+    token_blocks = fp4::quant_blocks(q, lane_rows);
   }
   a.x_scale = q.scale;
   fp4::RepackArgs r{};
@@ -443,8 +454,10 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
 
   cudaError_t e = cudaSuccess;
   if (blocks > 0) {
-#define CALL(D, F) \
-  fp4::prepare_kernel<D, F><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q, r, static_cast<uint32_t>(token_blocks))
+    auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
+#define CALL(D, F)                                                                                            \
+  if (lane_rows == 1) fp4::prepare_kernel<D, F, 1><<<grid, fp4::kQuantThreads, 0, s>>>(q, r, tokens_grid);     \
+  else fp4::prepare_kernel<D, F, fp4::kQuantRows><<<grid, fp4::kQuantThreads, 0, s>>>(q, r, tokens_grid)
     FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
     e = launched();

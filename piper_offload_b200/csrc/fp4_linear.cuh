@@ -73,12 +73,17 @@ struct LinearShape {
   static constexpr int kRoom = kSmemMax - 2048 - kOut;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + 1024 + 512;
-  static constexpr int kThreads = 224 + (kFused ? 32 * kQuantWarps : 0);
+  
   static constexpr bool kCanSplit = BN * kTileRows * 4 <= kStages * kStage;
   // tensor memory: two accumulators, then buffers of scales, one per stage if they fit
   static constexpr int kScaleCols = kTiles * 4 * (1 + kXBlocks);
   static constexpr int kBufs = (512 - 2 * BN) / kScaleCols < kStages ? (512 - 2 * BN) / kScaleCols : kStages;
   static constexpr int kCols = 2 * BN + kBufs * kScaleCols;
+  // with fewer buffers than stages the copies of scales wait for products, and get a warp of their own: 4096 tokens x
+  // 14336 x 4096 NVFP4 136 us against 145; with a buffer per stage one warp does both, 6 to 10 % faster on small calls
+  static constexpr bool kCopyWarp = kBufs < kStages;
+  static constexpr int kFirstQuantWarp = kCopyWarp ? 8 : 7;
+  static constexpr int kThreads = 32 * kFirstQuantWarp + (kFused ? 32 * kQuantWarps : 0);
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
 };
@@ -205,24 +210,43 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
   uint8_t* out = smem + S::kStages * S::kStage;
   uint64_t* full = reinterpret_cast<uint64_t*>(out + S::kOut);
   uint64_t* empty = full + S::kStages;
-  uint64_t* acc_full = empty + S::kStages;
+  uint64_t* scales_in = empty + S::kStages;  // a buffer of scales is in tensor memory
+  uint64_t* acc_full = scales_in + S::kBufs;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (warp == 0 && lane == 0) {
-    pm::prefetch_tmap(&p.w_map);
-    if (!kFused) pm::prefetch_tmap(&p.x_map);
+  warm_arguments(p);
+  // this block's part of every tile's stages
+  const int all = (p.k_steps + 3) / 4;
+  const int rank = p.split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int from = p.split > 1 ? all * rank / p.split : 0, to = p.split > 1 ? all * (rank + 1) / p.split : all, stages = to - from;
+  const int first_item = p.split > 1 ? blockIdx.x / p.split : blockIdx.x, item_step = p.split > 1 ? gridDim.x / p.split : gridDim.x;
+  const bool bulk = p.scale_source == kScalesBulk;
+  // every warp finds the first tile, and has its first loads under way, while the barriers and tensor memory are set up
+  TileAt t;
+  bool have = first_item < p.items && find_tile(p.groups, first_item, BN, t);
+  const auto next_tile = [&](int& id) {
+    id += item_step;
+    return id < p.items && find_tile(p.groups, id, BN, t);
+  };
+  TokenBlock<DT> first_tokens;  // kFused: of this quantising warp's first stage
+  if constexpr (kFused)
+    if (warp >= S::kFirstQuantWarp && have && t.expert != p.groups.experts && from + warp - S::kFirstQuantWarp < to)
+      first_tokens = load_tokens<DT>(p, t, from + warp - S::kFirstQuantWarp, 0);
+  if (warp == 0 && elect_one()) {
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1 + (p.scale_source != kScalesBulk) + kFused);
       pm::mbar_init(&empty[s], 1);
     }
+    for (int b = 0; b < S::kBufs; ++b) pm::mbar_init(&scales_in[b], 1);
     for (int b = 0; b < 2; ++b) {
       pm::mbar_init(&acc_full[b], 1);
       pm::mbar_init(&acc_empty[b], 4);
     }
     pm::fence_mbar_init();
-  } else if (warp == 1) {
+  }
+  if (warp == 1) {
     pm::tmem_alloc(tmem_at, S::kAlloc);
     pm::tmem_relinquish();
   }
@@ -230,22 +254,32 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
   __syncthreads();
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
-  // this block's part of every tile's stages
-  const int all = (p.k_steps + 3) / 4;
-  const int rank = p.split > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int from = all * rank / p.split, to = all * (rank + 1) / p.split, stages = to - from;
-  const int first_item = blockIdx.x / p.split, item_step = gridDim.x / p.split;
-  TileAt t;
+  // the scales of stage i from shared to tensor memory
+  const auto copy_scales = [&](int i, int slot, int buf) {
+    const uint32_t at = pm::smem_u32(smem) + slot * S::kStage;
+    const uint32_t sw = tmem + 2 * BN + buf * S::kScaleCols, sx = sw + S::kTiles * 4;
+    const int tiles = p.scale_tiles - i * S::kTiles;
+    const uint64_t ws = pm::smem_desc(at + S::kW + S::kX, 0, 128);
+    const uint64_t xs = pm::smem_desc(at + S::kW + S::kX + S::kSW, 0, 128);
+#pragma unroll
+    for (int j = 0; j < S::kTiles; ++j) {
+      if (j < tiles) {
+        tmem_cp_scales(sw + j * 4, ws + j * (512 >> 4));
+#pragma unroll
+        for (int k = 0; k < S::kXBlocks; ++k)
+          tmem_cp_scales(sx + (j * S::kXBlocks + k) * 4, xs + (k * S::kTiles + j) * (512 >> 4));
+      }
+    }
+  };
 
   if (warp == 0) {
     Ring<S::kStages> ring;
     int it = 0;  // stages issued
     bool ok = true, waited = false;
-    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+    for (int id = first_item; ok && have; have = next_tile(id)) {
       if (t.expert == p.groups.experts) continue;
       const int w_row = __shfl_sync(0xFFFFFFFFu, t.expert * p.rows + t.row_tile * kTileRows, 0);
       const int x_row = __shfl_sync(0xFFFFFFFFu, t.first, 0);
-      const bool bulk = p.scale_source == kScalesBulk;
       const uint8_t* w_scale =
           p.w_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.expert * p.groups.row_tiles + t.row_tile, 0)) * p.scale_tiles * 512;
       const uint8_t* x_scale = p.x_scale + static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, t.scale_row >> 7, 0)) * p.scale_tiles * 512;
@@ -296,10 +330,11 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
       pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
     __syncwarp();
   } else if (warp == 1) {
-    Ring<S::kStages> ring, old;  // this stage; the one kBufs stages ago
-    int it = 0, n = 0;           // stages used, tiles begun
+    Ring<S::kStages> ring;
+    Ring<S::kBufs> buf;
+    int it = 0, n = 0;  // stages used, tiles begun
     bool ok = true;
-    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+    for (int id = first_item; ok && have; have = next_tile(id)) {
       if (t.expert == p.groups.experts) continue;
       const int b = n & 1;
       const uint32_t d = tmem + b * BN;
@@ -308,31 +343,15 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
       if (elect_one()) {
         ok = n < 2 || pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
         pm::tc_fence_after();
-        int buf = it % S::kBufs;
-        for (int i = from; ok && i < to; ++i, ++it, ring.next()) {
-          if (S::kBufs < S::kStages && it >= S::kBufs) {
-            // the scale buffer's last readers have finished
-            ok = pm::mbar_wait(&empty[old.slot], old.round, pm::kStatusTimeoutMma);
-            old.next();
-          }
-          ok = ok && pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+        for (int i = from; ok && i < to; ++i, ++it, ring.next(), buf.next()) {
+          ok = pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+          if (S::kCopyWarp) ok = ok && pm::mbar_wait(&scales_in[buf.slot], buf.round, pm::kStatusTimeoutMma);
           if (!ok) break;
           pm::tc_fence_after();
+          if (!S::kCopyWarp) copy_scales(i, ring.slot, buf.slot);
           const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
-          const uint32_t sw = tmem + 2 * BN + buf * S::kScaleCols, sx = sw + S::kTiles * 4;
-          if (++buf == S::kBufs) buf = 0;
-          const int tiles = p.scale_tiles - i * S::kTiles, steps = p.k_steps - i * 4;
-          const uint64_t ws = pm::smem_desc(at + S::kW + S::kX, 0, 128);
-          const uint64_t xs = pm::smem_desc(at + S::kW + S::kX + S::kSW, 0, 128);
-#pragma unroll
-          for (int j = 0; j < S::kTiles; ++j) {
-            if (j < tiles) {
-              tmem_cp_scales(sw + j * 4, ws + j * (512 >> 4));
-#pragma unroll
-              for (int k = 0; k < S::kXBlocks; ++k)
-                tmem_cp_scales(sx + (j * S::kXBlocks + k) * 4, xs + (k * S::kTiles + j) * (512 >> 4));
-            }
-          }
+          const uint32_t sw = tmem + 2 * BN + buf.slot * S::kScaleCols, sx = sw + S::kTiles * 4;
+          const int steps = p.k_steps - i * 4;
           const uint64_t a = pm::smem_desc_sw(at, 16, 1024, 2), x = pm::smem_desc_sw(at + S::kW, 16, 1024, 2);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -352,6 +371,36 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok);
       it = __reduce_max_sync(0xFFFFFFFFu, it);
       ring.at(it);
+      buf.at(it);
+    }
+    __syncwarp();
+  } else if (S::kCopyWarp && warp == 7) {
+    // scales from shared to tensor memory: up to twelve copies a stage, which take their issuer as long as the products
+    Ring<S::kStages> ring, old;  // this stage; the one kBufs stages ago
+    Ring<S::kBufs> buf;
+    int it = 0;
+    bool ok = true;
+    for (int id = first_item; ok && have; have = next_tile(id)) {
+      if (t.expert == p.groups.experts) continue;
+      if (elect_one()) {
+        for (int i = from; i < to; ++i, ++it, ring.next(), buf.next()) {
+          if (S::kBufs < S::kStages && it >= S::kBufs) {
+            // the buffer's last readers have finished
+            ok = pm::mbar_wait(&empty[old.slot], old.round, pm::kStatusTimeoutMma);
+            old.next();
+          }
+          ok = ok && pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+          if (!ok) break;
+          pm::tc_fence_after();
+          copy_scales(i, ring.slot, buf.slot);
+          pm::umma_commit(&scales_in[buf.slot]);
+        }
+      }
+      __syncwarp();
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      it = __reduce_max_sync(0xFFFFFFFFu, it);
+      ring.at(it);
+      buf.at(it);
       old.at(max(it - S::kBufs, 0));
     }
     __syncwarp();
@@ -359,7 +408,7 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
     const float x_second = p.x_second != nullptr ? *p.x_second : 1.0f;
     uint8_t* mine = out + (warp & 3) * 2048;
     int n = 0;
-    for (int id = first_item; id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+    for (int id = first_item; have; have = next_tile(id)) {
       if (t.expert == p.groups.experts) {
         if (rank == 0) store_zeros<DT>(p.y, t, p.rows, threadIdx.x - 64, 128);
         continue;
@@ -385,7 +434,7 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
       Ring<S::kStages> ring;
       int it = 0;
       bool ok = true;
-      for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+      for (int id = first_item; ok && have; have = next_tile(id)) {
         if (t.expert == p.groups.experts) continue;
         ScaleWords<FMT> ahead[2];  // loads in flight
 #pragma unroll
@@ -413,12 +462,12 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
     Ring<S::kStages> ring;
     int it = 0;
     bool ok = true;
-    for (int id = first_item; ok && id < p.items && find_tile(p.groups, id, BN, t); id += item_step) {
+    for (int id = first_item; ok && have; have = next_tile(id)) {
       if (t.expert == p.groups.experts) continue;
-      const int mine = warp - 7;
+      const int mine = warp - S::kFirstQuantWarp;
       int i = from + ((mine - it) & (kQuantWarps - 1));  // every eighth stage is this warp's
-      TokenBlock<DT> next;
-      if (i < to) next = load_tokens<DT>(p, t, i, 0);
+      TokenBlock<DT> next = first_tokens;
+      if (it > 0 && i < to) next = load_tokens<DT>(p, t, i, 0);
       for (; i < to; i += kQuantWarps) {
         const TokenBlock<DT> now = next;
         if (i + kQuantWarps < to) next = load_tokens<DT>(p, t, i + kQuantWarps, 0);

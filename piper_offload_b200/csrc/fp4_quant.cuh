@@ -28,7 +28,7 @@ enum : int { kFloor = 0, kRceil = 1, kCeil = 2, kEven = 3 };
 enum : int { kSecondNone = 0, kSecondGiven = 1, kSecondCompute = 2 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantRows = 4;   // rows in flight per lane
+constexpr int kQuantRows = 4;   // rows in flight per lane where there are many
 constexpr int kUnit = 16;       // values per lane and row
 constexpr int kSmallThreads = 512;
 
@@ -54,15 +54,24 @@ __host__ __device__ __forceinline__ int64_t first_scale_row(int64_t start, int64
   return (start / tile + e) * scale_rows_per_tile(tile);
 }
 
-// Expert whose rows hold row t (the first with ends[e] > t, or `experts`).
-__device__ __forceinline__ int expert_of_row(const int32_t* ends, int experts, int64_t t) {
-  int lo = 0, hi = experts;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ends[mid] > t) hi = mid;
-    else lo = mid + 1;
+// Experts of `rows` rows from row0 on: lane j gets row row0 + j's, as how many
+// ends are at or before it, and the last of those (0 without one). A warp
+// calls; one load of the ends serves all rows (a search by halves a lane took
+// five, 2 us of a 4 us launch).
+__device__ __forceinline__ void experts_of_rows(const int32_t* ends, int experts, int64_t row0, int rows, int& expert, int& start) {
+  const int lane = threadIdx.x & 31;
+  expert = start = 0;
+  for (int e0 = 0; e0 < experts; e0 += 32) {
+    const int32_t v = e0 + lane < experts ? ends[e0 + lane] : 0x7FFFFFFF;
+    for (int j = 0; j < rows; ++j) {
+      const uint32_t before = __ballot_sync(0xFFFFFFFFu, v <= row0 + j);
+      const int32_t last = __shfl_sync(0xFFFFFFFFu, v, before != 0u ? 31 - __clz(before) : 0);
+      if (lane == j && before != 0u) {
+        expert += __popc(before);
+        start = last;
+      }
+    }
   }
-  return lo;
 }
 
 struct QuantArgs {
@@ -96,12 +105,12 @@ struct QuantArgs {
 // Lanes that share a row: 32, or fewer (at least a tile of scales) for short rows.
 __host__ __device__ __forceinline__ int lanes_per_row(int units) { return units > 16 ? 32 : units > 8 ? 16 : 8; }
 // Blocks of kQuantThreads threads that a walk takes.
-__host__ __device__ __forceinline__ int64_t quant_row_blocks(const QuantArgs& q) {
-  const int rows = kQuantThreads / lanes_per_row(q.units) * kQuantRows;
+__host__ __device__ __forceinline__ int64_t quant_row_blocks(const QuantArgs& q, int rows_per_lane) {
+  const int rows = kQuantThreads / lanes_per_row(q.units) * rows_per_lane;
   return (q.rows_padded + rows - 1) / rows;
 }
-__host__ __device__ __forceinline__ int64_t quant_blocks(const QuantArgs& q) {
-  return q.batch * quant_row_blocks(q) * ((q.units + 31) / 32);
+__host__ __device__ __forceinline__ int64_t quant_blocks(const QuantArgs& q, int rows_per_lane) {
+  return q.batch * quant_row_blocks(q, rows_per_lane) * ((q.units + 31) / 32);
 }
 
 // 16 neighbouring values as they are stored.
@@ -257,8 +266,8 @@ __device__ __forceinline__ float second_of_amax(uint32_t amax) {
   return g < 1.1920928955078125e-07f ? 1.1920928955078125e-07f : g;
 }
 
-// A warp quantizes kQuantRows rows (more where a row is short) x 512 columns of matrix e.
-template <int DT, int FMT>
+// A warp quantizes R rows (more where a row is short) x 512 columns of matrix e.
+template <int DT, int FMT, int R>
 __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk, float g, float inv_g) {
   constexpr int kLanes = FMT == kMX ? 2 : 1;  // lanes per block
   const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
@@ -267,9 +276,9 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
   const int64_t first = row0 + lane / per;
   const bool in_row = unit < q.units, in_cols = unit * kUnit < q.cols;
 
-  Raw<DT> raw[kQuantRows];
+  Raw<DT> raw[R];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < R; ++u) {
     const int64_t r = first + u * step;
     if (in_cols && r < q.rows) {
       raw[u] = load_unit<DT>(q.x, (e * q.rows + r) * q.x_stride + unit * kUnit, q.vec != 0);
@@ -282,13 +291,9 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
   int64_t place = 0;
   if (q.token_tile != 0) {
     const int64_t r = row0 + lane;
-    int x = 0;
-    int64_t start = 0;
-    if (q.ends != nullptr && lane < kQuantRows * step && r < q.rows) {
-      x = expert_of_row(q.ends, q.experts, r);
-      start = x > 0 ? q.ends[x - 1] : 0;
-    }
-    if (q.ends != nullptr && (x >= q.experts || start < 0 || start > r)) {
+    int x = 0, start = 0;
+    if (q.ends != nullptr) experts_of_rows(q.ends, q.experts, row0, R * step, x, start);
+    if (x >= q.experts || start < 0 || start > r) {
       place = -1;  // a row of no expert
     } else {
       const int o = static_cast<int>(r - start);
@@ -299,7 +304,7 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
   const bool two = FMT == kNV && q.second_mode != kSecondNone;
   const int c = unit / kLanes;
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < R; ++u) {
     const int64_t r = first + u * step;
     float v[16];
     to_floats(raw[u], v);
@@ -329,13 +334,13 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
 }
 
 // Block `b` of quant_blocks(q).
-template <int DT, int FMT>
+template <int DT, int FMT, int R>
 __device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
   const int chunks = (q.units + 31) / 32;
-  const int64_t per = quant_row_blocks(q);
+  const int64_t per = quant_row_blocks(q, R);
   const int64_t rb = b / chunks, e = q.batch == 1 ? 0 : rb / per;
   const int chunk = static_cast<int>(b - rb * chunks);
-  const int rows = 32 / lanes_per_row(q.units) * kQuantRows;  // per warp
+  const int rows = 32 / lanes_per_row(q.units) * R;  // per warp
   const int64_t row0 = (rb - e * per) * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows;
   float g = 1.0f, inv_g = 1.0f;
   if (FMT == kNV && q.second_mode != kSecondNone) {
@@ -343,12 +348,12 @@ __device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
     inv_g = __fdiv_rn(1.0f, g);
     if (q.second_mode == kSecondCompute && rb == e * per && chunk == 0 && threadIdx.x == 0) q.second[e] = g;
   }
-  quantize_rows<DT, FMT>(q, e, row0, chunk, g, inv_g);
+  quantize_rows<DT, FMT, R>(q, e, row0, chunk, g, inv_g);
 }
 
-template <int DT, int FMT>
+template <int DT, int FMT, int R>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantArgs q) {
-  quantize_block<DT, FMT>(q, q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x);
+  quantize_block<DT, FMT, R>(q, q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x);
 }
 
 // Bits of the largest magnitude of a warp's rows x 512 columns, in every lane.
@@ -383,7 +388,7 @@ __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) amax_kernel(const __grid_constant__ QuantArgs q, uint32_t* amax) {
   const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * kQuantRows;
-  const int64_t blocks = quant_row_blocks(q) * chunks;
+  const int64_t blocks = quant_row_blocks(q, kQuantRows) * chunks;
   uint32_t m = 0u;
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int64_t rb = b / chunks;
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __g
   if (threadIdx.x == 0) q.second[e] = g;
   const float inv_g = __fdiv_rn(1.0f, g);
   for (int i = warp; i < pieces; i += kSmallThreads / 32)
-    quantize_rows<DT, FMT>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, g, inv_g);
+    quantize_rows<DT, FMT, kQuantRows>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, g, inv_g);
 }
 
 // ------------------------------------------------------------ back to values
@@ -565,11 +570,11 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
 
 // What a product needs ahead of it, in one launch: blocks below
 // `token_blocks` quantize tokens, the others lay codes out.
-template <int DT, int FMT>
+template <int DT, int FMT, int R>
 __global__ void __launch_bounds__(kQuantThreads)
     prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t token_blocks) {
   grid_launch_dependents();
-  if (blockIdx.x < token_blocks) quantize_block<DT, FMT>(q, blockIdx.x);
+  if (blockIdx.x < token_blocks) quantize_block<DT, FMT, R>(q, blockIdx.x);
   else repack(p, static_cast<int64_t>(blockIdx.x - token_blocks) * kQuantThreads + threadIdx.x);
 }
 
