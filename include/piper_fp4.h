@@ -55,7 +55,8 @@ typedef struct piper_fp4_matrix {
 
 /* Quantises x (batch * rows rows of `cols` values, `x_stride` values apart)
  * into m's buffers. Swizzle padding is zeroed. `maxima`: scratch of `batch`
- * words when second_mode is PIPER_FP4_SECOND_COMPUTE, else NULL. */
+ * words when second_mode is PIPER_FP4_SECOND_COMPUTE and a matrix has more
+ * than 65536 values; else it is not used. */
 int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_stride, int32_t dtype, int32_t scale_mode,
                        int32_t second_mode, uint32_t* maxima, void* stream);
 

@@ -24,6 +24,8 @@ DT_F32 = 2
 SECOND_NONE = 0
 SECOND_GIVEN = 1
 SECOND_COMPUTE = 2
+# Matrices of at most so many values need no room for the maxima (include/piper_fp4.h).
+SMALL_MATRIX = 65536
 
 EXPORTED_SYMBOLS = (
     "piper_fp4_quantize",
@@ -102,6 +104,14 @@ def check(rc: int) -> None:
     if rc == EINVAL:
         raise ValueError(msg)
     raise RuntimeError(f"piper fp4 failed (status {rc}): {msg}")
+
+
+# The current stream's handle by device index, without making a stream object (2 us of a 10 us call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else current_stream_handle(torch.device("cuda", index))
 
 
 def device_status(device: torch.device) -> int:

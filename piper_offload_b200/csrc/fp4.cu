@@ -294,9 +294,7 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
   q.second_mode = second_mode;
   q.second = m->second;
   if (second_mode == PIPER_FP4_SECOND_COMPUTE) {
-    FP4_REQUIRE(maxima != nullptr, "FP4 quantisation: computing second-level scales needs room for the maxima.");
     FP4_REQUIRE(m->batch <= 65535, "FP4 quantisation: at most 65535 matrices with second-level scales.");
-    q.amax = maxima;
     q.reverse = 1;
     if (m->rows * m->cols <= kSmallMatrix) {
 #define CALL(D, F) fp4::quantize_small_kernel<D, F><<<static_cast<unsigned>(m->batch), fp4::kSmallThreads, 0, s>>>(q)
@@ -305,6 +303,8 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
       const cudaError_t e = launched();
       return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("quantize kernel", e);
     }
+    FP4_REQUIRE(maxima != nullptr, "FP4 quantisation: computing second-level scales needs room for the maxima.");
+    q.amax = maxima;
     cudaError_t e = cudaMemsetAsync(maxima, 0, sizeof(uint32_t) * m->batch, s);
     if (e != cudaSuccess) return cuda_fail("cudaMemsetAsync", e);
     const int64_t blocks = fp4::quant_row_blocks(q, fp4::kQuantRows) * ((q.units + 31) / 32);

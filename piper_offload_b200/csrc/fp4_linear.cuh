@@ -216,7 +216,6 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  warm_arguments(p);
   // this block's part of every tile's stages
   const int all = (p.k_steps + 3) / 4;
   const int rank = p.split > 1 ? static_cast<int>(cluster_rank()) : 0;

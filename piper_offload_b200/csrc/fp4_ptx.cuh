@@ -135,16 +135,6 @@ __device__ __forceinline__ float4 load_cluster(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
-// Touches every line of a kernel's arguments at once, so that the first uses
-// of them do not miss the constant cache one after another.
-template <class Args>
-__device__ __forceinline__ void warm_arguments(const Args& args) {
-  constexpr int kWords = sizeof(Args) / 4;
-  const int at = (threadIdx.x & 31) * 16;
-  const int v = reinterpret_cast<const int*>(&args)[at < kWords ? at : kWords - 1];
-  asm volatile("" ::"r"(v));
-}
-
 // Programmatic launches: let the next kernel start its own set-up / wait for
 // everything the previous one wrote.
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -54,24 +54,29 @@ def _dtype(t: torch.Tensor, what: str) -> int:
 def _matrix(w: Any) -> tuple[nat.Matrix, int, torch.Tensor]:
     """(descriptor, MX scaling mode of activations, codes) of a packed weight or stack, checked."""
     q, s = w.qdata, w.scale
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError("FP4 operators require CUDA tensors.")
     if q.dtype is not torch.uint8:
         raise ValueError(f"FP4 operators expect packed uint8 codes, got {q.dtype}.")
-    if q.ndim not in (2, 3) or s.ndim != q.ndim:
+    shape, scale_shape = q.shape, s.shape
+    if len(shape) == 2:
+        batch, (rows, cols) = 1, shape
+    elif len(shape) == 3:
+        batch, rows, cols = shape
+        if len(scale_shape) == 3 and scale_shape[0] != batch:
+            raise ValueError(f"FP4 scale shape {tuple(scale_shape)} does not match its layout.")
+    if len(shape) not in (2, 3) or len(scale_shape) != len(shape):
         raise ValueError("FP4 operators expect rank-two weights, or rank-three stacks of experts.")
+    cols *= 2
     if not q.is_contiguous() or not s.is_contiguous():
         raise ValueError("FP4 operators require contiguous codes and scales.")
     if s.device != q.device:
         raise ValueError("FP4 operators require all tensors on one CUDA device.")
-    batch = q.shape[0] if q.ndim == 3 else 1
-    rows, cols = q.shape[-2], q.shape[-1] * 2
     if batch == 0 or rows == 0 or cols == 0:
         raise ValueError("FP4 operators require non-empty weights.")
     swizzled = bool(w.is_swizzled_scales)
     second = None
     elem = getattr(w, "elem_dtype", None)
-    mode: int | None = 0
     if elem is not None:
         if elem is not _FP4 or _FP4 is None:
             raise ValueError(f"FP4 operators support MX weights with e2m1 elements, got {elem}.")
@@ -94,33 +99,25 @@ def _matrix(w: Any) -> tuple[nat.Matrix, int, torch.Tensor]:
         if second is not None and (second.dtype is not torch.float32 or second.numel() != batch
                                    or second.device != q.device or not second.is_contiguous()):
             raise ValueError("NVFP4 second-level scales are one contiguous float32 value per matrix on its device.")
-        fmt = nat.FMT_NV
-    if s.shape[-2:] != expected or (q.ndim == 3 and s.shape[0] != batch):
-        raise ValueError(f"FP4 scale shape {tuple(s.shape)} does not match its layout.")
+        fmt, mode = nat.FMT_NV, 0
+    if scale_shape[-2:] != expected:
+        raise ValueError(f"FP4 scale shape {tuple(scale_shape)} does not match its layout.")
     m = nat.Matrix(q.data_ptr(), s.data_ptr(), None if second is None else second.data_ptr(), batch, rows, cols, fmt,
                    swizzled)
     return m, mode, q
 
 
-class _on:
-    """The device of a call, entered only where it is not the current one."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device) -> None:
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self) -> None:
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc: Any) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(function: Any, device: torch.device, *args: Any) -> None:
+    """A library call on the current stream of ``device``, which is entered where it is not the current one."""
+    if torch.cuda.current_device() == device.index:
+        nat.check(function(*args, nat.raw_stream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            nat.check(function(*args, nat.raw_stream(device.index)))
 
 
 def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor | None:
-    need = ctypes.c_size_t(0)
+    need = ctypes.c_size_t()
     nat.check(query(*args, ctypes.byref(need)))
     return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
 
@@ -142,7 +139,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torch.Tensor | None,
               second_mode: int) -> tuple[torch.Tensor, torch.Tensor]:
     block = 32 if fmt == nat.FMT_MX else 16
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("FP4 quantisation requires CUDA tensors.")
     dt = _dtype(x, "quantisation")
     if x.ndim not in (2, 3):
@@ -155,15 +152,15 @@ def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torc
     x2 = _rows(x.detach())
     lead = x.shape[:-2]
     shape = (K.mx_expected_scale_shape if fmt == nat.FMT_MX else K.nvfp4_expected_scale_shape)(rows, cols, swizzled=swizzled)
-    codes = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((*lead, *shape), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty((*lead, rows, cols // 2), dtype=torch.uint8)
+    scale = x.new_empty((*lead, *shape), dtype=torch.uint8 if fmt == nat.FMT_MX else torch.float8_e4m3fn)
     m = nat.Matrix(codes.data_ptr(), scale.data_ptr(), None if second is None else second.data_ptr(),
                    lead[0] if lead else 1, rows, cols, fmt, swizzled)
-    maxima = torch.empty(m.batch, dtype=torch.int32, device=x.device) if second_mode == nat.SECOND_COMPUTE else None
-    with _on(x.device):
-        nat.check(nat.load().piper_fp4_quantize(
-            ctypes.byref(m), x2.data_ptr(), x2.stride(0), dt, mode, second_mode,
-            None if maxima is None else maxima.data_ptr(), nat.current_stream_handle(x.device)))
+    maxima = None
+    if second_mode == nat.SECOND_COMPUTE and rows * cols > nat.SMALL_MATRIX:
+        maxima = x.new_empty(m.batch, dtype=torch.int32)
+    _call(nat.load().piper_fp4_quantize, x.device, ctypes.byref(m), x2.data_ptr(), x2.stride(0), dt, mode, second_mode,
+          None if maxima is None else maxima.data_ptr())
     return codes, scale
 
 
@@ -199,20 +196,18 @@ def quantize_nvfp4(x: torch.Tensor, *, two_level: bool = True, per_tensor_scale:
                 or per_tensor_scale.device != x.device):
             raise ValueError("NVFP4 second-level scales are one float32 value per matrix on its device.")
         second, second_mode = per_tensor_scale.detach().reshape(batch).contiguous(), nat.SECOND_GIVEN
-    elif two_level and x.device.type == "cuda":
-        second, second_mode = torch.empty(batch, dtype=torch.float32, device=x.device), nat.SECOND_COMPUTE
+    elif two_level and x.is_cuda:
+        second, second_mode = x.new_empty(batch, dtype=torch.float32), nat.SECOND_COMPUTE
     codes, scale = _quantize(x, nat.FMT_NV, 0, swizzled, second, second_mode)
     kind = NVFP4Experts if x.ndim == 3 else NVFP4Weight
-    return kind(codes, scale.view(torch.float8_e4m3fn), second, orig_dtype=x.dtype, is_swizzled_scales=swizzled)
+    return kind(codes, scale, second, orig_dtype=x.dtype, is_swizzled_scales=swizzled)
 
 
 def dequantize_fp4(weight: Any, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values of a packed weight or stack, rounded once to ``dtype`` (default: the weight's original type)."""
     m, _, q = _matrix(weight)
-    y = torch.empty((*q.shape[:-1], m.cols), dtype=dtype or weight.orig_dtype, device=q.device)
-    dt = _dtype(y, "dequantisation")
-    with _on(q.device):
-        nat.check(nat.load().piper_fp4_dequantize(ctypes.byref(m), y.data_ptr(), dt, nat.current_stream_handle(q.device)))
+    y = q.new_empty((*q.shape[:-1], m.cols), dtype=dtype or weight.orig_dtype)
+    _call(nat.load().piper_fp4_dequantize, q.device, ctypes.byref(m), y.data_ptr(), _dtype(y, "dequantisation"))
     return y
 
 
@@ -239,17 +234,13 @@ def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: 
             raise ValueError("The activations' second-level scale is one float32 value on their device.")
     x2 = _rows(x)
     tokens = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], m.rows), dtype=x.dtype, device=device)
+    y = x.new_empty((tokens, m.rows) if x2 is x else (*x.shape[:-1], m.rows))
     if tokens == 0:
         return y
-    lib = nat.load()
-    ref = ctypes.byref(m)
+    lib, ref = nat.load(), ctypes.byref(m)
     ws = _workspace(lib.piper_fp4_linear_workspace, device, ref, tokens)
-    with _on(device):
-        nat.check(lib.piper_fp4_linear(
-            ref, x2.data_ptr(), x2.stride(0), tokens, None if ends is None else ends.data_ptr(),
-            None if act_scale is None else act_scale.data_ptr(), mode, y.data_ptr(), dt, *_span(ws),
-            nat.current_stream_handle(device)))
+    _call(lib.piper_fp4_linear, device, ref, x2.data_ptr(), x2.stride(0), tokens, None if ends is None else ends.data_ptr(),
+          None if act_scale is None else act_scale.data_ptr(), mode, y.data_ptr(), dt, *_span(ws))
     return y
 
 
@@ -263,16 +254,15 @@ def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> t
         raise ValueError(f"FP4 gradient: the output's gradient has {tuple(grad.shape)}, the weight {m.rows} rows.")
     g2 = _rows(grad)
     tokens = g2.shape[0]
-    dx = torch.empty((*grad.shape[:-1], m.cols), dtype=grad.dtype, device=device)
+    dx = grad.new_empty((tokens, m.cols) if g2 is grad else (*grad.shape[:-1], m.cols))
     if tokens == 0:
         return dx
-    lib = nat.load()
-    ref = ctypes.byref(m)
-    ws = _workspace(lib.piper_fp4_grad_input_workspace, device, ref, g2.data_ptr(), g2.stride(0), tokens, dt)
-    with _on(device):
-        nat.check(lib.piper_fp4_grad_input(
-            ref, g2.data_ptr(), g2.stride(0), tokens, None if ends is None else ends.data_ptr(), dx.data_ptr(), dt,
-            *_span(ws), nat.current_stream_handle(device)))
+    lib, ref = nat.load(), ctypes.byref(m)
+    ws = None
+    if dt != nat.DT_BF16 or g2.data_ptr() % 16 or g2.stride(0) % 8:  # bf16 rows that bulk copies can read need none
+        ws = _workspace(lib.piper_fp4_grad_input_workspace, device, ref, g2.data_ptr(), g2.stride(0), tokens, dt)
+    _call(lib.piper_fp4_grad_input, device, ref, g2.data_ptr(), g2.stride(0), tokens, None if ends is None else ends.data_ptr(),
+          dx.data_ptr(), dt, *_span(ws))
     return dx
 
 

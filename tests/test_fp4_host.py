@@ -102,7 +102,7 @@ def test_bad_arguments_are_refused():
 
     for m2, kw, match in ((m, {"x": None}, "null"), (m, {"stride": 64}, "overlap"), (m, {"dtype": 1}, "bfloat16"),
                           (m, {"mode": 9}, "scaling mode"), (m, {"second": 3}, "second-level mode"), (m, {"second": 1}, "match"),
-                          (matrix(second=0x3000), {}, "match"), (matrix(second=0x3000), {"second": 2}, "maxima"),
+                          (matrix(second=0x3000), {}, "match"), (matrix(second=0x3000, rows=4096), {"second": 2}, "maxima"),
                           (matrix(codes=0x1002), {}, "4-byte")):
         with pytest.raises(ValueError, match=match):
             nat.check(quantize(m2, **kw))
