@@ -245,14 +245,44 @@ GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, in
   return p;
 }
 
-template <int DT, int FMT, int BN>
-cudaError_t launch_grad(const fp4::GradArgs& args, int64_t items, cudaStream_t stream) {
-  using S = fp4::GradShape<BN>;
-  auto kernel = fp4::grad_kernel<DT, FMT, BN>;
+// Tiles of a gradient: tokens x (rows x 128) columns. The least of a rough
+// account in cycles: a stage keeps a block busy for about 1060 (256 x 256),
+// 330 (128 x 128, two blocks an SM) or 300 (32 x 128, likewise).
+struct GradTile {
+  int bn, rows;
+};
+GradTile grad_tile(const piper_fp4_matrix& w, int64_t tokens) {
+  const int64_t per_expert = tokens / w.batch;
+  if (per_expert <= 32) return {32, 1};
+  const auto waves = [&](int64_t bn, int64_t cols, int blocks_per_sm) {
+    const int64_t tiles = w.batch * ((per_expert + bn - 1) / bn) * ((w.cols + cols - 1) / cols);
+    const int64_t slots = static_cast<int64_t>(sm_count()) * blocks_per_sm;
+    return static_cast<double>((tiles + slots - 1) / slots);
+  };
+  return waves(256, 256, 1) * 1060.0 <= waves(128, 128, 2) * 660.0 ? GradTile{256, 2} : GradTile{128, 1};
+}
+
+template <int DT, int FMT, int BN, int kRows>
+cudaError_t launch_grad(fp4::GradArgs& args, int64_t items, cudaStream_t stream) {
+  using S = fp4::GradShape<BN, kRows>;
+  auto kernel = fp4::grad_kernel<DT, FMT, BN, kRows>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  kernel<<<static_cast<unsigned>(items), fp4::kGradThreads, S::kSmem, stream>>>(args);
-  return launched();
+  const int stages = (args.rows + fp4::kGradStageRows - 1) / fp4::kGradStageRows * args.terms;
+  args.split = split_of<S>(items, stages, static_cast<int>(std::min<int64_t>(args.groups.tokens, BN)));
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(args.split);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(items * args.split));
+  config.blockDim = dim3(fp4::kGradThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = args.split > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&config, kernel, args);
+  return e == cudaSuccess ? launched() : e;
 }
 
 }  // namespace
@@ -501,7 +531,8 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   a.codes = static_cast<const uint8_t*>(w->codes);
   a.scale = static_cast<const uint8_t*>(w->scale);
   a.second = w->second;
-  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 127) / 128)};
+  const GradTile tile = grad_tile(*w, tokens);
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 128 * tile.rows - 1) / (128 * tile.rows))};
   a.dx = dx;
   a.code_pitch = w->cols / 2;
   a.rows = static_cast<int32_t>(w->rows);
@@ -512,15 +543,14 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   a.vec = aligned(dx, 16) && w->cols % 8 == 0;
   a.piece = aligned(w->codes, 16) && a.code_pitch % 16 == 0 ? 16 : aligned(w->codes, 8) ? 8 : 1;
 
-  const int64_t per_expert = tokens / w->batch;
-  const int bn = per_expert <= 32 ? 32 : per_expert <= 128 ? 128 : 256;
+  const int bn = tile.bn;
   const void* src = p.move ? workspace : dy;
   const int64_t pitch = p.move ? p.pitch : tokens > 1 ? dy_stride : up(w->rows, 8);
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, src, w->rows, p.terms * tokens, pitch * 2, fp4::kGradStageRows, bn))
     return fail(PIPER_FP4_ECUDA, "FP4 gradient: cuTensorMapEncodeTiled failed.");
   const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
   const int64_t split_blocks = tokens * ((w->rows + 255) / 256);
-  FP4_REQUIRE(items < (int64_t{1} << 31) && split_blocks < (int64_t{1} << 31), "FP4 gradient: too many tiles for one call.");
+  FP4_REQUIRE(items < (int64_t{1} << 31) / fp4::kMaxSplit && split_blocks < (int64_t{1} << 31), "FP4 gradient: too many tiles for one call.");
   cudaError_t e = cudaSuccess;
   if (p.move) {
     auto kernel = dtype == PIPER_FP4_BF16 ? fp4::split_kernel<fp4::kBF16> : fp4::split_kernel<fp4::kF32>;
@@ -528,9 +558,9 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
                                                                static_cast<__nv_bfloat16*>(workspace));
     if ((e = launched()) != cudaSuccess) return cuda_fail("split kernel", e);
   }
-#define CALL(D, F)                                    \
-  e = bn == 32 ? launch_grad<D, F, 32>(a, items, s)   \
-               : bn == 128 ? launch_grad<D, F, 128>(a, items, s) : launch_grad<D, F, 256>(a, items, s)
+#define CALL(D, F)                                       \
+  e = bn == 32 ? launch_grad<D, F, 32, 1>(a, items, s)   \
+               : bn == 128 ? launch_grad<D, F, 128, 1>(a, items, s) : launch_grad<D, F, 256, 2>(a, items, s)
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("gradient kernel", e);
