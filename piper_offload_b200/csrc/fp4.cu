@@ -276,7 +276,7 @@ cudaError_t launch_grad(fp4::GradArgs& args, int64_t items, cudaStream_t stream)
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(items * args.split));
-  config.blockDim = dim3(fp4::kGradThreads);
+  config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
   config.attrs = &attribute;

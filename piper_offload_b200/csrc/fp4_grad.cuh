@@ -26,8 +26,7 @@
 namespace fp4 {
 
 constexpr int kGradStageRows = 64;   // rows of w per stage
-constexpr int kGradThreads = 320;    // producer warp, tensor-core warp, eight decoding and epilogue warps
-constexpr int kDecodeWarps = 8;
+constexpr int kDecodeWarps = 8;      // for each 128 columns of a tile; they run the epilogue too
 
 struct GradArgs {
   CUtensorMap dy_map;   // (terms * tokens, rows of w) bf16
@@ -55,6 +54,7 @@ struct GradShape {
   static constexpr int kRoom = kSmemMax / kCtas - 3072;
   static constexpr int kStages = kRoom / kStage < 5 ? kRoom / kStage : 5;
   static constexpr int kSmem = kStages * kStage + 1024 + 256;
+  static constexpr int kThreads = 64 + 32 * kDecodeWarps * kRows;  // producer warp, tensor-core warp, decoding warps
   static constexpr int kAlloc = kRows * BN;
   static constexpr bool kCanSplit = kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
   static_assert(kAlloc >= 32 && kAlloc * kCtas <= 512 && kStages >= 3, "the tile does not fit");
@@ -138,7 +138,7 @@ struct PieceWalk {
 };
 
 template <int DT, int FMT, int BN, int kRows>
-__global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) grad_kernel(const __grid_constant__ GradArgs p) {
+__global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, kRows>::kCtas) grad_kernel(const __grid_constant__ GradArgs p) {
   using S = GradShape<BN, kRows>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) gra
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1);
-      pm::mbar_init(&ready[s], kDecodeWarps);
+      pm::mbar_init(&ready[s], kDecodeWarps * kRows);
       pm::mbar_init(&empty[s], 1);
     }
     pm::mbar_init(done, 1);
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) gra
       for (int h = 0; h < kRows; ++h) {
         TileAt part = t;
         part.row_tile = t.row_tile * kRows + h;
-        store_zeros<DT>(p.dx, part, p.cols, threadIdx.x, kGradThreads);
+        store_zeros<DT>(p.dx, part, p.cols, threadIdx.x, S::kThreads);
       }
   } else if (sums) {
     if (warp == 0) {
@@ -230,60 +230,45 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) gra
       }
       __syncwarp();
     } else {
-      const int tid = threadIdx.x - 64;
-      const int r = tid >> 2, quarter = tid & 3;  // row of the stage, 32 of every 128 columns
-      PieceWalk<FMT> walk[kRows];
-      Piece soon[kRows], later[kRows];  // the next stage's, the one after's
+      // eight warps for each 128 columns: a warp decodes eight rows of a stage, a lane 32 columns of one, and the eight
+      // lanes whose 16-byte stores go together write different rows, so the swizzle gives them different banks
+      const int h = (warp - 2) / kDecodeWarps;
+      const int r = (warp - 2) % kDecodeWarps * 8 + (lane & 7), quarter = lane >> 3;
+      const int col = (t.row_tile * kRows + h) * kTileRows + quarter * 32;
+      uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (quarter >> 1) * (kGradStageRows * 128) + r * 128;
+      PieceWalk<FMT> walk;
       int block = from % blocks;  // of the next loads
-#pragma unroll
-      for (int h = 0; h < kRows; ++h)
-        walk[h].begin(p, t.expert, block, r, (t.row_tile * kRows + h) * kTileRows + quarter * 32);
-      const auto load_next = [&](Piece(&into)[kRows]) {
-#pragma unroll
-        for (int h = 0; h < kRows; ++h) {
-          into[h] = walk[h].load();
-          walk[h].next();
-        }
+      walk.begin(p, t.expert, block, r, col);
+      const auto load_next = [&]() {
+        const Piece piece = walk.load();
+        walk.next();
         if (++block == blocks) {  // the next term
           block = 0;
-#pragma unroll
-          for (int h = 0; h < kRows; ++h)
-            walk[h].begin(p, t.expert, 0, r, (t.row_tile * kRows + h) * kTileRows + quarter * 32);
+          walk.begin(p, t.expert, 0, r, col);
         }
+        return piece;
       };
-      load_next(soon);
-      load_next(later);
+      Piece soon = load_next(), later = load_next();  // the next stage's, the one after's
       Ring<S::kStages> ring;
       bool ok = true;
       for (int i = from; i < to; ++i, ring.next()) {
-        Piece now[kRows];
-#pragma unroll
-        for (int h = 0; h < kRows; ++h) {
-          now[h] = soon[h];
-          soon[h] = later[h];
-        }
-        if (i + 2 < to) load_next(later);
+        const Piece now = soon;
+        soon = later;
+        if (i + 2 < to) later = load_next();
         if (i - from >= S::kStages) {
           ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad));
           if (!ok) break;
         }
+        uint8_t* row = to_row + ring.slot * S::kStage;
+        const uint32_t c[4] = {now.codes.x, now.codes.y, now.codes.z, now.codes.w};
+        const __nv_bfloat162 scale[2] = {__float2bfloat162_rn(scale_value<FMT>(now.scale[0])),
+                                         __float2bfloat162_rn(scale_value<FMT>(now.scale[1]))};
 #pragma unroll
-        for (int h = 0; h < kRows; ++h) {
-          uint8_t* row = smem + ring.slot * S::kStage + h * (kGradStageRows * kTileRows * 2) + (quarter >> 1) * (kGradStageRows * 128) + r * 128;
-          const uint32_t c[4] = {now[h].codes.x, now[h].codes.y, now[h].codes.z, now[h].codes.w};
-          const __nv_bfloat162 scale[2] = {__float2bfloat162_rn(scale_value<FMT>(now[h].scale[0])),
-                                           __float2bfloat162_rn(scale_value<FMT>(now[h].scale[1]))};
-          // the two 64-column blocks go through their 16-byte pieces in another order, so that eight lanes hit eight banks
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t code = quarter >> 1 ? c[q ^ 2] : c[q];
-            const __nv_bfloat162 unit = FMT == kMX ? scale[0] : quarter >> 1 ? scale[(q ^ 2) >> 1] : scale[q >> 1];
-            const int piece = q ^ ((quarter >> 1) * 2);
-            uint4 v;
-            decode4(code, unit, v.x, v.y);
-            decode4(code >> 16, unit, v.z, v.w);
-            *reinterpret_cast<uint4*>(row + ((((quarter & 1) * 4 + piece) ^ (r & 7)) << 4)) = v;
-          }
+        for (int q = 0; q < 4; ++q) {
+          uint4 v;
+          decode4(c[q], scale[q >> 1], v.x, v.y);
+          decode4(c[q] >> 16, scale[q >> 1], v.z, v.w);
+          *reinterpret_cast<uint4*>(row + ((((quarter & 1) * 4 + q) ^ (r & 7)) << 4)) = v;
         }
         pm::fence_proxy_async_smem();
         __syncwarp();
@@ -298,16 +283,13 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) gra
         } else {
           const float alpha = p.second != nullptr ? p.second[t.expert] : 1.0f;
           uint8_t* mine = smem + (warp - 2) * 2048;
-#pragma unroll
-          for (int h = 0; h < kRows; ++h) {
-            TileAt part = t;
-            part.row_tile = t.row_tile * kRows + h;
-            if constexpr (BN >= 64) {  // two warps share each quarter of the lanes: halves of the tokens
-              const int half = warp >= 6;
-              store_tile<DT>(tmem + h * BN, p.dx, part, p.cols, alpha, half * (BN / 2), (half + 1) * (BN / 2), mine, p.vec != 0);
-            } else if (warp < 6) {
-              store_tile<DT>(tmem + h * BN, p.dx, part, p.cols, alpha, 0, BN, mine, p.vec != 0);
-            }
+          TileAt part = t;
+          part.row_tile = t.row_tile * kRows + h;
+          if constexpr (BN >= 64) {  // two warps share each quarter of the lanes: halves of the tokens
+            const int half = (warp - 2) % kDecodeWarps >= 4;
+            store_tile<DT>(tmem + h * BN, p.dx, part, p.cols, alpha, half * (BN / 2), (half + 1) * (BN / 2), mine, p.vec != 0);
+          } else if (warp < 6) {
+            store_tile<DT>(tmem, p.dx, part, p.cols, alpha, 0, BN, mine, p.vec != 0);
           }
         }
       }
@@ -319,7 +301,7 @@ __global__ void __launch_bounds__(kGradThreads, GradShape<BN, kRows>::kCtas) gra
     cluster_sync();  // every block's sums are written
     if (sums)
       add_cluster_sums<DT>(reinterpret_cast<const float*>(smem), p.dx, t, p.cols, p.second != nullptr ? p.second[t.expert] : 1.0f,
-                           rank, p.split, kGradThreads, p.vec != 0);
+                           rank, p.split, S::kThreads, p.vec != 0);
     __syncwarp();
     cluster_sync();  // nobody's shared memory goes while others read it
   }
