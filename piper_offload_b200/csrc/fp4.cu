@@ -245,21 +245,20 @@ GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, in
   return p;
 }
 
-// Tiles of a gradient: tokens x (rows x 128) columns. The least of a rough
-// account in cycles: a stage keeps a block busy for about 1060 (256 x 256),
-// 330 (128 x 128, two blocks an SM) or 300 (32 x 128, likewise).
+// Tiles of a gradient: tokens x (rows x 128) columns. Decoding costs the same
+// whatever the tokens, so tiles are as wide in tokens as they go; 256 columns
+// where that fills the SMs (a rough account in cycles a stage: 1060 and 600).
 struct GradTile {
   int bn, rows;
 };
 GradTile grad_tile(const piper_fp4_matrix& w, int64_t tokens) {
   const int64_t per_expert = tokens / w.batch;
-  if (per_expert <= 32) return {32, 1};
-  const auto waves = [&](int64_t bn, int64_t cols, int blocks_per_sm) {
-    const int64_t tiles = w.batch * ((per_expert + bn - 1) / bn) * ((w.cols + cols - 1) / cols);
-    const int64_t slots = static_cast<int64_t>(sm_count()) * blocks_per_sm;
-    return static_cast<double>((tiles + slots - 1) / slots);
+  if (per_expert <= 48) return {64, 1};
+  const auto waves = [&](int64_t cols) {
+    const int64_t tiles = w.batch * ((per_expert + 255) / 256) * ((w.cols + cols - 1) / cols);
+    return static_cast<double>((tiles + sm_count() - 1) / sm_count());
   };
-  return waves(256, 256, 1) * 1060.0 <= waves(128, 128, 2) * 660.0 ? GradTile{256, 2} : GradTile{128, 1};
+  return waves(256) * 1060.0 <= waves(128) * 600.0 ? GradTile{256, 2} : GradTile{256, 1};
 }
 
 template <int DT, int FMT, int BN, int kRows>
@@ -559,8 +558,8 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
     if ((e = launched()) != cudaSuccess) return cuda_fail("split kernel", e);
   }
 #define CALL(D, F)                                       \
-  e = bn == 32 ? launch_grad<D, F, 32, 1>(a, items, s)   \
-               : bn == 128 ? launch_grad<D, F, 128, 1>(a, items, s) : launch_grad<D, F, 256, 2>(a, items, s)
+  e = bn == 64 ? launch_grad<D, F, 64, 1>(a, items, s)   \
+               : tile.rows == 1 ? launch_grad<D, F, 256, 1>(a, items, s) : launch_grad<D, F, 256, 2>(a, items, s)
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("gradient kernel", e);

@@ -26,7 +26,7 @@
 namespace fp4 {
 
 constexpr int kGradStageRows = 64;   // rows of w per stage
-constexpr int kDecodeWarps = 8;      // for each 128 columns of a tile; they run the epilogue too
+constexpr int kDecodeWarps = 8;      // for 64 rows x 128 columns; two such teams a block, which run the epilogue too
 
 struct GradArgs {
   CUtensorMap dy_map;   // (terms * tokens, rows of w) bf16
@@ -50,14 +50,14 @@ struct GradShape {
   static constexpr int kA = kRows * kGradStageRows * kTileRows * 2;
   static constexpr int kB = BN * kGradStageRows * 2;
   static constexpr int kStage = kA + kB;
-  static constexpr int kCtas = BN <= 128 ? 2 : 1;
-  static constexpr int kRoom = kSmemMax / kCtas - 3072;
-  static constexpr int kStages = kRoom / kStage < 5 ? kRoom / kStage : 5;
+  static constexpr int kRoom = kSmemMax - 3072;
+  static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + 1024 + 256;
-  static constexpr int kThreads = 64 + 32 * kDecodeWarps * kRows;  // producer warp, tensor-core warp, decoding warps
+  static constexpr int kThreads = 64 + 32 * kDecodeWarps * 2;  // producer warp, tensor-core warp, decoding warps
+  static constexpr int kTurns = 2 / kRows;  // teams that take stages in turn
   static constexpr int kAlloc = kRows * BN;
   static constexpr bool kCanSplit = kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
-  static_assert(kAlloc >= 32 && kAlloc * kCtas <= 512 && kStages >= 3, "the tile does not fit");
+  static_assert(kAlloc >= 32 && kAlloc <= 512 && kStages >= 3, "the tile does not fit");
 };
 
 // kind::f16, bf16 operands, fp32 sums, A stored M-major (bit 15), B K-major, M = 128.
@@ -138,7 +138,7 @@ struct PieceWalk {
 };
 
 template <int DT, int FMT, int BN, int kRows>
-__global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, kRows>::kCtas) grad_kernel(const __grid_constant__ GradArgs p) {
+__global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel(const __grid_constant__ GradArgs p) {
   using S = GradShape<BN, kRows>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, 
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1);
-      pm::mbar_init(&ready[s], kDecodeWarps * kRows);
+      pm::mbar_init(&ready[s], kDecodeWarps * kRows);  // of one team, or of both halves'
       pm::mbar_init(&empty[s], 1);
     }
     pm::mbar_init(done, 1);
@@ -230,31 +230,37 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, 
       }
       __syncwarp();
     } else {
-      // eight warps for each 128 columns: a warp decodes eight rows of a stage, a lane 32 columns of one, and the eight
-      // lanes whose 16-byte stores go together write different rows, so the swizzle gives them different banks
-      const int h = (warp - 2) / kDecodeWarps;
+      // a team has 128 columns of every stage, or of every second one: a warp decodes eight rows, a lane 32 columns of
+      // one, and the eight lanes whose 16-byte stores go together write different rows, so the swizzle gives them
+      // different banks
+      const int team = (warp - 2) / kDecodeWarps;
+      const int h = kRows == 2 ? team : 0, turn = kRows == 2 ? 0 : team;
       const int r = (warp - 2) % kDecodeWarps * 8 + (lane & 7), quarter = lane >> 3;
       const int col = (t.row_tile * kRows + h) * kTileRows + quarter * 32;
       uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (quarter >> 1) * (kGradStageRows * 128) + r * 128;
       PieceWalk<FMT> walk;
-      int block = from % blocks;  // of the next loads
+      int block = (from + turn) % blocks;  // of the next loads
       walk.begin(p, t.expert, block, r, col);
       const auto load_next = [&]() {
         const Piece piece = walk.load();
-        walk.next();
-        if (++block == blocks) {  // the next term
-          block = 0;
-          walk.begin(p, t.expert, 0, r, col);
+#pragma unroll
+        for (int j = 0; j < S::kTurns; ++j) {
+          walk.next();
+          if (++block == blocks) {  // the next term
+            block = 0;
+            walk.begin(p, t.expert, 0, r, col);
+          }
         }
         return piece;
       };
-      Piece soon = load_next(), later = load_next();  // the next stage's, the one after's
+      Piece soon = load_next(), later = load_next();  // this team's next stage's, the one after's
       Ring<S::kStages> ring;
+      if (turn == 1) ring.next();
       bool ok = true;
-      for (int i = from; i < to; ++i, ring.next()) {
+      for (int i = from + turn; i < to; i += S::kTurns) {
         const Piece now = soon;
         soon = later;
-        if (i + 2 < to) later = load_next();
+        if (i + 2 * S::kTurns < to) later = load_next();
         if (i - from >= S::kStages) {
           ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad));
           if (!ok) break;
@@ -273,6 +279,8 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, 
         pm::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) pm::mbar_arrive(&ready[ring.slot]);
+#pragma unroll
+        for (int j = 0; j < S::kTurns; ++j) ring.next();
       }
       ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(done, 0, pm::kStatusTimeoutMma));
       pm::tc_fence_after();
@@ -285,12 +293,10 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, GradShape<BN, 
           uint8_t* mine = smem + (warp - 2) * 2048;
           TileAt part = t;
           part.row_tile = t.row_tile * kRows + h;
-          if constexpr (BN >= 64) {  // two warps share each quarter of the lanes: halves of the tokens
-            const int half = (warp - 2) % kDecodeWarps >= 4;
-            store_tile<DT>(tmem + h * BN, p.dx, part, p.cols, alpha, half * (BN / 2), (half + 1) * (BN / 2), mine, p.vec != 0);
-          } else if (warp < 6) {
-            store_tile<DT>(tmem, p.dx, part, p.cols, alpha, 0, BN, mine, p.vec != 0);
-          }
+          // 4 / kRows warps for each quarter of the lanes: a share of the tokens each
+          constexpr int kShare = BN * kRows / 4 < 32 ? 32 : BN * kRows / 4;
+          const int share = (kRows == 2 ? (warp - 2) % kDecodeWarps : warp - 2) / 4;
+          store_tile<DT>(tmem + h * BN, p.dx, part, p.cols, alpha, share * kShare, min((share + 1) * kShare, BN), mine, p.vec != 0);
         }
       }
       pm::tc_fence_before();
