@@ -179,7 +179,7 @@ __device__ __forceinline__ TokenBlock<DT> load_tokens(const LinearArgs& p, const
 // A warp quantizes them into the operand's swizzled rows and its scale tiles.
 template <int DT, int FMT>
 __device__ __forceinline__ void quantize_tokens(const LinearArgs& p, const TileAt& t, const TokenBlock<DT>& b, int stage, int row0,
-                                                uint8_t* codes, uint8_t* scales, bool two, float g, float inv_g) {
+                                                uint8_t* codes, uint8_t* scales, const Second& second) {
   const int lane = threadIdx.x & 31, unit = lane & 15;
   const bool in_cols = stage * kStageCols + unit * kUnit < p.cols;
 #pragma unroll
@@ -188,7 +188,7 @@ __device__ __forceinline__ void quantize_tokens(const LinearArgs& p, const TileA
     const int r = row0 + 2 * u + (lane >> 4);
     float v[16];
     to_floats(b.raw[u], v);
-    const Coded c = quantize16<FMT>(v, p.scale_mode, two, g, inv_g);
+    const Coded c = quantize16<FMT>(v, p.scale_mode, second);
     const uint32_t word = gather_scales<FMT>(in_cols ? c.byte : 0u);
     if (r < t.count) {
       *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
     }
   } else if constexpr (kFused) {
     const bool two = FMT == kNV && p.x_second != nullptr;
-    const float g = two ? *p.x_second : 1.0f, inv_g = __fdiv_rn(1.0f, g);
+    const Second second = second_of(two, two ? *p.x_second : 1.0f);
     Ring<S::kStages> ring;
     int it = 0;
     bool ok = true;
@@ -475,9 +475,9 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         uint8_t* at = smem + ring.slot * S::kStage;
-        quantize_tokens<DT, FMT>(p, t, now, i, 0, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
+        quantize_tokens<DT, FMT>(p, t, now, i, 0, at + S::kW, at + S::kW + S::kX + S::kSW, second);
         for (int r0 = 8; r0 < t.count; r0 += 8)
-          quantize_tokens<DT, FMT>(p, t, load_tokens<DT>(p, t, i, r0), i, r0, at + S::kW, at + S::kW + S::kX + S::kSW, two, g, inv_g);
+          quantize_tokens<DT, FMT>(p, t, load_tokens<DT>(p, t, i, r0), i, r0, at + S::kW, at + S::kW + S::kX + S::kSW, second);
         pm::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) pm::mbar_arrive(&full[ring.slot]);

@@ -179,10 +179,26 @@ __device__ __forceinline__ uint32_t amax16(const float (&v)[16]) {
   return __float_as_uint(max3_abs_nan(max3_abs_nan(m, v[14], v[15]), n, n)) & 0x7FFFFFFFu;
 }
 
+// a / b rounded to nearest, from r = 1 / b rounded to nearest: Markstein's
+// theorem ("Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990) makes one residual step exact while nothing under- or
+// overflows. For magnitudes within 2^+-60; three instructions.
+__device__ __forceinline__ float near_quotient(float a, float b, float r) {
+  const float q = __fmul_rn(a, r);
+  return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
+}
+// Whether a magnitude's bits are those of a number within 2^+-60.
+__device__ __forceinline__ bool near_one(uint32_t bits) { return bits - (67u << 23) < (120u << 23); }
+
+__device__ __forceinline__ float sixth(uint32_t amax) {
+  const float a = __uint_as_float(amax);
+  return near_one(amax) ? near_quotient(a, 6.0f, 1.0f / 6.0f) : __fdiv_rn(a, 6.0f);
+}
+
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax, int mode) {
   if (amax > 0x7F800000u) return 255u;
   uint32_t bits = amax;
-  if (mode == kRceil) bits = __float_as_uint(__fdiv_rn(__uint_as_float(amax), 6.0f));
+  if (mode == kRceil) bits = __float_as_uint(sixth(amax));
   else if (mode == kEven) bits += 1u << 21;
   int e = static_cast<int>(bits >> 23);
   // above a power of two; 2^-127, the least scale, is half the least normal number
@@ -196,11 +212,47 @@ __device__ __forceinline__ float mx_inverse(uint32_t byte) {
   return __uint_as_float(byte >= 254u ? (1u << 22) : (254u - byte) << 23);
 }
 
-__device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax, bool two, float g) {
-  float s = __fdiv_rn(__uint_as_float(amax), 6.0f);
-  if (two) s = __fdiv_rn(s, g);
+// What a lane keeps of a second level for all its blocks.
+struct Second {
+  float g, inv_g;  // 1 without one
+  bool two, near;  // near: g is within 2^+-60
+  float inv_mantissa;  // 1 / (1 + (lane % 8) / 8)
+};
+__device__ __forceinline__ Second second_of(bool two, float g) {
+  Second s;
+  s.two = two;
+  s.g = g;
+  s.inv_g = __fdiv_rn(1.0f, g);
+  s.near = near_one(__float_as_uint(g));
+  s.inv_mantissa = __frcp_rn(1.0f + static_cast<float>(threadIdx.x & 7) * 0.125f);
+  return s;
+}
+
+__device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax, const Second& second) {
+  float s = sixth(amax);
+  if (second.two) s = second.near && near_one(__float_as_uint(s)) ? near_quotient(s, second.g, second.inv_g) : __fdiv_rn(s, second.g);
   if (s != s) return 127u;
   return pm::enc_e4m3(fminf(fmaxf(s, 0.015625f), 448.0f));
+}
+
+// 1 / unit rounded to nearest, of the e4m3 number that a byte from 8 to 126
+// stands for: the reciprocal of its 4-bit significand, from another lane, with
+// the exponent taken off (the whole warp calls).
+__device__ __forceinline__ float inverse_unit(uint32_t byte, const Second& second) {
+  const float m = __shfl_sync(0xFFFFFFFFu, second.inv_mantissa, byte & 7u);
+  return __uint_as_float(__float_as_uint(m) + ((7u - (byte >> 3)) << 23));
+}
+
+// Eight values to codes (nearest, ties to even, saturating), the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float2* q) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(q[0].x), "f"(q[0].y), "f"(q[1].x), "f"(q[1].y), "f"(q[2].x), "f"(q[2].y), "f"(q[3].x), "f"(q[3].y));
+  return w;
 }
 
 // Codes of 16 values (the first in the lowest nibble). kQuotient: v / unit is
@@ -210,16 +262,15 @@ __device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax, bool two, float
 // ulp away from it, and one that is comes out exactly.
 template <bool kQuotient>
 __device__ __forceinline__ uint2 encode16(const float (&v)[16], float mul, float unit) {
-  uint32_t w[2] = {0u, 0u};
+  float2 q[8];
   const float2 m2 = make_float2(mul, mul), u2 = make_float2(-unit, -unit);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 x = make_float2(v[2 * i], v[2 * i + 1]);
-    float2 q = __fmul2_rn(x, m2);
-    if constexpr (kQuotient) q = __ffma2_rn(__ffma2_rn(q, u2, x), m2, q);
-    w[i >> 2] |= pm::enc_e2m1x2(q.x, q.y) << (8 * (i & 3));
+    q[i] = __fmul2_rn(x, m2);
+    if constexpr (kQuotient) q[i] = __ffma2_rn(__ffma2_rn(q[i], u2, x), m2, q[i]);
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint2(e2m1x8(q), e2m1x8(q + 4));
 }
 
 struct Coded {
@@ -229,7 +280,7 @@ struct Coded {
 
 // One lane's 16 values; an MXFP4 block is two neighbouring lanes (the whole warp calls).
 template <int FMT>
-__device__ __forceinline__ Coded quantize16(float (&v)[16], int mode, bool two, float g, float inv_g) {
+__device__ __forceinline__ Coded quantize16(float (&v)[16], int mode, const Second& second) {
   uint32_t m = amax16(v);
   Coded out;
   if constexpr (FMT == kMX) {
@@ -237,16 +288,17 @@ __device__ __forceinline__ Coded quantize16(float (&v)[16], int mode, bool two, 
     out.byte = mx_scale_byte(m, mode);
     out.codes = encode16<false>(v, mx_inverse(out.byte), 0.0f);
   } else {
-    out.byte = nv_scale_byte(m, two, g);
-    const float unit = pm::dec_e4m3(out.byte);
-    if (two) {
-      out.codes = encode16<false>(v, __fdiv_rn(inv_g, unit), 0.0f);
+    out.byte = nv_scale_byte(m, second);
+    const float unit = pm::dec_e4m3(out.byte), inverse = inverse_unit(out.byte, second);
+    if (second.two) {
+      const float mul = second.near ? near_quotient(second.inv_g, unit, inverse) : __fdiv_rn(second.inv_g, unit);
+      out.codes = encode16<false>(v, mul, 0.0f);
     } else {
       if (m >= 0x7F800000u) {  // keep infinities out of the residual: 2^20 saturates as they do
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = fminf(fmaxf(v[i], -1048576.0f), 1048576.0f);
       }
-      out.codes = encode16<true>(v, __fdiv_rn(1.0f, unit), unit);
+      out.codes = encode16<true>(v, inverse, unit);
     }
   }
   return out;
@@ -268,26 +320,29 @@ __device__ __forceinline__ float second_of_amax(uint32_t amax) {
 
 // A warp quantizes R rows (more where a row is short) x 512 columns of matrix e.
 template <int DT, int FMT, int R>
-__device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk, float g, float inv_g) {
+__device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk, const Second& second) {
   constexpr int kLanes = FMT == kMX ? 2 : 1;  // lanes per block
   const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
   const int unit = chunk * 32 + (lane & (per - 1));
   const int step = 32 / per;  // rows side by side in the warp
   const int64_t first = row0 + lane / per;
   const bool in_row = unit < q.units, in_cols = unit * kUnit < q.cols;
+  // rows that exist, and rows that get scales, from this lane's first on
+  const int live = static_cast<int>(min(max(q.rows - first, int64_t{0}), int64_t{R * 32}));
+  const int kept = in_row ? static_cast<int>(min(max(q.rows_padded - first, int64_t{0}), int64_t{R * 32})) : 0;
 
   Raw<DT> raw[R];
+  int64_t from = (e * q.rows + first) * q.x_stride + unit * kUnit;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {
-    const int64_t r = first + u * step;
-    if (in_cols && r < q.rows) {
-      raw[u] = load_unit<DT>(q.x, (e * q.rows + r) * q.x_stride + unit * kUnit, q.vec != 0);
+  for (int u = 0; u < R; ++u, from += step * q.x_stride) {
+    if (in_cols && u * step < live) {
+      raw[u] = load_unit<DT>(q.x, from, q.vec != 0);
     } else {
 #pragma unroll
       for (auto& w : raw[u].w) w = 0u;
     }
   }
-  // the warp's rows' experts, one row a lane, while the values are on their way
+  // where the warp's tokens' scales go, one row a lane, while the values are on their way
   int64_t place = 0;
   if (q.token_tile != 0) {
     const int64_t r = row0 + lane;
@@ -300,34 +355,42 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
       place = first_scale_row(start, x, q.token_tile) +
               static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
     }
+    if (q.ends == nullptr) place = __shfl_sync(0xFFFFFFFFu, place, lane / per);  // this lane's first row's
   }
-  const bool two = FMT == kNV && q.second_mode != kSecondNone;
+  // the rows of a warp are aligned to their number, so in the swizzled layout they follow one another by 16 bytes
   const int c = unit / kLanes;
+  uint8_t* scale = q.swizzled ? q.scale + e * (q.rows_padded >> 7) * q.scale_cols * 512 +
+                                    swizzled_byte(q.token_tile != 0 ? place : first, c, q.scale_cols)
+                              : q.scale + (e * q.rows + first) * q.scale_cols + c;
+  const int64_t scale_step = q.swizzled ? step * 16 : static_cast<int64_t>(step) * q.scale_cols;
+  uint8_t* codes = q.codes + (e * q.rows + first) * q.code_pitch + unit * 8;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {
-    const int64_t r = first + u * step;
+  for (int u = 0; u < R; ++u, scale += scale_step, codes += step * q.code_pitch) {
     float v[16];
     to_floats(raw[u], v);
-    const Coded s = quantize16<FMT>(v, q.scale_mode, two, g, inv_g);
-    const bool live = r < q.rows;
-    const uint32_t byte = live && in_cols ? s.byte : 0u;
+    const Coded s = quantize16<FMT>(v, q.scale_mode, second);
+    const bool value = u * step < live && in_cols;
+    const uint32_t byte = value ? s.byte : 0u;
     const uint32_t word = gather_scales<FMT>(byte);
-    const int64_t srow = q.token_tile != 0 ? __shfl_sync(0xFFFFFFFFu, place, u * step + lane / per) : r;
-    if (!in_row || r >= q.rows_padded || srow < 0) continue;
-    uint8_t* at = q.swizzled ? q.scale + e * (q.rows_padded >> 7) * q.scale_cols * 512 + swizzled_byte(srow, c, q.scale_cols)
-                             : q.scale + (e * q.rows + r) * q.scale_cols + c;
+    uint8_t* at = scale;
+    bool keep = u * step < kept;
+    if (q.ends != nullptr) {
+      const int64_t srow = __shfl_sync(0xFFFFFFFFu, place, u * step + lane / per);
+      keep = keep && srow >= 0;
+      at = q.scale + swizzled_byte(max(srow, int64_t{0}), c, q.scale_cols);
+    }
+    if (!keep) continue;
     if (q.words) {
       if (lane % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(at) = word;
     } else if (lane % kLanes == 0) {
       *at = static_cast<uint8_t>(byte);
     }
-    if (live && (q.pad_codes || in_cols)) {
-      uint8_t* to = q.codes + (e * q.rows + r) * q.code_pitch + unit * 8;
+    if (value || (q.pad_codes && u * step < live)) {
       if (q.pairs) {
-        *reinterpret_cast<uint2*>(to) = s.codes;
+        *reinterpret_cast<uint2*>(codes) = s.codes;
       } else {
-        reinterpret_cast<uint32_t*>(to)[0] = s.codes.x;
-        reinterpret_cast<uint32_t*>(to)[1] = s.codes.y;
+        reinterpret_cast<uint32_t*>(codes)[0] = s.codes.x;
+        reinterpret_cast<uint32_t*>(codes)[1] = s.codes.y;
       }
     }
   }
@@ -342,13 +405,13 @@ __device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
   const int chunk = static_cast<int>(b - rb * chunks);
   const int rows = 32 / lanes_per_row(q.units) * R;  // per warp
   const int64_t row0 = (rb - e * per) * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows;
-  float g = 1.0f, inv_g = 1.0f;
-  if (FMT == kNV && q.second_mode != kSecondNone) {
+  float g = 1.0f;
+  const bool two = FMT == kNV && q.second_mode != kSecondNone;
+  if (two) {
     g = q.second_mode == kSecondGiven ? q.second[e] : second_of_amax(q.amax[e]);
-    inv_g = __fdiv_rn(1.0f, g);
     if (q.second_mode == kSecondCompute && rb == e * per && chunk == 0 && threadIdx.x == 0) q.second[e] = g;
   }
-  quantize_rows<DT, FMT, R>(q, e, row0, chunk, g, inv_g);
+  quantize_rows<DT, FMT, R>(q, e, row0, chunk, second_of(two, g));
 }
 
 template <int DT, int FMT, int R>
@@ -421,9 +484,9 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __g
   __syncthreads();
   const float g = second_of_amax(__reduce_max_sync(0xFFFFFFFFu, part[lane % (kSmallThreads / 32)]));
   if (threadIdx.x == 0) q.second[e] = g;
-  const float inv_g = __fdiv_rn(1.0f, g);
+  const Second second = second_of(true, g);
   for (int i = warp; i < pieces; i += kSmallThreads / 32)
-    quantize_rows<DT, FMT, kQuantRows>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, g, inv_g);
+    quantize_rows<DT, FMT, kQuantRows>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, second);
 }
 
 // ------------------------------------------------------------ back to values
