@@ -119,8 +119,9 @@ int scale_cols(const piper_fp4_matrix& m) {
 
 // Rows that a lane quantizes: several, whose loads are in flight together, once there are blocks for every SM;
 // before that one, as a lane's rows come one after another (777 x 1072: TODO us with 1, TODO with 4).
-int rows_per_lane(const fp4::QuantArgs& q) {
-  return fp4::quant_blocks(q, fp4::kQuantRows) < 2 * sm_count() ? 1 : fp4::kQuantRows;
+int many_rows(int dtype) { return dtype == PIPER_FP4_BF16 ? fp4::quant_rows<fp4::kBF16>() : fp4::quant_rows<fp4::kF32>(); }
+int rows_per_lane(const fp4::QuantArgs& q, int dtype) {
+  return fp4::quant_blocks(q, many_rows(dtype)) < 2 * sm_count() ? 1 : many_rows(dtype);
 }
 
 // Matrices of at most so many values get their second-level scale and their codes in one launch of one block
@@ -336,18 +337,18 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
     q.amax = maxima;
     cudaError_t e = cudaMemsetAsync(maxima, 0, sizeof(uint32_t) * m->batch, s);
     if (e != cudaSuccess) return cuda_fail("cudaMemsetAsync", e);
-    const int64_t blocks = fp4::quant_row_blocks(q, fp4::kQuantRows) * ((q.units + 31) / 32);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 8)), static_cast<unsigned>(m->batch));
+    const int64_t blocks = fp4::quant_row_blocks(q, many_rows(dtype)) * ((q.units + 31) / 32);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 32)), static_cast<unsigned>(m->batch));
     if (dtype == PIPER_FP4_BF16) fp4::amax_kernel<fp4::kBF16><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     else fp4::amax_kernel<fp4::kF32><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     if ((e = launched()) != cudaSuccess) return cuda_fail("amax kernel", e);
   }
-  const int lane_rows = rows_per_lane(q);
+  const int lane_rows = rows_per_lane(q, dtype);
   const int64_t blocks = fp4::quant_blocks(q, lane_rows);
   FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 quantisation: too many values for one call.");
 #define CALL(D, F)                                                                                                \
   if (lane_rows == 1) fp4::quantize_kernel<D, F, 1><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q); \
-  else fp4::quantize_kernel<D, F, fp4::kQuantRows><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q)
+  else fp4::quantize_kernel<D, F, fp4::quant_rows<D>()><<<static_cast<unsigned>(blocks), fp4::kQuantThreads, 0, s>>>(q)
   FP4_DISPATCH(dtype, m->format, CALL);
 #undef CALL
   const cudaError_t e = launched();
@@ -371,7 +372,7 @@ int piper_fp4_dequantize(const piper_fp4_matrix* m, void* y, int32_t dtype, void
   d.scale_cols = scale_cols(*m);
   d.vec = aligned(m->codes, 8) && aligned(y, 32);
   const int units = d.cols / fp4::kUnit;
-  const int64_t block_rows = fp4::kQuantThreads / fp4::lanes_per_row(units) * fp4::kQuantRows;
+  const int64_t block_rows = fp4::kQuantThreads / fp4::lanes_per_row(units) * fp4::kDequantRows;
   const int64_t blocks = m->batch * ((m->rows + block_rows - 1) / block_rows) * ((units + 31) / 32);
   FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 dequantisation: too many values for one call.");
 #define CALL(D, F) \
@@ -462,7 +463,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     q.token_tile = p.bn;
     q.ends = ends;
     q.experts = static_cast<int32_t>(w->batch);
-    lane_rows = rows_per_lane(q);
+    lane_rows = rows_per_lane(q, dtype);
     token_blocks = fp4::quant_blocks(q, lane_rows);
   }
   a.x_scale = q.scale;
@@ -486,7 +487,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
 #define CALL(D, F)                                                                                            \
   if (lane_rows == 1) fp4::prepare_kernel<D, F, 1><<<grid, fp4::kQuantThreads, 0, s>>>(q, r, tokens_grid);     \
-  else fp4::prepare_kernel<D, F, fp4::kQuantRows><<<grid, fp4::kQuantThreads, 0, s>>>(q, r, tokens_grid)
+  else fp4::prepare_kernel<D, F, fp4::quant_rows<D>()><<<grid, fp4::kQuantThreads, 0, s>>>(q, r, tokens_grid)
     FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
     e = launched();

@@ -28,8 +28,14 @@ enum : int { kFloor = 0, kRceil = 1, kCeil = 2, kEven = 3 };
 enum : int { kSecondNone = 0, kSecondGiven = 1, kSecondCompute = 2 };
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantRows = 4;   // rows in flight per lane where there are many
-constexpr int kUnit = 16;       // values per lane and row
+// Rows in flight per lane where there are many (12288 x 3072 bf16 with 4, 2, 1: 23, 26, 31 us; 4096 x 14336 fp32
+// two-level: 62, 52, 53), and the blocks per SM that registers leave room for.
+template <int DT>
+__host__ __device__ constexpr int quant_rows() { return DT == kBF16 ? 4 : 2; }
+template <int DT>
+constexpr int quant_ctas() { return DT == kBF16 ? 4 : 2; }
+constexpr int kDequantRows = 4;
+constexpr int kUnit = 16;  // values per lane and row
 constexpr int kSmallThreads = 512;
 
 template <int FMT>
@@ -415,7 +421,7 @@ __device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
 }
 
 template <int DT, int FMT, int R>
-__global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantArgs q) {
+__global__ void __launch_bounds__(kQuantThreads, quant_ctas<DT>()) quantize_kernel(const __grid_constant__ QuantArgs q) {
   quantize_block<DT, FMT, R>(q, q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x);
 }
 
@@ -426,9 +432,9 @@ __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int
   const int unit = chunk * 32 + (lane & (per - 1));
   const int step = 32 / per;
   const int64_t first = row0 + lane / per;
-  Raw<DT> raw[kQuantRows];
+  Raw<DT> raw[quant_rows<DT>()];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < quant_rows<DT>(); ++u) {
     const int64_t r = first + u * step;
     if (unit * kUnit < q.cols && r < q.rows) {
       raw[u] = load_unit<DT>(q.x, (e * q.rows + r) * q.x_stride + unit * kUnit, q.vec != 0);
@@ -439,7 +445,7 @@ __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int
   }
   uint32_t m = 0u;
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < quant_rows<DT>(); ++u) {
     float v[16];
     to_floats(raw[u], v);
     m = max(m, amax16(v));
@@ -450,8 +456,8 @@ __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int
 // max|x| of each matrix as integer bits (order does not matter to a maximum).
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) amax_kernel(const __grid_constant__ QuantArgs q, uint32_t* amax) {
-  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * kQuantRows;
-  const int64_t blocks = quant_row_blocks(q, kQuantRows) * chunks;
+  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * quant_rows<DT>();
+  const int64_t blocks = quant_row_blocks(q, quant_rows<DT>()) * chunks;
   uint32_t m = 0u;
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
     const int64_t rb = b / chunks;
@@ -474,7 +480,7 @@ template <int DT, int FMT>
 __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __grid_constant__ QuantArgs q) {
   __shared__ uint32_t part[kSmallThreads / 32];
   const int64_t e = blockIdx.x;
-  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * kQuantRows;
+  const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * quant_rows<DT>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pieces = static_cast<int>((q.rows_padded + rows - 1) / rows) * chunks;
   uint32_t m = 0u;
@@ -486,7 +492,7 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __g
   if (threadIdx.x == 0) q.second[e] = g;
   const Second second = second_of(true, g);
   for (int i = warp; i < pieces; i += kSmallThreads / 32)
-    quantize_rows<DT, FMT, kQuantRows>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, second);
+    quantize_rows<DT, FMT, quant_rows<DT>()>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, second);
 }
 
 // ------------------------------------------------------------ back to values
@@ -529,20 +535,20 @@ template <int DT, int FMT>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_constant__ DequantArgs d) {
   constexpr int kLanes = FMT == kMX ? 2 : 1;
   const int units = d.cols / kUnit, per = lanes_per_row(units), chunks = (units + 31) / 32, step = 32 / per;
-  const int block_rows = kQuantThreads / per * kQuantRows;
+  const int block_rows = kQuantThreads / per * kDequantRows;
   const int64_t row_blocks = (d.rows + block_rows - 1) / block_rows;
   const int64_t rb = blockIdx.x / chunks, e = d.batch == 1 ? 0 : rb / row_blocks;
   const int lane = threadIdx.x & 31;
   const int unit = static_cast<int>(blockIdx.x - rb * chunks) * 32 + (lane & (per - 1));
-  const int64_t first = (rb - e * row_blocks) * block_rows + (threadIdx.x >> 5) * (step * kQuantRows) + lane / per;
+  const int64_t first = (rb - e * row_blocks) * block_rows + (threadIdx.x >> 5) * (step * kDequantRows) + lane / per;
   const uint8_t* scales = d.swizzled ? d.scale + e * ((d.rows + 127) >> 7) * d.scale_cols * 512 : d.scale + e * d.rows * d.scale_cols;
   const float g = d.second != nullptr ? d.second[e] : 1.0f;
   if (unit >= units) return;
   const int c = unit / kLanes;
-  uint2 codes[kQuantRows];
-  uint32_t byte[kQuantRows];
+  uint2 codes[kDequantRows];
+  uint32_t byte[kDequantRows];
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kDequantRows; ++u) {
     const int64_t r = first + u * step;
     codes[u] = make_uint2(0u, 0u);
     byte[u] = 0u;
@@ -561,7 +567,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
     }
   }
 #pragma unroll
-  for (int u = 0; u < kQuantRows; ++u) {
+  for (int u = 0; u < kDequantRows; ++u) {
     const int64_t r = first + u * step;
     if (r >= d.rows) break;
     const __nv_bfloat162 s = __float2bfloat162_rn(scale_value<FMT>(byte[u]));
@@ -634,7 +640,7 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
 // What a product needs ahead of it, in one launch: blocks below
 // `token_blocks` quantize tokens, the others lay codes out.
 template <int DT, int FMT, int R>
-__global__ void __launch_bounds__(kQuantThreads)
+__global__ void __launch_bounds__(kQuantThreads, quant_ctas<DT>())
     prepare_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs p, uint32_t token_blocks) {
   grid_launch_dependents();
   if (blockIdx.x < token_blocks) quantize_block<DT, FMT, R>(q, blockIdx.x);
