@@ -473,6 +473,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     r.codes_out = ws + p.w_codes;
     r.row_bytes = w->cols / 2;
     r.pitch = p.w_code_pitch;
+    r.aligned = aligned(w->codes, 8);
     r.pieces = w->batch * w->rows * (p.w_code_pitch / 16);
   }
   const int64_t blocks = token_blocks + (r.pieces + fp4::kQuantThreads - 1) / fp4::kQuantThreads;

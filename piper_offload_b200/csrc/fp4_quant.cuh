@@ -624,17 +624,23 @@ struct RepackArgs {
   int64_t row_bytes;
   int64_t pitch;       // bytes between rows of codes_out (a multiple of 16)
   int64_t pieces;      // 16-byte pieces of codes_out
+  int32_t aligned;     // rows start on 8-byte boundaries
 };
 
 __device__ __forceinline__ void repack(const RepackArgs& p, int64_t i) {
   if (i >= p.pieces) return;
   const int64_t per = p.pitch >> 4;
   const int64_t row = i / per, at = (i - row * per) * 16;
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (at + j < p.row_bytes) w[j >> 2] |= static_cast<uint32_t>(p.codes[row * p.row_bytes + at + j]) << (8 * (j & 3));
-  *reinterpret_cast<uint4*>(p.codes_out + row * p.pitch + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  const uint8_t* from = p.codes + row * p.row_bytes + at;
+  const int bytes = static_cast<int>(min(p.row_bytes - at, int64_t{16}));  // 16 or 8
+  uint64_t w[2] = {0u, 0u};
+  if (p.aligned) {
+    w[0] = *reinterpret_cast<const uint64_t*>(from);
+    if (bytes == 16) w[1] = *reinterpret_cast<const uint64_t*>(from + 8);
+  } else {
+    for (int j = 0; j < bytes; ++j) w[j >> 3] |= static_cast<uint64_t>(from[j]) << (8 * (j & 7));
+  }
+  *reinterpret_cast<ulonglong2*>(p.codes_out + row * p.pitch + at) = make_ulonglong2(w[0], w[1]);
 }
 
 // What a product needs ahead of it, in one launch: blocks below
