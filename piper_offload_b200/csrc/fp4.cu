@@ -118,7 +118,7 @@ int scale_cols(const piper_fp4_matrix& m) {
 }
 
 // Rows that a lane quantizes: several, whose loads are in flight together, once there are blocks for every SM;
-// before that one, as a lane's rows come one after another (777 x 1072: TODO us with 1, TODO with 4).
+// before that one, as a lane's rows come one after another (24 x 4096: 2.3 us with 1, 3.6 with 4).
 int many_rows(int dtype) { return dtype == PIPER_FP4_BF16 ? fp4::quant_rows<fp4::kBF16>() : fp4::quant_rows<fp4::kF32>(); }
 int rows_per_lane(const fp4::QuantArgs& q, int dtype) {
   return fp4::quant_blocks(q, many_rows(dtype)) < 2 * sm_count() ? 1 : many_rows(dtype);
@@ -145,17 +145,47 @@ constexpr int64_t kSmallMatrix = 65536;
 struct LinearPlan {
   bool fused;       // tokens are quantized by the product itself
   bool move_codes;
-  int bn;           // tokens per tile
+  int bn, split;    // tokens per tile, blocks per tile
   int64_t k_padded; // columns up to a whole scale tile
   int64_t x_codes, x_scale, w_codes, total;  // byte offsets
   int64_t w_code_pitch, scale_tiles, scale_rows;
 };
 
+// Tokens per tile and blocks of a cluster that share a tile's stages, by a
+// rough account in cycles: a stage takes `stage`, leaving sums and adding them
+// up 2500 and 30 for each token of the tile, and every wave of tiles 2000.
+struct TilePlan {
+  int bn, split;
+  double cycles;
+};
+TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t tile_tokens, bool can_split) {
+  TilePlan best{bn, 1, 0.0};
+  for (int split = 1; split <= (can_split ? fp4::kMaxSplit : 1); split *= 2) {
+    if (split > 1 && (items * split > sm_count() || stages < 2 * split)) break;
+    const int64_t waves = (items * split + sm_count() - 1) / sm_count();
+    double cycles = static_cast<double>(waves) * (static_cast<double>((stages + split - 1) / split) * stage + 2000.0);
+    if (split > 1) cycles += 2500.0 + 30.0 * static_cast<double>(tile_tokens);
+    if (split == 1 || cycles < best.cycles) best = {bn, split, cycles};
+  }
+  return best;
+}
+
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
-  const int64_t per_expert = tokens / w.batch;
-  p.fused = per_expert <= 8;
-  p.bn = per_expert <= 32 ? 32 : per_expert <= 512 ? 128 : 192;
+  const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
+  p.fused = tokens / w.batch <= 8;
+  // 333 tokens x 1000 x 2080: 10.4 us in tiles of 32, 11.4 of 128
+  TilePlan best{};
+  for (const int bn : {32, 128, 192}) {
+    if (p.fused && bn > 32) break;
+    const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
+    const int64_t items = std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + 127) / 128);
+    const TilePlan t = plan_tile(bn, items, (w.cols + fp4::kStageCols - 1) / fp4::kStageCols,
+                                 330.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1);
+    if (best.bn == 0 || t.cycles < best.cycles) best = t;
+  }
+  p.bn = best.bn;
+  p.split = best.split;
   const int tile = block_of(w) * 4;
   p.scale_tiles = (w.cols + tile - 1) / tile;
   p.k_padded = p.scale_tiles * tile;
@@ -186,30 +216,13 @@ int64_t token_tiles(const fp4::Groups& g, int bn) {
   return g.ends == nullptr ? (g.tokens + bn - 1) / bn : g.tokens / bn + std::min<int64_t>(g.experts + 1, g.tokens);
 }
 
-// Blocks of a cluster that share a tile's K: where the tiles leave SMs idle, as
-// many as shorten the run by a rough account in cycles (a stage takes about
-// 450; leaving and adding up sums 2500 and 30 for each token of the tile).
-template <class S>
-int split_of(int64_t items, int stages, int tokens) {
-  int best = 1;
-  double least = 450.0 * stages;
-  for (int split = 2; S::kCanSplit && split <= fp4::kMaxSplit && items * split <= sm_count() && stages >= 2 * split; split *= 2) {
-    const double cycles = 450.0 * ((stages + split - 1) / split) + 2500.0 + 30.0 * tokens;
-    if (cycles < least) {
-      least = cycles;
-      best = split;
-    }
-  }
-  return best;
-}
-
 template <int DT, int FMT, int BN, bool kFused>
 cudaError_t launch_linear(fp4::LinearArgs& args, int64_t items, cudaStream_t stream) {
   using S = fp4::LinearShape<FMT, BN, kFused>;
   auto kernel = fp4::linear_kernel<DT, FMT, BN, kFused>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  args.split = split_of<S>(items, (args.k_steps + 3) / 4, static_cast<int>(std::min<int64_t>(args.groups.tokens, BN)));
+  static_assert(S::kCanSplit, "the plan may split any tile");
   cudaLaunchAttribute attributes[2] = {};
   // may start while the launch before it still quantizes; the kernel waits where it needs that
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -269,7 +282,7 @@ cudaError_t launch_grad(fp4::GradArgs& args, int64_t items, cudaStream_t stream)
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   const int stages = (args.rows + fp4::kGradStageRows - 1) / fp4::kGradStageRows * args.terms;
-  args.split = split_of<S>(items, stages, static_cast<int>(std::min<int64_t>(args.groups.tokens, BN)));
+  args.split = plan_tile(BN, items, stages, 600.0, std::min<int64_t>(args.groups.tokens, BN), S::kCanSplit && args.groups.ends == nullptr).split;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
   attribute.val.clusterDim.x = static_cast<unsigned>(args.split);
@@ -422,6 +435,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
   a.cols = static_cast<int32_t>(w->cols);
   a.k_steps = static_cast<int32_t>((w->cols + 63) / 64);
   a.scale_tiles = static_cast<int32_t>(p.scale_tiles);
+  a.split = p.split;
   a.early = !p.move_codes;
   a.vec = aligned(y, 16) && w->rows % 8 == 0;
   a.x_vec = x_vec;
