@@ -43,6 +43,9 @@ enum { PIPER_FP4_FLOOR = 0, PIPER_FP4_RCEIL = 1, PIPER_FP4_CEIL = 2, PIPER_FP4_E
  * as max(max|x| / 2688, 2^-23) of each matrix of the batch and written there. */
 enum { PIPER_FP4_SECOND_NONE = 0, PIPER_FP4_SECOND_GIVEN = 1, PIPER_FP4_SECOND_COMPUTE = 2 };
 
+/* Matrices of at most so many values need no room for maxima (piper_fp4_quantize). */
+enum { PIPER_FP4_SMALL_MATRIX = 65536 };
+
 /* A packed matrix, or `batch` of them one after another (experts). */
 typedef struct piper_fp4_matrix {
   void* codes;    /* (batch, rows, cols / 2) */
@@ -56,7 +59,7 @@ typedef struct piper_fp4_matrix {
 /* Quantises x (batch * rows rows of `cols` values, `x_stride` values apart)
  * into m's buffers. Swizzle padding is zeroed. `maxima`: scratch of `batch`
  * words when second_mode is PIPER_FP4_SECOND_COMPUTE and a matrix has more
- * than 65536 values; else it is not used. */
+ * than PIPER_FP4_SMALL_MATRIX values; else it is not used. */
 int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_stride, int32_t dtype, int32_t scale_mode,
                        int32_t second_mode, uint32_t* maxima, void* stream);
 

@@ -10,6 +10,7 @@ import ctypes
 import os
 import threading
 from pathlib import Path
+from typing import Any
 
 import torch
 
@@ -24,8 +25,7 @@ DT_F32 = 2
 SECOND_NONE = 0
 SECOND_GIVEN = 1
 SECOND_COMPUTE = 2
-# Matrices of at most so many values need no room for the maxima (include/piper_fp4.h).
-SMALL_MATRIX = 65536
+SMALL_MATRIX = 65536  # PIPER_FP4_SMALL_MATRIX
 
 EXPORTED_SYMBOLS = (
     "piper_fp4_quantize",
@@ -95,6 +95,25 @@ def load() -> ctypes.CDLL:
         lib.piper_fp4_launches.restype = ctypes.c_uint64
         _lib = lib
         return lib
+
+
+_calls = None
+
+
+def calls() -> Any:
+    """The compiled calls (``csrc/fp4_calls.cpp``), bound to the library's entry points. Loads both once."""
+    global _calls
+    if _calls is None:
+        lib = load()
+        try:
+            from . import _fp4_calls as module
+        except ImportError as exc:
+            raise RuntimeError("the FP4 operators' compiled calls are missing or do not fit this torch; build them with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`.") from exc
+        module.bind(getattr(torch, "float4_e2m1fn_x2", None),
+                    *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTED_SYMBOLS[:6]))
+        _calls = module
+    return _calls
 
 
 def check(rc: int) -> None:

@@ -1,4 +1,4 @@
-"""Build ``libpiper_merge.so`` and ``libpiper_fp4.so`` in-tree with nvcc for sm_100a.
+"""Build ``libpiper_merge.so`` and ``libpiper_fp4.so`` in-tree with nvcc for sm_100a, and the latter's calls with g++.
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
 ``__graft_entry__.build()``). A library newer than every source file of its
@@ -10,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -23,6 +24,9 @@ FP4_DEPS = FP4_SOURCES + [
     ROOT / "include" / "piper_fp4.h",
 ]
 FP4_OUT = PKG / "libpiper_fp4.so"
+CALLS_SOURCES = [PKG / "csrc" / "fp4_calls.cpp"]
+CALLS_DEPS = CALLS_SOURCES + [ROOT / "include" / "piper_fp4.h"]
+CALLS_OUT = PKG / "_fp4_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -71,10 +75,31 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 def build_fp4(force: bool = False, verbose: bool = False) -> Path:
     if force or not up_to_date(FP4_OUT, FP4_DEPS):
         _compile(FP4_OUT, FP4_SOURCES, verbose)
+    build_calls(force, verbose)
     return FP4_OUT
+
+
+def build_calls(force: bool = False, verbose: bool = False) -> Path:
+    """The operators' calls from Python: host code against this interpreter's torch."""
+    if force or not up_to_date(CALLS_OUT, CALLS_DEPS):
+        import torch
+
+        base = Path(torch.__file__).resolve().parent
+        tmp = CALLS_OUT.with_suffix(".so.tmp")
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *(f"-I{d}" for d in (base / "include", base / "include" / "torch" / "csrc" / "api" / "include",
+                                    Path(nvcc()).resolve().parents[1] / "include", sysconfig.get_paths()["include"])),
+               "-o", str(tmp), *map(str, CALLS_SOURCES), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True, cwd=str(ROOT))
+        os.replace(tmp, CALLS_OUT)
+    return CALLS_OUT
 
 
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(OUT)
     print(FP4_OUT)
+    print(CALLS_OUT)

@@ -24,7 +24,9 @@ of the tokens.
 
 All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
 take workspaces from PyTorch's caching allocator on it, do not synchronise,
-and raise ``ValueError`` for arguments that they do not take.
+and raise ``ValueError`` for arguments that they do not take. Calls with plain
+arguments are made by compiled code (``csrc/fp4_calls.cpp``); what it declines
+takes the path written out here, to the same kernels.
 """
 
 from __future__ import annotations
@@ -137,7 +139,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 # ------------------------------------------------------------------ quantisation
 def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torch.Tensor | None,
-              second_mode: int) -> tuple[torch.Tensor, torch.Tensor]:
+              second_mode: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    done = nat.calls().quantize(x, fmt, mode, swizzled, second_mode)
+    if done is not None:
+        return done
     block = 32 if fmt == nat.FMT_MX else 16
     if not x.is_cuda:
         raise ValueError("FP4 quantisation requires CUDA tensors.")
@@ -154,6 +159,8 @@ def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torc
     shape = (K.mx_expected_scale_shape if fmt == nat.FMT_MX else K.nvfp4_expected_scale_shape)(rows, cols, swizzled=swizzled)
     codes = x.new_empty((*lead, rows, cols // 2), dtype=torch.uint8)
     scale = x.new_empty((*lead, *shape), dtype=torch.uint8 if fmt == nat.FMT_MX else torch.float8_e4m3fn)
+    if second_mode == nat.SECOND_COMPUTE:
+        second = x.new_empty(lead[0] if lead else 1, dtype=torch.float32)
     m = nat.Matrix(codes.data_ptr(), scale.data_ptr(), None if second is None else second.data_ptr(),
                    lead[0] if lead else 1, rows, cols, fmt, swizzled)
     maxima = None
@@ -161,7 +168,7 @@ def _quantize(x: torch.Tensor, fmt: int, mode: int, swizzled: bool, second: torc
         maxima = x.new_empty(m.batch, dtype=torch.int32)
     _call(nat.load().piper_fp4_quantize, x.device, ctypes.byref(m), x2.data_ptr(), x2.stride(0), dt, mode, second_mode,
           None if maxima is None else maxima.data_ptr())
-    return codes, scale
+    return codes, scale, second
 
 
 def quantize_mxfp4(x: torch.Tensor, *, scaling_mode: str | int = "floor", swizzled: bool = False) -> MXWeight | MXExperts:
@@ -174,7 +181,7 @@ def quantize_mxfp4(x: torch.Tensor, *, scaling_mode: str | int = "floor", swizzl
         raise ValueError(f"Unsupported MX scaling mode {scaling_mode!r}.")
     if _FP4 is None:
         raise ValueError("MXFP4 weights need torch.float4_e2m1fn_x2.")
-    codes, scale = _quantize(x, nat.FMT_MX, K._MX_SCALING_MODES[name], swizzled, None, nat.SECOND_NONE)
+    codes, scale, _ = _quantize(x, nat.FMT_MX, K._MX_SCALING_MODES[name], swizzled, None, nat.SECOND_NONE)
     kind = MXExperts if x.ndim == 3 else MXWeight
     return kind(codes, scale, _FP4, orig_dtype=x.dtype, is_swizzled_scales=swizzled,
                 act_quant_kwargs=MXActQuantKwargs(MXScalingMode(name)))
@@ -196,15 +203,18 @@ def quantize_nvfp4(x: torch.Tensor, *, two_level: bool = True, per_tensor_scale:
                 or per_tensor_scale.device != x.device):
             raise ValueError("NVFP4 second-level scales are one float32 value per matrix on its device.")
         second, second_mode = per_tensor_scale.detach().reshape(batch).contiguous(), nat.SECOND_GIVEN
-    elif two_level and x.is_cuda:
-        second, second_mode = x.new_empty(batch, dtype=torch.float32), nat.SECOND_COMPUTE
-    codes, scale = _quantize(x, nat.FMT_NV, 0, swizzled, second, second_mode)
+    elif two_level:
+        second_mode = nat.SECOND_COMPUTE
+    codes, scale, second = _quantize(x, nat.FMT_NV, 0, swizzled, second, second_mode)
     kind = NVFP4Experts if x.ndim == 3 else NVFP4Weight
     return kind(codes, scale, second, orig_dtype=x.dtype, is_swizzled_scales=swizzled)
 
 
 def dequantize_fp4(weight: Any, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values of a packed weight or stack, rounded once to ``dtype`` (default: the weight's original type)."""
+    done = nat.calls().dequantize(weight, weight.qdata.ndim, dtype)
+    if done is not None:
+        return done
     m, _, q = _matrix(weight)
     y = q.new_empty((*q.shape[:-1], m.cols), dtype=dtype or weight.orig_dtype)
     _call(nat.load().piper_fp4_dequantize, q.device, ctypes.byref(m), y.data_ptr(), _dtype(y, "dequantisation"))
@@ -220,6 +230,9 @@ def _check_ends(ends: torch.Tensor, batch: int, device: torch.device) -> None:
 
 
 def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: torch.Tensor | None) -> torch.Tensor:
+    done = nat.calls().linear(x, weight, ends, act_scale)
+    if done is not None:
+        return done
     m, mode, q = _matrix(weight)
     device = q.device
     if x.device != device:
@@ -245,6 +258,9 @@ def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: 
 
 
 def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> torch.Tensor:
+    done = nat.calls().grad_input(grad, weight, ends)
+    if done is not None:
+        return done
     m, _, q = _matrix(weight)
     device = q.device
     if grad.device != device:

@@ -500,6 +500,35 @@ def test_repeats_are_bitwise_equal(tokens, cuda_device):
         assert torch.equal(fp4.linear_fp4(x, w), y) and torch.equal(fp4.linear_fp4_grad_input(dy, w), dx)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_compiled_calls_and_the_written_out_path_agree(fmt, cuda_device, monkeypatch):
+    w, _ = make_weight(fmt, 136, 192, cuda_device, second=0.5 if fmt == "nvfp4" else None)
+    stack, _ = make_weight(fmt, 136, 192, cuda_device, swizzled=False, experts=3)
+    x = to_torch(rng(61).standard_normal((50, 192)), torch.bfloat16, cuda_device)
+    dy = to_torch(rng(62).standard_normal((50, 136)), torch.float32, cuda_device)
+    ends = torch.tensor([20, 20, 45], dtype=torch.int32, device=cuda_device)
+
+    def results():
+        packed = [fp4.quantize_mxfp4(x, scaling_mode="even", swizzled=1)] if fmt == "mxfp4" else [
+            fp4.quantize_nvfp4(x), fp4.quantize_nvfp4(x.repeat(8, 8)), fp4.quantize_nvfp4(x, two_level=False, swizzled=True)]
+        out = [t for p in packed for t in (p.qdata, p.scale.view(torch.uint8), fp4.dequantize_fp4(p, torch.float32))]
+        out += [p.per_tensor_scale for p in packed if fmt == "nvfp4" and p.per_tensor_scale is not None]
+        return out + [fp4.dequantize_fp4(stack), fp4.linear_fp4(x, w), fp4.linear_fp4(x[:3].float(), w),
+                      fp4.grouped_linear_fp4(x, stack, ends), fp4.linear_fp4_grad_input(dy, w),
+                      fp4.grouped_linear_fp4_grad_input(dy.bfloat16(), stack, ends)]
+
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    fast = results()
+    monkeypatch.setattr(nat, "calls", lambda: Declines())
+    slow = results()
+    assert len(fast) == len(slow)
+    for a, b in zip(fast, slow):
+        assert a.dtype is b.dtype and torch.equal(a, b)
+
+
 def test_launches_are_counted(cuda_device):
     w, _ = make_weight("mxfp4", 128, 128, cuda_device)
     x = torch.ones((4, 128), dtype=torch.bfloat16, device=cuda_device)
