@@ -356,6 +356,7 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
     if ((e = launched()) != cudaSuccess) return cuda_fail("amax kernel", e);
   }
   const int lane_rows = rows_per_lane(q, dtype);
+  q.row_blocks = static_cast<int32_t>(fp4::quant_row_blocks(q, lane_rows));
   const int64_t blocks = fp4::quant_blocks(q, lane_rows);
   FP4_REQUIRE(blocks < (int64_t{1} << 31), "FP4 quantisation: too many values for one call.");
 #define CALL(D, F)                                                                                                \
@@ -477,6 +478,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     q.ends = ends;
     q.experts = static_cast<int32_t>(w->batch);
     lane_rows = rows_per_lane(q, dtype);
+    q.row_blocks = static_cast<int32_t>(fp4::quant_row_blocks(q, lane_rows));
     token_blocks = fp4::quant_blocks(q, lane_rows);
   }
   a.x_scale = q.scale;

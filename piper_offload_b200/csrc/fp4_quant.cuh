@@ -88,6 +88,7 @@ struct QuantArgs {
   int64_t batch;
   int32_t cols;
   int32_t units;         // units of 16 columns per row that are walked (padding included)
+  int32_t row_blocks;    // quant_row_blocks of the launch
   int32_t vec;           // rows of x start on 32-byte boundaries
   uint8_t* codes;
   int64_t code_pitch;    // bytes between rows
@@ -110,13 +111,14 @@ struct QuantArgs {
 
 // Lanes that share a row: 32, or fewer (at least a tile of scales) for short rows.
 __host__ __device__ __forceinline__ int lanes_per_row(int units) { return units > 16 ? 32 : units > 8 ? 16 : 8; }
-// Blocks of kQuantThreads threads that a walk takes.
+// Blocks of kQuantThreads threads that a walk takes: by rows of one matrix, by chunks of 512 columns, in all.
 __host__ __device__ __forceinline__ int64_t quant_row_blocks(const QuantArgs& q, int rows_per_lane) {
   const int rows = kQuantThreads / lanes_per_row(q.units) * rows_per_lane;
   return (q.rows_padded + rows - 1) / rows;
 }
+__host__ __device__ __forceinline__ int quant_chunks(const QuantArgs& q) { return (q.units + 31) / 32; }
 __host__ __device__ __forceinline__ int64_t quant_blocks(const QuantArgs& q, int rows_per_lane) {
-  return q.batch * quant_row_blocks(q, rows_per_lane) * ((q.units + 31) / 32);
+  return q.batch * quant_row_blocks(q, rows_per_lane) * quant_chunks(q);
 }
 
 // 16 neighbouring values as they are stored.
@@ -326,19 +328,20 @@ __device__ __forceinline__ float second_of_amax(uint32_t amax) {
 
 // A warp quantizes R rows (more where a row is short) x 512 columns of matrix e.
 template <int DT, int FMT, int R>
-__device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk, const Second& second) {
+__device__ __forceinline__ void quantize_rows(const QuantArgs& q, int e, int row0, int chunk, const Second& second) {
   constexpr int kLanes = FMT == kMX ? 2 : 1;  // lanes per block
   const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
   const int unit = chunk * 32 + (lane & (per - 1));
   const int step = 32 / per;  // rows side by side in the warp
-  const int64_t first = row0 + lane / per;
+  const int first = row0 + lane / per;
   const bool in_row = unit < q.units, in_cols = unit * kUnit < q.cols;
   // rows that exist, and rows that get scales, from this lane's first on
-  const int live = static_cast<int>(min(max(q.rows - first, int64_t{0}), int64_t{R * 32}));
-  const int kept = in_row ? static_cast<int>(min(max(q.rows_padded - first, int64_t{0}), int64_t{R * 32})) : 0;
+  const int live = static_cast<int>(q.rows) - first;
+  const int kept = in_row ? static_cast<int>(q.rows_padded) - first : 0;
+  const int64_t row = e * q.rows + first;
 
   Raw<DT> raw[R];
-  int64_t from = (e * q.rows + first) * q.x_stride + unit * kUnit;
+  int64_t from = row * q.x_stride + unit * kUnit;
 #pragma unroll
   for (int u = 0; u < R; ++u, from += step * q.x_stride) {
     if (in_cols && u * step < live) {
@@ -351,15 +354,15 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
   // where the warp's tokens' scales go, one row a lane, while the values are on their way
   int64_t place = 0;
   if (q.token_tile != 0) {
-    const int64_t r = row0 + lane;
+    const int r = row0 + lane;
     int x = 0, start = 0;
     if (q.ends != nullptr) experts_of_rows(q.ends, q.experts, row0, R * step, x, start);
     if (x >= q.experts || start < 0 || start > r) {
       place = -1;  // a row of no expert
     } else {
-      const int o = static_cast<int>(r - start);
-      place = first_scale_row(start, x, q.token_tile) +
-              static_cast<int64_t>(o / q.token_tile) * scale_rows_per_tile(q.token_tile) + o % q.token_tile;
+      const int o = r - start, tile = o / q.token_tile;
+      place = first_scale_row(start, x, q.token_tile) + static_cast<int64_t>(tile) * scale_rows_per_tile(q.token_tile) +
+              (o - tile * q.token_tile);
     }
     if (q.ends == nullptr) place = __shfl_sync(0xFFFFFFFFu, place, lane / per);  // this lane's first row's
   }
@@ -367,9 +370,9 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
   const int c = unit / kLanes;
   uint8_t* scale = q.swizzled ? q.scale + e * (q.rows_padded >> 7) * q.scale_cols * 512 +
                                     swizzled_byte(q.token_tile != 0 ? place : first, c, q.scale_cols)
-                              : q.scale + (e * q.rows + first) * q.scale_cols + c;
+                              : q.scale + row * q.scale_cols + c;
   const int64_t scale_step = q.swizzled ? step * 16 : static_cast<int64_t>(step) * q.scale_cols;
-  uint8_t* codes = q.codes + (e * q.rows + first) * q.code_pitch + unit * 8;
+  uint8_t* codes = q.codes + row * q.code_pitch + unit * 8;
 #pragma unroll
   for (int u = 0; u < R; ++u, scale += scale_step, codes += step * q.code_pitch) {
     float v[16];
@@ -404,25 +407,24 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int64_t e, int
 
 // Block `b` of quant_blocks(q).
 template <int DT, int FMT, int R>
-__device__ __forceinline__ void quantize_block(const QuantArgs& q, int64_t b) {
-  const int chunks = (q.units + 31) / 32;
-  const int64_t per = quant_row_blocks(q, R);
-  const int64_t rb = b / chunks, e = q.batch == 1 ? 0 : rb / per;
+__device__ __forceinline__ void quantize_block(const QuantArgs& q, uint32_t b) {
+  const uint32_t chunks = quant_chunks(q), per = static_cast<uint32_t>(q.row_blocks);
+  const uint32_t rb = b / chunks, e = q.batch == 1 ? 0 : rb / per;
   const int chunk = static_cast<int>(b - rb * chunks);
   const int rows = 32 / lanes_per_row(q.units) * R;  // per warp
-  const int64_t row0 = (rb - e * per) * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows;
+  const int row0 = static_cast<int>(rb - e * per) * (rows * (kQuantThreads / 32)) + (threadIdx.x >> 5) * rows;
   float g = 1.0f;
   const bool two = FMT == kNV && q.second_mode != kSecondNone;
   if (two) {
     g = q.second_mode == kSecondGiven ? q.second[e] : second_of_amax(q.amax[e]);
     if (q.second_mode == kSecondCompute && rb == e * per && chunk == 0 && threadIdx.x == 0) q.second[e] = g;
   }
-  quantize_rows<DT, FMT, R>(q, e, row0, chunk, second_of(two, g));
+  quantize_rows<DT, FMT, R>(q, static_cast<int>(e), row0, chunk, second_of(two, g));
 }
 
 template <int DT, int FMT, int R>
 __global__ void __launch_bounds__(kQuantThreads, quant_ctas<DT>()) quantize_kernel(const __grid_constant__ QuantArgs q) {
-  quantize_block<DT, FMT, R>(q, q.reverse ? gridDim.x - 1 - static_cast<int64_t>(blockIdx.x) : blockIdx.x);
+  quantize_block<DT, FMT, R>(q, q.reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 // Bits of the largest magnitude of a warp's rows x 512 columns, in every lane.
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const __g
   if (threadIdx.x == 0) q.second[e] = g;
   const Second second = second_of(true, g);
   for (int i = warp; i < pieces; i += kSmallThreads / 32)
-    quantize_rows<DT, FMT, quant_rows<DT>()>(q, e, static_cast<int64_t>(i / chunks) * rows, i % chunks, second);
+    quantize_rows<DT, FMT, quant_rows<DT>()>(q, static_cast<int>(e), i / chunks * rows, i % chunks, second);
 }
 
 // ------------------------------------------------------------ back to values
