@@ -169,9 +169,10 @@ TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t 
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
-  // a handful of tokens, and few enough tiles that no block quantizes them again for another (8 tokens x 28672 x 4096:
-  // 16.8 us prepared, 19.7 fused; 1 token x 14336 x 4096: 9.9 fused)
-  p.fused = tokens / w.batch <= 8 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= sm_count();
+  // One or two tokens, and few enough tiles that no block quantizes them again for another: one launch less (5.5 us of
+  // host time against 8.6). On the device, fused against prepared, x 14336 x 4096 NVFP4: 1 token 10.4 and 10.7 us,
+  // 4 tokens 10.2 and 9.8, 8 tokens 11.4 and 10.3; with more tiles than SMs, 8 x 28672 x 4096: 19.7 and 16.8.
+  p.fused = tokens / w.batch <= 2 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= sm_count();
   // 333 tokens x 1000 x 2080: 10.4 us in tiles of 32, 11.4 of 128
   TilePlan best{};
   for (const int bn : {32, 128, 192}) {
