@@ -7,6 +7,7 @@
  *   NVFP4  e2m1 codes, 16 of a row share one e4m3 scale, optionally with one
  *          fp32 second-level scale over the whole matrix.
  *
+ * Scales are not negative: products take an e4m3 scale's magnitude.
  * Codes are packed two to a byte, the even column in the low nibble. Scales
  * are row-major (rows x cols / block) or swizzled: tiles of 128 rows x 4
  * scales, byte (r % 32) * 16 + (r / 32) * 4 + c, tiles row-major with both

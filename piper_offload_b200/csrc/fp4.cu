@@ -7,8 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstring>
-#include <string>
+#include <cstdio>
 
 #include "fp4_grad.cuh"
 #include "fp4_linear.cuh"
@@ -16,16 +15,17 @@
 
 namespace {
 
-thread_local std::string g_error;
+// No std::string: nothing here throws across the C boundary.
+thread_local char g_error[256];
 std::atomic<uint64_t> g_launches{0};
 
 int fail(int code, const char* message) {
-  g_error = message;
+  std::snprintf(g_error, sizeof(g_error), "%s", message);
   return code;
 }
 
 int cuda_fail(const char* what, cudaError_t e) {
-  g_error = std::string(what) + ": " + cudaGetErrorString(e);
+  std::snprintf(g_error, sizeof(g_error), "%s: %s", what, cudaGetErrorString(e));
   return PIPER_FP4_ECUDA;
 }
 
@@ -351,7 +351,7 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
     cudaError_t e = cudaMemsetAsync(maxima, 0, sizeof(uint32_t) * m->batch, s);
     if (e != cudaSuccess) return cuda_fail("cudaMemsetAsync", e);
     const int64_t blocks = fp4::quant_row_blocks(q, many_rows(dtype)) * ((q.units + 31) / 32);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 148 * 32)), static_cast<unsigned>(m->batch));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, int64_t{32} * sm_count())), static_cast<unsigned>(m->batch));
     if (dtype == PIPER_FP4_BF16) fp4::amax_kernel<fp4::kBF16><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     else fp4::amax_kernel<fp4::kF32><<<grid, fp4::kQuantThreads, 0, s>>>(q, maxima);
     if ((e = launched()) != cudaSuccess) return cuda_fail("amax kernel", e);
@@ -583,7 +583,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("gradient kernel", e);
 }
 
-const char* piper_fp4_last_error(void) { return g_error.c_str(); }
+const char* piper_fp4_last_error(void) { return g_error; }
 
 int piper_fp4_device_status(void* stream, uint32_t* status) {
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));

@@ -212,6 +212,8 @@ def quantize_nvfp4(x: torch.Tensor, *, two_level: bool = True, per_tensor_scale:
 
 def dequantize_fp4(weight: Any, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The values of a packed weight or stack, rounded once to ``dtype`` (default: the weight's original type)."""
+    if getattr(weight, "qdata", None) is None:
+        raise ValueError(f"FP4 operators take MXFP4 and NVFP4 weights, got {type(weight).__name__}.")
     done = nat.calls().dequantize(weight, weight.qdata.ndim, dtype)
     if done is not None:
         return done
@@ -222,6 +224,13 @@ def dequantize_fp4(weight: Any, dtype: torch.dtype | None = None) -> torch.Tenso
 
 
 # ---------------------------------------------------------------------- products
+def _check_kind(weight: Any, dims: int, message: str) -> None:
+    if getattr(weight, "qdata", None) is None:
+        raise ValueError(f"FP4 operators take MXFP4 and NVFP4 weights, got {type(weight).__name__}.")
+    if weight.qdata.ndim != dims:
+        raise ValueError(message)
+
+
 def _check_ends(ends: torch.Tensor, batch: int, device: torch.device) -> None:
     if ends.dtype is not torch.int32 or ends.ndim != 1 or ends.shape[0] != batch or not ends.is_contiguous():
         raise ValueError("Group ends are one contiguous int32 vector with an entry per expert.")
@@ -311,8 +320,7 @@ def linear_fp4(x: torch.Tensor, weight: MXWeight | NVFP4Weight, *,
     ``act_per_tensor_scale`` where one is given. Differentiable with respect to
     ``x`` (straight through its quantisation); the weight is constant.
     """
-    if weight.qdata.ndim != 2:
-        raise ValueError("linear_fp4 takes one weight; grouped_linear_fp4 takes a stack of experts.")
+    _check_kind(weight, 2, "linear_fp4 takes one weight; grouped_linear_fp4 takes a stack of experts.")
     return _product(x, weight, None, act_per_tensor_scale)
 
 
@@ -324,7 +332,8 @@ def grouped_linear_fp4(x: torch.Tensor, experts: MXExperts | NVFP4Experts, group
     ``group_ends[e]`` (int32 on the device, non-decreasing, not read by the
     host). Experts may have no rows; rows past the last end come out as zeros.
     """
-    if experts.qdata.ndim != 3 or x.ndim != 2:
+    _check_kind(experts, 3, "grouped_linear_fp4 takes a stack of experts and rank-two tokens.")
+    if x.ndim != 2:
         raise ValueError("grouped_linear_fp4 takes a stack of experts and rank-two tokens.")
     _check_ends(group_ends, experts.qdata.shape[0], experts.qdata.device)
     return _product(x, experts, group_ends, act_per_tensor_scale)
@@ -332,15 +341,15 @@ def grouped_linear_fp4(x: torch.Tensor, experts: MXExperts | NVFP4Experts, group
 
 def linear_fp4_grad_input(grad: torch.Tensor, weight: MXWeight | NVFP4Weight) -> torch.Tensor:
     """``grad @ dequantised(weight)`` for ``grad`` (..., rows): :func:`linear_fp4`'s gradient, in the type of ``grad``."""
-    if weight.qdata.ndim != 2:
-        raise ValueError("linear_fp4_grad_input takes one weight; grouped_linear_fp4_grad_input takes a stack of experts.")
+    _check_kind(weight, 2, "linear_fp4_grad_input takes one weight; grouped_linear_fp4_grad_input takes a stack of experts.")
     return _grad_input(grad, weight, None)
 
 
 def grouped_linear_fp4_grad_input(grad: torch.Tensor, experts: MXExperts | NVFP4Experts,
                                   group_ends: torch.Tensor) -> torch.Tensor:
     """:func:`grouped_linear_fp4`'s gradient with respect to its tokens; rows past the last end get zeros."""
-    if experts.qdata.ndim != 3 or grad.ndim != 2:
+    _check_kind(experts, 3, "grouped_linear_fp4_grad_input takes a stack of experts and a rank-two gradient.")
+    if grad.ndim != 2:
         raise ValueError("grouped_linear_fp4_grad_input takes a stack of experts and a rank-two gradient.")
     _check_ends(group_ends, experts.qdata.shape[0], experts.qdata.device)
     return _grad_input(grad, experts, group_ends)

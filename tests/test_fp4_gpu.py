@@ -262,6 +262,37 @@ def test_linear_nvfp4_columns_of_sixteen(cols, tokens, cuda_device):
         assert_product(fp4.linear_fp4(x, w), quantized_values(x, "nvfp4"), v[0])
 
 
+@pytest.mark.parametrize("swizzled", [False, True], ids=["rows", "swizzled"])
+@pytest.mark.parametrize("tokens", [1, 2, 20, 100, 130])
+@pytest.mark.parametrize("fmt,rows,cols", [("mxfp4", 130, 4128), ("nvfp4", 130, 4112), ("nvfp4", 64, 8192), ("mxfp4", 300, 16384)])
+def test_long_rows_are_split_over_a_cluster(fmt, rows, cols, tokens, swizzled, cuda_device):
+    """Few outputs and many columns: several blocks share a tile's columns and add their sums up."""
+    w, v = make_weight(fmt, rows, cols, cuda_device, swizzled=swizzled, second=0.25 if fmt == "nvfp4" else None)
+    for dtype in DTYPES:
+        x = to_torch(rng(tokens, cols).standard_normal((tokens, cols)), dtype, cuda_device)
+        assert_product(fp4.linear_fp4(x, w), quantized_values(x, fmt), v[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("tokens,rows,cols", [(1, 4100, 160), (40, 4096, 96), (200, 2111, 224)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_long_gradients_are_split_over_a_cluster(fmt, tokens, rows, cols, dtype, cuda_device):
+    w, v = make_weight(fmt, rows, cols, cuda_device)
+    dy = to_torch(rng(tokens, rows).standard_normal((tokens, rows)), dtype, cuda_device)
+    assert_product(fp4.linear_fp4_grad_input(dy, w), exact(dy), v[0].T)
+
+
+@pytest.mark.parametrize("tokens,rows,cols", [(3000, 700, 288), (1600, 4000, 96)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_many_tokens(fmt, tokens, rows, cols, cuda_device):
+    """More tiles than SMs, in every direction."""
+    w, v = make_weight(fmt, rows, cols, cuda_device)
+    x = to_torch(rng(tokens, cols).standard_normal((tokens, cols)), torch.bfloat16, cuda_device)
+    assert_product(fp4.linear_fp4(x, w), quantized_values(x, fmt), v[0])
+    dy = to_torch(rng(tokens, rows).standard_normal((tokens, rows)), torch.bfloat16, cuda_device)
+    assert_product(fp4.linear_fp4_grad_input(dy, w), exact(dy), v[0].T)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("cols", [96, 160, 224])
 def test_scale_padding_may_hold_anything(fmt, cols, cuda_device):
@@ -329,7 +360,7 @@ def test_nan_tokens_reach_only_their_rows(cuda_device):
 
 # --------------------------------------------------------------------- experts
 GROUPS = [[5], [0, 3, 0], [1, 1, 1, 1, 1, 1, 1], [130, 0, 7, 64], [33, 257, 1, 0, 0, 90], [0, 0, 0], [300, 300],
-          [2] * 40, [60, 0, 2, 1, 1, 95, 0, 33], [100] + [0] * 9]
+          [2] * 40, [60, 0, 2, 1, 1, 95, 0, 33], [100] + [0] * 9, [40] + [0] * 30]
 
 
 @pytest.mark.parametrize("tail", [0, 37])

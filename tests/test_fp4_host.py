@@ -127,6 +127,17 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_other_weights_are_refused():
+    x = torch.ones(4, 64, dtype=torch.bfloat16)
+    gguf = W.GGUFWeight(torch.zeros(8, 68, dtype=torch.uint8), 8)
+    fp8 = W.Float8Weight(torch.zeros(8, 64, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.ones(8, 1), (1, 64))
+    for call in (lambda w: fp4.linear_fp4(x, w), lambda w: fp4.linear_fp4_grad_input(x[:, :8], w), fp4.dequantize_fp4):
+        with pytest.raises(ValueError, match="MXFP4 and NVFP4 weights, got GGUFWeight"):
+            call(gguf)
+        with pytest.raises(ValueError):
+            call(fp8)
+
+
 def test_experts_are_views_of_their_stack():
     stack = W.NVFP4Experts(torch.zeros(3, 4, 16, dtype=torch.uint8), torch.zeros(3, 4, 2, dtype=torch.uint8),
                            torch.ones(3), is_swizzled_scales=False)
