@@ -334,10 +334,11 @@ __global__ void __launch_bounds__(256) split_kernel(const void* dy, int64_t stri
     float v = static_cast<const float*>(dy)[token * stride + n];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const __nv_bfloat16 b = __float2bfloat16_rn(v);
+      // the largest fp32 values round beyond bf16's range: its last number first, and the terms after make up for it
+      const float most = __uint_as_float(0x7F7F0000u);
+      const __nv_bfloat16 b = __float2bfloat16_rn(isfinite(v) ? fminf(fmaxf(v, -most), most) : v);
       out[i * tokens * pitch + at] = b;
-      v = __fsub_rn(v, __bfloat162float(b));
-      if (!isfinite(__bfloat162float(b))) v = 0.0f;  // an infinity or a NaN is its first term alone
+      v = isfinite(v) ? __fsub_rn(v, __bfloat162float(b)) : 0.0f;  // an infinity or a NaN is its first term alone
     }
   }
 }

@@ -20,7 +20,8 @@ from ``a``. NVFP4: ``s = e4m3(clamp(a / 6 / g, 2**-6, 448)) * g``, where the
 second-level scale ``g`` is 1, given, or ``max(max|x| / 2688, 2**-23)`` over
 the matrix. A block that holds a NaN reads back as NaN; infinities saturate.
 Products are over these values, summed in fp32 and rounded once to the type
-of the tokens.
+of the tokens. Second-level scales multiply the sum, so it is the sum before
+them that has to fit fp32.
 
 All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
 take workspaces from PyTorch's caching allocator on it, do not synchronise,

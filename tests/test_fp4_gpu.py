@@ -448,6 +448,26 @@ def test_grad_input_strides(cuda_device):
     assert fp4.linear_fp4_grad_input(base[:0, 0, :128], w).shape == (0, 96)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_gradients_at_the_end_of_the_range(fmt, cuda_device):
+    """fp32 gradients that bf16 cannot hold, an infinity and a NaN: each reaches its own row as the formula says."""
+    dense = to_torch(rng(13).standard_normal((96, 160)) * 0.02, torch.bfloat16, cuda_device)
+    # no second level: it multiplies the sum, which has to stay finite before that
+    w = fp4.quantize_mxfp4(dense) if fmt == "mxfp4" else fp4.quantize_nvfp4(dense, two_level=False)
+    v = exact(fp4.dequantize_fp4(w, torch.float32))
+    assert np.abs(v).max() < 1  # no product of a finite row overflows
+    dy = to_torch(rng(14).standard_normal((40, 96)), torch.float32, cuda_device)
+    dy[:4] = 0
+    dy[0, 2], dy[1, 3] = torch.finfo(torch.float32).max, -3.4e38
+    dy[2, 5], dy[3, 7] = float("inf"), float("nan")
+    dx = fp4.linear_fp4_grad_input(dy, w)
+    rows = [0, 1, *range(4, 40)]
+    assert_product(dx[rows], exact(dy[rows]), v.T)
+    with np.errstate(invalid="ignore"):
+        np.testing.assert_array_equal(exact(dx[2]), np.inf * v[5])  # an infinity times a zero is a NaN
+    assert dx[3].isnan().all()
+
+
 def test_gradient_against_differences(cuda_device):
     """Along directions in which the quantised tokens move exactly (whole codes), the product is linear: its
     difference is the gradient's inner product."""
