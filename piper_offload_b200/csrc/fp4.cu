@@ -150,6 +150,8 @@ struct LinearPlan {
 // Tokens per tile and blocks of a cluster that share a tile's stages, by a
 // rough account in cycles: a stage takes `stage`, leaving sums and adding them
 // up 2500 and 30 for each token of the tile, and every wave of tiles 2000.
+// Split against not: 1 x 4096 x 14336 NVFP4 10.9 and 19.1 us, 24 x 4096 x 4096 MXFP4
+// 9.0 and 10.5, 128 x 4096 x 14336 NVFP4 15.5 and 19.3.
 struct TilePlan {
   int bn, split;
   double cycles;
@@ -173,7 +175,8 @@ LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   // host time against 8.6). On the device, fused against prepared, x 14336 x 4096 NVFP4: 1 token 10.4 and 10.7 us,
   // 4 tokens 10.2 and 9.8, 8 tokens 11.4 and 10.3; with more tiles than SMs, 8 x 28672 x 4096: 19.7 and 16.8.
   p.fused = tokens / w.batch <= 2 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= sm_count();
-  // 333 tokens x 1000 x 2080: 10.4 us in tiles of 32, 11.4 of 128
+  // 333 tokens x 1000 x 2080 MXFP4: 10.1 us in tiles of 32, 12.2 of 192; 512 x 4096 x 14336 NVFP4: 24.7 of 128, 32.9 of
+  // 192; 4096 x 14336 x 4224: 145.5 of 128, 141 of 192
   TilePlan best{};
   for (const int bn : {32, 128, 192}) {
     if (p.fused && bn > 32) break;
@@ -259,8 +262,11 @@ GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, in
 }
 
 // Tiles of a gradient: tokens x (rows x 128) columns. Decoding costs the same
-// whatever the tokens, so tiles are as wide in tokens as they go; 256 columns
-// where that fills the SMs (a rough account in cycles a stage: 1060 and 600).
+// whatever the tokens, so tiles are as wide in tokens as they go, but for a few,
+// which leave room for more stages (32 x 14336 x 4096 NVFP4: 31.1 us in tiles of 64,
+// 36.6 of 256); 256 columns where that fills the SMs (a rough account in cycles a
+// stage: 1060 and 600; 2048 x 14336 x 4096 198 us against 231 with 128 columns,
+// 512 x 4096 x 4096 60 against 25.8).
 struct GradTile {
   int bn, rows;
 };

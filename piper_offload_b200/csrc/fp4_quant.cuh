@@ -10,12 +10,15 @@
 // rule of its own: a NaN in a block makes its scale NaN (e8m0 255, e4m3 127),
 // so the whole block and what is computed from it read as NaN.
 //
-// Bound: HBM, with instructions close behind (a first version with 8 values a
-// lane and a division per lane for its place took 45 instructions a value and
-// 4.7x the time). A lane holds 16 neighbouring values: one 32-byte load
-// (bf16), one 8-byte store, no shuffle for an NVFP4 block and one for an
-// MXFP4 block; four rows are in flight per lane, and only a block of threads
-// divides to find its place.
+// Bound: HBM, with instructions close behind (8 values a lane and a division
+// per lane for its place cost twice the time of the whole). A lane holds 16
+// neighbouring values: one 32-byte load (bf16), one 8-byte store, no shuffle
+// for an NVFP4 block and one for an MXFP4 block; four rows are in flight per
+// lane, and only a block of threads divides to find its place.
+//
+// Measured on a B200 (copies run at 6.5 TB/s): 12288 x 3072 bf16 to MXFP4 21.7 us
+// (4.4 TB/s) and back 15.9 (6.0); 4096 x 14336 fp32 to two-level NVFP4 46 us for
+// the maximum (5.1 TB/s) and 49 for the codes (5.5), back 41 (6.5).
 #pragma once
 #include "fp4_ptx.cuh"
 #include "numerics.cuh"
