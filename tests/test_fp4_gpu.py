@@ -174,6 +174,23 @@ def test_two_level(shape, swizzled, cuda_device):
     assert torch.equal(given.qdata, w.qdata) and torch.equal(given.scale.view(torch.uint8), w.scale.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("swizzled", [False, True], ids=["rows", "swizzled"])
+@pytest.mark.parametrize("shape", [(3, 700, 2080), (5, 1030, 544), (1, 9000, 96), (40, 70, 544)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_many_rows_of_several_matrices(fmt, shape, swizzled, dtype, cuda_device):
+    """Enough rows that a block quantises several places, with its last one in any matrix, row and column."""
+    dense = rng(*shape).standard_normal(shape) * np.linspace(0.01, 1.0, shape[0])[:, None, None]
+    x = to_torch(dense, dtype, cuda_device)
+    w = fp4.quantize_mxfp4(x, swizzled=swizzled) if fmt == "mxfp4" else fp4.quantize_nvfp4(x, swizzled=swizzled)
+    for i, m in enumerate(exact(x)):
+        second = None if fmt == "mxfp4" else float(w.per_tensor_scale[i])
+        assert second is None or second == R.second_of(m)
+        codes, byte = R.quantize(m, fmt, second=second)
+        np.testing.assert_array_equal(codes_of(w.expert(i)), codes)
+        np.testing.assert_array_equal(bytes_of(w.expert(i)), R.lay_out(byte, swizzled))
+
+
 def test_quantize_strided_and_unaligned_rows(cuda_device):
     base = to_torch(rng(3).standard_normal((40, 300)), torch.bfloat16, cuda_device)
     for view in (base[:, :256], base[:, 3:259], base[1::3, 8:264], base.t()[:, :32], base[::2, 5:101].t()[:64, :16]):
