@@ -14,8 +14,9 @@
 // tokens keeps the pipe busy for 1024 cycles; the pipe reads 96 KB for it and 64
 // are written, 1280 cycles at 128 bytes each, and decoding takes its warps about
 // 900 issue slots of each scheduler. 2048 x 14336 x 4096 NVFP4: 198 us, 1.2
-// PFLOP/s, on 128 of the 148 SMs, the pipe active 53 % of the time; in tiles of 128
-// columns, whose stages bring 36 KB for 512 cycles, 231. Few tokens: decoding,
+// PFLOP/s, on 128 of the 148 SMs, the pipe active 53 % of the time; copies and
+// products without the decoding would take 176, decoding with a quarter of the
+// products 174. In tiles of 128 columns, whose stages bring 36 KB for 512 cycles, 231. Few tokens: decoding,
 // since every value of w is decoded once a tile; 64 x 4096 x 4096 MXFP4 14.2 us
 // (cluster of 4, without it 36.5).
 //
