@@ -313,7 +313,7 @@ int piper_fp4_quantize(const piper_fp4_matrix* m, const void* x, int64_t x_strid
   if (int rc = check_buffers(m)) return rc;
   if (int rc = check_dtype(dtype)) return rc;
   FP4_REQUIRE(x != nullptr, "FP4 quantisation: null input.");
-  FP4_REQUIRE(x_stride >= m->cols, "FP4 quantisation: rows of the input overlap.");
+  FP4_REQUIRE(x_stride >= m->cols || (m->rows == 1 && m->batch == 1), "FP4 quantisation: rows of the input overlap.");
   FP4_REQUIRE(scale_mode >= 0 && scale_mode <= 3, "Unsupported MX scaling mode id.");
   FP4_REQUIRE(second_mode >= 0 && second_mode <= 2, "FP4 quantisation: unknown second-level mode.");
   FP4_REQUIRE((second_mode == PIPER_FP4_SECOND_NONE) == (m->second == nullptr),

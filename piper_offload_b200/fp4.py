@@ -319,7 +319,8 @@ def linear_fp4(x: torch.Tensor, weight: MXWeight | NVFP4Weight, *,
     ``x`` is quantised in the weight's format: MXFP4 with the weight's
     ``act_quant_kwargs.scaling_mode``, NVFP4 with the second-level scale
     ``act_per_tensor_scale`` where one is given. Differentiable with respect to
-    ``x`` (straight through its quantisation); the weight is constant.
+    ``x`` (straight through its quantisation); the weight is constant. A merge
+    into it between the two passes is not noticed: the gradient is the merged one's.
     """
     _check_kind(weight, 2, "linear_fp4 takes one weight; grouped_linear_fp4 takes a stack of experts.")
     return _product(x, weight, None, act_per_tensor_scale)

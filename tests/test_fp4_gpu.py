@@ -203,6 +203,19 @@ def test_quantize_strided_and_unaligned_rows(cuda_device):
             assert torch.equal(w.qdata, d.qdata) and torch.equal(w.per_tensor_scale, d.per_tensor_scale)
 
 
+def test_a_single_row_may_have_any_stride(cuda_device):
+    column = to_torch(rng(15).standard_normal((64, 1)), torch.bfloat16, cuda_device)
+    scale = torch.tensor([0.01], device=cuda_device)
+    for x in (column.t(), column.t()[:, :48]):
+        assert x.stride(0) < x.shape[1]
+        w = fp4.quantize_nvfp4(x, per_tensor_scale=scale)
+        again = fp4.quantize_nvfp4(x.reshape(-1).clone()[None], per_tensor_scale=scale)
+        assert torch.equal(w.qdata, again.qdata) and w.qdata.shape == (1, x.shape[1] // 2)
+        y = fp4.linear_fp4(x, w)
+        assert torch.equal(y, fp4.linear_fp4(x.reshape(-1).clone(), w)[None])
+        assert torch.equal(fp4.linear_fp4_grad_input(y, w), fp4.linear_fp4_grad_input(y.reshape(-1).clone(), w)[None])
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_nan_blocks_and_infinities(fmt, cuda_device):
     x = torch.ones((4, 128), device=cuda_device)
