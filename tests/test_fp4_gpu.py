@@ -610,6 +610,58 @@ def test_compiled_calls_and_the_written_out_path_agree(fmt, cuda_device, monkeyp
         assert a.dtype is b.dtype and torch.equal(a, b)
 
 
+def test_offsets_beyond_32_bits(cuda_device):
+    """Codes, inputs and outputs whose ends lie past 2**32 bytes and 2**31 values.
+
+    Scales are one and inputs small integers, so every sum is a multiple of 1/2 far below 2**23: exact in any order.
+    """
+    if torch.cuda.mem_get_info(cuda_device)[0] < 48 << 30:
+        pytest.skip("needs 48 GB of device memory")
+    g = torch.Generator(cuda_device).manual_seed(16)
+
+    def codes_like(rows, cols):
+        return torch.randint(0, 256, (rows, cols // 2), dtype=torch.uint8, device=cuda_device, generator=g)
+
+    def weight(codes):
+        scale = torch.full((codes.shape[0], codes.shape[1] // 16), 127, dtype=torch.uint8, device=cuda_device)
+        return W.MXWeight(codes.contiguous(), scale, torch.float4_e2m1fn_x2, orig_dtype=torch.bfloat16)
+
+    def values(codes):
+        return exact(fp4.dequantize_fp4(weight(codes)))
+
+    def integers(rows, cols, most):
+        return torch.randint(-most, most + 1, (rows, cols), dtype=torch.int8, device=cuda_device, generator=g).to(torch.bfloat16)
+
+    def tokens(rows, cols):
+        x = integers(rows, cols, 4)
+        x[:, ::32] = 4  # so that every block's scale is one
+        return x
+
+    # a weight of 4.6 GB of codes: its last rows in the product, its last columns in the gradient
+    codes = codes_like(70000, 131072)
+    w = weight(codes)
+    x = tokens(2, 131072)
+    y = fp4.linear_fp4(x.float(), w)
+    np.testing.assert_array_equal(exact(y[:, -5:]), exact(x) @ values(codes[-5:]).T)
+    dy = integers(2, 70000, 3)
+    dx = fp4.linear_fp4_grad_input(dy.float(), w)
+    np.testing.assert_array_equal(exact(dx[:, -32:]), exact(dy) @ values(codes[:, -16:]))
+    del w
+    # 2.8e9 outputs, as many gradients, and as many values to quantise
+    codes = codes_like(40000, 64)
+    w, v = weight(codes), values(codes)
+    x = tokens(70000, 64)
+    y = fp4.linear_fp4(x, w)
+    assert torch.equal(y[-3:].cpu(), torch.from_numpy(exact(x[-3:]) @ v.T).to(torch.bfloat16))
+    q, tail = fp4.quantize_mxfp4(y), fp4.quantize_mxfp4(y[-3:])
+    assert torch.equal(q.qdata[-3:], tail.qdata) and torch.equal(q.scale[-3:], tail.scale)
+    assert torch.equal(fp4.dequantize_fp4(q)[-3:], fp4.dequantize_fp4(tail))
+    del q, y
+    dy = integers(70000, 40000, 3)
+    dx = fp4.linear_fp4_grad_input(dy, w)
+    assert torch.equal(dx[-3:].cpu(), torch.from_numpy(exact(dy[-3:]) @ v).to(torch.bfloat16))
+
+
 def test_launches_are_counted(cuda_device):
     w, _ = make_weight("mxfp4", 128, 128, cuda_device)
     x = torch.ones((4, 128), dtype=torch.bfloat16, device=cuda_device)
