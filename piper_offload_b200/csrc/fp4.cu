@@ -150,17 +150,19 @@ struct LinearPlan {
 // Tokens per tile and blocks of a cluster that share a tile's stages, by a
 // rough account in cycles: a stage takes `stage`, leaving sums and adding them
 // up 2500 and 30 for each token of the tile, and every wave of tiles 2000.
-// Split against not: 1 x 4096 x 14336 NVFP4 10.9 and 19.1 us, 24 x 4096 x 4096 MXFP4
-// 9.0 and 10.5, 128 x 4096 x 14336 NVFP4 15.5 and 19.3.
+// Split against not: 1 x 4096 x 14336 NVFP4 10.7 and 19.1 us, 24 x 4096 x 4096 MXFP4
+// 9.0 and 10.5, 128 x 4096 x 14336 NVFP4 15.5 and 19.3. `room` is how many blocks
+// the GPU holds; with two on an SM fewer than four stages a block do not pay (1 x
+// 4096 x 4096 MXFP4 split in 8 8.2 us, in 4 6.1).
 struct TilePlan {
   int bn, split;
   double cycles;
 };
-TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t tile_tokens, bool can_split) {
+TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t tile_tokens, bool can_split, int64_t room) {
   TilePlan best{bn, 1, 0.0};
   for (int split = 1; split <= (can_split ? fp4::kMaxSplit : 1); split *= 2) {
-    if (split > 1 && (items * split > sm_count() || stages < 2 * split)) break;
-    const int64_t waves = (items * split + sm_count() - 1) / sm_count();
+    if (split > 1 && (items * split > room || stages < (room > sm_count() ? 4 : 2) * split)) break;
+    const int64_t waves = (items * split + room - 1) / room;
     double cycles = static_cast<double>(waves) * (static_cast<double>((stages + split - 1) / split) * stage + 2000.0);
     if (split > 1) cycles += 2500.0 + 30.0 * static_cast<double>(tile_tokens);
     if (split == 1 || cycles < best.cycles) best = {bn, split, cycles};
@@ -171,10 +173,14 @@ TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t 
 LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
-  // One or two tokens, and few enough tiles that no block quantizes them again for another: one launch less (5.5 us of
-  // host time against 8.6). On the device, fused against prepared, x 14336 x 4096 NVFP4: 1 token 10.4 and 10.7 us,
-  // 4 tokens 10.2 and 9.8, 8 tokens 11.4 and 10.3; with more tiles than SMs, 8 x 28672 x 4096: 19.7 and 16.8.
-  p.fused = tokens / w.batch <= 2 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= sm_count();
+  // One or two tokens a weight, and few enough tiles that no block quantizes them again for another: one launch less
+  // (5.5 us of host time against 8.6). On the device, fused against prepared: 1 x 14336 x 4096 NVFP4 10.1 and 10.4 us,
+  // 1 x 28672 x 4096 15.2 and 17.6, 2 x 4096 x 4096 MXFP4 6.3 and 7.3, 8 rows over 8 experts of 2816 x 1024 6.1 and 8.2.
+  // A block quantizes two tokens of a stage at a time, so the product of both is bounded in case one expert has all the
+  // rows (128 over 64 experts of 512 x 1024 NVFP4: 8.0 and 8.7 us evenly, 13.1 and 7.2 most in one).
+  const int64_t stages = (w.cols + fp4::kStageCols - 1) / fp4::kStageCols;
+  p.fused = tokens / w.batch <= 2 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= fp4::kFusedCtas * sm_count() &&
+            (w.batch == 1 || tokens * stages <= 128);
   // 333 tokens x 1000 x 2080 MXFP4: 10.1 us in tiles of 32, 12.2 of 192; 512 x 4096 x 14336 NVFP4: 24.7 of 128, 32.9 of
   // 192; 4096 x 14336 x 4224: 145.5 of 128, 141 of 192
   TilePlan best{};
@@ -182,8 +188,8 @@ LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
     if (p.fused && bn > 32) break;
     const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
     const int64_t items = std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + 127) / 128);
-    const TilePlan t = plan_tile(bn, items, (w.cols + fp4::kStageCols - 1) / fp4::kStageCols,
-                                 330.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1);
+    const TilePlan t = plan_tile(bn, items, stages,
+                                 330.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, (p.fused ? fp4::kFusedCtas : 1) * sm_count());
     if (best.bn == 0 || t.cycles < best.cycles) best = t;
   }
   p.bn = best.bn;
@@ -234,7 +240,7 @@ cudaError_t launch_linear(fp4::LinearArgs& args, int64_t items, cudaStream_t str
   attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(
-      args.split > 1 ? items * args.split : std::min<int64_t>(items, sm_count())));
+      args.split > 1 ? items * args.split : std::min<int64_t>(items, S::kCtas * sm_count())));
   config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
@@ -287,7 +293,7 @@ cudaError_t launch_grad(fp4::GradArgs& args, int64_t items, cudaStream_t stream)
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   const int stages = (args.rows + fp4::kGradStageRows - 1) / fp4::kGradStageRows * args.terms;
-  args.split = plan_tile(BN, items, stages, 600.0, std::min<int64_t>(args.groups.tokens, BN), S::kCanSplit && args.groups.ends == nullptr).split;
+  args.split = plan_tile(BN, items, stages, 600.0, std::min<int64_t>(args.groups.tokens, BN), S::kCanSplit && args.groups.ends == nullptr, sm_count()).split;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
   attribute.val.clusterDim.x = static_cast<unsigned>(args.split);

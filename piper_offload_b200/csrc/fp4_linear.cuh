@@ -12,14 +12,15 @@
 //
 // Many tokens: their codes and scales are made by a launch before (prepare_kernel),
 // tiles are 32, 128 or 192 tokens wide. A handful (kFused): the kernel is a
-// stream of weight bytes, so eight warps quantize the tokens on the way, each
-// every eighth stage, and there is no launch before. Where there are too few tiles for the
-// SMs, a cluster of blocks splits K; each leaves its sums in its own shared
+// stream of weight bytes, so four warps quantize the tokens on the way, each
+// every fourth stage, there is no launch before, and two blocks share an SM, one
+// starting or ending while the other streams. Where there are too few tiles for
+// the SMs, a cluster of blocks splits K; each leaves its sums in its own shared
 // memory and every block adds up its share of the tokens over the cluster, in
 // rank order, so that results do not depend on timing.
 //
 // Bounds and times on a B200, whole calls. Few tokens: HBM, after about 5 us of
-// launch and first loads; 1 x 14336 x 4096 NVFP4 9.9 us (3.3 TB/s), 16 tokens
+// launch and first loads; 1 x 14336 x 4096 NVFP4 9.6 us (3.4 TB/s), x 28672 14.9 (4.4), 16 tokens
 // over 8 experts of 14336 x 4096 two-level 37.8 us (5.3 TB/s). Many: what shared
 // memory gives the tensor core. A 128 x 192 step of 64 values keeps it for 96
 // cycles and brings 11.5 KB in and out again, about 184 cycles at 128 bytes; 170 to
@@ -38,7 +39,8 @@ namespace fp4 {
 
 constexpr int kStageCols = 256;      // K values per stage
 constexpr int kStageBytes = kStageCols / 2;
-constexpr int kQuantWarps = 8;       // kFused
+constexpr int kQuantWarps = 4;       // kFused
+constexpr int kFusedCtas = 2;        // kFused: blocks per SM
 constexpr int kMaxSplit = 8;
 
 // Where the weight's scales come from: whole swizzled tiles by bulk copies, or
@@ -73,6 +75,7 @@ struct LinearArgs {
 template <int FMT, int BN, bool kFused>
 struct LinearShape {
   static constexpr int kTiles = FMT == kNV ? 4 : 2;                 // scale tiles per stage and 128 rows
+  static constexpr int kCtas = kFused ? kFusedCtas : 1;             // per SM
   static constexpr int kXBlocks = (BN + 127) / 128;                 // 128-token scale blocks per tile
   static constexpr int kW = kTileRows * kStageBytes;
   static constexpr int kX = BN * kStageBytes;
@@ -80,13 +83,13 @@ struct LinearShape {
   static constexpr int kSX = kXBlocks * kTiles * 512;
   static constexpr int kStage = kW + kX + kSW + kSX;
   static constexpr int kOut = 4 * 2048;                             // 32 tokens x 32 outputs of each epilogue warp
-  static constexpr int kRoom = kSmemMax - 2048 - kOut;
+  static constexpr int kRoom = kSmemMax / kCtas - 2048 - kOut;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + 1024 + 512;
   static constexpr bool kCanSplit = BN * kTileRows * 4 <= kStages * kStage;
   // tensor memory: two accumulators, then buffers of scales, one per stage if they fit
   static constexpr int kScaleCols = kTiles * 4 * (1 + kXBlocks);
-  static constexpr int kBufs = (512 - 2 * BN) / kScaleCols < kStages ? (512 - 2 * BN) / kScaleCols : kStages;
+  static constexpr int kBufs = (512 / kCtas - 2 * BN) / kScaleCols < kStages ? (512 / kCtas - 2 * BN) / kScaleCols : kStages;
   static constexpr int kCols = 2 * BN + kBufs * kScaleCols;
   // with fewer buffers than stages the copies of scales wait for products, and get a warp of their own: 4096 tokens x
   // 14336 x 4096 NVFP4 136 us against 145 (as measured when it was added); with a buffer per stage one warp does both, 6 to 10 % faster on small calls
@@ -94,7 +97,9 @@ struct LinearShape {
   static constexpr int kFirstQuantWarp = kCopyWarp ? 8 : 7;
   static constexpr int kThreads = 32 * kFirstQuantWarp + (kFused ? 32 * kQuantWarps : 0);
   static constexpr int kAlloc = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-  static_assert(kCols <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
+  static_assert(kAlloc * kCtas <= 512 && kStages >= 4 && kBufs >= 2, "the tile does not fit");
+  // a warp's next stage is at most one round of the ring away: further, a wait on a slot's parity could pass a round early
+  static_assert(!kFused || kQuantWarps <= kStages, "more quantising warps than stages");
 };
 
 // The scales that one stage needs of the weight: 128 rows x kTiles words, four rows a lane.
@@ -161,28 +166,17 @@ __device__ __forceinline__ ScaleWords<FMT> load_scale_words(const LinearArgs& p,
   return s;
 }
 
-// Eight tokens of a stage, as a warp holds them: half a warp a row.
+// Two tokens of a stage, as a warp holds them: half a warp a row.
 template <int DT>
-struct TokenBlock {
-  Raw<DT> raw[4];
-};
+using TokenBlock = Raw<DT>;
 
 template <int DT>
 __device__ __forceinline__ TokenBlock<DT> load_tokens(const LinearArgs& p, const TileAt& t, int stage, int row0) {
   const int lane = threadIdx.x & 31;
   const int col = stage * kStageCols + (lane & 15) * kUnit;
-  TokenBlock<DT> b;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int r = row0 + 2 * u + (lane >> 4);
-    if (r < t.count && col < p.cols) {
-      b.raw[u] = load_unit<DT>(p.x, (t.first + r) * p.x_stride + col, p.x_vec != 0);
-    } else {
-#pragma unroll
-      for (auto& w : b.raw[u].w) w = 0u;
-    }
-  }
-  return b;
+  const int r = row0 + (lane >> 4);
+  if (r < t.count && col < p.cols) return load_unit<DT>(p.x, (t.first + r) * p.x_stride + col, p.x_vec != 0);
+  return TokenBlock<DT>{};
 }
 
 // A warp quantizes them into the operand's swizzled rows and its scale tiles.
@@ -191,19 +185,15 @@ __device__ __forceinline__ void quantize_tokens(const LinearArgs& p, const TileA
                                                 uint8_t* codes, uint8_t* scales, const Second& second) {
   const int lane = threadIdx.x & 31, unit = lane & 15;
   const bool in_cols = stage * kStageCols + unit * kUnit < p.cols;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if (row0 + 2 * u >= t.count) break;  // the same in all lanes
-    const int r = row0 + 2 * u + (lane >> 4);
-    float v[16];
-    to_floats(b.raw[u], v);
-    const Coded c = quantize16<FMT>(v, p.scale_mode, second);
-    const uint32_t word = gather_scales<FMT>(in_cols ? c.byte : 0u);
-    if (r < t.count) {
-      *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
-      constexpr int kLanes = FMT == kNV ? 4 : 8;  // units per scale tile
-      if (unit % kLanes == 0) *reinterpret_cast<uint32_t*>(scales + (unit / kLanes) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
-    }
+  const int r = row0 + (lane >> 4);
+  float v[16];
+  to_floats(b, v);
+  const Coded c = quantize16<FMT>(v, p.scale_mode, second);
+  const uint32_t word = gather_scales<FMT>(in_cols ? c.byte : 0u);
+  if (r < t.count) {
+    *reinterpret_cast<uint2*>(codes + r * kStageBytes + (((unit >> 1) ^ (r & 7)) << 4) + (unit & 1) * 8) = c.codes;
+    constexpr int kLanes = FMT == kNV ? 4 : 8;  // units per scale tile
+    if (unit % kLanes == 0) *reinterpret_cast<uint32_t*>(scales + (unit / kLanes) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
   }
 }
 
@@ -211,7 +201,7 @@ __device__ __forceinline__ void quantize_tokens(const LinearArgs& p, const TileA
 // producers and the tensor-core warp are up to two accumulators ahead of the
 // epilogue.
 template <int DT, int FMT, int BN, bool kFused>
-__global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
+__global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, LinearShape<FMT, BN, kFused>::kCtas)
     linear_kernel(const __grid_constant__ LinearArgs p) {
   using S = LinearShape<FMT, BN, kFused>;
   extern __shared__ uint8_t raw[];
@@ -473,7 +463,7 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
     for (int id = first_item; ok && have; have = next_tile(id)) {
       if (t.expert == p.groups.experts) continue;
       const int mine = warp - S::kFirstQuantWarp;
-      int i = from + ((mine - it) & (kQuantWarps - 1));  // every eighth stage is this warp's
+      int i = from + ((mine - it) & (kQuantWarps - 1));  // every fourth stage is this warp's
       TokenBlock<DT> next = first_tokens;
       if (it > 0 && i < to) next = load_tokens<DT>(p, t, i, 0);
       for (; i < to; i += kQuantWarps) {
@@ -485,7 +475,7 @@ __global__ void __launch_bounds__(LinearShape<FMT, BN, kFused>::kThreads, 1)
         if (!ok) break;
         uint8_t* at = smem + ring.slot * S::kStage;
         quantize_tokens<DT, FMT>(p, t, now, i, 0, at + S::kW, at + S::kW + S::kX + S::kSW, second);
-        for (int r0 = 8; r0 < t.count; r0 += 8)
+        for (int r0 = 2; r0 < t.count; r0 += 2)
           quantize_tokens<DT, FMT>(p, t, load_tokens<DT>(p, t, i, r0), i, r0, at + S::kW, at + S::kW + S::kX + S::kSW, second);
         pm::fence_proxy_async_smem();
         __syncwarp();
