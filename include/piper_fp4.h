@@ -78,7 +78,8 @@ int piper_fp4_grad_input_workspace(const piper_fp4_matrix* w, const void* dy, in
  * `scale_mode` for MXFP4 and the optional second-level scale `act_second` for
  * NVFP4. With `ends` (int32, w->batch of them, non-decreasing) matrix e
  * multiplies the rows [ends[e-1], ends[e]); rows past the last end become
- * zero. Without it w->batch is 1. The workspace is 256-byte aligned. */
+ * zero. An end below one before it counts as that one, one past the tokens as
+ * theirs. Without it w->batch is 1. The workspace is 256-byte aligned. */
 int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride, int64_t tokens, const int32_t* ends,
                      const float* act_second, int32_t scale_mode, void* y, int32_t dtype, void* workspace,
                      size_t workspace_bytes, void* stream);

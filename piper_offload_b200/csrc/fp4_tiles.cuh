@@ -25,9 +25,9 @@ struct TileAt {
 
 // The tile of work item `id`: token tiles are the inner index, so that the
 // tiles of one weight strip run together and its bytes are read from HBM once.
-// One warp calls; false past the last item. The ends are used as they are
-// found: values out of order give other rows' results, never an address
-// outside the buffers.
+// One warp calls; false past the last item. Ends are taken within the tokens,
+// and one below an end before it as that end, so that every row has one tile of
+// one expert; ends that are in order cost one vote for it.
 __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileAt& t) {
   const int tokens = static_cast<int>(p.tokens);
   if (p.ends == nullptr) {
@@ -42,14 +42,22 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
   }
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
+  int last = 0;  // the end before the first lane's
   for (int e0 = 0; e0 <= p.experts; e0 += 32) {
     const int e = e0 + lane;
-    int start = 0, n = 0;
-    if (e <= p.experts) {
-      start = e > 0 ? min(max(p.ends[e - 1], 0), tokens) : 0;
-      n = max((e < p.experts ? min(max(p.ends[e], 0), tokens) : tokens) - start, 0);
+    int start = e > 0 && e <= p.experts ? min(max(p.ends[e - 1], 0), tokens) : e > 0 ? tokens : 0;
+    int end = e < p.experts ? min(max(p.ends[e], 0), tokens) : tokens;
+    if (__any_sync(0xFFFFFFFFu, end < start || start < last)) {
+      end = max(end, last);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
+        if (lane >= o) end = max(end, up);
+      }
+      start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+      if (lane == 0) start = last;
     }
-    const int per = (n + bn - 1) / bn;
+    const int n = end - start, per = (n + bn - 1) / bn;
     int64_t sum = static_cast<int64_t>(per) * p.row_tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -73,6 +81,7 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
       return true;
     }
     before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    last = __shfl_sync(0xFFFFFFFFu, end, 31);
   }
   return false;
 }

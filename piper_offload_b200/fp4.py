@@ -333,6 +333,7 @@ def grouped_linear_fp4(x: torch.Tensor, experts: MXExperts | NVFP4Experts, group
     ``x`` is (tokens, cols); expert ``e`` has the rows ``group_ends[e - 1]`` to
     ``group_ends[e]`` (int32 on the device, non-decreasing, not read by the
     host). Experts may have no rows; rows past the last end come out as zeros.
+    An end below one before it counts as that one, one past the tokens as theirs.
     """
     _check_kind(experts, 3, "grouped_linear_fp4 takes a stack of experts and rank-two tokens.")
     if x.ndim != 2:
