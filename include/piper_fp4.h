@@ -41,7 +41,8 @@ enum { PIPER_FP4_BF16 = 0, PIPER_FP4_F32 = 2 };
 /* How the e8m0 exponent follows a block's maximum (MXFP4). */
 enum { PIPER_FP4_FLOOR = 0, PIPER_FP4_RCEIL = 1, PIPER_FP4_CEIL = 2, PIPER_FP4_EVEN = 3 };
 /* Second-level scale of a quantisation: none, read from `second`, or computed
- * as max(max|x| / 2688, 2^-23) of each matrix of the batch and written there. */
+ * as max(max|x| / 2688, 2^-23) over the finite values of each matrix of the
+ * batch and written there. */
 enum { PIPER_FP4_SECOND_NONE = 0, PIPER_FP4_SECOND_GIVEN = 1, PIPER_FP4_SECOND_COMPUTE = 2 };
 
 /* Matrices of at most so many values need no room for maxima (piper_fp4_quantize). */

@@ -108,7 +108,7 @@ struct QuantArgs {
   int32_t second_mode;
   int32_t reverse;       // walk from the end: the maximum pass left that in L2
   float* second;         // (batch): read (given) or written (compute)
-  const uint32_t* amax;  // (batch) bits of max|x| (compute)
+  const uint32_t* amax;  // (batch) bits of max|x| over finite values (compute)
   // tokens of experts
   const int32_t* ends;   // NULL: one weight for all
   int32_t experts;
@@ -326,10 +326,9 @@ __device__ __forceinline__ uint32_t gather_scales(uint32_t byte) {
   return word | (__shfl_down_sync(0xFFFFFFFFu, word, 2 * kLanes) << 16);
 }
 
-// The second-level scale that a maximum gives; not fmaxf: a NaN stays one.
+// The second-level scale that a finite maximum gives.
 __device__ __forceinline__ float second_of_amax(uint32_t amax) {
-  const float g = __fdiv_rn(__uint_as_float(amax), 2688.0f);
-  return g < 1.1920928955078125e-07f ? 1.1920928955078125e-07f : g;
+  return fmaxf(__fdiv_rn(__uint_as_float(amax), 2688.0f), 1.1920928955078125e-07f);
 }
 
 // A warp quantizes R rows (more where a row is short) x 512 columns of matrix e.
@@ -433,7 +432,8 @@ __global__ void __launch_bounds__(kQuantThreads, quant_ctas<DT>()) quantize_kern
   quantize_block<DT, FMT, R>(q, q.reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-// Bits of the largest magnitude of a warp's rows x 512 columns, in every lane.
+// Bits of the largest finite magnitude of a warp's rows x 512 columns, in every
+// lane: an infinity or a NaN would take the whole matrix's scale with it.
 template <int DT>
 __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int64_t row0, int chunk) {
   const int lane = threadIdx.x & 31, per = lanes_per_row(q.units);
@@ -458,10 +458,23 @@ __device__ __forceinline__ uint32_t amax_rows(const QuantArgs& q, int64_t e, int
     to_floats(raw[u], v);
     m = max(m, amax16(v));
   }
+  if (m >= 0x7F800000u) {  // rare: again without them
+    m = 0u;
+#pragma unroll
+    for (int u = 0; u < quant_rows<DT>(); ++u) {
+      float v[16];
+      to_floats(raw[u], v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+        m = max(m, bits < 0x7F800000u ? bits : 0u);
+      }
+    }
+  }
   return __reduce_max_sync(0xFFFFFFFFu, m);
 }
 
-// max|x| of each matrix as integer bits (order does not matter to a maximum).
+// max|x| over the finite values of each matrix as integer bits (order does not matter to a maximum).
 template <int DT>
 __global__ void __launch_bounds__(kQuantThreads) amax_kernel(const __grid_constant__ QuantArgs q, uint32_t* amax) {
   const int chunks = (q.units + 31) / 32, rows = 32 / lanes_per_row(q.units) * quant_rows<DT>();

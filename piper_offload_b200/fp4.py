@@ -18,7 +18,8 @@ largest magnitude ``a`` is stored as ``e2m1(clamp(x / s, -6, 6)) * s``, nearest
 with ties to even. MXFP4: ``s`` is a power of two that ``scaling_mode`` derives
 from ``a``. NVFP4: ``s = e4m3(clamp(a / 6 / g, 2**-6, 448)) * g``, where the
 second-level scale ``g`` is 1, given, or ``max(max|x| / 2688, 2**-23)`` over
-the matrix. A block that holds a NaN reads back as NaN; infinities saturate.
+the matrix's finite values. A block that holds a NaN reads back as NaN; an
+infinity saturates its block's scale.
 Products are over these values, summed in fp32 and rounded once to the type
 of the tokens. Second-level scales multiply the sum, so it is the sum before
 them that has to fit fp32.
