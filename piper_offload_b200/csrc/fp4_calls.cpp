@@ -50,10 +50,11 @@ bool attribute(PyObject* from, PyObject* name, Ref& to) {
   return to.o != nullptr;
 }
 
+// Without a forward-mode tangent, which the Python path refuses.
 const at::Tensor* plain_tensor(PyObject* o) {
   if (o == nullptr || !THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.layout() == at::kStrided ? &t : nullptr;
+  return t.is_cuda() && t.layout() == at::kStrided && !t._fw_grad(/*level=*/0).defined() ? &t : nullptr;
 }
 
 int dtype_of(const at::Tensor& t) {

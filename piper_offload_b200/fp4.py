@@ -11,7 +11,9 @@ and their stacks of experts), on sm_100a kernels of ``libpiper_fp4.so``:
   sorted by expert and the ends of their groups on the device;
 * :func:`linear_fp4_grad_input`, :func:`grouped_linear_fp4_grad_input`: the
   gradients with respect to the tokens. The two products are differentiable:
-  they use these when their input requires a gradient.
+  they use these when their input requires a gradient. Weights and second-level
+  scales are constants, the gradients are not differentiable themselves, and
+  inputs with a forward-mode tangent are refused.
 
 Definitions. A block of a row (32 values in MXFP4, 16 in NVFP4) with the
 largest magnitude ``a`` is stored as ``e2m1(clamp(x / s, -6, 6)) * s``, nearest
@@ -37,6 +39,7 @@ import ctypes
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native_fp4 as nat
 from . import kernels as K
@@ -233,6 +236,11 @@ def _check_kind(weight: Any, dims: int, message: str) -> None:
         raise ValueError(message)
 
 
+def _check_tangents(*tensors: torch.Tensor | None) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("FP4 operators have no forward-mode derivatives; detach the input's tangent.")
+
+
 def _check_ends(ends: torch.Tensor, batch: int, device: torch.device) -> None:
     if ends.dtype is not torch.int32 or ends.ndim != 1 or ends.shape[0] != batch or not ends.is_contiguous():
         raise ValueError("Group ends are one contiguous int32 vector with an entry per expert.")
@@ -244,6 +252,7 @@ def _linear(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: 
     done = nat.calls().linear(x, weight, ends, act_scale)
     if done is not None:
         return done
+    _check_tangents(x, act_scale)
     m, mode, q = _matrix(weight)
     device = q.device
     if x.device != device:
@@ -272,6 +281,7 @@ def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> t
     done = nat.calls().grad_input(grad, weight, ends)
     if done is not None:
         return done
+    _check_tangents(grad)
     m, _, q = _matrix(weight)
     device = q.device
     if grad.device != device:
@@ -309,6 +319,7 @@ class _Product(torch.autograd.Function):
 
 def _product(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: torch.Tensor | None) -> torch.Tensor:
     if x.requires_grad and torch.is_grad_enabled():
+        _check_tangents(x, act_scale)
         return _Product.apply(x, weight, ends, act_scale)
     return _linear(x, weight, ends, act_scale)
 
