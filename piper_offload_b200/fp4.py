@@ -303,18 +303,36 @@ def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> t
     return dx
 
 
+class _Frozen:
+    """The parts of a weight as its product found them, for the backward pass: a part that is put in another's place
+    in between changes nothing. Not saved tensors, since hooks on those would move a weight that stays in use."""
+
+    def __init__(self, weight: Any):
+        for name in ("qdata", "scale", "per_tensor_scale", "block_size", "elem_dtype", "is_swizzled_scales", "act_quant_kwargs"):
+            if hasattr(weight, name):
+                setattr(self, name, getattr(weight, name))
+        tensors = (self.qdata, self.scale, getattr(self, "per_tensor_scale", None))
+        self._versions = [(t, t._version) for t in tensors if t is not None and not t.is_inference()]
+
+    def check(self) -> None:
+        if any(t._version != version for t, version in self._versions):
+            raise RuntimeError("a tensor of an FP4 weight has been modified by an inplace operation since its product, "
+                               "whose gradient needs it as it was.")
+
+
 class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, ends, act_scale):
-        # saved so that a buffer changed by torch before the backward pass raises instead of giving another's gradient
-        ctx.save_for_backward(weight.qdata, weight.scale, getattr(weight, "per_tensor_scale", None), ends)
-        ctx.weight = weight
+        ctx.save_for_backward(ends)
+        ctx.weight = _Frozen(weight)
         return _linear(x, weight, ends, act_scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        return _grad_input(grad, ctx.weight, ctx.saved_tensors[3]), None, None, None
+        (ends,) = ctx.saved_tensors
+        ctx.weight.check()
+        return _grad_input(grad, ctx.weight, ends), None, None, None
 
 
 def _product(x: torch.Tensor, weight: Any, ends: torch.Tensor | None, act_scale: torch.Tensor | None) -> torch.Tensor:
@@ -331,8 +349,10 @@ def linear_fp4(x: torch.Tensor, weight: MXWeight | NVFP4Weight, *,
     ``x`` is quantised in the weight's format: MXFP4 with the weight's
     ``act_quant_kwargs.scaling_mode``, NVFP4 with the second-level scale
     ``act_per_tensor_scale`` where one is given. Differentiable with respect to
-    ``x`` (straight through its quantisation); the weight is constant. A merge
-    into it between the two passes is not noticed: the gradient is the merged one's.
+    ``x`` (straight through its quantisation); the weight is constant. Between the
+    two passes its tensors may be replaced, and an operation of torch that
+    changes them raises. A merge into them is not noticed: the gradient is the
+    merged one's.
     """
     _check_kind(weight, 2, "linear_fp4 takes one weight; grouped_linear_fp4 takes a stack of experts.")
     return _product(x, weight, None, act_per_tensor_scale)
