@@ -114,18 +114,23 @@ def _matrix(w: Any) -> tuple[nat.Matrix, int, torch.Tensor]:
     return m, mode, q
 
 
-def _call(function: Any, device: torch.device, *args: Any) -> None:
-    """A library call on the current stream of ``device``, which is entered where it is not the current one."""
+def _on(device: torch.device, function: Any, *args: Any) -> None:
+    """A library call with ``device`` current: plans and launches alike depend on it."""
     if torch.cuda.current_device() == device.index:
-        nat.check(function(*args, nat.raw_stream(device.index)))
+        nat.check(function(*args))
     else:
         with torch.cuda.device(device):
-            nat.check(function(*args, nat.raw_stream(device.index)))
+            nat.check(function(*args))
+
+
+def _call(function: Any, device: torch.device, *args: Any) -> None:
+    """A library call on the current stream of ``device``."""
+    _on(device, function, *args, nat.raw_stream(device.index))
 
 
 def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor | None:
     need = ctypes.c_size_t()
-    nat.check(query(*args, ctypes.byref(need)))
+    _on(device, query, *args, ctypes.byref(need))
     return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
 
 
