@@ -2,7 +2,8 @@
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
 ``__graft_entry__.build()``). A library newer than every source file of its
-own is left as it is.
+own is left as it is, the calls if they were also built for this interpreter
+and torch.
 """
 
 from __future__ import annotations
@@ -80,10 +81,12 @@ def build_fp4(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
-    """The operators' calls from Python: host code against this interpreter's torch."""
-    if force or not up_to_date(CALLS_OUT, CALLS_DEPS):
-        import torch
+    """The operators' calls from Python: host code against this interpreter's torch, which is noted beside it."""
+    import torch
 
+    fits = f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    note = CALLS_OUT.with_suffix(".so.fits")
+    if force or not up_to_date(CALLS_OUT, CALLS_DEPS) or not note.exists() or note.read_text() != fits:
         base = Path(torch.__file__).resolve().parent
         tmp = CALLS_OUT.with_suffix(".so.tmp")
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
@@ -95,6 +98,7 @@ def build_calls(force: bool = False, verbose: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=str(ROOT))
         os.replace(tmp, CALLS_OUT)
+        note.write_text(fits)
     return CALLS_OUT
 
 
