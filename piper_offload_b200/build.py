@@ -9,6 +9,7 @@ and torch.
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -45,7 +46,7 @@ NVCC_FLAGS = [
 
 def nvcc() -> str:
     cand = os.environ.get("NVCC") or "/usr/local/cuda/bin/nvcc"
-    return cand if Path(cand).exists() else "nvcc"
+    return cand if Path(cand).exists() else shutil.which("nvcc") or "nvcc"
 
 
 def up_to_date(out: Path = OUT, deps: list[Path] = DEPS) -> bool:

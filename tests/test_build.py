@@ -65,3 +65,20 @@ def test_a_failed_build_is_tried_again(commands, monkeypatch):
                 build.build_calls()
     build.build_calls()
     assert len(commands) == 2
+
+
+def test_cuda_headers_come_from_the_compiler_that_is_found(commands, monkeypatch, tmp_path):
+    """With nvcc on PATH alone its headers are the toolkit's beside it, through links too."""
+    toolkit = tmp_path / "toolkit"
+    (toolkit / "bin").mkdir(parents=True)
+    real = toolkit / "bin" / "nvcc"
+    real.write_text("#!/bin/sh\n")
+    real.chmod(0o755)
+    links = tmp_path / "links"
+    links.mkdir()
+    (links / "nvcc").symlink_to(real)
+    monkeypatch.setenv("NVCC", str(tmp_path / "none"))
+    for folder in (toolkit / "bin", links):
+        monkeypatch.setenv("PATH", str(folder))
+        build.build_calls(force=True)
+        assert f"-I{toolkit / 'include'}" in commands[-1]
