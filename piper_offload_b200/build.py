@@ -67,10 +67,10 @@ def _compile(out: Path, sources: list[Path], verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """The merges' library; the FP4 operators' is built beside it."""
-    build_fp4(force, verbose)
+    """The merges' library, and then the FP4 operators' beside it."""
     if force or not up_to_date():
         _compile(OUT, SOURCES, verbose)
+    build_fp4(force, verbose)
     return OUT
 
 

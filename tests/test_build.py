@@ -82,3 +82,18 @@ def test_cuda_headers_come_from_the_compiler_that_is_found(commands, monkeypatch
         monkeypatch.setenv("PATH", str(folder))
         build.build_calls(force=True)
         assert f"-I{toolkit / 'include'}" in commands[-1]
+
+
+def test_the_merges_do_not_wait_for_the_calls_compiler(commands, monkeypatch):
+    """Without a host compiler for the FP4 calls the merges' library is built all the same, and the error is raised."""
+    run = build.subprocess.run
+
+    def only_nvcc(cmd, **kwargs):
+        if "nvcc" not in cmd[0]:
+            raise FileNotFoundError(cmd[0])
+        run(cmd, **kwargs)
+
+    monkeypatch.setattr(build.subprocess, "run", only_nvcc)
+    with pytest.raises(FileNotFoundError):
+        build.build(force=True)
+    assert build.OUT.exists() and build.FP4_OUT.exists() and not build.CALLS_OUT.exists()
