@@ -91,6 +91,21 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
                          const int32_t* ends, void* dx, int32_t dtype, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* How the product of `tokens` tokens, or its gradient, runs on the current
+ * device: what its tiles are and who works on them. Results do not depend on
+ * it but for the order of sums. */
+typedef struct piper_fp4_plan {
+  int32_t tile_tokens;
+  int32_t tile_columns; /* of y, or of dx */
+  int32_t split;        /* blocks that share the sums of a tile */
+  int32_t fused;        /* the product quantises its tokens itself */
+} piper_fp4_plan;
+
+int piper_fp4_linear_plan(const piper_fp4_matrix* w, int64_t tokens, piper_fp4_plan* plan);
+/* `grouped`: with the ends of the matrices' rows. */
+int piper_fp4_grad_input_plan(const piper_fp4_matrix* w, int64_t tokens, int32_t grouped, int32_t dtype,
+                              piper_fp4_plan* plan);
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char* piper_fp4_last_error(void);
 

@@ -34,6 +34,8 @@ EXPORTED_SYMBOLS = (
     "piper_fp4_grad_input_workspace",
     "piper_fp4_linear",
     "piper_fp4_grad_input",
+    "piper_fp4_linear_plan",
+    "piper_fp4_grad_input_plan",
     "piper_fp4_last_error",
     "piper_fp4_device_status",
     "piper_fp4_version",
@@ -54,6 +56,13 @@ class Matrix(ctypes.Structure):
         ("format", ctypes.c_int32),
         ("swizzled", ctypes.c_int32),
     ]
+
+
+class Plan(ctypes.Structure):
+    """Mirror of ``piper_fp4_plan``."""
+
+    _fields_ = [("tile_tokens", ctypes.c_int32), ("tile_columns", ctypes.c_int32), ("split", ctypes.c_int32),
+                ("fused", ctypes.c_int32)]
 
 
 _lib = None
@@ -87,8 +96,10 @@ def load() -> ctypes.CDLL:
         lib.piper_fp4_grad_input_workspace.argtypes = [mat, vp, i64, i64, i32, ctypes.POINTER(sz)]
         lib.piper_fp4_linear.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, i32, vp, sz, vp]
         lib.piper_fp4_grad_input.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, sz, vp]
+        lib.piper_fp4_linear_plan.argtypes = [mat, i64, ctypes.POINTER(Plan)]
+        lib.piper_fp4_grad_input_plan.argtypes = [mat, i64, i32, i32, ctypes.POINTER(Plan)]
         lib.piper_fp4_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint32)]
-        for name in EXPORTED_SYMBOLS[:6] + ("piper_fp4_device_status",):
+        for name in EXPORTED_SYMBOLS[:8] + ("piper_fp4_device_status",):
             getattr(lib, name).restype = ctypes.c_int
         lib.piper_fp4_last_error.restype = ctypes.c_char_p
         lib.piper_fp4_version.restype = ctypes.c_char_p
@@ -145,6 +156,20 @@ def device_status(device: torch.device) -> int:
 
 def version() -> str:
     return load().piper_fp4_version().decode()
+
+
+def linear_plan(m: Matrix, tokens: int) -> Plan:
+    """How the product of a matrix (or a stack of them) and ``tokens`` tokens runs on the current device."""
+    plan = Plan()
+    check(load().piper_fp4_linear_plan(ctypes.byref(m), tokens, ctypes.byref(plan)))
+    return plan
+
+
+def grad_input_plan(m: Matrix, tokens: int, *, grouped: bool, dtype: int) -> Plan:
+    """How the product's gradient runs."""
+    plan = Plan()
+    check(load().piper_fp4_grad_input_plan(ctypes.byref(m), tokens, grouped, dtype, ctypes.byref(plan)))
+    return plan
 
 
 def launches() -> int:

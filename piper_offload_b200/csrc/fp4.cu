@@ -219,9 +219,10 @@ bool code_map(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t pit
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, row_bytes, rows, pitch, fp4::kStageBytes, box_rows);
 }
 
-// Token tiles of all experts and of the rows after them: an upper bound where the ends are on the device.
-int64_t token_tiles(const fp4::Groups& g, int bn) {
-  return g.ends == nullptr ? (g.tokens + bn - 1) / bn : g.tokens / bn + std::min<int64_t>(g.experts + 1, g.tokens);
+// Token tiles of all experts and of the rows after them (an upper bound: the ends are on the device), or of one
+// weight's tokens (0 experts).
+int64_t token_tiles(int64_t tokens, int64_t experts, int bn) {
+  return experts == 0 ? (tokens + bn - 1) / bn : tokens / bn + std::min<int64_t>(experts + 1, tokens);
 }
 
 template <int DT, int FMT, int BN, bool kFused>
@@ -258,9 +259,11 @@ struct GradPlan {
   int64_t total;  // bytes
 };
 
+int grad_terms(int dtype) { return dtype == PIPER_FP4_F32 ? 3 : 1; }
+
 GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, int64_t tokens, int dtype) {
   GradPlan p{};
-  p.terms = dtype == PIPER_FP4_F32 ? 3 : 1;
+  p.terms = grad_terms(dtype);
   p.move = p.terms > 1 || !aligned(dy, 16) || (stride % 8 != 0 && tokens > 1);
   p.pitch = up(w.rows, 8);
   p.total = p.move ? align256(p.terms * tokens * p.pitch * 2) : 0;
@@ -274,26 +277,34 @@ GradPlan plan_grad(const piper_fp4_matrix& w, const void* dy, int64_t stride, in
 // stage: 1060 and 600; 2048 x 14336 x 4096 198 us against 231 with 128 columns,
 // 512 x 4096 x 4096 60 against 25.8).
 struct GradTile {
-  int bn, rows;
+  int bn, rows, split;
+  int64_t items;  // bound on the tiles
 };
-GradTile grad_tile(const piper_fp4_matrix& w, int64_t tokens) {
+GradTile grad_tile(const piper_fp4_matrix& w, int64_t tokens, int terms, bool grouped) {
   const int64_t per_expert = tokens / w.batch;
-  if (per_expert <= 48) return {64, 1};
-  const auto waves = [&](int64_t cols) {
-    const int64_t tiles = w.batch * ((per_expert + 255) / 256) * ((w.cols + cols - 1) / cols);
-    return static_cast<double>((tiles + sm_count() - 1) / sm_count());
-  };
-  return waves(256) * 1060.0 <= waves(128) * 600.0 ? GradTile{256, 2} : GradTile{256, 1};
+  GradTile t{256, 1, 1, 0};
+  if (per_expert <= 48) {
+    t.bn = 64;
+  } else {
+    const auto waves = [&](int64_t cols) {
+      const int64_t tiles = w.batch * ((per_expert + 255) / 256) * ((w.cols + cols - 1) / cols);
+      return static_cast<double>((tiles + sm_count() - 1) / sm_count());
+    };
+    if (waves(256) * 1060.0 <= waves(128) * 600.0) t.rows = 2;
+  }
+  t.items = token_tiles(tokens, grouped ? w.batch : 0, t.bn) * ((w.cols + 128 * t.rows - 1) / (128 * t.rows));
+  const int64_t stages = (w.rows + fp4::kGradStageRows - 1) / fp4::kGradStageRows * terms;
+  t.split = plan_tile(t.bn, t.items, stages, 600.0, std::min<int64_t>(tokens, t.bn), t.rows == 1 && !grouped, sm_count()).split;
+  return t;
 }
 
 template <int DT, int FMT, int BN, int kRows>
-cudaError_t launch_grad(fp4::GradArgs& args, int64_t items, cudaStream_t stream) {
+cudaError_t launch_grad(const fp4::GradArgs& args, int64_t items, cudaStream_t stream) {
   using S = fp4::GradShape<BN, kRows>;
+  static_assert(S::kCanSplit == (kRows == 1), "the plan splits tiles of 128 columns");
   auto kernel = fp4::grad_kernel<DT, FMT, BN, kRows>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  const int stages = (args.rows + fp4::kGradStageRows - 1) / fp4::kGradStageRows * args.terms;
-  args.split = plan_tile(BN, items, stages, 600.0, std::min<int64_t>(args.groups.tokens, BN), S::kCanSplit && args.groups.ends == nullptr, sm_count()).split;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
   attribute.val.clusterDim.x = static_cast<unsigned>(args.split);
@@ -464,7 +475,7 @@ int piper_fp4_linear(const piper_fp4_matrix* w, const void* x, int64_t x_stride,
     for (a.scale_piece = 16; a.scale_piece > 1 && (a.scale_cols % a.scale_piece != 0 || !aligned(w->scale, a.scale_piece));)
       a.scale_piece /= 2;
   }
-  const int64_t items = token_tiles(a.groups, p.bn) * a.groups.row_tiles;
+  const int64_t items = token_tiles(tokens, ends == nullptr ? 0 : w->batch, p.bn) * a.groups.row_tiles;
   a.items = static_cast<int32_t>(items);
   FP4_REQUIRE(items < (int64_t{1} << 31) / fp4::kMaxSplit, "FP4 product: too many tiles for one call.");
 
@@ -560,7 +571,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   a.codes = static_cast<const uint8_t*>(w->codes);
   a.scale = static_cast<const uint8_t*>(w->scale);
   a.second = w->second;
-  const GradTile tile = grad_tile(*w, tokens);
+  const GradTile tile = grad_tile(*w, tokens, p.terms, ends != nullptr);
   a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 128 * tile.rows - 1) / (128 * tile.rows))};
   a.dx = dx;
   a.code_pitch = w->cols / 2;
@@ -569,6 +580,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   a.swizzled = w->swizzled != 0;
   a.scale_cols = scale_cols(*w);
   a.terms = p.terms;
+  a.split = tile.split;
   a.vec = aligned(dx, 16) && w->cols % 8 == 0;
   a.piece = aligned(w->codes, 16) && a.code_pitch % 16 == 0 ? 16 : aligned(w->codes, 8) ? 8 : 1;
 
@@ -577,7 +589,7 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   const int64_t pitch = p.move ? p.pitch : tokens > 1 ? dy_stride : up(w->rows, 8);
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, src, w->rows, p.terms * tokens, pitch * 2, fp4::kGradStageRows, bn))
     return fail(PIPER_FP4_ECUDA, "FP4 gradient: cuTensorMapEncodeTiled failed.");
-  const int64_t items = token_tiles(a.groups, bn) * a.groups.row_tiles;
+  const int64_t items = tile.items;
   const int64_t split_blocks = tokens * ((w->rows + 255) / 256);
   FP4_REQUIRE(items < (int64_t{1} << 31) / fp4::kMaxSplit && split_blocks < (int64_t{1} << 31), "FP4 gradient: too many tiles for one call.");
   cudaError_t e = cudaSuccess;
@@ -593,6 +605,23 @@ int piper_fp4_grad_input(const piper_fp4_matrix* w, const void* dy, int64_t dy_s
   FP4_DISPATCH(dtype, w->format, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_FP4_OK : cuda_fail("gradient kernel", e);
+}
+
+int piper_fp4_linear_plan(const piper_fp4_matrix* w, int64_t tokens, piper_fp4_plan* plan) {
+  if (int rc = check_matrix(w)) return rc;
+  FP4_REQUIRE(plan != nullptr && tokens > 0, "FP4 product: bad plan query.");
+  const LinearPlan p = plan_linear(*w, tokens);
+  *plan = {p.bn, 128, p.split, p.fused};
+  return PIPER_FP4_OK;
+}
+
+int piper_fp4_grad_input_plan(const piper_fp4_matrix* w, int64_t tokens, int32_t grouped, int32_t dtype, piper_fp4_plan* plan) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  FP4_REQUIRE(plan != nullptr && tokens > 0 && (grouped != 0 || w->batch == 1), "FP4 gradient: bad plan query.");
+  const GradTile t = grad_tile(*w, tokens, grad_terms(dtype), grouped != 0);
+  *plan = {t.bn, 128 * t.rows, t.split, 0};
+  return PIPER_FP4_OK;
 }
 
 const char* piper_fp4_last_error(void) { return g_error; }

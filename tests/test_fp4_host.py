@@ -183,3 +183,36 @@ def test_reference_places_are_the_oracles():
     for rows, blocks in ((1, 1), (70, 13), (128, 4), (300, 9)):
         for swizzled in (False, True):
             np.testing.assert_array_equal(R.scale_places(rows, blocks, swizzled), M.scale_index(rows, blocks, swizzled))
+
+
+# ------------------------------------------------------------------------ plans
+def test_plan_queries():
+    """Without a device the plan is made for 148 SMs."""
+    def linear(tokens, **kw):
+        p = nat.linear_plan(matrix(**kw), tokens)
+        return p.tile_tokens, p.tile_columns, p.split, p.fused
+
+    def grad(tokens, dtype=nat.DT_BF16, **kw):
+        p = nat.grad_input_plan(matrix(**kw), tokens, grouped=kw.get("batch", 1) > 1, dtype=dtype)
+        return p.tile_tokens, p.tile_columns, p.split, p.fused
+
+    for tokens in (1, 40, 700, 5000):
+        tile, columns, split, fused = linear(tokens, rows=4096, cols=4096)
+        assert tile in (32, 128, 192) and columns == 128 and split in (1, 2, 4, 8) and fused == (tokens <= 2)
+        tile, columns, split, fused = grad(tokens, rows=4096, cols=4096)
+        assert tile in (64, 256) and columns in (128, 256) and not fused
+        assert split == 1 or columns == 128
+    # sums of groups, whose tiles are found on the device, and of wide tiles are not shared
+    assert linear(64, batch=8, rows=128, cols=8192)[2] == grad(64, batch=8, rows=8192, cols=128)[2] == 1
+    m = matrix()
+    for call in (lambda: nat.linear_plan(m, 0), lambda: nat.grad_input_plan(m, 0, grouped=False, dtype=0),
+                 lambda: nat.grad_input_plan(matrix(batch=2), 8, grouped=False, dtype=0)):
+        with pytest.raises(ValueError, match="plan query"):
+            call()
+    with pytest.raises(ValueError, match="bfloat16 and float32"):
+        nat.grad_input_plan(m, 8, grouped=False, dtype=1)
+    for change, match in BAD_MATRICES:
+        with pytest.raises(ValueError, match=match):
+            nat.linear_plan(matrix(**change), 8)
+        with pytest.raises(ValueError, match=match):
+            nat.grad_input_plan(matrix(**change), 8, grouped=True, dtype=0)
