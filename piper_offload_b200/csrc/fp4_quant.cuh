@@ -69,18 +69,16 @@ __host__ __device__ __forceinline__ int64_t first_scale_row(int64_t start, int64
 // serves all rows (a search by halves a lane took five, 2 us of a 4 us launch).
 __device__ __forceinline__ void experts_of_rows(const int32_t* ends, int experts, int64_t row0, int rows, int& expert, int& start) {
   const int lane = threadIdx.x & 31;
-  bool found = false;
   expert = start = 0;
   for (int e0 = 0; e0 < experts; e0 += 32) {
     const int32_t v = e0 + lane < experts ? max(ends[e0 + lane], 0) : 0x7FFFFFFF;
     for (int j = 0; j < rows; ++j) {
-      const uint32_t past = __ballot_sync(0xFFFFFFFFu, v > row0 + j);
-      const int n = past != 0u ? __ffs(past) - 1 : 32;
-      const int32_t before = __reduce_max_sync(0xFFFFFFFFu, lane < n ? v : 0);
-      if (lane == j && !found) {
-        expert += n;
+      // lanes below the first past end
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, v > row0 + j), first = past & (0u - past);
+      const int32_t before = __reduce_max_sync(0xFFFFFFFFu, (first - 1u) >> lane & 1u ? v : 0);
+      if (lane == j && expert == e0) {
+        expert += __popc(first - 1u);
         start = max(start, before);
-        found = past != 0u;
       }
     }
   }
@@ -362,7 +360,7 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& q, int e, int row
     const int r = row0 + lane;
     int x = 0, start = 0;
     if (q.ends != nullptr) experts_of_rows(q.ends, q.experts, row0, R * step, x, start);
-    if (x >= q.experts) {
+    if (x >= q.experts || start < 0 || start > r) {
       place = -1;  // a row of no expert
     } else {
       const int o = r - start, tile = o / q.token_tile;

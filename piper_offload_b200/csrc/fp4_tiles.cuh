@@ -27,7 +27,8 @@ struct TileAt {
 // tiles of one weight strip run together and its bytes are read from HBM once.
 // One warp calls; false past the last item. Ends are taken within the tokens,
 // and one below an end before it as that end, so that every row has one tile of
-// one expert; ends that are in order cost one vote for it.
+// one expert: a vote where they are in order. Few instructions, since every role
+// of a block has a copy (a scan by halves cost 24 x 4096 x 4096 MXFP4 0.2 us of 9).
 __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileAt& t) {
   const int tokens = static_cast<int>(p.tokens);
   if (p.ends == nullptr) {
@@ -41,37 +42,30 @@ __device__ __forceinline__ bool find_tile(const Groups& p, int id, int bn, TileA
     return t.row_tile < p.row_tiles;
   }
   const int lane = threadIdx.x & 31;
-  int64_t before = 0;
+  int before = 0;  // tiles of tokens
   int last = 0;  // the end before the first lane's
   for (int e0 = 0; e0 <= p.experts; e0 += 32) {
     const int e = e0 + lane;
-    int start = e > 0 && e <= p.experts ? min(max(p.ends[e - 1], 0), tokens) : e > 0 ? tokens : 0;
-    int end = e < p.experts ? min(max(p.ends[e], 0), tokens) : tokens;
-    if (__any_sync(0xFFFFFFFFu, end < start || start < last)) {
-      end = max(end, last);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xFFFFFFFFu, end, o);
-        if (lane >= o) end = max(end, up);
-      }
+    int start, end = e < p.experts ? min(max(p.ends[e], 0), tokens) : tokens;
+    for (;; end = max(end, start)) {
       start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
       if (lane == 0) start = last;
+      if (!__any_sync(0xFFFFFFFFu, end < start)) break;
     }
     const int n = end - start, per = (n + bn - 1) / bn;
-    int64_t sum = static_cast<int64_t>(per) * p.row_tiles;
+    int sum = per;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
       if (lane >= o) sum += up;
     }
-    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + sum > id);
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, static_cast<int64_t>(before + sum) * p.row_tiles > id);
     if (hit != 0u) {
       const int l = __ffs(hit) - 1;
       const int per_l = __shfl_sync(0xFFFFFFFFu, per, l);
       const int start_l = __shfl_sync(0xFFFFFFFFu, start, l);
       const int n_l = __shfl_sync(0xFFFFFFFFu, n, l);
-      const int64_t base = before + __shfl_sync(0xFFFFFFFFu, sum, l) - static_cast<int64_t>(per_l) * p.row_tiles;
-      const int in = static_cast<int>(id - base);
+      const int in = id - (before + __shfl_sync(0xFFFFFFFFu, sum, l) - per_l) * p.row_tiles;
       t.expert = e0 + l;
       t.row_tile = in / per_l;
       const int nt = in - t.row_tile * per_l;
