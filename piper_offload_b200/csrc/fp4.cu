@@ -174,10 +174,11 @@ LinearPlan plan_linear(const piper_fp4_matrix& w, int64_t tokens) {
   LinearPlan p{};
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
   // One or two tokens a weight, and few enough tiles that no block quantizes them again for another: one launch less
-  // (5.5 us of host time against 8.6). On the device, fused against prepared: 1 x 14336 x 4096 NVFP4 10.1 and 10.4 us,
-  // 1 x 28672 x 4096 15.2 and 17.6, 2 x 4096 x 4096 MXFP4 6.3 and 7.3, 8 rows over 8 experts of 2816 x 1024 6.1 and 8.2.
+  // (5.8 us of host time against 8.6). On the device, fused against prepared: 1 x 14336 x 4096 NVFP4 9.6 and 10.0 us,
+  // 1 x 28672 x 4096 14.5 and 17.5, 2 x 4096 x 4096 MXFP4 6.2 and 7.3, 8 rows over 8 experts of 2816 x 1024 6.3 and 8.0.
   // A block quantizes two tokens of a stage at a time, so the product of both is bounded in case one expert has all the
-  // rows (128 over 64 experts of 512 x 1024 NVFP4: 8.0 and 8.7 us evenly, 13.1 and 7.2 most in one).
+  // rows (128 over 64 experts of 512 x 1024 NVFP4, fused without that bound: 8.0 us evenly, 13.1 with most in one;
+  // prepared 8.4 and 7.3).
   const int64_t stages = (w.cols + fp4::kStageCols - 1) / fp4::kStageCols;
   p.fused = tokens / w.batch <= 2 && std::min(w.batch, tokens) * ((w.rows + 127) / 128) <= fp4::kFusedCtas * sm_count() &&
             (w.batch == 1 || tokens * stages <= 128);

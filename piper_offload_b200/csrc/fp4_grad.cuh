@@ -10,18 +10,21 @@
 // thread and 128 columns, loaded two stages ahead, looked up by byte permutes,
 // scaled by packed bf16 products and written in the 128-byte swizzle.
 //
-// Bound: shared memory, then the bf16 tensor pipe. A stage of 256 columns x 256
-// tokens keeps the pipe busy for 1024 cycles; the pipe reads 96 KB for it and 64
-// are written, 1280 cycles at 128 bytes each, and decoding takes its warps about
-// 900 issue slots of each scheduler. 2048 x 14336 x 4096 NVFP4: 198 us, 1.2
-// PFLOP/s, on 128 of the 148 SMs, the pipe active 53 % of the time; copies and
-// products without the decoding would take 176, decoding with a quarter of the
-// products 174. In tiles of 128 columns, whose stages bring 36 KB for 512 cycles, 231. Few tokens: decoding,
-// since every value of w is decoded once a tile; 64 x 4096 x 4096 MXFP4 14.2 us
-// (cluster of 4, without it 36.5).
+// A stage of 256 columns x 256 tokens keeps the pipe busy for 1024 cycles; the
+// pipe reads 96 KB for it and 64 are written, 1280 cycles at 128 bytes each, and
+// decoding takes its warps about 900 issue slots of each scheduler, 320 of them
+// conversion. A stage takes about 1740 cycles: 2048 x 14336 x 4096 NVFP4 199 us, 1.2
+// PFLOP/s (240 in a running program, under the power cap), on 128 of the 148 SMs,
+// the pipe active 53 % of the time. Neither side alone bounds it: copies and products
+// without the decoding would take 176, decoding with a quarter of the products 174.
+// In tiles of 128 columns, whose stages bring 36 KB for 512 cycles, 231. Few tokens:
+// decoding, since every value of w is decoded once a tile; 64 x 4096 x 4096 MXFP4
+// 14.2 us (cluster of 4, without it 36.5).
 //
 // fp32 gradients are the sum of three bf16 terms (24 bits): the stages go
-// over the weight once per term.
+// over the weight once per term (2048 x 14336 x 4096 720 to 740 us). The tensor
+// core's fp32 additions lose more than rounding to nearest would: over 14336 rows
+// 5.5e-6 of the result's norm, against 4.4e-7.
 #pragma once
 #include <cuda.h>
 

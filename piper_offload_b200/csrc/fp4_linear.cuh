@@ -19,15 +19,23 @@
 // memory and every block adds up its share of the tokens over the cluster, in
 // rank order, so that results do not depend on timing.
 //
-// Bounds and times on a B200, whole calls. Few tokens: HBM, after about 5 us of
-// launch and first loads; 1 x 14336 x 4096 NVFP4 9.6 us (3.4 TB/s), x 28672 14.9 (4.4), 16 tokens
-// over 8 experts of 14336 x 4096 two-level 37.8 us (5.3 TB/s). Many: what shared
-// memory gives the tensor core. A 128 x 192 step of 64 values keeps it for 96
-// cycles and brings 11.5 KB in and out again, about 184 cycles at 128 bytes; 170 to
-// 176 a step are measured. 4096 x 14336 x 4096 NVFP4 133 us
-// (3.6 PFLOP/s), its tokens' quantisation included; 2048 x 4096 x 4096 MXFP4 26 us
-// (2.6 PFLOP/s). Wider tiles do not fit beside two accumulators; 256 x 192 over a
-// pair of SMs took 226 us.
+// Times on a B200, whole calls back to back at 1965 MHz, and what bounds them.
+// Few tokens: HBM, after about 5 us of launch and first loads; 1 x 14336 x 4096
+// NVFP4 9.6 us (3.5 TB/s; called from a program 10.3), x 28672 14.5 (4.6), 16 tokens
+// over 8 experts of 14336 x 4096 two-level 38.0 us (5.2 TB/s). Many: not known.
+// 4096 x 14336 x 4096, the tokens' quantisation included, takes 135 us in NVFP4
+// (3.6 PFLOP/s, the pipe 43 % active; 164 us in a running program, under the power
+// cap) and 117 in MXFP4 (4.1), which has half the scales and a buffer of them in
+// tensor memory for each stage, where NVFP4 has two for four stages. What a step of
+// 64 values brings into shared memory and out again, 11.5 KB each at 128 bytes a
+// cycle, would take more than the 170 to 176 cycles measured, so that account does
+// not hold. 2048 x 4096 x 4096 MXFP4 26 us (2.6 PFLOP/s). Wider tiles do not fit
+// beside two accumulators; 256 x 192 over a pair of SMs took 226 us.
+//
+// Weight scales in rows are read by one warp, in pieces as wide as their count a
+// row allows. In single bytes or pairs that warp sets the pace: 1 x 4096 x 2880
+// MXFP4 (90 scales a row) 23.5 us, 6.1 from swizzled tiles; 333 tokens 25.4 and
+// 9.6; x 2896 NVFP4 (181) 55 and 20. With 128 scales a row 8.5 and 7.
 #pragma once
 #include <cuda.h>
 
@@ -92,7 +100,7 @@ struct LinearShape {
   static constexpr int kBufs = (512 / kCtas - 2 * BN) / kScaleCols < kStages ? (512 / kCtas - 2 * BN) / kScaleCols : kStages;
   static constexpr int kCols = 2 * BN + kBufs * kScaleCols;
   // with fewer buffers than stages the copies of scales wait for products, and get a warp of their own: 4096 tokens x
-  // 14336 x 4096 NVFP4 136 us against 145 (as measured when it was added); with a buffer per stage one warp does both, 6 to 10 % faster on small calls
+  // 14336 x 4096 NVFP4 136 us against 145; with a buffer per stage one warp does both, 6 to 10 % faster on small calls
   static constexpr bool kCopyWarp = kBufs < kStages;
   static constexpr int kFirstQuantWarp = kCopyWarp ? 8 : 7;
   static constexpr int kThreads = 32 * kFirstQuantWarp + (kFused ? 32 * kQuantWarps : 0);

@@ -10,15 +10,18 @@
 // rule of its own: a NaN in a block makes its scale NaN (e8m0 255, e4m3 127),
 // so the whole block and what is computed from it read as NaN.
 //
-// Bound: HBM, with instructions close behind (8 values a lane and a division
-// per lane for its place cost twice the time of the whole). A lane holds 16
-// neighbouring values: one 32-byte load (bf16), one 8-byte store, no shuffle
-// for an NVFP4 block and one for an MXFP4 block; four rows are in flight per
-// lane, and only a block of threads divides to find its place.
+// A lane holds 16 neighbouring values: one 32-byte load (bf16), one 8-byte
+// store, no shuffle for an NVFP4 block and one for an MXFP4 block; four rows are
+// in flight per lane, and only a block of threads divides to find its place (8
+// values a lane and a division per lane cost twice the time). Bound: HBM for
+// fp32 and for dequantising. Codes of bf16 reach neither HBM's rate nor the
+// issue slots' (58 % active): rows that wait in registers leave room for four
+// blocks an SM, 43 % of the warps, whose first stall is the loads'.
 //
-// Measured on a B200 (copies run at 6.5 TB/s): 12288 x 3072 bf16 to MXFP4 21.7 us
-// (4.4 TB/s) and back 15.9 (6.0); 4096 x 14336 fp32 to two-level NVFP4 46 us for
-// the maximum (5.1 TB/s) and 49 for the codes (5.5), back 41 (6.5).
+// Measured on a B200 (copies run at 6.5 TB/s), one direction again and again:
+// 12288 x 3072 bf16 to MXFP4 19.4 us (4.9 TB/s) and back 15.4 (6.2); 4096 x 14336
+// to NVFP4, bf16 one level 32 us (4.7), two levels 56, back 25.5 (5.9); fp32 two
+// levels 88 us for both passes (5.7), back 43 (6.2).
 #pragma once
 #include "fp4_ptx.cuh"
 #include "numerics.cuh"
