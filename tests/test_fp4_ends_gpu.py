@@ -42,3 +42,23 @@ def test_ends_out_of_order_count_as_the_largest_before_them(ends, fmt, cuda_devi
     for got, want in zip(results[1], results[0]):
         assert want.isfinite().all() and torch.equal(got, want)
         assert not want[int(ordered[-1]):].any()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_ends_out_of_order_of_few_rows_by_many_experts(fmt, cuda_device):
+    """The product quantises its tokens itself, and finds tiles in three lots of ends."""
+    experts, tokens, rows, cols = 70, 100, 136, 160
+    g = torch.Generator(cuda_device).manual_seed(5)
+    dense = torch.randn((experts, rows, cols), generator=g, device=cuda_device).bfloat16()
+    w = fp4.quantize_mxfp4(dense, swizzled=True) if fmt == "mxfp4" else fp4.quantize_nvfp4(dense)
+    assert nat.linear_plan(fp4._matrix(w)[0], tokens).fused
+    x = torch.randn((tokens, cols), generator=g, device=cuda_device).bfloat16()
+    ends = np.arange(experts) + np.random.default_rng(6).integers(-12, 13, experts)
+    ordered = np.maximum.accumulate(np.clip(ends, 0, tokens))
+    results = []
+    for e in (ordered, ends):
+        junk = [torch.full((1 << n,), 255, dtype=torch.uint8, device=cuda_device) for n in range(14, 20) for _ in range(8)]
+        del junk
+        results.append(fp4.grouped_linear_fp4(x, w, torch.tensor(e, dtype=torch.int32, device=cuda_device)))
+    assert results[0].isfinite().all() and torch.equal(*results)
+    assert not results[0][int(ordered[-1]):].any() and results[0][:int(ordered[-1])].any(dim=1).all()
