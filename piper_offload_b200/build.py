@@ -1,4 +1,5 @@
-"""Build ``libpiper_merge.so`` and ``libpiper_fp4.so`` in-tree with nvcc for sm_100a, and the latter's calls with g++.
+"""Build the libraries (``libpiper_merge.so``, ``libpiper_fp4.so``, ``libpiper_int8.so``) in-tree with nvcc for sm_100a, and
+the FP4 operators' calls with g++.
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
 ``__graft_entry__.build()``). A library newer than every source file of its
@@ -29,6 +30,14 @@ FP4_OUT = PKG / "libpiper_fp4.so"
 CALLS_SOURCES = [PKG / "csrc" / "fp4_calls.cpp"]
 CALLS_DEPS = CALLS_SOURCES + [ROOT / "include" / "piper_fp4.h"]
 CALLS_OUT = PKG / "_fp4_calls.so"
+
+INT8_SOURCES = [PKG / "csrc" / "int8.cu"]
+INT8_DEPS = INT8_SOURCES + [
+    *(PKG / "csrc" / n for n in ("int8_quant.cuh", "int8_tiles.cuh", "int8_linear.cuh", "int8_grad.cuh", "fp4_tiles.cuh",
+                                 "fp4_quant.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
+    ROOT / "include" / "piper_int8.h",
+]
+INT8_OUT = PKG / "libpiper_int8.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -67,10 +76,11 @@ def _compile(out: Path, sources: list[Path], verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """The merges' library, and then the FP4 operators' beside it."""
+    """The merges' library, and then the operators' beside it."""
     if force or not up_to_date():
         _compile(OUT, SOURCES, verbose)
     build_fp4(force, verbose)
+    build_int8(force, verbose)
     return OUT
 
 
@@ -79,6 +89,12 @@ def build_fp4(force: bool = False, verbose: bool = False) -> Path:
         _compile(FP4_OUT, FP4_SOURCES, verbose)
     build_calls(force, verbose)
     return FP4_OUT
+
+
+def build_int8(force: bool = False, verbose: bool = False) -> Path:
+    if force or not up_to_date(INT8_OUT, INT8_DEPS):
+        _compile(INT8_OUT, INT8_SOURCES, verbose)
+    return INT8_OUT
 
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
@@ -108,3 +124,4 @@ if __name__ == "__main__":
     print(OUT)
     print(FP4_OUT)
     print(CALLS_OUT)
+    print(INT8_OUT)

@@ -1,0 +1,475 @@
+// int8.cu - host side and C ABI (include/piper_int8.h) of the 8-bit integer products.
+#include "../../include/piper_int8.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdio>
+
+#include "int8_grad.cuh"
+#include "int8_linear.cuh"
+#include "int8_quant.cuh"
+
+namespace {
+
+// No std::string: nothing here throws across the C boundary.
+thread_local char g_error[256];
+std::atomic<uint64_t> g_launches{0};
+
+int fail(int code, const char* message) {
+  std::snprintf(g_error, sizeof(g_error), "%s", message);
+  return code;
+}
+
+int cuda_fail(const char* what, cudaError_t e) {
+  std::snprintf(g_error, sizeof(g_error), "%s: %s", what, cudaGetErrorString(e));
+  return PIPER_INT8_ECUDA;
+}
+
+#define INT8_REQUIRE(condition, message) \
+  if (!(condition)) return fail(PIPER_INT8_EINVAL, message)
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    cudaGetLastError();
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr) : nullptr;
+  }();
+  return fn;
+}
+
+// Encodes a 2-D map of 128-byte wide, 128-byte swizzled boxes. The encoder wants a current context, which a thread that has
+// made no runtime call yet (autograd's own, for one) lacks: then the runtime makes its device's current first.
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t cols, int64_t rows, int64_t pitch_bytes,
+                int box_cols, int box_rows) {
+  const auto enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t one[2] = {1u, 1u};
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    if (enc(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+      return true;
+    if (cudaFree(nullptr) != cudaSuccess) return false;
+  }
+  return false;
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+int64_t align256(int64_t a) { return up(a, 256); }
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+size_t width(int dtype) { return dtype == PIPER_INT8_F32 ? 4 : 2; }
+
+int check_dtype(int dtype) {
+  INT8_REQUIRE(dtype == PIPER_INT8_BF16 || dtype == PIPER_INT8_F16 || dtype == PIPER_INT8_F32,
+               "INT8 supports bfloat16, float16 and float32 values.");
+  return PIPER_INT8_OK;
+}
+
+int check_matrix(const piper_int8_matrix* m) {
+  INT8_REQUIRE(m != nullptr, "INT8: null matrix.");
+  INT8_REQUIRE(m->batch > 0 && m->rows > 0 && m->cols > 0, "INT8 requires a non-empty matrix.");
+  INT8_REQUIRE(m->cols <= PIPER_INT8_MAX_COLS, "INT8: at most 65536 columns, so that sums fit 32 bits.");
+  INT8_REQUIRE(m->batch <= (int64_t{1} << 20) && m->rows < (int64_t{1} << 31) - 256 && m->batch * up(m->rows, 128) < (int64_t{1} << 31),
+               "INT8: a matrix has at most 2^31 rows over its batch.");
+  INT8_REQUIRE(m->scale_dtype >= 0 && m->scale_dtype <= 2, "INT8 scales are bfloat16, float16 or float32.");
+  INT8_REQUIRE(m->per_row != 0 || m->batch == 1, "INT8: experts have a scale for each row.");
+  return PIPER_INT8_OK;
+}
+
+int check_buffers(const piper_int8_matrix* m) {
+  INT8_REQUIRE(m->codes != nullptr && m->scale != nullptr, "INT8: null codes or scales.");
+  INT8_REQUIRE(aligned(m->scale, width(m->scale_dtype)), "INT8: scales are not aligned to their type.");
+  return PIPER_INT8_OK;
+}
+
+int sm_count() {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> cached[kMaxDevices] = {};
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < kMaxDevices && (n = cached[dev].load(std::memory_order_relaxed)) > 0) return n;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  n = n > 0 ? n : 148;
+  if (dev >= 0 && dev < kMaxDevices) cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+cudaError_t launched() {
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return cudaGetLastError();
+}
+
+i8::RowScales row_scales(const piper_int8_matrix& w) {
+  return {w.scale, w.scale_dtype, w.per_row != 0 ? 1 : 0, w.over_127 != 0};
+}
+
+// Codes are used where they are if bulk copies can read them.
+bool moves_codes(const piper_int8_matrix& w) { return w.cols % 16 != 0 || !aligned(w.codes, 16); }
+int64_t code_pitch(const piper_int8_matrix& w) { return moves_codes(w) ? up(w.cols, 16) : w.cols; }
+
+i8::RepackArgs repack_args(const piper_int8_matrix& w, uint8_t* out) {
+  i8::RepackArgs r{};
+  if (!moves_codes(w)) return r;
+  r.codes = static_cast<const uint8_t*>(w.codes);
+  r.out = out;
+  r.cols = w.cols;
+  r.pitch = code_pitch(w);
+  r.pieces = w.batch * w.rows * (r.pitch / 16);
+  return r;
+}
+
+// Blocks for `rows` rows of `units` units: a warp a row where that is enough for its registers.
+bool narrow(int64_t units) { return units <= 64; }
+int64_t row_blocks(int64_t rows, int64_t units) { return narrow(units) ? (rows + 7) / 8 : rows; }
+
+// ---------------------------------------------------------------- the product
+struct TilePlan {
+  int bn, split;
+  double cycles;
+};
+
+// Blocks of a cluster that share a tile's stages, by a rough account in cycles: a stage takes `stage`, leaving sums and
+// adding them up 2500 and 30 for each token of the tile, and every wave of tiles 2000.
+TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t tile_tokens, bool can_split, int64_t room) {
+  TilePlan best{bn, 1, 0.0};
+  for (int split = 1; split <= (can_split ? i8::kMaxSplit : 1); split *= 2) {
+    if (split > 1 && (items * split > room || stages < 2 * split)) break;
+    const int64_t waves = (items * split + room - 1) / room;
+    double cycles = static_cast<double>(waves) * (static_cast<double>((stages + split - 1) / split) * stage + 2000.0);
+    if (split > 1) cycles += 2500.0 + 30.0 * static_cast<double>(tile_tokens);
+    if (split == 1 || cycles < best.cycles) best = {bn, split, cycles};
+  }
+  return best;
+}
+
+struct LinearPlan {
+  int bn, split;
+  int64_t x_pitch;
+  int64_t x_codes, x_scale, x_sums, w_codes, total;  // byte offsets
+};
+
+LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
+  LinearPlan p{};
+  const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
+  const int64_t stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
+  TilePlan best{};
+  for (const int bn : {32, 128, 256}) {
+    const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
+    const int64_t items = std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + 127) / 128);
+    const TilePlan t = plan_tile(bn, items, stages, 300.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, sm_count());
+    if (best.bn == 0 || t.cycles < best.cycles) best = t;
+  }
+  p.bn = best.bn;
+  p.split = best.split;
+  p.x_pitch = up(w.cols, 16);
+  int64_t at = 0;
+  p.x_codes = at;
+  at += align256(tokens * p.x_pitch);
+  p.x_scale = at;
+  at += align256(tokens * 4);
+  p.x_sums = at;
+  if (w.zero != nullptr) at += align256(tokens * 4);
+  p.w_codes = at;
+  if (moves_codes(w)) at += align256(w.batch * w.rows * code_pitch(w));
+  p.total = at;
+  return p;
+}
+
+// Token tiles of all experts and of the rows after them (an upper bound: the ends are on the device), or of one weight's
+// tokens (0 experts).
+int64_t token_tiles(int64_t tokens, int64_t experts, int bn) {
+  return experts == 0 ? (tokens + bn - 1) / bn : tokens / bn + std::min<int64_t>(experts + 1, tokens);
+}
+
+// A launch that may start while the one before it still runs; the kernel waits where it needs that one's results.
+template <class Args>
+cudaError_t launch(void (*kernel)(Args), const Args& args, int64_t blocks, int threads, int smem, int split, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = static_cast<unsigned>(split);
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.stream = stream;
+  config.attrs = attributes;
+  config.numAttrs = split > 1 ? 2 : 1;
+  e = cudaLaunchKernelEx(&config, kernel, args);
+  return e == cudaSuccess ? launched() : e;
+}
+
+template <int DT, int BN>
+cudaError_t launch_linear(const i8::LinearArgs& args, int64_t items, cudaStream_t stream) {
+  using S = i8::LinearShape<BN, 1>;
+  return launch<i8::LinearArgs>(i8::linear_kernel<DT, BN, 1>, args, args.split > 1 ? items * args.split : std::min<int64_t>(items, sm_count()),
+                                i8::kLinearThreads, S::kSmem, args.split, stream);
+}
+
+// --------------------------------------------------------------- the gradient
+struct GradPlan {
+  int terms;      // fp16 terms per value
+  int64_t pitch;  // values between rows of terms
+  int64_t values, back, w_codes, total;  // byte offsets
+};
+
+int grad_terms(int dtype) { return dtype == PIPER_INT8_F32 ? 2 : 1; }
+
+GradPlan plan_grad(const piper_int8_matrix& w, int64_t tokens, int dtype) {
+  GradPlan p{};
+  p.terms = grad_terms(dtype);
+  p.pitch = up(w.rows, i8::kUnit);
+  int64_t at = 0;
+  p.values = at;
+  at += align256(p.terms * tokens * p.pitch * 2);
+  p.back = at;
+  at += align256(tokens * 4);
+  p.w_codes = at;
+  if (moves_codes(w)) at += align256(w.batch * w.rows * code_pitch(w));
+  p.total = at;
+  return p;
+}
+
+// Tiles of a gradient: tokens x (rows x 128) columns. Decoding costs the same whatever the tokens, so tiles are as wide in
+// tokens as they go, but for a few, which leave room for more stages; 256 columns where that fills the SMs.
+struct GradTile {
+  int bn, rows, split;
+  int64_t items;  // bound on the tiles
+};
+GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool grouped) {
+  const int64_t per_expert = tokens / w.batch;
+  GradTile t{256, 1, 1, 0};
+  if (per_expert <= 48) {
+    t.bn = 64;
+  } else {
+    const auto waves = [&](int64_t cols) {
+      const int64_t tiles = w.batch * ((per_expert + 255) / 256) * ((w.cols + cols - 1) / cols);
+      return static_cast<double>((tiles + sm_count() - 1) / sm_count());
+    };
+    if (waves(256) * 1060.0 <= waves(128) * 600.0) t.rows = 2;
+  }
+  t.items = token_tiles(tokens, grouped ? w.batch : 0, t.bn) * ((w.cols + 128 * t.rows - 1) / (128 * t.rows));
+  const int64_t stages = (w.rows + i8::kGradStageRows - 1) / i8::kGradStageRows * terms;
+  t.split = plan_tile(t.bn, t.items, stages, 600.0, std::min<int64_t>(tokens, t.bn), t.rows == 1 && !grouped, sm_count()).split;
+  return t;
+}
+
+template <int DT, int BN, int kRows>
+cudaError_t launch_grad(const i8::GradArgs& args, int64_t items, cudaStream_t stream) {
+  using S = i8::GradShape<BN, kRows>;
+  static_assert(S::kCanSplit == (kRows == 1), "the plan splits tiles of 128 columns");
+  return launch<i8::GradArgs>(i8::grad_kernel<DT, BN, kRows>, args, items * args.split, S::kThreads, S::kSmem, args.split, stream);
+}
+
+#define INT8_DISPATCH(dtype, CALL)                              \
+  do {                                                          \
+    if ((dtype) == PIPER_INT8_BF16) { CALL(i8::kBF16); }        \
+    else if ((dtype) == PIPER_INT8_F16) { CALL(i8::kF16); }     \
+    else { CALL(i8::kF32); }                                    \
+  } while (0)
+
+int check_call(const piper_int8_matrix* w, int64_t tokens, const int32_t* ends, int dtype) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_buffers(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  INT8_REQUIRE(tokens >= 0 && tokens < (int64_t{1} << 28), "INT8: too many tokens for one call.");
+  INT8_REQUIRE(ends != nullptr || w->batch == 1, "INT8: several matrices need the ends of their rows.");
+  return PIPER_INT8_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int piper_int8_linear_workspace(const piper_int8_matrix* w, int64_t tokens, size_t* bytes) {
+  if (int rc = check_matrix(w)) return rc;
+  INT8_REQUIRE(bytes != nullptr && tokens >= 0, "INT8 product: bad workspace query.");
+  *bytes = tokens == 0 ? 0 : static_cast<size_t>(plan_linear(*w, tokens).total);
+  return PIPER_INT8_OK;
+}
+
+int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_stride, int64_t tokens, const int32_t* ends,
+                      void* y, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_call(w, tokens, ends, dtype)) return rc;
+  if (tokens == 0) return PIPER_INT8_OK;
+  INT8_REQUIRE(x != nullptr && y != nullptr, "INT8 product: null input or output.");
+  INT8_REQUIRE(aligned(x, width(dtype)) && aligned(y, width(dtype)), "INT8 product: input or output not aligned to its type.");
+  INT8_REQUIRE(x_stride >= w->cols || tokens == 1, "INT8 product: rows of the input overlap.");
+  const LinearPlan p = plan_linear(*w, tokens);
+  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256))
+    return fail(PIPER_INT8_EWORKSPACE, "INT8 product: workspace missing, too small or not 256-byte aligned.");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+
+  i8::QuantArgs q{};
+  q.x = x;
+  q.x_stride = x_stride;
+  q.tokens = tokens;
+  q.cols = static_cast<int32_t>(w->cols);
+  q.vec = aligned(x, 16) && (x_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  q.pitch = p.x_pitch;
+  q.codes = reinterpret_cast<int8_t*>(ws + p.x_codes);
+  q.scale = reinterpret_cast<float*>(ws + p.x_scale);
+  q.sums = w->zero != nullptr ? reinterpret_cast<int32_t*>(ws + p.x_sums) : nullptr;
+  const i8::RepackArgs r = repack_args(*w, ws + p.w_codes);
+
+  i8::LinearArgs a{};
+  a.x_scale = q.scale;
+  a.x_sums = q.sums;
+  a.rows_of = {row_scales(*w), static_cast<const int8_t*>(w->zero), w->per_row != 0 ? 1 : 0};
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->rows + 127) / 128)};
+  a.y = y;
+  a.rows = static_cast<int32_t>(w->rows);
+  a.cols = static_cast<int32_t>(w->cols);
+  a.split = p.split;
+  a.early = r.pieces == 0;
+  a.vec = aligned(y, 16) && (w->rows * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  const int64_t items = token_tiles(tokens, ends == nullptr ? 0 : w->batch, p.bn) * a.groups.row_tiles;
+  a.items = static_cast<int32_t>(items);
+  INT8_REQUIRE(items < (int64_t{1} << 31) / i8::kMaxSplit, "INT8 product: too many tiles for one call.");
+  const int64_t units = p.x_pitch / i8::kUnit, token_blocks = row_blocks(tokens, units);
+  const int64_t blocks = token_blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  INT8_REQUIRE(blocks < (int64_t{1} << 31), "INT8 product: too many values for one call.");
+  const void* codes = r.pieces > 0 ? r.out : w->codes;
+  if (!encode_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, w->cols, w->batch * w->rows, code_pitch(*w), i8::kStageCols, fp4::kTileRows) ||
+      !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.bn))
+    return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
+
+  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
+#define CALL(D)                                                                                          \
+  if (narrow(units)) i8::quantize_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid); \
+  else i8::quantize_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid)
+  INT8_DISPATCH(dtype, CALL);
+#undef CALL
+  cudaError_t e = launched();
+  if (e != cudaSuccess) return cuda_fail("quantize kernel", e);
+#define CALL(D)                                           \
+  e = p.bn == 32    ? launch_linear<D, 32>(a, items, s)   \
+      : p.bn == 128 ? launch_linear<D, 128>(a, items, s)  \
+                    : launch_linear<D, 256>(a, items, s)
+  INT8_DISPATCH(dtype, CALL);
+#undef CALL
+  return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("linear kernel", e);
+}
+
+int piper_int8_grad_input_workspace(const piper_int8_matrix* w, int64_t tokens, int32_t dtype, size_t* bytes) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  INT8_REQUIRE(bytes != nullptr && tokens >= 0, "INT8 gradient: bad workspace query.");
+  *bytes = tokens == 0 ? 0 : static_cast<size_t>(plan_grad(*w, tokens, dtype).total);
+  return PIPER_INT8_OK;
+}
+
+int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy_stride, int64_t tokens,
+                          const int32_t* ends, void* dx, int32_t dtype, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  if (int rc = check_call(w, tokens, ends, dtype)) return rc;
+  if (tokens == 0) return PIPER_INT8_OK;
+  INT8_REQUIRE(dy != nullptr && dx != nullptr, "INT8 gradient: null gradient or output.");
+  INT8_REQUIRE(aligned(dy, width(dtype)) && aligned(dx, width(dtype)), "INT8 gradient: gradient or output not aligned to its type.");
+  INT8_REQUIRE(dy_stride >= w->rows || tokens == 1, "INT8 gradient: rows of the gradient overlap.");
+  const GradPlan p = plan_grad(*w, tokens, dtype);
+  if (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256))
+    return fail(PIPER_INT8_EWORKSPACE, "INT8 gradient: workspace missing, too small or not 256-byte aligned.");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+
+  i8::ScaleArgs v{};
+  v.dy = dy;
+  v.dy_stride = dy_stride;
+  v.tokens = tokens;
+  v.rows = static_cast<int32_t>(w->rows);
+  v.vec = aligned(dy, 16) && (dy_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  v.pitch = p.pitch;
+  v.out = reinterpret_cast<__half*>(ws + p.values);
+  v.back = reinterpret_cast<float*>(ws + p.back);
+  v.scales = row_scales(*w);
+  v.ends = ends;
+  v.experts = static_cast<int32_t>(w->batch);
+  const i8::RepackArgs r = repack_args(*w, ws + p.w_codes);
+
+  i8::GradArgs a{};
+  const GradTile tile = grad_tile(*w, tokens, p.terms, ends != nullptr);
+  a.codes = r.pieces > 0 ? r.out : static_cast<const uint8_t*>(w->codes);
+  a.zero = static_cast<const int8_t*>(w->zero);
+  a.back = v.back;
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 128 * tile.rows - 1) / (128 * tile.rows))};
+  a.dx = dx;
+  a.code_pitch = code_pitch(*w);
+  a.zero_step = w->per_row != 0 ? 1 : 0;
+  a.rows = static_cast<int32_t>(w->rows);
+  a.cols = static_cast<int32_t>(w->cols);
+  a.terms = p.terms;
+  a.split = tile.split;
+  a.vec = aligned(dx, 16) && (w->cols * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  const int64_t units = p.pitch / i8::kUnit, token_blocks = row_blocks(tokens, units);
+  const int64_t blocks = token_blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  INT8_REQUIRE(tile.items < (int64_t{1} << 31) / i8::kMaxSplit && blocks < (int64_t{1} << 31), "INT8 gradient: too many tiles for one call.");
+  if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.bn))
+    return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
+
+  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
+#define CALL(D)                                                                                       \
+  if (narrow(units)) i8::scale_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid); \
+  else i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid)
+  INT8_DISPATCH(dtype, CALL);
+#undef CALL
+  cudaError_t e = launched();
+  if (e != cudaSuccess) return cuda_fail("scale kernel", e);
+#define CALL(D)                                                  \
+  e = tile.bn == 64     ? launch_grad<D, 64, 1>(a, tile.items, s)  \
+      : tile.rows == 1 ? launch_grad<D, 256, 1>(a, tile.items, s) \
+                       : launch_grad<D, 256, 2>(a, tile.items, s)
+  INT8_DISPATCH(dtype, CALL);
+#undef CALL
+  return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("gradient kernel", e);
+}
+
+int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, piper_int8_plan* plan) {
+  if (int rc = check_matrix(w)) return rc;
+  INT8_REQUIRE(plan != nullptr && tokens > 0, "INT8 product: bad plan query.");
+  const LinearPlan p = plan_linear(*w, tokens);
+  *plan = {p.bn, 128, p.split, 1};
+  return PIPER_INT8_OK;
+}
+
+int piper_int8_grad_input_plan(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, int32_t dtype, piper_int8_plan* plan) {
+  if (int rc = check_matrix(w)) return rc;
+  if (int rc = check_dtype(dtype)) return rc;
+  INT8_REQUIRE(plan != nullptr && tokens > 0 && (grouped != 0 || w->batch == 1), "INT8 gradient: bad plan query.");
+  const GradTile t = grad_tile(*w, tokens, grad_terms(dtype), grouped != 0);
+  *plan = {t.bn, 128 * t.rows, t.split, 1};
+  return PIPER_INT8_OK;
+}
+
+const char* piper_int8_last_error(void) { return g_error; }
+
+int piper_int8_device_status(void* stream, uint32_t* status) {
+  cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("cudaStreamSynchronize", e);
+  unsigned int v = 0, zero = 0;
+  e = cudaMemcpyFromSymbol(&v, pm::g_status, sizeof(v));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(pm::g_status, &zero, sizeof(zero));
+  if (e != cudaSuccess) return cuda_fail("status word", e);
+  if (status) *status = v;
+  return v == 0 ? PIPER_INT8_OK : fail(PIPER_INT8_ETIMEOUT, "a bounded device-side wait timed out.");
+}
+
+const char* piper_int8_version(void) { return "piper-int8 0.1 sm_100a"; }
+
+uint64_t piper_int8_launches(void) { return g_launches.load(std::memory_order_relaxed); }
+
+}  // extern "C"

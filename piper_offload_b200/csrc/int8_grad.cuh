@@ -1,0 +1,286 @@
+// int8_grad.cuh - dx[t, k] = sum_n dy[t, n] s_w[n] (w[n, k] - z[n]) with w in 8 bits.
+//
+// The sum runs over the weight's rows, which the scales belong to, so they go into the gradient: a launch before makes
+// fp16 values of dy[t, n] s_w[n] (int8_quant.cuh, scale_rows). The weight is decoded on chip to fp16, which holds every
+// code less its zero point exactly (nine bits), and multiplied on the fp16 tensor pipe with fp32 sums. A tile is
+// kRows x 128 columns of w (the tensor core's 128-row operand, stored with its columns contiguous) x up to BN tokens; a
+// stage is 64 rows of w. Gradients come by bulk tensor copies; sixteen warps decode, loads two stages ahead: a byte
+// permute puts each code beside the exponent of 1024, and a packed difference takes 1024, the offset and the zero point off.
+#pragma once
+#include <cuda.h>
+
+#include "int8_tiles.cuh"
+
+namespace i8 {
+
+constexpr int kGradStageRows = 64;   // rows of w per stage
+constexpr int kDecodeWarps = 8;      // for 64 rows x 128 columns; two such teams a block, which run the epilogue too
+
+struct GradArgs {
+  CUtensorMap dy_map;   // (terms * tokens, rows of w) fp16
+  const uint8_t* codes; // rows start on 16-byte boundaries
+  const int8_t* zero;   // or NULL
+  const float* back;    // (tokens)
+  fp4::Groups groups;   // row tiles: of kRows x 128 columns of w
+  void* dx;
+  int64_t code_pitch;
+  int32_t zero_step;
+  int32_t rows, cols;   // of w
+  int32_t terms;
+  int32_t split;        // blocks of a cluster that share a tile's stages
+  int32_t vec;          // rows of dx start on 16-byte boundaries
+};
+
+template <int BN, int kRows>
+struct GradShape {
+  static constexpr int kA = kRows * kGradStageRows * kTileRows * 2;
+  static constexpr int kB = BN * kGradStageRows * 2;
+  static constexpr int kStage = kA + kB;
+  static constexpr int kTokens = BN * 4;
+  static constexpr int kRoom = kSmemMax - 3072 - kTokens;
+  static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
+  static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 256;
+  static constexpr int kThreads = 64 + 32 * kDecodeWarps * 2;  // producer warp, tensor-core warp, decoding warps
+  static constexpr int kTurns = 2 / kRows;  // teams that take stages in turn
+  static constexpr int kAlloc = kRows * BN;
+  static constexpr bool kCanSplit = kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
+  static_assert(kAlloc >= 32 && kAlloc <= 512 && kStages >= 3, "the tile does not fit");
+};
+
+// A thread's share of 64 rows x 128 columns: 32 codes of one row and the row's zero point.
+struct Piece {
+  uint4 codes[2];
+  int32_t zero;
+};
+
+// Walks down the weight in stages: this thread's row of each, 32 columns from `col` on.
+struct PieceWalk {
+  const uint8_t* codes;
+  const int8_t* zero;
+  int64_t code_step;  // to the next stage
+  int row, rows, bytes, zero_step;
+
+  __device__ __forceinline__ void begin(const GradArgs& p, int64_t expert, int block, int in_stage, int col) {
+    row = block * kGradStageRows + in_stage;
+    rows = p.rows;
+    bytes = p.code_pitch > col ? 32 : 0;  // the pitch is a multiple of 16, so a half may be missing
+    if (bytes != 0 && p.code_pitch - col < 32) bytes = 16;
+    const int64_t r = expert * p.rows + row;
+    codes = p.codes + r * p.code_pitch + (bytes > 0 ? col : 0);
+    code_step = kGradStageRows * p.code_pitch;
+    zero_step = kGradStageRows * p.zero_step;
+    zero = p.zero != nullptr ? p.zero + r * p.zero_step : nullptr;
+  }
+
+  __device__ __forceinline__ Piece load() const {
+    // a code of zero where there is none
+    Piece out{{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, 0};
+    if (row >= rows) return out;
+    if (bytes >= 16) out.codes[0] = *reinterpret_cast<const uint4*>(codes);
+    if (bytes == 32) out.codes[1] = *reinterpret_cast<const uint4*>(codes + 16);
+    if (zero != nullptr) out.zero = *zero;
+    return out;
+  }
+
+  __device__ __forceinline__ void next() {
+    codes += code_step;
+    if (zero != nullptr) zero += zero_step;
+    row += kGradStageRows;
+  }
+};
+
+// Four codes less the zero point, as fp16 in their order. `off`: 1024 + 128 + zero point, twice.
+__device__ __forceinline__ void decode4(uint32_t codes, __half2 off, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = codes ^ 0x80808080u;  // code + 128
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);  // 1024 + code + 128
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+
+template <int DT, int BN, int kRows>
+__global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel(const __grid_constant__ GradArgs p) {
+  using S = GradShape<BN, kRows>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
+  float* token_scale = reinterpret_cast<float*>(smem + S::kStages * S::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(token_scale + BN);  // gradients landed
+  uint64_t* ready = full + S::kStages;                             // w decoded
+  uint64_t* empty = ready + S::kStages;
+  uint64_t* done = empty + S::kStages;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
+
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    pm::prefetch_tmap(&p.dy_map);
+    for (int s = 0; s < S::kStages; ++s) {
+      pm::mbar_init(&full[s], 1);
+      pm::mbar_init(&ready[s], kDecodeWarps * kRows);  // of one team, or of both halves'
+      pm::mbar_init(&empty[s], 1);
+    }
+    pm::mbar_init(done, 1);
+    pm::fence_mbar_init();
+  } else if (warp == 1) {
+    pm::tmem_alloc(tmem_at, S::kAlloc);
+    pm::tmem_relinquish();
+  }
+  const int rank = p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
+  TileAt t;
+  const bool have = fp4::find_tile(p.groups, p.split > 1 ? blockIdx.x / p.split : blockIdx.x, BN, t);
+  pm::tc_fence_before();
+  __syncthreads();
+  pm::tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
+  const int blocks = (p.rows + kGradStageRows - 1) / kGradStageRows;  // of 64 rows of w
+  const int all = blocks * p.terms;
+  const int from = p.split > 1 ? all * rank / p.split : 0, to = p.split > 1 ? all * (rank + 1) / p.split : all;
+  const bool sums = have && t.expert != p.groups.experts;
+  const RowsOf none{};
+  fp4::grid_wait();  // gradients, and codes that were laid out, come from the launch before
+
+  if (have && !sums) {
+    if (rank == 0)
+      for (int h = 0; h < kRows; ++h) {
+        TileAt part = t;
+        part.row_tile = t.row_tile * kRows + h;
+        zero_tile<DT>(p.dx, part, p.cols, threadIdx.x, S::kThreads);
+      }
+  } else if (sums) {
+    if (warp == 0) {
+      const int first = __shfl_sync(0xFFFFFFFFu, t.first, 0);
+      int issued = 0;
+      if (fp4::elect_one()) {
+        fp4::Ring<S::kStages> ring;
+        int block = from % blocks, row = first + from / blocks * static_cast<int>(p.groups.tokens);
+        for (int i = from; i < to; ++i, ring.next()) {
+          if (issued >= S::kStages && !pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad)) break;
+          pm::mbar_arrive_expect_tx(&full[ring.slot], S::kB);
+          pm::tma_load_2d(smem + ring.slot * S::kStage + S::kA, &p.dy_map, block * kGradStageRows, row, &full[ring.slot]);
+          ++issued;
+          if (++block == blocks) {  // the next term
+            block = 0;
+            row += static_cast<int>(p.groups.tokens);
+          }
+        }
+      }
+      __syncwarp();
+      issued = __reduce_max_sync(0xFFFFFFFFu, issued);
+      // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
+      for (int i = max(0, issued - S::kStages); i < issued; ++i)
+        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+      __syncwarp();
+    } else if (warp == 1) {
+      const uint32_t idesc = idesc_grad((static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t.count, 0)) + 15u) & ~15u);
+      if (fp4::elect_one()) {
+        fp4::Ring<S::kStages> ring;
+        for (int i = from; i < to; ++i, ring.next()) {
+          if (!pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma) ||
+              !pm::mbar_wait(&ready[ring.slot], ring.round, pm::kStatusTimeoutMma))
+            break;
+          pm::tc_fence_after();
+          const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
+          // w: 64-column blocks 8 KB apart, groups of 8 rows 1 KB apart; gradients: 128-byte rows of 64 values
+          const uint64_t a = pm::smem_desc_sw(at, kGradStageRows * 128, 1024, 2);
+          const uint64_t b = pm::smem_desc_sw(at + S::kA, 16, 1024, 2);
+#pragma unroll
+          for (int j = 0; j < kGradStageRows / 16; ++j)
+#pragma unroll
+            for (int h = 0; h < kRows; ++h)
+              pm::umma_f16(tmem + h * BN, a + h * (kGradStageRows * kTileRows * 2 >> 4) + j * (2048 >> 4), b + j * (32 >> 4), idesc,
+                           i != from || j != 0);
+          pm::umma_commit(&empty[ring.slot]);
+        }
+        pm::umma_commit(done);
+      }
+      __syncwarp();
+    } else {
+      // a team has 128 columns of every stage, or of every second one: a warp decodes eight rows, a lane 32 columns of
+      // one, and the eight lanes whose 16-byte stores go together write different rows, so the swizzle gives them
+      // different banks
+      const int team = (warp - 2) / kDecodeWarps;
+      const int h = kRows == 2 ? team : 0, turn = kRows == 2 ? 0 : team;
+      const int r = (warp - 2) % kDecodeWarps * 8 + (lane & 7), quarter = lane >> 3;
+      const int col = (t.row_tile * kRows + h) * kTileRows + quarter * 32;
+      uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (quarter >> 1) * (kGradStageRows * 128) + r * 128;
+      PieceWalk walk;
+      int block = (from + turn) % blocks;  // of the next loads
+      walk.begin(p, t.expert, block, r, col);
+      const auto load_next = [&]() {
+        const Piece piece = walk.load();
+#pragma unroll
+        for (int j = 0; j < S::kTurns; ++j) {
+          walk.next();
+          if (++block == blocks) {  // the next term
+            block = 0;
+            walk.begin(p, t.expert, 0, r, col);
+          }
+        }
+        return piece;
+      };
+      if (const int i = threadIdx.x - 64; i < BN) token_scale[i] = i < t.count ? p.back[t.first + i] : 0.0f;
+      Piece soon = load_next(), later = load_next();  // this team's next stage's, the one after's
+      fp4::Ring<S::kStages> ring;
+      if (turn == 1) ring.next();
+      bool ok = true;
+      for (int i = from + turn; i < to; i += S::kTurns) {
+        const Piece now = soon;
+        soon = later;
+        if (i + 2 * S::kTurns < to) later = load_next();
+        if (i - from >= S::kStages) {
+          ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad));
+          if (!ok) break;
+        }
+        uint8_t* row = to_row + ring.slot * S::kStage;
+        const __half2 off = __half2half2(__int2half_rn(1152 + now.zero));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint4& c = now.codes[q >> 1];
+          uint4 v;
+          decode4(q & 1 ? c.z : c.x, off, v.x, v.y);
+          decode4(q & 1 ? c.w : c.y, off, v.z, v.w);
+          *reinterpret_cast<uint4*>(row + ((((quarter & 1) * 4 + q) ^ (r & 7)) << 4)) = v;
+        }
+        pm::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) pm::mbar_arrive(&ready[ring.slot]);
+#pragma unroll
+        for (int j = 0; j < S::kTurns; ++j) ring.next();
+      }
+      pm::named_bar_sync(1, 32 * kDecodeWarps * 2);  // the tokens' scales are written
+      ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(done, 0, pm::kStatusTimeoutMma));
+      pm::tc_fence_after();
+      if (ok) {
+        // the sums are complete, so the stages are free
+        if (S::kCanSplit && p.split > 1) {
+          if (warp < 6) fp4::store_sums(tmem, t, reinterpret_cast<float*>(smem));
+        } else {
+          uint8_t* mine = smem + (warp - 2) * 2048;
+          TileAt part = t;
+          part.row_tile = t.row_tile * kRows + h;
+          // 4 / kRows warps for each quarter of the lanes: a share of the tokens each
+          constexpr int kShare = BN * kRows / 4 < 32 ? 32 : BN * kRows / 4;
+          const int share = (kRows == 2 ? (warp - 2) % kDecodeWarps : warp - 2) / 4;
+          store_tile<DT, false>(tmem + h * BN, p.dx, part, p.cols, none, 0, token_scale, nullptr, share * kShare,
+                                min((share + 1) * kShare, BN), mine, p.vec != 0);
+        }
+      }
+      pm::tc_fence_before();
+    }
+  }
+  if (S::kCanSplit && p.split > 1) {
+    __syncwarp();
+    fp4::cluster_sync();  // every block's sums are written
+    if (sums)
+      add_cluster_sums<DT, false>(reinterpret_cast<const float*>(smem), p.dx, t, p.cols, none, 0, token_scale, nullptr, rank, p.split,
+                                  S::kThreads, p.vec != 0);
+    __syncwarp();
+    fp4::cluster_sync();  // nobody's shared memory goes while others read it
+  }
+  __syncthreads();
+  if (warp == 1) {
+    pm::tc_fence_after();
+    pm::tmem_dealloc(tmem, S::kAlloc);
+  }
+}
+
+}  // namespace i8

@@ -31,6 +31,28 @@ class Int8Weight:
 
 
 @dataclass
+class Int8Experts:
+    """A layer's experts in INT8 with a scale (and, where there is one, a zero point)
+    for each row, stacked: ``qdata`` (experts, rows, cols), ``scale`` and ``zero_point``
+    (experts, rows, 1). :meth:`expert` gives one of them as a weight over the same
+    storage, so that a merge into it changes the stack."""
+
+    qdata: torch.Tensor
+    scale: torch.Tensor
+    block_size: tuple[int, int]
+    dtype: torch.dtype = torch.bfloat16
+    zero_point: torch.Tensor | None = None
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.qdata.shape
+
+    def expert(self, index: int) -> Int8Weight:
+        zero = None if self.zero_point is None else self.zero_point[index]
+        return Int8Weight(self.qdata[index], self.scale[index], self.block_size, self.dtype, zero)
+
+
+@dataclass
 class Float8Weight:
     qdata: torch.Tensor
     scale: torch.Tensor
