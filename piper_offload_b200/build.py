@@ -1,5 +1,5 @@
-"""Build the libraries (``libpiper_merge.so``, ``libpiper_fp4.so``, ``libpiper_int8.so``) in-tree with nvcc for sm_100a, and
-the FP4 operators' calls with g++.
+"""Build the libraries (``libpiper_merge.so``, ``libpiper_fp4.so``, ``libpiper_int8.so``, ``libpiper_routing.so``) in-tree with nvcc
+for sm_100a, and the FP4 operators' calls with g++.
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
 ``__graft_entry__.build()``). A library newer than every source file of its
@@ -38,6 +38,12 @@ INT8_DEPS = INT8_SOURCES + [
     ROOT / "include" / "piper_int8.h",
 ]
 INT8_OUT = PKG / "libpiper_int8.so"
+ROUTING_SOURCES = [PKG / "csrc" / "routing.cu"]
+ROUTING_DEPS = ROUTING_SOURCES + [
+    *(PKG / "csrc" / n for n in ("routing_route.cuh", "routing_exchange.cuh", "fp4_ptx.cuh", "ptx.cuh")),
+    ROOT / "include" / "piper_routing.h",
+]
+ROUTING_OUT = PKG / "libpiper_routing.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -81,6 +87,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         _compile(OUT, SOURCES, verbose)
     build_fp4(force, verbose)
     build_int8(force, verbose)
+    build_routing(force, verbose)
     return OUT
 
 
@@ -95,6 +102,12 @@ def build_int8(force: bool = False, verbose: bool = False) -> Path:
     if force or not up_to_date(INT8_OUT, INT8_DEPS):
         _compile(INT8_OUT, INT8_SOURCES, verbose)
     return INT8_OUT
+
+
+def build_routing(force: bool = False, verbose: bool = False) -> Path:
+    if force or not up_to_date(ROUTING_OUT, ROUTING_DEPS):
+        _compile(ROUTING_OUT, ROUTING_SOURCES, verbose)
+    return ROUTING_OUT
 
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
@@ -125,3 +138,4 @@ if __name__ == "__main__":
     print(FP4_OUT)
     print(CALLS_OUT)
     print(INT8_OUT)
+    print(ROUTING_OUT)

@@ -1,0 +1,211 @@
+// routing_exchange.cuh - tokens to their places among the experts' rows, and the experts' rows added up again.
+//
+// All of it is memory: every row is read once and written once, 16 bytes a thread where rows start on 16-byte boundaries
+// (one value otherwise). What does not fit: a row index outside the rows counts as none.
+#pragma once
+#include "routing_route.cuh"
+
+namespace routing {
+
+constexpr int kExchangeThreads = 256;
+
+struct ExchangeArgs {
+  const void* in;        // dispatch: tokens; combine: rows
+  int64_t in_stride;
+  const void* dout;      // combine's gradient: of its result
+  int64_t dout_stride;
+  const float* weights;  // or NULL: ones
+  void* out;
+  float* dweights;
+  const int32_t* rows;   // (tokens, top_k)
+  const int32_t* total;
+  int64_t tokens;
+  int32_t top_k, hidden;
+  int32_t pieces;        // of a row
+};
+
+// V values of a row at once, as they lie.
+template <int DT, int V>
+struct Pack {
+  static constexpr int kWords = V * (DT == kF32 ? 4 : 2) / 4;
+  uint32_t w[kWords > 0 ? kWords : 1];
+};
+
+template <int DT, int V>
+__device__ __forceinline__ Pack<DT, V> load_pack(const void* p, int64_t at) {
+  Pack<DT, V> r;
+  if constexpr (V == 1) {
+    if constexpr (DT == kF32) r.w[0] = static_cast<const uint32_t*>(p)[at];
+    else r.w[0] = static_cast<const uint16_t*>(p)[at];
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == kF32 ? 4 : 2));
+    r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+  }
+  return r;
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void store_pack(void* p, int64_t at, const Pack<DT, V>& r) {
+  if constexpr (V == 1) {
+    if constexpr (DT == kF32) static_cast<uint32_t*>(p)[at] = r.w[0];
+    else static_cast<uint16_t*>(p)[at] = static_cast<uint16_t>(r.w[0]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + at * (DT == kF32 ? 4 : 2)) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+  }
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void to_floats(const Pack<DT, V>& r, float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (DT == kF32) f[i] = __uint_as_float(r.w[i]);
+    else {
+      const uint32_t h = r.w[i >> 1] >> (16 * (i & 1)) & 0xFFFFu;
+      if constexpr (DT == kBF16) f[i] = __uint_as_float(h << 16);
+      else f[i] = __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+    }
+  }
+}
+
+template <int DT, int V>
+__device__ __forceinline__ Pack<DT, V> from_floats(const float (&f)[V]) {
+  Pack<DT, V> r{};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (DT == kF32) r.w[i] = __float_as_uint(f[i]);
+    else {
+      const uint32_t h = DT == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[i])) : __half_as_ushort(__float2half_rn(f[i]));
+      r.w[i >> 1] |= h << (16 * (i & 1));
+    }
+  }
+  return r;
+}
+
+// The place of choice j of a token, or -1.
+__device__ __forceinline__ int64_t place_of(const ExchangeArgs& p, int64_t token, int j) {
+  const int64_t r = p.rows[token * p.top_k + j];
+  return r >= 0 && r < p.tokens * p.top_k ? r : -1;
+}
+
+// A thread has a piece of a token. It writes the copies, and zeros in the rows of no choice among [t top_k, (t + 1) top_k).
+template <int DT, int V>
+__global__ void __launch_bounds__(kExchangeThreads) dispatch_kernel(const __grid_constant__ ExchangeArgs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kExchangeThreads + threadIdx.x;
+  const int64_t token = i / p.pieces;
+  if (token >= p.tokens) return;
+  const int64_t col = (i - token * p.pieces) * V;
+  const Pack<DT, V> v = load_pack<DT, V>(p.in, token * p.in_stride + col);
+  const int64_t total = *p.total;
+  for (int j = 0; j < p.top_k; ++j) {
+    const int64_t r = place_of(p, token, j);
+    if (r >= 0 && r < total) store_pack<DT, V>(p.out, r * p.hidden + col, v);
+    if (token * p.top_k + j >= total) store_pack<DT, V>(p.out, (token * p.top_k + j) * p.hidden + col, Pack<DT, V>{});
+  }
+}
+
+constexpr int kAtOnce = 8;  // rows whose loads are in flight together
+
+// A thread has a piece of a token's result.
+template <int DT, int V>
+__global__ void __launch_bounds__(kExchangeThreads) combine_kernel(const __grid_constant__ ExchangeArgs p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kExchangeThreads + threadIdx.x;
+  const int64_t token = i / p.pieces;
+  if (token >= p.tokens) return;
+  const int64_t col = (i - token * p.pieces) * V;
+  float sum[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) sum[k] = 0.0f;
+  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
+    Pack<DT, V> v[kAtOnce];
+    float w[kAtOnce];
+    bool has[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int64_t r = j0 + k < p.top_k ? place_of(p, token, j0 + k) : -1;
+      has[k] = r >= 0;
+      if (has[k]) {
+        v[k] = load_pack<DT, V>(p.in, r * p.in_stride + col);
+        w[k] = p.weights != nullptr ? p.weights[token * p.top_k + j0 + k] : 1.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (has[k]) {
+        float f[V];
+        to_floats(v[k], f);
+#pragma unroll
+        for (int n = 0; n < V; ++n) sum[n] = fmaf(w[k], f[n], sum[n]);
+      }
+  }
+  store_pack<DT, V>(p.out, token * p.hidden + col, from_floats<DT, V>(sum));
+}
+
+// kWarps warps have a token: each piece of the result's gradient goes to the rows' gradients, and with the rows into the
+// weights' gradients.
+template <int DT, int V, int kWarps>
+__global__ void __launch_bounds__(kExchangeThreads) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
+  __shared__ float parts[kWarps > 1 ? kAtOnce * 8 : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t token = kWarps == 1 ? static_cast<int64_t>(blockIdx.x) * (kExchangeThreads / 32) + warp : blockIdx.x;
+  if (kWarps == 1 && token >= p.tokens) return;
+  const int first = kWarps == 1 ? lane : threadIdx.x;
+  const int64_t total = *p.total;
+  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
+    int64_t row[kAtOnce];
+    float w[kAtOnce], dot[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const bool in = j0 + k < p.top_k;
+      row[k] = in ? place_of(p, token, j0 + k) : -1;
+      if (row[k] >= total) row[k] = -1;
+      w[k] = in ? p.weights[token * p.top_k + j0 + k] : 0.0f;
+      dot[k] = 0.0f;
+    }
+    for (int piece = first; piece < p.pieces; piece += 32 * kWarps) {
+      const int64_t col = static_cast<int64_t>(piece) * V;
+      const Pack<DT, V> d = load_pack<DT, V>(p.dout, token * p.dout_stride + col);
+      Pack<DT, V> y[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (row[k] >= 0) y[k] = load_pack<DT, V>(p.in, row[k] * p.in_stride + col);
+      float g[V];
+      to_floats(d, g);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        if (row[k] >= 0) {
+          float f[V], dy[V];
+          to_floats(y[k], f);
+#pragma unroll
+          for (int n = 0; n < V; ++n) {
+            dot[k] = fmaf(f[n], g[n], dot[k]);
+            dy[n] = w[k] * g[n];
+          }
+          store_pack<DT, V>(p.out, row[k] * p.hidden + col, from_floats<DT, V>(dy));
+        }
+        const int64_t none = token * p.top_k + j0 + k;
+        if (j0 + k < p.top_k && none >= total) store_pack<DT, V>(p.out, none * p.hidden + col, Pack<DT, V>{});
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) dot[k] = warp_sum(dot[k]);
+    if constexpr (kWarps > 1) {
+      __syncthreads();  // the last ones are read
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (lane == 0) parts[k * 8 + warp] = dot[k];
+      __syncthreads();
+      if (threadIdx.x < kAtOnce && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kWarps; ++n) sum += parts[threadIdx.x * 8 + n];
+        p.dweights[token * p.top_k + j0 + threadIdx.x] = sum;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (lane == k && j0 + k < p.top_k) p.dweights[token * p.top_k + j0 + k] = dot[k];
+    }
+  }
+}
+
+}  // namespace routing

@@ -1,0 +1,475 @@
+// routing_route.cuh - a token's experts: scores, the best groups, the best experts in them, weights, and the order by expert.
+//
+// A warp has a token and a lane every 32nd expert. Choices are compared as whole numbers that order as the scores do (0 for
+// what is closed, 1 for a NaN), the largest found by redux, ties by a second redux for the lowest index.
+//
+// Choice scores. Without a bias the logits themselves decide: both scores grow with them. With one, or where a group counts
+// by its two best, sums of scores decide, and sums that are near each other in fp32 may be in another order than the
+// numbers they stand for. So each gap that decides anything is held against a margin that is above twice the sums' error
+// (expf is within 2 ulp, so a score is within 2^-20 of 1; 2^-24 of the sum for its own rounding), and a token with a gap
+// within it is done again in 64 bits: 1 to 2 % of the tokens where 256 experts' scores are spread over [0, 1].
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "fp4_ptx.cuh"
+
+namespace routing {
+
+enum : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
+enum : int { kSoftmax = 0, kSigmoid = 1 };
+enum : int { kMax = 0, kTop2 = 1 };
+
+constexpr uint32_t kFull = 0xFFFFFFFFu;
+
+struct RouteArgs {
+  const void* logits;
+  int64_t stride;
+  const float* bias;
+  const uint8_t* mask;
+  float* weights;
+  int32_t* experts_out;
+  int32_t* ends;
+  int32_t* rows;
+  int32_t* source;
+  int32_t* counts;  // (chunks, experts)
+  int64_t tokens;
+  int32_t chunk;    // tokens of a block
+  int32_t chunks;
+  int32_t experts, top_k;
+  int32_t scoring, groups, top_groups, group_score, renormalize;
+  float scale;
+};
+
+template <int DT>
+__device__ __forceinline__ float value_at(const void* p, int64_t at) {
+  if constexpr (DT == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+  else if constexpr (DT == kF16) return __half2float(static_cast<const __half*>(p)[at]);
+  else return static_cast<const float*>(p)[at];
+}
+
+// ------------------------------------------------------------------ numbers that order as values do
+template <class T>
+struct Order;
+template <>
+struct Order<float> {
+  using Key = uint32_t;
+  static __device__ __forceinline__ Key of(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);  // -0 is 0
+    const uint32_t k = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return v == v ? k : 1u;
+  }
+  static __device__ __forceinline__ float value(Key k) {
+    return k == 1u ? NAN : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+  }
+  static __device__ __forceinline__ Key max_of(Key k) { return __reduce_max_sync(kFull, k); }
+  static __device__ __forceinline__ Key from(Key k, int lane) { return __shfl_sync(kFull, k, lane); }
+};
+template <>
+struct Order<double> {
+  using Key = uint64_t;
+  static __device__ __forceinline__ Key of(double v) {
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+    const uint64_t k = b ^ (static_cast<uint64_t>(static_cast<int64_t>(b) >> 63) | 0x8000000000000000ull);
+    return v == v ? k : 1u;
+  }
+  static __device__ __forceinline__ double value(Key k) {
+    return k == 1u ? static_cast<double>(NAN) : __longlong_as_double(static_cast<int64_t>(k >> 63 ? k ^ 0x8000000000000000ull : ~k));
+  }
+  static __device__ __forceinline__ Key max_of(Key k) {
+    const uint32_t hi = static_cast<uint32_t>(k >> 32), top = __reduce_max_sync(kFull, hi);
+    return static_cast<Key>(top) << 32 | __reduce_max_sync(kFull, hi == top ? static_cast<uint32_t>(k) : 0u);
+  }
+  static __device__ __forceinline__ Key from(Key k, int lane) { return __shfl_sync(kFull, k, lane); }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+__device__ __forceinline__ float quotient(float a, float b) { return __fdiv_rn(a, b); }
+__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
+
+// What a token's row of logits has: the largest (a NaN not counted), and whether one is a NaN or +infinity, for which
+// softmax is a NaN everywhere.
+struct Row {
+  float top;
+  bool broken;
+};
+
+// Whether sums of scores decide anything, or the logits alone.
+__device__ __forceinline__ bool scores_decide(const RouteArgs& p) { return p.bias != nullptr || (p.groups > 1 && p.group_score == kTop2); }
+
+constexpr float kMargin = 0x1p-17f, kMarginOfValue = 0x1p-21f;
+
+// Whether a value is so near one below it that fp32 may have put them in the wrong order. False for what is closed.
+__device__ __forceinline__ bool near_by(uint32_t upper, uint32_t lower) {
+  if (lower == 0u) return false;
+  const float a = Order<float>::value(upper), b = Order<float>::value(lower);
+  return !(a - b > kMargin + kMarginOfValue * fmaxf(fabsf(a), fabsf(b)));
+}
+
+// Lane j's expert of the token's choice j, or -1; N experts a lane. `near`: in fp32, whether some order is not certain.
+template <class T, int N>
+__device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane, bool& near) {
+  using O = Order<T>;
+  using Key = typename O::Key;
+  constexpr bool kCheck = sizeof(T) == 4;
+  near = false;
+  const bool by_score = scores_decide(p);
+  Key choice[N], part[N];  // part: what a group counts by
+  if (by_score) {
+    T score[N];
+    if (p.scoring == kSigmoid) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) score[i] = quotient(static_cast<T>(1), static_cast<T>(1) + exp_of(-static_cast<T>(logit[i])));
+    } else {
+      T sum = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        score[i] = exp_of(static_cast<T>(logit[i]) - static_cast<T>(row.top));
+        sum += i * 32 + lane < p.experts ? score[i] : static_cast<T>(0);
+      }
+      sum = warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < N; ++i) score[i] = row.broken ? static_cast<T>(NAN) : quotient(score[i], sum);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = i * 32 + lane;
+      const float bias = p.bias != nullptr && e < p.experts ? p.bias[e] : 0.0f;
+      const bool open = e < p.experts && logit[i] != -INFINITY && bias != -INFINITY;
+      part[i] = open ? O::of(score[i] + static_cast<T>(bias)) : 0;
+      choice[i] = p.bias != nullptr ? part[i] : open ? O::of(static_cast<T>(logit[i])) : 0;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i] = choice[i] = i * 32 + lane < p.experts && logit[i] != -INFINITY ? O::of(static_cast<T>(logit[i])) : 0;
+  }
+
+  if (p.groups > 1) {
+    const int per = p.experts / p.groups;
+    Key mine = 0;  // of group `lane`
+    for (int g = 0; g < p.groups; ++g) {
+      const int first = g * per, last = first + per;
+      Key best = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = i * 32 + lane;
+        const Key k = p.group_score == kTop2 ? part[i] : choice[i];
+        if (e >= first && e < last && k > best) best = k;
+      }
+      Key top = O::max_of(best);
+      if (p.group_score == kTop2 && top != 0) {
+        // the second best: without one of the best, the lowest lane's first
+        const bool owner = lane == __ffs(__ballot_sync(kFull, best == top)) - 1;
+        Key second = 0;
+        bool left_out = !owner;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int e = i * 32 + lane;
+          const bool in = e >= first && e < last;
+          if (in && !left_out && part[i] == top) left_out = true;
+          else if (in && part[i] > second) second = part[i];
+        }
+        second = O::max_of(second);
+        if (second != 0) top = O::of(O::value(top) + O::value(second));
+      }
+      if (lane == g) mine = top;
+    }
+    int before = 0;  // groups that come before this lane's
+    for (int g = 0; g < p.groups; ++g) {
+      const Key other = O::from(mine, g);
+      before += other > mine || (other == mine && g < lane);
+    }
+    const bool kept = lane < p.groups && before < p.top_groups;
+    const uint32_t groups_kept = __ballot_sync(kFull, kept);
+    if (kCheck && by_score && p.top_groups < p.groups) {
+      const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(mine) : 0xFFFFFFFFu);
+      const uint32_t highest = __reduce_max_sync(kFull, kept || lane >= p.groups ? 0u : static_cast<uint32_t>(mine));
+      near |= near_by(lowest, highest);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = i * 32 + lane;
+      if (e < p.experts && !(groups_kept >> (e / per) & 1u)) choice[i] = 0;
+    }
+  }
+
+  int chosen = -1;
+  Key last = 0;
+  const int rounds = p.top_k + (kCheck && p.bias != nullptr);  // one more to see how near the next one is
+  for (int j = 0; j < rounds; ++j) {
+    Key best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = choice[i] > best ? choice[i] : best;
+    const Key top = O::max_of(best);
+    if (kCheck && p.bias != nullptr && j > 0) near |= near_by(static_cast<uint32_t>(last), static_cast<uint32_t>(top));
+    last = top;
+    if (top == 0 || j == p.top_k) break;
+    int e = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) e = choice[i] == top ? i * 32 + lane : e;
+    e = __reduce_min_sync(kFull, e);
+    if (lane == j) chosen = e;
+#pragma unroll
+    for (int i = 0; i < N; ++i) choice[i] = i * 32 + lane == e ? 0 : choice[i];
+  }
+  return chosen;
+}
+
+template <int N>
+__device__ __noinline__ int choose_in_64_bits(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
+  bool near;
+  return choose<double, N>(p, logit, row, lane, near);
+}
+
+// A lane's share of a token's weights, before the scale: the score of its expert, renormalised or not.
+struct Share {
+  float score;  // of the expert
+  float rest;   // 1 - score (sigmoid)
+  float sum;    // what the score is divided by: of the token's scores, or 1
+  bool floor;   // the sum is below 2^-100 and counts as that
+};
+
+constexpr float kLeast = 0x1p-100f;
+
+// `logit`: of this lane's expert, if it has one. `total`: sum of all exp(logit - top) (softmax without renormalising).
+__device__ __forceinline__ Share share_of(int scoring, bool renormalize, float logit, bool has, const Row& row, float total) {
+  Share s{0.0f, 1.0f, 1.0f, false};
+  if (scoring == kSigmoid) {
+    if (has) {
+      s.score = __fdiv_rn(1.0f, 1.0f + expf(-logit));
+      s.rest = __fdiv_rn(1.0f, 1.0f + expf(logit));
+    }
+    if (renormalize) {
+      s.sum = warp_sum(s.score);
+      s.floor = s.sum < kLeast;
+      if (s.floor) s.sum = kLeast;
+    }
+    return s;
+  }
+  if (renormalize) {
+    // the scores' own denominator cancels: relative to the largest of the token's
+    const uint32_t top = Order<float>::max_of(has ? Order<float>::of(logit) : 0u);
+    if (has) s.score = expf(logit - Order<float>::value(top));
+    s.sum = top == 0u ? 1.0f : warp_sum(s.score);
+  } else {
+    if (has) s.score = expf(logit - row.top);
+    s.sum = total;
+  }
+  if (row.broken) s.score = NAN;
+  return s;
+}
+
+template <int DT, int N>
+__device__ __forceinline__ void load_row(const RouteArgs& p, int64_t token, int lane, float (&logit)[N], Row& row) {
+  bool broken = false;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    logit[i] = e < p.experts ? value_at<DT>(p.logits, token * p.stride + e) : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    broken |= !(logit[i] < INFINITY);
+    top = fmaxf(top, logit[i]);
+  }
+  row.broken = __any_sync(kFull, broken);
+  row.top = Order<float>::value(__reduce_max_sync(kFull, Order<float>::of(top)));
+  if (row.top == -INFINITY) row.top = 0.0f;  // nothing is open
+}
+
+// All of softmax's exponentials of a row, relative to its largest.
+template <int N>
+__device__ __forceinline__ float total_of(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum += i * 32 + lane < p.experts ? expf(logit[i] - row.top) : 0.0f;
+  return warp_sum(sum);
+}
+
+// --------------------------------------------------------------------- the order by expert
+// The places of a block's choices, in the order of experts and within one of tokens. `count(chunk, e)` are the choices of
+// each chunk of tokens. start: shared, (experts + 33) words.
+template <class Count>
+__device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, const Count& count) {
+  const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int32_t* warp_sums = start + p.experts;
+  // this chunk's first place within each expert, and the experts' totals, scanned 32 * warps experts at a time
+  int carry = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += threads) {
+    const int e = e0 + threadIdx.x;
+    int before = 0, total = 0;
+    if (e < p.experts) {
+#pragma unroll 8
+      for (int c = 0; c < p.chunks; ++c) {
+        const int n = count(c, e);
+        total += n;
+        before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+    }
+    int scan = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(kFull, scan, o);
+      if (lane >= o) scan += up;
+    }
+    if (lane == 31) warp_sums[warp] = scan;
+    __syncthreads();
+    int all = lane < threads / 32 ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(kFull, all, o);
+      if (lane >= o) all += up;
+    }
+    const int below = warp == 0 ? 0 : __shfl_sync(kFull, all, warp - 1);
+    const int block_total = __shfl_sync(kFull, all, 31);
+    scan += carry + below;
+    if (e < p.experts) {
+      start[e] = scan - total + before;
+      if (blockIdx.x == 0) p.ends[e] = scan;
+    }
+    carry += block_total;
+    __syncthreads();
+  }
+  // places of no choice
+  const int64_t places = p.tokens * p.top_k;
+  for (int64_t i = carry + static_cast<int64_t>(blockIdx.x) * threads + threadIdx.x; i < places; i += static_cast<int64_t>(p.chunks) * threads)
+    p.source[i] = -1;
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * p.chunk * p.top_k;
+  const int items = static_cast<int>(min(static_cast<int64_t>(p.chunk) * p.top_k, places - from));
+  // 32 choices of a warp at once, one warp after another
+  for (int i0 = 0; i0 < items; i0 += threads) {
+    const int i = i0 + threadIdx.x;
+    const int e = i < items ? p.experts_out[from + i] : -1;
+    const uint32_t same = __match_any_sync(kFull, e);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    int at = -1;
+    for (int w = 0; w < threads / 32 && i0 + w * 32 < items; ++w) {
+      if (w == warp && e >= 0) at = start[e] + rank;
+      if (w == warp) __syncwarp();
+      if (w == warp && e >= 0 && rank == 0) start[e] += __popc(same);
+      __syncthreads();
+    }
+    if (i < items) p.rows[from + i] = at;
+    if (at >= 0) p.source[at] = static_cast<int32_t>(from + i);
+  }
+}
+
+// A block has a chunk of tokens, its warps take them in turn. kOne: the one block of the call, which places its choices too.
+template <int DT, int N, bool kOne>
+__global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __grid_constant__ RouteArgs p) {
+  extern __shared__ int32_t shared[];  // choices of each expert; kOne: and the starts
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  fp4::grid_launch_dependents();
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) shared[e] = 0;
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk, end = min(first + p.chunk, p.tokens);
+  for (int64_t token = first + warp; token < end; token += warps) {
+    int chosen = -1;
+    float weight = 0.0f;
+    if (p.mask == nullptr || p.mask[token] != 0) {
+      float logit[N];
+      Row row;
+      load_row<DT, N>(p, token, lane, logit, row);
+      bool near;
+      chosen = choose<float, N>(p, logit, row, lane, near);
+      if (near) chosen = choose_in_64_bits<N>(p, logit, row, lane);
+      const float total = p.scoring == kSoftmax && p.renormalize == 0 ? total_of<N>(p, logit, row, lane) : 1.0f;
+      const float mine = chosen >= 0 ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
+      const Share s = share_of(p.scoring, p.renormalize != 0, mine, chosen >= 0, row, total);
+      weight = chosen >= 0 ? __fdiv_rn(s.score, s.sum) * p.scale : 0.0f;
+    }
+    if (lane < p.top_k) {
+      p.experts_out[token * p.top_k + lane] = chosen;
+      p.weights[token * p.top_k + lane] = weight;
+      if (chosen >= 0) atomicAdd(&shared[chosen], 1);  // a count, whatever the order
+    }
+  }
+  __syncthreads();
+  if constexpr (kOne) {
+    place(p, shared + p.experts, [&](int, int e) { return shared[e]; });
+  } else {
+    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = shared[e];
+  }
+}
+
+__global__ void __launch_bounds__(1024) place_kernel(const __grid_constant__ RouteArgs p) {
+  extern __shared__ int32_t shared[];
+  fp4::grid_wait();
+  place(p, shared, [&](int c, int e) { return p.counts[static_cast<int64_t>(c) * p.experts + e]; });
+}
+
+// --------------------------------------------------------------------------- backward
+struct RouteGradArgs {
+  RouteArgs route;  // logits, experts_out and the rules
+  const float* grad;
+  void* dlogits;
+};
+
+template <int DT>
+__device__ __forceinline__ void store_at(void* p, int64_t at, float v) {
+  if constexpr (DT == kBF16) static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
+  else if constexpr (DT == kF16) static_cast<__half*>(p)[at] = __float2half_rn(v);
+  else static_cast<float*>(p)[at] = v;
+}
+
+// With the shares w of a token's weights and their gradients g (times the scale), S the sum that they were divided by:
+// renormalised softmax: dl_j = w_j (g_j - sum g w), 0 for the others; softmax: dl_e = s_e ([e chosen] g - sum g s);
+// sigmoid: dl_j = g_j s_j (1 - s_j), with (g_j - sum g w) / S in g_j's place where renormalised (g_j / 2^-100 where the
+// sum is below that).
+template <int DT, int N>
+__global__ void __launch_bounds__(256) route_grad_kernel(const __grid_constant__ RouteGradArgs a) {
+  const RouteArgs& p = a.route;
+  const int lane = threadIdx.x & 31;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  const int chosen = lane < p.top_k ? p.experts_out[token * p.top_k + lane] : -1;
+  const bool has = chosen >= 0 && chosen < p.experts;
+  const bool any = __any_sync(kFull, has);
+  const bool whole = p.scoring == kSoftmax && any;  // the row itself is needed
+  float logit[N];
+  Row row{0.0f, false};
+  float total = 1.0f;
+  if (whole) {
+    load_row<DT, N>(p, token, lane, logit, row);
+    if (p.renormalize == 0) total = total_of<N>(p, logit, row, lane);
+  }
+  const float mine = has ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
+  const Share s = share_of(p.scoring, p.renormalize != 0, mine, has, row, total);
+  const float g = has ? a.grad[token * p.top_k + lane] * p.scale : 0.0f;
+  const float w = __fdiv_rn(s.score, s.sum);
+  const float mean = warp_sum(has ? g * w : 0.0f);
+  float d;
+  if (p.scoring == kSigmoid) {
+    const float inner = p.renormalize == 0 ? g : __fdiv_rn(s.floor ? g : g - mean, s.sum);
+    d = inner * s.score * s.rest;
+  } else {
+    d = w * (g - mean);
+  }
+  const bool others = whole && p.renormalize == 0;
+  const int64_t at = token * p.experts;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = i * 32 + lane;
+    if (e < p.experts)
+      store_at<DT>(a.dlogits, at + e, others ? (row.broken ? NAN : -__fdiv_rn(expf(logit[i] - row.top), total) * mean) : 0.0f);
+  }
+  __syncwarp();
+  if (has) store_at<DT>(a.dlogits, at + chosen, d);
+}
+
+}  // namespace routing
