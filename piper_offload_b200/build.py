@@ -1,5 +1,5 @@
 """Build the libraries (``libpiper_merge.so``, ``libpiper_fp4.so``, ``libpiper_int8.so``, ``libpiper_routing.so``) in-tree with nvcc
-for sm_100a, and the FP4 operators' calls with g++.
+for sm_100a, and the operators' compiled calls with g++.
 
 Usage: ``python -m piper_offload_b200.build`` (also called by
 ``__graft_entry__.build()``). A library newer than every source file of its
@@ -44,6 +44,9 @@ ROUTING_DEPS = ROUTING_SOURCES + [
     ROOT / "include" / "piper_routing.h",
 ]
 ROUTING_OUT = PKG / "libpiper_routing.so"
+EXPERT_CALLS_SOURCES = [PKG / "csrc" / "expert_calls.cpp"]
+EXPERT_CALLS_DEPS = EXPERT_CALLS_SOURCES + [ROOT / "include" / "piper_int8.h", ROOT / "include" / "piper_routing.h"]
+EXPERT_CALLS_OUT = PKG / "_expert_calls.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -88,6 +91,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     build_fp4(force, verbose)
     build_int8(force, verbose)
     build_routing(force, verbose)
+    build_expert_calls(force, verbose)
     return OUT
 
 
@@ -111,25 +115,35 @@ def build_routing(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_calls(force: bool = False, verbose: bool = False) -> Path:
-    """The operators' calls from Python: host code against this interpreter's torch, which is noted beside it."""
+    """The FP4 operators' calls from Python."""
+    return _compile_calls(CALLS_OUT, CALLS_SOURCES, CALLS_DEPS, force, verbose)
+
+
+def build_expert_calls(force: bool = False, verbose: bool = False) -> Path:
+    """The calls of the INT8 products, routing and the exchange."""
+    return _compile_calls(EXPERT_CALLS_OUT, EXPERT_CALLS_SOURCES, EXPERT_CALLS_DEPS, force, verbose)
+
+
+def _compile_calls(out: Path, sources: list[Path], deps: list[Path], force: bool, verbose: bool) -> Path:
+    """Host code against this interpreter's torch, which is noted beside it."""
     import torch
 
     fits = f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
-    note = CALLS_OUT.with_suffix(".so.fits")
-    if force or not up_to_date(CALLS_OUT, CALLS_DEPS) or not note.exists() or note.read_text() != fits:
+    note = out.with_suffix(".so.fits")
+    if force or not up_to_date(out, deps) or not note.exists() or note.read_text() != fits:
         base = Path(torch.__file__).resolve().parent
-        tmp = CALLS_OUT.with_suffix(".so.tmp")
+        tmp = out.with_suffix(".so.tmp")
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                *(f"-I{d}" for d in (base / "include", base / "include" / "torch" / "csrc" / "api" / "include",
                                     Path(nvcc()).resolve().parents[1] / "include", sysconfig.get_paths()["include"])),
-               "-o", str(tmp), *map(str, CALLS_SOURCES), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+               "-o", str(tmp), *map(str, sources), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=str(ROOT))
-        os.replace(tmp, CALLS_OUT)
+        os.replace(tmp, out)
         note.write_text(fits)
-    return CALLS_OUT
+    return out
 
 
 if __name__ == "__main__":
@@ -139,3 +153,4 @@ if __name__ == "__main__":
     print(CALLS_OUT)
     print(INT8_OUT)
     print(ROUTING_OUT)
+    print(EXPERT_CALLS_OUT)

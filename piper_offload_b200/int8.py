@@ -32,7 +32,9 @@ with fp32 sums, in which ``dy * scale`` has 11 bits (22 for fp32 gradients).
 
 All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
 take workspaces from PyTorch's caching allocator on it, do not synchronise,
-and raise ``ValueError`` for arguments that they do not take.
+and raise ``ValueError`` for arguments that they do not take. Calls with plain
+arguments are made by compiled code (``csrc/expert_calls.cpp``); what it
+declines takes the path written out here, to the same kernels.
 """
 
 from __future__ import annotations
@@ -45,6 +47,7 @@ from torch.autograd import forward_ad
 
 from . import _native_int8 as nat
 from . import kernels as K
+from ._native_calls import calls
 from ._native_fp4 import raw_stream
 from .adapters import Bnb8Adapter, Int8Adapter, QuantoAdapter
 from .weights import Bnb8Weight, Int8Experts, Int8Weight, QuantoWeight
@@ -138,6 +141,7 @@ def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as a matrix whose rows are contiguous and do not overlap (a view where it is one)."""
+    x = x.resolve_neg()
     if x.ndim != 2:
         x = x.reshape(-1, x.shape[-1])
     if x.stride(1) != 1 or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
@@ -201,11 +205,22 @@ class _Product(torch.autograd.Function):
 
 
 def _product(x: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> torch.Tensor:
+    done = calls().int8(x, weight, ends, False)
+    if done is not None:
+        return done
     w = _Frozen(weight, 2 if ends is None else 3)
     _check_tangents(x)
     if x.requires_grad and torch.is_grad_enabled():
         return _Product.apply(x, w, ends)
     return _run(x, w, ends, False)
+
+
+def _grad_input(grad: torch.Tensor, weight: Any, ends: torch.Tensor | None) -> torch.Tensor:
+    done = calls().int8(grad, weight, ends, True)
+    if done is not None:
+        return done
+    _check_tangents(grad)
+    return _run(grad, _Frozen(weight, 2 if ends is None else 3), ends, True)
 
 
 def linear_int8(x: torch.Tensor, weight: Int8Weight | Bnb8Weight | QuantoWeight) -> torch.Tensor:
@@ -234,13 +249,11 @@ def grouped_linear_int8(x: torch.Tensor, experts: Int8Experts, group_ends: torch
 
 def linear_int8_grad_input(grad: torch.Tensor, weight: Int8Weight | Bnb8Weight | QuantoWeight) -> torch.Tensor:
     """``grad @ values(weight)`` for ``grad`` (..., rows): :func:`linear_int8`'s gradient, in the type of ``grad``."""
-    _check_tangents(grad)
-    return _run(grad, _Frozen(weight, 2), None, True)
+    return _grad_input(grad, weight, None)
 
 
 def grouped_linear_int8_grad_input(grad: torch.Tensor, experts: Int8Experts, group_ends: torch.Tensor) -> torch.Tensor:
     """:func:`grouped_linear_int8`'s gradient with respect to its tokens; rows past the last end get zeros."""
     if grad.ndim != 2:
         raise ValueError("grouped_linear_int8_grad_input takes a stack of experts and a rank-two gradient.")
-    _check_tangents(grad)
-    return _run(grad, _Frozen(experts, 3), group_ends, True)
+    return _grad_input(grad, experts, group_ends)

@@ -19,7 +19,9 @@ experts is::
 All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
 take workspaces from PyTorch's caching allocator on it, do not synchronise,
 give the same bits on every run, and raise ``ValueError`` for arguments that
-they do not take.
+they do not take. Calls with plain arguments are made by compiled code
+(``csrc/expert_calls.cpp``); what it declines takes the path written out here,
+to the same kernels.
 """
 
 from __future__ import annotations
@@ -32,6 +34,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _native_routing as nat
+from ._native_calls import calls
 from ._native_fp4 import raw_stream
 
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
@@ -71,6 +74,7 @@ def _call(function: Any, device: torch.device, *args: Any) -> None:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x with contiguous rows that do not overlap (x itself where it has them)."""
+    x = x.resolve_neg()
     if x.stride(1) != 1 or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
         x = x.contiguous()
     return x
@@ -142,15 +146,20 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", 
     False gets no expert. The weights are differentiable with respect to the
     logits; ``bias`` gets no gradient.
     """
+    if scoring not in _SCORING:
+        raise ValueError(f"Routing scores are softmax or sigmoid, got {scoring!r}.")
+    if group_score not in _GROUP_SCORE:
+        raise ValueError(f"A group's score is max or top2, got {group_score!r}.")
+    if top_groups is None:
+        top_groups = groups
+    done = calls().route(logits, top_k, _SCORING[scoring], bias, groups, top_groups, _GROUP_SCORE[group_score], renormalize, scale, mask)
+    if done is not None:
+        return Routing(*done)
     if not logits.is_cuda:
         raise ValueError("Routing requires CUDA tensors.")
     if logits.ndim != 2:
         raise ValueError("route_tokens takes logits (tokens, experts).")
     _dtype(logits, "Routing")
-    if scoring not in _SCORING:
-        raise ValueError(f"Routing scores are softmax or sigmoid, got {scoring!r}.")
-    if group_score not in _GROUP_SCORE:
-        raise ValueError(f"A group's score is max or top2, got {group_score!r}.")
     tokens, experts = logits.shape
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (experts,) or bias.device != logits.device:
@@ -164,8 +173,7 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", 
     for value, most, what in limits:
         if not 1 <= value <= most:
             raise ValueError(f"Routing takes 1 to {most} {what}, got {value}.")
-    config = nat.Config(tokens, experts, top_k, _SCORING[scoring], groups, groups if top_groups is None else top_groups,
-                        _GROUP_SCORE[group_score], bool(renormalize), scale)
+    config = nat.Config(tokens, experts, top_k, _SCORING[scoring], groups, top_groups, _GROUP_SCORE[group_score], bool(renormalize), scale)
     _check_tangents(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return Routing(*_Route.apply(logits, config, bias, mask))
@@ -244,6 +252,9 @@ def dispatch_tokens(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """``x`` (tokens, hidden) copied to the places of its choices: (tokens * top_k, hidden), sorted by expert, zeros past the
     last end. Its gradient adds the copies' up, in fp32 in the order of the slots, rounded once."""
     rows, ends = routing.rows, routing.ends
+    done = calls().dispatch(x, rows, ends)
+    if done is not None:
+        return done
     _check_tangents(x)
     if x.requires_grad and torch.is_grad_enabled():
         return _Dispatch.apply(x, rows, ends)
@@ -255,6 +266,9 @@ def combine_tokens(y: torch.Tensor, routing: Routing) -> torch.Tensor:
     order of the slots, rounded once. A token without a choice gets zeros. Differentiable with respect to ``y`` and to the
     routing's weights."""
     rows, ends, weights = routing.rows, routing.ends, routing.weights
+    done = calls().combine(y, weights, rows, ends)
+    if done is not None:
+        return done
     if weights.dtype is not torch.float32 or weights.shape != rows.shape or weights.device != rows.device:
         raise ValueError("A routing's weights are float32, one for each choice.")
     weights = weights.contiguous()
