@@ -127,9 +127,17 @@ i8::RepackArgs repack_args(const piper_int8_matrix& w, uint8_t* out) {
   return r;
 }
 
-// Blocks for `rows` rows of `units` units: a warp a row where that is enough for its registers.
-bool narrow(int64_t units) { return units <= 64; }
-int64_t row_blocks(int64_t rows, int64_t units) { return narrow(units) ? (rows + 7) / 8 : rows; }
+// Which threads work on a row of `units` units: a warp, which waits for no other, where its registers hold the row and
+// there are rows for all SMs, else the eight warps of a block.
+struct RowPlan {
+  int warps, hold;
+  int64_t blocks;
+};
+RowPlan plan_rows(int64_t rows, int64_t units, int most) {
+  if (units <= 64) return {1, 2, (rows + 7) / 8};
+  if (units <= 32 * most && rows >= 8 * sm_count()) return {1, most, (rows + 7) / 8};
+  return {8, units <= 512 ? 2 : 4, rows};
+}
 
 // ---------------------------------------------------------------- the product
 struct TilePlan {
@@ -340,17 +348,20 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   const int64_t items = token_tiles(tokens, ends == nullptr ? 0 : w->batch, p.bn) * a.groups.row_tiles;
   a.items = static_cast<int32_t>(items);
   INT8_REQUIRE(items < (int64_t{1} << 31) / i8::kMaxSplit, "INT8 product: too many tiles for one call.");
-  const int64_t units = p.x_pitch / i8::kUnit, token_blocks = row_blocks(tokens, units);
-  const int64_t blocks = token_blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  const int most = dtype == PIPER_INT8_F32 ? 4 : 8;
+  const RowPlan rows = plan_rows(tokens, p.x_pitch / i8::kUnit, most);
+  const int64_t blocks = rows.blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
   INT8_REQUIRE(blocks < (int64_t{1} << 31), "INT8 product: too many values for one call.");
   const void* codes = r.pieces > 0 ? r.out : w->codes;
   if (!encode_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, w->cols, w->batch * w->rows, code_pitch(*w), i8::kStageCols, fp4::kTileRows) ||
       !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
-#define CALL(D)                                                                                          \
-  if (narrow(units)) i8::quantize_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid); \
+  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
+#define CALL(D)                                                                                                                     \
+  if (rows.warps == 1 && rows.hold == 2) i8::quantize_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid);        \
+  else if (rows.warps == 1) i8::quantize_kernel<D, 1, D == i8::kF32 ? 4 : 8><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid); \
+  else if (rows.hold == 2) i8::quantize_kernel<D, 8, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid);                      \
   else i8::quantize_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
@@ -415,15 +426,17 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   a.terms = p.terms;
   a.split = tile.split;
   a.vec = aligned(dx, 16) && (w->cols * static_cast<int64_t>(width(dtype))) % 16 == 0;
-  const int64_t units = p.pitch / i8::kUnit, token_blocks = row_blocks(tokens, units);
-  const int64_t blocks = token_blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, 4);
+  const int64_t blocks = rows.blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
   INT8_REQUIRE(tile.items < (int64_t{1} << 31) / i8::kMaxSplit && blocks < (int64_t{1} << 31), "INT8 gradient: too many tiles for one call.");
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(token_blocks);
-#define CALL(D)                                                                                       \
-  if (narrow(units)) i8::scale_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid); \
+  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
+#define CALL(D)                                                                                                            \
+  if (rows.warps == 1 && rows.hold == 2) i8::scale_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid); \
+  else if (rows.warps == 1) i8::scale_kernel<D, 1, 4><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid);               \
+  else if (rows.hold == 2) i8::scale_kernel<D, 8, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid);                \
   else i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL

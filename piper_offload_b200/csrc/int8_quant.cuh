@@ -264,11 +264,29 @@ struct ScaleArgs {
   int32_t experts;
 };
 
-__device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
-
+// The scales of sixteen rows of the weight from `n` on, 0 past the last. A lane takes them as it takes its values.
 template <int DT>
-__device__ __forceinline__ float scaled_value(const Unit<DT>& u, int i, const ScaleArgs& p, int64_t scale0, int n) {
-  return n < p.rows ? unit_value<DT>(u, i) * row_scale(p.scales, scale0 + n) : 0.0f;
+__device__ __forceinline__ void unit_scales(const void* scale, int64_t row0, int n, int rows, float (&s)[kUnit]) {
+  const uint8_t* from = static_cast<const uint8_t*>(scale) + row0 * (DT == kF32 ? 4 : 2);
+  const Unit<DT> u = load_unit<DT>(from, n, rows, (reinterpret_cast<uintptr_t>(from) & 15) == 0);
+#pragma unroll
+  for (int i = 0; i < kUnit; ++i) s[i] = unit_value<DT>(u, i);
+}
+
+__device__ __forceinline__ void scales_of(const ScaleArgs& p, int64_t row0, int n, float (&s)[kUnit]) {
+  if (p.scales.step == 0) {
+    const float one = row_scale(p.scales, 0);
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) s[i] = n + i < p.rows ? one : 0.0f;
+    return;
+  }
+  if (p.scales.dtype == kBF16) unit_scales<kBF16>(p.scales.scale, row0, n, p.rows, s);
+  else if (p.scales.dtype == kF16) unit_scales<kF16>(p.scales.scale, row0, n, p.rows, s);
+  else unit_scales<kF32>(p.scales.scale, row0, n, p.rows, s);
+  if (p.scales.over_127 != 0) {
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) s[i] = __fdiv_rn(s[i], 127.0f);
+  }
 }
 
 template <int DT, int kWarps, int kHold>
@@ -278,40 +296,54 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   const int expert = expert_of(p.ends, p.experts, static_cast<int>(team.row));
   if (expert == p.experts) return;  // rows of no expert are not read
   constexpr int kStep = 32 * kWarps;
-  const int64_t scale0 = static_cast<int64_t>(expert) * p.rows;
+  const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
   const uint8_t* row = static_cast<const uint8_t*>(p.dy) + team.row * p.dy_stride * (DT == kF32 ? 4 : 2);
   const int units = static_cast<int>(p.pitch / kUnit);
   Unit<DT> held[kHold];
   float top = 0.0f;
-  const auto see = [&](const Unit<DT>& u, int unit) {
+  const auto see = [&](const Unit<DT>& u, int unit, bool finite) {
+    float s[kUnit];
+    scales_of(p, row0, unit * kUnit, s);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) top = fmaxf(top, finite_or_zero(scaled_value<DT>(u, i, p, scale0, unit * kUnit + i)));
+    for (int i = 0; i < kUnit; ++i) {
+      const float v = fabsf(unit_value<DT>(u, i) * s[i]);
+      top = fmaxf(top, finite && !(v < INFINITY) ? 0.0f : v);  // a NaN is not counted
+    }
   };
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
     if (team.thread + k * kStep < units) held[k] = load_unit<DT>(row, (team.thread + k * kStep) * kUnit, p.rows, p.vec != 0);
+  const auto see_all = [&](bool finite) {
 #pragma unroll
-  for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) see(held[k], team.thread + k * kStep);
-  for (int u = team.thread + kHold * kStep; u < units; u += kStep) see(load_unit<DT>(row, u * kUnit, p.rows, p.vec != 0), u);
-  const uint32_t bits = team.max_of(__float_as_uint(top), words);
+    for (int k = 0; k < kHold; ++k)
+      if (team.thread + k * kStep < units) see(held[k], team.thread + k * kStep, finite);
+    for (int u = team.thread + kHold * kStep; u < units; u += kStep) see(load_unit<DT>(row, u * kUnit, p.rows, p.vec != 0), u, finite);
+  };
+  see_all(false);
+  uint32_t bits = team.max_of(__float_as_uint(top), words);
+  if (bits == __float_as_uint(INFINITY)) {
+    top = 0.0f;
+    see_all(true);
+    if constexpr (kWarps > 1) __syncthreads();  // the words are read
+    bits = team.max_of(__float_as_uint(top), words);
+  }
   // 2^(14 - exponent), within fp32's normal numbers; 1 for a row of zeros
   const int exponent = bits == 0u ? 14 : max(static_cast<int>(bits >> 23) - 127, -112);
   const float power = __uint_as_float(static_cast<uint32_t>(141 - exponent) << 23);
   const auto write = [&](const Unit<DT>& u, int unit) {
+    float s[kUnit];
+    scales_of(p, row0, unit * kUnit, s);
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
-      __half h[2], l[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float v = scaled_value<DT>(u, i + k, p, scale0, unit * kUnit + i + k) * power;
-        h[k] = __float2half_rn(v);
+      const float a = unit_value<DT>(u, i) * s[i] * power, b = unit_value<DT>(u, i + 1) * s[i + 1] * power;
+      const __half2 h = __floats2half2_rn(a, b);
+      hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+      if constexpr (DT == kF32) {
         // an infinity or a NaN is its first term alone
-        if constexpr (DT == kF32) l[k] = __float2half_rn(fabsf(v) < INFINITY ? v - __half2float(h[k]) : 0.0f);
+        const __half2 l = __floats2half2_rn(fabsf(a) < INFINITY ? a - __low2float(h) : 0.0f, fabsf(b) < INFINITY ? b - __high2float(h) : 0.0f);
+        lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
       }
-      hi[i / 2] = static_cast<uint32_t>(__half_as_ushort(h[0])) | static_cast<uint32_t>(__half_as_ushort(h[1])) << 16;
-      if constexpr (DT == kF32) lo[i / 2] = static_cast<uint32_t>(__half_as_ushort(l[0])) | static_cast<uint32_t>(__half_as_ushort(l[1])) << 16;
     }
     uint4* to = reinterpret_cast<uint4*>(p.out + team.row * p.pitch + static_cast<int64_t>(unit) * kUnit);
     to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);

@@ -73,8 +73,13 @@ int check_config(const piper_routing_config* c) {
 
 constexpr int64_t kOneBlockTokens = 128;
 
-// Threads of a block that has the tokens of a chunk: registers for more experts a lane leave fewer.
-int route_threads(int experts) { return experts > 256 ? 512 : 1024; }
+// Threads of a block that has the tokens of a chunk, a power of two: a warp a token, as many as registers for the experts of
+// a lane leave.
+int route_threads(int experts, int chunk) {
+  int threads = 256;
+  while (threads < chunk * 32 && threads < (experts > 256 ? 512 : 1024)) threads *= 2;
+  return threads;
+}
 
 // A chunk of tokens for every SM, whole rounds of a block's warps where there are enough.
 struct Chunks {
@@ -82,7 +87,7 @@ struct Chunks {
 };
 Chunks chunks_of(const piper_routing_config& c) {
   if (c.tokens <= kOneBlockTokens) return {1, static_cast<int>(std::max<int64_t>(c.tokens, 1))};
-  const int64_t size = std::max<int64_t>((c.tokens + sm_count() - 1) / sm_count(), 8);
+  const int64_t size = std::max<int64_t>((c.tokens + sm_count() - 1) / sm_count(), 4);
   return {static_cast<int>((c.tokens + size - 1) / size), static_cast<int>(size)};
 }
 
@@ -107,10 +112,18 @@ routing::RouteArgs route_args(const piper_routing_config& c) {
     else { CALL(routing::kF32); }                                      \
   } while (0)
 
+// Whether a lane's N neighbouring logits lie in pieces that one load takes, each there or not as a whole.
+bool whole_pieces(const routing::RouteArgs& a, int n, size_t size) {
+  const size_t bytes = std::min<size_t>(16, n * size);
+  return bytes >= 4 && aligned(a.logits, bytes) && (a.stride * static_cast<int64_t>(size)) % static_cast<int64_t>(bytes) == 0 &&
+         a.experts % static_cast<int>(bytes / size) == 0;
+}
+
 template <int DT, int N>
-cudaError_t launch_route(const routing::RouteArgs& a, int threads, cudaStream_t s) {
+cudaError_t launch_route(routing::RouteArgs a, int threads, cudaStream_t s) {
+  a.vec = whole_pieces(a, N, width(DT));
   if (a.chunks == 1) {
-    routing::route_kernel<DT, N, true><<<1, threads, (2 * a.experts + 32) * 4, s>>>(a);
+    routing::route_kernel<DT, N, true><<<1, threads, (2 * a.experts + 32 + 2 * threads) * 4, s>>>(a);
     return launched();
   }
   routing::route_kernel<DT, N, false><<<static_cast<unsigned>(a.chunks), threads, a.experts * 4, s>>>(a);
@@ -119,7 +132,7 @@ cudaError_t launch_route(const routing::RouteArgs& a, int threads, cudaStream_t 
 
 template <int DT>
 cudaError_t launch_route(const routing::RouteArgs& a, cudaStream_t s) {
-  const int threads = route_threads(a.experts);
+  const int threads = route_threads(a.experts, a.chunk);
   if (a.experts <= 32) return launch_route<DT, 1>(a, threads, s);
   if (a.experts <= 64) return launch_route<DT, 2>(a, threads, s);
   if (a.experts <= 128) return launch_route<DT, 4>(a, threads, s);
@@ -128,17 +141,22 @@ cudaError_t launch_route(const routing::RouteArgs& a, cudaStream_t s) {
   return launch_route<DT, 32>(a, threads, s);
 }
 
+template <int DT, int N>
+cudaError_t launch_route_grad(routing::RouteGradArgs a, cudaStream_t s) {
+  a.route.vec = whole_pieces(a.route, N, width(DT));
+  routing::route_grad_kernel<DT, N><<<static_cast<unsigned>((a.route.tokens + 7) / 8), 256, 0, s>>>(a);
+  return launched();
+}
+
 template <int DT>
 cudaError_t launch_route_grad(const routing::RouteGradArgs& a, cudaStream_t s) {
-  const auto grid = static_cast<unsigned>((a.route.tokens + 7) / 8);
   const int n = a.route.experts;
-  if (n <= 32) routing::route_grad_kernel<DT, 1><<<grid, 256, 0, s>>>(a);
-  else if (n <= 64) routing::route_grad_kernel<DT, 2><<<grid, 256, 0, s>>>(a);
-  else if (n <= 128) routing::route_grad_kernel<DT, 4><<<grid, 256, 0, s>>>(a);
-  else if (n <= 256) routing::route_grad_kernel<DT, 8><<<grid, 256, 0, s>>>(a);
-  else if (n <= 512) routing::route_grad_kernel<DT, 16><<<grid, 256, 0, s>>>(a);
-  else routing::route_grad_kernel<DT, 32><<<grid, 256, 0, s>>>(a);
-  return launched();
+  if (n <= 32) return launch_route_grad<DT, 1>(a, s);
+  if (n <= 64) return launch_route_grad<DT, 2>(a, s);
+  if (n <= 128) return launch_route_grad<DT, 4>(a, s);
+  if (n <= 256) return launch_route_grad<DT, 8>(a, s);
+  if (n <= 512) return launch_route_grad<DT, 16>(a, s);
+  return launch_route_grad<DT, 32>(a, s);
 }
 
 int check_exchange(const piper_routing_exchange* e) {
@@ -241,7 +259,7 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(n.count));
   config.blockDim = dim3(1024);
-  config.dynamicSmemBytes = (a.experts + 32) * 4;
+  config.dynamicSmemBytes = (a.experts + 32 + 2 * 1024) * 4;
   config.stream = s;
   config.attrs = &attribute;
   config.numAttrs = 1;

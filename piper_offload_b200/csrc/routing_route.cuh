@@ -1,13 +1,17 @@
 // routing_route.cuh - a token's experts: scores, the best groups, the best experts in them, weights, and the order by expert.
 //
-// A warp has a token and a lane every 32nd expert. Choices are compared as whole numbers that order as the scores do (0 for
-// what is closed, 1 for a NaN), the largest found by redux, ties by a second redux for the lowest index.
+// A warp has a token and each lane N neighbouring experts. Choices are compared as whole numbers that order as the scores
+// do (0 for what is closed, 1 for a NaN): the largest is found by redux, its lane by a vote, so that ties go to the lowest
+// index. Where a group's experts fill a power of two of lanes, all groups' two best are found at once by shuffles.
 //
 // Choice scores. Without a bias the logits themselves decide: both scores grow with them. With one, or where a group counts
 // by its two best, sums of scores decide, and sums that are near each other in fp32 may be in another order than the
-// numbers they stand for. So each gap that decides anything is held against a margin that is above twice the sums' error
-// (expf is within 2 ulp, so a score is within 2^-20 of 1; 2^-24 of the sum for its own rounding), and a token with a gap
-// within it is done again in 64 bits: 1 to 2 % of the tokens where 256 experts' scores are spread over [0, 1].
+// numbers they stand for. So each gap that decides anything is held against a margin, and a token with a gap within it is
+// done again in 64 bits: 1 to 2 % of the tokens where 256 experts' scores are spread over [0, 1]. The margin of 2^-17 is
+// above twice the error of two scores added up, which are at most 1 (of sigmoids 2): the fast exponential is off by 2 steps
+// of 2^-23 and 1.2 more for each unit of its argument d, where d exp(-d) is below 0.37, the fast quotient by 2 steps, a
+// softmax's sum by a step of 2^-24 for each of at most 37 additions; together 2^-18.5 for softmax, 2^-20 for sigmoids.
+// 2^-21 of the sum is above twice its own rounding.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,6 +44,7 @@ struct RouteArgs {
   int32_t chunks;
   int32_t experts, top_k;
   int32_t scoring, groups, top_groups, group_score, renormalize;
+  int32_t vec;      // a lane's logits may be read in pieces of 16 bytes, or of all its bytes
   float scale;
 };
 
@@ -96,9 +101,10 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+// For scores that are compared: the fast forms in fp32 (the margin below covers them).
+__device__ __forceinline__ float exp_of(float v) { return __expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
-__device__ __forceinline__ float quotient(float a, float b) { return __fdiv_rn(a, b); }
+__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }
 __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
 // What a token's row of logits has: the largest (a NaN not counted), and whether one is a NaN or +infinity, for which
@@ -120,14 +126,36 @@ __device__ __forceinline__ bool near_by(uint32_t upper, uint32_t lower) {
   return !(a - b > kMargin + kMarginOfValue * fmaxf(fabsf(a), fabsf(b)));
 }
 
-// Lane j's expert of the token's choice j, or -1; N experts a lane. `near`: in fp32, whether some order is not certain.
+// The two largest of a group's keys, as it counts: the best one, or both added up; 0 for a group with nothing open.
+template <class T>
+__device__ __forceinline__ typename Order<T>::Key group_key(int group_score, typename Order<T>::Key best, typename Order<T>::Key second) {
+  using O = Order<T>;
+  return group_score == kMax || second == 0 ? best : O::of(O::value(best) + O::value(second));
+}
+
+template <class K>
+__device__ __forceinline__ void take(K& best, K& second, K k) {
+  const K low = k < best ? k : best;
+  second = low > second ? low : second;
+  best = k > best ? k : best;
+}
+
+// What decides about a token: lane j's choice j and the logit behind it (NaN: not known), or -1. `near`: in fp32, whether
+// some order is not certain.
+struct Choice {
+  int expert;
+  float logit;
+  bool near;
+};
+
 template <class T, int N>
-__device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane, bool& near) {
+__device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
   using O = Order<T>;
   using Key = typename O::Key;
   constexpr bool kCheck = sizeof(T) == 4;
-  near = false;
+  Choice out{-1, NAN, false};
   const bool by_score = scores_decide(p);
+  const int e0 = lane * N;
   Key choice[N], part[N];  // part: what a group counts by
   if (by_score) {
     T score[N];
@@ -138,8 +166,8 @@ __device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N
       T sum = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        score[i] = exp_of(static_cast<T>(logit[i]) - static_cast<T>(row.top));
-        sum += i * 32 + lane < p.experts ? score[i] : static_cast<T>(0);
+        score[i] = exp_of(static_cast<T>(logit[i]) - static_cast<T>(row.top));  // 0 where there is no expert
+        sum += score[i];
       }
       sum = warp_sum(sum);
 #pragma unroll
@@ -147,92 +175,91 @@ __device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = i * 32 + lane;
-      const float bias = p.bias != nullptr && e < p.experts ? p.bias[e] : 0.0f;
-      const bool open = e < p.experts && logit[i] != -INFINITY && bias != -INFINITY;
+      const float bias = p.bias != nullptr && e0 + i < p.experts ? p.bias[e0 + i] : 0.0f;
+      const bool open = logit[i] != -INFINITY && bias != -INFINITY;
       part[i] = open ? O::of(score[i] + static_cast<T>(bias)) : 0;
       choice[i] = p.bias != nullptr ? part[i] : open ? O::of(static_cast<T>(logit[i])) : 0;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) part[i] = choice[i] = i * 32 + lane < p.experts && logit[i] != -INFINITY ? O::of(static_cast<T>(logit[i])) : 0;
+    for (int i = 0; i < N; ++i) part[i] = choice[i] = logit[i] != -INFINITY ? O::of(static_cast<T>(logit[i])) : 0;
   }
 
   if (p.groups > 1) {
-    const int per = p.experts / p.groups;
-    Key mine = 0;  // of group `lane`
-    for (int g = 0; g < p.groups; ++g) {
-      const int first = g * per, last = first + per;
-      Key best = 0;
+    const int per = p.experts / p.groups, span = per / N;
+    Key mine = 0;  // of the group that this lane's experts are in; else of group `lane`
+    const bool whole = span * N == per && (span & (span - 1)) == 0;
+    if (whole) {
+      Key best = 0, second = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int e = i * 32 + lane;
-        const Key k = p.group_score == kTop2 ? part[i] : choice[i];
-        if (e >= first && e < last && k > best) best = k;
+      for (int i = 0; i < N; ++i) take(best, second, p.group_score == kTop2 ? part[i] : choice[i]);
+      for (int o = 1; o < span; o <<= 1) {
+        const Key b = __shfl_xor_sync(kFull, best, o), s = __shfl_xor_sync(kFull, second, o);
+        take(best, second, b);
+        take(best, second, s);
       }
-      Key top = O::max_of(best);
-      if (p.group_score == kTop2 && top != 0) {
-        // the second best: without one of the best, the lowest lane's first
-        const bool owner = lane == __ffs(__ballot_sync(kFull, best == top)) - 1;
-        Key second = 0;
-        bool left_out = !owner;
+      mine = group_key<T>(p.group_score, best, second);
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        Key best = 0, second = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int e = i * 32 + lane;
-          const bool in = e >= first && e < last;
-          if (in && !left_out && part[i] == top) left_out = true;
-          else if (in && part[i] > second) second = part[i];
+        for (int i = 0; i < N; ++i)
+          if (e0 + i >= g * per && e0 + i < g * per + per) take(best, second, p.group_score == kTop2 ? part[i] : choice[i]);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const Key b = __shfl_xor_sync(kFull, best, o), s = __shfl_xor_sync(kFull, second, o);
+          take(best, second, b);
+          take(best, second, s);
         }
-        second = O::max_of(second);
-        if (second != 0) top = O::of(O::value(top) + O::value(second));
+        if (lane == g) mine = group_key<T>(p.group_score, best, second);
       }
-      if (lane == g) mine = top;
     }
+    const int group = whole ? lane / span : lane;
     int before = 0;  // groups that come before this lane's
     for (int g = 0; g < p.groups; ++g) {
-      const Key other = O::from(mine, g);
-      before += other > mine || (other == mine && g < lane);
+      const Key other = O::from(mine, whole ? g * span : g);
+      before += other > mine || (other == mine && g < group);
     }
-    const bool kept = lane < p.groups && before < p.top_groups;
-    const uint32_t groups_kept = __ballot_sync(kFull, kept);
+    const bool kept = group < p.groups && before < p.top_groups;
     if (kCheck && by_score && p.top_groups < p.groups) {
       const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(mine) : 0xFFFFFFFFu);
-      const uint32_t highest = __reduce_max_sync(kFull, kept || lane >= p.groups ? 0u : static_cast<uint32_t>(mine));
-      near |= near_by(lowest, highest);
+      const uint32_t highest = __reduce_max_sync(kFull, kept || group >= p.groups ? 0u : static_cast<uint32_t>(mine));
+      out.near |= near_by(lowest, highest);
     }
+    const uint32_t groups_kept = __ballot_sync(kFull, kept);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = i * 32 + lane;
-      if (e < p.experts && !(groups_kept >> (e / per) & 1u)) choice[i] = 0;
-    }
+    for (int i = 0; i < N; ++i)
+      if (whole ? !kept : e0 + i < p.experts && !(groups_kept >> ((e0 + i) / per) & 1u)) choice[i] = 0;
   }
 
-  int chosen = -1;
   Key last = 0;
   const int rounds = p.top_k + (kCheck && p.bias != nullptr);  // one more to see how near the next one is
   for (int j = 0; j < rounds; ++j) {
-    Key best = 0;
+    Key best = choice[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = choice[i] > best ? choice[i] : best;
+    for (int i = 1; i < N; ++i) best = choice[i] > best ? choice[i] : best;
     const Key top = O::max_of(best);
-    if (kCheck && p.bias != nullptr && j > 0) near |= near_by(static_cast<uint32_t>(last), static_cast<uint32_t>(top));
+    if (kCheck && p.bias != nullptr && j > 0) out.near |= near_by(static_cast<uint32_t>(last), static_cast<uint32_t>(top));
     last = top;
     if (top == 0 || j == p.top_k) break;
-    int e = 0x7FFFFFFF;
+    const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
+    int at = 0;  // the first of this lane's that is as large
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) e = choice[i] == top ? i * 32 + lane : e;
-    e = __reduce_min_sync(kFull, e);
-    if (lane == j) chosen = e;
+    for (int i = N - 1; i >= 0; --i) at = choice[i] == top ? i : at;
+    const int expert = __shfl_sync(kFull, e0 + at, owner);
+    if (lane == j) {
+      out.expert = expert;
+      if (p.bias == nullptr) out.logit = static_cast<float>(O::value(top));
+    }
 #pragma unroll
-    for (int i = 0; i < N; ++i) choice[i] = i * 32 + lane == e ? 0 : choice[i];
+    for (int i = 0; i < N; ++i) choice[i] = lane == owner && i == at ? 0 : choice[i];
   }
-  return chosen;
+  return out;
 }
 
 template <int N>
 __device__ __noinline__ int choose_in_64_bits(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
-  bool near;
-  return choose<double, N>(p, logit, row, lane, near);
+  return choose<double, N>(p, logit, row, lane).expert;
 }
 
 // A lane's share of a token's weights, before the scale: the score of its expert, renormalised or not.
@@ -273,15 +300,46 @@ __device__ __forceinline__ Share share_of(int scoring, bool renormalize, float l
   return s;
 }
 
+// A lane's N neighbouring values of a row, from value `at` on; -infinity past the last.
+template <int DT, int N>
+__device__ __forceinline__ void load_values(const void* from, int64_t at, int count, bool vec, float (&v)[N]) {
+  constexpr int kSize = DT == kF32 ? 4 : 2, kBytes = N * kSize < 16 ? N * kSize : 16, kEach = kBytes / kSize;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = -INFINITY;
+  if (vec && kBytes >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += kEach) {
+      if (i >= count) continue;  // a piece is there or not as a whole
+      uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
+      const uint8_t* q = static_cast<const uint8_t*>(from) + (at + i) * kSize;
+      if constexpr (kBytes == 16) {
+        const uint4 r = *reinterpret_cast<const uint4*>(q);
+        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+      } else if constexpr (kBytes == 8) {
+        const uint2 r = *reinterpret_cast<const uint2*>(q);
+        w[0] = r.x; w[1] = r.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(q);
+      }
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        if constexpr (DT == kF32) v[i + k] = __uint_as_float(w[k]);
+        else if constexpr (DT == kBF16) v[i + k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
+        else v[i + k] = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1)))));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < count) v[i] = value_at<DT>(from, at + i);
+  }
+}
+
 template <int DT, int N>
 __device__ __forceinline__ void load_row(const RouteArgs& p, int64_t token, int lane, float (&logit)[N], Row& row) {
+  load_values<DT, N>(p.logits, token * p.stride + lane * N, p.experts - lane * N, p.vec != 0, logit);
   bool broken = false;
   float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    logit[i] = e < p.experts ? value_at<DT>(p.logits, token * p.stride + e) : -INFINITY;
-  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     broken |= !(logit[i] < INFINITY);
@@ -294,32 +352,46 @@ __device__ __forceinline__ void load_row(const RouteArgs& p, int64_t token, int 
 
 // All of softmax's exponentials of a row, relative to its largest.
 template <int N>
-__device__ __forceinline__ float total_of(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
+__device__ __forceinline__ float total_of(const float (&logit)[N], const Row& row) {
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum += i * 32 + lane < p.experts ? expf(logit[i] - row.top) : 0.0f;
+  for (int i = 0; i < N; ++i) sum += expf(logit[i] - row.top);  // 0 where there is no expert
   return warp_sum(sum);
 }
 
 // --------------------------------------------------------------------- the order by expert
 // The places of a block's choices, in the order of experts and within one of tokens. `count(chunk, e)` are the choices of
-// each chunk of tokens. start: shared, (experts + 33) words.
+// each chunk of tokens. start: shared, (experts + 32) words; parts: 2 words a thread.
 template <class Count>
-__device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, const Count& count) {
+__device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, int32_t* parts, const Count& count) {
   const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int32_t* warp_sums = start + p.experts;
-  // this chunk's first place within each expert, and the experts' totals, scanned 32 * warps experts at a time
+  // experts are taken `wide` at a time, and several threads share the chunks of one
+  const int wide = p.experts >= threads ? threads : p.experts <= 32 ? 32 : 1 << (32 - __clz(p.experts - 1));
+  const int shares = threads / wide, share = threadIdx.x / wide, in = threadIdx.x % wide;
+  // this chunk's first place within each expert, and the experts' totals, scanned
   int carry = 0;
-  for (int e0 = 0; e0 < p.experts; e0 += threads) {
-    const int e = e0 + threadIdx.x;
+  for (int e0 = 0; e0 < p.experts; e0 += wide) {
+    const int e = e0 + in;
     int before = 0, total = 0;
     if (e < p.experts) {
 #pragma unroll 8
-      for (int c = 0; c < p.chunks; ++c) {
+      for (int c = share; c < p.chunks; c += shares) {
         const int n = count(c, e);
         total += n;
         before += c < static_cast<int>(blockIdx.x) ? n : 0;
       }
+    }
+    if (shares > 1) {
+      parts[threadIdx.x] = total;
+      parts[threads + threadIdx.x] = before;
+      __syncthreads();
+      total = before = 0;
+      if (share == 0)
+        for (int k = 0; k < shares; ++k) {
+          total += parts[k * wide + in];
+          before += parts[threads + k * wide + in];
+        }
     }
     int scan = total;
 #pragma unroll
@@ -329,16 +401,15 @@ __device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, const 
     }
     if (lane == 31) warp_sums[warp] = scan;
     __syncthreads();
-    int all = lane < threads / 32 ? warp_sums[lane] : 0;
+    int all = lane < wide / 32 ? warp_sums[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(kFull, all, o);
       if (lane >= o) all += up;
     }
-    const int below = warp == 0 ? 0 : __shfl_sync(kFull, all, warp - 1);
-    const int block_total = __shfl_sync(kFull, all, 31);
-    scan += carry + below;
-    if (e < p.experts) {
+    const int below = __shfl_sync(kFull, all, (warp + 31) & 31), block_total = __shfl_sync(kFull, all, 31);
+    scan += carry + (warp == 0 ? 0 : below);
+    if (share == 0 && e < p.experts) {
       start[e] = scan - total + before;
       if (blockIdx.x == 0) p.ends[e] = scan;
     }
@@ -385,11 +456,11 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
       float logit[N];
       Row row;
       load_row<DT, N>(p, token, lane, logit, row);
-      bool near;
-      chosen = choose<float, N>(p, logit, row, lane, near);
-      if (near) chosen = choose_in_64_bits<N>(p, logit, row, lane);
-      const float total = p.scoring == kSoftmax && p.renormalize == 0 ? total_of<N>(p, logit, row, lane) : 1.0f;
-      const float mine = chosen >= 0 ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
+      const Choice c = choose<float, N>(p, logit, row, lane);
+      chosen = c.near ? choose_in_64_bits<N>(p, logit, row, lane) : c.expert;
+      const float total = p.scoring == kSoftmax && p.renormalize == 0 ? total_of<N>(logit, row) : 1.0f;
+      float mine = c.logit;
+      if (chosen >= 0 && (p.bias != nullptr || c.near)) mine = value_at<DT>(p.logits, token * p.stride + chosen);
       const Share s = share_of(p.scoring, p.renormalize != 0, mine, chosen >= 0, row, total);
       weight = chosen >= 0 ? __fdiv_rn(s.score, s.sum) * p.scale : 0.0f;
     }
@@ -401,7 +472,7 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
   }
   __syncthreads();
   if constexpr (kOne) {
-    place(p, shared + p.experts, [&](int, int e) { return shared[e]; });
+    place(p, shared + p.experts, shared + 2 * p.experts + 32, [&](int, int e) { return shared[e]; });
   } else {
     for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = shared[e];
   }
@@ -410,7 +481,7 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
 __global__ void __launch_bounds__(1024) place_kernel(const __grid_constant__ RouteArgs p) {
   extern __shared__ int32_t shared[];
   fp4::grid_wait();
-  place(p, shared, [&](int c, int e) { return p.counts[static_cast<int64_t>(c) * p.experts + e]; });
+  place(p, shared, shared + p.experts + 32, [&](int c, int e) { return p.counts[static_cast<int64_t>(c) * p.experts + e]; });
 }
 
 // --------------------------------------------------------------------------- backward
@@ -446,7 +517,7 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const __grid_constant__
   float total = 1.0f;
   if (whole) {
     load_row<DT, N>(p, token, lane, logit, row);
-    if (p.renormalize == 0) total = total_of<N>(p, logit, row, lane);
+    if (p.renormalize == 0) total = total_of<N>(logit, row);
   }
   const float mine = has ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
   const Share s = share_of(p.scoring, p.renormalize != 0, mine, has, row, total);
@@ -462,11 +533,20 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const __grid_constant__
   }
   const bool others = whole && p.renormalize == 0;
   const int64_t at = token * p.experts;
+  if (others) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = i * 32 + lane;
-    if (e < p.experts)
-      store_at<DT>(a.dlogits, at + e, others ? (row.broken ? NAN : -__fdiv_rn(expf(logit[i] - row.top), total) * mean) : 0.0f);
+    for (int i = 0; i < N; ++i)
+      if (lane * N + i < p.experts)
+        store_at<DT>(a.dlogits, at + lane * N + i, row.broken ? NAN : -__fdiv_rn(expf(logit[i] - row.top), total) * mean);
+  } else {
+    // zeros, in words where rows start on them
+    constexpr int kEach = DT == kF32 ? 1 : 2;
+    if ((p.experts % kEach) == 0 && (reinterpret_cast<uintptr_t>(a.dlogits) & 3) == 0) {
+      uint32_t* words = static_cast<uint32_t*>(a.dlogits) + at / kEach;
+      for (int i = lane; i < p.experts / kEach; i += 32) words[i] = 0u;
+    } else {
+      for (int e = lane; e < p.experts; e += 32) store_at<DT>(a.dlogits, at + e, 0.0f);
+    }
   }
   __syncwarp();
   if (has) store_at<DT>(a.dlogits, at + chosen, d);
