@@ -36,7 +36,7 @@ typedef struct piper_routing_config {
   float scale;
 } piper_routing_config;
 
-/* Scratch bytes of piper_routing_route (0: none). */
+/* Scratch bytes of piper_routing_route (0: none), 16-byte aligned. */
 int piper_routing_workspace(const piper_routing_config* c, size_t* bytes);
 
 /* logits (tokens, experts), rows `stride` values apart. `bias`: fp32

@@ -139,6 +139,20 @@ RowPlan plan_rows(int64_t rows, int64_t units, int most) {
   return {8, units <= 512 ? 2 : 4, rows};
 }
 
+// Rows that start on 16-byte boundaries and have whole units.
+bool whole_units(const void* p, int64_t stride, int64_t rows, int64_t cols, int dtype) {
+  return aligned(p, 16) && cols % i8::kUnit == 0 && (rows == 1 || (stride * static_cast<int64_t>(width(dtype))) % 16 == 0);
+}
+
+template <class Args, class Kernel>
+void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, unsigned row_blocks,
+                 Kernel warp_short, Kernel warp_long, Kernel block_short, Kernel block_long, Kernel warp_any, Kernel block_any) {
+  const Kernel kernel = !vec             ? (rows.warps == 1 ? warp_any : block_any)
+                        : rows.warps == 1 ? (rows.hold == 2 ? warp_short : warp_long)
+                                          : (rows.hold == 2 ? block_short : block_long);
+  kernel<<<grid, i8::kPrepareThreads, 0, s>>>(args, r, row_blocks);
+}
+
 // ---------------------------------------------------------------- the product
 struct TilePlan {
   int bn, split;
@@ -327,7 +341,6 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   q.x_stride = x_stride;
   q.tokens = tokens;
   q.cols = static_cast<int32_t>(w->cols);
-  q.vec = aligned(x, 16) && (x_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
   q.pitch = p.x_pitch;
   q.codes = reinterpret_cast<int8_t*>(ws + p.x_codes);
   q.scale = reinterpret_cast<float*>(ws + p.x_scale);
@@ -358,11 +371,11 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
     return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
 
   const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
-#define CALL(D)                                                                                                                     \
-  if (rows.warps == 1 && rows.hold == 2) i8::quantize_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid);        \
-  else if (rows.warps == 1) i8::quantize_kernel<D, 1, D == i8::kF32 ? 4 : 8><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid); \
-  else if (rows.hold == 2) i8::quantize_kernel<D, 8, 2><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid);                      \
-  else i8::quantize_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(q, r, tokens_grid)
+  const bool vec = whole_units(x, x_stride, tokens, w->cols, dtype);
+#define CALL(D)                                                                                                            \
+  launch_rows(grid, s, rows, vec, q, r, tokens_grid, i8::quantize_kernel<D, 1, 2, true>, i8::quantize_kernel<D, 1, D == i8::kF32 ? 4 : 8, true>, \
+              i8::quantize_kernel<D, 8, 2, true>, i8::quantize_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>,                    \
+              i8::quantize_kernel<D, 1, 2, false>, i8::quantize_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   cudaError_t e = launched();
@@ -403,7 +416,6 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   v.dy_stride = dy_stride;
   v.tokens = tokens;
   v.rows = static_cast<int32_t>(w->rows);
-  v.vec = aligned(dy, 16) && (dy_stride * static_cast<int64_t>(width(dtype))) % 16 == 0;
   v.pitch = p.pitch;
   v.out = reinterpret_cast<__half*>(ws + p.values);
   v.back = reinterpret_cast<float*>(ws + p.back);
@@ -433,11 +445,11 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
     return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
 
   const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
+  const bool vec = whole_units(dy, dy_stride, tokens, w->rows, dtype) && aligned(w->scale, 16);
 #define CALL(D)                                                                                                            \
-  if (rows.warps == 1 && rows.hold == 2) i8::scale_kernel<D, 1, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid); \
-  else if (rows.warps == 1) i8::scale_kernel<D, 1, 4><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid);               \
-  else if (rows.hold == 2) i8::scale_kernel<D, 8, 2><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid);                \
-  else i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4><<<grid, i8::kPrepareThreads, 0, s>>>(v, r, tokens_grid)
+  launch_rows(grid, s, rows, vec, v, r, tokens_grid, i8::scale_kernel<D, 1, 2, true>, i8::scale_kernel<D, 1, 4, true>,       \
+              i8::scale_kernel<D, 8, 2, true>, i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>,                          \
+              i8::scale_kernel<D, 1, 2, false>, i8::scale_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   cudaError_t e = launched();

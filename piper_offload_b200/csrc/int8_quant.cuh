@@ -35,12 +35,13 @@ __device__ __forceinline__ float unit_value(const Unit<DT>& u, int i) {
   return i & 1 ? __high2float(h) : __low2float(h);
 }
 
-// Values [col, col + 16) of the row at `row`; those from `cols` on are zero. `vec`: rows start on 16-byte boundaries.
-template <int DT>
-__device__ __forceinline__ Unit<DT> load_unit(const void* row, int col, int cols, bool vec) {
+// Values [col, col + 16) of the row at `row`; those from `cols` on are zero. kVec: rows start on 16-byte boundaries and have
+// whole units, so that a row's loads are all in flight together; with a second form of load beside it they are not.
+template <int DT, bool kVec>
+__device__ __forceinline__ Unit<DT> load_unit(const void* row, int col, int cols) {
   constexpr int kWords = DT == kF32 ? 16 : 8;
   Unit<DT> u;
-  if (vec && col + kUnit <= cols) {
+  if constexpr (kVec) {
     const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + static_cast<int64_t>(col) * (DT == kF32 ? 4 : 2));
 #pragma unroll
     for (int i = 0; i < kWords / 4; ++i) {
@@ -147,7 +148,6 @@ struct QuantArgs {
   int64_t x_stride;
   int64_t tokens;
   int32_t cols;
-  int32_t vec;     // rows of x start on 16-byte boundaries
   int64_t pitch;   // bytes between rows of codes, a multiple of 16
   int8_t* codes;
   float* scale;    // (tokens)
@@ -214,7 +214,7 @@ __device__ __forceinline__ int store_codes(const Unit<DT>& u, const Quotient& q,
 }
 
 // One or eight rows. Codes behind the last column are zero up to the pitch.
-template <int DT, int kWarps, int kHold>
+template <int DT, int kWarps, int kHold, bool kVec>
 __device__ __forceinline__ void quantize_rows(const QuantArgs& p, int64_t block, uint32_t* words) {
   const RowTeam<kWarps> team(block);
   if (kWarps == 1 && team.row >= p.tokens) return;
@@ -225,11 +225,11 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& p, int64_t block,
   uint32_t top = 0u;
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) {
-      held[k] = load_unit<DT>(row, (team.thread + k * kStep) * kUnit, p.cols, p.vec != 0);
-      top = max(top, unit_top<DT>(held[k]));
-    }
-  for (int u = team.thread + kHold * kStep; u < units; u += kStep) top = max(top, unit_top<DT>(load_unit<DT>(row, u * kUnit, p.cols, p.vec != 0)));
+    if (team.thread + k * kStep < units) held[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.cols);
+#pragma unroll
+  for (int k = 0; k < kHold; ++k)
+    if (team.thread + k * kStep < units) top = max(top, unit_top<DT>(held[k]));
+  for (int u = team.thread + kHold * kStep; u < units; u += kStep) top = max(top, unit_top<DT>(load_unit<DT, kVec>(row, u * kUnit, p.cols)));
   const Quotient q = quotient_of(team.max_of(top, words));
   int8_t* to = p.codes + team.row * p.pitch;
   int sum = 0;
@@ -237,7 +237,7 @@ __device__ __forceinline__ void quantize_rows(const QuantArgs& p, int64_t block,
   for (int k = 0; k < kHold; ++k)
     if (team.thread + k * kStep < units) sum += store_codes<DT>(held[k], q, to + (team.thread + k * kStep) * kUnit);
   for (int u = team.thread + kHold * kStep; u < units; u += kStep)
-    sum += store_codes<DT>(load_unit<DT>(row, u * kUnit, p.cols, p.vec != 0), q, to + u * kUnit);
+    sum += store_codes<DT>(load_unit<DT, kVec>(row, u * kUnit, p.cols), q, to + u * kUnit);
   if (p.sums != nullptr) sum = team.sum_of(sum, words);
   if (team.thread == 0) {
     p.scale[team.row] = q.scale;
@@ -255,7 +255,6 @@ struct ScaleArgs {
   int64_t dy_stride;
   int64_t tokens;
   int32_t rows;    // of one weight: values in a row of dy
-  int32_t vec;     // rows of dy start on 16-byte boundaries
   int64_t pitch;   // values between rows of out, a multiple of 16
   __half* out;     // (terms, tokens, pitch)
   float* back;     // (tokens): what a row's sums are multiplied by
@@ -265,14 +264,15 @@ struct ScaleArgs {
 };
 
 // The scales of sixteen rows of the weight from `n` on, 0 past the last. A lane takes them as it takes its values.
-template <int DT>
+template <int DT, bool kVec>
 __device__ __forceinline__ void unit_scales(const void* scale, int64_t row0, int n, int rows, float (&s)[kUnit]) {
   const uint8_t* from = static_cast<const uint8_t*>(scale) + row0 * (DT == kF32 ? 4 : 2);
-  const Unit<DT> u = load_unit<DT>(from, n, rows, (reinterpret_cast<uintptr_t>(from) & 15) == 0);
+  const Unit<DT> u = load_unit<DT, kVec>(from, n, rows);
 #pragma unroll
   for (int i = 0; i < kUnit; ++i) s[i] = unit_value<DT>(u, i);
 }
 
+template <bool kVec>
 __device__ __forceinline__ void scales_of(const ScaleArgs& p, int64_t row0, int n, float (&s)[kUnit]) {
   if (p.scales.step == 0) {
     const float one = row_scale(p.scales, 0);
@@ -280,16 +280,16 @@ __device__ __forceinline__ void scales_of(const ScaleArgs& p, int64_t row0, int 
     for (int i = 0; i < kUnit; ++i) s[i] = n + i < p.rows ? one : 0.0f;
     return;
   }
-  if (p.scales.dtype == kBF16) unit_scales<kBF16>(p.scales.scale, row0, n, p.rows, s);
-  else if (p.scales.dtype == kF16) unit_scales<kF16>(p.scales.scale, row0, n, p.rows, s);
-  else unit_scales<kF32>(p.scales.scale, row0, n, p.rows, s);
+  if (p.scales.dtype == kBF16) unit_scales<kBF16, kVec>(p.scales.scale, row0, n, p.rows, s);
+  else if (p.scales.dtype == kF16) unit_scales<kF16, kVec>(p.scales.scale, row0, n, p.rows, s);
+  else unit_scales<kF32, kVec>(p.scales.scale, row0, n, p.rows, s);
   if (p.scales.over_127 != 0) {
 #pragma unroll
     for (int i = 0; i < kUnit; ++i) s[i] = __fdiv_rn(s[i], 127.0f);
   }
 }
 
-template <int DT, int kWarps, int kHold>
+template <int DT, int kWarps, int kHold, bool kVec>
 __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, uint32_t* words) {
   const RowTeam<kWarps> team(block);
   if (kWarps == 1 && team.row >= p.tokens) return;
@@ -303,7 +303,7 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   float top = 0.0f;
   const auto see = [&](const Unit<DT>& u, int unit, bool finite) {
     float s[kUnit];
-    scales_of(p, row0, unit * kUnit, s);
+    scales_of<kVec>(p, row0, unit * kUnit, s);
 #pragma unroll
     for (int i = 0; i < kUnit; ++i) {
       const float v = fabsf(unit_value<DT>(u, i) * s[i]);
@@ -312,12 +312,12 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   };
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) held[k] = load_unit<DT>(row, (team.thread + k * kStep) * kUnit, p.rows, p.vec != 0);
+    if (team.thread + k * kStep < units) held[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
   const auto see_all = [&](bool finite) {
 #pragma unroll
     for (int k = 0; k < kHold; ++k)
       if (team.thread + k * kStep < units) see(held[k], team.thread + k * kStep, finite);
-    for (int u = team.thread + kHold * kStep; u < units; u += kStep) see(load_unit<DT>(row, u * kUnit, p.rows, p.vec != 0), u, finite);
+    for (int u = team.thread + kHold * kStep; u < units; u += kStep) see(load_unit<DT, kVec>(row, u * kUnit, p.rows), u, finite);
   };
   see_all(false);
   uint32_t bits = team.max_of(__float_as_uint(top), words);
@@ -332,7 +332,7 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   const float power = __uint_as_float(static_cast<uint32_t>(141 - exponent) << 23);
   const auto write = [&](const Unit<DT>& u, int unit) {
     float s[kUnit];
-    scales_of(p, row0, unit * kUnit, s);
+    scales_of<kVec>(p, row0, unit * kUnit, s);
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
@@ -357,7 +357,7 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
     if (team.thread + k * kStep < units) write(held[k], team.thread + k * kStep);
-  for (int u = team.thread + kHold * kStep; u < units; u += kStep) write(load_unit<DT>(row, u * kUnit, p.rows, p.vec != 0), u);
+  for (int u = team.thread + kHold * kStep; u < units; u += kStep) write(load_unit<DT, kVec>(row, u * kUnit, p.rows), u);
   if (team.thread == 0) p.back[team.row] = __uint_as_float(static_cast<uint32_t>(113 + exponent) << 23);
 }
 
@@ -393,22 +393,22 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t piece) {
 }
 
 // The launch before a product: blocks of token rows, then of codes.
-template <int DT, int kWarps, int kHold>
+template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(kPrepareThreads) quantize_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs r,
                                                                    uint32_t token_blocks) {
   __shared__ uint32_t words[16];
   fp4::grid_launch_dependents();
-  if (blockIdx.x < token_blocks) quantize_rows<DT, kWarps, kHold>(q, blockIdx.x, words);
+  if (blockIdx.x < token_blocks) quantize_rows<DT, kWarps, kHold, kVec>(q, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * kPrepareThreads + threadIdx.x);
 }
 
 // The launch before a gradient.
-template <int DT, int kWarps, int kHold>
+template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(kPrepareThreads) scale_kernel(const __grid_constant__ ScaleArgs s, const __grid_constant__ RepackArgs r,
                                                                 uint32_t token_blocks) {
   __shared__ uint32_t words[16];
   fp4::grid_launch_dependents();
-  if (blockIdx.x < token_blocks) scale_rows<DT, kWarps, kHold>(s, blockIdx.x, words);
+  if (blockIdx.x < token_blocks) scale_rows<DT, kWarps, kHold, kVec>(s, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * kPrepareThreads + threadIdx.x);
 }
 

@@ -91,10 +91,15 @@ Chunks chunks_of(const piper_routing_config& c) {
   return {static_cast<int>((c.tokens + size - 1) / size), static_cast<int>(size)};
 }
 
+size_t counts_bytes(const piper_routing_config& c, const Chunks& n) {
+  return n.count > 1 ? static_cast<size_t>(n.count) * ((c.experts + 3) / 4 * 4) * 4 : 0;
+}
+
 routing::RouteArgs route_args(const piper_routing_config& c) {
   routing::RouteArgs a{};
   a.tokens = c.tokens;
   a.experts = c.experts;
+  a.pitch = (c.experts + 3) / 4 * 4;
   a.top_k = c.top_k;
   a.scoring = c.scoring;
   a.groups = c.groups;
@@ -112,21 +117,22 @@ routing::RouteArgs route_args(const piper_routing_config& c) {
     else { CALL(routing::kF32); }                                      \
   } while (0)
 
-// Whether a lane's N neighbouring logits lie in pieces that one load takes, each there or not as a whole.
-bool whole_pieces(const routing::RouteArgs& a, int n, size_t size) {
+// Whether a lane's N neighbouring values lie in pieces that one load takes, each there or not as a whole.
+bool whole_pieces(const void* p, int64_t stride, int experts, int n, size_t size) {
   const size_t bytes = std::min<size_t>(16, n * size);
-  return bytes >= 4 && aligned(a.logits, bytes) && (a.stride * static_cast<int64_t>(size)) % static_cast<int64_t>(bytes) == 0 &&
-         a.experts % static_cast<int>(bytes / size) == 0;
+  return bytes >= 4 && aligned(p, bytes) && (stride * static_cast<int64_t>(size)) % static_cast<int64_t>(bytes) == 0 &&
+         experts % static_cast<int>(bytes / size) == 0;
 }
 
 template <int DT, int N>
 cudaError_t launch_route(routing::RouteArgs a, int threads, cudaStream_t s) {
-  a.vec = whole_pieces(a, N, width(DT));
+  a.vec = whole_pieces(a.logits, a.stride, a.experts, N, width(DT));
+  a.bias_vec = whole_pieces(a.bias, 0, a.experts, N, 4);
   if (a.chunks == 1) {
-    routing::route_kernel<DT, N, true><<<1, threads, (2 * a.experts + 32 + 2 * threads) * 4, s>>>(a);
+    routing::route_kernel<DT, N, true><<<1, threads, (2 * a.pitch + 32 + 8 * threads) * 4, s>>>(a);
     return launched();
   }
-  routing::route_kernel<DT, N, false><<<static_cast<unsigned>(a.chunks), threads, a.experts * 4, s>>>(a);
+  routing::route_kernel<DT, N, false><<<static_cast<unsigned>(a.chunks), threads, a.pitch * 4, s>>>(a);
   return launched();
 }
 
@@ -143,7 +149,7 @@ cudaError_t launch_route(const routing::RouteArgs& a, cudaStream_t s) {
 
 template <int DT, int N>
 cudaError_t launch_route_grad(routing::RouteGradArgs a, cudaStream_t s) {
-  a.route.vec = whole_pieces(a.route, N, width(DT));
+  a.route.vec = whole_pieces(a.route.logits, a.route.stride, a.route.experts, N, width(DT));
   routing::route_grad_kernel<DT, N><<<static_cast<unsigned>((a.route.tokens + 7) / 8), 256, 0, s>>>(a);
   return launched();
 }
@@ -210,7 +216,7 @@ int piper_routing_workspace(const piper_routing_config* c, size_t* bytes) {
   if (int rc = check_config(c)) return rc;
   ROUTING_REQUIRE(bytes != nullptr, "Routing: bad workspace query.");
   const Chunks n = chunks_of(*c);
-  *bytes = n.count > 1 ? static_cast<size_t>(n.count) * c->experts * 4 : 0;
+  *bytes = counts_bytes(*c, n);
   return PIPER_ROUTING_OK;
 }
 
@@ -230,8 +236,8 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
   ROUTING_REQUIRE(aligned(logits, width(dtype)), "Routing: logits not aligned to their type.");
   ROUTING_REQUIRE(stride >= c->experts || c->tokens == 1, "Routing: rows of the logits overlap.");
   const Chunks n = chunks_of(*c);
-  const size_t need = n.count > 1 ? static_cast<size_t>(n.count) * c->experts * 4 : 0;
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 4)))
+  const size_t need = counts_bytes(*c, n);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(PIPER_ROUTING_EWORKSPACE, "Routing: workspace missing, too small or not aligned.");
   routing::RouteArgs a = route_args(*c);
   a.logits = logits;
@@ -259,7 +265,7 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(n.count));
   config.blockDim = dim3(1024);
-  config.dynamicSmemBytes = (a.experts + 32 + 2 * 1024) * 4;
+  config.dynamicSmemBytes = (a.pitch + 32 + 8 * 1024) * 4;
   config.stream = s;
   config.attrs = &attribute;
   config.numAttrs = 1;

@@ -38,13 +38,14 @@ struct RouteArgs {
   int32_t* ends;
   int32_t* rows;
   int32_t* source;
-  int32_t* counts;  // (chunks, experts)
+  int32_t* counts;  // (chunks, pitch)
   int64_t tokens;
   int32_t chunk;    // tokens of a block
   int32_t chunks;
   int32_t experts, top_k;
+  int32_t pitch;    // experts up to a multiple of four
   int32_t scoring, groups, top_groups, group_score, renormalize;
-  int32_t vec;      // a lane's logits may be read in pieces of 16 bytes, or of all its bytes
+  int32_t vec, bias_vec;  // a lane's logits, or biases, may be read in pieces of 16 bytes, or of all its bytes
   float scale;
 };
 
@@ -53,6 +54,41 @@ __device__ __forceinline__ float value_at(const void* p, int64_t at) {
   if constexpr (DT == kBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
   else if constexpr (DT == kF16) return __half2float(static_cast<const __half*>(p)[at]);
   else return static_cast<const float*>(p)[at];
+}
+
+// A lane's N neighbouring values of a row, from value `at` on; -infinity past the last.
+template <int DT, int N>
+__device__ __forceinline__ void load_values(const void* from, int64_t at, int count, bool vec, float (&v)[N]) {
+  constexpr int kSize = DT == kF32 ? 4 : 2, kBytes = N * kSize < 16 ? N * kSize : 16, kEach = kBytes / kSize;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = -INFINITY;
+  if (vec && kBytes >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += kEach) {
+      if (i >= count) continue;  // a piece is there or not as a whole
+      uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
+      const uint8_t* q = static_cast<const uint8_t*>(from) + (at + i) * kSize;
+      if constexpr (kBytes == 16) {
+        const uint4 r = *reinterpret_cast<const uint4*>(q);
+        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+      } else if constexpr (kBytes == 8) {
+        const uint2 r = *reinterpret_cast<const uint2*>(q);
+        w[0] = r.x; w[1] = r.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(q);
+      }
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        if constexpr (DT == kF32) v[i + k] = __uint_as_float(w[k]);
+        else if constexpr (DT == kBF16) v[i + k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
+        else v[i + k] = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1)))));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < count) v[i] = value_at<DT>(from, at + i);
+  }
 }
 
 // ------------------------------------------------------------------ numbers that order as values do
@@ -121,7 +157,7 @@ constexpr float kMargin = 0x1p-17f, kMarginOfValue = 0x1p-21f;
 
 // Whether a value is so near one below it that fp32 may have put them in the wrong order. False for what is closed.
 __device__ __forceinline__ bool near_by(uint32_t upper, uint32_t lower) {
-  if (lower == 0u) return false;
+  if (upper == 0u || lower == 0u) return false;
   const float a = Order<float>::value(upper), b = Order<float>::value(lower);
   return !(a - b > kMargin + kMarginOfValue * fmaxf(fabsf(a), fabsf(b)));
 }
@@ -173,12 +209,18 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
 #pragma unroll
       for (int i = 0; i < N; ++i) score[i] = row.broken ? static_cast<T>(NAN) : quotient(score[i], sum);
     }
+    if (p.bias != nullptr) {
+      float bias[N];
+      load_values<kF32, N>(p.bias, e0, p.experts - e0, p.bias_vec != 0, bias);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float bias = p.bias != nullptr && e0 + i < p.experts ? p.bias[e0 + i] : 0.0f;
-      const bool open = logit[i] != -INFINITY && bias != -INFINITY;
-      part[i] = open ? O::of(score[i] + static_cast<T>(bias)) : 0;
-      choice[i] = p.bias != nullptr ? part[i] : open ? O::of(static_cast<T>(logit[i])) : 0;
+      for (int i = 0; i < N; ++i)
+        part[i] = choice[i] = logit[i] != -INFINITY && bias[i] != -INFINITY ? O::of(score[i] + static_cast<T>(bias[i])) : 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        part[i] = logit[i] != -INFINITY ? O::of(score[i]) : 0;
+        choice[i] = logit[i] != -INFINITY ? O::of(static_cast<T>(logit[i])) : 0;
+      }
     }
   } else {
 #pragma unroll
@@ -187,7 +229,7 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
 
   if (p.groups > 1) {
     const int per = p.experts / p.groups, span = per / N;
-    Key mine = 0;  // of the group that this lane's experts are in; else of group `lane`
+    Key own = 0;  // of the group that this lane's experts are in; else of group `lane`
     const bool whole = span * N == per && (span & (span - 1)) == 0;
     if (whole) {
       Key best = 0, second = 0;
@@ -198,7 +240,7 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
         take(best, second, b);
         take(best, second, s);
       }
-      mine = group_key<T>(p.group_score, best, second);
+      own = group_key<T>(p.group_score, best, second);
     } else {
       for (int g = 0; g < p.groups; ++g) {
         Key best = 0, second = 0;
@@ -211,19 +253,19 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
           take(best, second, b);
           take(best, second, s);
         }
-        if (lane == g) mine = group_key<T>(p.group_score, best, second);
+        if (lane == g) own = group_key<T>(p.group_score, best, second);
       }
     }
     const int group = whole ? lane / span : lane;
     int before = 0;  // groups that come before this lane's
     for (int g = 0; g < p.groups; ++g) {
-      const Key other = O::from(mine, whole ? g * span : g);
-      before += other > mine || (other == mine && g < group);
+      const Key other = O::from(own, whole ? g * span : g);
+      before += other > own || (other == own && g < group);
     }
     const bool kept = group < p.groups && before < p.top_groups;
     if (kCheck && by_score && p.top_groups < p.groups) {
-      const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(mine) : 0xFFFFFFFFu);
-      const uint32_t highest = __reduce_max_sync(kFull, kept || group >= p.groups ? 0u : static_cast<uint32_t>(mine));
+      const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(own) : 0xFFFFFFFFu);
+      const uint32_t highest = __reduce_max_sync(kFull, kept || group >= p.groups ? 0u : static_cast<uint32_t>(own));
       out.near |= near_by(lowest, highest);
     }
     const uint32_t groups_kept = __ballot_sync(kFull, kept);
@@ -232,27 +274,66 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
       if (whole ? !kept : e0 + i < p.experts && !(groups_kept >> ((e0 + i) / per) & 1u)) choice[i] = 0;
   }
 
-  Key last = 0;
-  const int rounds = p.top_k + (kCheck && p.bias != nullptr);  // one more to see how near the next one is
-  for (int j = 0; j < rounds; ++j) {
-    Key best = choice[0];
+  // A lane's largest come first, equal ones by index (neighbours change places only where the second is larger), so that
+  // its next one is always in choice[0]; for more experts a lane sorting costs more than looking for the largest each time.
+  constexpr bool kSorted = N <= 8;
+  int at[N];
 #pragma unroll
-    for (int i = 1; i < N; ++i) best = choice[i] > best ? choice[i] : best;
+  for (int i = 0; i < N; ++i) at[i] = e0 + i;
+  if constexpr (kSorted) {
+#pragma unroll
+    for (int pass = 0; pass < N; ++pass)
+#pragma unroll
+      for (int i = pass & 1; i + 1 < N; i += 2) {
+        const bool swap = choice[i + 1] > choice[i];
+        const Key k = choice[i];
+        const int e = at[i];
+        choice[i] = swap ? choice[i + 1] : choice[i];
+        at[i] = swap ? at[i + 1] : at[i];
+        choice[i + 1] = swap ? k : choice[i + 1];
+        at[i + 1] = swap ? e : at[i + 1];
+      }
+  }
+  Key mine = 0;  // of this lane's choice
+  Key next = 0;  // the largest that was not chosen
+  for (int j = 0;; ++j) {
+    Key best = choice[0];
+    int place = at[0];
+    if constexpr (!kSorted) {
+#pragma unroll
+      for (int i = 1; i < N; ++i) {
+        place = choice[i] > best ? e0 + i : place;
+        best = choice[i] > best ? choice[i] : best;
+      }
+    }
     const Key top = O::max_of(best);
-    if (kCheck && p.bias != nullptr && j > 0) out.near |= near_by(static_cast<uint32_t>(last), static_cast<uint32_t>(top));
-    last = top;
+    if (j == p.top_k) next = top;
     if (top == 0 || j == p.top_k) break;
     const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
-    int at = 0;  // the first of this lane's that is as large
-#pragma unroll
-    for (int i = N - 1; i >= 0; --i) at = choice[i] == top ? i : at;
-    const int expert = __shfl_sync(kFull, e0 + at, owner);
+    const int expert = __shfl_sync(kFull, place, owner);
     if (lane == j) {
       out.expert = expert;
-      if (p.bias == nullptr) out.logit = static_cast<float>(O::value(top));
+      mine = top;
     }
+    if (j + 1 == p.top_k && !(kCheck && p.bias != nullptr)) break;  // one more round to see how near the next one is
+    if constexpr (kSorted) {
+      if (lane == owner) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) choice[i] = lane == owner && i == at ? 0 : choice[i];
+        for (int i = 0; i + 1 < N; ++i) {
+          choice[i] = choice[i + 1];
+          at[i] = at[i + 1];
+        }
+        choice[N - 1] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) choice[i] = e0 + i == expert ? 0 : choice[i];
+    }
+  }
+  if (p.bias == nullptr && out.expert >= 0) out.logit = static_cast<float>(O::value(mine));
+  if (kCheck && p.bias != nullptr) {
+    const Key below = __shfl_down_sync(kFull, mine, 1);
+    out.near |= __any_sync(kFull, near_by(static_cast<uint32_t>(mine), static_cast<uint32_t>(lane + 1 == p.top_k ? next : lane == 31 ? 0 : below)));
   }
   return out;
 }
@@ -300,41 +381,6 @@ __device__ __forceinline__ Share share_of(int scoring, bool renormalize, float l
   return s;
 }
 
-// A lane's N neighbouring values of a row, from value `at` on; -infinity past the last.
-template <int DT, int N>
-__device__ __forceinline__ void load_values(const void* from, int64_t at, int count, bool vec, float (&v)[N]) {
-  constexpr int kSize = DT == kF32 ? 4 : 2, kBytes = N * kSize < 16 ? N * kSize : 16, kEach = kBytes / kSize;
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = -INFINITY;
-  if (vec && kBytes >= 4) {
-#pragma unroll
-    for (int i = 0; i < N; i += kEach) {
-      if (i >= count) continue;  // a piece is there or not as a whole
-      uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
-      const uint8_t* q = static_cast<const uint8_t*>(from) + (at + i) * kSize;
-      if constexpr (kBytes == 16) {
-        const uint4 r = *reinterpret_cast<const uint4*>(q);
-        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-      } else if constexpr (kBytes == 8) {
-        const uint2 r = *reinterpret_cast<const uint2*>(q);
-        w[0] = r.x; w[1] = r.y;
-      } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(q);
-      }
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        if constexpr (DT == kF32) v[i + k] = __uint_as_float(w[k]);
-        else if constexpr (DT == kBF16) v[i + k] = __uint_as_float(k & 1 ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
-        else v[i + k] = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1)))));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < count) v[i] = value_at<DT>(from, at + i);
-  }
-}
-
 template <int DT, int N>
 __device__ __forceinline__ void load_row(const RouteArgs& p, int64_t token, int lane, float (&logit)[N], Row& row) {
   load_values<DT, N>(p.logits, token * p.stride + lane * N, p.experts - lane * N, p.vec != 0, logit);
@@ -360,40 +406,47 @@ __device__ __forceinline__ float total_of(const float (&logit)[N], const Row& ro
 }
 
 // --------------------------------------------------------------------- the order by expert
-// The places of a block's choices, in the order of experts and within one of tokens. `count(chunk, e)` are the choices of
-// each chunk of tokens. start: shared, (experts + 32) words; parts: 2 words a thread.
-template <class Count>
-__device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, int32_t* parts, const Count& count) {
+// The places of a block's choices, in the order of experts and within one of tokens. counts: choices of each chunk of
+// tokens (chunks, pitch), 16-byte aligned, zeros behind the last expert. Shared: start (pitch + 32) words, parts 8 words a
+// thread. A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
+__device__ __forceinline__ void place(const RouteArgs& p, const int32_t* counts, int32_t* start, int32_t* parts) {
   const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int32_t* warp_sums = start + p.experts;
-  // experts are taken `wide` at a time, and several threads share the chunks of one
-  const int wide = p.experts >= threads ? threads : p.experts <= 32 ? 32 : 1 << (32 - __clz(p.experts - 1));
-  const int shares = threads / wide, share = threadIdx.x / wide, in = threadIdx.x % wide;
-  // this chunk's first place within each expert, and the experts' totals, scanned
-  int carry = 0;
-  for (int e0 = 0; e0 < p.experts; e0 += wide) {
-    const int e = e0 + in;
-    int before = 0, total = 0;
-    if (e < p.experts) {
-#pragma unroll 8
-      for (int c = share; c < p.chunks; c += shares) {
-        const int n = count(c, e);
-        total += n;
-        before += c < static_cast<int>(blockIdx.x) ? n : 0;
+  const int quads = p.pitch >> 2, wide = min(threads, quads <= 32 ? 32 : 1 << (32 - __clz(quads - 1)));
+  const int shares = threads / wide, share = threadIdx.x / wide, quad = threadIdx.x % wide;
+  int4 total = make_int4(0, 0, 0, 0), before = total;
+  if (quad < quads) {
+    const int4* from = reinterpret_cast<const int4*>(counts) + quad;
+    for (int c0 = share; c0 < p.chunks; c0 += 8 * shares) {
+      int4 n[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = c0 + k * shares;
+        n[k] = c < p.chunks ? from[static_cast<int64_t>(c) * quads] : make_int4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int has = c0 + k * shares < static_cast<int>(blockIdx.x) ? -1 : 0;
+        total.x += n[k].x; total.y += n[k].y; total.z += n[k].z; total.w += n[k].w;
+        before.x += n[k].x & has; before.y += n[k].y & has; before.z += n[k].z & has; before.w += n[k].w & has;
       }
     }
-    if (shares > 1) {
-      parts[threadIdx.x] = total;
-      parts[threads + threadIdx.x] = before;
-      __syncthreads();
-      total = before = 0;
-      if (share == 0)
-        for (int k = 0; k < shares; ++k) {
-          total += parts[k * wide + in];
-          before += parts[threads + k * wide + in];
-        }
-    }
-    int scan = total;
+  }
+  int4* totals = reinterpret_cast<int4*>(parts);
+  totals[threadIdx.x] = total;
+  totals[threads + threadIdx.x] = before;
+  __syncthreads();
+  // this chunk's first place within each expert: the experts' totals, scanned (wide * 4 of them, at most threads * 4)
+  int32_t* warp_sums = start + p.pitch;
+  int carry = 0;
+  for (int e0 = 0; e0 < p.experts; e0 += threads) {
+    const int e = e0 + threadIdx.x;
+    int all = 0, mine = 0;
+    if (e < p.experts)
+      for (int k = 0; k < shares; ++k) {
+        all += parts[k * wide * 4 + e];
+        mine += parts[threads * 4 + k * wide * 4 + e];
+      }
+    int scan = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(kFull, scan, o);
@@ -401,16 +454,16 @@ __device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, int32_
     }
     if (lane == 31) warp_sums[warp] = scan;
     __syncthreads();
-    int all = lane < wide / 32 ? warp_sums[lane] : 0;
+    int sums = lane < threads / 32 ? warp_sums[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(kFull, all, o);
-      if (lane >= o) all += up;
+      const int up = __shfl_up_sync(kFull, sums, o);
+      if (lane >= o) sums += up;
     }
-    const int below = __shfl_sync(kFull, all, (warp + 31) & 31), block_total = __shfl_sync(kFull, all, 31);
+    const int below = __shfl_sync(kFull, sums, (warp + 31) & 31), block_total = __shfl_sync(kFull, sums, 31);
     scan += carry + (warp == 0 ? 0 : below);
-    if (share == 0 && e < p.experts) {
-      start[e] = scan - total + before;
+    if (e < p.experts) {
+      start[e] = scan - all + mine;
       if (blockIdx.x == 0) p.ends[e] = scan;
     }
     carry += block_total;
@@ -443,10 +496,10 @@ __device__ __forceinline__ void place(const RouteArgs& p, int32_t* start, int32_
 // A block has a chunk of tokens, its warps take them in turn. kOne: the one block of the call, which places its choices too.
 template <int DT, int N, bool kOne>
 __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __grid_constant__ RouteArgs p) {
-  extern __shared__ int32_t shared[];  // choices of each expert; kOne: and the starts
+  extern __shared__ __align__(16) int32_t shared[];  // choices of each expert; kOne: and the starts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   fp4::grid_launch_dependents();
-  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) shared[e] = 0;
+  for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) shared[e] = 0;
   __syncthreads();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk, end = min(first + p.chunk, p.tokens);
   for (int64_t token = first + warp; token < end; token += warps) {
@@ -472,16 +525,16 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
   }
   __syncthreads();
   if constexpr (kOne) {
-    place(p, shared + p.experts, shared + 2 * p.experts + 32, [&](int, int e) { return shared[e]; });
+    place(p, shared, shared + p.pitch, shared + 2 * p.pitch + 32);
   } else {
-    for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.experts + e] = shared[e];
+    for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + e] = shared[e];
   }
 }
 
 __global__ void __launch_bounds__(1024) place_kernel(const __grid_constant__ RouteArgs p) {
-  extern __shared__ int32_t shared[];
+  extern __shared__ __align__(16) int32_t shared[];
   fp4::grid_wait();
-  place(p, shared, shared + p.experts + 32, [&](int c, int e) { return p.counts[static_cast<int64_t>(c) * p.experts + e]; });
+  place(p, p.counts, shared, shared + p.pitch + 32);
 }
 
 // --------------------------------------------------------------------------- backward
