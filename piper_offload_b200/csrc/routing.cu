@@ -124,15 +124,23 @@ bool whole_pieces(const void* p, int64_t stride, int experts, int n, size_t size
          experts % static_cast<int>(bytes / size) == 0;
 }
 
+// Shared memory of placing choices: starts, and then in the same room sums of a thread's four experts or counts of each warp.
+size_t place_bytes(int pitch, int threads) {
+  return (pitch + 32 + std::max<size_t>(8 * threads, threads / 32 * static_cast<size_t>(pitch) / 2 + pitch)) * 4;
+}
+
 template <int DT, int N>
 cudaError_t launch_route(routing::RouteArgs a, int threads, cudaStream_t s) {
   a.vec = whole_pieces(a.logits, a.stride, a.experts, N, width(DT));
   a.bias_vec = whole_pieces(a.bias, 0, a.experts, N, 4);
-  if (a.chunks == 1) {
-    routing::route_kernel<DT, N, true><<<1, threads, (2 * a.pitch + 32 + 8 * threads) * 4, s>>>(a);
-    return launched();
-  }
-  routing::route_kernel<DT, N, false><<<static_cast<unsigned>(a.chunks), threads, a.pitch * 4, s>>>(a);
+  const int span = a.experts / a.groups / N;
+  a.quick = a.groups == 1 || (span > 0 && span * N * a.groups == a.experts && (span & (span - 1)) == 0);
+  const size_t lists = threads / 32 * sizeof(routing::Lists<N>), places = place_bytes(a.pitch, threads);
+  const auto kernel = a.chunks == 1 ? routing::route_kernel<DT, N, true> : routing::route_kernel<DT, N, false>;
+  const size_t smem = a.pitch * 4 + (a.chunks == 1 ? std::max(lists, places) : lists);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  kernel<<<static_cast<unsigned>(a.chunks), threads, smem, s>>>(a);
   return launched();
 }
 
@@ -265,7 +273,9 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(n.count));
   config.blockDim = dim3(1024);
-  config.dynamicSmemBytes = (a.pitch + 32 + 8 * 1024) * 4;
+  config.dynamicSmemBytes = place_bytes(a.pitch, 1024);
+  e = cudaFuncSetAttribute(routing::place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes));
+  if (e != cudaSuccess) return cuda_fail("place kernel", e);
   config.stream = s;
   config.attrs = &attribute;
   config.numAttrs = 1;

@@ -2,16 +2,23 @@
 //
 // A warp has a token and each lane N neighbouring experts. Choices are compared as whole numbers that order as the scores
 // do (0 for what is closed, 1 for a NaN): the largest is found by redux, its lane by a vote, so that ties go to the lowest
-// index. Where a group's experts fill a power of two of lanes, all groups' two best are found at once by shuffles.
+// index.
 //
-// Choice scores. Without a bias the logits themselves decide: both scores grow with them. With one, or where a group counts
-// by its two best, sums of scores decide, and sums that are near each other in fp32 may be in another order than the
-// numbers they stand for. So each gap that decides anything is held against a margin, and a token with a gap within it is
-// done again in 64 bits: 1 to 2 % of the tokens where 256 experts' scores are spread over [0, 1]. The margin of 2^-17 is
-// above twice the error of two scores added up, which are at most 1 (of sigmoids 2): the fast exponential is off by 2 steps
-// of 2^-23 and 1.2 more for each unit of its argument d, where d exp(-d) is below 0.37, the fast quotient by 2 steps, a
-// softmax's sum by a step of 2^-24 for each of at most 37 additions; together 2^-18.5 for softmax, 2^-20 for sigmoids.
-// 2^-21 of the sum is above twice its own rounding.
+// With up to eight experts a lane (choose_quickly) a key's last three bits give way to the expert's place in the lane, so
+// that a lane sorts its keys by 19 minima and maxima and keeps the list in shared memory; a round then is a redux, a vote
+// and one load by the lane whose largest is taken. Groups whose experts fill a power of two of lanes are compared all at
+// once by shuffles. What this leaves open is decided in 64 bits: between groups over all their experts, between the
+// experts next to each other over those alone, a lane each. Only what that cannot separate (more than 32 scores next to
+// each other) is done again as a whole, in choose(). Open are
+// - Choice scores. Without a bias the logits decide, since both scores grow with them. With one, or where a group counts by
+//   its two best, sums of scores do, and sums near each other in fp32 may be in another order than the numbers they stand
+//   for. Each gap that decides anything is held against 2^-16, which is above twice the error of two scores added up: they
+//   are at most 1 (of sigmoids 2), the fast exponential is off by 2 steps of 2^-23 and 1.2 more for each unit of its
+//   argument d, where d exp(-d) is below 0.37, the fast quotient by 2 steps, a softmax's sum by a step of 2^-24 for each of
+//   at most 37 additions, the cut of three bits by 8 steps of 2^-24 for the sum and of a quarter of that for a logit;
+//   together below 2^-17.5. 2^-19 of the sum is above twice its rounding and cut. 256 experts' scores spread over [0, 1]
+//   leave 1 % of the tokens open; all of such a token done again by one warp in 64 bits took 8 us, while its block waited.
+// - fp32 logits that are equal but for the last three bits (16-bit ones lose nothing).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,6 +52,7 @@ struct RouteArgs {
   int32_t experts, top_k;
   int32_t pitch;    // experts up to a multiple of four
   int32_t scoring, groups, top_groups, group_score, renormalize;
+  int32_t quick;    // choose_quickly() takes the groups
   int32_t vec, bias_vec;  // a lane's logits, or biases, may be read in pieces of 16 bytes, or of all its bytes
   float scale;
 };
@@ -153,7 +161,7 @@ struct Row {
 // Whether sums of scores decide anything, or the logits alone.
 __device__ __forceinline__ bool scores_decide(const RouteArgs& p) { return p.bias != nullptr || (p.groups > 1 && p.group_score == kTop2); }
 
-constexpr float kMargin = 0x1p-17f, kMarginOfValue = 0x1p-21f;
+constexpr float kMargin = 0x1p-16f, kMarginOfValue = 0x1p-19f;
 
 // Whether a value is so near one below it that fp32 may have put them in the wrong order. False for what is closed.
 __device__ __forceinline__ bool near_by(uint32_t upper, uint32_t lower) {
@@ -176,20 +184,14 @@ __device__ __forceinline__ void take(K& best, K& second, K k) {
   best = k > best ? k : best;
 }
 
-// What decides about a token: lane j's choice j and the logit behind it (NaN: not known), or -1. `near`: in fp32, whether
-// some order is not certain.
-struct Choice {
-  int expert;
-  float logit;
-  bool near;
-};
-
+// Lane j's expert of the token's choice j, or -1; for any number of experts and groups. `near`: in fp32, whether some order is
+// not certain.
 template <class T, int N>
-__device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
+__device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane, bool& near) {
   using O = Order<T>;
   using Key = typename O::Key;
   constexpr bool kCheck = sizeof(T) == 4;
-  Choice out{-1, NAN, false};
+  near = false;
   const bool by_score = scores_decide(p);
   const int e0 = lane * N;
   Key choice[N], part[N];  // part: what a group counts by
@@ -228,119 +230,293 @@ __device__ __forceinline__ Choice choose(const RouteArgs& p, const float (&logit
   }
 
   if (p.groups > 1) {
-    const int per = p.experts / p.groups, span = per / N;
-    Key own = 0;  // of the group that this lane's experts are in; else of group `lane`
-    const bool whole = span * N == per && (span & (span - 1)) == 0;
-    if (whole) {
+    const int per = p.experts / p.groups;
+    Key own = 0;  // of group `lane`
+    for (int g = 0; g < p.groups; ++g) {
       Key best = 0, second = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) take(best, second, p.group_score == kTop2 ? part[i] : choice[i]);
-      for (int o = 1; o < span; o <<= 1) {
+      for (int i = 0; i < N; ++i)
+        if (e0 + i >= g * per && e0 + i < g * per + per) take(best, second, p.group_score == kTop2 ? part[i] : choice[i]);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
         const Key b = __shfl_xor_sync(kFull, best, o), s = __shfl_xor_sync(kFull, second, o);
         take(best, second, b);
         take(best, second, s);
       }
-      own = group_key<T>(p.group_score, best, second);
-    } else {
-      for (int g = 0; g < p.groups; ++g) {
-        Key best = 0, second = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (e0 + i >= g * per && e0 + i < g * per + per) take(best, second, p.group_score == kTop2 ? part[i] : choice[i]);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const Key b = __shfl_xor_sync(kFull, best, o), s = __shfl_xor_sync(kFull, second, o);
-          take(best, second, b);
-          take(best, second, s);
-        }
-        if (lane == g) own = group_key<T>(p.group_score, best, second);
-      }
+      if (lane == g) own = group_key<T>(p.group_score, best, second);
     }
-    const int group = whole ? lane / span : lane;
     int before = 0;  // groups that come before this lane's
     for (int g = 0; g < p.groups; ++g) {
-      const Key other = O::from(own, whole ? g * span : g);
-      before += other > own || (other == own && g < group);
+      const Key other = O::from(own, g);
+      before += other > own || (other == own && g < lane);
     }
-    const bool kept = group < p.groups && before < p.top_groups;
+    const bool kept = lane < p.groups && before < p.top_groups;
     if (kCheck && by_score && p.top_groups < p.groups) {
       const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(own) : 0xFFFFFFFFu);
-      const uint32_t highest = __reduce_max_sync(kFull, kept || group >= p.groups ? 0u : static_cast<uint32_t>(own));
-      out.near |= near_by(lowest, highest);
+      const uint32_t highest = __reduce_max_sync(kFull, kept || lane >= p.groups ? 0u : static_cast<uint32_t>(own));
+      near |= near_by(lowest, highest);
     }
     const uint32_t groups_kept = __ballot_sync(kFull, kept);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (whole ? !kept : e0 + i < p.experts && !(groups_kept >> ((e0 + i) / per) & 1u)) choice[i] = 0;
+      if (e0 + i < p.experts && !(groups_kept >> ((e0 + i) / per) & 1u)) choice[i] = 0;
   }
 
-  // A lane's largest come first, equal ones by index (neighbours change places only where the second is larger), so that
-  // its next one is always in choice[0]; for more experts a lane sorting costs more than looking for the largest each time.
-  constexpr bool kSorted = N <= 8;
-  int at[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) at[i] = e0 + i;
-  if constexpr (kSorted) {
-#pragma unroll
-    for (int pass = 0; pass < N; ++pass)
-#pragma unroll
-      for (int i = pass & 1; i + 1 < N; i += 2) {
-        const bool swap = choice[i + 1] > choice[i];
-        const Key k = choice[i];
-        const int e = at[i];
-        choice[i] = swap ? choice[i + 1] : choice[i];
-        at[i] = swap ? at[i + 1] : at[i];
-        choice[i + 1] = swap ? k : choice[i + 1];
-        at[i + 1] = swap ? e : at[i + 1];
-      }
-  }
+  int chosen = -1;
   Key mine = 0;  // of this lane's choice
   Key next = 0;  // the largest that was not chosen
-  for (int j = 0;; ++j) {
+  const int rounds = p.top_k + (kCheck && p.bias != nullptr);  // one more to see how near the next one is
+  for (int j = 0; j < rounds; ++j) {
     Key best = choice[0];
-    int place = at[0];
-    if constexpr (!kSorted) {
+    int place = e0;
 #pragma unroll
-      for (int i = 1; i < N; ++i) {
-        place = choice[i] > best ? e0 + i : place;
-        best = choice[i] > best ? choice[i] : best;
-      }
+    for (int i = 1; i < N; ++i) {
+      place = choice[i] > best ? e0 + i : place;
+      best = choice[i] > best ? choice[i] : best;
     }
     const Key top = O::max_of(best);
     if (j == p.top_k) next = top;
     if (top == 0 || j == p.top_k) break;
-    const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
-    const int expert = __shfl_sync(kFull, place, owner);
+    const int expert = __shfl_sync(kFull, place, __ffs(__ballot_sync(kFull, best == top)) - 1);
     if (lane == j) {
-      out.expert = expert;
+      chosen = expert;
       mine = top;
     }
-    if (j + 1 == p.top_k && !(kCheck && p.bias != nullptr)) break;  // one more round to see how near the next one is
-    if constexpr (kSorted) {
-      if (lane == owner) {
 #pragma unroll
-        for (int i = 0; i + 1 < N; ++i) {
-          choice[i] = choice[i + 1];
-          at[i] = at[i + 1];
-        }
-        choice[N - 1] = 0;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) choice[i] = e0 + i == expert ? 0 : choice[i];
-    }
+    for (int i = 0; i < N; ++i) choice[i] = e0 + i == expert ? 0 : choice[i];
   }
-  if (p.bias == nullptr && out.expert >= 0) out.logit = static_cast<float>(O::value(mine));
   if (kCheck && p.bias != nullptr) {
     const Key below = __shfl_down_sync(kFull, mine, 1);
-    out.near |= __any_sync(kFull, near_by(static_cast<uint32_t>(mine), static_cast<uint32_t>(lane + 1 == p.top_k ? next : lane == 31 ? 0 : below)));
+    near |= __any_sync(kFull, near_by(static_cast<uint32_t>(mine), static_cast<uint32_t>(lane + 1 == p.top_k ? next : lane == 31 ? 0 : below)));
   }
-  return out;
+  return chosen;
 }
 
+template <class T, int N>
+__device__ __noinline__ int choose_apart(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane, bool& near) {
+  return choose<T, N>(p, logit, row, lane, near);
+}
+
+// A warp's sorted lists (choose_quickly): each lane's keys after its largest, and the experts chosen.
 template <int N>
-__device__ __noinline__ int choose_in_64_bits(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane) {
-  return choose<double, N>(p, logit, row, lane).expert;
+struct Lists {
+  static constexpr bool kUsed = N <= 8;
+  uint32_t key[kUsed ? N : 1][kUsed ? 32 : 1];
+  uint16_t chosen[kUsed ? 32 : 2];
+};
+
+// The largest key first.
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
+  constexpr int kPairs = N == 8 ? 19 : N == 4 ? 5 : N == 2 ? 1 : 0;
+  constexpr int kFirst[19] = {0, 1, 4, 5, 0, 1, 2, 3, 0, 2, 4, 6, 2, 3, 1, 3, 1, 3, 5}, kSecond[19] = {2, 3, 6, 7, 4, 5, 6, 7, 1, 3, 5, 7, 4, 5, 4, 6, 2, 4, 6};
+  constexpr int kFirst4[5] = {0, 2, 0, 1, 1}, kSecond4[5] = {1, 3, 2, 3, 2};
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int a = N == 8 ? kFirst[i] : N == 4 ? kFirst4[i] : 0, b = N == 8 ? kSecond[i] : N == 4 ? kSecond4[i] : 1;
+    const uint32_t high = max(k[a], k[b]), low = min(k[a], k[b]);
+    k[a] = high;
+    k[b] = low;
+  }
+}
+
+constexpr uint32_t kKeyBits = ~7u;
+
+// A value's key with the expert's place in its lane; 0 for what is closed.
+__device__ __forceinline__ uint32_t placed_key(float v, int i, bool open) {
+  const uint32_t k = Order<float>::of(v);
+  return open ? ((k == 1u ? 8u : k) & kKeyBits) | static_cast<uint32_t>(7 - i) : 0u;
+}
+
+__device__ __forceinline__ float key_value(uint32_t k) { return Order<float>::value((k & kKeyBits) == 8u ? 1u : k & kKeyBits); }
+
+// What choices go by, in 64 bits, of an expert with this logit and bias.
+__device__ __forceinline__ double choice_score(const RouteArgs& p, float logit, float bias, const Row& row, double sum) {
+  if (p.bias == nullptr) return logit;
+  const double score = p.scoring == kSigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(logit)))
+                       : row.broken          ? static_cast<double>(NAN)
+                                             : exp(static_cast<double>(logit) - static_cast<double>(row.top)) / sum;
+  return score + static_cast<double>(bias);
+}
+
+// The sum of a softmax.
+template <int N>
+__device__ __forceinline__ double sum_in_64_bits(const float (&logit)[N], const Row& row) {
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum += exp(static_cast<double>(logit[i]) - static_cast<double>(row.top));  // 0 where there is no expert
+  return warp_sum(sum);
+}
+
+// The key of each lane's group in 64 bits, for groups of `span` lanes.
+template <int N>
+__device__ __noinline__ uint64_t group_in_64_bits(const RouteArgs& p, const float (&logit)[N], const Row& row, int lane, int span) {
+  const bool sums = p.group_score == kTop2;
+  const double sum = p.scoring == kSoftmax && p.bias != nullptr ? sum_in_64_bits<N>(logit, row) : 1.0;
+  uint64_t first = 0, second = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = lane * N + i;
+    const float bias = p.bias != nullptr && e < p.experts ? p.bias[e] : 0.0f;
+    if (logit[i] == -INFINITY || bias == -INFINITY) continue;
+    double v = choice_score(p, logit[i], bias, row, sum);
+    if (sums && p.bias == nullptr)
+      // a softmax's without its denominator, which is the same for all groups
+      v = p.scoring == kSigmoid ? 1.0 / (1.0 + exp(-v)) : row.broken ? static_cast<double>(NAN) : exp(v - static_cast<double>(row.top));
+    take(first, second, Order<double>::of(v));
+  }
+  for (int o = 1; o < span; o <<= 1) {
+    const uint64_t b = __shfl_xor_sync(kFull, first, o), s = __shfl_xor_sync(kFull, second, o);
+    take(first, second, b);
+    take(first, second, s);
+  }
+  return group_key<double>(p.group_score, first, second);
+}
+
+// Whether this lane's group, of `span` lanes, is among the best.
+template <class K>
+__device__ __forceinline__ bool group_kept(const RouteArgs& p, K own, int lane, int span) {
+  // the lanes of a group compare it with every span-th
+  const int group = lane / span, mine = lane & (span - 1);
+  int before = 0;  // groups that come before this lane's
+  for (int g0 = 0; g0 < p.groups; g0 += span) {
+    const int g = g0 + mine;
+    const K other = __shfl_sync(kFull, own, g * span);
+    before += g < p.groups && (other > own || (other == own && g < group));
+  }
+  for (int o = 1; o < span; o <<= 1) before += __shfl_xor_sync(kFull, before, o);
+  return group < p.groups && before < p.top_groups;
+}
+
+// The first `count` experts in `chosen`, put in order in 64 bits. A lane has one.
+template <int N>
+__device__ __noinline__ void order_in_64_bits(const RouteArgs& p, const float (&logit)[N], float mine, const Row& row, int lane, uint16_t* chosen,
+                                              int count) {
+  const double sum = p.scoring == kSoftmax && p.bias != nullptr ? sum_in_64_bits<N>(logit, row) : 1.0;
+  const int expert = lane < count ? chosen[lane] : 0;
+  const float bias = p.bias != nullptr && lane < count ? p.bias[expert] : 0.0f;
+  const uint64_t key = Order<double>::of(choice_score(p, mine, bias, row, sum));
+  int before = 0;
+  for (int i = 0; i < count; ++i) {
+    const uint64_t other = __shfl_sync(kFull, key, i);
+    const int e = __shfl_sync(kFull, expert, i);
+    before += other > key || (other == key && e < expert);
+  }
+  __syncwarp();
+  if (lane < count) chosen[before] = static_cast<uint16_t>(expert);
+  __syncwarp();
+}
+
+// choose() for up to eight experts a lane, and groups that fill a power of two of lanes. `open`: not decided.
+template <int DT, int N>
+__device__ __forceinline__ int choose_quickly(const RouteArgs& p, int64_t token, const float (&logit)[N], const Row& row, int lane, Lists<N>& lists,
+                                              bool& open) {
+  constexpr bool kNarrow = DT != kF32;  // no bits are lost
+  open = false;
+  const int e0 = lane * N;
+  uint32_t key[N];
+  if (p.bias != nullptr) {
+    float score[N], bias[N];
+    load_values<kF32, N>(p.bias, e0, p.experts - e0, p.bias_vec != 0, bias);
+    if (p.scoring == kSigmoid) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) score[i] = quotient(1.0f, 1.0f + exp_of(-logit[i]));
+    } else {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        score[i] = exp_of(logit[i] - row.top);  // 0 where there is no expert
+        sum += score[i];
+      }
+      const float unit = row.broken ? NAN : quotient(1.0f, warp_sum(sum));
+#pragma unroll
+      for (int i = 0; i < N; ++i) score[i] *= unit;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] = placed_key(score[i] + bias[i], i, logit[i] != -INFINITY && bias[i] != -INFINITY);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] = placed_key(logit[i], i, logit[i] != -INFINITY);
+  }
+  sort_keys<N>(key);
+  uint32_t best = key[0];  // this lane's largest
+  const auto apart = [&](uint32_t upper, uint32_t lower) {  // certainly in this order
+    if (upper == 0u || lower == 0u) return true;
+    return p.bias != nullptr ? !near_by(upper == 8u ? 1u : upper, lower == 8u ? 1u : lower) : kNarrow || upper != lower;
+  };
+
+  if (p.groups > 1) {
+    const int span = p.experts / p.groups / N;  // lanes of a group
+    uint32_t first = key[0], second = N > 1 ? key[N > 1 ? 1 : 0] : 0u;
+    const bool sums = p.group_score == kTop2;
+    if (sums && p.bias == nullptr) {
+      // of the two best logits; a softmax's without its denominator, which is the same for all groups
+      const float a = key_value(first), b = key_value(second);
+      const auto score = [&](float v) { return p.scoring == kSigmoid ? quotient(1.0f, 1.0f + exp_of(-v)) : row.broken ? NAN : exp_of(v - row.top); };
+      first = first == 0u ? 0u : Order<float>::of(score(a));
+      second = second == 0u ? 0u : Order<float>::of(score(b));
+    } else {
+      first &= kKeyBits;
+      second &= kKeyBits;
+    }
+    for (int o = 1; o < span; o <<= 1) {
+      const uint32_t b = __shfl_xor_sync(kFull, first, o), s = __shfl_xor_sync(kFull, second, o);
+      take(first, second, b);
+      take(first, second, s);
+    }
+    uint32_t own = first;
+    if (sums && second != 0u) own = Order<float>::of(key_value(first) + key_value(second));
+    bool kept = group_kept(p, own, lane, span);
+    if ((sums || p.bias != nullptr || !kNarrow) && p.top_groups < p.groups) {
+      const uint32_t lowest = __reduce_min_sync(kFull, kept ? own : 0xFFFFFFFFu);
+      const uint32_t highest = __reduce_max_sync(kFull, kept || lane / span >= p.groups ? 0u : own);
+      if (sums || p.bias != nullptr ? near_by(lowest == 8u ? 1u : lowest, highest == 8u ? 1u : highest) : lowest == highest && lowest != 0u)
+        kept = group_kept(p, group_in_64_bits<N>(p, logit, row, lane, span), lane, span);
+    }
+    if (!kept) best = 0u;
+  }
+
+#pragma unroll
+  for (int i = 1; i < N; ++i) lists.key[i - 1][lane] = key[i];
+  lists.key[N - 1][lane] = 0u;
+  uint32_t mine = 0u;  // the key of this lane's choice
+  int taken = 0;       // of this lane's list
+  const auto choose_next = [&](int j, uint32_t largest) {
+    if (lane == j) mine = largest;
+    if (lane == __ffs(__ballot_sync(kFull, (best & kKeyBits) == largest)) - 1) {
+      lists.chosen[j] = static_cast<uint16_t>(e0 + 7 - static_cast<int>(best & 7u));
+      best = lists.key[taken++][lane];
+    }
+  };
+  int count = 0;
+  for (; count < p.top_k; ++count) {
+    const uint32_t largest = __reduce_max_sync(kFull, best & kKeyBits);
+    if (largest == 0u) break;
+    choose_next(count, largest);
+  }
+  if (!kNarrow || p.bias != nullptr) {
+    uint32_t next = __reduce_max_sync(kFull, best & kKeyBits);
+    const uint32_t down = __shfl_down_sync(kFull, mine, 1), below = lane + 1 >= p.top_k ? next : down;
+    if (__any_sync(kFull, lane < p.top_k && !apart(mine, below))) {
+      // more experts, until one is certainly below: these are put in order
+      uint32_t last = __shfl_sync(kFull, mine, p.top_k - 1);
+      while (!apart(last, next) && count < 32) {
+        choose_next(count++, next);
+        last = next;
+        next = __reduce_max_sync(kFull, best & kKeyBits);
+      }
+      open = !apart(last, next);
+      __syncwarp();
+      if (!open) {
+        const float own = lane < count ? value_at<DT>(p.logits, token * p.stride + lists.chosen[lane]) : 0.0f;
+        order_in_64_bits<N>(p, logit, own, row, lane, lists.chosen, count);
+      }
+    }
+  }
+  __syncwarp();
+  const int chosen = lane < min(count, p.top_k) ? lists.chosen[lane] : -1;
+  __syncwarp();  // before the next token's
+  return chosen;
 }
 
 // A lane's share of a token's weights, before the scale: the score of its expert, renormalised or not.
@@ -381,19 +557,19 @@ __device__ __forceinline__ Share share_of(int scoring, bool renormalize, float l
   return s;
 }
 
-template <int DT, int N>
-__device__ __forceinline__ void load_row(const RouteArgs& p, int64_t token, int lane, float (&logit)[N], Row& row) {
-  load_values<DT, N>(p.logits, token * p.stride + lane * N, p.experts - lane * N, p.vec != 0, logit);
-  bool broken = false;
-  float top = -INFINITY;
+template <int N>
+__device__ __forceinline__ Row row_of(const float (&logit)[N]) {
+  float all = logit[0], top = logit[0];  // a NaN if there is one; without NaNs
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    broken |= !(logit[i] < INFINITY);
+  for (int i = 1; i < N; ++i) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(all) : "f"(logit[i]));
     top = fmaxf(top, logit[i]);
   }
-  row.broken = __any_sync(kFull, broken);
-  row.top = Order<float>::value(__reduce_max_sync(kFull, Order<float>::of(top)));
+  Row row;
+  row.broken = __any_sync(kFull, !(all < INFINITY));
+  row.top = Order<float>::value(__reduce_max_sync(kFull, top == top ? Order<float>::of(top) : 0x007FFFFFu));
   if (row.top == -INFINITY) row.top = 0.0f;  // nothing is open
+  return row;
 }
 
 // All of softmax's exponentials of a row, relative to its largest.
@@ -407,8 +583,8 @@ __device__ __forceinline__ float total_of(const float (&logit)[N], const Row& ro
 
 // --------------------------------------------------------------------- the order by expert
 // The places of a block's choices, in the order of experts and within one of tokens. counts: choices of each chunk of
-// tokens (chunks, pitch), 16-byte aligned, zeros behind the last expert. Shared: start (pitch + 32) words, parts 8 words a
-// thread. A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
+// tokens (chunks, pitch), 16-byte aligned, zeros behind the last expert. Shared: start (pitch + 32) words, parts
+// (place_words). A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
 __device__ __forceinline__ void place(const RouteArgs& p, const int32_t* counts, int32_t* start, int32_t* parts) {
   const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quads = p.pitch >> 2, wide = min(threads, quads <= 32 ? 32 : 1 << (32 - __clz(quads - 1)));
@@ -475,21 +651,35 @@ __device__ __forceinline__ void place(const RouteArgs& p, const int32_t* counts,
     p.source[i] = -1;
   const int64_t from = static_cast<int64_t>(blockIdx.x) * p.chunk * p.top_k;
   const int items = static_cast<int>(min(static_cast<int64_t>(p.chunk) * p.top_k, places - from));
-  // 32 choices of a warp at once, one warp after another
+  // A warp takes 32 choices and leaves how many each expert has among them (table: warps x pitch, 16 bits); a thread an
+  // expert then makes of the counts what the warps before have.
+  uint16_t* table = reinterpret_cast<uint16_t*>(parts);
   for (int i0 = 0; i0 < items; i0 += threads) {
+    const int warps = min(threads, items - i0 + 31) / 32;  // that have choices
+    for (int i = threadIdx.x; i < warps * p.pitch / 2; i += threads) reinterpret_cast<uint32_t*>(table)[i] = 0u;
+    __syncthreads();
     const int i = i0 + threadIdx.x;
     const int e = i < items ? p.experts_out[from + i] : -1;
     const uint32_t same = __match_any_sync(kFull, e);
     const int rank = __popc(same & ((1u << lane) - 1u));
-    int at = -1;
-    for (int w = 0; w < threads / 32 && i0 + w * 32 < items; ++w) {
-      if (w == warp && e >= 0) at = start[e] + rank;
-      if (w == warp) __syncwarp();
-      if (w == warp && e >= 0 && rank == 0) start[e] += __popc(same);
-      __syncthreads();
+    if (e >= 0 && rank == 0) table[warp * p.pitch + e] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    for (int x = threadIdx.x; x < p.experts; x += threads) {
+      int sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < warps; ++w) {
+        const int n = table[w * p.pitch + x];
+        table[w * p.pitch + x] = static_cast<uint16_t>(sum);
+        sum += n;
+      }
+      parts[warps * p.pitch / 2 + x] = sum;
     }
+    __syncthreads();
+    const int at = e >= 0 ? start[e] + table[warp * p.pitch + e] + rank : -1;
     if (i < items) p.rows[from + i] = at;
     if (at >= 0) p.source[at] = static_cast<int32_t>(from + i);
+    __syncthreads();
+    for (int x = threadIdx.x; x < p.experts; x += threads) start[x] += parts[warps * p.pitch / 2 + x];
   }
 }
 
@@ -502,18 +692,25 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
   for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) shared[e] = 0;
   __syncthreads();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk, end = min(first + p.chunk, p.tokens);
+  // the lists lie behind the counts, where choices are placed later
+  auto& lists = reinterpret_cast<Lists<N>*>(shared + p.pitch)[warp];
   for (int64_t token = first + warp; token < end; token += warps) {
     int chosen = -1;
     float weight = 0.0f;
     if (p.mask == nullptr || p.mask[token] != 0) {
       float logit[N];
-      Row row;
-      load_row<DT, N>(p, token, lane, logit, row);
-      const Choice c = choose<float, N>(p, logit, row, lane);
-      chosen = c.near ? choose_in_64_bits<N>(p, logit, row, lane) : c.expert;
+      load_values<DT, N>(p.logits, token * p.stride + lane * N, p.experts - lane * N, p.vec != 0, logit);
+      const Row row = row_of<N>(logit);
+      bool near, none;
+      if constexpr (Lists<N>::kUsed) {
+        if (p.quick != 0) chosen = choose_quickly<DT, N>(p, token, logit, row, lane, lists, near);
+        else chosen = choose_apart<float, N>(p, logit, row, lane, near);
+      } else {
+        chosen = choose<float, N>(p, logit, row, lane, near);
+      }
+      if (near) chosen = choose_apart<double, N>(p, logit, row, lane, none);
       const float total = p.scoring == kSoftmax && p.renormalize == 0 ? total_of<N>(logit, row) : 1.0f;
-      float mine = c.logit;
-      if (chosen >= 0 && (p.bias != nullptr || c.near)) mine = value_at<DT>(p.logits, token * p.stride + chosen);
+      const float mine = chosen >= 0 ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
       const Share s = share_of(p.scoring, p.renormalize != 0, mine, chosen >= 0, row, total);
       weight = chosen >= 0 ? __fdiv_rn(s.score, s.sum) * p.scale : 0.0f;
     }
@@ -525,7 +722,7 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
   }
   __syncthreads();
   if constexpr (kOne) {
-    place(p, shared, shared + p.pitch, shared + 2 * p.pitch + 32);
+    place(p, shared, shared + p.pitch, shared + 2 * p.pitch + 32);  // over the lists, which are done with
   } else {
     for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) p.counts[static_cast<int64_t>(blockIdx.x) * p.pitch + e] = shared[e];
   }
@@ -569,7 +766,8 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const __grid_constant__
   Row row{0.0f, false};
   float total = 1.0f;
   if (whole) {
-    load_row<DT, N>(p, token, lane, logit, row);
+    load_values<DT, N>(p.logits, token * p.stride + lane * N, p.experts - lane * N, p.vec != 0, logit);
+    row = row_of<N>(logit);
     if (p.renormalize == 0) total = total_of<N>(logit, row);
   }
   const float mine = has ? value_at<DT>(p.logits, token * p.stride + chosen) : 0.0f;
