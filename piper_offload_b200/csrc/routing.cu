@@ -193,6 +193,9 @@ int values_at_once(const piper_routing_exchange& e, std::initializer_list<const 
   return e.hidden % n == 0 ? n : 1;
 }
 
+// Choices whose rows a thread loads at once; with few it takes more pieces.
+int choices_at_once(int top_k) { return top_k <= 2 ? 2 : top_k <= 4 ? 4 : 8; }
+
 routing::ExchangeArgs exchange_args(const piper_routing_exchange& e, int values) {
   routing::ExchangeArgs a{};
   a.rows = e.rows;
@@ -339,9 +342,15 @@ int piper_routing_combine(const piper_routing_exchange* x, const void* y, int64_
   a.in_stride = y_stride;
   a.weights = weights;
   a.out = out;
-  const int64_t blocks = (x->tokens * a.pieces + routing::kExchangeThreads - 1) / routing::kExchangeThreads;
+  const int64_t each = routing::kExchangeThreads * (routing::kAtOnce / choices_at_once(x->top_k));
+  const int64_t blocks = (x->tokens * a.pieces + each - 1) / each;
   ROUTING_REQUIRE(blocks < (int64_t{1} << 31), "Combine: too many values for one call.");
-#define CALL(D, V) routing::combine_kernel<D, V><<<static_cast<unsigned>(blocks), routing::kExchangeThreads, 0, static_cast<cudaStream_t>(stream)>>>(a)
+  const auto grid = static_cast<unsigned>(blocks);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define CALL(D, V)                                                                                                            \
+  if (choices_at_once(x->top_k) == 2) routing::combine_kernel<D, V, 2><<<grid, routing::kExchangeThreads, 0, s>>>(a);            \
+  else if (choices_at_once(x->top_k) == 4) routing::combine_kernel<D, V, 4><<<grid, routing::kExchangeThreads, 0, s>>>(a);       \
+  else routing::combine_kernel<D, V, 8><<<grid, routing::kExchangeThreads, 0, s>>>(a)
   EXCHANGE_DISPATCH(x->dtype, values > 1, CALL);
 #undef CALL
   const cudaError_t e = launched();
@@ -367,12 +376,18 @@ int piper_routing_combine_grad(const piper_routing_exchange* x, const void* y, i
   a.out = dy;
   a.dweights = dweights;
   const bool wide_blocks = x->tokens < 32 * sm_count();  // too few tokens to fill the SMs with a warp each
-  const int64_t blocks = wide_blocks ? x->tokens : (x->tokens + 7) / 8;
-#define CALL(D, V)                                                                                                              \
-  if (wide_blocks) routing::combine_grad_kernel<D, V, 8><<<static_cast<unsigned>(blocks), routing::kExchangeThreads, 0, static_cast<cudaStream_t>(stream)>>>(a); \
-  else routing::combine_grad_kernel<D, V, 1><<<static_cast<unsigned>(blocks), routing::kExchangeThreads, 0, static_cast<cudaStream_t>(stream)>>>(a)
+  const auto grid = static_cast<unsigned>(wide_blocks ? x->tokens : (x->tokens + 7) / 8);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define LAUNCH(D, V, K)                                                                                                  \
+  if (wide_blocks) routing::combine_grad_kernel<D, V, K, 8><<<grid, routing::kExchangeThreads, 0, s>>>(a);                \
+  else routing::combine_grad_kernel<D, V, K, 1><<<grid, routing::kExchangeThreads, 0, s>>>(a)
+#define CALL(D, V)                                              \
+  if (choices_at_once(x->top_k) == 2) { LAUNCH(D, V, 2); }      \
+  else if (choices_at_once(x->top_k) == 4) { LAUNCH(D, V, 4); } \
+  else { LAUNCH(D, V, 8); }
   EXCHANGE_DISPATCH(x->dtype, values > 1, CALL);
 #undef CALL
+#undef LAUNCH
   const cudaError_t e = launched();
   return e == cudaSuccess ? PIPER_ROUTING_OK : cuda_fail("combine gradient kernel", e);
 }

@@ -81,9 +81,9 @@ __device__ __forceinline__ Pack<DT, V> from_floats(const float (&f)[V]) {
   return r;
 }
 
-// The place of choice j of a token, or -1.
-__device__ __forceinline__ int64_t place_of(const ExchangeArgs& p, int64_t token, int j) {
-  const int64_t r = p.rows[token * p.top_k + j];
+// The place of choice j of a token, or -1. There are fewer than 2^31 places.
+__device__ __forceinline__ int32_t place_of(const ExchangeArgs& p, int64_t token, int j) {
+  const int32_t r = p.rows[token * p.top_k + j];
   return r >= 0 && r < p.tokens * p.top_k ? r : -1;
 }
 
@@ -97,104 +97,125 @@ __global__ void __launch_bounds__(kExchangeThreads) dispatch_kernel(const __grid
   const Pack<DT, V> v = load_pack<DT, V>(p.in, token * p.in_stride + col);
   const int64_t total = *p.total;
   for (int j = 0; j < p.top_k; ++j) {
-    const int64_t r = place_of(p, token, j);
-    if (r >= 0 && r < total) store_pack<DT, V>(p.out, r * p.hidden + col, v);
+    const int32_t r = place_of(p, token, j);
+    if (r >= 0 && r < total) store_pack<DT, V>(p.out, static_cast<int64_t>(r) * p.hidden + col, v);
     if (token * p.top_k + j >= total) store_pack<DT, V>(p.out, (token * p.top_k + j) * p.hidden + col, Pack<DT, V>{});
   }
 }
 
-constexpr int kAtOnce = 8;  // rows whose loads are in flight together
+constexpr int kAtOnce = 8;  // loads of rows that a thread has in flight: of K choices for each of kAtOnce / K pieces
 
-// A thread has a piece of a token's result.
-template <int DT, int V>
-__global__ void __launch_bounds__(kExchangeThreads) combine_kernel(const __grid_constant__ ExchangeArgs p) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kExchangeThreads + threadIdx.x;
-  const int64_t token = i / p.pieces;
-  if (token >= p.tokens) return;
-  const int64_t col = (i - token * p.pieces) * V;
-  float sum[V];
+// A thread has kAtOnce / K pieces of tokens' results.
+template <int DT, int V, int K>
+__global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2) combine_kernel(const __grid_constant__ ExchangeArgs p) {
+  constexpr int kPieces = kAtOnce / K;
+  int64_t token[kPieces], col[kPieces];
+  float sum[kPieces][V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) sum[k] = 0.0f;
-  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
-    Pack<DT, V> v[kAtOnce];
-    float w[kAtOnce];
-    bool has[kAtOnce];
+  for (int q = 0; q < kPieces; ++q) {
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * kPieces + q) * kExchangeThreads + threadIdx.x;
+    token[q] = i / p.pieces;
+    col[q] = (i - token[q] * p.pieces) * V;
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int64_t r = j0 + k < p.top_k ? place_of(p, token, j0 + k) : -1;
-      has[k] = r >= 0;
-      if (has[k]) {
-        v[k] = load_pack<DT, V>(p.in, r * p.in_stride + col);
-        w[k] = p.weights != nullptr ? p.weights[token * p.top_k + j0 + k] : 1.0f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k)
-      if (has[k]) {
-        float f[V];
-        to_floats(v[k], f);
-#pragma unroll
-        for (int n = 0; n < V; ++n) sum[n] = fmaf(w[k], f[n], sum[n]);
-      }
+    for (int k = 0; k < V; ++k) sum[q][k] = 0.0f;
   }
-  store_pack<DT, V>(p.out, token * p.hidden + col, from_floats<DT, V>(sum));
+  for (int j0 = 0; j0 < p.top_k; j0 += K) {
+    Pack<DT, V> v[kPieces][K];
+    float w[kPieces][K];
+    bool has[kPieces][K];
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int32_t r = token[q] < p.tokens && j0 + k < p.top_k ? place_of(p, token[q], j0 + k) : -1;
+        has[q][k] = r >= 0;
+        if (r >= 0) {
+          v[q][k] = load_pack<DT, V>(p.in, static_cast<int64_t>(r) * p.in_stride + col[q]);
+          w[q][k] = p.weights != nullptr ? p.weights[token[q] * p.top_k + j0 + k] : 1.0f;
+        }
+      }
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (has[q][k]) {
+          float f[V];
+          to_floats(v[q][k], f);
+#pragma unroll
+          for (int n = 0; n < V; ++n) sum[q][n] = fmaf(w[q][k], f[n], sum[q][n]);
+        }
+  }
+#pragma unroll
+  for (int q = 0; q < kPieces; ++q)
+    if (token[q] < p.tokens) store_pack<DT, V>(p.out, token[q] * p.hidden + col[q], from_floats<DT, V>(sum[q]));
 }
 
 // kWarps warps have a token: each piece of the result's gradient goes to the rows' gradients, and with the rows into the
 // weights' gradients.
-template <int DT, int V, int kWarps>
-__global__ void __launch_bounds__(kExchangeThreads) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
-  __shared__ float parts[kWarps > 1 ? kAtOnce * 8 : 1];
+template <int DT, int V, int K, int kWarps>
+__global__ void __launch_bounds__(kExchangeThreads, 2) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
+  constexpr int kPieces = kAtOnce / K, kStep = 32 * kWarps;
+  __shared__ float parts[kWarps > 1 ? K * 8 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t token = kWarps == 1 ? static_cast<int64_t>(blockIdx.x) * (kExchangeThreads / 32) + warp : blockIdx.x;
   if (kWarps == 1 && token >= p.tokens) return;
   const int first = kWarps == 1 ? lane : threadIdx.x;
   const int64_t total = *p.total;
-  for (int j0 = 0; j0 < p.top_k; j0 += kAtOnce) {
-    int64_t row[kAtOnce];
-    float w[kAtOnce], dot[kAtOnce];
+  for (int j0 = 0; j0 < p.top_k; j0 += K) {
+    int32_t row[K];
+    float w[K], dot[K];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
+    for (int k = 0; k < K; ++k) {
       const bool in = j0 + k < p.top_k;
       row[k] = in ? place_of(p, token, j0 + k) : -1;
       if (row[k] >= total) row[k] = -1;
       w[k] = in ? p.weights[token * p.top_k + j0 + k] : 0.0f;
       dot[k] = 0.0f;
     }
-    for (int piece = first; piece < p.pieces; piece += 32 * kWarps) {
-      const int64_t col = static_cast<int64_t>(piece) * V;
-      const Pack<DT, V> d = load_pack<DT, V>(p.dout, token * p.dout_stride + col);
-      Pack<DT, V> y[kAtOnce];
+    for (int piece0 = first; piece0 < p.pieces; piece0 += kStep * kPieces) {
+      Pack<DT, V> d[kPieces], y[kPieces][K];
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
-        if (row[k] >= 0) y[k] = load_pack<DT, V>(p.in, row[k] * p.in_stride + col);
-      float g[V];
-      to_floats(d, g);
+      for (int q = 0; q < kPieces; ++q) {
+        const int piece = piece0 + q * kStep;
+        if (piece >= p.pieces) continue;
+        d[q] = load_pack<DT, V>(p.dout, token * p.dout_stride + static_cast<int64_t>(piece) * V);
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        if (row[k] >= 0) {
-          float f[V], dy[V];
-          to_floats(y[k], f);
+        for (int k = 0; k < K; ++k)
+          if (row[k] >= 0) y[q][k] = load_pack<DT, V>(p.in, static_cast<int64_t>(row[k]) * p.in_stride + static_cast<int64_t>(piece) * V);
+      }
 #pragma unroll
-          for (int n = 0; n < V; ++n) {
-            dot[k] = fmaf(f[n], g[n], dot[k]);
-            dy[n] = w[k] * g[n];
+      for (int q = 0; q < kPieces; ++q) {
+        const int piece = piece0 + q * kStep;
+        if (piece >= p.pieces) continue;
+        const int64_t col = static_cast<int64_t>(piece) * V;
+        float g[V];
+        to_floats(d[q], g);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (row[k] >= 0) {
+            float f[V], dy[V];
+            to_floats(y[q][k], f);
+#pragma unroll
+            for (int n = 0; n < V; ++n) {
+              dot[k] = fmaf(f[n], g[n], dot[k]);
+              dy[n] = w[k] * g[n];
+            }
+            store_pack<DT, V>(p.out, static_cast<int64_t>(row[k]) * p.hidden + col, from_floats<DT, V>(dy));
           }
-          store_pack<DT, V>(p.out, row[k] * p.hidden + col, from_floats<DT, V>(dy));
+          const int64_t none = token * p.top_k + j0 + k;
+          if (j0 + k < p.top_k && none >= total) store_pack<DT, V>(p.out, none * p.hidden + col, Pack<DT, V>{});
         }
-        const int64_t none = token * p.top_k + j0 + k;
-        if (j0 + k < p.top_k && none >= total) store_pack<DT, V>(p.out, none * p.hidden + col, Pack<DT, V>{});
       }
     }
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) dot[k] = warp_sum(dot[k]);
+    for (int k = 0; k < K; ++k) dot[k] = warp_sum(dot[k]);
     if constexpr (kWarps > 1) {
       __syncthreads();  // the last ones are read
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
+      for (int k = 0; k < K; ++k)
         if (lane == 0) parts[k * 8 + warp] = dot[k];
       __syncthreads();
-      if (threadIdx.x < kAtOnce && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
+      if (threadIdx.x < K && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < kWarps; ++n) sum += parts[threadIdx.x * 8 + n];
@@ -202,7 +223,7 @@ __global__ void __launch_bounds__(kExchangeThreads) combine_grad_kernel(const __
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
+      for (int k = 0; k < K; ++k)
         if (lane == k && j0 + k < p.top_k) p.dweights[token * p.top_k + j0 + k] = dot[k];
     }
   }
