@@ -11,6 +11,7 @@
 
 #include "int8_grad.cuh"
 #include "int8_linear.cuh"
+#include "int8_pair.cuh"
 #include "int8_quant.cuh"
 
 namespace {
@@ -175,6 +176,7 @@ TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t 
 
 struct LinearPlan {
   int bn, split;
+  bool pair;  // of SMs, on tiles of 256 outputs
   int64_t x_pitch;
   int64_t x_codes, x_scale, x_sums, w_codes, total;  // byte offsets
 };
@@ -184,11 +186,20 @@ LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
   const int64_t stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
   TilePlan best{};
+  const auto items_of = [&](int bn, int64_t outputs) { return std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + outputs - 1) / outputs); };
   for (const int bn : {32, 128, 256}) {
     const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
-    const int64_t items = std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + 127) / 128);
-    const TilePlan t = plan_tile(bn, items, stages, 300.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, sm_count());
+    const TilePlan t = plan_tile(bn, items_of(bn, 128), stages, 300.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, sm_count());
     if (best.bn == 0 || t.cycles < best.cycles) best = t;
+  }
+  for (const int bn : {128, 256}) {
+    if (per_expert <= 64) break;
+    const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 32), bn);
+    const TilePlan t = plan_tile(bn, items_of(bn, 256), stages, 290.0 + static_cast<double>(tile_tokens), tile_tokens, false, sm_count() / 2);
+    if (t.cycles < best.cycles) {
+      best = t;
+      p.pair = true;
+    }
   }
   p.bn = best.bn;
   p.split = best.split;
@@ -239,6 +250,12 @@ cudaError_t launch_linear(const i8::LinearArgs& args, int64_t items, cudaStream_
   using S = i8::LinearShape<BN, 1>;
   return launch<i8::LinearArgs>(i8::linear_kernel<DT, BN, 1>, args, args.split > 1 ? items * args.split : std::min<int64_t>(items, sm_count()),
                                 i8::kLinearThreads, S::kSmem, args.split, stream);
+}
+
+template <int DT, int BN>
+cudaError_t launch_pairs(const i8::LinearArgs& args, int64_t items, cudaStream_t stream) {
+  return launch<i8::LinearArgs>(i8::linear_pair_kernel<DT, BN>, args, 2 * std::min<int64_t>(items, sm_count() / 2), i8::kLinearThreads,
+                                i8::PairShape<BN>::kSmem, 2, stream);
 }
 
 // --------------------------------------------------------------- the gradient
@@ -351,7 +368,7 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   a.x_scale = q.scale;
   a.x_sums = q.sums;
   a.rows_of = {row_scales(*w), static_cast<const int8_t*>(w->zero), w->per_row != 0 ? 1 : 0};
-  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->rows + 127) / 128)};
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>(p.pair ? (w->rows + 255) / 256 : (w->rows + 127) / 128)};
   a.y = y;
   a.rows = static_cast<int32_t>(w->rows);
   a.cols = static_cast<int32_t>(w->cols);
@@ -367,7 +384,7 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   INT8_REQUIRE(blocks < (int64_t{1} << 31), "INT8 product: too many values for one call.");
   const void* codes = r.pieces > 0 ? r.out : w->codes;
   if (!encode_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, w->cols, w->batch * w->rows, code_pitch(*w), i8::kStageCols, fp4::kTileRows) ||
-      !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.bn))
+      !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.pair ? p.bn / 2 : p.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
 
   const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
@@ -381,7 +398,8 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   cudaError_t e = launched();
   if (e != cudaSuccess) return cuda_fail("quantize kernel", e);
 #define CALL(D)                                           \
-  e = p.bn == 32    ? launch_linear<D, 32>(a, items, s)   \
+  e = p.pair        ? (p.bn == 128 ? launch_pairs<D, 128>(a, items, s) : launch_pairs<D, 256>(a, items, s)) \
+      : p.bn == 32  ? launch_linear<D, 32>(a, items, s)   \
       : p.bn == 128 ? launch_linear<D, 128>(a, items, s)  \
                     : launch_linear<D, 256>(a, items, s)
   INT8_DISPATCH(dtype, CALL);
@@ -467,7 +485,7 @@ int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, piper_int
   if (int rc = check_matrix(w)) return rc;
   INT8_REQUIRE(plan != nullptr && tokens > 0, "INT8 product: bad plan query.");
   const LinearPlan p = plan_linear(*w, tokens);
-  *plan = {p.bn, 128, p.split, 1};
+  *plan = {p.bn, p.pair ? 256 : 128, p.split, 1};
   return PIPER_INT8_OK;
 }
 
