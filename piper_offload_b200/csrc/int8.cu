@@ -128,16 +128,21 @@ i8::RepackArgs repack_args(const piper_int8_matrix& w, uint8_t* out) {
   return r;
 }
 
-// Which threads work on a row of `units` units: a warp, which waits for no other, where its registers hold the row and
-// there are rows for all SMs, else the eight warps of a block.
+// Warps that work on a row of `units` units: as few as hold it in their registers, four units a lane (two of fp32), so that
+// rows wait for few others (4096 x 4096 bf16 to codes: 10.4 us with two warps, 14.3 with one or eight; x 8192 18.5 with
+// four, 27.4 with one, 20.5 with eight; x 14336 30.8 with eight, 36.9 with four); eight where there are too few rows for
+// all SMs, or where rows have no whole units.
 struct RowPlan {
-  int warps, hold;
+  int warps;
   int64_t blocks;
 };
-RowPlan plan_rows(int64_t rows, int64_t units, int most) {
-  if (units <= 64) return {1, 2, (rows + 7) / 8};
-  if (units <= 32 * most && rows >= 8 * sm_count()) return {1, most, (rows + 7) / 8};
-  return {8, units <= 512 ? 2 : 4, rows};
+RowPlan plan_rows(int64_t rows, int64_t units, int dtype, bool vec) {
+  const int64_t lane = dtype == PIPER_INT8_F32 ? 2 : 4;
+  int warps = 1;
+  while (warps < 8 && units > 32 * lane * warps) warps *= 2;
+  if (units > 64 && (rows < 8 * sm_count() || !vec)) warps = 8;
+  if (!vec && units <= 64) warps = 1;
+  return {warps, warps == 1 ? (rows + 7) / 8 : rows};
 }
 
 // Rows that start on 16-byte boundaries and have whole units.
@@ -146,12 +151,15 @@ bool whole_units(const void* p, int64_t stride, int64_t rows, int64_t cols, int 
 }
 
 template <class Args, class Kernel>
-void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, unsigned row_blocks,
-                 Kernel warp_short, Kernel warp_long, Kernel block_short, Kernel block_long, Kernel warp_any, Kernel block_any) {
-  const Kernel kernel = !vec             ? (rows.warps == 1 ? warp_any : block_any)
-                        : rows.warps == 1 ? (rows.hold == 2 ? warp_short : warp_long)
-                                          : (rows.hold == 2 ? block_short : block_long);
-  kernel<<<grid, i8::kPrepareThreads, 0, s>>>(args, r, row_blocks);
+void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, Kernel one, Kernel two,
+                 Kernel four, Kernel eight, Kernel one_any, Kernel eight_any) {
+  const Kernel kernel = !vec ? (rows.warps == 1 ? one_any : eight_any) : rows.warps == 1 ? one : rows.warps == 2 ? two : rows.warps == 4 ? four : eight;
+  kernel<<<grid, i8::prepare_threads(rows.warps), 0, s>>>(args, r, static_cast<unsigned>(rows.blocks));
+}
+
+int64_t repack_blocks(const i8::RepackArgs& r, const RowPlan& rows) {
+  const int64_t threads = i8::prepare_threads(rows.warps);
+  return (r.pieces + threads - 1) / threads;
 }
 
 // ---------------------------------------------------------------- the product
@@ -378,21 +386,21 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   const int64_t items = token_tiles(tokens, ends == nullptr ? 0 : w->batch, p.bn) * a.groups.row_tiles;
   a.items = static_cast<int32_t>(items);
   INT8_REQUIRE(items < (int64_t{1} << 31) / i8::kMaxSplit, "INT8 product: too many tiles for one call.");
-  const int most = dtype == PIPER_INT8_F32 ? 4 : 8;
-  const RowPlan rows = plan_rows(tokens, p.x_pitch / i8::kUnit, most);
-  const int64_t blocks = rows.blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  const bool vec = whole_units(x, x_stride, tokens, w->cols, dtype);
+  const RowPlan rows = plan_rows(tokens, p.x_pitch / i8::kUnit, dtype, vec);
+  const int64_t blocks = rows.blocks + repack_blocks(r, rows);
   INT8_REQUIRE(blocks < (int64_t{1} << 31), "INT8 product: too many values for one call.");
   const void* codes = r.pieces > 0 ? r.out : w->codes;
   if (!encode_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, w->cols, w->batch * w->rows, code_pitch(*w), i8::kStageCols, fp4::kTileRows) ||
       !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.pair ? p.bn / 2 : p.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
-  const bool vec = whole_units(x, x_stride, tokens, w->cols, dtype);
-#define CALL(D)                                                                                                            \
-  launch_rows(grid, s, rows, vec, q, r, tokens_grid, i8::quantize_kernel<D, 1, 2, true>, i8::quantize_kernel<D, 1, D == i8::kF32 ? 4 : 8, true>, \
-              i8::quantize_kernel<D, 8, 2, true>, i8::quantize_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>,                    \
-              i8::quantize_kernel<D, 1, 2, false>, i8::quantize_kernel<D, 8, 2, false>)
+  const auto grid = static_cast<unsigned>(blocks);
+#define CALL(D)                                                                                                              \
+  constexpr int kHold = D == i8::kF32 ? 2 : 4;                                                                                \
+  launch_rows(grid, s, rows, vec, q, r, i8::quantize_kernel<D, 1, kHold, true>, i8::quantize_kernel<D, 2, kHold, true>,            \
+              i8::quantize_kernel<D, 4, kHold, true>, i8::quantize_kernel<D, 8, kHold, true>, i8::quantize_kernel<D, 1, 2, false>,       \
+              i8::quantize_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   cudaError_t e = launched();
@@ -456,18 +464,19 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   a.terms = p.terms;
   a.split = tile.split;
   a.vec = aligned(dx, 16) && (w->cols * static_cast<int64_t>(width(dtype))) % 16 == 0;
-  const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, 4);
-  const int64_t blocks = rows.blocks + (r.pieces + i8::kPrepareThreads - 1) / i8::kPrepareThreads;
+  const bool vec = whole_units(dy, dy_stride, tokens, w->rows, dtype) && aligned(w->scale, 16);
+  const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, dtype, vec);
+  const int64_t blocks = rows.blocks + repack_blocks(r, rows);
   INT8_REQUIRE(tile.items < (int64_t{1} << 31) / i8::kMaxSplit && blocks < (int64_t{1} << 31), "INT8 gradient: too many tiles for one call.");
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks), tokens_grid = static_cast<unsigned>(rows.blocks);
-  const bool vec = whole_units(dy, dy_stride, tokens, w->rows, dtype) && aligned(w->scale, 16);
-#define CALL(D)                                                                                                            \
-  launch_rows(grid, s, rows, vec, v, r, tokens_grid, i8::scale_kernel<D, 1, 2, true>, i8::scale_kernel<D, 1, 4, true>,       \
-              i8::scale_kernel<D, 8, 2, true>, i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>,                          \
-              i8::scale_kernel<D, 1, 2, false>, i8::scale_kernel<D, 8, 2, false>)
+  const auto grid = static_cast<unsigned>(blocks);
+#define CALL(D)                                                                                                              \
+  constexpr int kHold = D == i8::kF32 ? 2 : 4;                                                                                \
+  launch_rows(grid, s, rows, vec, v, r, i8::scale_kernel<D, 1, kHold, true>, i8::scale_kernel<D, 2, kHold, true>,            \
+              i8::scale_kernel<D, 4, kHold, true>, i8::scale_kernel<D, 8, kHold, true>, i8::scale_kernel<D, 1, 2, false>,       \
+              i8::scale_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   cudaError_t e = launched();

@@ -17,7 +17,8 @@ namespace i8 {
 
 enum : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
 
-constexpr int kPrepareThreads = 256;
+// Threads of a block whose rows are worked on by so many warps: a row a warp, or a row a block.
+__host__ __device__ constexpr int prepare_threads(int warps) { return warps == 1 ? 256 : 32 * warps; }
 constexpr int kUnit = 16;  // values that a lane takes at once
 
 // Sixteen values as they lie in memory.
@@ -109,8 +110,8 @@ __device__ __forceinline__ int expert_of(const int32_t* ends, int experts, int r
 }
 
 // ------------------------------------------------------------------ rows of threads
-// A row is worked on by kWarps warps: one, eight rows a block, or all eight of a block. A lane holds the first kHold units
-// of its row in registers between the maximum and the codes, and reads the others again.
+// A row is worked on by kWarps warps: one, eight rows a block, or all of a block. A lane holds the first kHold units of its
+// row in registers between the maximum and the codes, and reads the others again.
 template <int kWarps>
 struct RowTeam {
   int64_t row;
@@ -118,27 +119,27 @@ struct RowTeam {
 
   __device__ __forceinline__ RowTeam(int64_t block) {
     if constexpr (kWarps == 1) {
-      row = block * (kPrepareThreads / 32) + (threadIdx.x >> 5);
+      row = block * 8 + (threadIdx.x >> 5);
       thread = threadIdx.x & 31;
     } else {
       row = block;
       thread = threadIdx.x;
     }
   }
-  // Of all the row's threads; `words` is shared memory of two uses of this function.
+  // Of all the row's threads; `words` is shared memory, eight words for each function.
   __device__ __forceinline__ uint32_t max_of(uint32_t v, uint32_t* words) const {
     v = __reduce_max_sync(0xFFFFFFFFu, v);
     if constexpr (kWarps == 1) return v;
     if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
     __syncthreads();
-    return __reduce_max_sync(0xFFFFFFFFu, words[threadIdx.x & 7]);
+    return __reduce_max_sync(0xFFFFFFFFu, words[threadIdx.x & (kWarps - 1)]);
   }
   __device__ __forceinline__ int sum_of(int v, uint32_t* words) const {
     v = __reduce_add_sync(0xFFFFFFFFu, v);
     if constexpr (kWarps == 1) return v;
     if ((threadIdx.x & 31) == 0) words[8 + (threadIdx.x >> 5)] = static_cast<uint32_t>(v);
     __syncthreads();
-    return __reduce_add_sync(0xFFFFFFFFu, (threadIdx.x & 31) < 8 ? static_cast<int>(words[8 + (threadIdx.x & 7)]) : 0);
+    return __reduce_add_sync(0xFFFFFFFFu, (threadIdx.x & 31) < kWarps ? static_cast<int>(words[8 + (threadIdx.x & (kWarps - 1))]) : 0);
   }
 };
 
@@ -394,22 +395,22 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t piece) {
 
 // The launch before a product: blocks of token rows, then of codes.
 template <int DT, int kWarps, int kHold, bool kVec>
-__global__ void __launch_bounds__(kPrepareThreads) quantize_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs r,
+__global__ void __launch_bounds__(prepare_threads(kWarps)) quantize_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs r,
                                                                    uint32_t token_blocks) {
   __shared__ uint32_t words[16];
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) quantize_rows<DT, kWarps, kHold, kVec>(q, blockIdx.x, words);
-  else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * kPrepareThreads + threadIdx.x);
+  else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);
 }
 
 // The launch before a gradient.
 template <int DT, int kWarps, int kHold, bool kVec>
-__global__ void __launch_bounds__(kPrepareThreads) scale_kernel(const __grid_constant__ ScaleArgs s, const __grid_constant__ RepackArgs r,
+__global__ void __launch_bounds__(prepare_threads(kWarps)) scale_kernel(const __grid_constant__ ScaleArgs s, const __grid_constant__ RepackArgs r,
                                                                 uint32_t token_blocks) {
   __shared__ uint32_t words[16];
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) scale_rows<DT, kWarps, kHold, kVec>(s, blockIdx.x, words);
-  else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * kPrepareThreads + threadIdx.x);
+  else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);
 }
 
 }  // namespace i8
