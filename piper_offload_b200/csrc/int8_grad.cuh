@@ -42,9 +42,9 @@ struct GradShape {
   static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 256;
   static constexpr int kThreads = 64 + 32 * kDecodeWarps * 2;  // producer warp, tensor-core warp, decoding warps
   static constexpr int kTurns = 2 / kRows;  // teams that take stages in turn
-  static constexpr int kAlloc = kRows * BN;
+  static constexpr int kAlloc = tmem_columns(kRows * BN);
   static constexpr bool kCanSplit = kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
-  static_assert(kAlloc >= 32 && kAlloc <= 512 && kStages >= 3, "the tile does not fit");
+  static_assert(kRows * BN <= kAlloc && kStages >= 3, "the tile does not fit");
 };
 
 // A thread's share of 64 rows x 128 columns: 32 codes of one row and the row's zero point.

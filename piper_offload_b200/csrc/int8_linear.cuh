@@ -44,8 +44,8 @@ struct LinearShape {
   static constexpr int kRoom = kSmemMax / kCtas - 2048 - kOut - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + kTokens + 1024 + 512;
-  static constexpr int kAlloc = 2 * BN;  // two accumulators
-  static_assert(kAlloc * kCtas <= 512 && kAlloc >= 32 && kStages >= 4, "the tile does not fit");
+  static constexpr int kAlloc = tmem_columns(2 * BN);  // two accumulators
+  static_assert(2 * BN <= kAlloc && kAlloc * kCtas <= 512 && kStages >= 4, "the tile does not fit");
   static_assert(BN * kTileRows * 4 <= kStages * kStage, "a tile's sums have to fit in the stages");
 };
 

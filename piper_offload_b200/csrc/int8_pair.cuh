@@ -22,8 +22,8 @@ struct PairShape {
   static constexpr int kRoom = kSmemMax - 2048 - kOut - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kOut + kTokens + 1024 + 512;
-  static constexpr int kAlloc = 2 * BN;  // two accumulators
-  static_assert(kAlloc <= 512 && kStages >= 4, "the tile does not fit");
+  static constexpr int kAlloc = tmem_columns(2 * BN);  // two accumulators
+  static_assert(2 * BN <= kAlloc && kStages >= 4, "the tile does not fit");
 };
 
 // signed 8-bit operands, both K-major, 32-bit sums, M = 256.

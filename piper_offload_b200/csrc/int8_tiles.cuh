@@ -9,6 +9,9 @@ using fp4::kSmemMax;
 using fp4::kTileRows;
 using fp4::TileAt;
 
+// Columns of tensor memory are allocated in powers of two from 32 on (any other number is an illegal instruction).
+__host__ __device__ constexpr int tmem_columns(int used) { return used <= 32 ? 32 : used <= 64 ? 64 : used <= 128 ? 128 : used <= 256 ? 256 : 512; }
+
 // kind::i8: signed 8-bit operands, both K-major, 32-bit sums, M = 128.
 __host__ __device__ constexpr uint32_t idesc_i8(uint32_t n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
