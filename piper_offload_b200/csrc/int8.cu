@@ -182,6 +182,12 @@ TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t 
   return best;
 }
 
+// Token tiles to expect: of one weight's tokens, or of experts' that end inside their last tiles.
+int64_t likely_tiles(int64_t batch, int64_t tokens, int64_t tile) {
+  if (batch == 1) return (tokens + tile - 1) / tile;
+  return std::max(std::min(batch, tokens), (tokens + tile * std::min(batch, tokens) / 2) / tile);
+}
+
 struct LinearPlan {
   int bn, split;
   bool pair;  // of SMs, on tiles of 256 outputs
@@ -194,7 +200,7 @@ LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
   const int64_t stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
   TilePlan best{};
-  const auto items_of = [&](int bn, int64_t outputs) { return std::min(w.batch, tokens) * ((per_expert + bn - 1) / bn) * ((w.rows + outputs - 1) / outputs); };
+  const auto items_of = [&](int bn, int64_t outputs) { return likely_tiles(w.batch, tokens, bn) * ((w.rows + outputs - 1) / outputs); };
   for (const int bn : {32, 128, 256}) {
     const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
     const TilePlan t = plan_tile(bn, items_of(bn, 128), stages, 300.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, sm_count());
@@ -290,35 +296,53 @@ GradPlan plan_grad(const piper_int8_matrix& w, int64_t tokens, int dtype) {
   return p;
 }
 
-// Tiles of a gradient: tokens x (rows x 128) columns. Decoding costs the same whatever the tokens, so tiles are as wide in
-// tokens as they go, but for a few, which leave room for more stages; 256 columns where that fills the SMs.
+// Tiles of a gradient: tokens x columns. Decoding costs the same whatever the tokens, so tiles are as wide in tokens as they
+// go, but for a few, which leave room for more stages. The rough account in cycles a stage is measured: one SM takes 810 for
+// 128 columns x 256 tokens and 560 for few, a pair 1330 for 512 x 256 and 750 for 256 x 256 (2048 x 14336 x 4096 200 us in
+// tiles of 512 on pairs, 222 of 256, on single SMs 220 of 256, 239 of 128; 512 x 4096 x 4096 28.4 on single SMs that share
+// sums, 34 on pairs).
 struct GradTile {
   int bn, rows, split;
+  bool pair;
+  int tokens;     // of a tile
   int64_t items;  // bound on the tiles
+  int columns() const { return 128 * rows * (pair ? 2 : 1); }
 };
 GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool grouped) {
-  const int64_t per_expert = tokens / w.batch;
-  GradTile t{256, 1, 1, 0};
-  if (per_expert <= 48) {
-    t.bn = 64;
-  } else {
-    const auto waves = [&](int64_t cols) {
-      const int64_t tiles = w.batch * ((per_expert + 255) / 256) * ((w.cols + cols - 1) / cols);
-      return static_cast<double>((tiles + sm_count() - 1) / sm_count());
-    };
-    if (waves(256) * 1060.0 <= waves(128) * 600.0) t.rows = 2;
-  }
-  t.items = token_tiles(tokens, grouped ? w.batch : 0, t.bn) * ((w.cols + 128 * t.rows - 1) / (128 * t.rows));
+  const int64_t per_expert = std::max<int64_t>(tokens / w.batch, 1);
   const int64_t stages = (w.rows + i8::kGradStageRows - 1) / i8::kGradStageRows * terms;
-  t.split = plan_tile(t.bn, t.items, stages, 600.0, std::min<int64_t>(tokens, t.bn), t.rows == 1 && !grouped, sm_count()).split;
+  GradTile t{per_expert <= 48 ? 64 : 256, 1, 1, false, 0, 0};
+  t.tokens = t.bn;
+  const auto tiles = [&](int64_t columns, int64_t tile) { return likely_tiles(w.batch, tokens, tile) * ((w.cols + columns - 1) / columns); };
+  const double one = std::max(560.0, 250.0 + 2.2 * static_cast<double>(std::min<int64_t>(per_expert, t.bn)));
+  const TilePlan alone = plan_tile(t.bn, tiles(128, t.bn), stages, one, std::min<int64_t>(per_expert, t.bn), !grouped, sm_count());
+  double best = alone.cycles;
+  if (t.bn == 256)
+    for (int rows = 1; rows <= 2; ++rows)
+      for (int tile = 256; tile >= 128; tile -= 32) {
+        const double n = static_cast<double>(std::min<int64_t>(up(per_expert, 32), tile));
+        const double stage = rows == 2 ? std::max(1000.0, 5.2 * n) : std::max(600.0, 2.95 * n);
+        const int64_t room = sm_count() / 2, waves = (tiles(256 * rows, tile) + room - 1) / room;
+        const double cycles = static_cast<double>(waves) * (static_cast<double>(stages) * stage + 2000.0);
+        if (cycles < best) {
+          best = cycles;
+          t.pair = true;
+          t.rows = rows;
+          t.tokens = tile;
+        }
+      }
+  t.items = token_tiles(tokens, grouped ? w.batch : 0, t.tokens) * ((w.cols + t.columns() - 1) / t.columns());
+  // the account goes by even experts: there may be more tiles, which then are not shared
+  if (!t.pair) t.split = plan_tile(t.bn, t.items, stages, one, std::min<int64_t>(tokens, t.bn), !grouped, sm_count()).split;
   return t;
 }
 
-template <int DT, int BN, int kRows>
+template <int DT, int BN, int kRows, bool kPair>
 cudaError_t launch_grad(const i8::GradArgs& args, int64_t items, cudaStream_t stream) {
-  using S = i8::GradShape<BN, kRows>;
-  static_assert(S::kCanSplit == (kRows == 1), "the plan splits tiles of 128 columns");
-  return launch<i8::GradArgs>(i8::grad_kernel<DT, BN, kRows>, args, items * args.split, S::kThreads, S::kSmem, args.split, stream);
+  using S = i8::GradShape<BN, kRows, kPair>;
+  static_assert(S::kCanSplit == !kPair, "the plan splits tiles that no pair has");
+  const int cluster = kPair ? 2 : args.split;
+  return launch<i8::GradArgs>(i8::grad_kernel<DT, BN, kRows, kPair>, args, items * cluster, S::kThreads, S::kSmem, cluster, stream);
 }
 
 #define INT8_DISPATCH(dtype, CALL)                              \
@@ -455,7 +479,7 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   a.codes = r.pieces > 0 ? r.out : static_cast<const uint8_t*>(w->codes);
   a.zero = static_cast<const int8_t*>(w->zero);
   a.back = v.back;
-  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + 128 * tile.rows - 1) / (128 * tile.rows))};
+  a.groups = {ends, tokens, static_cast<int32_t>(w->batch), static_cast<int32_t>((w->cols + tile.columns() - 1) / tile.columns())};
   a.dx = dx;
   a.code_pitch = code_pitch(*w);
   a.zero_step = w->per_row != 0 ? 1 : 0;
@@ -463,12 +487,13 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   a.cols = static_cast<int32_t>(w->cols);
   a.terms = p.terms;
   a.split = tile.split;
+  a.tile_tokens = tile.tokens;
   a.vec = aligned(dx, 16) && (w->cols * static_cast<int64_t>(width(dtype))) % 16 == 0;
   const bool vec = whole_units(dy, dy_stride, tokens, w->rows, dtype) && aligned(w->scale, 16);
   const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, dtype, vec);
   const int64_t blocks = rows.blocks + repack_blocks(r, rows);
   INT8_REQUIRE(tile.items < (int64_t{1} << 31) / i8::kMaxSplit && blocks < (int64_t{1} << 31), "INT8 gradient: too many tiles for one call.");
-  if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.bn))
+  if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.pair ? tile.bn / 2 : tile.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
 
   const auto grid = static_cast<unsigned>(blocks);
@@ -481,10 +506,10 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
 #undef CALL
   cudaError_t e = launched();
   if (e != cudaSuccess) return cuda_fail("scale kernel", e);
-#define CALL(D)                                                  \
-  e = tile.bn == 64     ? launch_grad<D, 64, 1>(a, tile.items, s)  \
-      : tile.rows == 1 ? launch_grad<D, 256, 1>(a, tile.items, s) \
-                       : launch_grad<D, 256, 2>(a, tile.items, s)
+#define CALL(D)                                                                                              \
+  e = tile.pair       ? (tile.rows == 2 ? launch_grad<D, 256, 2, true>(a, tile.items, s) : launch_grad<D, 256, 1, true>(a, tile.items, s)) \
+      : tile.bn == 64 ? launch_grad<D, 64, 1, false>(a, tile.items, s)                                         \
+                      : launch_grad<D, 256, 1, false>(a, tile.items, s)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("gradient kernel", e);
@@ -503,7 +528,7 @@ int piper_int8_grad_input_plan(const piper_int8_matrix* w, int64_t tokens, int32
   if (int rc = check_dtype(dtype)) return rc;
   INT8_REQUIRE(plan != nullptr && tokens > 0 && (grouped != 0 || w->batch == 1), "INT8 gradient: bad plan query.");
   const GradTile t = grad_tile(*w, tokens, grad_terms(dtype), grouped != 0);
-  *plan = {t.bn, 128 * t.rows, t.split, 1};
+  *plan = {t.tokens, t.columns(), t.split, 1};
   return PIPER_INT8_OK;
 }
 

@@ -6,6 +6,10 @@
 // kRows x 128 columns of w (the tensor core's 128-row operand, stored with its columns contiguous) x up to BN tokens; a
 // stage is 64 rows of w. Gradients come by bulk tensor copies; sixteen warps decode, loads two stages ahead: a byte
 // permute puts each code beside the exponent of 1024, and a packed difference takes 1024, the offset and the zero point off.
+//
+// Shared memory is what bounds it: for 256 columns x 256 tokens of a stage one SM brings in and reads 176 KB, 1375 cycles
+// at 128 bytes, for 1024 cycles of products. So many tokens run on pairs of SMs (kPair): each decodes 2 x 128 of a tile's
+// 512 columns and holds half of the tokens, which the tensor cores of both read: 128 KB for the same 1024 cycles.
 #pragma once
 #include <cuda.h>
 
@@ -28,63 +32,68 @@ struct GradArgs {
   int32_t rows, cols;   // of w
   int32_t terms;
   int32_t split;        // blocks of a cluster that share a tile's stages
+  int32_t tile_tokens;  // at most BN; of a pair a multiple of 32
   int32_t vec;          // rows of dx start on 16-byte boundaries
 };
 
-template <int BN, int kRows>
+template <int BN, int kRows, bool kPair>
 struct GradShape {
   static constexpr int kA = kRows * kGradStageRows * kTileRows * 2;
-  static constexpr int kB = BN * kGradStageRows * 2;
+  static constexpr int kB = (kPair ? BN / 2 : BN) * kGradStageRows * 2;
   static constexpr int kStage = kA + kB;
   static constexpr int kTokens = BN * 4;
   static constexpr int kRoom = kSmemMax - 3072 - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
-  static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 256;
+  static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 512;
   static constexpr int kThreads = 64 + 32 * kDecodeWarps * 2;  // producer warp, tensor-core warp, decoding warps
   static constexpr int kTurns = 2 / kRows;  // teams that take stages in turn
   static constexpr int kAlloc = tmem_columns(kRows * BN);
-  static constexpr bool kCanSplit = kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
+  static constexpr bool kCanSplit = !kPair && kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
   static_assert(kRows * BN <= kAlloc && kStages >= 3, "the tile does not fit");
 };
 
-// A thread's share of 64 rows x 128 columns: 32 codes of one row and the row's zero point.
+// A thread's share of 64 rows x 128 columns: 16 codes of a row, 16 of the fourth after it, and their zero points. The eight
+// lanes of a row load its 128 bytes together.
 struct Piece {
   uint4 codes[2];
-  int32_t zero;
+  int32_t zero[2];
 };
 
-// Walks down the weight in stages: this thread's row of each, 32 columns from `col` on.
+// Walks down the weight in stages: this thread's rows of each, 16 columns from `col` on.
 struct PieceWalk {
   const uint8_t* codes;
   const int8_t* zero;
-  int64_t code_step;  // to the next stage
-  int row, rows, bytes, zero_step;
+  int64_t second, step;  // bytes to the second row; to the next stage
+  int row, rows, zero_step;
+  bool there;
 
   __device__ __forceinline__ void begin(const GradArgs& p, int64_t expert, int block, int in_stage, int col) {
     row = block * kGradStageRows + in_stage;
     rows = p.rows;
-    bytes = p.code_pitch > col ? 32 : 0;  // the pitch is a multiple of 16, so a half may be missing
-    if (bytes != 0 && p.code_pitch - col < 32) bytes = 16;
+    there = col < p.code_pitch;  // the pitch is a multiple of 16
     const int64_t r = expert * p.rows + row;
-    codes = p.codes + r * p.code_pitch + (bytes > 0 ? col : 0);
-    code_step = kGradStageRows * p.code_pitch;
-    zero_step = kGradStageRows * p.zero_step;
+    codes = p.codes + r * p.code_pitch + (there ? col : 0);
+    second = 4 * p.code_pitch;
+    step = kGradStageRows * p.code_pitch;
+    zero_step = p.zero_step;
     zero = p.zero != nullptr ? p.zero + r * p.zero_step : nullptr;
   }
 
   __device__ __forceinline__ Piece load() const {
     // a code of zero where there is none
-    Piece out{{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, 0};
-    if (row >= rows) return out;
-    if (bytes >= 16) out.codes[0] = *reinterpret_cast<const uint4*>(codes);
-    if (bytes == 32) out.codes[1] = *reinterpret_cast<const uint4*>(codes + 16);
-    if (zero != nullptr) out.zero = *zero;
+    Piece out{{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, {0, 0}};
+    if (there && row < rows) out.codes[0] = *reinterpret_cast<const uint4*>(codes);
+    if (there && row + 4 < rows) out.codes[1] = *reinterpret_cast<const uint4*>(codes + second);
+    if (zero != nullptr) {
+      if (row < rows) out.zero[0] = *zero;
+      if (row + 4 < rows) out.zero[1] = zero[4 * zero_step];
+    }
     return out;
   }
 
   __device__ __forceinline__ void next() {
-    codes += code_step;
-    if (zero != nullptr) zero += zero_step;
+    codes += step;
+    if (zero != nullptr) zero += kGradStageRows * zero_step;
     row += kGradStageRows;
   }
 };
@@ -98,14 +107,23 @@ __device__ __forceinline__ void decode4(uint32_t codes, __half2 off, uint32_t& l
   hi = *reinterpret_cast<const uint32_t*>(&y);
 }
 
-template <int DT, int BN, int kRows>
-__global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel(const __grid_constant__ GradArgs p) {
-  using S = GradShape<BN, kRows>;
+// kind::f16 of a pair, M = 256.
+__device__ __forceinline__ void umma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int DT, int BN, int kRows, bool kPair>
+__global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad_kernel(const __grid_constant__ GradArgs p) {
+  using S = GradShape<BN, kRows, kPair>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
   float* token_scale = reinterpret_cast<float*>(smem + S::kStages * S::kStage);
-  uint64_t* full = reinterpret_cast<uint64_t*>(token_scale + BN);  // gradients landed
-  uint64_t* ready = full + S::kStages;                             // w decoded
+  uint64_t* full = reinterpret_cast<uint64_t*>(token_scale + BN);  // gradients landed (of a pair: both blocks', counted in the even one)
+  uint64_t* ready = full + S::kStages;                             // w decoded (the same)
   uint64_t* empty = ready + S::kStages;
   uint64_t* done = empty + S::kStages;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
@@ -115,47 +133,65 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1);
-      pm::mbar_init(&ready[s], kDecodeWarps * kRows);  // of one team, or of both halves'
+      pm::mbar_init(&ready[s], kDecodeWarps * kRows * (kPair ? 2 : 1));  // of one team, or of both halves'
       pm::mbar_init(&empty[s], 1);
     }
     pm::mbar_init(done, 1);
     pm::fence_mbar_init();
   } else if (warp == 1) {
-    pm::tmem_alloc(tmem_at, S::kAlloc);
-    pm::tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_at, S::kAlloc);
+    } else {
+      pm::tmem_alloc(tmem_at, S::kAlloc);
+      pm::tmem_relinquish();
+    }
   }
-  const int rank = p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
+  const uint32_t half = kPair ? fp4::cluster_rank() : 0u;  // of a pair
+  const int rank = !kPair && p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
+  const int sharers = kPair ? 2 : p.split;  // blocks with the same tile
   TileAt t;
-  const bool have = fp4::find_tile(p.groups, p.split > 1 ? blockIdx.x / p.split : blockIdx.x, BN, t);
+  const bool have = fp4::find_tile(p.groups, sharers > 1 ? blockIdx.x / sharers : blockIdx.x, p.tile_tokens, t);
   pm::tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) fp4::cluster_sync();  // both blocks' barriers are there
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
   const int blocks = (p.rows + kGradStageRows - 1) / kGradStageRows;  // of 64 rows of w
   const int all = blocks * p.terms;
-  const int from = p.split > 1 ? all * rank / p.split : 0, to = p.split > 1 ? all * (rank + 1) / p.split : all;
+  const int from = p.split > 1 && !kPair ? all * rank / p.split : 0, to = p.split > 1 && !kPair ? all * (rank + 1) / p.split : all;
   const bool sums = have && t.expert != p.groups.experts;
   const RowsOf none{};
+  // 128 columns of a tile: the h-th that this block decodes
+  const auto column_tile = [&](int h) { return kPair ? (t.row_tile * kRows + h) * 2 + static_cast<int>(half) : t.row_tile * kRows + h; };
+  // the tokens that a tile's products take: in sixteens, of a pair in thirty-twos
+  constexpr uint32_t kEach = kPair ? 32u : 16u;
+  const uint32_t computed = (static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t.count, 0)) + kEach - 1u) & ~(kEach - 1u);
   fp4::grid_wait();  // gradients, and codes that were laid out, come from the launch before
 
   if (have && !sums) {
     if (rank == 0)
       for (int h = 0; h < kRows; ++h) {
         TileAt part = t;
-        part.row_tile = t.row_tile * kRows + h;
+        part.row_tile = column_tile(h);
         zero_tile<DT>(p.dx, part, p.cols, threadIdx.x, S::kThreads);
       }
   } else if (sums) {
     if (warp == 0) {
-      const int first = __shfl_sync(0xFFFFFFFFu, t.first, 0);
+      const int first = __shfl_sync(0xFFFFFFFFu, t.first, 0) + static_cast<int>(half * (computed / 2));
       int issued = 0;
       if (fp4::elect_one()) {
         fp4::Ring<S::kStages> ring;
         int block = from % blocks, row = first + from / blocks * static_cast<int>(p.groups.tokens);
         for (int i = from; i < to; ++i, ring.next()) {
           if (issued >= S::kStages && !pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad)) break;
-          pm::mbar_arrive_expect_tx(&full[ring.slot], S::kB);
-          pm::tma_load_2d(smem + ring.slot * S::kStage + S::kA, &p.dy_map, block * kGradStageRows, row, &full[ring.slot]);
+          uint8_t* at = smem + ring.slot * S::kStage + S::kA;
+          if constexpr (kPair) {
+            if (half == 0) pm::mbar_arrive_expect_tx(&full[ring.slot], 2 * S::kB);
+            tma_load_2d_pair(at, &p.dy_map, block * kGradStageRows, row, in_block(pm::smem_u32(&full[ring.slot]), 0));
+          } else {
+            pm::mbar_arrive_expect_tx(&full[ring.slot], S::kB);
+            pm::tma_load_2d(at, &p.dy_map, block * kGradStageRows, row, &full[ring.slot]);
+          }
           ++issued;
           if (++block == blocks) {  // the next term
             block = 0;
@@ -166,12 +202,13 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
       __syncwarp();
       issued = __reduce_max_sync(0xFFFFFFFFu, issued);
       // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
-      for (int i = max(0, issued - S::kStages); i < issued; ++i)
-        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+      if (half == 0)
+        for (int i = max(0, issued - S::kStages); i < issued; ++i)
+          pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
       __syncwarp();
     } else if (warp == 1) {
-      const uint32_t idesc = idesc_grad((static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, t.count, 0)) + 15u) & ~15u);
-      if (fp4::elect_one()) {
+      const uint32_t idesc = idesc_grad(computed, kPair ? 256u : 128u);
+      if (half == 0 && fp4::elect_one()) {
         fp4::Ring<S::kStages> ring;
         for (int i = from; i < to; ++i, ring.next()) {
           if (!pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma) ||
@@ -185,23 +222,25 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
 #pragma unroll
           for (int j = 0; j < kGradStageRows / 16; ++j)
 #pragma unroll
-            for (int h = 0; h < kRows; ++h)
-              pm::umma_f16(tmem + h * BN, a + h * (kGradStageRows * kTileRows * 2 >> 4) + j * (2048 >> 4), b + j * (32 >> 4), idesc,
-                           i != from || j != 0);
-          pm::umma_commit(&empty[ring.slot]);
+            for (int h = 0; h < kRows; ++h) {
+              const uint64_t ah = a + h * (kGradStageRows * kTileRows * 2 >> 4) + j * (2048 >> 4), bj = b + j * (32 >> 4);
+              if constexpr (kPair) umma_f16_pair(tmem + h * BN, ah, bj, idesc, i != from || j != 0);
+              else pm::umma_f16(tmem + h * BN, ah, bj, idesc, i != from || j != 0);
+            }
+          if constexpr (kPair) umma_commit_pair(&empty[ring.slot]);
+          else pm::umma_commit(&empty[ring.slot]);
         }
-        pm::umma_commit(done);
+        if constexpr (kPair) umma_commit_pair(done);
+        else pm::umma_commit(done);
       }
       __syncwarp();
     } else {
-      // a team has 128 columns of every stage, or of every second one: a warp decodes eight rows, a lane 32 columns of
-      // one, and the eight lanes whose 16-byte stores go together write different rows, so the swizzle gives them
-      // different banks
+      // a team has 128 columns of every stage, or of every second one: a warp decodes eight rows, eight lanes a row
       const int team = (warp - 2) / kDecodeWarps;
       const int h = kRows == 2 ? team : 0, turn = kRows == 2 ? 0 : team;
-      const int r = (warp - 2) % kDecodeWarps * 8 + (lane & 7), quarter = lane >> 3;
-      const int col = (t.row_tile * kRows + h) * kTileRows + quarter * 32;
-      uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (quarter >> 1) * (kGradStageRows * 128) + r * 128;
+      const int r = (warp - 2) % kDecodeWarps * 8 + (lane >> 3), chunk = lane & 7;
+      const int col = column_tile(h) * kTileRows + chunk * 16;
+      uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (chunk >> 2) * (kGradStageRows * 128) + r * 128;
       PieceWalk walk;
       int block = (from + turn) % blocks;  // of the next loads
       walk.begin(p, t.expert, block, r, col);
@@ -230,19 +269,28 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
           ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad));
           if (!ok) break;
         }
-        uint8_t* row = to_row + ring.slot * S::kStage;
-        const __half2 off = __half2half2(__int2half_rn(1152 + now.zero));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint4& c = now.codes[q >> 1];
-          uint4 v;
-          decode4(q & 1 ? c.z : c.x, off, v.x, v.y);
-          decode4(q & 1 ? c.w : c.y, off, v.z, v.w);
-          *reinterpret_cast<uint4*>(row + ((((quarter & 1) * 4 + q) ^ (r & 7)) << 4)) = v;
+        for (int q = 0; q < 2; ++q) {
+          const __half2 off = __half2half2(__int2half_rn(1152 + now.zero[q]));
+          uint4 lo, hi;
+          decode4(now.codes[q].x, off, lo.x, lo.y);
+          decode4(now.codes[q].y, off, lo.z, lo.w);
+          decode4(now.codes[q].z, off, hi.x, hi.y);
+          decode4(now.codes[q].w, off, hi.z, hi.w);
+          // 16-byte pieces 2 (chunk % 4) and the next, XORed with the row; the lanes of one 64-column block begin with the
+          // first and those of the other with the second, so that the eight of a row write to different banks
+          uint8_t* row = to_row + ring.slot * S::kStage + q * 4 * 128;
+          const int at = (chunk & 3) * 2, swizzle = (r + q * 4) & 7;
+          const bool other = chunk >= 4;
+          *reinterpret_cast<uint4*>(row + (((at + other) ^ swizzle) << 4)) = other ? hi : lo;
+          *reinterpret_cast<uint4*>(row + (((at + !other) ^ swizzle) << 4)) = other ? lo : hi;
         }
         pm::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) pm::mbar_arrive(&ready[ring.slot]);
+        if (lane == 0) {
+          if constexpr (kPair) mbar_arrive_pair(in_block(pm::smem_u32(&ready[ring.slot]), 0));
+          else pm::mbar_arrive(&ready[ring.slot]);
+        }
 #pragma unroll
         for (int j = 0; j < S::kTurns; ++j) ring.next();
       }
@@ -256,7 +304,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
         } else {
           uint8_t* mine = smem + (warp - 2) * 2048;
           TileAt part = t;
-          part.row_tile = t.row_tile * kRows + h;
+          part.row_tile = column_tile(h);
           // 4 / kRows warps for each quarter of the lanes: a share of the tokens each
           constexpr int kShare = BN * kRows / 4 < 32 ? 32 : BN * kRows / 4;
           const int share = (kRows == 2 ? (warp - 2) % kDecodeWarps : warp - 2) / 4;
@@ -277,9 +325,11 @@ __global__ void __launch_bounds__(GradShape<BN, kRows>::kThreads, 1) grad_kernel
     fp4::cluster_sync();  // nobody's shared memory goes while others read it
   }
   __syncthreads();
+  if constexpr (kPair) fp4::cluster_sync();  // nobody's shared or tensor memory goes while the other block uses it
   if (warp == 1) {
     pm::tc_fence_after();
-    pm::tmem_dealloc(tmem, S::kAlloc);
+    if constexpr (kPair) tmem_dealloc_pair(tmem, S::kAlloc);
+    else pm::tmem_dealloc(tmem, S::kAlloc);
   }
 }
 

@@ -37,66 +37,6 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d, uint64_t a, uint64_t b,
       : "memory");
 }
 
-// Arrive once on the barrier at this place in both blocks when every product issued before is done.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(pm::smem_u32(bar)),
-               "h"(static_cast<uint16_t>(3))
-               : "memory");
-}
-
-// A tile into this block's shared memory, counted on the barrier at `bar` of the cluster's address space: the even block's.
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-          "r"(pm::smem_u32(dst)),
-      "l"(tmap), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-
-// The cluster's address of this block's shared-memory address in block `rank`.
-__device__ __forceinline__ uint32_t in_block(uint32_t saddr, uint32_t rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
-  return remote;
-}
-
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// mbar_wait for arrivals that come from the other block too.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, unsigned int code) {
-  const auto try_wait = [&]() {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(pm::smem_u32(bar)), "r"(parity), "r"(pm::kSuspendHintNs)
-        : "memory");
-    return ok != 0;
-  };
-  if (try_wait()) return true;
-  const uint64_t t0 = pm::global_timer_ns();
-  for (uint32_t spin = 0;; ++spin) {
-    if (try_wait()) return true;
-    if ((spin & 63u) == 63u && pm::global_timer_ns() - t0 > pm::kWaitLimitNs) {
-      atomicOr(&pm::g_status, code);
-      return false;
-    }
-  }
-}
-
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pm::smem_u32(dst)), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-
 // Persistent pairs of blocks (a cluster of two). Row tiles: of 256 outputs.
 template <int DT, int BN>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __grid_constant__ LinearArgs p) {
@@ -169,7 +109,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
           for (int j = 0; j < ahead; ++j, ++i, ++it, ring.next()) load_x(i, j);
         }
         for (; i < stages; ++i, ++it, ring.next()) {
-          ok = it < S::kStages || mbar_wait_cluster(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+          ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
           if (!ok) break;
           load_w(i, ring.slot);
           load_x(i, ring.slot);
@@ -186,7 +126,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
     // the last copies of both blocks land before either's shared memory goes, even if the tensor-core warp gave up
     if (rank == 0)
       for (int i = max(0, it - S::kStages); i < it; ++i)
-        mbar_wait_cluster(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
     __syncwarp();
   } else if (warp == 1 && rank == 0) {
     fp4::Ring<S::kStages> ring;
@@ -198,10 +138,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
       const uint32_t d = tmem + b * BN;
       const uint32_t idesc = idesc_i8_pair(computed(__shfl_sync(0xFFFFFFFFu, t.count, 0)));
       if (fp4::elect_one()) {
-        ok = n < 2 || mbar_wait_cluster(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
+        ok = n < 2 || pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
         pm::tc_fence_after();
         for (int i = 0; ok && i < stages; ++i, ++it, ring.next()) {
-          ok = mbar_wait_cluster(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+          ok = pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
           if (!ok) break;
           pm::tc_fence_after();
           const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
@@ -240,14 +180,14 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
       }
       pm::named_bar_sync(1, 128);
       const int b = n & 1;
-      const bool ok = mbar_wait_cluster(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
+      const bool ok = pm::mbar_wait(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
       if (!pm::named_bar_and(2, 128, ok)) break;
       pm::tc_fence_after();
       store_tile<DT, true>(tmem + b * BN, p.y, half, p.rows, p.rows_of, static_cast<int64_t>(t.expert) * p.rows, token_scale, token_sum, 0, BN,
                            mine, p.vec != 0);
       pm::tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(in_block(pm::smem_u32(&acc_empty[b]), 0));
+      if (lane == 0) mbar_arrive_pair(in_block(pm::smem_u32(&acc_empty[b]), 0));
       ++n;
     }
   }

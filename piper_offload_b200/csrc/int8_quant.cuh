@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "fp4_ptx.cuh"
 
@@ -264,30 +265,28 @@ struct ScaleArgs {
   int32_t experts;
 };
 
-// The scales of sixteen rows of the weight from `n` on, 0 past the last. A lane takes them as it takes its values.
-template <int DT, bool kVec>
-__device__ __forceinline__ void unit_scales(const void* scale, int64_t row0, int n, int rows, float (&s)[kUnit]) {
-  const uint8_t* from = static_cast<const uint8_t*>(scale) + row0 * (DT == kF32 ? 4 : 2);
-  const Unit<DT> u = load_unit<DT, kVec>(from, n, rows);
-#pragma unroll
-  for (int i = 0; i < kUnit; ++i) s[i] = unit_value<DT>(u, i);
-}
-
-template <bool kVec>
-__device__ __forceinline__ void scales_of(const ScaleArgs& p, int64_t row0, int n, float (&s)[kUnit]) {
+// Sixteen values times the scales of the weight's rows from `n` on, 0 past the last. A lane takes scales as it takes values.
+template <int DT, int SDT, bool kVec>
+__device__ __forceinline__ void scaled_unit(const ScaleArgs& p, const Unit<DT>& u, int64_t row0, int n, float (&v)[kUnit]) {
   if (p.scales.step == 0) {
     const float one = row_scale(p.scales, 0);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) s[i] = n + i < p.rows ? one : 0.0f;
+    for (int i = 0; i < kUnit; ++i) v[i] = n + i < p.rows ? unit_value<DT>(u, i) * one : 0.0f;
     return;
   }
-  if (p.scales.dtype == kBF16) unit_scales<kBF16, kVec>(p.scales.scale, row0, n, p.rows, s);
-  else if (p.scales.dtype == kF16) unit_scales<kF16, kVec>(p.scales.scale, row0, n, p.rows, s);
-  else unit_scales<kF32, kVec>(p.scales.scale, row0, n, p.rows, s);
-  if (p.scales.over_127 != 0) {
+  const Unit<SDT> s = load_unit<SDT, kVec>(static_cast<const uint8_t*>(p.scales.scale) + row0 * (SDT == kF32 ? 4 : 2), n, p.rows);
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) s[i] = __fdiv_rn(s[i], 127.0f);
+  for (int i = 0; i < kUnit; ++i) {
+    const float scale = unit_value<SDT>(s, i);
+    v[i] = unit_value<DT>(u, i) * (p.scales.over_127 != 0 ? __fdiv_rn(scale, 127.0f) : scale);
   }
+}
+
+template <int DT, bool kVec>
+__device__ __forceinline__ void scaled_unit_any(const ScaleArgs& p, const Unit<DT>& u, int64_t row0, int n, float (&v)[kUnit]) {
+  if (p.scales.dtype == kBF16) scaled_unit<DT, kBF16, kVec>(p, u, row0, n, v);
+  else if (p.scales.dtype == kF16) scaled_unit<DT, kF16, kVec>(p, u, row0, n, v);
+  else scaled_unit<DT, kF32, kVec>(p, u, row0, n, v);
 }
 
 template <int DT, int kWarps, int kHold, bool kVec>
@@ -300,44 +299,60 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
   const uint8_t* row = static_cast<const uint8_t*>(p.dy) + team.row * p.dy_stride * (DT == kF32 ? 4 : 2);
   const int units = static_cast<int>(p.pitch / kUnit);
-  Unit<DT> held[kHold];
-  float top = 0.0f;
-  const auto see = [&](const Unit<DT>& u, int unit, bool finite) {
-    float s[kUnit];
-    scales_of<kVec>(p, row0, unit * kUnit, s);
-#pragma unroll
-    for (int i = 0; i < kUnit; ++i) {
-      const float v = fabsf(unit_value<DT>(u, i) * s[i]);
-      top = fmaxf(top, finite && !(v < INFINITY) ? 0.0f : v);  // a NaN is not counted
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) held[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
-  const auto see_all = [&](bool finite) {
+  const int first_loose = team.thread + kHold * kStep;
+  // the first units stay in registers as products
+  float held[kHold][kUnit];
+  const auto load_held = [&](auto scale_type) {
+    constexpr int SDT = decltype(scale_type)::value;
+    Unit<DT> u[kHold];
 #pragma unroll
     for (int k = 0; k < kHold; ++k)
-      if (team.thread + k * kStep < units) see(held[k], team.thread + k * kStep, finite);
-    for (int u = team.thread + kHold * kStep; u < units; u += kStep) see(load_unit<DT, kVec>(row, u * kUnit, p.rows), u, finite);
+      if (team.thread + k * kStep < units) u[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      if (team.thread + k * kStep < units) {
+        scaled_unit<DT, SDT, kVec>(p, u[k], row0, (team.thread + k * kStep) * kUnit, held[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) held[k][i] = 0.0f;
+      }
+    }
   };
-  see_all(false);
-  uint32_t bits = team.max_of(__float_as_uint(top), words);
+  if (p.scales.dtype == kBF16) load_held(std::integral_constant<int, kBF16>{});
+  else if (p.scales.dtype == kF16) load_held(std::integral_constant<int, kF16>{});
+  else load_held(std::integral_constant<int, kF32>{});
+  const auto loose = [&](int unit, float (&v)[kUnit]) {
+    scaled_unit_any<DT, kVec>(p, load_unit<DT, kVec>(row, unit * kUnit, p.rows), row0, unit * kUnit, v);
+  };
+  // the largest magnitude that is a number; infinities only cost a second look
+  const auto largest = [&](bool finite) {
+    float top = 0.0f;
+    const auto see = [&](const float (&v)[kUnit]) {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) top = fmaxf(top, finite && !(fabsf(v[i]) < INFINITY) ? 0.0f : fabsf(v[i]));  // a NaN is not counted
+    };
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) see(held[k]);
+    for (int u = first_loose; u < units; u += kStep) {
+      float v[kUnit];
+      loose(u, v);
+      see(v);
+    }
+    return team.max_of(__float_as_uint(top), words);
+  };
+  uint32_t bits = largest(false);
   if (bits == __float_as_uint(INFINITY)) {
-    top = 0.0f;
-    see_all(true);
     if constexpr (kWarps > 1) __syncthreads();  // the words are read
-    bits = team.max_of(__float_as_uint(top), words);
+    bits = largest(true);
   }
   // 2^(14 - exponent), within fp32's normal numbers; 1 for a row of zeros
   const int exponent = bits == 0u ? 14 : max(static_cast<int>(bits >> 23) - 127, -112);
   const float power = __uint_as_float(static_cast<uint32_t>(141 - exponent) << 23);
-  const auto write = [&](const Unit<DT>& u, int unit) {
-    float s[kUnit];
-    scales_of<kVec>(p, row0, unit * kUnit, s);
+  const auto write = [&](const float (&v)[kUnit], int unit) {
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
-      const float a = unit_value<DT>(u, i) * s[i] * power, b = unit_value<DT>(u, i + 1) * s[i + 1] * power;
+      const float a = v[i] * power, b = v[i + 1] * power;
       const __half2 h = __floats2half2_rn(a, b);
       hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
       if constexpr (DT == kF32) {
@@ -358,7 +373,11 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
     if (team.thread + k * kStep < units) write(held[k], team.thread + k * kStep);
-  for (int u = team.thread + kHold * kStep; u < units; u += kStep) write(load_unit<DT, kVec>(row, u * kUnit, p.rows), u);
+  for (int u = first_loose; u < units; u += kStep) {
+    float v[kUnit];
+    loose(u, v);
+    write(v, u);
+  }
   if (team.thread == 0) p.back[team.row] = __uint_as_float(static_cast<uint32_t>(113 + exponent) << 23);
 }
 

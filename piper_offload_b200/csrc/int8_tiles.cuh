@@ -25,8 +25,48 @@ __device__ __forceinline__ void umma_i8(uint32_t d, uint64_t a, uint64_t b, uint
       : "memory");
 }
 
-// kind::f16: fp16 operands, fp32 sums, A stored M-major (bit 15), B K-major, M = 128.
-__host__ __device__ constexpr uint32_t idesc_grad(uint32_t n) { return (1u << 4) | (1u << 15) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
+// kind::f16: fp16 operands, fp32 sums, A stored M-major (bit 15), B K-major.
+__host__ __device__ constexpr uint32_t idesc_grad(uint32_t n, uint32_t m) { return (1u << 4) | (1u << 15) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+// ------------------------------------------------------------ pairs of SMs (cta_group::2)
+// Arrive once on the barrier at this place in both blocks when every product issued before is done.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(pm::smem_u32(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+
+// A tile into this block's shared memory, counted on the barrier at `bar` of the cluster's address space: the even block's.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(pm::smem_u32(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// The cluster's address of this block's shared-memory address in block `rank`.
+__device__ __forceinline__ uint32_t in_block(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  return remote;
+}
+
+// One arrival on the barrier at `bar` of the cluster's address space. What the arriving block wrote to its own shared
+// memory before is there when the products that follow the wait read it in that block. (A release over the cluster makes
+// the thread wait for its loads under way too: the gradient's decoding warps took 318 us with it, 2048 x 14336 x 4096.)
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pm::smem_u32(dst)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
 
 template <int DT>
 __device__ __forceinline__ void store_value(void* y, int64_t at, float v) {
