@@ -128,21 +128,23 @@ i8::RepackArgs repack_args(const piper_int8_matrix& w, uint8_t* out) {
   return r;
 }
 
-// Warps that work on a row of `units` units: as few as hold it in their registers, four units a lane (two of fp32), so that
-// rows wait for few others (4096 x 4096 bf16 to codes: 10.4 us with two warps, 14.3 with one or eight; x 8192 18.5 with
-// four, 27.4 with one, 20.5 with eight; x 14336 30.8 with eight, 36.9 with four); eight where there are too few rows for
-// all SMs, or where rows have no whole units.
+// Warps that work on a row of `units` units: as few as hold it in their registers, `lane` units a lane, so that rows wait
+// for few others; eight where there are too few rows for all SMs, or where rows have no whole units. bf16 to codes, four
+// units a lane: 4096 x 4096 10.4 us with two warps, 14.3 with one or eight; x 8192 18.5 with four, 27.4 with one, 20.5 with
+// eight; x 14336 30.8 with eight, 36.9 with four. bf16 gradients, two a lane while that is enough: 2048 x 4096 10.3 us with
+// four warps, 12.3 with two or eight; x 8192 16.5 with eight, 20.0 with four; x 14336 31.9 with eight and four units, 34.4
+// with two.
 struct RowPlan {
   int warps;
   int64_t blocks;
+  bool more;  // rows longer than two units a lane of eight warps
 };
-RowPlan plan_rows(int64_t rows, int64_t units, int dtype, bool vec) {
-  const int64_t lane = dtype == PIPER_INT8_F32 ? 2 : 4;
+RowPlan plan_rows(int64_t rows, int64_t units, int64_t lane, bool vec) {
   int warps = 1;
   while (warps < 8 && units > 32 * lane * warps) warps *= 2;
   if (units > 64 && (rows < 8 * sm_count() || !vec)) warps = 8;
   if (!vec && units <= 64) warps = 1;
-  return {warps, warps == 1 ? (rows + 7) / 8 : rows};
+  return {warps, warps == 1 ? (rows + 7) / 8 : rows, units > 512};
 }
 
 // Rows that start on 16-byte boundaries and have whole units.
@@ -152,8 +154,13 @@ bool whole_units(const void* p, int64_t stride, int64_t rows, int64_t cols, int 
 
 template <class Args, class Kernel>
 void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, Kernel one, Kernel two,
-                 Kernel four, Kernel eight, Kernel one_any, Kernel eight_any) {
-  const Kernel kernel = !vec ? (rows.warps == 1 ? one_any : eight_any) : rows.warps == 1 ? one : rows.warps == 2 ? two : rows.warps == 4 ? four : eight;
+                 Kernel four, Kernel eight, Kernel eight_more, Kernel one_any, Kernel eight_any) {
+  const Kernel kernel = !vec              ? (rows.warps == 1 ? one_any : eight_any)
+                        : rows.warps == 1 ? one
+                        : rows.warps == 2 ? two
+                        : rows.warps == 4 ? four
+                        : rows.more       ? eight_more
+                                          : eight;
   kernel<<<grid, i8::prepare_threads(rows.warps), 0, s>>>(args, r, static_cast<unsigned>(rows.blocks));
 }
 
@@ -169,14 +176,16 @@ struct TilePlan {
 };
 
 // Blocks of a cluster that share a tile's stages, by a rough account in cycles: a stage takes `stage`, leaving sums and
-// adding them up 2500 and 30 for each token of the tile, and every wave of tiles 2000.
+// adding them up 2500 and 80 for each token of the tile, and every wave of tiles 2000. Shared by four against not shared: 1 x
+// 4096 x 4096 9.5 and 11.1 us, 24 tokens 9.9 and 11.2, 8 x 4096 x 14336 16.2 and 23.0, 128 x 4096 x 4096 in tiles of 128
+// 14.6 and 14.1.
 TilePlan plan_tile(int bn, int64_t items, int64_t stages, double stage, int64_t tile_tokens, bool can_split, int64_t room) {
   TilePlan best{bn, 1, 0.0};
   for (int split = 1; split <= (can_split ? i8::kMaxSplit : 1); split *= 2) {
     if (split > 1 && (items * split > room || stages < 2 * split)) break;
     const int64_t waves = (items * split + room - 1) / room;
     double cycles = static_cast<double>(waves) * (static_cast<double>((stages + split - 1) / split) * stage + 2000.0);
-    if (split > 1) cycles += 2500.0 + 30.0 * static_cast<double>(tile_tokens);
+    if (split > 1) cycles += 2500.0 + 80.0 * static_cast<double>(tile_tokens);
     if (split == 1 || cycles < best.cycles) best = {bn, split, cycles};
   }
   return best;
@@ -190,10 +199,16 @@ int64_t likely_tiles(int64_t batch, int64_t tokens, int64_t tile) {
 
 struct LinearPlan {
   int bn, split;
-  bool pair;  // of SMs, on tiles of 256 outputs
+  bool pair;   // of SMs, on tiles of 256 outputs
+  int blocks;  // on an SM
   int64_t x_pitch;
   int64_t x_codes, x_scale, x_sums, w_codes, total;  // byte offsets
 };
+
+// Whether two blocks share an SM, one starting or ending while the other streams: in small tiles, once there are more of them
+// than SMs, and where blocks share sums (16 rows of 8 experts of 14336 x 4096 74.5 us, 76.6 with one block; 1024 rows of 32 of
+// 2048 x 2048 31.4 and 35.4; 1 x 4096 x 4096 shared by four 9.5 and 10.1, but 24 x 4096 x 4096 not shared 11.7 and 11.2).
+bool two_blocks(int bn, int64_t items, int split) { return bn <= 64 && (items > sm_count() || (bn == 32 && split > 1)); }
 
 LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
   LinearPlan p{};
@@ -201,18 +216,29 @@ LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
   const int64_t stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
   TilePlan best{};
   const auto items_of = [&](int bn, int64_t outputs) { return likely_tiles(w.batch, tokens, bn) * ((w.rows + outputs - 1) / outputs); };
-  for (const int bn : {32, 128, 256}) {
-    const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn);
-    const TilePlan t = plan_tile(bn, items_of(bn, 128), stages, 300.0 + 2.0 * static_cast<double>(tile_tokens), tile_tokens, w.batch == 1, sm_count());
-    if (best.bn == 0 || t.cycles < best.cycles) best = t;
+  for (const int bn : {32, 64, 128, 256}) {
+    // experts' weights stream from HBM: narrower tiles leave room for more of it under way (4096 rows of 32 experts of 2048 x
+    // 2048 37.6 us in tiles of 128, 39.8 of 256)
+    if (w.batch > 1 && bn == 256 && per_expert <= 192) break;
+    const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 16), bn), items = items_of(bn, 128);
+    const int blocks = two_blocks(bn, items, 1) ? 2 : 1;
+    const double stage = (300.0 + 2.0 * static_cast<double>(tile_tokens)) * (blocks == 2 ? 1.7 : 1.0);
+    const TilePlan t = plan_tile(bn, items, stages, stage, tile_tokens, w.batch == 1 && blocks == 1, blocks * sm_count());
+    if (best.bn == 0 || t.cycles < best.cycles) {
+      best = t;
+      p.blocks = two_blocks(bn, items, t.split) ? 2 : 1;
+    }
   }
+  // 4096 x 14336 x 4096 163 us on pairs, 184 on single SMs; 2048 x 4096 x 4096 34.0 and 35.0, 1024 23.9 and 23.5; 4096 rows
+  // of 8 experts of 4096 x 2048 48.5 and 47.1
   for (const int bn : {128, 256}) {
-    if (per_expert <= 64) break;
+    if (per_expert <= (w.batch == 1 ? 256 : 512)) break;
     const int64_t tile_tokens = std::min<int64_t>(up(per_expert, 32), bn);
     const TilePlan t = plan_tile(bn, items_of(bn, 256), stages, 290.0 + static_cast<double>(tile_tokens), tile_tokens, false, sm_count() / 2);
     if (t.cycles < best.cycles) {
       best = t;
       p.pair = true;
+      p.blocks = 1;
     }
   }
   p.bn = best.bn;
@@ -259,10 +285,10 @@ cudaError_t launch(void (*kernel)(Args), const Args& args, int64_t blocks, int t
   return e == cudaSuccess ? launched() : e;
 }
 
-template <int DT, int BN>
+template <int DT, int BN, int kCtas>
 cudaError_t launch_linear(const i8::LinearArgs& args, int64_t items, cudaStream_t stream) {
-  using S = i8::LinearShape<BN, 1>;
-  return launch<i8::LinearArgs>(i8::linear_kernel<DT, BN, 1>, args, args.split > 1 ? items * args.split : std::min<int64_t>(items, sm_count()),
+  using S = i8::LinearShape<BN, kCtas>;
+  return launch<i8::LinearArgs>(i8::linear_kernel<DT, BN, kCtas>, args, args.split > 1 ? items * args.split : std::min<int64_t>(items, kCtas * sm_count()),
                                 i8::kLinearThreads, S::kSmem, args.split, stream);
 }
 
@@ -411,7 +437,7 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   a.items = static_cast<int32_t>(items);
   INT8_REQUIRE(items < (int64_t{1} << 31) / i8::kMaxSplit, "INT8 product: too many tiles for one call.");
   const bool vec = whole_units(x, x_stride, tokens, w->cols, dtype);
-  const RowPlan rows = plan_rows(tokens, p.x_pitch / i8::kUnit, dtype, vec);
+  const RowPlan rows = plan_rows(tokens, p.x_pitch / i8::kUnit, dtype == PIPER_INT8_F32 ? 2 : 4, vec);
   const int64_t blocks = rows.blocks + repack_blocks(r, rows);
   INT8_REQUIRE(blocks < (int64_t{1} << 31), "INT8 product: too many values for one call.");
   const void* codes = r.pieces > 0 ? r.out : w->codes;
@@ -423,17 +449,19 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
 #define CALL(D)                                                                                                              \
   constexpr int kHold = D == i8::kF32 ? 2 : 4;                                                                                \
   launch_rows(grid, s, rows, vec, q, r, i8::quantize_kernel<D, 1, kHold, true>, i8::quantize_kernel<D, 2, kHold, true>,            \
-              i8::quantize_kernel<D, 4, kHold, true>, i8::quantize_kernel<D, 8, kHold, true>, i8::quantize_kernel<D, 1, 2, false>,       \
+              i8::quantize_kernel<D, 4, kHold, true>, i8::quantize_kernel<D, 8, 2, true>, i8::quantize_kernel<D, 8, kHold, true>,  \
+              i8::quantize_kernel<D, 1, 2, false>,                                                                            \
               i8::quantize_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   cudaError_t e = launched();
   if (e != cudaSuccess) return cuda_fail("quantize kernel", e);
-#define CALL(D)                                           \
-  e = p.pair        ? (p.bn == 128 ? launch_pairs<D, 128>(a, items, s) : launch_pairs<D, 256>(a, items, s)) \
-      : p.bn == 32  ? launch_linear<D, 32>(a, items, s)   \
-      : p.bn == 128 ? launch_linear<D, 128>(a, items, s)  \
-                    : launch_linear<D, 256>(a, items, s)
+#define CALL(D)                                                                                                          \
+  e = p.pair        ? (p.bn == 128 ? launch_pairs<D, 128>(a, items, s) : launch_pairs<D, 256>(a, items, s))                \
+      : p.bn == 32  ? (p.blocks == 2 ? launch_linear<D, 32, 2>(a, items, s) : launch_linear<D, 32, 1>(a, items, s))        \
+      : p.bn == 64  ? (p.blocks == 2 ? launch_linear<D, 64, 2>(a, items, s) : launch_linear<D, 64, 1>(a, items, s))        \
+      : p.bn == 128 ? launch_linear<D, 128, 1>(a, items, s)                                                                \
+                    : launch_linear<D, 256, 1>(a, items, s)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
   return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("linear kernel", e);
@@ -490,7 +518,7 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   a.tile_tokens = tile.tokens;
   a.vec = aligned(dx, 16) && (w->cols * static_cast<int64_t>(width(dtype))) % 16 == 0;
   const bool vec = whole_units(dy, dy_stride, tokens, w->rows, dtype) && aligned(w->scale, 16);
-  const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, dtype, vec);
+  const RowPlan rows = plan_rows(tokens, p.pitch / i8::kUnit, 2, vec);
   const int64_t blocks = rows.blocks + repack_blocks(r, rows);
   INT8_REQUIRE(tile.items < (int64_t{1} << 31) / i8::kMaxSplit && blocks < (int64_t{1} << 31), "INT8 gradient: too many tiles for one call.");
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.pair ? tile.bn / 2 : tile.bn))
@@ -498,9 +526,8 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
 
   const auto grid = static_cast<unsigned>(blocks);
 #define CALL(D)                                                                                                              \
-  constexpr int kHold = D == i8::kF32 ? 2 : 4;                                                                                \
-  launch_rows(grid, s, rows, vec, v, r, i8::scale_kernel<D, 1, kHold, true>, i8::scale_kernel<D, 2, kHold, true>,            \
-              i8::scale_kernel<D, 4, kHold, true>, i8::scale_kernel<D, 8, kHold, true>, i8::scale_kernel<D, 1, 2, false>,       \
+  launch_rows(grid, s, rows, vec, v, r, i8::scale_kernel<D, 1, 2, true>, i8::scale_kernel<D, 2, 2, true>, i8::scale_kernel<D, 4, 2, true>, \
+              i8::scale_kernel<D, 8, 2, true>, i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>, i8::scale_kernel<D, 1, 2, false>,       \
               i8::scale_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
@@ -519,7 +546,7 @@ int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, piper_int
   if (int rc = check_matrix(w)) return rc;
   INT8_REQUIRE(plan != nullptr && tokens > 0, "INT8 product: bad plan query.");
   const LinearPlan p = plan_linear(*w, tokens);
-  *plan = {p.bn, p.pair ? 256 : 128, p.split, 1};
+  *plan = {p.bn, p.pair ? 256 : 128, p.split, p.blocks};
   return PIPER_INT8_OK;
 }
 

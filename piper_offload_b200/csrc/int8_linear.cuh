@@ -6,8 +6,8 @@
 // point's share z[n] sum_k q[t, k] is taken off them exactly, and the roundings are those of the sum to fp32, of the two
 // products with the scales, and of the result to its type.
 //
-// Tokens are quantised by a launch before, which the set-up and the first loads of the weight overlap. Tiles are 32, 128 or
-// 256 tokens wide. Where there are too few tiles for the SMs, a cluster of blocks splits K; each leaves its sums in its own
+// Tokens are quantised by a launch before, which the set-up and the first loads of the weight overlap. Tiles are 32, 64,
+// 128 or 256 tokens wide. Where there are too few tiles for the SMs, a cluster of blocks splits K; each leaves its sums in its own
 // shared memory and every block adds up its share of the tokens over the cluster.
 #pragma once
 #include <cuda.h>

@@ -127,7 +127,7 @@ struct RowTeam {
       thread = threadIdx.x;
     }
   }
-  // Of all the row's threads; `words` is shared memory, eight words for each function.
+  // Of all the row's threads; `words` is shared memory, kWarps words for each function.
   __device__ __forceinline__ uint32_t max_of(uint32_t v, uint32_t* words) const {
     v = __reduce_max_sync(0xFFFFFFFFu, v);
     if constexpr (kWarps == 1) return v;
@@ -138,9 +138,9 @@ struct RowTeam {
   __device__ __forceinline__ int sum_of(int v, uint32_t* words) const {
     v = __reduce_add_sync(0xFFFFFFFFu, v);
     if constexpr (kWarps == 1) return v;
-    if ((threadIdx.x & 31) == 0) words[8 + (threadIdx.x >> 5)] = static_cast<uint32_t>(v);
+    if ((threadIdx.x & 31) == 0) words[kWarps + (threadIdx.x >> 5)] = static_cast<uint32_t>(v);
     __syncthreads();
-    return __reduce_add_sync(0xFFFFFFFFu, (threadIdx.x & 31) < kWarps ? static_cast<int>(words[8 + (threadIdx.x & (kWarps - 1))]) : 0);
+    return __reduce_add_sync(0xFFFFFFFFu, (threadIdx.x & 31) < kWarps ? static_cast<int>(words[kWarps + (threadIdx.x & (kWarps - 1))]) : 0);
   }
 };
 
@@ -416,7 +416,7 @@ __device__ __forceinline__ void repack(const RepackArgs& p, int64_t piece) {
 template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(prepare_threads(kWarps)) quantize_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs r,
                                                                    uint32_t token_blocks) {
-  __shared__ uint32_t words[16];
+  __shared__ uint32_t words[2 * kWarps];
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) quantize_rows<DT, kWarps, kHold, kVec>(q, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(prepare_threads(kWarps)) quantize_kernel(const
 template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(prepare_threads(kWarps)) scale_kernel(const __grid_constant__ ScaleArgs s, const __grid_constant__ RepackArgs r,
                                                                 uint32_t token_blocks) {
-  __shared__ uint32_t words[16];
+  __shared__ uint32_t words[2 * kWarps];
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) scale_rows<DT, kWarps, kHold, kVec>(s, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);

@@ -106,10 +106,11 @@ def test_plan_queries():
     """Without a device the plan is made for 148 SMs."""
     for tokens in (1, 40, 700, 5000):
         p = nat.linear_plan(matrix(rows=4096, cols=4096), tokens)
-        assert p.tile_tokens in (32, 128, 256) and p.tile_columns in (128, 256) and p.split in (1, 2, 4, 8) and p.blocks in (1, 2)
+        assert p.tile_tokens in (32, 64, 128, 256) and p.tile_columns in (128, 256) and p.split in (1, 2, 4, 8) and p.blocks in (1, 2)
         p = nat.grad_input_plan(matrix(rows=4096, cols=4096), tokens, grouped=False, dtype=0)
-        assert p.tile_tokens in (64, 256) and p.tile_columns in (128, 256)
+        assert p.tile_tokens in (64, 128, 160, 192, 224, 256) and p.tile_columns in (128, 256, 512)
         assert p.split == 1 or p.tile_columns == 128
+        assert p.tile_tokens in (64, 256) or p.tile_columns > 128
     m = matrix()
     for call in (lambda: nat.linear_plan(m, 0), lambda: nat.grad_input_plan(m, 0, grouped=False, dtype=0),
                  lambda: nat.grad_input_plan(matrix(batch=2), 8, grouped=False, dtype=0)):
