@@ -50,6 +50,11 @@ cudaError_t launched() {
   return cudaGetLastError();
 }
 
+// Above 48 KB a kernel has to be allowed its shared memory.
+cudaError_t allow_shared(const void* kernel, size_t bytes) {
+  return bytes <= 48 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
 int check_dtype(int dtype) {
   ROUTING_REQUIRE(dtype == PIPER_ROUTING_BF16 || dtype == PIPER_ROUTING_F16 || dtype == PIPER_ROUTING_F32,
                   "Routing supports bfloat16, float16 and float32 values.");
@@ -138,8 +143,7 @@ cudaError_t launch_route(routing::RouteArgs a, int threads, cudaStream_t s) {
   const size_t lists = threads / 32 * sizeof(routing::Lists<N>), places = place_bytes(a.pitch, threads);
   const auto kernel = a.chunks == 1 ? routing::route_kernel<DT, N, true> : routing::route_kernel<DT, N, false>;
   const size_t smem = a.pitch * 4 + (a.chunks == 1 ? std::max(lists, places) : lists);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
+  if (const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), smem); e != cudaSuccess) return e;
   kernel<<<static_cast<unsigned>(a.chunks), threads, smem, s>>>(a);
   return launched();
 }
@@ -277,8 +281,8 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
   config.gridDim = dim3(static_cast<unsigned>(n.count));
   config.blockDim = dim3(1024);
   config.dynamicSmemBytes = place_bytes(a.pitch, 1024);
-  e = cudaFuncSetAttribute(routing::place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(config.dynamicSmemBytes));
-  if (e != cudaSuccess) return cuda_fail("place kernel", e);
+  if ((e = allow_shared(reinterpret_cast<const void*>(routing::place_kernel), config.dynamicSmemBytes)) != cudaSuccess)
+    return cuda_fail("place kernel", e);
   config.stream = s;
   config.attrs = &attribute;
   config.numAttrs = 1;
