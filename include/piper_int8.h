@@ -50,8 +50,9 @@ typedef struct piper_int8_matrix {
   int32_t over_127;    /* scales are rows' largest magnitudes: codes / 127 of them */
 } piper_int8_matrix;
 
-/* Scratch bytes that piper_int8_linear / piper_int8_grad_input need. */
-int piper_int8_linear_workspace(const piper_int8_matrix* w, int64_t tokens, size_t* bytes);
+/* Scratch bytes that piper_int8_linear / piper_int8_grad_input need (0: none).
+ * `grouped`: with the ends of the matrices' rows. */
+int piper_int8_linear_workspace(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, size_t* bytes);
 int piper_int8_grad_input_workspace(const piper_int8_matrix* w, int64_t tokens, int32_t dtype, size_t* bytes);
 
 /* y[t] = w . quantised(x[t]): y is (tokens, rows), x is (tokens, cols) with
@@ -72,14 +73,13 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
 /* How the product of `tokens` tokens, or its gradient, runs on the current
  * device. Results do not depend on it but for the order of a gradient's sums. */
 typedef struct piper_int8_plan {
-  int32_t tile_tokens;
+  int32_t tile_tokens;  /* 8: the product quantises its tokens itself */
   int32_t tile_columns; /* of y, or of dx */
   int32_t split;        /* blocks that share the sums of a tile */
   int32_t blocks;       /* on an SM at a time */
 } piper_int8_plan;
 
-int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, piper_int8_plan* plan);
-/* `grouped`: with the ends of the matrices' rows. */
+int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, piper_int8_plan* plan);
 int piper_int8_grad_input_plan(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, int32_t dtype,
                                piper_int8_plan* plan);
 

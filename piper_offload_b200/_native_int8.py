@@ -84,11 +84,11 @@ def load() -> ctypes.CDLL:
         lib = ctypes.CDLL(str(path))
         vp, i32, i64, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t
         mat = ctypes.POINTER(Matrix)
-        lib.piper_int8_linear_workspace.argtypes = [mat, i64, ctypes.POINTER(sz)]
+        lib.piper_int8_linear_workspace.argtypes = [mat, i64, i32, ctypes.POINTER(sz)]
         lib.piper_int8_grad_input_workspace.argtypes = [mat, i64, i32, ctypes.POINTER(sz)]
         lib.piper_int8_linear.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, sz, vp]
         lib.piper_int8_grad_input.argtypes = [mat, vp, i64, i64, vp, vp, i32, vp, sz, vp]
-        lib.piper_int8_linear_plan.argtypes = [mat, i64, ctypes.POINTER(Plan)]
+        lib.piper_int8_linear_plan.argtypes = [mat, i64, i32, ctypes.POINTER(Plan)]
         lib.piper_int8_grad_input_plan.argtypes = [mat, i64, i32, i32, ctypes.POINTER(Plan)]
         lib.piper_int8_device_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint32)]
         for name in EXPORTED_SYMBOLS[:6] + ("piper_int8_device_status",):
@@ -123,10 +123,10 @@ def version() -> str:
     return load().piper_int8_version().decode()
 
 
-def linear_plan(m: Matrix, tokens: int) -> Plan:
+def linear_plan(m: Matrix, tokens: int, *, grouped: bool) -> Plan:
     """How the product of a matrix (or a stack of them) and ``tokens`` tokens runs on the current device."""
     plan = Plan()
-    check(load().piper_int8_linear_plan(ctypes.byref(m), tokens, ctypes.byref(plan)))
+    check(load().piper_int8_linear_plan(ctypes.byref(m), tokens, grouped, ctypes.byref(plan)))
     return plan
 
 

@@ -33,7 +33,7 @@ CALLS_OUT = PKG / "_fp4_calls.so"
 
 INT8_SOURCES = [PKG / "csrc" / "int8.cu"]
 INT8_DEPS = INT8_SOURCES + [
-    *(PKG / "csrc" / n for n in ("int8_quant.cuh", "int8_tiles.cuh", "int8_linear.cuh", "int8_pair.cuh", "int8_grad.cuh", "fp4_tiles.cuh",
+    *(PKG / "csrc" / n for n in ("int8_quant.cuh", "int8_tiles.cuh", "int8_linear.cuh", "int8_pair.cuh", "int8_few.cuh", "int8_grad.cuh", "fp4_tiles.cuh",
                                  "fp4_quant.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
     ROOT / "include" / "piper_int8.h",
 ]

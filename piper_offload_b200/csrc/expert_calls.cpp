@@ -209,12 +209,13 @@ struct Weight {
 Tensor product(const Weight& w, const Tensor& x, int64_t stride, int64_t tokens, const Tensor& ends, bool grad) {
   const int dtype = dtype_of(x);
   size_t need = 0;
-  check_int8(grad ? g_entry.grad_workspace(&w.m, tokens, dtype, &need) : g_entry.linear_workspace(&w.m, tokens, &need));
+  check_int8(grad ? g_entry.grad_workspace(&w.m, tokens, dtype, &need) : g_entry.linear_workspace(&w.m, tokens, ends.defined(), &need));
   Tensor y = at::empty(shape_with_last(x, grad ? w.m.cols : w.m.rows), x.options().requires_grad(false));
-  const Tensor workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte).requires_grad(false));
+  Tensor workspace;
+  if (need > 0) workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte).requires_grad(false));
   const auto call = grad ? g_entry.grad_input : g_entry.linear;
   check_int8(call(&w.m, x.const_data_ptr(), stride, tokens, ends.defined() ? ends.const_data_ptr<int32_t>() : nullptr, y.mutable_data_ptr(),
-                  dtype, workspace.mutable_data_ptr(), need, stream_of(static_cast<c10::DeviceIndex>(x.get_device()))));
+                  dtype, need > 0 ? workspace.mutable_data_ptr() : nullptr, need, stream_of(static_cast<c10::DeviceIndex>(x.get_device()))));
   return y;
 }
 

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <cstdio>
 
+#include "int8_few.cuh"
 #include "int8_grad.cuh"
 #include "int8_linear.cuh"
 #include "int8_pair.cuh"
@@ -200,6 +201,8 @@ int64_t likely_tiles(int64_t batch, int64_t tokens, int64_t tile) {
 struct LinearPlan {
   int bn, split;
   bool pair;   // of SMs, on tiles of 256 outputs
+  bool few;    // tokens, which the product quantises itself
+  int x_stages, ring;  // of that: stages of a block, and how many are under way
   int blocks;  // on an SM
   int64_t x_pitch;
   int64_t x_codes, x_scale, x_sums, w_codes, total;  // byte offsets
@@ -210,8 +213,33 @@ struct LinearPlan {
 // 2048 x 2048 31.4 and 35.4; 1 x 4096 x 4096 shared by four 9.5 and 10.1, but 24 x 4096 x 4096 not shared 11.7 and 11.2).
 bool two_blocks(int bn, int64_t items, int split) { return bn <= 64 && (items > sm_count() || (bn == 32 && split > 1)); }
 
-LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens) {
+// A few tokens of one weight: one launch, if a block a tile, or a share of one, is enough and the tokens have so few values
+// that every block can quantise them. One launch against two: 1 x 14336 x 4096 13.6 and 15.4 us, two tokens 13.7 and 15.5,
+// four 16.0 and 15.5; 1 x 4096 x 4096 8.7 and 9.7; 8 x 1024 x 1024 5.8 and 6.3; 1 x 4096 x 14336 16.3 and 16.1. Clusters of
+// eight blocks that fill their SMs find room for half of the SMs at most (1 x 2048 x 8192 shared by eight 13.9 us).
+bool plan_few(const piper_int8_matrix& w, int64_t tokens, bool grouped, LinearPlan& plan) {
+  const int64_t tiles = (w.rows + 127) / 128, stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
+  if (grouped || w.batch > 1 || tokens > i8::kFewTokens || tokens * w.cols > 8192 || moves_codes(w) || tiles > sm_count()) return false;
+  int split = 1;
+  while (split < 4 && tiles * split * 2 <= sm_count() && stages >= 8 * split) split *= 2;
+  if (split == 4 && tiles * 16 <= sm_count() && stages >= 32) split = 8;
+  const int64_t most = (stages + split - 1) / split;
+  const int64_t ring = (i8::kSmemMax - 1024 - i8::few_smem(static_cast<int>(most), 0)) / i8::kFewStage;
+  if (ring < 6) return false;
   LinearPlan p{};
+  p.few = true;
+  p.bn = i8::kFewTokens;
+  p.blocks = 1;
+  p.split = split;
+  p.x_stages = static_cast<int>(most);
+  p.ring = static_cast<int>(std::min<int64_t>(std::min<int64_t>(ring, i8::kFewRing), most));
+  plan = p;
+  return true;
+}
+
+LinearPlan plan_linear(const piper_int8_matrix& w, int64_t tokens, bool grouped) {
+  LinearPlan p{};
+  if (plan_few(w, tokens, grouped, p)) return p;
   const int64_t per_expert = (tokens + w.batch - 1) / w.batch;
   const int64_t stages = (w.cols + i8::kStageCols - 1) / i8::kStageCols;
   TilePlan best{};
@@ -298,6 +326,9 @@ cudaError_t launch_pairs(const i8::LinearArgs& args, int64_t items, cudaStream_t
                                 i8::PairShape<BN>::kSmem, 2, stream);
 }
 
+int launch_few(const piper_int8_matrix& w, const LinearPlan& p, const void* x, int64_t x_stride, int64_t tokens, void* y, int dtype,
+               cudaStream_t stream);
+
 // --------------------------------------------------------------- the gradient
 struct GradPlan {
   int terms;      // fp16 terms per value
@@ -378,6 +409,52 @@ cudaError_t launch_grad(const i8::GradArgs& args, int64_t items, cudaStream_t st
     else { CALL(i8::kF32); }                                    \
   } while (0)
 
+template <int DT>
+cudaError_t launch_few(const i8::FewArgs& args, int64_t tiles, cudaStream_t stream) {
+  auto kernel = i8::linear_few_kernel<DT>;
+  const int smem = i8::few_smem(args.x_stages, args.ring);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(args.split);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(tiles * args.split));
+  config.blockDim = dim3(i8::kFewThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = args.split > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&config, kernel, args);
+  return e == cudaSuccess ? launched() : e;
+}
+
+int launch_few(const piper_int8_matrix& w, const LinearPlan& p, const void* x, int64_t x_stride, int64_t tokens, void* y, int dtype,
+               cudaStream_t stream) {
+  i8::FewArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.rows_of = {row_scales(w), static_cast<const int8_t*>(w.zero), w.per_row != 0 ? 1 : 0};
+  a.y = y;
+  a.tokens = static_cast<int32_t>(tokens);
+  a.rows = static_cast<int32_t>(w.rows);
+  a.cols = static_cast<int32_t>(w.cols);
+  a.split = p.split;
+  a.x_stages = p.x_stages;
+  a.ring = p.ring;
+  a.vec = aligned(y, 16) && (w.rows * static_cast<int64_t>(width(dtype))) % 16 == 0;
+  a.x_vec = whole_units(x, x_stride, tokens, w.cols, dtype);
+  if (!encode_map(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, w.cols, w.rows, w.cols, i8::kStageCols, fp4::kTileRows))
+    return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
+  const int64_t tiles = (w.rows + 127) / 128;
+  cudaError_t e = cudaSuccess;
+#define CALL(D) e = launch_few<D>(a, tiles, stream)
+  INT8_DISPATCH(dtype, CALL);
+#undef CALL
+  return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("product kernel", e);
+}
+
 int check_call(const piper_int8_matrix* w, int64_t tokens, const int32_t* ends, int dtype) {
   if (int rc = check_matrix(w)) return rc;
   if (int rc = check_buffers(w)) return rc;
@@ -391,10 +468,10 @@ int check_call(const piper_int8_matrix* w, int64_t tokens, const int32_t* ends, 
 
 extern "C" {
 
-int piper_int8_linear_workspace(const piper_int8_matrix* w, int64_t tokens, size_t* bytes) {
+int piper_int8_linear_workspace(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, size_t* bytes) {
   if (int rc = check_matrix(w)) return rc;
-  INT8_REQUIRE(bytes != nullptr && tokens >= 0, "INT8 product: bad workspace query.");
-  *bytes = tokens == 0 ? 0 : static_cast<size_t>(plan_linear(*w, tokens).total);
+  INT8_REQUIRE(bytes != nullptr && tokens >= 0 && (grouped != 0 || w->batch == 1), "INT8 product: bad workspace query.");
+  *bytes = tokens == 0 ? 0 : static_cast<size_t>(plan_linear(*w, tokens, grouped != 0).total);
   return PIPER_INT8_OK;
 }
 
@@ -405,7 +482,8 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
   INT8_REQUIRE(x != nullptr && y != nullptr, "INT8 product: null input or output.");
   INT8_REQUIRE(aligned(x, width(dtype)) && aligned(y, width(dtype)), "INT8 product: input or output not aligned to its type.");
   INT8_REQUIRE(x_stride >= w->cols || tokens == 1, "INT8 product: rows of the input overlap.");
-  const LinearPlan p = plan_linear(*w, tokens);
+  const LinearPlan p = plan_linear(*w, tokens, ends != nullptr);
+  if (p.few) return launch_few(*w, p, x, x_stride, tokens, y, dtype, static_cast<cudaStream_t>(stream));
   if (workspace == nullptr || workspace_bytes < static_cast<size_t>(p.total) || !aligned(workspace, 256))
     return fail(PIPER_INT8_EWORKSPACE, "INT8 product: workspace missing, too small or not 256-byte aligned.");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -542,10 +620,10 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   return e == cudaSuccess ? PIPER_INT8_OK : cuda_fail("gradient kernel", e);
 }
 
-int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, piper_int8_plan* plan) {
+int piper_int8_linear_plan(const piper_int8_matrix* w, int64_t tokens, int32_t grouped, piper_int8_plan* plan) {
   if (int rc = check_matrix(w)) return rc;
-  INT8_REQUIRE(plan != nullptr && tokens > 0, "INT8 product: bad plan query.");
-  const LinearPlan p = plan_linear(*w, tokens);
+  INT8_REQUIRE(plan != nullptr && tokens > 0 && (grouped != 0 || w->batch == 1), "INT8 product: bad plan query.");
+  const LinearPlan p = plan_linear(*w, tokens, grouped != 0);
   *plan = {p.bn, p.pair ? 256 : 128, p.split, p.blocks};
   return PIPER_INT8_OK;
 }

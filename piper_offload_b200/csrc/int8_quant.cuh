@@ -50,15 +50,15 @@ __device__ __forceinline__ Unit<DT> load_unit(const void* row, int col, int cols
       const uint4 q = from[i];
       u.w[4 * i] = q.x; u.w[4 * i + 1] = q.y; u.w[4 * i + 2] = q.z; u.w[4 * i + 3] = q.w;
     }
-    return u;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) u.w[i] = 0u;
+    for (int i = 0; i < kWords; ++i) u.w[i] = 0u;
 #pragma unroll
-  for (int i = 0; i < kUnit; ++i) {
-    if (col + i < cols) {
-      if constexpr (DT == kF32) u.w[i] = static_cast<const uint32_t*>(row)[col + i];
-      else u.w[i >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[col + i]) << (16 * (i & 1));
+    for (int i = 0; i < kUnit; ++i) {
+      if (col + i < cols) {
+        if constexpr (DT == kF32) u.w[i] = static_cast<const uint32_t*>(row)[col + i];
+        else u.w[i >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(row)[col + i]) << (16 * (i & 1));
+      }
     }
   }
   return u;

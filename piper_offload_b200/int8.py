@@ -133,10 +133,10 @@ def _on(device: torch.device, function: Any, *args: Any) -> None:
             nat.check(function(*args))
 
 
-def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor:
+def _workspace(query: Any, device: torch.device, *args: Any) -> torch.Tensor | None:
     need = ctypes.c_size_t()
     _on(device, query, *args, ctypes.byref(need))
-    return torch.empty(need.value, dtype=torch.uint8, device=device)
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -182,9 +182,10 @@ def _run(x: torch.Tensor, w: _Frozen, ends: torch.Tensor | None, grad: bool) -> 
     if grad:
         ws = _workspace(lib.piper_int8_grad_input_workspace, device, ref, tokens, dt)
     else:
-        ws = _workspace(lib.piper_int8_linear_workspace, device, ref, tokens)
+        ws = _workspace(lib.piper_int8_linear_workspace, device, ref, tokens, ends is not None)
     _on(device, lib.piper_int8_grad_input if grad else lib.piper_int8_linear, ref, x2.data_ptr(), x2.stride(0), tokens,
-        None if ends is None else ends.data_ptr(), y.data_ptr(), dt, ws.data_ptr(), ws.numel(), raw_stream(device.index))
+        None if ends is None else ends.data_ptr(), y.data_ptr(), dt, *((None, 0) if ws is None else (ws.data_ptr(), ws.numel())),
+        raw_stream(device.index))
     return y
 
 

@@ -42,7 +42,7 @@ BAD_MATRICES = [({"rows": 0}, "non-empty"), ({"batch": 0}, "non-empty"), ({"cols
 def calls(m: nat.Matrix):
     """Every entry point with arguments that are good but for `m`; none is enqueued when m is bad."""
     lib, ref, n = nat.load(), ctypes.byref(m), ctypes.c_size_t()
-    yield lambda: lib.piper_int8_linear_workspace(ref, 8, ctypes.byref(n))
+    yield lambda: lib.piper_int8_linear_workspace(ref, 8, 1, ctypes.byref(n))
     yield lambda: lib.piper_int8_grad_input_workspace(ref, 8, 0, ctypes.byref(n))
     yield lambda: lib.piper_int8_linear(ref, 0x4000, max(m.cols, 1), 8, 0x5000, 0x6000, 0, 0x100000, 1 << 40, None)
     yield lambda: lib.piper_int8_grad_input(ref, 0x4000, max(m.rows, 1), 8, 0x5000, 0x6000, 0, 0x100000, 1 << 40, None)
@@ -54,7 +54,7 @@ def test_bad_matrices_are_refused(change, match):
         with pytest.raises(ValueError, match=match):
             nat.check(call())
     with pytest.raises(ValueError, match=match):
-        nat.linear_plan(matrix(**change), 8)
+        nat.linear_plan(matrix(**change), 8, grouped=True)
     with pytest.raises(ValueError, match=match):
         nat.grad_input_plan(matrix(**change), 8, grouped=True, dtype=0)
 
@@ -72,7 +72,7 @@ def test_bad_arguments_are_refused(name):
     function = getattr(lib, f"piper_int8_{name}")
 
     def call(m=matrix(), **kw):
-        a = {"x": 0x4000, "stride": 96, "tokens": 8, "ends": None, "y": 0x6000, "dtype": 0, "ws": 0x100000, "bytes": 1 << 30, **kw}
+        a = {"x": 0x4000, "stride": 96, "tokens": 9, "ends": None, "y": 0x6000, "dtype": 0, "ws": 0x100000, "bytes": 1 << 30, **kw}
         return function(ctypes.byref(m), *a.values(), None)
 
     for kw, match in (({"x": None}, "null"), ({"y": None}, "null"), ({"stride": 63}, "overlap"), ({"tokens": -1}, "tokens"),
@@ -92,11 +92,11 @@ def test_workspace_needs_are_modest():
     """Aligned codes are used in place: only the tokens need room."""
     lib, n = nat.load(), ctypes.c_size_t()
     m = matrix(rows=4096, cols=4096, codes=1 << 20)
-    nat.check(lib.piper_int8_linear_workspace(ctypes.byref(m), 1024, ctypes.byref(n)))
+    nat.check(lib.piper_int8_linear_workspace(ctypes.byref(m), 1024, 0, ctypes.byref(n)))
     assert 1024 * 4096 < n.value < 1024 * 4200
     nat.check(lib.piper_int8_grad_input_workspace(ctypes.byref(m), 1024, 0, ctypes.byref(n)))
     assert 2 * 1024 * 4096 < n.value < 2 * 1024 * 4200
-    for query in (lambda: lib.piper_int8_linear_workspace(ctypes.byref(m), 0, ctypes.byref(n)),
+    for query in (lambda: lib.piper_int8_linear_workspace(ctypes.byref(m), 0, 0, ctypes.byref(n)),
                   lambda: lib.piper_int8_grad_input_workspace(ctypes.byref(m), 0, 0, ctypes.byref(n))):
         nat.check(query())
         assert n.value == 0
@@ -105,14 +105,14 @@ def test_workspace_needs_are_modest():
 def test_plan_queries():
     """Without a device the plan is made for 148 SMs."""
     for tokens in (1, 40, 700, 5000):
-        p = nat.linear_plan(matrix(rows=4096, cols=4096), tokens)
-        assert p.tile_tokens in (32, 64, 128, 256) and p.tile_columns in (128, 256) and p.split in (1, 2, 4, 8) and p.blocks in (1, 2)
+        p = nat.linear_plan(matrix(rows=4096, cols=4096, codes=1 << 20), tokens, grouped=False)
+        assert (p.tile_tokens == 8) == (tokens <= 2) and p.tile_tokens in (8, 32, 64, 128, 256) and p.tile_columns in (128, 256) and p.split in (1, 2, 4, 8) and p.blocks in (1, 2)
         p = nat.grad_input_plan(matrix(rows=4096, cols=4096), tokens, grouped=False, dtype=0)
         assert p.tile_tokens in (64, 128, 160, 192, 224, 256) and p.tile_columns in (128, 256, 512)
         assert p.split == 1 or p.tile_columns == 128
         assert p.tile_tokens in (64, 256) or p.tile_columns > 128
     m = matrix()
-    for call in (lambda: nat.linear_plan(m, 0), lambda: nat.grad_input_plan(m, 0, grouped=False, dtype=0),
+    for call in (lambda: nat.linear_plan(m, 0, grouped=False), lambda: nat.linear_plan(matrix(batch=2), 8, grouped=False), lambda: nat.grad_input_plan(m, 0, grouped=False, dtype=0),
                  lambda: nat.grad_input_plan(matrix(batch=2), 8, grouped=False, dtype=0)):
         with pytest.raises(ValueError, match="plan query"):
             call()
