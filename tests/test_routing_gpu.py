@@ -339,6 +339,26 @@ def test_rows_outside_count_as_none(cuda_device):
     assert routing.dispatch_tokens(x[:0], no_tokens).shape == (0, 8) and routing.combine_tokens(x[:0], no_tokens).shape == (0, 8)
 
 
+def test_offsets_beyond_32_bits(cuda_device):
+    """Rows that end more than 2^32 bytes into their tensors."""
+    if torch.cuda.get_device_properties(cuda_device).total_memory < 60e9:
+        pytest.skip("needs 30 GB")
+    tokens, top_k, hidden = 70000, 8, 4096
+    r = routing.route_tokens(torch.randn(tokens, 16, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(0)), top_k)
+    x = torch.randn(tokens, hidden, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(1)).bfloat16()
+    sent = routing.dispatch_tokens(x, r)
+    assert sent.numel() > 2 ** 31
+    for part in (slice(0, 300), slice(-300, None)):
+        assert torch.equal(sent[part], x[r.source[part].long() // top_k])
+    y = sent.requires_grad_()
+    back = routing.combine_tokens(y, r)
+    assert ((back.float() - x.float()).abs() <= x.float().abs() * (2.0 ** -8 + 1e-5)).all()  # a token's weights add up to one
+    (dy,) = torch.autograd.grad(back, y, x)
+    for part in (slice(0, 300), slice(-300, None)):
+        want = x[r.source[part].long() // top_k].double() * r.weights.reshape(-1)[r.source[part].long()].double()[:, None]
+        assert ((dy[part].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -23) + R.TINY["bfloat16"]).all()
+
+
 # ------------------------------------------------------------- streams, graphs, same bits
 def test_same_bits_on_every_run(cuda_device):
     logits = normal_logits(3000, 64, torch.bfloat16, cuda_device)
