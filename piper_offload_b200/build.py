@@ -33,14 +33,14 @@ CALLS_OUT = PKG / "_fp4_calls.so"
 
 INT8_SOURCES = [PKG / "csrc" / "int8.cu"]
 INT8_DEPS = INT8_SOURCES + [
-    *(PKG / "csrc" / n for n in ("int8_quant.cuh", "int8_tiles.cuh", "int8_linear.cuh", "int8_pair.cuh", "int8_few.cuh", "int8_grad.cuh", "fp4_tiles.cuh",
+    *(PKG / "csrc" / n for n in ("int8_quant.cuh", "int8_tiles.cuh", "int8_linear.cuh", "int8_pair.cuh", "int8_few.cuh", "launch.cuh", "int8_grad.cuh", "fp4_tiles.cuh",
                                  "fp4_quant.cuh", "fp4_ptx.cuh", "ptx.cuh", "numerics.cuh")),
     ROOT / "include" / "piper_int8.h",
 ]
 INT8_OUT = PKG / "libpiper_int8.so"
 ROUTING_SOURCES = [PKG / "csrc" / "routing.cu"]
 ROUTING_DEPS = ROUTING_SOURCES + [
-    *(PKG / "csrc" / n for n in ("routing_route.cuh", "routing_exchange.cuh", "fp4_ptx.cuh", "ptx.cuh")),
+    *(PKG / "csrc" / n for n in ("routing_route.cuh", "routing_exchange.cuh", "launch.cuh", "fp4_ptx.cuh", "ptx.cuh")),
     ROOT / "include" / "piper_routing.h",
 ]
 ROUTING_OUT = PKG / "libpiper_routing.so"

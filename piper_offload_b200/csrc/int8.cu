@@ -14,6 +14,7 @@
 #include "int8_linear.cuh"
 #include "int8_pair.cuh"
 #include "int8_quant.cuh"
+#include "launch.cuh"
 
 namespace {
 
@@ -154,7 +155,7 @@ bool whole_units(const void* p, int64_t stride, int64_t rows, int64_t cols, int 
 }
 
 template <class Args, class Kernel>
-void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, Kernel one, Kernel two,
+cudaError_t launch_rows(int64_t blocks, cudaStream_t s, const RowPlan& rows, bool vec, const Args& args, const i8::RepackArgs& r, Kernel one, Kernel two,
                  Kernel four, Kernel eight, Kernel eight_more, Kernel one_any, Kernel eight_any) {
   const Kernel kernel = !vec              ? (rows.warps == 1 ? one_any : eight_any)
                         : rows.warps == 1 ? one
@@ -162,7 +163,8 @@ void launch_rows(unsigned grid, cudaStream_t s, const RowPlan& rows, bool vec, c
                         : rows.warps == 4 ? four
                         : rows.more       ? eight_more
                                           : eight;
-  kernel<<<grid, i8::prepare_threads(rows.warps), 0, s>>>(args, r, static_cast<unsigned>(rows.blocks));
+  const cudaError_t e = piper::launch(kernel, blocks, i8::prepare_threads(rows.warps), 0, 1, s, args, r, static_cast<uint32_t>(rows.blocks));
+  return e == cudaSuccess ? launched() : e;
 }
 
 int64_t repack_blocks(const i8::RepackArgs& r, const RowPlan& rows) {
@@ -291,25 +293,11 @@ int64_t token_tiles(int64_t tokens, int64_t experts, int bn) {
   return experts == 0 ? (tokens + bn - 1) / bn : tokens / bn + std::min<int64_t>(experts + 1, tokens);
 }
 
-// A launch that may start while the one before it still runs; the kernel waits where it needs that one's results.
 template <class Args>
-cudaError_t launch(void (*kernel)(Args), const Args& args, int64_t blocks, int threads, int smem, int split, cudaStream_t stream) {
+cudaError_t launch(void (*kernel)(Args), const Args& args, int64_t blocks, int threads, int smem, int cluster, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attributes[2] = {};
-  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[0].val.programmaticStreamSerializationAllowed = 1;
-  attributes[1].id = cudaLaunchAttributeClusterDimension;
-  attributes[1].val.clusterDim.x = static_cast<unsigned>(split);
-  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(static_cast<unsigned>(threads));
-  config.dynamicSmemBytes = static_cast<size_t>(smem);
-  config.stream = stream;
-  config.attrs = attributes;
-  config.numAttrs = split > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&config, kernel, args);
+  e = piper::launch(kernel, blocks, threads, static_cast<size_t>(smem), cluster, stream, args);
   return e == cudaSuccess ? launched() : e;
 }
 
@@ -413,21 +401,7 @@ template <int DT>
 cudaError_t launch_few(const i8::FewArgs& args, int64_t tiles, cudaStream_t stream) {
   auto kernel = i8::linear_few_kernel<DT>;
   const int smem = i8::few_smem(args.x_stages, args.ring);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(args.split);
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(tiles * args.split));
-  config.blockDim = dim3(i8::kFewThreads);
-  config.dynamicSmemBytes = static_cast<size_t>(smem);
-  config.stream = stream;
-  config.attrs = &attribute;
-  config.numAttrs = args.split > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&config, kernel, args);
-  return e == cudaSuccess ? launched() : e;
+  return launch<i8::FewArgs>(kernel, args, tiles * args.split, i8::kFewThreads, smem, args.split, stream);
 }
 
 int launch_few(const piper_int8_matrix& w, const LinearPlan& p, const void* x, int64_t x_stride, int64_t tokens, void* y, int dtype,
@@ -523,16 +497,15 @@ int piper_int8_linear(const piper_int8_matrix* w, const void* x, int64_t x_strid
       !encode_map(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, w->cols, tokens, p.x_pitch, i8::kStageCols, p.pair ? p.bn / 2 : p.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 product: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks);
+  cudaError_t e = cudaSuccess;
 #define CALL(D)                                                                                                              \
   constexpr int kHold = D == i8::kF32 ? 2 : 4;                                                                                \
-  launch_rows(grid, s, rows, vec, q, r, i8::quantize_kernel<D, 1, kHold, true>, i8::quantize_kernel<D, 2, kHold, true>,            \
+  e = launch_rows(blocks, s, rows, vec, q, r, i8::quantize_kernel<D, 1, kHold, true>, i8::quantize_kernel<D, 2, kHold, true>,            \
               i8::quantize_kernel<D, 4, kHold, true>, i8::quantize_kernel<D, 8, 2, true>, i8::quantize_kernel<D, 8, kHold, true>,  \
               i8::quantize_kernel<D, 1, 2, false>,                                                                            \
               i8::quantize_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
-  cudaError_t e = launched();
   if (e != cudaSuccess) return cuda_fail("quantize kernel", e);
 #define CALL(D)                                                                                                          \
   e = p.pair        ? (p.bn == 128 ? launch_pairs<D, 128>(a, items, s) : launch_pairs<D, 256>(a, items, s))                \
@@ -602,14 +575,13 @@ int piper_int8_grad_input(const piper_int8_matrix* w, const void* dy, int64_t dy
   if (!encode_map(&a.dy_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v.out, w->rows, p.terms * tokens, p.pitch * 2, i8::kGradStageRows, tile.pair ? tile.bn / 2 : tile.bn))
     return fail(PIPER_INT8_ECUDA, "INT8 gradient: cuTensorMapEncodeTiled failed.");
 
-  const auto grid = static_cast<unsigned>(blocks);
+  cudaError_t e = cudaSuccess;
 #define CALL(D)                                                                                                              \
-  launch_rows(grid, s, rows, vec, v, r, i8::scale_kernel<D, 1, 2, true>, i8::scale_kernel<D, 2, 2, true>, i8::scale_kernel<D, 4, 2, true>, \
+  e = launch_rows(blocks, s, rows, vec, v, r, i8::scale_kernel<D, 1, 2, true>, i8::scale_kernel<D, 2, 2, true>, i8::scale_kernel<D, 4, 2, true>, \
               i8::scale_kernel<D, 8, 2, true>, i8::scale_kernel<D, 8, D == i8::kF32 ? 2 : 4, true>, i8::scale_kernel<D, 1, 2, false>,       \
               i8::scale_kernel<D, 8, 2, false>)
   INT8_DISPATCH(dtype, CALL);
 #undef CALL
-  cudaError_t e = launched();
   if (e != cudaSuccess) return cuda_fail("scale kernel", e);
 #define CALL(D)                                                                                              \
   e = tile.pair       ? (tile.rows == 2 ? launch_grad<D, 256, 2, true>(a, tile.items, s) : launch_grad<D, 256, 1, true>(a, tile.items, s)) \

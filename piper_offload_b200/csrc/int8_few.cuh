@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
   const int rank = p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
   const int from = all * rank / p.split, to = all * (rank + 1) / p.split;
   const TileAt t{0, static_cast<int32_t>(blockIdx.x) / p.split, 0, p.tokens, 0};
-  // one, two, four or eight warps a token; their first loads are under way while the barriers and tensor memory are set up
+  // one, two, four or eight warps a token
   const int mine = warp - 2, each = p.tokens > 4 ? 1 : p.tokens > 2 ? 2 : p.tokens > 1 ? 4 : 8;
   const int token = max(mine, 0) / each, step = 32 * each, first = (max(mine, 0) % each) * 32 + lane;
   const bool has = mine >= 0 && token < p.tokens;
@@ -65,10 +65,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     return p.x_vec != 0 ? load_unit<DT, true>(row, unit * kUnit, p.cols) : load_unit<DT, false>(row, unit * kUnit, p.cols);
   };
   const int units = (p.cols + kUnit - 1) / kUnit;
-  Unit<DT> held[kFewHold];
-#pragma unroll
-  for (int k = 0; k < kFewHold; ++k)
-    if (has && first + k * step < units) held[k] = load(first + k * step);
+  fp4::grid_launch_dependents();
   if (warp == 0 && fp4::elect_one()) {
     pm::prefetch_tmap(&p.w_map);
     for (int s = 0; s < p.ring; ++s) {
@@ -83,6 +80,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) linear_few_kernel(const __grid
     pm::tmem_alloc(tmem_at, 32);
     pm::tmem_relinquish();
   }
+  fp4::grid_wait();
+  Unit<DT> held[kFewHold];
+#pragma unroll
+  for (int k = 0; k < kFewHold; ++k)
+    if (has && first + k * step < units) held[k] = load(first + k * step);
   pm::tc_fence_before();
   __syncthreads();
   pm::tc_fence_after();

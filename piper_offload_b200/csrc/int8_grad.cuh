@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  fp4::grid_launch_dependents();
   if (warp == 0 && lane == 0) {
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {

@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  fp4::grid_launch_dependents();
   const uint32_t rank = fp4::cluster_rank();
   const int stages = (p.cols + kStageCols - 1) / kStageCols;
   const int first_item = blockIdx.x / 2, item_step = gridDim.x / 2;

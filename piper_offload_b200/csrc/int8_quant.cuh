@@ -417,6 +417,8 @@ template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(prepare_threads(kWarps)) quantize_kernel(const __grid_constant__ QuantArgs q, const __grid_constant__ RepackArgs r,
                                                                    uint32_t token_blocks) {
   __shared__ uint32_t words[2 * kWarps];
+  // in this order: the product that follows reads the ends of groups and loads its weight as soon as it begins
+  fp4::grid_wait();
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) quantize_rows<DT, kWarps, kHold, kVec>(q, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);
@@ -427,6 +429,7 @@ template <int DT, int kWarps, int kHold, bool kVec>
 __global__ void __launch_bounds__(prepare_threads(kWarps)) scale_kernel(const __grid_constant__ ScaleArgs s, const __grid_constant__ RepackArgs r,
                                                                 uint32_t token_blocks) {
   __shared__ uint32_t words[2 * kWarps];
+  fp4::grid_wait();  // first, as in quantize_kernel
   fp4::grid_launch_dependents();
   if (blockIdx.x < token_blocks) scale_rows<DT, kWarps, kHold, kVec>(s, blockIdx.x, words);
   else repack(r, static_cast<int64_t>(blockIdx.x - token_blocks) * prepare_threads(kWarps) + threadIdx.x);

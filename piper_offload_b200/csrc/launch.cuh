@@ -1,0 +1,32 @@
+// launch.cuh - launches that may begin while the launch before them ends (programmatic stream serialization).
+//
+// A kernel launched so begins with grid_launch_dependents(), which lets the next such launch set itself up, and
+// grid_wait(), which ends when all launches before it have ended and their writes are visible; it touches no memory before.
+// What a kernel does before its wait has to need nothing of them: an INT8 product loads its weight then and reads the ends of
+// its groups, as a gradient does, so the launches before those (quantize_kernel, scale_kernel) wait first and let them begin
+// after. In a program's stream this takes the start of a launch,
+// 1.5 to 2.5 us, out of the time between two of them: 1 x 14336 x 4096 16.0 -> 13.3 us a call.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace piper {
+
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), int64_t blocks, int threads, size_t smem, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attributes;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+}  // namespace piper

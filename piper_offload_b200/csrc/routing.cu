@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <initializer_list>
 
+#include "launch.cuh"
 #include "routing_exchange.cuh"
 #include "routing_route.cuh"
 
@@ -50,9 +51,13 @@ cudaError_t launched() {
   return cudaGetLastError();
 }
 
-// Above 48 KB a kernel has to be allowed its shared memory.
-cudaError_t allow_shared(const void* kernel, size_t bytes) {
-  return bytes <= 48 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+template <class Args>
+cudaError_t enqueue(void (*kernel)(Args), int64_t blocks, int threads, size_t smem, cudaStream_t stream, const Args& args) {
+  cudaError_t e = cudaSuccess;
+  // above 48 KB a kernel has to be allowed its shared memory
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess) e = piper::launch(kernel, blocks, threads, smem, 1, stream, args);
+  return e == cudaSuccess ? launched() : e;
 }
 
 int check_dtype(int dtype) {
@@ -143,9 +148,7 @@ cudaError_t launch_route(routing::RouteArgs a, int threads, cudaStream_t s) {
   const size_t lists = threads / 32 * sizeof(routing::Lists<N>), places = place_bytes(a.pitch, threads);
   const auto kernel = a.chunks == 1 ? routing::route_kernel<DT, N, true> : routing::route_kernel<DT, N, false>;
   const size_t smem = a.pitch * 4 + (a.chunks == 1 ? std::max(lists, places) : lists);
-  if (const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), smem); e != cudaSuccess) return e;
-  kernel<<<static_cast<unsigned>(a.chunks), threads, smem, s>>>(a);
-  return launched();
+  return enqueue(kernel, a.chunks, threads, smem, s, a);
 }
 
 template <int DT>
@@ -162,8 +165,7 @@ cudaError_t launch_route(const routing::RouteArgs& a, cudaStream_t s) {
 template <int DT, int N>
 cudaError_t launch_route_grad(routing::RouteGradArgs a, cudaStream_t s) {
   a.route.vec = whole_pieces(a.route.logits, a.route.stride, a.route.experts, N, width(DT));
-  routing::route_grad_kernel<DT, N><<<static_cast<unsigned>((a.route.tokens + 7) / 8), 256, 0, s>>>(a);
-  return launched();
+  return enqueue(routing::route_grad_kernel<DT, N>, (a.route.tokens + 7) / 8, 256, 0, s, a);
 }
 
 template <int DT>
@@ -273,21 +275,7 @@ int piper_routing_route(const piper_routing_config* c, const void* logits, int64
 #undef CALL
   if (e != cudaSuccess) return cuda_fail("route kernel", e);
   if (n.count == 1) return PIPER_ROUTING_OK;
-  // may start while the choices are still made; it waits for them
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(n.count));
-  config.blockDim = dim3(1024);
-  config.dynamicSmemBytes = place_bytes(a.pitch, 1024);
-  if ((e = allow_shared(reinterpret_cast<const void*>(routing::place_kernel), config.dynamicSmemBytes)) != cudaSuccess)
-    return cuda_fail("place kernel", e);
-  config.stream = s;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  e = cudaLaunchKernelEx(&config, routing::place_kernel, a);
-  if (e == cudaSuccess) e = launched();
+  e = enqueue(routing::place_kernel, n.count, 1024, place_bytes(a.pitch, 1024), s, a);
   return e == cudaSuccess ? PIPER_ROUTING_OK : cuda_fail("place kernel", e);
 }
 
@@ -326,10 +314,10 @@ int piper_routing_dispatch(const piper_routing_exchange* x, const void* in, int6
   a.out = out;
   const int64_t blocks = (x->tokens * a.pieces + routing::kExchangeThreads - 1) / routing::kExchangeThreads;
   ROUTING_REQUIRE(blocks < (int64_t{1} << 31), "Dispatch: too many values for one call.");
-#define CALL(D, V) routing::dispatch_kernel<D, V><<<static_cast<unsigned>(blocks), routing::kExchangeThreads, 0, static_cast<cudaStream_t>(stream)>>>(a)
+  cudaError_t e = cudaSuccess;
+#define CALL(D, V) e = enqueue(routing::dispatch_kernel<D, V>, blocks, routing::kExchangeThreads, 0, static_cast<cudaStream_t>(stream), a)
   EXCHANGE_DISPATCH(x->dtype, values > 1, CALL);
 #undef CALL
-  const cudaError_t e = launched();
   return e == cudaSuccess ? PIPER_ROUTING_OK : cuda_fail("dispatch kernel", e);
 }
 
@@ -349,15 +337,14 @@ int piper_routing_combine(const piper_routing_exchange* x, const void* y, int64_
   const int64_t each = routing::kExchangeThreads * (routing::kAtOnce / choices_at_once(x->top_k));
   const int64_t blocks = (x->tokens * a.pieces + each - 1) / each;
   ROUTING_REQUIRE(blocks < (int64_t{1} << 31), "Combine: too many values for one call.");
-  const auto grid = static_cast<unsigned>(blocks);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define CALL(D, V)                                                                                                            \
-  if (choices_at_once(x->top_k) == 2) routing::combine_kernel<D, V, 2><<<grid, routing::kExchangeThreads, 0, s>>>(a);            \
-  else if (choices_at_once(x->top_k) == 4) routing::combine_kernel<D, V, 4><<<grid, routing::kExchangeThreads, 0, s>>>(a);       \
-  else routing::combine_kernel<D, V, 8><<<grid, routing::kExchangeThreads, 0, s>>>(a)
+  cudaError_t e = cudaSuccess;
+#define CALL(D, V)                                                                                                       \
+  e = choices_at_once(x->top_k) == 2   ? enqueue(routing::combine_kernel<D, V, 2>, blocks, routing::kExchangeThreads, 0, s, a) \
+      : choices_at_once(x->top_k) == 4 ? enqueue(routing::combine_kernel<D, V, 4>, blocks, routing::kExchangeThreads, 0, s, a) \
+                                       : enqueue(routing::combine_kernel<D, V, 8>, blocks, routing::kExchangeThreads, 0, s, a)
   EXCHANGE_DISPATCH(x->dtype, values > 1, CALL);
 #undef CALL
-  const cudaError_t e = launched();
   return e == cudaSuccess ? PIPER_ROUTING_OK : cuda_fail("combine kernel", e);
 }
 
@@ -380,19 +367,16 @@ int piper_routing_combine_grad(const piper_routing_exchange* x, const void* y, i
   a.out = dy;
   a.dweights = dweights;
   const bool wide_blocks = x->tokens < 32 * sm_count();  // too few tokens to fill the SMs with a warp each
-  const auto grid = static_cast<unsigned>(wide_blocks ? x->tokens : (x->tokens + 7) / 8);
+  const int64_t blocks = wide_blocks ? x->tokens : (x->tokens + 7) / 8;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define LAUNCH(D, V, K)                                                                                                  \
-  if (wide_blocks) routing::combine_grad_kernel<D, V, K, 8><<<grid, routing::kExchangeThreads, 0, s>>>(a);                \
-  else routing::combine_grad_kernel<D, V, K, 1><<<grid, routing::kExchangeThreads, 0, s>>>(a)
-#define CALL(D, V)                                              \
-  if (choices_at_once(x->top_k) == 2) { LAUNCH(D, V, 2); }      \
-  else if (choices_at_once(x->top_k) == 4) { LAUNCH(D, V, 4); } \
-  else { LAUNCH(D, V, 8); }
+  cudaError_t e = cudaSuccess;
+#define ENQUEUE(D, V, K)                                                                                               \
+  (wide_blocks ? enqueue(routing::combine_grad_kernel<D, V, K, 8>, blocks, routing::kExchangeThreads, 0, s, a)          \
+               : enqueue(routing::combine_grad_kernel<D, V, K, 1>, blocks, routing::kExchangeThreads, 0, s, a))
+#define CALL(D, V) e = choices_at_once(x->top_k) == 2 ? ENQUEUE(D, V, 2) : choices_at_once(x->top_k) == 4 ? ENQUEUE(D, V, 4) : ENQUEUE(D, V, 8)
   EXCHANGE_DISPATCH(x->dtype, values > 1, CALL);
 #undef CALL
-#undef LAUNCH
-  const cudaError_t e = launched();
+#undef ENQUEUE
   return e == cudaSuccess ? PIPER_ROUTING_OK : cuda_fail("combine gradient kernel", e);
 }
 

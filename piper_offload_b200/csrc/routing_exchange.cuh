@@ -90,6 +90,8 @@ __device__ __forceinline__ int32_t place_of(const ExchangeArgs& p, int64_t token
 // A thread has a piece of a token. It writes the copies, and zeros in the rows of no choice among [t top_k, (t + 1) top_k).
 template <int DT, int V>
 __global__ void __launch_bounds__(kExchangeThreads) dispatch_kernel(const __grid_constant__ ExchangeArgs p) {
+  fp4::grid_launch_dependents();
+  fp4::grid_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kExchangeThreads + threadIdx.x;
   const int64_t token = i / p.pieces;
   if (token >= p.tokens) return;
@@ -108,6 +110,8 @@ constexpr int kAtOnce = 8;  // loads of rows that a thread has in flight: of K c
 // A thread has kAtOnce / K pieces of tokens' results.
 template <int DT, int V, int K>
 __global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2) combine_kernel(const __grid_constant__ ExchangeArgs p) {
+  fp4::grid_launch_dependents();
+  fp4::grid_wait();
   constexpr int kPieces = kAtOnce / K;
   int64_t token[kPieces], col[kPieces];
   float sum[kPieces][V];
@@ -154,6 +158,8 @@ __global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2)
 // weights' gradients.
 template <int DT, int V, int K, int kWarps>
 __global__ void __launch_bounds__(kExchangeThreads, 2) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
+  fp4::grid_launch_dependents();
+  fp4::grid_wait();
   constexpr int kPieces = kAtOnce / K, kStep = 32 * kWarps;
   __shared__ float parts[kWarps > 1 ? K * 8 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

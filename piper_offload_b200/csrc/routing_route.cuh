@@ -689,6 +689,7 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
   extern __shared__ __align__(16) int32_t shared[];  // choices of each expert; kOne: and the starts
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   fp4::grid_launch_dependents();
+  fp4::grid_wait();
   for (int e = threadIdx.x; e < p.pitch; e += blockDim.x) shared[e] = 0;
   __syncthreads();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.chunk, end = min(first + p.chunk, p.tokens);
@@ -730,6 +731,7 @@ __global__ void __launch_bounds__(N >= 16 ? 512 : 1024) route_kernel(const __gri
 
 __global__ void __launch_bounds__(1024) place_kernel(const __grid_constant__ RouteArgs p) {
   extern __shared__ __align__(16) int32_t shared[];
+  fp4::grid_launch_dependents();
   fp4::grid_wait();
   place(p, p.counts, shared, shared + p.pitch + 32);
 }
@@ -756,6 +758,8 @@ template <int DT, int N>
 __global__ void __launch_bounds__(256) route_grad_kernel(const __grid_constant__ RouteGradArgs a) {
   const RouteArgs& p = a.route;
   const int lane = threadIdx.x & 31;
+  fp4::grid_launch_dependents();
+  fp4::grid_wait();
   const int64_t token = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (token >= p.tokens) return;
   const int chosen = lane < p.top_k ? p.experts_out[token * p.top_k + lane] : -1;
