@@ -44,6 +44,16 @@ __device__ __forceinline__ Pack<DT, V> load_pack(const void* p, int64_t at) {
   return r;
 }
 
+// The same, of what nothing reads again: it leaves the cache first.
+template <int DT, int V>
+__device__ __forceinline__ Pack<DT, V> load_pack_once(const void* p, int64_t at) {
+  if constexpr (V == 1) return load_pack<DT, V>(p, at);
+  Pack<DT, V> r;
+  const uint4 q = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == kF32 ? 4 : 2)));
+  r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+  return r;
+}
+
 template <int DT, int V>
 __device__ __forceinline__ void store_pack(void* p, int64_t at, const Pack<DT, V>& r) {
   if constexpr (V == 1) {
@@ -107,7 +117,8 @@ __global__ void __launch_bounds__(kExchangeThreads) dispatch_kernel(const __grid
 
 constexpr int kAtOnce = 8;  // loads of rows that a thread has in flight: of K choices for each of kAtOnce / K pieces
 
-// A thread has kAtOnce / K pieces of tokens' results.
+// A thread has kAtOnce / K pieces of tokens' results. Of eight choices the rows leave the cache first (8,192 tokens of 8 x
+// 2,048 bf16: 51 us, 56 without; 8,192 of 6 x 1,000: 24 and 27), of fewer not (4,096 of 4 x 4,096: 37 with, 36 without).
 template <int DT, int V, int K>
 __global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2) combine_kernel(const __grid_constant__ ExchangeArgs p) {
   fp4::grid_launch_dependents();
@@ -134,7 +145,8 @@ __global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2)
         const int32_t r = token[q] < p.tokens && j0 + k < p.top_k ? place_of(p, token[q], j0 + k) : -1;
         has[q][k] = r >= 0;
         if (r >= 0) {
-          v[q][k] = load_pack<DT, V>(p.in, static_cast<int64_t>(r) * p.in_stride + col[q]);
+          const int64_t at = static_cast<int64_t>(r) * p.in_stride + col[q];
+          v[q][k] = K == 8 ? load_pack_once<DT, V>(p.in, at) : load_pack<DT, V>(p.in, at);
           w[q][k] = p.weights != nullptr ? p.weights[token[q] * p.top_k + j0 + k] : 1.0f;
         }
       }
@@ -155,9 +167,11 @@ __global__ void __launch_bounds__(kExchangeThreads, K == 8 ? 4 : K == 4 ? 3 : 2)
 }
 
 // kWarps warps have a token: each piece of the result's gradient goes to the rows' gradients, and with the rows into the
-// weights' gradients.
+// weights' gradients. Blocks an SM: with eight choices more than two cost registers that the loads in flight need (8,192
+// tokens of 8 x 2,048 bf16: 105 us with two, 113 with three); fewer choices gain (4,096 of 4 x 4,096: 48 with four, 51 with
+// three, 59 with two), and so do single values (3,000 of 8 x 2,047: 80 with three, 93 with four, 114 with two).
 template <int DT, int V, int K, int kWarps>
-__global__ void __launch_bounds__(kExchangeThreads, 2) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
+__global__ void __launch_bounds__(kExchangeThreads, V == 1 ? 3 : K == 8 ? 2 : 4) combine_grad_kernel(const __grid_constant__ ExchangeArgs p) {
   fp4::grid_launch_dependents();
   fp4::grid_wait();
   constexpr int kPieces = kAtOnce / K, kStep = 32 * kWarps;
