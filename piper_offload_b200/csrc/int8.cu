@@ -362,7 +362,6 @@ GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool g
   const double one = std::max(560.0, 250.0 + 2.2 * static_cast<double>(std::min<int64_t>(per_expert, t.bn)));
   const TilePlan alone = plan_tile(t.bn, tiles(128, t.bn), stages, one, std::min<int64_t>(per_expert, t.bn), !grouped, sm_count());
   double best = alone.cycles;
-  if (t.bn == 256)
     for (int rows = 1; rows <= 2; ++rows)
       for (int tile = 256; tile >= 128; tile -= 32) {
         const double n = static_cast<double>(std::min<int64_t>(up(per_expert, 32), tile));
@@ -372,6 +371,7 @@ GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool g
         if (cycles < best) {
           best = cycles;
           t.pair = true;
+          t.bn = 256;
           t.rows = rows;
           t.tokens = tile;
         }

@@ -18,7 +18,7 @@
 namespace i8 {
 
 constexpr int kGradStageRows = 64;   // rows of w per stage
-constexpr int kDecodeWarps = 8;      // for 64 rows x 128 columns; two such teams a block, which run the epilogue too
+constexpr int kDecodeWarps = 16;     // of a block, which run the epilogue too
 
 struct GradArgs {
   CUtensorMap dy_map;   // (terms * tokens, rows of w) fp16
@@ -45,64 +45,65 @@ struct GradShape {
   static constexpr int kRoom = kSmemMax - 3072 - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 512;
-  static constexpr int kThreads = 64 + 32 * kDecodeWarps * 2;  // producer warp, tensor-core warp, decoding warps
-  static constexpr int kTurns = 2 / kRows;  // teams that take stages in turn
+  static constexpr int kThreads = 64 + 32 * kDecodeWarps;  // producer warp, tensor-core warp, decoding warps
+  static constexpr int kTeams = 4 / kRows;  // of decoding warps, which take stages in turn: 64 codes a thread and stage
+  static constexpr int kTeamWarps = kDecodeWarps / kTeams;
   static constexpr int kAlloc = tmem_columns(kRows * BN);
   static constexpr bool kCanSplit = !kPair && kRows == 1 && BN * kTileRows * 4 <= kStages * kStage;
-  static_assert(kRows * BN <= kAlloc && kStages >= 3, "the tile does not fit");
+  static_assert(kRows * BN <= kAlloc && kStages >= kTeams, "the tile does not fit");
 };
 
-// A thread's share of 64 rows x 128 columns: 16 codes of a row, 16 of the fourth after it, and their zero points. The eight
-// lanes of a row load its 128 bytes together.
+// A thread's share of a stage: 16 codes of every fourth row of four / kRows, of each 128 columns, and the rows' zero points.
+template <int kRows>
 struct Piece {
-  uint4 codes[2];
-  int32_t zero[2];
+  uint4 codes[4 / kRows][kRows];
+  int32_t zero[4 / kRows];
 };
 
-// Walks down the weight in stages: this thread's rows of each, 16 columns from `col` on.
+// Walks down the weight in every kTeams-th stage: this thread's rows of each, at its columns. What lies past the last row or
+// column is some other code: gradients are zero there, and columns past the last are not stored.
+template <int kRows>
 struct PieceWalk {
+  static constexpr int kTeams = 4 / kRows;
   const uint8_t* codes;
   const int8_t* zero;
-  int64_t second, step;  // bytes to the second row; to the next stage
-  int row, rows, zero_step;
-  bool there;
+  uint32_t pitch, zero_step, next_columns;  // bytes to the second 128 columns
+  int in_stage, last, block, blocks;
 
-  __device__ __forceinline__ void begin(const GradArgs& p, int64_t expert, int block, int in_stage, int col) {
-    row = block * kGradStageRows + in_stage;
-    rows = p.rows;
-    there = col < p.code_pitch;  // the pitch is a multiple of 16
-    const int64_t r = expert * p.rows + row;
-    codes = p.codes + r * p.code_pitch + (there ? col : 0);
-    second = 4 * p.code_pitch;
-    step = kGradStageRows * p.code_pitch;
-    zero_step = p.zero_step;
+  __device__ __forceinline__ void begin(const GradArgs& p, int64_t expert, int row_in_stage, int col, int apart, int first, int all) {
+    const int64_t r = expert * p.rows;
+    const int64_t at = col < p.code_pitch ? col : 0;  // the pitch is a multiple of 16
+    codes = p.codes + r * p.code_pitch + at;
+    next_columns = at + apart < p.code_pitch ? apart : 0;
     zero = p.zero != nullptr ? p.zero + r * p.zero_step : nullptr;
+    pitch = static_cast<uint32_t>(p.code_pitch);
+    zero_step = static_cast<uint32_t>(p.zero_step);
+    in_stage = row_in_stage;
+    last = p.rows - 1;
+    block = first;
+    blocks = all;
   }
 
-  __device__ __forceinline__ Piece load() const {
-    // a code of zero where there is none
-    Piece out{{make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)}, {0, 0}};
-    if (there && row < rows) out.codes[0] = *reinterpret_cast<const uint4*>(codes);
-    if (there && row + 4 < rows) out.codes[1] = *reinterpret_cast<const uint4*>(codes + second);
-    if (zero != nullptr) {
-      if (row < rows) out.zero[0] = *zero;
-      if (row + 4 < rows) out.zero[1] = zero[4 * zero_step];
+  __device__ __forceinline__ void load(Piece<kRows>& out) {
+#pragma unroll
+    for (int q = 0; q < 4 / kRows; ++q) {
+      const uint64_t row = static_cast<uint32_t>(min(block * kGradStageRows + in_stage + 4 * q, last));
+      const uint8_t* at = codes + row * pitch;
+#pragma unroll
+      for (int h = 0; h < kRows; ++h) out.codes[q][h] = *reinterpret_cast<const uint4*>(at + (h == 0 ? 0u : next_columns));
+      if (zero != nullptr) out.zero[q] = zero[row * zero_step];
     }
-    return out;
-  }
-
-  __device__ __forceinline__ void next() {
-    codes += step;
-    if (zero != nullptr) zero += kGradStageRows * zero_step;
-    row += kGradStageRows;
+    block += kTeams;
+    if (block >= blocks) block %= blocks;  // the next term
   }
 };
 
-// Four codes less the zero point, as fp16 in their order. `off`: 1024 + 128 + zero point, twice.
-__device__ __forceinline__ void decode4(uint32_t codes, __half2 off, uint32_t& lo, uint32_t& hi) {
-  const uint32_t u = codes ^ 0x80808080u;  // code + 128
+// Four codes, their signs flipped (code + 128), less the zero point, as fp16 in their order. `off`: 1024 + 128 + zero point,
+// twice.
+__device__ __forceinline__ void decode4(uint32_t u, uint32_t off, uint32_t& lo, uint32_t& hi) {
   const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);  // 1024 + code + 128
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  const __half2 o = *reinterpret_cast<const __half2*>(&off);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), o), y = __hsub2(*reinterpret_cast<const __half2*>(&b), o);
   lo = *reinterpret_cast<const uint32_t*>(&x);
   hi = *reinterpret_cast<const uint32_t*>(&y);
 }
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1);
-      pm::mbar_init(&ready[s], kDecodeWarps * kRows * (kPair ? 2 : 1));  // of one team, or of both halves'
+      pm::mbar_init(&ready[s], S::kTeamWarps * (kPair ? 2 : 1));
       pm::mbar_init(&empty[s], 1);
     }
     pm::mbar_init(done, 1);
@@ -236,66 +237,66 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
       }
       __syncwarp();
     } else {
-      // a team has 128 columns of every stage, or of every second one: a warp decodes eight rows, eight lanes a row
-      const int team = (warp - 2) / kDecodeWarps;
-      const int h = kRows == 2 ? team : 0, turn = kRows == 2 ? 0 : team;
-      const int r = (warp - 2) % kDecodeWarps * 8 + (lane >> 3), chunk = lane & 7;
-      const int col = column_tile(h) * kTileRows + chunk * 16;
-      uint8_t* const to_row = smem + h * (kGradStageRows * kTileRows * 2) + (chunk >> 2) * (kGradStageRows * 128) + r * 128;
-      PieceWalk walk;
-      int block = (from + turn) % blocks;  // of the next loads
-      walk.begin(p, t.expert, block, r, col);
-      const auto load_next = [&]() {
-        const Piece piece = walk.load();
-#pragma unroll
-        for (int j = 0; j < S::kTurns; ++j) {
-          walk.next();
-          if (++block == blocks) {  // the next term
-            block = 0;
-            walk.begin(p, t.expert, 0, r, col);
-          }
-        }
-        return piece;
-      };
+      // Eight lanes have 64 columns of two rows: of a row's eight 16-byte pieces, XORed with the row, four lanes write the
+      // even ones while the four of the row below write the odd ones, to all banks at once.
+      const int turn = (warp - 2) / S::kTeamWarps;
+      const int r = (warp - 2) % S::kTeamWarps * (16 / kRows) + (lane >> 4) * 2 + (lane >> 2 & 1), right = lane >> 3 & 1, chunk = lane & 3;
+      const int at = right * (kGradStageRows * 128) + r * 128 + ((chunk * 2 ^ (r & 7)) << 4);
+      const int places[4] = {at, at ^ 16, at ^ 64, at ^ 80};  // of both halves of 16 codes, in rows r + 8 n; in rows r + 4 + 8 n
       if (const int i = threadIdx.x - 64; i < BN) token_scale[i] = i < t.count ? p.back[t.first + i] : 0.0f;
-      Piece soon = load_next(), later = load_next();  // this team's next stage's, the one after's
-      fp4::Ring<S::kStages> ring;
-      if (turn == 1) ring.next();
+      PieceWalk<kRows> walk;
+      walk.begin(p, t.expert, r, column_tile(0) * kTileRows + right * 64 + chunk * 16, kPair ? 2 * kTileRows : kTileRows,
+                 (from + turn) % blocks, blocks);
+      Piece<kRows> piece;
+      walk.load(piece);
+      const bool zeros = p.zero != nullptr;
+      int slot = turn;
+      uint32_t round = 0;
       bool ok = true;
-      for (int i = from + turn; i < to; i += S::kTurns) {
-        const Piece now = soon;
-        soon = later;
-        if (i + 2 * S::kTurns < to) later = load_next();
+      for (int i = from + turn; i < to; i += S::kTeams) {
+        uint32_t u[4 / kRows][kRows][4], off[4 / kRows];
+#pragma unroll
+        for (int q = 0; q < 4 / kRows; ++q) {
+#pragma unroll
+          for (int h = 0; h < kRows; ++h) {
+            u[q][h][0] = piece.codes[q][h].x ^ 0x80808080u;
+            u[q][h][1] = piece.codes[q][h].y ^ 0x80808080u;
+            u[q][h][2] = piece.codes[q][h].z ^ 0x80808080u;
+            u[q][h][3] = piece.codes[q][h].w ^ 0x80808080u;
+          }
+          off[q] = 0x64806480u + (zeros ? static_cast<uint32_t>(piece.zero[q]) * 0x10001u : 0u);  // fp16's whole numbers from 1024 on
+        }
+        if (i + S::kTeams < to) walk.load(piece);
         if (i - from >= S::kStages) {
-          ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad));
+          ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[slot], round ^ 1u, pm::kStatusTimeoutLoad));
           if (!ok) break;
         }
+        uint8_t* const stage = smem + slot * S::kStage;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const __half2 off = __half2half2(__int2half_rn(1152 + now.zero[q]));
-          uint4 lo, hi;
-          decode4(now.codes[q].x, off, lo.x, lo.y);
-          decode4(now.codes[q].y, off, lo.z, lo.w);
-          decode4(now.codes[q].z, off, hi.x, hi.y);
-          decode4(now.codes[q].w, off, hi.z, hi.w);
-          // 16-byte pieces 2 (chunk % 4) and the next, XORed with the row; the lanes of one 64-column block begin with the
-          // first and those of the other with the second, so that the eight of a row write to different banks
-          uint8_t* row = to_row + ring.slot * S::kStage + q * 4 * 128;
-          const int at = (chunk & 3) * 2, swizzle = (r + q * 4) & 7;
-          const bool other = chunk >= 4;
-          *reinterpret_cast<uint4*>(row + (((at + other) ^ swizzle) << 4)) = other ? hi : lo;
-          *reinterpret_cast<uint4*>(row + (((at + !other) ^ swizzle) << 4)) = other ? lo : hi;
-        }
+        for (int q = 0; q < 4 / kRows; ++q)
+#pragma unroll
+          for (int h = 0; h < kRows; ++h) {
+            uint4 lo, hi;
+            decode4(u[q][h][0], off[q], lo.x, lo.y);
+            decode4(u[q][h][1], off[q], lo.z, lo.w);
+            decode4(u[q][h][2], off[q], hi.x, hi.y);
+            decode4(u[q][h][3], off[q], hi.z, hi.w);
+            uint8_t* const to_piece = stage + h * (kGradStageRows * kTileRows * 2) + q * 512;
+            *reinterpret_cast<uint4*>(to_piece + places[2 * (q & 1)]) = lo;
+            *reinterpret_cast<uint4*>(to_piece + places[2 * (q & 1) + 1]) = hi;
+          }
         pm::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (kPair) mbar_arrive_pair(in_block(pm::smem_u32(&ready[ring.slot]), 0));
-          else pm::mbar_arrive(&ready[ring.slot]);
+          if constexpr (kPair) mbar_arrive_pair(in_block(pm::smem_u32(&ready[slot]), 0));
+          else pm::mbar_arrive(&ready[slot]);
         }
-#pragma unroll
-        for (int j = 0; j < S::kTurns; ++j) ring.next();
+        if ((slot += S::kTeams) >= S::kStages) {
+          slot -= S::kStages;
+          round ^= 1u;
+        }
       }
-      pm::named_bar_sync(1, 32 * kDecodeWarps * 2);  // the tokens' scales are written
+      pm::named_bar_sync(1, 32 * kDecodeWarps);  // the tokens' scales are written
       ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(done, 0, pm::kStatusTimeoutMma));
       pm::tc_fence_after();
       if (ok) {
@@ -304,11 +305,12 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
           if (warp < 6) fp4::store_sums(tmem, t, reinterpret_cast<float*>(smem));
         } else {
           uint8_t* mine = smem + (warp - 2) * 2048;
+          const int h = kRows == 2 ? (warp - 2) / 8 : 0;
           TileAt part = t;
           part.row_tile = column_tile(h);
           // 4 / kRows warps for each quarter of the lanes: a share of the tokens each
           constexpr int kShare = BN * kRows / 4 < 32 ? 32 : BN * kRows / 4;
-          const int share = (kRows == 2 ? (warp - 2) % kDecodeWarps : warp - 2) / 4;
+          const int share = (kRows == 2 ? (warp - 2) % 8 : warp - 2) / 4;
           store_tile<DT, false>(tmem + h * BN, p.dx, part, p.cols, none, 0, token_scale, nullptr, share * kShare,
                                 min((share + 1) * kShare, BN), mine, p.vec != 0);
         }

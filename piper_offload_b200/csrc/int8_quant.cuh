@@ -293,21 +293,21 @@ template <int DT, int kWarps, int kHold, bool kVec>
 __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, uint32_t* words) {
   const RowTeam<kWarps> team(block);
   if (kWarps == 1 && team.row >= p.tokens) return;
-  const int expert = expert_of(p.ends, p.experts, static_cast<int>(team.row));
-  if (expert == p.experts) return;  // rows of no expert are not read
   constexpr int kStep = 32 * kWarps;
-  const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
   const uint8_t* row = static_cast<const uint8_t*>(p.dy) + team.row * p.dy_stride * (DT == kF32 ? 4 : 2);
   const int units = static_cast<int>(p.pitch / kUnit);
   const int first_loose = team.thread + kHold * kStep;
+  Unit<DT> u[kHold];  // under way while the expert is found
+#pragma unroll
+  for (int k = 0; k < kHold; ++k)
+    if (team.thread + k * kStep < units) u[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
+  const int expert = expert_of(p.ends, p.experts, static_cast<int>(team.row));
+  if (expert == p.experts) return;  // rows of no expert
+  const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
   // the first units stay in registers as products
   float held[kHold][kUnit];
   const auto load_held = [&](auto scale_type) {
     constexpr int SDT = decltype(scale_type)::value;
-    Unit<DT> u[kHold];
-#pragma unroll
-    for (int k = 0; k < kHold; ++k)
-      if (team.thread + k * kStep < units) u[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
 #pragma unroll
     for (int k = 0; k < kHold; ++k) {
       if (team.thread + k * kStep < units) {
