@@ -56,8 +56,8 @@ int piper_routing_route_grad(const piper_routing_config* c, const void* logits, 
                              const int32_t* experts, const float* grad, void* dlogits, void* stream);
 
 /* How tokens and choices lie: rows (tokens, top_k) as above, `total` the
- * number of places in use (the last of the ends). A row outside
- * [0, tokens * top_k) counts as none. */
+ * number of places in use (the last of the ends; all of them where it is
+ * larger). A row outside [0, total) counts as none. */
 typedef struct piper_routing_exchange {
   int64_t tokens;
   int32_t top_k;

@@ -342,10 +342,10 @@ GradPlan plan_grad(const piper_int8_matrix& w, int64_t tokens, int dtype) {
 }
 
 // Tiles of a gradient: tokens x columns. Decoding costs the same whatever the tokens, so tiles are as wide in tokens as they
-// go, but for a few, which leave room for more stages. The rough account in cycles a stage is measured: one SM takes 810 for
-// 128 columns x 256 tokens and 560 for few, a pair 1330 for 512 x 256 and 750 for 256 x 256 (2048 x 14336 x 4096 200 us in
-// tiles of 512 on pairs, 222 of 256, on single SMs 220 of 256, 239 of 128; 512 x 4096 x 4096 28.4 on single SMs that share
-// sums, 34 on pairs).
+// go, but for a few, which leave room for more stages. The rough account in cycles a stage was measured: one SM takes 810 for
+// 128 columns x 256 tokens and 560 for few, a pair 1330 for 512 x 256 and 750 for 256 x 256 (2048 x 14336 x 4096 189 us in
+// tiles of 512 on pairs, 200 of 256, on single SMs 233 of 128 x 256; 512 x 4096 x 4096 27 on single SMs that share sums, 30 on
+// pairs; 512 rows of 16 experts of 2048 x 2048 26 in tiles of 512 on pairs, 30 of 128 x 64 on single SMs).
 struct GradTile {
   int bn, rows, split;
   bool pair;
@@ -362,20 +362,20 @@ GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool g
   const double one = std::max(560.0, 250.0 + 2.2 * static_cast<double>(std::min<int64_t>(per_expert, t.bn)));
   const TilePlan alone = plan_tile(t.bn, tiles(128, t.bn), stages, one, std::min<int64_t>(per_expert, t.bn), !grouped, sm_count());
   double best = alone.cycles;
-    for (int rows = 1; rows <= 2; ++rows)
-      for (int tile = 256; tile >= 128; tile -= 32) {
-        const double n = static_cast<double>(std::min<int64_t>(up(per_expert, 32), tile));
-        const double stage = rows == 2 ? std::max(1000.0, 5.2 * n) : std::max(600.0, 2.95 * n);
-        const int64_t room = sm_count() / 2, waves = (tiles(256 * rows, tile) + room - 1) / room;
-        const double cycles = static_cast<double>(waves) * (static_cast<double>(stages) * stage + 2000.0);
-        if (cycles < best) {
-          best = cycles;
-          t.pair = true;
-          t.bn = 256;
-          t.rows = rows;
-          t.tokens = tile;
-        }
+  for (int rows = 1; rows <= 2; ++rows)
+    for (int tile = 256; tile >= 128; tile -= 32) {
+      const double n = static_cast<double>(std::min<int64_t>(up(per_expert, 32), tile));
+      const double stage = rows == 2 ? std::max(1000.0, 5.2 * n) : std::max(600.0, 2.95 * n);
+      const int64_t room = sm_count() / 2, waves = (tiles(256 * rows, tile) + room - 1) / room;
+      const double cycles = static_cast<double>(waves) * (static_cast<double>(stages) * stage + 2000.0);
+      if (cycles < best) {
+        best = cycles;
+        t.pair = true;
+        t.bn = 256;
+        t.rows = rows;
+        t.tokens = tile;
       }
+    }
   t.items = token_tiles(tokens, grouped ? w.batch : 0, t.tokens) * ((w.cols + t.columns() - 1) / t.columns());
   // the account goes by even experts: there may be more tiles, which then are not shared
   if (!t.pair) t.split = plan_tile(t.bn, t.items, stages, one, std::min<int64_t>(tokens, t.bn), !grouped, sm_count()).split;

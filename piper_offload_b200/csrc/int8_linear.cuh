@@ -9,6 +9,10 @@
 // Tokens are quantised by a launch before, which the set-up and the first loads of the weight overlap. Tiles are 32, 64,
 // 128 or 256 tokens wide. Where there are too few tiles for the SMs, a cluster of blocks splits K; each leaves its sums in its own
 // shared memory and every block adds up its share of the tokens over the cluster.
+//
+// With few tokens a weight the weight's bytes bound it (16 rows of 8 experts of 14336 x 4096 59 us, 6.0 TB/s for the 353 MB
+// of the experts that have rows), with some hundred a weight the operands' way from L2: a tile of 128 x 128 brings 32 KB for
+// 256 cycles of products (4096 rows of 32 experts of 2048 x 2048 38 us, 8 of them quantising; 370 MB in the rest).
 #pragma once
 #include <cuda.h>
 

@@ -71,7 +71,7 @@ int check_config(const piper_routing_config* c) {
   ROUTING_REQUIRE(c->experts >= 1 && c->experts <= PIPER_ROUTING_MAX_EXPERTS, "Routing takes 1 to 1024 experts.");
   ROUTING_REQUIRE(c->top_k >= 1 && c->top_k <= PIPER_ROUTING_MAX_TOP_K && c->top_k <= c->experts,
                   "Routing: a token gets 1 to 32 experts, and no more than there are.");
-  ROUTING_REQUIRE(c->tokens >= 0 && c->tokens * c->top_k < (int64_t{1} << 31), "Routing: at most 2^31 choices.");
+  ROUTING_REQUIRE(c->tokens >= 0 && c->tokens < (int64_t{1} << 31) / c->top_k, "Routing: at most 2^31 choices.");
   ROUTING_REQUIRE(c->scoring == PIPER_ROUTING_SOFTMAX || c->scoring == PIPER_ROUTING_SIGMOID, "Routing: unknown scoring.");
   ROUTING_REQUIRE(c->groups >= 1 && c->groups <= PIPER_ROUTING_MAX_GROUPS && c->experts % c->groups == 0,
                   "Routing: 1 to 32 groups of equally many experts.");
@@ -183,7 +183,7 @@ int check_exchange(const piper_routing_exchange* e) {
   ROUTING_REQUIRE(e != nullptr, "Exchange: null description.");
   if (int rc = check_dtype(e->dtype)) return rc;
   ROUTING_REQUIRE(e->top_k >= 1 && e->top_k <= PIPER_ROUTING_MAX_TOP_K, "Exchange: a token has 1 to 32 choices.");
-  ROUTING_REQUIRE(e->tokens >= 0 && e->tokens * e->top_k < (int64_t{1} << 31), "Exchange: at most 2^31 choices.");
+  ROUTING_REQUIRE(e->tokens >= 0 && e->tokens < (int64_t{1} << 31) / e->top_k, "Exchange: at most 2^31 choices.");
   ROUTING_REQUIRE(e->hidden >= 1 && e->hidden <= (1 << 24), "Exchange: tokens have 1 to 2^24 values.");
   ROUTING_REQUIRE(e->tokens == 0 || (e->rows != nullptr && e->total != nullptr), "Exchange: null rows or total.");
   return PIPER_ROUTING_OK;

@@ -19,6 +19,11 @@
 //   together below 2^-17.5. 2^-19 of the sum is above twice its rounding and cut. 256 experts' scores spread over [0, 1]
 //   leave 1 % of the tokens open; all of such a token done again by one warp in 64 bits took 8 us, while its block waited.
 // - fp32 logits that are equal but for the last three bits (16-bit ones lose nothing).
+//
+// The order by expert is two steps: a block counts its tokens' choices by expert, and when all have, every block adds up the
+// counts of the chunks before its own and places its choices. Up to 128 tokens are one launch of one block (64 x 8 logits
+// 7.5 us), else two: 16,384 x 256 fp32 logits in eight groups take 35 us, of which reading them is 3 and issue most of the
+// rest; 777 x 60 take 8, launches and latency. The gradient reads what was chosen again: 9 and 4 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -584,7 +589,7 @@ __device__ __forceinline__ float total_of(const float (&logit)[N], const Row& ro
 // --------------------------------------------------------------------- the order by expert
 // The places of a block's choices, in the order of experts and within one of tokens. counts: choices of each chunk of
 // tokens (chunks, pitch), 16-byte aligned, zeros behind the last expert. Shared: start (pitch + 32) words, parts
-// (place_words). A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
+// (place_bytes of routing.cu). A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
 __device__ __forceinline__ void place(const RouteArgs& p, const int32_t* counts, int32_t* start, int32_t* parts) {
   const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quads = p.pitch >> 2, wide = min(threads, quads <= 32 ? 32 : 1 << (32 - __clz(quads - 1)));

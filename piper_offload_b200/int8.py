@@ -100,7 +100,7 @@ class _Frozen:
             raise ValueError("INT8 operators require non-empty weights.")
         if dims == 3 and not per_row:
             raise ValueError("INT8 experts have a scale for each row.")
-        values = batch * rows if per_row else 1
+        values, scale = batch * rows if per_row else 1, scale.resolve_neg()
         if scale.dtype not in _DTYPES:
             raise ValueError(f"INT8 scales are bfloat16, float16 or float32, got {scale.dtype}.")
         if scale.numel() != values:

@@ -120,7 +120,7 @@ class _Route(torch.autograd.Function):
         x = _rows(logits.detach())
         dlogits = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _call(nat.load().piper_routing_route_grad, x.device, ctypes.byref(ctx.config), x.data_ptr(), x.stride(0), _DTYPES[x.dtype],
-              experts.data_ptr(), grad.contiguous().data_ptr(), dlogits.data_ptr())
+              experts.data_ptr(), grad.resolve_neg().contiguous().data_ptr(), dlogits.data_ptr())
         return dlogits, None, None, None
 
 
@@ -164,7 +164,7 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", 
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (experts,) or bias.device != logits.device:
             raise ValueError("A routing bias is one float32 value per expert on the logits' device.")
-        bias = bias.detach().contiguous()
+        bias = bias.detach().resolve_neg().contiguous()
     if mask is not None:
         if mask.dtype is not torch.bool or mask.shape != (tokens,) or mask.device != logits.device:
             raise ValueError("A routing mask is one bool per token on the logits' device.")
@@ -271,7 +271,7 @@ def combine_tokens(y: torch.Tensor, routing: Routing) -> torch.Tensor:
         return done
     if weights.dtype is not torch.float32 or weights.shape != rows.shape or weights.device != rows.device:
         raise ValueError("A routing's weights are float32, one for each choice.")
-    weights = weights.contiguous()
+    weights = weights.resolve_neg().contiguous()
     _check_tangents(y, weights)
     if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         return _Combine.apply(y, weights, rows, ends)

@@ -59,6 +59,36 @@ def test_layer_in_a_graph(cuda_device):
             assert torch.equal(y, again) and torch.equal(r.source, s.source)
 
 
+def test_training_step_in_a_graph(cuda_device):
+    """The layer with its gradients, captured once and replayed on other tokens and logits: the eager step's bits."""
+    g = torch.Generator(cuda_device).manual_seed(1)
+    up, down = (example.pack(torch.randn(shape, generator=g, device=cuda_device).bfloat16()) for shape in ((6, 80, 128), (6, 128, 80)))
+    x, dy = (torch.randn(300, 128, generator=g, device=cuda_device).bfloat16() for _ in range(2))
+    logits = torch.randn(300, 6, generator=g, device=cuda_device)
+    x.requires_grad_(), logits.requires_grad_()
+
+    def step():
+        r = routing.route_tokens(logits, 2, scoring="sigmoid", bias=logits.detach()[0].clone())
+        h = int8.grouped_linear_int8(routing.dispatch_tokens(x, r), up, r.ends)
+        y = routing.combine_tokens(int8.grouped_linear_int8(h, down, r.ends), r)
+        return y.detach(), *torch.autograd.grad(y, (x, logits), dy)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(300, 128, generator=g, device=cuda_device))
+            logits.copy_(torch.randn(300, 6, generator=g, device=cuda_device))
+        graph.replay()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
+
+
 def test_routing_feeds_the_fp4_products_too(cuda_device):
     g = torch.Generator(cuda_device).manual_seed(0)
     dense = torch.randn(5, 96, 128, generator=g, device=cuda_device).bfloat16()

@@ -339,6 +339,29 @@ def test_rows_outside_count_as_none(cuda_device):
     assert routing.dispatch_tokens(x[:0], no_tokens).shape == (0, 8) and routing.combine_tokens(x[:0], no_tokens).shape == (0, 8)
 
 
+@pytest.mark.parametrize("end", [3, 0, -7, 100])
+def test_places_past_the_last_end_count_as_none(cuda_device, end):
+    """A routing that was not made by route_tokens: the last end decides which places are in use, in every pass alike; an end
+    past all places counts as their number, one below none as none."""
+    rows = torch.tensor([[0, 5], [4, 1], [2, 3]], dtype=torch.int32, device=cuda_device)
+    ends = torch.tensor([1, end], dtype=torch.int32, device=cuda_device)
+    weights = torch.full((3, 2), 2.0, device=cuda_device, requires_grad=True)
+    r = routing.Routing(weights, rows, ends, rows, rows.reshape(-1))
+    used = [max(0, min(6, end)) > place for place in range(6)]
+    x = torch.tensor([[1.0], [2.0], [3.0]], device=cuda_device).expand(3, 8).contiguous().requires_grad_()
+    sent = routing.dispatch_tokens(x, r)
+    assert sent[:, 0].tolist() == [v * u for v, u in zip([1, 2, 3, 3, 2, 1], used)]
+    taken = [[used[p] for p in token] for token in rows.tolist()]
+    (dx,) = torch.autograd.grad(sent.sum(), x)
+    assert dx[:, 0].tolist() == [sum(t) for t in taken]
+    y = torch.arange(1.0, 7, device=cuda_device)[:, None].expand(6, 8).contiguous().requires_grad_()
+    out = routing.combine_tokens(y, r)
+    assert out[:, 0].tolist() == [sum(2 * (p + 1) * u for p, u in zip(*both)) for both in zip(rows.tolist(), taken)]
+    dy, dweights = torch.autograd.grad(out.sum(), (y, weights))
+    assert dy[:, 0].tolist() == [2 * u for u in used]
+    assert dweights.tolist() == [[8 * (p + 1) * u for p, u in zip(*both)] for both in zip(rows.tolist(), taken)]
+
+
 def test_offsets_beyond_32_bits(cuda_device):
     """Rows that end more than 2^32 bytes into their tensors."""
     if torch.cuda.get_device_properties(cuda_device).total_memory < 60e9:
