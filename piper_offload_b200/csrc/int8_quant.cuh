@@ -6,14 +6,13 @@
 // to half a code, where fp32 has 2^-23. For fp32 tokens the remainder decides where the quotient rounds onto a half.
 // A row that holds an infinity or a NaN gets the scale NaN: its products are NaN, and no other row's are touched.
 //
-// Memory bounds it: 4096 x 4096 bf16 to codes 10.4 us, 4.8 TB/s; 2048 x 14336 bf16 gradients to fp16 31 us, 3.8 TB/s, the
-// products that lanes hold leaving registers for two blocks an SM.
+// Memory bounds it, less its latency, which the blocks that registers leave room for do not cover: 4096 x 4096 bf16 to codes
+// 10.4 us, 4.8 TB/s; 2048 x 14336 bf16 gradients to fp16 30 us, 3.9 TB/s.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
-#include <type_traits>
 
 #include "fp4_ptx.cuh"
 
@@ -285,47 +284,17 @@ __device__ __forceinline__ void scaled_unit(const ScaleArgs& p, const Unit<DT>& 
   }
 }
 
-template <int DT, bool kVec>
-__device__ __forceinline__ void scaled_unit_any(const ScaleArgs& p, const Unit<DT>& u, int64_t row0, int n, float (&v)[kUnit]) {
-  if (p.scales.dtype == kBF16) scaled_unit<DT, kBF16, kVec>(p, u, row0, n, v);
-  else if (p.scales.dtype == kF16) scaled_unit<DT, kF16, kVec>(p, u, row0, n, v);
-  else scaled_unit<DT, kF32, kVec>(p, u, row0, n, v);
-}
-
-template <int DT, int kWarps, int kHold, bool kVec>
-__device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, uint32_t* words) {
-  const RowTeam<kWarps> team(block);
-  if (kWarps == 1 && team.row >= p.tokens) return;
+// A row whose values lie at `row`, the first units in `held`. Products are made once for their maximum and once to be
+// written, with scales from L1: kept in between they would take twice the registers of the values.
+template <int DT, int SDT, int kWarps, int kHold, bool kVec>
+__device__ __forceinline__ void scale_row(const ScaleArgs& p, const RowTeam<kWarps>& team, const uint8_t* row, const Unit<DT> (&held)[kHold],
+                                          int64_t row0, int units, uint32_t* words) {
   constexpr int kStep = 32 * kWarps;
-  const uint8_t* row = static_cast<const uint8_t*>(p.dy) + team.row * p.dy_stride * (DT == kF32 ? 4 : 2);
-  const int units = static_cast<int>(p.pitch / kUnit);
-  const int first_loose = team.thread + kHold * kStep;
-  Unit<DT> u[kHold];  // under way while the expert is found
-#pragma unroll
-  for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) u[k] = load_unit<DT, kVec>(row, (team.thread + k * kStep) * kUnit, p.rows);
-  const int expert = expert_of(p.ends, p.experts, static_cast<int>(team.row));
-  if (expert == p.experts) return;  // rows of no expert
-  const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
-  // the first units stay in registers as products
-  float held[kHold][kUnit];
-  const auto load_held = [&](auto scale_type) {
-    constexpr int SDT = decltype(scale_type)::value;
-#pragma unroll
-    for (int k = 0; k < kHold; ++k) {
-      if (team.thread + k * kStep < units) {
-        scaled_unit<DT, SDT, kVec>(p, u[k], row0, (team.thread + k * kStep) * kUnit, held[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) held[k][i] = 0.0f;
-      }
-    }
-  };
-  if (p.scales.dtype == kBF16) load_held(std::integral_constant<int, kBF16>{});
-  else if (p.scales.dtype == kF16) load_held(std::integral_constant<int, kF16>{});
-  else load_held(std::integral_constant<int, kF32>{});
-  const auto loose = [&](int unit, float (&v)[kUnit]) {
-    scaled_unit_any<DT, kVec>(p, load_unit<DT, kVec>(row, unit * kUnit, p.rows), row0, unit * kUnit, v);
+  // of unit k of this lane, one of the row's last units again where it has no more
+  const auto products = [&](int k, float (&v)[kUnit]) {
+    const int n = min(team.thread + k * kStep, units - 1) * kUnit;
+    if (k < kHold) scaled_unit<DT, SDT, kVec>(p, held[k], row0, n, v);
+    else scaled_unit<DT, SDT, kVec>(p, load_unit<DT, kVec>(row, n, p.rows), row0, n, v);
   };
   // the largest magnitude that is a number; infinities only cost a second look
   const auto largest = [&](bool finite) {
@@ -334,11 +303,14 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) top = fmaxf(top, finite && !(fabsf(v[i]) < INFINITY) ? 0.0f : fabsf(v[i]));  // a NaN is not counted
     };
+    float v[kUnit];
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) see(held[k]);
-    for (int u = first_loose; u < units; u += kStep) {
-      float v[kUnit];
-      loose(u, v);
+    for (int k = 0; k < kHold; ++k) {
+      products(k, v);
+      see(v);
+    }
+    for (int k = kHold; team.thread + k * kStep < units; ++k) {
+      products(k, v);
       see(v);
     }
     return team.max_of(__float_as_uint(top), words);
@@ -351,7 +323,9 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
   // 2^(14 - exponent), within fp32's normal numbers; 1 for a row of zeros
   const int exponent = bits == 0u ? 14 : max(static_cast<int>(bits >> 23) - 127, -112);
   const float power = __uint_as_float(static_cast<uint32_t>(141 - exponent) << 23);
-  const auto write = [&](const float (&v)[kUnit], int unit) {
+  const auto write = [&](int k) {
+    float v[kUnit];
+    products(k, v);
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < kUnit; i += 2) {
@@ -364,24 +338,38 @@ __device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, ui
         lo[i / 2] = *reinterpret_cast<const uint32_t*>(&l);
       }
     }
-    uint4* to = reinterpret_cast<uint4*>(p.out + team.row * p.pitch + static_cast<int64_t>(unit) * kUnit);
+    const int64_t at = static_cast<int64_t>(team.thread + k * kStep) * kUnit;
+    uint4* to = reinterpret_cast<uint4*>(p.out + team.row * p.pitch + at);
     to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
     if constexpr (DT == kF32) {
-      to = reinterpret_cast<uint4*>(p.out + (p.tokens + team.row) * p.pitch + static_cast<int64_t>(unit) * kUnit);
+      to = reinterpret_cast<uint4*>(p.out + (p.tokens + team.row) * p.pitch + at);
       to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
     }
   };
 #pragma unroll
   for (int k = 0; k < kHold; ++k)
-    if (team.thread + k * kStep < units) write(held[k], team.thread + k * kStep);
-  for (int u = first_loose; u < units; u += kStep) {
-    float v[kUnit];
-    loose(u, v);
-    write(v, u);
-  }
+    if (team.thread + k * kStep < units) write(k);
+  for (int k = kHold; team.thread + k * kStep < units; ++k) write(k);
   if (team.thread == 0) p.back[team.row] = __uint_as_float(static_cast<uint32_t>(113 + exponent) << 23);
+}
+
+template <int DT, int kWarps, int kHold, bool kVec>
+__device__ __forceinline__ void scale_rows(const ScaleArgs& p, int64_t block, uint32_t* words) {
+  const RowTeam<kWarps> team(block);
+  if (kWarps == 1 && team.row >= p.tokens) return;
+  const uint8_t* row = static_cast<const uint8_t*>(p.dy) + team.row * p.dy_stride * (DT == kF32 ? 4 : 2);
+  const int units = static_cast<int>(p.pitch / kUnit);
+  Unit<DT> held[kHold];  // under way while the expert is found
+#pragma unroll
+  for (int k = 0; k < kHold; ++k) held[k] = load_unit<DT, kVec>(row, min(team.thread + k * 32 * kWarps, units - 1) * kUnit, p.rows);
+  const int expert = expert_of(p.ends, p.experts, static_cast<int>(team.row));
+  if (expert == p.experts) return;  // a row of no expert
+  const int64_t row0 = static_cast<int64_t>(expert) * p.rows;
+  if (p.scales.dtype == kBF16) scale_row<DT, kBF16, kWarps, kHold, kVec>(p, team, row, held, row0, units, words);
+  else if (p.scales.dtype == kF16) scale_row<DT, kF16, kWarps, kHold, kVec>(p, team, row, held, row0, units, words);
+  else scale_row<DT, kF32, kWarps, kHold, kVec>(p, team, row, held, row0, units, words);
 }
 
 // -------------------------------------------------------------------------- codes
