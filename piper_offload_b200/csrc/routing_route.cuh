@@ -589,7 +589,8 @@ __device__ __forceinline__ float total_of(const float (&logit)[N], const Row& ro
 // --------------------------------------------------------------------- the order by expert
 // The places of a block's choices, in the order of experts and within one of tokens. counts: choices of each chunk of
 // tokens (chunks, pitch), 16-byte aligned, zeros behind the last expert. Shared: start (pitch + 32) words, parts
-// (place_bytes of routing.cu). A thread adds up four experts over a share of the chunks, so that most loads of a share are in flight at once.
+// (place_bytes of routing.cu). A thread adds up four experts over a share of the chunks, so that most loads of a share are in
+// flight at once.
 __device__ __forceinline__ void place(const RouteArgs& p, const int32_t* counts, int32_t* start, int32_t* parts) {
   const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quads = p.pitch >> 2, wide = min(threads, quads <= 32 ? 32 : 1 << (32 - __clz(quads - 1)));
