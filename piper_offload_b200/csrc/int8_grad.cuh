@@ -49,7 +49,7 @@ struct GradShape {
   static constexpr int kB = (kPair ? BN / 2 : BN) * kGradStageRows * 2;
   static constexpr int kStage = kA + kB;
   static constexpr int kTokens = BN * 4;
-  static constexpr int kRoom = kSmemMax - 3072 - kTokens;
+  static constexpr int kRoom = kSmemMax - 3 * 1024 - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 512;
   static constexpr int kThreads = 64 + 32 * kDecodeWarps;  // producer warp, tensor-core warp, decoding warps
