@@ -125,10 +125,13 @@ def build_expert_calls(force: bool = False, verbose: bool = False) -> Path:
 
 
 def _compile_calls(out: Path, sources: list[Path], deps: list[Path], force: bool, verbose: bool) -> Path:
-    """Host code against this interpreter's torch, which is noted beside it."""
+    """Host code against this interpreter's torch, which is noted beside it, and the C++ runtime that torch uses. A compiler
+    that comes with the archive of that runtime alone would link a second one in, and a number written into the message of an
+    error then ends the process: its formatting asks the one's locale for the other's parts."""
     import torch
 
-    fits = f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+    runtime = "libstdc++.so.6"
+    fits = f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} {runtime}"
     note = out.with_suffix(".so.fits")
     if force or not up_to_date(out, deps) or not note.exists() or note.read_text() != fits:
         base = Path(torch.__file__).resolve().parent
@@ -137,7 +140,8 @@ def _compile_calls(out: Path, sources: list[Path], deps: list[Path], force: bool
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                *(f"-I{d}" for d in (base / "include", base / "include" / "torch" / "csrc" / "api" / "include",
                                     Path(nvcc()).resolve().parents[1] / "include", sysconfig.get_paths()["include"])),
-               "-o", str(tmp), *map(str, sources), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+               "-o", str(tmp), *map(str, sources), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+               f"-l:{runtime}"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=str(ROOT))
