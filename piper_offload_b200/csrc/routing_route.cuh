@@ -17,14 +17,16 @@
 //   argument d, where d exp(-d) is below 0.37, the fast quotient by 2 steps, a softmax's sum by a step of 2^-24 for each of
 //   at most 37 additions, the cut of three bits by 8 steps of 2^-24 for the sum; together below 2^-17.5. Where scores of
 //   logits are added up they are made of the whole logits: a softmax's error by three bits of a logit grows with the logit,
-//   whatever the score (7 steps of 2^-14 at 1000; 34.1 us without a bias for 16,384 x 256, 32.7 of cut ones). 2^-19 of the
-//   sum is above twice its rounding and cut. 256 experts' scores spread over [0, 1]
+//   whatever the score (7 steps of 2^-14 at 1000; 1.4 us of 34.6 without a bias for 16,384 x 256). 2^-19 of the
+//   sum is above twice its rounding and cut. A group's two best may cancel (biases of +1000 and -1000), so its bounds are
+//   half of 2^-16 and 9 steps of 2^-23 of what was added up: 7 of them cut, a half each for the sum with the bias, for that
+//   of the two and for the bound's own. 256 experts' scores spread over [0, 1]
 //   leave 1 % of the tokens open; all of such a token done again by one warp in 64 bits took 8 us, while its block waited.
 // - fp32 logits that are equal but for the last three bits (16-bit ones lose nothing).
 //
 // The order by expert is two steps: a block counts its tokens' choices by expert, and when all have, every block adds up the
 // counts of the chunks before its own and places its choices. Up to 128 tokens are one launch of one block (64 x 8 logits
-// 7.5 us), else two: 16,384 x 256 fp32 logits in eight groups take 35 us, of which reading them is 3 and issue most of the
+// 7.4 us), else two: 16,384 x 256 fp32 logits in eight groups take 36 us, of which reading them is 3 and issue most of the
 // rest; 777 x 60 take 8, launches and latency. The gradient reads what was chosen again: 9 and 4 us.
 #pragma once
 #include <cuda_bf16.h>
@@ -168,13 +170,22 @@ struct Row {
 // Whether sums of scores decide anything, or the logits alone.
 __device__ __forceinline__ bool scores_decide(const RouteArgs& p) { return p.bias != nullptr || (p.groups > 1 && p.group_score == kTop2); }
 
-constexpr float kMargin = 0x1p-16f, kMarginOfValue = 0x1p-19f;
+constexpr float kMargin = 0x1p-16f, kMarginOfValue = 0x1p-19f, kErrorOfParts = 9 * 0x1p-23f;
 
 // Whether a value is so near one below it that fp32 may have put them in the wrong order. False for what is closed.
 __device__ __forceinline__ bool near_by(uint32_t upper, uint32_t lower) {
   if (upper == 0u || lower == 0u) return false;
   const float a = Order<float>::value(upper), b = Order<float>::value(lower);
   return !(a - b > kMargin + kMarginOfValue * fmaxf(fabsf(a), fabsf(b)));
+}
+
+// Whether the numbers of a kept group and of one that is not may be in another order than their fp32 keys. A lane has a group's
+// key (0 for none, and for one with nothing open) and the magnitudes that it was added up of.
+__device__ __forceinline__ bool groups_near(uint32_t own, bool kept, float size) {
+  const float v = Order<float>::value(own), off = 0.5f * kMargin + kErrorOfParts * size;
+  const uint32_t lowest = __reduce_min_sync(kFull, !kept ? 0xFFFFFFFFu : own == 0u ? 0u : Order<float>::of(v - off));
+  const uint32_t highest = __reduce_max_sync(kFull, kept || own == 0u ? 0u : Order<float>::of(v + off));
+  return lowest != 0u && highest != 0u && !(Order<float>::value(lowest) > Order<float>::value(highest));
 }
 
 // The two largest of a group's keys, as it counts: the best one, or both added up; 0 for a group with nothing open.
@@ -239,6 +250,7 @@ __device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N
   if (p.groups > 1) {
     const int per = p.experts / p.groups;
     Key own = 0;  // of group `lane`
+    float size = 0.0f;
     for (int g = 0; g < p.groups; ++g) {
       Key best = 0, second = 0;
 #pragma unroll
@@ -250,7 +262,10 @@ __device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N
         take(best, second, b);
         take(best, second, s);
       }
-      if (lane == g) own = group_key<T>(p.group_score, best, second);
+      if (lane == g) {
+        own = group_key<T>(p.group_score, best, second);
+        if constexpr (kCheck) size = fabsf(O::value(best)) + (p.group_score == kMax || second == 0 ? 0.0f : fabsf(O::value(second)));
+      }
     }
     int before = 0;  // groups that come before this lane's
     for (int g = 0; g < p.groups; ++g) {
@@ -258,11 +273,7 @@ __device__ __forceinline__ int choose(const RouteArgs& p, const float (&logit)[N
       before += other > own || (other == own && g < lane);
     }
     const bool kept = lane < p.groups && before < p.top_groups;
-    if (kCheck && by_score && p.top_groups < p.groups) {
-      const uint32_t lowest = __reduce_min_sync(kFull, kept ? static_cast<uint32_t>(own) : 0xFFFFFFFFu);
-      const uint32_t highest = __reduce_max_sync(kFull, kept || lane >= p.groups ? 0u : static_cast<uint32_t>(own));
-      near |= near_by(lowest, highest);
-    }
+    if (kCheck && by_score && p.top_groups < p.groups) near |= groups_near(static_cast<uint32_t>(own), kept, size);
     const uint32_t groups_kept = __ballot_sync(kFull, kept);
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -478,14 +489,23 @@ __device__ __forceinline__ int choose_quickly(const RouteArgs& p, int64_t token,
       take(first, second, b);
       take(first, second, s);
     }
-    uint32_t own = first;
-    if (sums && second != 0u) own = Order<float>::of(key_value(first) + key_value(second));
+    uint32_t own = lane / span < p.groups ? first : 0u;
+    float size = fabsf(key_value(first));
+    if (sums && second != 0u) {
+      own = Order<float>::of(key_value(first) + key_value(second));
+      size += fabsf(key_value(second));
+    }
     bool kept = group_kept(p, own, lane, span);
     if ((sums || p.bias != nullptr || !kNarrow) && p.top_groups < p.groups) {
-      const uint32_t lowest = __reduce_min_sync(kFull, kept ? own : 0xFFFFFFFFu);
-      const uint32_t highest = __reduce_max_sync(kFull, kept || lane / span >= p.groups ? 0u : own);
-      if (sums || p.bias != nullptr ? near_by(lowest == 8u ? 1u : lowest, highest == 8u ? 1u : highest) : lowest == highest && lowest != 0u)
-        kept = group_kept(p, group_in_64_bits<N>(p, logit, row, lane, span), lane, span);
+      bool again;
+      if (sums || p.bias != nullptr) {
+        again = groups_near(own, kept, size);
+      } else {
+        const uint32_t lowest = __reduce_min_sync(kFull, kept ? own : 0xFFFFFFFFu);
+        const uint32_t highest = __reduce_max_sync(kFull, kept ? 0u : own);
+        again = lowest == highest && lowest != 0u;
+      }
+      if (again) kept = group_kept(p, group_in_64_bits<N>(p, logit, row, lane, span), lane, span);
     }
     if (!kept) best = 0u;
   }
