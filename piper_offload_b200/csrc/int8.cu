@@ -293,9 +293,11 @@ int64_t token_tiles(int64_t tokens, int64_t experts, int bn) {
   return experts == 0 ? (tokens + bn - 1) / bn : tokens / bn + std::min<int64_t>(experts + 1, tokens);
 }
 
+// A kernel's limit of shared memory is the same in every call, whatever the call takes: it is the kernel's, and another thread
+// may be between setting it and its launch.
 template <class Args>
 cudaError_t launch(void (*kernel)(Args), const Args& args, int64_t blocks, int threads, int smem, int cluster, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, i8::kSmemMax);
   if (e != cudaSuccess) return e;
   e = piper::launch(kernel, blocks, threads, static_cast<size_t>(smem), cluster, stream, args);
   return e == cudaSuccess ? launched() : e;

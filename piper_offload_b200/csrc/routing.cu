@@ -54,8 +54,9 @@ cudaError_t launched() {
 template <class Args>
 cudaError_t enqueue(void (*kernel)(Args), int64_t blocks, int threads, size_t smem, cudaStream_t stream, const Args& args) {
   cudaError_t e = cudaSuccess;
-  // above 48 KB a kernel has to be allowed its shared memory
-  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // above 48 KB a kernel has to be allowed its shared memory: in every call all that a block can have, since another thread may
+  // be between allowing it and its launch
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e == cudaSuccess) e = piper::launch(kernel, blocks, threads, smem, 1, stream, args);
   return e == cudaSuccess ? launched() : e;
 }
