@@ -15,8 +15,11 @@
 // With many tokens shared memory is the bound: for 256 columns x 256 tokens of a stage one SM brings in and reads 176 KB,
 // 1375 cycles at 128 bytes, for 1024 cycles of products. So they run on pairs of SMs (kPair): each decodes 2 x 128 of a
 // tile's 512 columns and holds half of the tokens, which the tensor cores of both read: 128 KB for the same 1024 cycles.
-// 2048 x 14336 x 4096 takes 187 us with the launch before (31), 1.5 PFLOP/s on the 128 SMs that have a tile (233 us without
-// pairs); in a program that runs long the power limit makes it 222.
+// The odd block's decoded codes are read by products that a thread of the even block issues, so that thread has to be
+// told over the cluster, by one that waits until all before is there. That takes 0.7 us and no decoding warp has it to spare, nor
+// one warp for all stages: four take them in turn (1024 x 4096 x 4096 36 us, 57 with one).
+// 2048 x 14336 x 4096 takes 190 us with the launch before (31), 1.5 PFLOP/s on the 128 SMs that have a tile; without pairs
+// 233 us.
 #pragma once
 #include <cuda.h>
 
@@ -52,7 +55,9 @@ struct GradShape {
   static constexpr int kRoom = kSmemMax - 3 * 1024 - kTokens;
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kTokens + 1024 + 512;
-  static constexpr int kThreads = 64 + 32 * kDecodeWarps;  // producer warp, tensor-core warp, decoding warps
+  // producer warp, tensor-core warp, decoding warps, and of a pair those that announce with the tensor-core warp what is decoded
+  static constexpr int kAnnounceWarps = kPair ? 4 : 1;
+  static constexpr int kThreads = 64 + 32 * kDecodeWarps + 32 * (kAnnounceWarps - 1);
   static constexpr int kTeams = 4 / kRows;  // of decoding warps, which take stages in turn: 64 codes a thread and stage
   static constexpr int kTeamWarps = kDecodeWarps / kTeams;
   static constexpr int kAlloc = tmem_columns(kRows * BN);
@@ -131,18 +136,19 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
   float* token_scale = reinterpret_cast<float*>(smem + S::kStages * S::kStage);
   uint64_t* full = reinterpret_cast<uint64_t*>(token_scale + BN);  // gradients landed (of a pair: both blocks', counted in the even one)
-  uint64_t* ready = full + S::kStages;                             // w decoded (the same)
+  uint64_t* ready = full + S::kStages;                             // w decoded by this block (in the even one: by both)
   uint64_t* empty = ready + S::kStages;
   uint64_t* done = empty + S::kStages;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   fp4::grid_launch_dependents();
+  const uint32_t half = kPair ? fp4::cluster_rank() : 0u;  // of a pair
   if (warp == 0 && lane == 0) {
     pm::prefetch_tmap(&p.dy_map);
     for (int s = 0; s < S::kStages; ++s) {
       pm::mbar_init(&full[s], 1);
-      pm::mbar_init(&ready[s], S::kTeamWarps * (kPair ? 2 : 1));
+      pm::mbar_init(&ready[s], S::kTeamWarps + (kPair && half == 0 ? 1 : 0));
       pm::mbar_init(&empty[s], 1);
     }
     pm::mbar_init(done, 1);
@@ -155,7 +161,6 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
       pm::tmem_relinquish();
     }
   }
-  const uint32_t half = kPair ? fp4::cluster_rank() : 0u;  // of a pair
   const int rank = !kPair && p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
   const int sharers = kPair ? 2 : p.split;  // blocks with the same tile
   TileAt t;
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
         fp4::Ring<S::kStages> ring;
         int block = from % blocks, row = first + from / blocks * static_cast<int>(p.groups.tokens);
         for (int i = from; i < to; ++i, ring.next()) {
-          if (issued >= S::kStages && !pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad)) break;
+          if (issued >= S::kStages && !mbar_wait_of<kPair>(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad)) break;
           uint8_t* at = smem + ring.slot * S::kStage + S::kA;
           if constexpr (kPair) {
             if (half == 0) pm::mbar_arrive_expect_tx(&full[ring.slot], 2 * S::kB);
@@ -213,15 +218,15 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
       // the last copies land before the block's shared memory goes, even if the tensor-core warp gave up
       if (half == 0)
         for (int i = max(0, issued - S::kStages); i < issued; ++i)
-          pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+          mbar_wait_of<kPair>(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
       __syncwarp();
     } else if (warp == 1) {
       const uint32_t idesc = idesc_grad(computed, kPair ? 256u : 128u);
       if (half == 0 && fp4::elect_one()) {
         fp4::Ring<S::kStages> ring;
         for (int i = from; i < to; ++i, ring.next()) {
-          if (!pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma) ||
-              !pm::mbar_wait(&ready[ring.slot], ring.round, pm::kStatusTimeoutMma))
+          if (!mbar_wait_of<kPair>(&full[ring.slot], ring.round, pm::kStatusTimeoutMma) ||
+              !mbar_wait_of<kPair>(&ready[ring.slot], ring.round, pm::kStatusTimeoutMma))
             break;
           pm::tc_fence_after();
           const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
@@ -243,7 +248,19 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
         else pm::umma_commit(done);
       }
       __syncwarp();
-    } else {
+    }
+    if (kPair && half != 0 && (warp == 1 || warp >= 2 + kDecodeWarps)) {
+      // the odd block's stages are announced to the even one, whose thread issues the products for both
+      if (fp4::elect_one()) {
+        const int first = warp == 1 ? 0 : warp - 1 - kDecodeWarps;
+        for (int i = first; i < to - from; i += S::kAnnounceWarps) {
+          const int slot = i % S::kStages;
+          if (!pm::mbar_wait(&ready[slot], (i / S::kStages) & 1, pm::kStatusTimeoutMma)) break;
+          mbar_arrive_pair(in_block(pm::smem_u32(&ready[slot]), 0));
+        }
+      }
+      __syncwarp();
+    } else if (warp >= 2 && warp < 2 + kDecodeWarps) {
       // Eight lanes have 64 columns of two rows: of a row's eight 16-byte pieces, XORed with the row, four lanes write the
       // even ones while the four of the row below write the odd ones, to all banks at once.
       const int turn = (warp - 2) / S::kTeamWarps;
@@ -275,7 +292,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
         }
         if (i + S::kTeams < to) walk.load(piece);
         if (i - from >= S::kStages) {
-          ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(&empty[slot], round ^ 1u, pm::kStatusTimeoutLoad));
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait_of<kPair>(&empty[slot], round ^ 1u, pm::kStatusTimeoutLoad));
           if (!ok) break;
         }
         uint8_t* const stage = smem + slot * S::kStage;
@@ -294,17 +311,14 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
           }
         pm::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (kPair) mbar_arrive_pair(in_block(pm::smem_u32(&ready[slot]), 0));
-          else pm::mbar_arrive(&ready[slot]);
-        }
+        if (lane == 0) pm::mbar_arrive(&ready[slot]);
         if ((slot += S::kTeams) >= S::kStages) {
           slot -= S::kStages;
           round ^= 1u;
         }
       }
       pm::named_bar_sync(1, 32 * kDecodeWarps);  // the tokens' scales are written
-      ok = __all_sync(0xFFFFFFFFu, pm::mbar_wait(done, 0, pm::kStatusTimeoutMma));
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_of<kPair>(done, 0, pm::kStatusTimeoutMma));
       pm::tc_fence_after();
       if (ok) {
         // the sums are complete, so the stages are free

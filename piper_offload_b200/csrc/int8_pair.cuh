@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
           for (int j = 0; j < ahead; ++j, ++i, ++it, ring.next()) load_x(i, j);
         }
         for (; i < stages; ++i, ++it, ring.next()) {
-          ok = it < S::kStages || pm::mbar_wait(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
+          ok = it < S::kStages || mbar_wait_pair(&empty[ring.slot], ring.round ^ 1u, pm::kStatusTimeoutLoad);
           if (!ok) break;
           load_w(i, ring.slot);
           load_x(i, ring.slot);
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
     // the last copies of both blocks land before either's shared memory goes, even if the tensor-core warp gave up
     if (rank == 0)
       for (int i = max(0, it - S::kStages); i < it; ++i)
-        pm::mbar_wait(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
+        mbar_wait_pair(&full[i % S::kStages], (i / S::kStages) & 1, pm::kStatusTimeoutLoad);
     __syncwarp();
   } else if (warp == 1 && rank == 0) {
     fp4::Ring<S::kStages> ring;
@@ -140,10 +140,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
       const uint32_t d = tmem + b * BN;
       const uint32_t idesc = idesc_i8_pair(computed(__shfl_sync(0xFFFFFFFFu, t.count, 0)));
       if (fp4::elect_one()) {
-        ok = n < 2 || pm::mbar_wait(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
+        ok = n < 2 || mbar_wait_pair(&acc_empty[b], ((n >> 1) - 1) & 1, pm::kStatusTimeoutMma);
         pm::tc_fence_after();
         for (int i = 0; ok && i < stages; ++i, ++it, ring.next()) {
-          ok = pm::mbar_wait(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
+          ok = mbar_wait_pair(&full[ring.slot], ring.round, pm::kStatusTimeoutMma);
           if (!ok) break;
           pm::tc_fence_after();
           const uint32_t at = pm::smem_u32(smem) + ring.slot * S::kStage;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
       }
       pm::named_bar_sync(1, 128);
       const int b = n & 1;
-      const bool ok = pm::mbar_wait(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
+      const bool ok = mbar_wait_pair(&acc_full[b], (n >> 1) & 1, pm::kStatusTimeoutMma);
       if (!pm::named_bar_and(2, 128, ok)) break;
       pm::tc_fence_after();
       store_tile<DT, true>(tmem + b * BN, p.y, half, p.rows, p.rows_of, static_cast<int64_t>(t.expert) * p.rows, token_scale, token_sum, 0, BN,

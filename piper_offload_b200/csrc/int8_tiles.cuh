@@ -52,11 +52,45 @@ __device__ __forceinline__ uint32_t in_block(uint32_t saddr, uint32_t rank) {
   return remote;
 }
 
-// One arrival on the barrier at `bar` of the cluster's address space. What the arriving block wrote to its own shared
-// memory before is there when the products that follow the wait read it in that block. (A release over the cluster makes
-// the thread wait for its loads under way too: the gradient's decoding warps took 318 us with it, 2048 x 14336 x 4096.)
+// One arrival on the barrier at `bar` of the cluster's address space. What the thread has written, or has seen through barriers
+// of its block, is there for a thread of either block that waits with mbar_wait_pair; with the default scope it would be
+// for threads of the arriving block alone. The thread waits for all that it has under way: a warp with loads in flight
+// arrives in its own block, where another passes it on (the gradient's decoding warps themselves took 318 us so, 2048 x
+// 14336 x 4096).
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The threads of a pair wait for everything that the other block may have a part in with the scope of the cluster too.
+__device__ __forceinline__ bool mbar_try_wait_pair(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(pm::smem_u32(bar)), "r"(parity), "r"(pm::kSuspendHintNs)
+      : "memory");
+  return ok != 0;
+}
+
+// pm::mbar_wait of such a thread.
+__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, unsigned int code) {
+  if (mbar_try_wait_pair(bar, parity)) return true;
+  const uint64_t t0 = pm::global_timer_ns();
+  for (uint32_t spin = 0;; ++spin) {
+    if (mbar_try_wait_pair(bar, parity)) return true;
+    if ((spin & 63u) == 63u && pm::global_timer_ns() - t0 > pm::kWaitLimitNs) {
+      atomicOr(&pm::g_status, code);
+      return false;
+    }
+  }
+}
+
+template <bool kPair>
+__device__ __forceinline__ bool mbar_wait_of(uint64_t* bar, uint32_t parity, unsigned int code) {
+  if constexpr (kPair) return mbar_wait_pair(bar, parity, code);
+  else return pm::mbar_wait(bar, parity, code);
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t cols) {
