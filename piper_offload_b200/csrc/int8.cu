@@ -365,7 +365,8 @@ GradTile grad_tile(const piper_int8_matrix& w, int64_t tokens, int terms, bool g
   const TilePlan alone = plan_tile(t.bn, tiles(128, t.bn), stages, one, std::min<int64_t>(per_expert, t.bn), !grouped, sm_count());
   double best = alone.cycles;
   for (int rows = 1; rows <= 2; ++rows)
-    for (int tile = 256; tile >= 128; tile -= 32) {
+    // a stage of 192 tokens and fewer takes the same
+    for (int tile = 256; tile >= 192; tile -= 32) {
       const double n = static_cast<double>(std::min<int64_t>(up(per_expert, 32), tile));
       const double stage = rows == 2 ? std::max(1000.0, 5.2 * n) : std::max(600.0, 2.95 * n);
       const int64_t room = sm_count() / 2, waves = (tiles(256 * rows, tile) + room - 1) / room;
