@@ -57,7 +57,8 @@ int piper_routing_route_grad(const piper_routing_config* c, const void* logits, 
 
 /* How tokens and choices lie: rows (tokens, top_k) as above, `total` the
  * number of places in use (the last of the ends; all of them where it is
- * larger). A row outside [0, total) counts as none. */
+ * larger). A row outside [0, total) counts as none. Each place in [0, total)
+ * is one row: what two name, or none, is left undefined in out and dy. */
 typedef struct piper_routing_exchange {
   int64_t tokens;
   int32_t top_k;

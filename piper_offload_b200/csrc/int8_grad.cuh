@@ -17,7 +17,7 @@
 // tile's 512 columns and holds half of the tokens, which the tensor cores of both read: 128 KB for the same 1024 cycles.
 // The odd block's decoded codes are read by products that a thread of the even block issues, so that thread has to be
 // told over the cluster, by one that waits until all before is there. That takes 0.7 us and no decoding warp has it to spare, nor
-// one warp for all stages: four take them in turn (1024 x 4096 x 4096 36 us, 57 with one).
+// one warp for all stages: four take them in turn (1024 x 4096 x 4096 36 us, 38 with three, 57 with one).
 // 2048 x 14336 x 4096 takes 190 us with the launch before (31), 1.5 PFLOP/s on the 128 SMs that have a tile; without pairs
 // 233 us.
 #pragma once

@@ -4,7 +4,7 @@
 // 128 cycles of products: 24 KB at 128 bytes a cycle, 192 cycles, and that is what a step takes (4096 x 14336 x 4096: 164 us
 // in tiles of 128 x 256). In a pair each SM holds 128 rows of the weight and half of the tokens, which the tensor cores of
 // both read: 16 KB for the same 128 cycles. 4096 x 14336 x 4096 then takes 154 us with the launch before (10), the tensor
-// pipe active for 92 % of the product while the power limit holds the clock at 1.6 GHz (3.3 POP/s); 183 us in a program.
+// pipe active for 92 % of the product while the power limit holds the clock at 1.6 GHz (3.3 POP/s); 184 to 189 us in a program.
 //
 // The even block of a pair issues the products for both; each block loads its own halves, counted on the even block's
 // barrier, and has its own 128 outputs in its tensor memory. Finished products are announced to both blocks.

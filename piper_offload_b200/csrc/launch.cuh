@@ -1,11 +1,11 @@
 // launch.cuh - launches that may begin while the launch before them ends (programmatic stream serialization).
 //
-// A kernel launched so begins with grid_launch_dependents(), which lets the next such launch set itself up, and
-// grid_wait(), which ends when all launches before it have ended and their writes are visible; it touches no memory before.
-// What a kernel does before its wait has to need nothing of them: an INT8 product loads its weight then and reads the ends of
-// its groups, as a gradient does, so the launches before those (quantize_kernel, scale_kernel) wait first and let them begin
-// after. In a program's stream this takes the start of a launch,
-// 1.5 to 2.5 us, out of the time between two of them: 1 x 14336 x 4096 16.0 -> 13.3 us a call.
+// A kernel launched so calls grid_launch_dependents(), which lets the next such launch set itself up, and grid_wait(), which
+// ends when all launches before it have ended and their writes are visible. Memory that a launch of another call may have
+// written is read after the wait. Before it, an INT8 product loads its weight and reads the ends of its groups, and a
+// gradient those: they may, because the launch before each is the same call's (quantize_kernel, scale_kernel), which waits
+// first and lets them begin after. In a program's stream this takes the start of a launch, 1.5 to 2.5 us, out of the time
+// between two of them: 1 x 14336 x 4096 16.0 -> 13.3 us a call.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -19,7 +19,8 @@ attributes): ``Int8Weight`` with a scale, and a zero point where there is one,
 for each row or for the whole weight; ``Int8Experts``, a stack of them with a
 scale for each row; ``Bnb8Weight`` (LLM.int8); ``QuantoWeight`` of qint8 with a
 scale for each row or one for all. Groups of columns, scales for columns and
-``act_pre_scale`` are refused.
+``act_pre_scale`` are refused. Tokens are quantised to 8 bits for all of them,
+also where the weight's library would multiply by dequantised weights.
 
 Definitions. A weight's value is ``(code - zero) * scale`` (LLM.int8: ``code *
 SCB / 127``). A token with the largest magnitude ``a`` is held as the codes
@@ -28,13 +29,18 @@ the whole-number sum of codes times both scales, ``(sum * token's) * row's`` in
 fp32, rounded once to the type of the token. A token that holds an infinity or
 a NaN gives a row of NaN and touches no other. The gradient goes straight
 through the quantisation of the tokens: ``dx = (dy * scale) @ (codes - zero)``
-with fp32 sums, in which ``dy * scale`` has 11 bits (22 for fp32 gradients).
+with fp32 sums, in which ``dy * scale`` is rounded to 11 bits for bf16 and fp16
+gradients: that adds 1 % to the error that the rounding of a bf16 result makes,
+and 40 % to an fp16 one's. For fp32 gradients it has 22 bits, at twice the
+products; a caller who wants them passes ``dy.float()`` (or ``x.float()`` to a
+product that is differentiated).
 
 All functions run on ``torch.cuda.current_stream()`` of their tensors' device,
 take workspaces from PyTorch's caching allocator on it, do not synchronise,
 and raise ``ValueError`` for arguments that they do not take. Calls with plain
 arguments are made by compiled code (``csrc/expert_calls.cpp``); what it
-declines takes the path written out here, to the same kernels.
+declines takes the path written out here, to the same kernels. Quanto weights
+always do: 18 us of host time a call, 5 for the others.
 """
 
 from __future__ import annotations

@@ -47,7 +47,9 @@ class Routing:
     """Where the tokens of a batch go. ``weights`` fp32 and ``experts`` int32 (tokens, top_k), the best choice first, 0 and -1
     where a token has none; ``ends`` int32 (experts), the ends of the experts' groups in the order by expert, in which one
     expert's choices are in the order of their tokens; ``rows`` int32 (tokens, top_k), the place of each choice in it, or -1;
-    ``source`` int32 (tokens * top_k), the choice ``token * top_k + slot`` at each place, or -1 past the last end."""
+    ``source`` int32 (tokens * top_k), the choice ``token * top_k + slot`` at each place, or -1 past the last end. Every place
+    below the last end belongs to one choice: a routing that is made otherwise has to keep to that, since the exchange neither
+    adds up two choices at a place nor writes a place that has none."""
 
     weights: torch.Tensor
     experts: torch.Tensor
@@ -137,7 +139,8 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", 
     best ``top_groups`` of them: by their best choice (``group_score`` "max") or
     the sum of their two best ("top2"), equal ones by index. Weights are the
     scores without the bias, divided by their sum over the token's choices where
-    ``renormalize`` (a sum below 2**-100 counts as that), times ``scale``.
+    ``renormalize``, times ``scale``. (A sum of sigmoids below 2**-100 counts as
+    that. Softmax shares keep their proportions however small the scores are.)
 
     An expert with a logit or a bias of -infinity is closed: it is not chosen,
     and a token with fewer open experts than ``top_k`` has no choice in its last
