@@ -142,7 +142,6 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  fp4::grid_launch_dependents();
   const uint32_t half = kPair ? fp4::cluster_rank() : 0u;  // of a pair
   if (warp == 0 && lane == 0) {
     pm::prefetch_tmap(&p.dy_map);
@@ -167,6 +166,7 @@ __global__ void __launch_bounds__(GradShape<BN, kRows, kPair>::kThreads, 1) grad
   const bool have = fp4::find_tile(p.groups, sharers > 1 ? blockIdx.x / sharers : blockIdx.x, p.tile_tokens, t);
   pm::tc_fence_before();
   __syncthreads();
+  fp4::grid_launch_dependents();  // after the allocation (launch.cuh)
   if constexpr (kPair) fp4::cluster_sync();  // both blocks' barriers are there
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);

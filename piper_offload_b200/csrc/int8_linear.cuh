@@ -71,7 +71,6 @@ __global__ void __launch_bounds__(kLinearThreads, kCtas) linear_kernel(const __g
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  fp4::grid_launch_dependents();
   // this block's part of every tile's stages
   const int all = (p.cols + kStageCols - 1) / kStageCols;
   const int rank = p.split > 1 ? static_cast<int>(fp4::cluster_rank()) : 0;
@@ -102,6 +101,7 @@ __global__ void __launch_bounds__(kLinearThreads, kCtas) linear_kernel(const __g
   }
   pm::tc_fence_before();
   __syncthreads();
+  fp4::grid_launch_dependents();  // after the allocation (launch.cuh)
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);
 

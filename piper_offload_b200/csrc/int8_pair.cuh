@@ -54,7 +54,6 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  fp4::grid_launch_dependents();
   const uint32_t rank = fp4::cluster_rank();
   const int stages = (p.cols + kStageCols - 1) / kStageCols;
   const int first_item = blockIdx.x / 2, item_step = gridDim.x / 2;
@@ -80,6 +79,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_pair_kernel(const __
   if (warp == 1) tmem_alloc_pair(tmem_at, S::kAlloc);
   pm::tc_fence_before();
   __syncthreads();
+  fp4::grid_launch_dependents();  // after the allocation (launch.cuh)
   fp4::cluster_sync();  // both blocks' barriers are there
   pm::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_at, 0);

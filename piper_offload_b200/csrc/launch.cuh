@@ -4,8 +4,11 @@
 // ends when all launches before it have ended and their writes are visible. Memory that a launch of another call may have
 // written is read after the wait. Before it, an INT8 product loads its weight and reads the ends of its groups, and a
 // gradient those: they may, because the launch before each is the same call's (quantize_kernel, scale_kernel), which waits
-// first and lets them begin after. In a program's stream this takes the start of a launch, 1.5 to 2.5 us, out of the time
-// between two of them: 1 x 14336 x 4096 16.0 -> 13.3 us a call.
+// first and lets them begin after. A kernel that allocates tensor memory lets the next begin when it has it: the next may
+// allocate before its own wait (the product of a few tokens does, 32 columns), and on an SM with a block that is still to
+// have all 512 each would wait for the other. Registers and shared memory keep the two apart as they are now, no rule does.
+// In a program's stream such launches take the start of a launch, 1.5 to 2.5 us, out of the time between two of them: 1 x
+// 14336 x 4096 16.0 -> 13.3 us a call.
 #pragma once
 #include <cuda_runtime.h>
 

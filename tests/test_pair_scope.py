@@ -1,5 +1,5 @@
-"""CPU: barriers between the two blocks of a pair, as the sources write them. No run can show a missing scope, so the sources
-are read: an arrival in another block's shared memory releases over the cluster, and who waits for it acquires so."""
+"""CPU: what the sources say of waits and barriers and no run can show. Between the two blocks of a pair an arrival in the other's
+shared memory releases over the cluster, and who waits for it acquires so."""
 
 from __future__ import annotations
 
@@ -21,3 +21,12 @@ def test_pairs_wait_over_the_cluster():
     assert "pm::mbar_wait(" not in (CSRC / "int8_pair.cuh").read_text()
     plain = re.findall(r"pm::mbar_wait\((&?\w+)", (CSRC / "int8_grad.cuh").read_text())
     assert plain == ["&ready"], plain
+
+
+def test_the_next_launch_begins_after_the_allocation():
+    """A launch that follows may allocate tensor memory before it waits for the one before it."""
+    for name in ("int8_linear.cuh", "int8_pair.cuh", "int8_grad.cuh"):
+        text = (CSRC / name).read_text()
+        kernel = text[text.index("__global__"):]
+        assert kernel.count("grid_launch_dependents()") == 1
+        assert max(m.start() for m in re.finditer(r"tmem_alloc(_pair)?\(", kernel)) < kernel.index("__syncthreads()") < kernel.index("grid_launch_dependents()")
