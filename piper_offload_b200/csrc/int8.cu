@@ -345,9 +345,9 @@ GradPlan plan_grad(const piper_int8_matrix& w, int64_t tokens, int dtype) {
 
 // Tiles of a gradient: tokens x columns. Decoding costs the same whatever the tokens, so tiles are as wide in tokens as they
 // go, but for a few, which leave room for more stages. The rough account in cycles a stage was measured: one SM takes 810 for
-// 128 columns x 256 tokens and 560 for few, a pair 1330 for 512 x 256 and 750 for 256 x 256 (2048 x 14336 x 4096 189 us in
+// 128 columns x 256 tokens and 560 for few, a pair 1330 for 512 x 256 and 750 for 256 x 256 (2048 x 14336 x 4096 190 us in
 // tiles of 512 on pairs, 200 of 256, on single SMs 233 of 128 x 256; 512 x 4096 x 4096 27 on single SMs that share sums, 30 on
-// pairs; 512 rows of 16 experts of 2048 x 2048 26 in tiles of 512 on pairs, 30 of 128 x 64 on single SMs).
+// pairs; 512 rows of 16 experts of 2048 x 2048 27 in tiles of 512 on pairs, 30 of 128 x 64 on single SMs).
 struct GradTile {
   int bn, rows, split;
   bool pair;

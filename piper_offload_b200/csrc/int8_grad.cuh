@@ -10,7 +10,8 @@
 //
 // Decoding is bound by issue: 40 instructions for 32 codes, and what a warp does once a stage (its wait, addresses, fence and
 // arrival) as many again. So a thread has 64 codes of a stage: with 32, and every warp in every stage, 2048 rows of 16
-// experts of 2048 x 2048 took 35 us (32 now), 512 rows 33 (26). Codes that a producer brings to L2 ahead changed neither.
+// experts of 2048 x 2048 took 35 us instead of 32, 512 rows 33 instead of 26 (36 and 27 since a pair's stages are announced
+// over the cluster). Codes that a producer brings to L2 ahead changed neither.
 //
 // With many tokens shared memory is the bound: for 256 columns x 256 tokens of a stage one SM brings in and reads 176 KB,
 // 1375 cycles at 128 bytes, for 1024 cycles of products. So they run on pairs of SMs (kPair): each decodes 2 x 128 of a
